@@ -420,6 +420,91 @@ int mace_profile_timeline(mace_ctx* ctx, int32_t max_entries, char* names, int32
  * (1 = an edge's reverse index did not point back to it). */
 int mace_ctx_error_flag(mace_ctx* ctx, int32_t* flag);
 
+/*
+ * Species operators: the parts of the model whose parameters are indexed by an
+ * atom's species (the node embedding, reference model.py:373-438, and the skip
+ * tensor product, reference tensor_product.py:1046-1305), by themselves and
+ * with their parameter gradients, for callers that train them.  No context:
+ * the caller owns every buffer, workspaces included; nothing here allocates or
+ * synchronises, so every call can be captured into a CUDA graph.  Calls use
+ * the current device, which must own the pointers.
+ *
+ * A species index outside [0, num_groups) marks a padding row (NaN features
+ * there are never read): it belongs to no group, its outputs are zero and it
+ * adds nothing to a gradient.  dtype is MACE_F32 or MACE_BF16 for the
+ * features, the parameters and their gradients alike; sums are kept in fp32
+ * and rounded once.  Feature rows are addressed as
+ *   data + node * node_stride + m * comp_stride + channel   (in elements)
+ * with m < d, so a slot of a node-feature table is passed in place.
+ */
+#define MACE_F32 0
+#define MACE_BF16 1
+#define MACE_SPECIES_MAX_GROUPS 512      /* of the species-indexed linear map */
+#define MACE_SPECIES_MAX_INDEX 1048575   /* num_groups of grouping and embedding */
+#define MACE_CHECKPOINT_BLOCK 128        /* channels that share one 8-bit scale */
+
+/*
+ * Stable grouping of n rows: order lists the rows by species (rows of one
+ * species in their original order, padding rows last), offsets[g] ..
+ * offsets[g + 1] is group g's range of it (num_groups + 1 entries).
+ */
+int mace_species_group_workspace(int64_t n, int32_t num_groups, int64_t* bytes);
+int mace_species_group(const int32_t* species, int64_t n, int32_t num_groups, int32_t* order, int32_t* offsets,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* out[i] = scale * table[species[i]]  (rows of C channels; strides in elements) */
+int mace_species_embed(int32_t dtype, const void* table, int64_t table_stride, int32_t num_groups, int32_t C,
+                       const int32_t* species, int64_t n, float scale, void* out, int64_t out_stride, void* stream);
+
+/* grad_table[g] = scale * sum of grad[order[i]] over offsets[g] <= i < offsets[g + 1]
+ * (grad_table is (num_groups, C) contiguous; rows of empty groups are zero).
+ * The summation order depends on the sizes only. */
+int mace_species_embed_grad_workspace(int64_t n, int32_t num_groups, int32_t C, int64_t* bytes);
+int mace_species_embed_grad(int32_t dtype, const void* grad, int64_t grad_stride, const int32_t* order,
+                            const int32_t* offsets, int64_t n, int32_t num_groups, int32_t C, float scale,
+                            void* grad_table, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * y[n, m, :] = alpha * x[n, m, :] . W[g(n)] for the rows of every group, zero for
+ * the others.  W is (num_groups, in_dim, out_dim) contiguous, or with
+ * transpose (num_groups, out_dim, in_dim): the input gradient of the map.
+ */
+int mace_species_linear(int32_t dtype, const void* x, int64_t x_node_stride, int64_t x_comp_stride,
+                        const void* weight, int32_t transpose, int32_t num_groups, int32_t in_dim, int32_t out_dim,
+                        const int32_t* order, const int32_t* offsets, int64_t n, int32_t d, float alpha, void* y,
+                        int64_t y_node_stride, int64_t y_comp_stride, void* stream);
+
+/*
+ * grad_weight[g] = alpha * sum over group g's rows of x[n, m, :]^T dy[n, m, :]
+ * (num_groups, in_dim, out_dim; empty groups are zero).  x_scale NULL: x holds
+ * dtype.  Else x is an 8-bit checkpoint: int8 values at the same strides, and
+ * x_scale (n, d, ceil(in_dim / MACE_CHECKPOINT_BLOCK)) contiguous.
+ */
+int mace_species_linear_wgrad_workspace(int64_t n, int32_t d, int32_t num_groups, int32_t in_dim, int32_t out_dim,
+                                        int64_t* bytes);
+int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x_node_stride, int64_t x_comp_stride,
+                              const float* x_scale, const void* dy, int64_t dy_node_stride, int64_t dy_comp_stride,
+                              int32_t num_groups, int32_t in_dim, int32_t out_dim, const int32_t* order,
+                              const int32_t* offsets, int64_t n, int32_t d, float alpha, void* grad_weight,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * 8-bit checkpoint of feature rows: per row and block of MACE_CHECKPOINT_BLOCK
+ * channels scale = max |x| * fl(1 / 127) and q = round-half-even(x / scale),
+ * each operation rounded to fp32; a block of zeros has scale 0.  q (n, d, C) and scale (n, d, blocks)
+ * are contiguous.  A block that holds an infinity or NaN is restored as NaN.
+ * mace_rows_restore writes q * scale, rounded to dtype, to contiguous rows.
+ */
+int mace_rows_checkpoint(int32_t dtype, const void* x, int64_t node_stride, int64_t comp_stride, int64_t n, int32_t d,
+                         int32_t C, int8_t* q, float* scale, void* stream);
+int mace_rows_restore(int32_t dtype, const int8_t* q, const float* scale, int64_t n, int32_t d, int32_t C, void* x,
+                      void* stream);
+
+/* Synchronise the current device, return and clear the species operators'
+ * error flag (0, or 2: a bounded wait inside a kernel gave up and its outputs
+ * are incomplete). */
+int mace_species_error_flag(int32_t* flag);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,7 +14,7 @@ from .weights import load_model_dir, write_random_model
 
 __all__ = [
     "Atoms", "Irrep", "Irreps", "ModelSpec", "UnsupportedModel", "load_model_dir", "write_random_model",
-    "MACECalculator", "MACEMLXCalculator", "mace_mp", "mace_off", "MACEModel",
+    "MACECalculator", "MACEMLXCalculator", "mace_mp", "mace_off", "MACEModel", "species",
 ]
 
 
@@ -27,4 +27,8 @@ def __getattr__(name):  # torch-dependent pieces load lazily
         from .model import MACEModel
 
         return MACEModel
+    if name == "species":
+        import importlib
+
+        return importlib.import_module(".species", __name__)
     raise AttributeError(name)

@@ -1,0 +1,54 @@
+// Device helpers shared by the species operators (species.cu, species_linear.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+namespace mace {
+
+using bf16 = __nv_bfloat16;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(int8_t x) { return (float)x; }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float x) { return __float2bfloat16_rn(x); }
+
+// V consecutive channels as fp32: one 16-byte load where V channels fill it, else one by one
+template <typename T, int V>
+__device__ __forceinline__ void load_channels(const T* __restrict__ src, float* v) {
+  if constexpr (V * sizeof(T) == 16) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
+    const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = to_f32(t[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = to_f32(src[k]);
+  }
+}
+
+// 8-bit value of x at scale s = max |x| / 127 (0 where s is 0, infinite or NaN);
+// the clamp only acts where s is subnormal and the quotient may pass 127
+__device__ __forceinline__ int8_t quantise8(float x, float s) {
+  if (!(s > 0.f) || s > 3.4028234e38f) return 0;
+  const float r = rintf(__fdiv_rn(x, s));
+  return (int8_t)fminf(fmaxf(r, -127.f), 127.f);
+}
+
+// rows [lo, hi) of `order` that belong to group g, kept inside [0, n] whatever offsets holds
+struct Range {
+  int64_t lo, hi;
+};
+__device__ __forceinline__ Range group_range(const int32_t* __restrict__ offsets, int g, int64_t n) {
+  Range r;
+  r.lo = min(max((int64_t)offsets[g], (int64_t)0), n);
+  r.hi = min(max((int64_t)offsets[g + 1], r.lo), n);
+  return r;
+}
+
+}  // namespace mace

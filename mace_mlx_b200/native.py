@@ -131,9 +131,20 @@ EXPORTED = (
     "mace_profile_timeline",
     "mace_nl_build_noalloc", "mace_fma_probe",
     "mace_halo_unique_id", "mace_halo_create", "mace_halo_plan", "mace_halo_destroy",
+    "mace_species_group_workspace", "mace_species_group", "mace_species_embed",
+    "mace_species_embed_grad_workspace", "mace_species_embed_grad", "mace_species_linear",
+    "mace_species_linear_wgrad_workspace", "mace_species_linear_wgrad", "mace_rows_checkpoint", "mace_rows_restore",
+    "mace_species_error_flag",
 )
 NOALLOC_MAX_ATOMS = 131072
 NOALLOC_MAX_GRAPH_ATOMS = 16384
+
+# species operators
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+SPECIES_MAX_GROUPS = 512
+SPECIES_MAX_INDEX = 1048575
+CHECKPOINT_BLOCK = 128
 
 _lib = None
 
@@ -176,6 +187,19 @@ def load_library(path: str | Path | None = None) -> C.CDLL:
                                C.POINTER(i32)], C.c_int),
         "mace_profile_timeline": ([vp, i32, C.c_char_p, C.POINTER(i32), C.POINTER(i32), C.POINTER(C.c_float),
                                    C.POINTER(C.c_float), C.POINTER(i32)], C.c_int),
+        "mace_species_group_workspace": ([i64, i32, C.POINTER(i64)], C.c_int),
+        "mace_species_group": ([vp, i64, i32, vp, vp, vp, i64, vp], C.c_int),
+        "mace_species_embed": ([i32, vp, i64, i32, i32, vp, i64, f32, vp, i64, vp], C.c_int),
+        "mace_species_embed_grad_workspace": ([i64, i32, i32, C.POINTER(i64)], C.c_int),
+        "mace_species_embed_grad": ([i32, vp, i64, vp, vp, i64, i32, i32, f32, vp, vp, i64, vp], C.c_int),
+        "mace_species_linear": ([i32, vp, i64, i64, vp, i32, i32, i32, i32, vp, vp, i64, i32, f32, vp, i64, i64, vp],
+                                C.c_int),
+        "mace_species_linear_wgrad_workspace": ([i64, i32, i32, i32, i32, C.POINTER(i64)], C.c_int),
+        "mace_species_linear_wgrad": ([i32, vp, i64, i64, vp, vp, i64, i64, i32, i32, i32, vp, vp, i64, i32, f32, vp,
+                                       vp, i64, vp], C.c_int),
+        "mace_rows_checkpoint": ([i32, vp, i64, i64, i64, i32, i32, vp, vp, vp], C.c_int),
+        "mace_rows_restore": ([i32, vp, vp, i64, i32, i32, vp, vp], C.c_int),
+        "mace_species_error_flag": ([C.POINTER(i32)], C.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

@@ -1,0 +1,544 @@
+"""Species operators on the GPU against their definitions in 64 bits.
+
+Bounds (u = 2^-24, the unit roundoff of fp32):
+
+* grouping, the embedding lookup and the 8-bit checkpoint are exact: the
+  definition's own fp32 arithmetic, each operation rounded once, compared for
+  equality;
+* a sum of n products in fp32, in any order, is within (n + 16) 2u of the sum
+  of the products' magnitudes (2u: the tensor core truncates where it adds;
+  16: the roundings of the split operands, the partial sums and alpha);
+  over a whole result those errors are random, so its relative error in the
+  2-norm also stays below 2^-19, far below what one dropped bf16 term or a
+  TF32 product would leave (2^-16, 2^-12);
+* a bf16 result (8-bit significand) adds half a unit in its last place, at most
+  2^-8 of its magnitude.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def sp():
+    from mace_mlx_b200 import species
+
+    return species
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(*shape, generator=gen(seed), device="cuda").to(dtype)
+
+
+def draw_species(n, g, seed, pad=0.0, only=None):
+    """int32 species in [0, g), ``pad`` of them outside (below and above); ``only``: the groups used."""
+    z = torch.randint(0, g, (n,), generator=gen(seed), device="cuda", dtype=torch.int32)
+    if only is not None:
+        z = torch.tensor(only, dtype=torch.int32, device="cuda")[z % len(only)]
+    if pad:
+        r = torch.rand(n, generator=gen(seed + 1), device="cuda")
+        z = torch.where(r < pad / 2, -1, torch.where(r < pad, g + 3, z))
+    return z
+
+
+def valid(z, g):
+    return (z >= 0) & (z < g)
+
+
+def groups_of(z, g):
+    """The grouping by its definition."""
+    key = torch.where(valid(z, g), z, g).cpu()
+    order = torch.tensor(sorted(range(len(key)), key=lambda i: int(key[i])), dtype=torch.int32)
+    offsets = torch.tensor([int((key < v).sum()) for v in range(g + 1)], dtype=torch.int32)
+    return order.cuda(), offsets.cuda()
+
+
+def assert_sum(got, want, mass, n, what=""):
+    """got (fp32 or bf16) against the 64-bit sum ``want`` of n products of total magnitude ``mass``."""
+    got64 = got.double()
+    bound = (n + 16) * 2 * U * mass
+    if got.dtype == torch.bfloat16:
+        bound = bound * (1 + 2.0**-8) + 2.0**-8 * want.abs()
+    bad = (got64 - want).abs() > bound
+    assert not bad.any(), f"{what}: {int(bad.sum())} values off, worst {float((got64 - want).abs().max()):.3e}"
+    norm = float(want.norm())
+    rel = float((got64 - want).norm())
+    limit = 2.0**-19 if got.dtype == torch.float32 else 2.0**-8 + 2.0**-19
+    assert rel <= limit * norm, f"{what}: relative error {rel / norm:.3e}"
+
+
+# ------------------------------------------------------------------ grouping
+@pytest.mark.parametrize("n", [0, 1, 2, 31, 33, 1000, 4096, 4097, 20011])
+@pytest.mark.parametrize("g", [1, 2, 89, 511, 1023, 1024, 7921])
+def test_grouping_is_the_stable_order(sp, n, g):
+    z = draw_species(n, g, n + g, pad=0.1 if n > 1 else 0.0)
+    got = sp.group_species(z, g)
+    order = torch.argsort(torch.where(valid(z, g), z, g).cpu().long(), stable=True).to(torch.int32)
+    counts = torch.bincount(z[valid(z, g)].cpu().long(), minlength=g)
+    assert torch.equal(got.order.cpu(), order)
+    assert torch.equal(got.offsets.cpu(), torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]).int())
+
+
+@pytest.mark.parametrize("z", [[], [-1, -1, -1], [2] * 5000, [5, 4, 3, 2, 1, 0], [2**31 - 1, -(2**31), 0, 6, 5]])
+def test_grouping_of_special_lists(sp, z):
+    z = torch.tensor(z, dtype=torch.int32, device="cuda")
+    order, offsets = groups_of(z, 6)
+    got = sp.group_species(z, 6)
+    assert torch.equal(got.order, order) and torch.equal(got.offsets, offsets)
+
+
+def test_grouping_of_many_rows(sp):
+    n, g = 1_500_001, 300_007  # two counting passes, most groups with a few rows
+    z = draw_species(n, g, 3, pad=0.01)
+    got = sp.group_species(z, g)
+    key = torch.where(valid(z, g), z, g)
+    key, order = torch.sort(key, stable=True)
+    assert torch.equal(got.order, order.int())
+    assert torch.equal(got.offsets, torch.searchsorted(key, torch.arange(g + 1, device="cuda", dtype=torch.int32),
+                                                       out_int32=True))
+
+
+# ----------------------------------------------------------------- embedding
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,c", [(1, 1), (7, 3), (1000, 128), (333, 97), (65, 256), (130, 300), (2000, 8)])
+def test_embedding_lookup(sp, dtype, n, c):
+    g, scale = 11, 0.3
+    table = randn(g, c, seed=1, dtype=dtype)
+    z = draw_species(n, g, 2, pad=0.2)
+    ok = valid(z, g)
+    want = torch.where(ok[:, None], table.float()[z.clamp(0, g - 1).long()] * torch.tensor(scale), 0.0).to(dtype)
+    assert torch.equal(sp.species_embedding(table, z, scale=scale), want)
+
+
+def test_embedding_of_strided_tables_and_outputs(sp):
+    g, n = 5, 257
+    z = draw_species(n, g, 4, pad=0.1)
+    for c, off in [(64, 0), (64, 1), (33, 2)]:
+        wide = randn(g, 200, seed=5)
+        node = torch.full((n, 150), 7.0, device="cuda")
+        out = node[:, off:off + c]
+        got = sp.species_embedding(wide[:, off:off + c], z, scale=2.0, out=out)
+        assert got.data_ptr() == out.data_ptr()
+        want = torch.where(valid(z, g)[:, None], wide[z.clamp(0, g - 1).long(), off:off + c] * 2.0, 0.0)
+        assert torch.equal(out, want)
+        assert (node[:, :off] == 7.0).all() and (node[:, off + c:] == 7.0).all()
+    one = randn(1, 16, seed=6).expand(g, 16)  # a broadcast table
+    assert torch.equal(sp.species_embedding(one, z.clamp(0, g - 1)), one[z.clamp(0, g - 1).long()])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,g,c,pad", [(0, 3, 8, 0), (1, 1, 1, 0), (1, 4, 128, 0), (1000, 89, 128, 0.1), (5000, 4, 97, 0),
+                                       (3001, 1, 64, 0.05), (700, 300, 33, 0.5), (40, 7, 16, 1.0),
+                                       (9000, 2, 256, 0.01), (2000, 1500, 300, 0.1)])
+def test_embedding_gradient(sp, dtype, n, g, c, pad):
+    scale = 0.37
+    z = draw_species(n, g, 7, pad=pad)
+    dy = randn(n, c, seed=8, dtype=dtype)
+    dy[~valid(z, g)] = float("nan")  # padding rows are never read
+    got = sp.species_embedding_grad(dy, sp.group_species(z, g), scale=scale)
+    want = torch.zeros(g, c, dtype=torch.float64, device="cuda")
+    mass = torch.zeros_like(want)
+    at = z[valid(z, g)].long()
+    s = float(torch.tensor(scale))  # the fp32 scale the kernel gets
+    want.index_add_(0, at, dy[valid(z, g)].double() * s)
+    mass.index_add_(0, at, dy[valid(z, g)].double().abs() * s)
+    assert got.shape == (g, c) and got.dtype == dtype
+    assert_sum(got, want, mass, n)
+
+
+def test_embedding_gradient_of_long_groups_and_strides(sp):
+    n, g, c = 300_011, 3, 40
+    z = draw_species(n, g, 9, only=[0, 2])
+    dy = randn(n, 3 * c, seed=10)[:, c + 1:2 * c + 1]
+    got = sp.species_embedding_grad(dy, sp.group_species(z, g))
+    want = torch.zeros(g, c, dtype=torch.float64, device="cuda").index_add_(0, z.long(), dy.double())
+    mass = torch.zeros(g, c, dtype=torch.float64, device="cuda").index_add_(0, z.long(), dy.double().abs())
+    # blocks of rows are summed apart and joined: far fewer than n roundings meet in one sum
+    assert_sum(got, want, mass, n)
+    assert torch.equal(got[1], torch.zeros(c, device="cuda"))
+    again = sp.species_embedding_grad(dy, sp.group_species(z, g))
+    assert torch.equal(got, again)
+    # every row the same: a broadcast gradient
+    ones = torch.ones(1, c, device="cuda").expand(n, c)
+    counts = torch.bincount(z.long(), minlength=g).float()
+    assert torch.equal(sp.species_embedding_grad(ones, sp.group_species(z, g)), counts[:, None].expand(g, c))
+
+
+# -------------------------------------------------------------------- linear
+def linear64(x, w, z, alpha):
+    """Output and product magnitudes of the map in 64 bits; x (n, d, k)."""
+    g = w.shape[0]
+    a = float(torch.tensor(alpha))
+    y = torch.zeros(*x.shape[:-1], w.shape[2], dtype=torch.float64, device="cuda")
+    mass = torch.zeros_like(y)
+    for i in range(g):
+        rows = (z == i).nonzero().flatten()
+        if rows.numel():
+            xi, wi = x[rows].double(), w[i].double()
+            y[rows] = a * (xi @ wi)
+            mass[rows] = abs(a) * (xi.abs() @ wi.abs())
+    return y, mass
+
+
+def wgrad64(x, dy, z, g, alpha):
+    a = float(torch.tensor(alpha))
+    dw = torch.zeros(g, x.shape[-1], dy.shape[-1], dtype=torch.float64, device="cuda")
+    mass = torch.zeros_like(dw)
+    for i in range(g):
+        rows = (z == i).nonzero().flatten()
+        if rows.numel():
+            xi, yi = x[rows].double().flatten(0, 1), dy[rows].double().flatten(0, 1)
+            dw[i] = a * (xi.T @ yi)
+            mass[i] = abs(a) * (xi.abs().T @ yi.abs())
+    return dw, mass
+
+
+LINEAR = [
+    # n, d, k, m, g, pad
+    (1, 1, 1, 1, 1, 0.0), (1, 3, 128, 128, 4, 0.0), (2, 1, 16, 16, 89, 0.0), (5, 7, 9, 5, 3, 0.4),
+    (127, 1, 128, 128, 1, 0.0), (128, 1, 128, 128, 1, 0.0), (129, 1, 128, 128, 2, 0.0), (1000, 3, 128, 128, 89, 0.0),
+    (1000, 1, 96, 96, 4, 0.05), (333, 5, 97, 61, 10, 0.1), (400, 3, 65, 130, 6, 0.02), (300, 1, 129, 33, 5, 0.0),
+    (257, 3, 256, 192, 3, 0.1), (100, 1, 300, 257, 2, 0.0), (64, 1, 64, 256, 7, 1.0), (700, 1, 48, 16, 500, 0.1),
+    (210, 1, 520, 24, 2, 0.0), (4000, 1, 8, 8, 3, 0.0), (513, 7, 40, 72, 512, 0.3),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,k,m,g,pad", LINEAR)
+def test_linear_and_its_gradients(sp, dtype, n, d, k, m, g, pad):
+    alpha = 1.0 / k**0.5
+    z = draw_species(n, g, 11, pad=pad)
+    x, w, dy = randn(n, d, k, seed=12, dtype=dtype), randn(g, k, m, seed=13, dtype=dtype), \
+        randn(n, d, m, seed=14, dtype=dtype)
+    out = ~valid(z, g)
+    x[out], dy[out] = float("nan"), float("inf")  # padding rows are never read
+    groups = sp.group_species(z, g)
+    y, mass = linear64(x, w, z, alpha)
+    assert_sum(sp.species_linear(x, w, groups, alpha=alpha), y, mass, k, "forward")
+    dx, mass = linear64(dy, w.transpose(1, 2), z, alpha)
+    dw, wmass = wgrad64(x, dy, z, g, alpha)
+    got_x, got_w = sp.species_linear_grad(x, dy, w, groups, alpha=alpha)
+    assert_sum(got_x, dx, mass, m, "input gradient")
+    assert_sum(got_w, dw, wmass, n * d, "weight gradient")
+    assert torch.equal(got_x, sp.species_linear(dy, w, groups, alpha=alpha, transpose=True))
+    assert torch.equal(got_w, sp.species_linear_grad_weight(x, dy, groups, alpha=alpha))  # same order of sums
+    assert sp.error_flag() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mix", ["one", "two of many", "none"])
+def test_linear_over_many_tiles(sp, dtype, mix):
+    """More row tiles than SMs, groups that start and end inside a CTA's share."""
+    n, d, k, m, g = 30_011, 3, 64, 48, 20
+    z = {"one": torch.full((n,), 13, dtype=torch.int32, device="cuda"), "two of many": draw_species(n, g, 20, only=[3, 17]),
+         "none": torch.full((n,), -1, dtype=torch.int32, device="cuda")}[mix]
+    x, w, dy = randn(n, d, k, seed=21, dtype=dtype), randn(g, k, m, seed=22, dtype=dtype), \
+        randn(n, d, m, seed=23, dtype=dtype)
+    groups = sp.group_species(z, g)
+    y, mass = linear64(x, w, z, 0.5)
+    assert_sum(sp.species_linear(x, w, groups, alpha=0.5), y, mass, k)
+    dw, mass = wgrad64(x, dy, z, g, 0.5)
+    got = sp.species_linear_grad_weight(x, dy, groups, alpha=0.5)
+    assert_sum(got, dw, mass, n * d)
+    assert torch.equal(got, sp.species_linear_grad_weight(x, dy, groups, alpha=0.5))
+
+
+def _views(x):
+    """x (n, d, k) in other layouts of the same values."""
+    n, d, k = x.shape
+    wide = torch.zeros(n, (d + 2) * k, dtype=x.dtype, device="cuda")
+    slot = wide[:, k:(d + 1) * k].view(n, d, k)  # a slot of a node-feature table
+    slot.copy_(x)
+    odd = torch.zeros(n * d * k + 3, dtype=x.dtype, device="cuda")[3:].view(n, d, k)  # not 16-byte aligned
+    odd.copy_(x)
+    turned = torch.zeros(d, n, k, dtype=x.dtype, device="cuda").transpose(0, 1)  # component-major
+    turned.copy_(x)
+    loose = torch.zeros(n, d, k + 1, dtype=x.dtype, device="cuda")[..., :k]  # an odd row pitch
+    loose.copy_(x)
+    return {"slot": slot, "odd": odd, "turned": turned, "loose": loose}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,m", [(128, 128), (40, 24), (33, 7)])
+def test_linear_layouts_agree(sp, dtype, k, m):
+    """Strides and alignment change how rows are fetched, never the result."""
+    n, d, g = 301, 3, 4
+    z = draw_species(n, g, 30, pad=0.1)
+    x, w, dy = randn(n, d, k, seed=31, dtype=dtype), randn(g, k, m, seed=32, dtype=dtype), \
+        randn(n, d, m, seed=33, dtype=dtype)
+    groups = sp.group_species(z, g)
+    y = sp.species_linear(x, w, groups)
+    dw = sp.species_linear_grad_weight(x, dy, groups)
+    ck = sp.checkpoint_rows(x)
+    xs, ys, outs = _views(x), _views(dy), _views(torch.zeros_like(y))
+    for name in xs:
+        assert torch.equal(sp.species_linear(xs[name], w, groups), y), name
+        assert torch.equal(sp.species_linear_grad_weight(xs[name], ys[name], groups), dw), name
+        assert torch.equal(sp.species_linear(x, w, groups, out=outs[name]), y), name
+        assert torch.equal(outs[name], y), name
+        again = sp.checkpoint_rows(xs[name])
+        assert torch.equal(again.q, ck.q) and torch.equal(again.scale, ck.scale), name
+    # rows shared by every atom (node stride 0)
+    shared = x[:1].expand(n, d, k)
+    assert torch.equal(sp.species_linear(shared, w, groups), sp.species_linear(shared.contiguous(), w, groups))
+    # (n, k) rows are (n, 1, k) rows
+    assert torch.equal(sp.species_linear(x[:, 0], w, groups), sp.species_linear(x[:, :1].contiguous(), w, groups)[:, 0])
+
+
+def test_linear_writes_only_its_slot(sp):
+    n, d, k, m, g = 200, 3, 64, 32, 3
+    z = draw_species(n, g, 40, pad=0.2)
+    x, w = randn(n, d, k, seed=41), randn(g, k, m, seed=42)
+    table = torch.full((n, 5 * m), 3.0, device="cuda")
+    sp.species_linear(x, w, sp.group_species(z, g), out=table[:, m:4 * m].view(n, d, m))
+    assert (table[:, :m] == 3.0).all() and (table[:, 4 * m:] == 3.0).all()
+    assert torch.equal(table[~valid(z, g), m:4 * m], torch.zeros(int((~valid(z, g)).sum()), 3 * m, device="cuda"))
+
+
+def test_rows_with_infinities_and_nan_stay_apart(sp):
+    n, k, m, g = 300, 128, 64, 2
+    z = draw_species(n, g, 50)
+    x, w = randn(n, 1, k, seed=51), randn(g, k, m, seed=52)
+    clean = sp.species_linear(x, w, sp.group_species(z, g))
+    x[17, 0, 5], x[200, 0, 127] = float("inf"), float("nan")
+    got = sp.species_linear(x, w, sp.group_species(z, g))
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[[17, 200]] = False
+    assert torch.equal(got[rest], clean[rest])
+    assert not got[17].isfinite().any() and got[200].isnan().all()
+
+
+def test_large_and_small_magnitudes(sp):
+    """The split operands keep fp32's range: nothing overflows or is lost near its ends."""
+    n, k, m = 130, 64, 32
+    z = torch.zeros(n, dtype=torch.int32, device="cuda")
+    groups = sp.group_species(z, 1)
+    for sx, sw in [(1e30, 1e-30), (1e-25, 1e25), (3e38 / 8, 1e-3), (1e-12, 1e-12)]:
+        x = (randn(n, 1, k, seed=60).clamp(-4, 4) * sx)
+        w = (randn(1, k, m, seed=61).clamp(-4, 4) * sw)
+        y, mass = linear64(x, w, z, 1.0)
+        assert_sum(sp.species_linear(x, w, groups), y, mass, k, f"{sx} {sw}")
+
+
+def test_linear_past_32_bit_offsets(sp):
+    """Rows whose element offsets pass 2^31."""
+    n, k, m, g = 1000, 64, 32, 2
+    table = torch.empty(n, 3_000_000, dtype=torch.bfloat16, device="cuda")  # 3e9 elements, 6 GB
+    x = table[:, -k:]
+    x.copy_(randn(n, k, seed=70, dtype=torch.bfloat16))
+    z = draw_species(n, g, 71)
+    w = randn(g, k, m, seed=72, dtype=torch.bfloat16)
+    groups = sp.group_species(z, g)
+    dense = x.contiguous()
+    assert torch.equal(sp.species_linear(x, w, groups), sp.species_linear(dense, w, groups))
+    dy = randn(n, m, seed=73, dtype=torch.bfloat16)
+    assert torch.equal(sp.species_linear_grad_weight(x, dy, groups), sp.species_linear_grad_weight(dense, dy, groups))
+    assert torch.equal(sp.species_embedding_grad(x, groups), sp.species_embedding_grad(dense, groups))
+    assert torch.equal(sp.checkpoint_rows(x).q, sp.checkpoint_rows(dense).q)
+    out = table[:, 2_000_000:2_000_000 + m]
+    assert torch.equal(sp.species_linear(dense, w, groups, out=out), sp.species_linear(dense, w, groups))
+
+
+# ---------------------------------------------------------------- checkpoint
+def quantise(x):
+    """The checkpoint's definition in fp32 (each operation rounded once)."""
+    n, d, c = x.shape
+    nb = -(-c // 128)
+    xb = torch.nn.functional.pad(x.float(), (0, nb * 128 - c)).view(n, d, nb, 128)
+    scale = xb.abs().amax(-1) * torch.tensor(1.0 / 127.0)
+    q = torch.round(xb / torch.where(scale > 0, scale, 1.0)[..., None]).clamp(-127, 127)
+    return q.to(torch.int8).view(n, d, nb * 128)[..., :c], scale
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,c", [(0, 1, 8), (1, 1, 1), (3, 5, 7), (100, 3, 128), (77, 1, 129), (65, 4, 96), (10, 1, 300),
+                                   (1000, 1, 256), (33, 7, 64)])
+def test_checkpoint_is_its_definition(sp, dtype, n, d, c):
+    x = randn(n, d, c, seed=80, dtype=dtype)
+    if n > 2:
+        x[1] = 0.0  # a block of zeros
+        x[2] *= 1e-30
+    ck = sp.checkpoint_rows(x)
+    q, scale = quantise(x)
+    assert torch.equal(ck.q, q) and torch.equal(ck.scale, scale)
+    values = q.float() * scale.repeat_interleave(128, dim=-1)[..., :c]
+    for out in DTYPES:
+        assert torch.equal(sp.restore_rows(ck, out), values.to(out))
+    off = (sp.restore_rows(ck).double() - x.double()).abs()
+    assert (off <= 0.5 * (1 + 2.0**-16) * scale.repeat_interleave(128, dim=-1)[..., :c].double()).all()
+
+
+def test_checkpoint_of_extreme_rows(sp):
+    x = torch.zeros(6, 1, 128, device="cuda")
+    x[0, 0, 3] = float("nan")
+    x[1, 0, 3] = float("inf")
+    x[2, 0, :] = 3.4e38
+    x[3, 0, 5] = 1e-44  # the scale underflows to zero
+    x[4, 0, 5] = 3e-43  # a subnormal scale: the quotient passes 127
+    x[5, 0, 100] = -1.0
+    ck = sp.checkpoint_rows(x)
+    v = sp.restore_rows(ck)
+    assert v[0].isnan().all() and v[1].isnan().all()
+    assert torch.equal(ck.q[2], torch.full_like(ck.q[2], 127)) and v[2].isfinite().all()
+    assert (v[3] == 0).all() and int(ck.q[4].max()) <= 127 and v[4].isfinite().all()
+    assert int(ck.q[5, 0, 100]) == -127 and abs(float(v[5, 0, 100]) + 1.0) <= 2 * U
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,k,m,g,pad", [c for c in LINEAR if c[0] * c[1] > 1])
+def test_weight_gradient_from_a_checkpoint(sp, dtype, n, d, k, m, g, pad):
+    z = draw_species(n, g, 90, pad=pad)
+    x, dy = randn(n, d, k, seed=91), randn(n, d, m, seed=92, dtype=dtype)
+    x[~valid(z, g)] = float("nan")
+    dy[~valid(z, g)] = float("nan")
+    ck = sp.checkpoint_rows(x)
+    values = ck.q.double() * ck.scale.double().repeat_interleave(128, dim=-1)[..., :k]
+    dw, mass = wgrad64(values, dy, z, g, 0.7)
+    assert_sum(sp.species_linear_grad_weight(ck, dy, sp.group_species(z, g), alpha=0.7), dw, mass, n * d)
+    assert sp.error_flag() == 0
+
+
+# ------------------------------------------------------- gradients as a user has them
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_autograd_matches_differences(sp, checkpoint):
+    """The maps are linear in each argument, so a difference over any step is the derivative."""
+    n, d, k, m, g = 150, 3, 48, 40, 5
+    z = draw_species(n, g, 100, pad=0.1)
+    groups = sp.group_species(z, g)
+    x, w, v = randn(n, d, k, seed=101), randn(g, k, m, seed=102), randn(n, d, m, seed=103)
+    x.requires_grad_(), w.requires_grad_()
+    y = sp.species_linear(x, w, groups, alpha=0.2, checkpoint=checkpoint)
+    (y * v).sum().backward()
+    with torch.no_grad():
+        for t, step, slack in ((x, randn(n, d, k, seed=104), 0.0), (w, randn(g, k, m, seed=105), 1.0)):
+            moved = (x + step, w) if t is x else (x, w + step)
+            y1 = sp.species_linear(*moved, groups, alpha=0.2).double()
+            diff = float(((y1 - y.double()) * v.double()).sum())
+            dot = float((t.grad.double() * step.double()).sum())
+            mass = float(((y1.abs() + y.double().abs()) * v.double().abs()).sum())
+            # y and y1 carry (k + 16) 2u each; the checkpoint moves x by half a scale (max / 254) at most
+            bound = (k + 16) * 2 * U * mass * 4
+            if checkpoint and slack:
+                top = x.detach().double().abs().amax(-1, keepdim=True).expand_as(x) / 254
+                bound += float(linear64(top, step.abs(), z, 0.2)[0].mul(v.double().abs()).sum())
+            assert abs(diff - dot) <= bound, (diff, dot, bound)
+
+
+def test_embedding_autograd_and_expanded_gradients(sp):
+    n, g, c = 500, 7, 24
+    z = draw_species(n, g, 110, pad=0.1)
+    table = randn(g, c, seed=111).requires_grad_()
+    sp.species_embedding(table, z, scale=0.5).sum().backward()  # the gradient arrives expanded from one value
+    counts = torch.stack([(z == i).sum() for i in range(g)]).float()
+    assert torch.equal(table.grad, 0.5 * counts[:, None].expand(g, c))
+    table.grad = None
+    groups = sp.group_species(z, g)
+    sp.species_embedding(table, z, scale=0.5, groups=groups).sum().backward()
+    assert torch.equal(table.grad, 0.5 * counts[:, None].expand(g, c))
+    # weights shared by several uses add up, and a frozen argument gets none
+    x, w = randn(n, 1, c, seed=112), randn(g, c, c, seed=113).requires_grad_()
+    (sp.species_linear(x, w, groups) + sp.species_linear(x, w, groups)).sum().backward()
+    once = sp.species_linear_grad_weight(x, torch.ones(n, 1, c, device="cuda"), groups)
+    assert torch.equal(w.grad, once + once) and x.grad is None
+
+
+# ------------------------------------------------------------ streams, graphs
+def test_other_streams_and_cuda_graphs(sp):
+    n, d, k, m, g = 2000, 3, 64, 64, 9
+    z = draw_species(n, g, 120, pad=0.05)
+    x, w, dy = randn(n, d, k, seed=121), randn(g, k, m, seed=122), randn(n, d, m, seed=123)
+
+    def step():
+        groups = sp.group_species(z, g)
+        ck = sp.checkpoint_rows(x)
+        emb = sp.species_embedding(w[:, 0], z)
+        return [groups.order, groups.offsets, sp.species_linear(x, w, groups), *sp.species_linear_grad(x, dy, w, groups),
+                sp.species_linear_grad_weight(ck, dy, groups), emb, sp.species_embedding_grad(emb, groups),
+                sp.restore_rows(ck)]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    x.mul_(2.0)
+    want = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals(sp):
+    z = torch.zeros(8, dtype=torch.int32, device="cuda")
+    groups = sp.group_species(z, 2)
+    x, w = torch.zeros(8, 3, 16, device="cuda"), torch.zeros(2, 16, 4, device="cuda")
+    dy = torch.zeros(8, 3, 4, device="cuda")
+    ck = sp.checkpoint_rows(x)
+    bad = [
+        lambda: sp.group_species(z.long(), 2), lambda: sp.group_species(z[::2], 2), lambda: sp.group_species(z, 0),
+        lambda: sp.group_species(z, sp.MAX_INDEX + 1), lambda: sp.group_species(z.view(2, 4), 2),
+        lambda: sp.species_embedding(w[:, :, 0], z),  # channels not contiguous
+        lambda: sp.species_embedding(w, z), lambda: sp.species_embedding(w[:, 0].half(), z),
+        lambda: sp.species_embedding(w[:, 0], z.cpu()), lambda: sp.species_embedding(w[:, 0], z, out=x[:, 0]),
+        lambda: sp.species_embedding_grad(x, groups), lambda: sp.species_embedding_grad(x[:4, 0], groups),
+        lambda: sp.species_linear(x.transpose(1, 2), w, groups), lambda: sp.species_linear(x.bfloat16(), w, groups),
+        lambda: sp.species_linear(x.double(), w.double(), groups), lambda: sp.species_linear(x[:7], w, groups),
+        lambda: sp.species_linear(x[..., :15], w, groups), lambda: sp.species_linear(x, w[:1], groups),
+        lambda: sp.species_linear(x, w.transpose(1, 2), groups), lambda: sp.species_linear(x[0, 0], w, groups),
+        lambda: sp.species_linear(x, w, groups, out=dy[:4]), lambda: sp.species_linear(x, w, groups, out=dy.bfloat16()),
+        lambda: sp.species_linear(x, w, groups, out=dy[:1].expand(8, 3, 4)),
+        lambda: sp.species_linear(x, w, groups, out=torch.zeros(8, 3, 4)),
+        lambda: sp.species_linear(x.cpu(), w, groups), lambda: sp.species_linear(x, w.cpu(), groups),
+        lambda: sp.species_linear(x, w, sp.SpeciesGroups(groups.order.cpu(), groups.offsets)),
+        lambda: sp.species_linear(x, w, sp.SpeciesGroups(groups.order, groups.offsets.long())),
+        lambda: sp.species_linear(x, w, sp.SpeciesGroups(groups.order, groups.offsets[:1])),
+        lambda: sp.species_linear(x, torch.zeros(513, 16, 4, device="cuda"), sp.group_species(z, 513)),
+        lambda: sp.species_linear_grad_weight(x[:4], dy, groups), lambda: sp.species_linear_grad_weight(x, dy[:, :2], groups),
+        lambda: sp.species_linear_grad_weight(x.bfloat16(), dy, groups),
+        lambda: sp.species_linear_grad_weight(sp.RowCheckpoint(ck.q, ck.scale[:, :2]), dy, groups),
+        lambda: sp.species_linear_grad_weight(sp.RowCheckpoint(ck.q.int(), ck.scale), dy, groups),
+        lambda: sp.species_linear_grad_weight(x, dy, sp.group_species(z, 513)),
+        lambda: sp.checkpoint_rows(x.half()), lambda: sp.checkpoint_rows(x[..., ::2]), lambda: sp.checkpoint_rows(x[0, 0]),
+        lambda: sp.checkpoint_rows(torch.zeros(1, 2000, 1, device="cuda")),
+        lambda: sp.restore_rows(ck, torch.float16), lambda: sp.restore_rows(sp.RowCheckpoint(ck.q, ck.scale.double())),
+        lambda: sp.species_linear(x.requires_grad_(), w, groups, transpose=True),
+        lambda: sp.species_embedding(torch.zeros(3, 4, device="cuda", requires_grad=True), z, groups=groups),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was accepted")
+    with pytest.raises(TypeError):
+        sp.group_species([0, 1], 2)
+    torch.cuda.synchronize()
+    assert sp.error_flag() == 0
+
+
+def test_groupings_that_are_not_permutations_stay_in_bounds(sp):
+    """order and offsets come from the caller: whatever they hold, no row outside the tensors is touched."""
+    n, k, g = 300, 32, 3
+    x, w, dy = randn(n, 1, k, seed=130), randn(g, k, k, seed=131), randn(n, 1, k, seed=132)
+    order = torch.randint(-5, n + 5, (n,), generator=gen(133), device="cuda", dtype=torch.int32)
+    for offsets in ([0, 500, -3, 2000], [200, 100, 50, 0], [-7, -7, -7, -7], [10, 20, 30, 40]):
+        bad = sp.SpeciesGroups(order, torch.tensor(offsets, dtype=torch.int32, device="cuda"))
+        sp.species_linear(x, w, bad)
+        sp.species_linear_grad_weight(x, dy, bad)
+        sp.species_linear_grad_weight(sp.checkpoint_rows(x), dy, bad)
+        sp.species_embedding_grad(dy[:, 0], bad)
+    torch.cuda.synchronize()
+    assert sp.error_flag() == 0

@@ -1,0 +1,68 @@
+"""Species operators without a GPU: refusals of the Python entry points and of
+the C ABI (host-side argument checks only, no launch)."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+import mace_mlx_b200
+from mace_mlx_b200 import native as nv
+from mace_mlx_b200 import species as sp
+
+
+def test_operators_are_public():
+    for name in sp.__all__:
+        assert hasattr(sp, name)
+    assert mace_mlx_b200.species is sp
+
+
+def test_cpu_tensors_are_refused():
+    z = torch.zeros(4, dtype=torch.int32)
+    groups = sp.SpeciesGroups(z, torch.zeros(2, dtype=torch.int32))
+    x, w = torch.zeros(4, 1, 8), torch.zeros(1, 8, 8)
+    for call in (lambda: sp.group_species(z, 1), lambda: sp.species_embedding(w[0], z),
+                 lambda: sp.species_embedding_grad(x[:, 0], groups), lambda: sp.species_linear(x, w, groups),
+                 lambda: sp.species_linear_grad(x, x, w, groups), lambda: sp.species_linear_grad_weight(x, x, groups),
+                 lambda: sp.checkpoint_rows(x),
+                 lambda: sp.restore_rows(sp.RowCheckpoint(x.to(torch.int8), torch.zeros(4, 1, 1)))):
+        with pytest.raises(ValueError, match="no CPU path"):
+            call()
+
+
+def test_c_entries_check_their_arguments():
+    lib = nv.load_library()
+    need = C.c_int64(-1)
+    one = C.c_void_p(16)  # never dereferenced: every call below is refused on the host
+    assert lib.mace_species_group_workspace(1000, 89, C.byref(need)) == nv.MACE_OK and need.value > 0
+    assert lib.mace_species_group_workspace(-1, 89, C.byref(need)) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_group_workspace(1, 0, C.byref(need)) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_group_workspace(1, nv.SPECIES_MAX_INDEX + 1, C.byref(need)) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_group_workspace(2**31, 1, C.byref(need)) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_group_workspace(1, 1, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_group(one, 5, 2, one, None, one, 1 << 20, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_group(one, 5, 2, one, one, one, 3, None) == nv.MACE_ERR_BAD_ARG
+    assert "workspace" in nv.last_error(lib)
+    assert lib.mace_species_embed(2, one, 8, 1, 8, one, 1, 1.0, one, 8, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_embed(0, one, 8, 1, 8, one, 1, 1.0, one, 7, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_embed(0, None, 8, 1, 8, one, 1, 1.0, one, 8, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_embed_grad_workspace(1, 1, 0, C.byref(need)) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_embed_grad(0, None, 8, one, one, 4, 1, 8, 1.0, one, one, 1 << 20, None) == nv.MACE_ERR_BAD_ARG
+    lin = (0, one, 8, 8, one, 0, 1, 8, 8, one, one, 4, 1, 1.0, one, 8, 8, None)
+    for at, value in ((0, 7), (1, None), (4, None), (6, 0), (6, nv.SPECIES_MAX_GROUPS + 1), (7, 0), (8, 0), (9, None),
+                      (10, None), (11, -1), (12, 0), (12, 5000), (14, None), (2, -1)):
+        args = list(lin)
+        args[at] = value
+        assert lib.mace_species_linear(*args) == nv.MACE_ERR_BAD_ARG, at
+    wg = (0, one, 8, 8, None, one, 8, 8, 1, 8, 8, one, one, 4, 1, 1.0, one, one, 1 << 30, None)
+    for at, value in ((0, 7), (1, None), (5, None), (8, 0), (9, 0), (10, 0), (11, None), (12, None), (13, -1), (14, 0),
+                      (16, None), (3, -1)):
+        args = list(wg)
+        args[at] = value
+        assert lib.mace_species_linear_wgrad(*args) == nv.MACE_ERR_BAD_ARG, at
+    assert lib.mace_species_linear_wgrad_workspace(-1, 1, 1, 1, 1, C.byref(need)) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_rows_checkpoint(0, None, 8, 8, 1, 1, 8, one, one, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_rows_checkpoint(3, one, 8, 8, 1, 1, 8, one, one, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_rows_restore(0, one, None, 1, 1, 8, one, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_rows_restore(0, one, one, 1, 0, 8, one, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_error_flag(None) == nv.MACE_ERR_BAD_ARG
