@@ -1,146 +1,999 @@
 // Species-indexed linear map (reference tensor_product.py:1046-1305 with a
-// one-hot second input) on rows grouped by species, and its weight gradient:
-//   y[r] = alpha x[r] W[g],   dW[g] = alpha sum_{r in g} x[r]^T dy[r].
+// one-hot second input) on rows grouped by species, and its weight gradient,
+// on the 5th-generation tensor cores:
+//   y[r]  = alpha x[r] W[g(r)]                    (128 grouped rows x NT columns per tile, K = channels)
+//   dW[g] = alpha sum over r in g of x[r]^T dy[r]  (128 input channels x NT columns per tile, K = rows)
+//
+// Arithmetic.  An fp32 operand is split into three bf16 pieces x = h + m + l
+// (h truncated, m rounded: the 24 bits of x exactly) and six of the nine
+// products are kept (h h, h m, m h, m m, h l, l h; the dropped ones are below
+// 2^-23 of x w), all kind::f16 MMAs: the instruction count of a 3xTF32 split
+// with 3/4 of its operand bytes.  bf16 data is one piece; 8-bit checkpoint
+// values are exact in one bf16 piece and their row scale is folded into dy.
+// The tensor core truncates when it accumulates, so an accumulator takes one
+// 64-wide step of K, smallest products first, and the epilogue warps add the
+// steps in fp32 registers.
+//
+// Roles of a CTA (16 warps, one CTA per SM, a contiguous share of the tiles):
+//   warps 0-3   operand A: own 32 TMEM lanes each, fetch their rows with 16-byte
+//               cp.async through a private ring (gathered by `order`), split
+//               them in registers and store them to TMEM
+//   warps 4-7   operand B: weights (map) or dy rows (weight gradient) into
+//               128B-swizzled K-major shared-memory images
+//   warps 8-15  epilogue: TMEM -> fp32 registers -> memory
+//   the MMAs are issued by warp 4 (map: its weight images rarely change) or
+//   warp 8 (weight gradient: it stores only at a group's end); a 17th warp
+//   would cut every thread to 96 registers
+// handing over through mbarriers only.  Every wait is bounded (about 2 s): one
+// that gives up raises the CTA's abort flag, which ends every other wait, and
+// TC_ERR_TIMEOUT in g_species_error.
+//
+// Rows may start at any alignment: a segment is fetched as the 16-byte units
+// that contain it (its end clipped by the copy's source size) and shifted when
+// it is read from shared memory (template VEC = 0; VEC = 1 when every row is
+// 16-byte aligned).
 #include <algorithm>
 
 #include "common.cuh"
 #include "species.cuh"
+#include "tc.cuh"
 
 namespace mace {
 
 namespace {
 
-constexpr int ST = 64;   // tile of the products
-constexpr int SK = 16;   // summation step
-
-template <typename T>
-__global__ void __launch_bounds__(256) k_species_linear(const T* __restrict__ x, int64_t xn, int64_t xm,
-                                                        const T* __restrict__ w, int transpose, int G, int K, int M,
-                                                        const int32_t* __restrict__ order,
-                                                        const int32_t* __restrict__ offsets, int64_t n, int d,
-                                                        float alpha, T* __restrict__ y, int64_t yn, int64_t ym) {
-  __shared__ float sx[SK][ST + 1], sw[SK][ST + 1];
-  // row tile blockIdx.x of the groups' tiles, then of the rows outside them
-  int64_t t = blockIdx.x;
-  int g = 0;
-  Range r{0, 0};
-  for (; g < G; ++g) {
-    r = group_range(offsets, g, n);
-    const int64_t nt = ((r.hi - r.lo) * d + ST - 1) / ST;
-    if (t < nt) break;
-    t -= nt;
-  }
-  const int64_t first = g == G ? min(max((int64_t)offsets[0], (int64_t)0), n) : 0;
-  if (g == G) {
-    const int64_t last = max(min(max((int64_t)offsets[G], (int64_t)0), n), first);
-    r.lo = 0;
-    r.hi = n - (last - first);
-  }
-  const int64_t r0 = r.lo * d + t * ST, r1 = r.hi * d;
-  if (r0 >= r1) return;
-  auto node_of = [&](int64_t row) -> int64_t {
-    int64_t at = row / d;
-    if (g == G && at >= first) at += n - r.hi;
-    const int64_t node = order[at];
-    return node >= 0 && node < n ? node : -1;
-  };
-  const int c0 = blockIdx.y * ST, tid = threadIdx.x;
-  float acc[4][4] = {};
-  if (g < G) {
-    for (int k0 = 0; k0 < K; k0 += SK) {
-      for (int i = tid; i < SK * ST; i += 256) {
-        const int rr = i / SK, k = k0 + i % SK;
-        const int64_t row = r0 + rr;
-        const int64_t node = row < r1 && k < K ? node_of(row) : -1;
-        sx[i % SK][rr] = node >= 0 ? to_f32(x[node * xn + (row % d) * xm + k]) : 0.f;
-      }
-      for (int i = tid; i < SK * ST; i += 256) {
-        const int kk = i / ST, k = k0 + kk, c = c0 + i % ST;
-        float v = 0.f;
-        if (k < K && c < M) v = to_f32(w[((int64_t)g * K * M) + (transpose ? (int64_t)c * K + k : (int64_t)k * M + c)]);
-        sw[kk][i % ST] = v;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < SK; ++k)
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-#pragma unroll
-          for (int b = 0; b < 4; ++b) acc[a][b] += sx[k][(tid >> 4) + 16 * a] * sw[k][(tid & 15) + 16 * b];
-      __syncthreads();
-    }
-  }
-  for (int a = 0; a < 4; ++a) {
-    const int64_t row = r0 + (tid >> 4) + 16 * a;
-    const int64_t node = row < r1 ? node_of(row) : -1;
-    if (node < 0) continue;
-    for (int b = 0; b < 4; ++b) {
-      const int c = c0 + (tid & 15) + 16 * b;
-      if (c < M) y[node * yn + (row % d) * ym + c] = from_f32<T>(alpha * acc[a][b]);
-    }
-  }
-}
-
-template <typename TX, typename T>
-__global__ void __launch_bounds__(256) k_species_wgrad(const TX* __restrict__ x, int64_t xn, int64_t xm,
-                                                       const float* __restrict__ xs, const T* __restrict__ dy,
-                                                       int64_t yn, int64_t ym, int K, int M,
-                                                       const int32_t* __restrict__ order,
-                                                       const int32_t* __restrict__ offsets, int64_t n, int d,
-                                                       float alpha, T* __restrict__ dw) {
-  __shared__ float sx[SK][ST + 1], sy[SK][ST + 1];
-  const int g = blockIdx.x, k0 = blockIdx.y * ST, c0 = blockIdx.z * ST, tid = threadIdx.x;
-  const int nb = (K + MACE_CHECKPOINT_BLOCK - 1) / MACE_CHECKPOINT_BLOCK;
-  const Range r = group_range(offsets, g, n);
-  // sums of 16 steps, then their sum: a single accumulator would round once per row
-  float acc[4][4] = {}, total[4][4] = {};
-  int step = 0;
-  for (int64_t base = r.lo * d; base < r.hi * d; base += SK) {
-    for (int i = tid; i < SK * ST; i += 256) {
-      const int64_t row = base + i / ST;
-      const int k = k0 + i % ST, c = c0 + i % ST;
-      int64_t node = row < r.hi * d ? order[row / d] : -1;
-      if (node >= n) node = -1;
-      const int m = (int)(row % d);
-      float vx = 0.f, vy = 0.f;
-      if (node >= 0 && k < K) {
-        vx = to_f32(x[node * xn + m * xm + k]);
-        if (xs) vx *= xs[(node * d + m) * nb + k / MACE_CHECKPOINT_BLOCK];
-      }
-      if (node >= 0 && c < M) vy = to_f32(dy[node * yn + m * ym + c]);
-      sx[i / ST][i % ST] = vx;
-      sy[i / ST][i % ST] = vy;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < SK; ++k)
-#pragma unroll
-      for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) acc[a][b] += sx[k][(tid >> 4) + 16 * a] * sy[k][(tid & 15) + 16 * b];
-    __syncthreads();
-    if (++step % 16 == 0 || base + SK >= r.hi * d) {
-#pragma unroll
-      for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          total[a][b] += acc[a][b];
-          acc[a][b] = 0.f;
-        }
-    }
-  }
-  for (int a = 0; a < 4; ++a)
-    for (int b = 0; b < 4; ++b) {
-      const int k = k0 + (tid >> 4) + 16 * a, c = c0 + (tid & 15) + 16 * b;
-      if (k < K && c < M) dw[((int64_t)g * K + k) * M + c] = from_f32<T>(alpha * total[a][b]);
-    }
-}
+constexpr int SL_THREADS = 16 * 32;
+constexpr int SL_KC = 64;              // K of one accumulation step
+constexpr int SL_D = 0;                // TMEM columns: two accumulators of 128
+constexpr int SL_A = 256;              // then two A stages
+constexpr uint32_t SL_TMEM = 512;
 
 __device__ int g_species_error;  // TC_ERR_TIMEOUT once a bounded wait gave up
 
+// feature rows: element (node, m, c) at data + node * node_stride + m * comp_stride + c
+struct RowView {
+  const char* data;
+  int64_t sn, sm;  // bytes
+  int width;       // channels
+};
+
+struct SlParams {
+  RowView a;            // map: x; weight gradient: x or its 8-bit checkpoint
+  RowView b;            // weight gradient: dy
+  const float* a_scale; // 8-bit checkpoint scales (n, d, ka_blocks)
+  int ka_blocks;
+  const void* w;        // map: weights (G, K, N), or (G, N, K) when transposed
+  int transposed;
+  void* out;            // map: y; weight gradient: dW (G, K, N)
+  int64_t out_sn, out_sm;  // map: elements
+  int vst;              // bytes of one vector store of `out` (32, 16), 0: element by element
+  float* part;          // weight gradient: partial tiles
+  const int32_t* order;
+  const int32_t* offsets;
+  int64_t n;
+  int d, G;
+  int K, N;             // map: K summed channels, N outputs; weight gradient: K x N of dW
+  int NT;               // tile columns: 32, 64, 96 or 128
+  int n_ct, n_kt;       // column tiles; weight gradient: row (channel) tiles
+  int shares;           // weight gradient: CTAs along the rows
+  float alpha;
+};
+
+// ------------------------------------------------------------------ helpers
+__device__ __forceinline__ constexpr uint32_t idesc_bf16(int N) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// D[tmem] (+)= A[tmem] . B[smem]^T in bf16: A's M rows are the TMEM lanes, two
+// consecutive K elements per 32-bit column
+__device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u)
+      : "memory");
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ float lds_as(uint32_t a, float) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float lds_as(uint32_t a, bf16) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+  return __uint_as_float((uint32_t)v << 16);
+}
+__device__ __forceinline__ float lds_as(uint32_t a, int8_t) {
+  int v;
+  asm volatile("ld.shared.s8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return (float)v;
+}
+
+// two values rounded to bf16, x0 in the low half
+__device__ __forceinline__ uint32_t pack_bf16(float x0, float x1) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x1), "f"(x0));
+  return r;
+}
+
+// the bf16 pieces of two values, packed: P = 3: h (truncated, so that no finite
+// value becomes infinite), m, l with x = h + m + l; P = 1: x rounded (exact here)
+template <int P>
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t* out) {
+  if constexpr (P == 1) {
+    out[0] = pack_bf16(x0, x1);
+  } else {
+    out[0] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+    const float r0 = x0 - __uint_as_float(__float_as_uint(x0) & 0xffff0000u);
+    const float r1 = x1 - __uint_as_float(__float_as_uint(x1) & 0xffff0000u);
+    out[1] = pack_bf16(r0, r1);
+    out[2] = pack_bf16(r0 - __uint_as_float(out[1] << 16), r1 - __uint_as_float(out[1] & 0xffff0000u));
+  }
+}
+
+__device__ __forceinline__ void tmem_st16u(uint32_t a, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16u(uint32_t a, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(a)
+      : "memory");
+}
+
+// 16 consecutive values of a result row, `left` of them inside it
+template <typename T>
+__device__ __forceinline__ void store16(T* dst, const float* v, int left, int vst) {
+  uint32_t w[16];
+  constexpr int W = 16 * sizeof(T) / 4;
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    if constexpr (sizeof(T) == 4)
+      w[k] = __float_as_uint(v[k]);
+    else
+      w[k] = pack_bf16(v[2 * k], v[2 * k + 1]);
+  }
+  if (left >= 16 && vst == 32) {
+#pragma unroll
+    for (int k = 0; k < W; k += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(dst) + k),
+                   "r"(w[k]), "r"(w[k + 1]), "r"(w[k + 2]), "r"(w[k + 3]), "r"(w[k + 4]), "r"(w[k + 5]), "r"(w[k + 6]),
+                   "r"(w[k + 7])
+                   : "memory");
+  } else if (left >= 16 && vst == 16) {
+#pragma unroll
+    for (int k = 0; k < W; k += 4)
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(dst) + k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (k < left) dst[k] = from_f32<T>(v[k]);
+  }
+}
+
+// the product list of PA x PB pieces, smallest terms first
+template <int PA, int PB>
+struct Products;
+template <>
+struct Products<3, 3> {
+  static constexpr int n = 6;
+  __device__ static constexpr int a(int i) { return i == 0 ? 2 : (i == 1 ? 0 : (i == 2 ? 1 : (i == 3 ? 1 : 0))); }
+  __device__ static constexpr int b(int i) { return i == 0 ? 0 : (i == 1 ? 2 : (i == 2 ? 1 : (i == 3 ? 0 : (i == 4 ? 1 : 0)))); }
+};
+template <>
+struct Products<1, 3> {
+  static constexpr int n = 3;
+  __device__ static constexpr int a(int) { return 0; }
+  __device__ static constexpr int b(int i) { return 2 - i; }
+};
+template <>
+struct Products<1, 1> {
+  static constexpr int n = 1;
+  __device__ static constexpr int a(int) { return 0; }
+  __device__ static constexpr int b(int) { return 0; }
+};
+
+// ------------------------------------------------------------------ layout
+// TA: stored type of A's rows, T: type of the parameters and of B, WG: weight gradient
+template <typename TA, typename T, bool WG, bool VEC>
+struct Sl {
+  static constexpr int PA = sizeof(TA) == 4 ? 3 : 1;
+  static constexpr int PB = sizeof(TA) == 2 ? 1 : 3;
+  static constexpr int SEG_A = WG ? 32 * (int)sizeof(TA) : 128;  // bytes of a row in one ring unit of 32 rows
+  static constexpr int SEG_B = 32 * (int)sizeof(T);
+  static constexpr int PITCH_A = SEG_A + (VEC ? 0 : 16), PITCH_B = SEG_B + (VEC ? 0 : 16);
+  static constexpr int UPC = WG ? 2 : SL_KC * (int)sizeof(TA) / 128;  // ring units per step of 64
+  static constexpr int NU = WG ? (VEC ? 4 : 3) : (sizeof(TA) == 4 ? 7 : 6);
+  static constexpr int UNIT_A = 32 * PITCH_A, UNIT_B = 32 * PITCH_B;
+  static constexpr int IMG = 128 * 128;  // one piece of a B image: NT <= 128 rows of 64 bf16
+  static constexpr int NSLOT = !WG && PB == 1 ? 4 : 2;
+  static constexpr int OFF_A = NSLOT * PB * IMG;
+  static constexpr int OFF_B = OFF_A + 4 * NU * UNIT_A;
+  static constexpr int OFF_MIS = OFF_B + (WG ? 4 * NU * UNIT_B : 0);        // per ring unit and row: misalignment
+  static constexpr int OFF_SCALE = OFF_MIS + (VEC ? 0 : (WG ? 8 : 4) * NU * 32);  // per B ring unit and row: A's scale
+  static constexpr int OFF_PRE = OFF_SCALE + (sizeof(TA) == 1 ? 4 * NU * 32 * 4 : 0);
+  static constexpr int OFF_BAR = OFF_PRE + ((MACE_SPECIES_MAX_GROUPS + 2) * 4 + 7) / 8 * 8;
+  static constexpr int NBAR = 8 + 2 * NSLOT + 1;
+  static constexpr int BYTES = OFF_BAR + NBAR * 8 + 32;
+  static_assert(BYTES <= 232448, "shared memory of a CTA");
+};
+
+__device__ __forceinline__ int64_t group_units(const SlParams& p, int g, int unit_rows) {
+  const Range r = group_range(p.offsets, g, p.n);
+  return ((r.hi - r.lo) * p.d + unit_rows - 1) / unit_rows;
+}
+
+// exclusive prefix of per-group tile counts into pre[0..G], by the whole CTA (G <= 512 = SL_THREADS)
+__device__ __forceinline__ void group_prefix(const SlParams& p, int unit_rows, int per_unit, int* pre,
+                                             int64_t* warp_sums) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t s = 0;
+  if (tid < p.G) s = group_units(p, tid, unit_rows) * per_unit;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) warp_sums[warp] = s;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) s += warp_sums[w];
+  if (tid < p.G) pre[tid + 1] = (int)min(s, (int64_t)INT32_MAX);  // beyond it: offsets that overlap
+  if (tid == 0) pre[0] = 0;
+  __syncthreads();
+}
+
+// largest g < G with pre[g] <= t (a group that holds unit t: empty groups have pre[g] == pre[g + 1])
+__device__ __forceinline__ int group_of_unit(const int* pre, int G, int t) {
+  int lo = 0, hi = G - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pre[mid] <= t)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// The steps of a CTA, in order; every role walks the same ones.
+// Map: tiles [t, t1) of (group, column tile, row tile), n_k steps each.
+// Weight gradient: 64-row units [t, t1) of the groups, one step each.
+template <bool WG>
+struct Walk {
+  int t, t0, t1, g;
+  int first, last;  // units of group g: [first, last)
+  int64_t lo, rows; // group's first grouped row (in components) and its row count
+  __device__ __forceinline__ void load(const SlParams& p, const int* pre) {
+    const Range r = group_range(p.offsets, g, p.n);
+    first = pre[g];
+    last = pre[g + 1];
+    lo = r.lo * p.d;
+    rows = (r.hi - r.lo) * p.d;
+  }
+  __device__ __forceinline__ void init(const SlParams& p, const int* pre, int t0_, int t1_) {
+    t = t0 = t0_;
+    t1 = t1_;
+    g = group_of_unit(pre, p.G, t);
+    load(p, pre);
+  }
+  __device__ __forceinline__ bool done() const { return t >= t1; }
+  __device__ __forceinline__ void next(const SlParams& p, const int* pre) {
+    if (++t < last || t >= t1) return;
+    do ++g;
+    while (pre[g + 1] <= t);
+    load(p, pre);
+  }
+  // map: row tiles of the group, this tile's column tile and row tile
+  __device__ __forceinline__ int row_tiles() const { return (int)((rows + 127) >> 7); }
+  __device__ __forceinline__ int col_tile() const { return (t - first) / row_tiles(); }
+  __device__ __forceinline__ int64_t row0() const { return (int64_t)((t - first) % row_tiles()) * 128; }
+  // map: first / last tile of its (group, column tile) in this CTA: the weight images are new / free after it
+  __device__ __forceinline__ bool new_weights() const { return t == t0 || (t - first) % row_tiles() == 0; }
+  __device__ __forceinline__ bool last_of_weights() const {
+    return t + 1 == t1 || (t + 1 - first) % row_tiles() == 0;
+  }
+};
+
+// this lane's row of a 32-row unit: bytes (node, m) of view v, or null outside the group
+__device__ __forceinline__ const char* row_pointer(const SlParams& p, const RowView& v, int64_t lo, int64_t rows,
+                                                   int64_t r, int64_t* scale_row) {
+  if (r >= rows) return nullptr;
+  const int64_t at = lo + r;
+  const int64_t i = p.d == 1 ? at : at / p.d;
+  const int m = (int)(at - i * p.d);
+  const int64_t node = p.order[i];
+  if (node < 0 || node >= p.n) return nullptr;
+  if (scale_row) *scale_row = node * p.d + m;
+  return v.data + node * v.sn + m * v.sm;
+}
+
+// 32 row segments of SEG bytes at byte `off` of each lane's row, into ring unit `dst`
+template <int SEG, int PITCH, bool VEC, bool SWZ>
+__device__ __forceinline__ void fetch_unit(uint32_t dst, const char* row, int64_t off, int64_t row_bytes,
+                                           const char* data, uint8_t* mis) {
+  const int lane = threadIdx.x & 31;
+  // copies of no bytes still name an aligned address
+  const char* const dummy = reinterpret_cast<const char*>(reinterpret_cast<uint64_t>(data) & ~(uint64_t)15);
+  if constexpr (VEC) {
+    constexpr int PPR = SEG / 16, RPI = 32 / PPR;  // pieces per row, rows per instruction
+#pragma unroll
+    for (int i = 0; i < PPR; ++i) {
+      const int r = i * RPI + lane / PPR, j = lane % PPR;
+      const char* base = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row), r));
+      const int64_t left = row_bytes - off - 16 * j;
+      const uint32_t bytes = base == nullptr || left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
+      const int pos = SWZ ? (j ^ (r & 7)) : j;
+      cp_async16(dst + r * PITCH + pos * 16, bytes ? base + off + 16 * j : dummy, bytes);
+    }
+  } else {
+    constexpr int PPR = SEG / 16 + 1;
+    const int shift = row ? (int)(reinterpret_cast<uint64_t>(row + off) & 15) : 0;
+    mis[lane] = (uint8_t)shift;
+#pragma unroll
+    for (int i = 0; i < PPR; ++i) {
+      const int q = i * 32 + lane;
+      const int r = q / PPR, j = q - r * PPR;
+      const char* base = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row), r));
+      const int64_t seg = min(row_bytes - off, (int64_t)SEG);  // bytes of the row in this segment
+      const char* src = reinterpret_cast<const char*>(reinterpret_cast<uint64_t>(base + off) & ~(uint64_t)15) + 16 * j;
+      const int64_t left = base + off + seg - src;
+      const uint32_t bytes = base == nullptr || seg <= 0 || left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
+      cp_async16(dst + r * PITCH + j * 16, bytes ? src : dummy, bytes);
+    }
+  }
+}
+
+// 16 bytes at byte offset s of the 32 bytes (a, b)
+__device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int s) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (s & 8) {
+#pragma unroll
+    for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+  }
+  if (s & 4) {
+#pragma unroll
+    for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+  }
+  const int bits = 8 * (s & 3);
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+template <typename TA, typename T, bool WG, bool VEC>
+__global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_constant__ SlParams p) {
+  using S = Sl<TA, T, WG, VEC>;
+  constexpr int PA = S::PA, PB = S::PB, NU = S::NU;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = tc::smem_u32(smem);
+  int* const pre = reinterpret_cast<int*>(smem + S::OFF_PRE);
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
+  uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + S::NBAR);
+  volatile int* const abort = reinterpret_cast<int*>(tslot + 1);
+  auto bar = [&](int i) { return tc::smem_u32(bars + i); };
+  auto A_FULL = [&](int s) { return bar(s); };
+  auto A_FREE = [&](int s) { return bar(2 + s); };
+  auto D_FULL = [&](int s) { return bar(4 + s); };
+  auto D_FREE = [&](int s) { return bar(6 + s); };
+  auto B_FULL = [&](int s) { return bar(8 + s); };
+  auto B_FREE = [&](int s) { return bar(8 + S::NSLOT + s); };
+  const uint32_t DONE = bar(8 + 2 * S::NSLOT);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (base & 1023u) {  // the images need 1024-byte alignment
+    if (tid == 0) atomicExch(&g_species_error, TC_ERR_ALIGN);
+    return;
+  }
+
+  if constexpr (!WG) {
+    // rows outside every group: zero
+    const int64_t b0 = min(max((int64_t)p.offsets[0], (int64_t)0), p.n);
+    const int64_t b1 = max(min(max((int64_t)p.offsets[p.G], (int64_t)0), p.n), b0);
+    const int64_t outside = (p.n - (b1 - b0)) * p.d;
+    T* out = static_cast<T*>(p.out);
+    for (int64_t r = blockIdx.x * (int64_t)(SL_THREADS / 32) + warp; r < outside; r += (int64_t)gridDim.x * (SL_THREADS / 32)) {
+      int64_t i = r / p.d;
+      const int m = (int)(r - i * p.d);
+      if (i >= b0) i += b1 - b0;
+      const int64_t node = p.order[i];
+      if (node < 0 || node >= p.n) continue;
+      for (int c = lane; c < p.N; c += 32) out[node * p.out_sn + m * p.out_sm + c] = from_f32<T>(0.f);
+    }
+  }
+
+  if (tid == 0) *abort = 0;
+  group_prefix(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, pre, reinterpret_cast<int64_t*>(smem));
+  // this CTA's share of the units; weight gradient: blockIdx.x = share * tiles + tile
+  const int total = pre[p.G];
+  const int tiles = WG ? p.n_ct * p.n_kt : 1;
+  const int nshare = WG ? min(p.shares, total) : gridDim.x;  // no share without a unit between two that have some
+  const int share = WG ? blockIdx.x / tiles : blockIdx.x;
+  if (share >= nshare) return;
+  const int tile = WG ? blockIdx.x % tiles : 0;
+  const int t0 = (int)((int64_t)share * total / nshare), t1 = (int)((int64_t)(share + 1) * total / nshare);
+  if (t0 >= t1) return;
+  const int wg_k0 = WG ? (tile / p.n_ct) * 128 : 0, wg_n0 = WG ? (tile % p.n_ct) * p.NT : 0;
+  const int n_k = WG ? 1 : (p.K + SL_KC - 1) / SL_KC;  // steps of a tile
+  const bool resident = n_k <= S::NSLOT;               // map: the weight images of a tile stay for the next row tile
+  const int NT = p.NT;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int s = 0; s < 2; ++s) {
+        tc::mbar_init(A_FULL(s), 128);
+        tc::mbar_init(A_FREE(s), 1);
+        tc::mbar_init(D_FULL(s), 1);
+        tc::mbar_init(D_FREE(s), 256);
+      }
+      for (int s = 0; s < S::NSLOT; ++s) {
+        tc::mbar_init(B_FULL(s), NT);
+        tc::mbar_init(B_FREE(s), 1);
+      }
+      tc::mbar_init(DONE, 1);
+      tc::fence_barrier_init();
+    }
+    __syncwarp();
+    tc::tmem_alloc(tc::smem_u32(tslot), SL_TMEM);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tslot;
+
+  // MMAs of step `it` with the images of slot bs (one thread); `use`: how often
+  // the slot was filled before, or -1 when its images were there already
+  auto issue = [&](int it, int bs, int use, bool release) -> bool {
+    using PR = Products<PA, PB>;
+    const uint32_t idesc = idesc_bf16(NT);
+    const int s = it & 1;
+    if (use >= 0 && !tc::mbar_wait_or_abort(B_FULL(bs), use & 1, abort)) return false;
+    if (!tc::mbar_wait_or_abort(A_FULL(s), (it >> 1) & 1, abort)) return false;
+    if (it >= 2 && !tc::mbar_wait_or_abort(D_FREE(s), ((it >> 1) - 1) & 1, abort)) return false;
+    tc::fence_after_sync();
+    const uint32_t img = base + bs * PB * S::IMG;
+#pragma unroll
+    for (int q = 0; q < PR::n; ++q)
+#pragma unroll
+      for (int ks = 0; ks < SL_KC / 16; ++ks)
+        mma_bf16_ta(tmem + SL_D + s * 128, tmem + SL_A + s * (PA * 32) + PR::a(q) * 32 + ks * 8,
+                    tc::sw128_desc(img + PR::b(q) * NT * 128 + ks * 32), idesc, q > 0 || ks > 0);
+    tc::mma_commit(A_FREE(s));
+    if (release) tc::mma_commit(B_FREE(bs));
+    tc::mma_commit(D_FULL(s));
+    return true;
+  };
+  auto drain = [&]() {  // every MMA issued is complete (bounded)
+    tc::mma_commit(DONE);
+    tc::mbar_wait(DONE, 0);
+  };
+
+  if (warp < 4) {
+    // ---------------- operand A: memory -> ring -> registers -> TMEM ----------------
+    const uint32_t ring = base + S::OFF_A + warp * NU * S::UNIT_A;
+    uint8_t* const mis = smem + S::OFF_MIS + warp * NU * 32;
+    const int64_t row_bytes = (int64_t)p.a.width * sizeof(TA);
+    const uint32_t tq = tmem + ((uint32_t)(warp * 32) << 16) + SL_A;
+    // the fetching side runs NU - 1 units ahead
+    Walk<WG> f;
+    f.init(p, pre, t0, t1);
+    int fk = 0, fu = 0, slot_f = 0;  // step of the tile, unit of the step, ring slot
+    const char *row = nullptr, *row_next = nullptr;
+    auto pointer = [&](const Walk<WG>& w, int u) -> const char* {
+      const int64_t r = WG ? (int64_t)(w.t - w.first) * SL_KC + u * 32 + lane : w.row0() + warp * 32 + lane;
+      return row_pointer(p, p.a, w.lo, w.rows, r, nullptr);
+    };
+    if constexpr (!WG) row = pointer(f, 0);
+    auto fetch = [&]() {
+      if (!f.done()) {
+        int64_t off;
+        if constexpr (WG) {
+          row = fu == 0 && f.t == t0 ? pointer(f, 0) : row_next;
+          off = (int64_t)(wg_k0 + warp * 32) * sizeof(TA);
+        } else {
+          off = (int64_t)fk * SL_KC * sizeof(TA) + fu * 128;
+        }
+        fetch_unit<S::SEG_A, S::PITCH_A, VEC, !WG>(ring + slot_f * S::UNIT_A, row, off, row_bytes, p.a.data,
+                                                   mis + slot_f * 32);
+        // pointers of the next unit (map: of the next tile), ahead of their use
+        if (++fu == S::UPC) {
+          fu = 0;
+          if (++fk == n_k) {
+            fk = 0;
+            f.next(p, pre);
+            if constexpr (!WG) {
+              row = row_next;
+            }
+          }
+        }
+        if constexpr (WG) {
+          if (!f.done()) row_next = pointer(f, fu);
+        } else if (fk == 0 && fu == 0) {
+          // the tile after the one whose fetch starts now
+          Walk<WG> nx = f;
+          if (!nx.done()) nx.next(p, pre);
+          row_next = nx.done() ? nullptr : pointer(nx, 0);
+        }
+        slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
+      }
+      cp_commit();
+    };
+    if constexpr (!WG) {
+      Walk<WG> nx = f;
+      nx.next(p, pre);
+      row_next = nx.done() ? nullptr : pointer(nx, 0);
+    }
+    for (int i = 0; i < NU - 1; ++i) fetch();
+    const int steps = (t1 - t0) * n_k;
+    int slot = 0;
+    bool ok = true;
+    for (int it = 0; it < steps && ok; ++it) {
+      const int s = it & 1;
+#pragma unroll
+      for (int u = 0; u < S::UPC; ++u) {
+        cp_wait<NU - 2>();
+        __syncwarp();
+        fetch();
+        const uint32_t src = ring + slot * S::UNIT_A;
+        const uint8_t* const ms = mis + slot * 32;
+        slot = slot + 1 == NU ? 0 : slot + 1;
+        if (u == 0) {
+          if (it >= 2) ok = tc::mbar_wait_or_abort(A_FREE(s), ((it >> 1) - 1) & 1, abort);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc::fence_after_sync();
+        }
+        const uint32_t ta = tq + s * (PA * 32);
+        if constexpr (!WG) {
+          // this lane's row: 128 bytes of it
+          const int sh = VEC ? 0 : ms[lane];
+          auto piece = [&](int j) {
+            return lds128(src + lane * S::PITCH_A + (VEC ? (j ^ (lane & 7)) : j) * 16);
+          };
+          uint32_t out[PA][16];
+          uint4 cur = piece(0);
+#pragma unroll
+          for (int h = 0; h < 8 / (sizeof(TA) == 4 ? 8 : 4); ++h) {
+#pragma unroll
+            for (int q = 0; q < (sizeof(TA) == 4 ? 8 : 4); ++q) {
+              const int j = h * 4 + q;
+              uint4 v = cur;
+              if constexpr (VEC) {
+                if (j < 7) cur = piece(j + 1);
+              } else {
+                const uint4 nx = piece(j + 1);
+                v = shifted(cur, nx, sh);
+                cur = nx;
+              }
+              if constexpr (sizeof(TA) == 4) {
+                uint32_t t[3];
+                split2<PA>(__uint_as_float(v.x), __uint_as_float(v.y), t);
+#pragma unroll
+                for (int a = 0; a < PA; ++a) out[a][2 * q] = t[a];
+                split2<PA>(__uint_as_float(v.z), __uint_as_float(v.w), t);
+#pragma unroll
+                for (int a = 0; a < PA; ++a) out[a][2 * q + 1] = t[a];
+              } else {
+                out[0][4 * q] = v.x;
+                out[0][4 * q + 1] = v.y;
+                out[0][4 * q + 2] = v.z;
+                out[0][4 * q + 3] = v.w;
+              }
+            }
+            if constexpr (sizeof(TA) == 2) tmem_st16u(ta + h * 16, out[0]);
+          }
+          if constexpr (sizeof(TA) == 4) {
+#pragma unroll
+            for (int a = 0; a < PA; ++a) tmem_st16u(ta + a * 32 + u * 16, out[a]);
+          }
+        } else {
+          // this lane's channel of 32 rows
+          uint32_t out[PA][16];
+#pragma unroll
+          for (int r = 0; r < 32; r += 2) {
+            const uint32_t a0 = src + r * S::PITCH_A + lane * (int)sizeof(TA) + (VEC ? 0 : ms[r]);
+            const uint32_t a1 = src + (r + 1) * S::PITCH_A + lane * (int)sizeof(TA) + (VEC ? 0 : ms[r + 1]);
+            uint32_t t[3];
+            split2<PA>(lds_as(a0, TA{}), lds_as(a1, TA{}), t);
+#pragma unroll
+            for (int a = 0; a < PA; ++a) out[a][r / 2] = t[a];
+          }
+#pragma unroll
+          for (int a = 0; a < PA; ++a) tmem_st16u(ta + a * 32 + u * 16, out[a]);
+        }
+      }
+      if (ok) {
+        tc::tmem_wait_st();
+        tc::fence_before_sync();
+        tc::mbar_arrive(A_FULL(s));
+      }
+    }
+    cp_wait<0>();
+  } else if (warp < 8) {
+    // ---------------- operand B: 64-wide images, one column n per thread ----------------
+    const int w4 = warp - 4, n = w4 * 32 + lane;
+    if (w4 * 32 < NT) {
+      auto put = [&](uint32_t img, int chunk, const float* v) {  // 8 K-values of column n
+        uint32_t t[4][3];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) split2<PB>(v[2 * q], v[2 * q + 1], t[q]);
+#pragma unroll
+        for (int b = 0; b < PB; ++b)
+          sts128(img + b * NT * 128 + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
+      };
+      bool ok = true;
+      if constexpr (!WG) {
+        Walk<WG> w;
+        int it = 0, fills = 0;  // steps; weight images written (slot fills % NSLOT, or the step's own when resident)
+        for (w.init(p, pre, t0, t1); !w.done() && ok; w.next(p, pre)) {
+          const bool fill = !resident || w.new_weights();
+          const bool release = !resident || w.last_of_weights();
+          const T* wt = static_cast<const T*>(p.w) + (int64_t)w.g * p.K * p.N;
+          const int col = fill ? w.col_tile() * NT + n : 0;
+          for (int k = 0; k < n_k && ok; ++k, ++it) {
+            const int s = resident ? k : fills % S::NSLOT;
+            const int use = resident ? fills / n_k : fills / S::NSLOT;
+            if (fill) {
+              ++fills;
+              float v[32];
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const int k0 = k * SL_KC + half * 32;
+                if (!p.transposed) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j)
+                    v[j] = col < p.N && k0 + j < p.K ? to_f32(wt[(int64_t)(k0 + j) * p.N + col]) : 0.f;
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j)
+                    v[j] = col < p.N && k0 + j < p.K ? to_f32(wt[(int64_t)col * p.K + k0 + j]) : 0.f;
+                }
+                if (half == 0 && use > 0) {
+                  ok = __all_sync(0xffffffffu, tc::mbar_wait_or_abort(B_FREE(s), (use - 1) & 1, abort));
+                  if (!ok) break;
+                }
+                const uint32_t img = base + s * PB * S::IMG;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) put(img, half * 4 + q, v + 8 * q);
+              }
+              if (!ok) break;
+              tc::fence_proxy_async();
+              tc::mbar_arrive(B_FULL(s));
+            }
+            if (warp == 4) {
+              if (lane == 0) ok = issue(it, s, fill ? use : -1, release);
+              ok = __shfl_sync(0xffffffffu, ok, 0);
+            }
+          }
+        }
+        if (warp == 4 && lane == 0) drain();
+      } else {
+        const uint32_t ring = base + S::OFF_B + w4 * NU * S::UNIT_B;
+        uint8_t* const mis = smem + S::OFF_MIS + (4 + w4) * NU * 32;
+        float* const sc = reinterpret_cast<float*>(smem + S::OFF_SCALE) + w4 * NU * 32;
+        const int64_t row_bytes = (int64_t)p.b.width * sizeof(T);
+        const int64_t off = (int64_t)(wg_n0 + w4 * 32) * sizeof(T);
+        Walk<WG> f;
+        f.init(p, pre, t0, t1);
+        int fu = 0, slot_f = 0;
+        const char* row_next = nullptr;
+        float sc_next = 0.f;
+        auto pointer = [&]() {
+          const int64_t r = (int64_t)(f.t - f.first) * SL_KC + fu * 32 + lane;
+          int64_t srow = 0;
+          row_next = row_pointer(p, p.b, f.lo, f.rows, r, &srow);
+          if constexpr (sizeof(TA) == 1)
+            sc_next = row_next ? p.a_scale[srow * p.ka_blocks + wg_k0 / MACE_CHECKPOINT_BLOCK] : 0.f;
+        };
+        pointer();
+        auto fetch = [&]() {
+          if (!f.done()) {
+            fetch_unit<S::SEG_B, S::PITCH_B, VEC, false>(ring + slot_f * S::UNIT_B, row_next, off, row_bytes, p.b.data,
+                                                         mis + slot_f * 32);
+            if constexpr (sizeof(TA) == 1) sc[slot_f * 32 + lane] = sc_next;
+            if (++fu == 2) {
+              fu = 0;
+              f.next(p, pre);
+            }
+            if (!f.done()) pointer();
+            slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
+          }
+          cp_commit();
+        };
+        for (int i = 0; i < NU - 1; ++i) fetch();
+        int slot = 0;
+        for (int it = 0; it < t1 - t0 && ok; ++it) {
+          const int s = it & 1;
+#pragma unroll 1
+          for (int u = 0; u < 2; ++u) {
+            cp_wait<NU - 2>();
+            __syncwarp();
+            fetch();
+            const uint32_t src = ring + slot * S::UNIT_B;
+            const uint8_t* const ms = mis + slot * 32;
+            const float* const ss = sc + slot * 32;
+            slot = slot + 1 == NU ? 0 : slot + 1;
+            if (u == 0 && it >= 2) {
+              ok = __all_sync(0xffffffffu, tc::mbar_wait_or_abort(B_FREE(s), ((it >> 1) - 1) & 1, abort));
+              if (!ok) break;
+            }
+            const uint32_t img = base + s * PB * S::IMG;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float v[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int r = 8 * q + j;
+                v[j] = lds_as(src + r * S::PITCH_B + lane * (int)sizeof(T) + (VEC ? 0 : ms[r]), T{});
+                if constexpr (sizeof(TA) == 1) v[j] *= ss[r];
+              }
+              put(img, u * 4 + q, v);
+            }
+          }
+          if (ok) {
+            tc::fence_proxy_async();
+            tc::mbar_arrive(B_FULL(s));
+          }
+        }
+        cp_wait<0>();
+      }
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    const int quad = warp & 3, half = (warp - 8) >> 2;
+    const int CW = NT / 2;  // columns of this warp: 16, 32, 48 or 64
+    const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16) + SL_D + half * CW;
+    Walk<WG> w;
+    w.init(p, pre, t0, t1);
+    float acc[64];
+    bool ok = true;
+    bool fresh = true;  // acc holds nothing yet
+    // weight gradient: warp 8 issues the next step's MMAs before it takes this step's result
+    auto issue_wg = [&](int it) {
+      if (WG && warp == 8 && it < t1 - t0) {
+        if (lane == 0) ok = issue(it, it & 1, it >> 1, true);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+    };
+    issue_wg(0);
+    for (int it = 0; !w.done() && ok; ++it) {
+      const int s = it & 1;
+      issue_wg(it + 1);
+      if (!ok) break;
+      ok = tc::mbar_wait_or_abort(D_FULL(s), (it >> 1) & 1, abort);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc::fence_after_sync();
+      const uint32_t td = tq + s * 128;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[32];
+        if (h * 32 < CW) tmem_ld16u(td + h * 32, v);
+        if (h * 32 + 16 < CW) tmem_ld16u(td + h * 32 + 16, v + 16);
+        tc::tmem_wait_ld();
+        if (h == 1) {
+          tc::fence_before_sync();
+          tc::mbar_arrive(D_FREE(s));
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          acc[h * 32 + k] = fresh ? __uint_as_float(v[k]) : acc[h * 32 + k] + __uint_as_float(v[k]);
+      }
+      fresh = false;
+      if constexpr (!WG) {
+        if ((it + 1) % n_k != 0) continue;
+        const int64_t r = w.row0() + quad * 32 + lane;
+        const int c0 = w.col_tile() * NT + half * CW;
+        if (r < w.rows) {
+          const int64_t at = w.lo + r;
+          const int64_t i = at / p.d;
+          const int64_t node = p.order[i];
+          if (node >= 0 && node < p.n) {
+            T* dst = static_cast<T*>(p.out) + node * p.out_sn + (at - i * p.d) * p.out_sm + c0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              if (b * 16 >= CW) break;
+#pragma unroll
+              for (int k = 0; k < 16; ++k) acc[b * 16 + k] *= p.alpha;
+              if (p.N - c0 - b * 16 > 0) store16<T>(dst + b * 16, acc + b * 16, p.N - c0 - b * 16, p.vst);
+            }
+          }
+        }
+        fresh = true;
+        w.next(p, pre);
+      } else {
+        const bool group_ends = w.t + 1 == w.last;
+        if (group_ends || w.t + 1 == w.t1) {
+          const bool whole = group_ends && w.first >= t0;
+          const int kl = quad * 32 + lane, c0 = half * CW;
+          if (whole) {
+            if (wg_k0 + kl < p.K) {
+              T* dst = static_cast<T*>(p.out) + ((int64_t)w.g * p.K + wg_k0 + kl) * p.N + wg_n0 + c0;
+              const int left = p.N - wg_n0 - c0;
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                if (b * 16 >= CW) break;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) acc[b * 16 + k] *= p.alpha;
+                if (left - b * 16 > 0) store16<T>(dst + b * 16, acc + b * 16, left - b * 16, p.vst);
+              }
+            }
+          } else {
+            // (share, group) pairs of one tile are a staircase: share + g numbers them
+            float* dst = p.part + (((int64_t)tile * (p.shares + p.G) + share + w.g) * 128 + kl) * NT + c0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              if (b * 16 < CW) store16<float>(dst + b * 16, acc + b * 16, 16, 32);
+          }
+          fresh = true;
+        }
+        w.next(p, pre);
+      }
+    }
+    if (WG && warp == 8 && lane == 0) drain();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (tid == 0 && *abort) atomicExch(&g_species_error, TC_ERR_TIMEOUT);
+  if (warp == 8) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, SL_TMEM);
+  }
+}
+
+// dW of the groups that several shares hold, in share order, and of empty groups (zero).
+// One CTA: group blockIdx.x, 256 consecutive elements of tile blockIdx.z (64 lanes of
+// four columns x 4 share lanes).
+template <typename T>
+__global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constant__ SlParams p) {
+  __shared__ unsigned long long sum[2];
+  __shared__ float4 part[4][64];
+  const int g = blockIdx.x, tid = threadIdx.x;
+  if (tid < 2) sum[tid] = 0;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+  for (int i = tid; i < p.G; i += 256) {
+    const int64_t c = group_units(p, i, SL_KC);
+    all += c;
+    if (i < g) before += c;
+  }
+  const int64_t mine = group_units(p, g, SL_KC);
+  atomicAdd(&sum[0], (unsigned long long)before);  // whole numbers: any order gives the same sum
+  atomicAdd(&sum[1], (unsigned long long)all);
+  __syncthreads();
+  // as in group_prefix
+  before = min((int64_t)sum[0], (int64_t)INT32_MAX);
+  all = min((int64_t)sum[1], (int64_t)INT32_MAX);
+  const int tile = blockIdx.z;
+  const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
+  const int lane = tid & 63, sl = tid >> 6;
+  const int e = blockIdx.y * 256 + lane * 4;  // element of the 128 x NT tile
+  const int kl = e / p.NT, c = e % p.NT;
+  const bool in = e < 128 * p.NT && k0 + kl < p.K;
+  T* dst = static_cast<T*>(p.out) + ((int64_t)g * p.K + k0 + kl) * p.N + n0 + c;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (mine > 0) {
+    // share of unit u: the largest s with floor(s all / shares) <= u
+    const int64_t shares = min((int64_t)p.shares, all);
+    const int s0 = (int)min(((before + 1) * shares - 1) / all, shares - 1);
+    const int s1 = (int)min(((before + mine) * shares - 1) / all, shares - 1);
+    if (s0 == s1) return;  // written by its only share
+    if (in) {
+      const float* src = p.part + (((int64_t)tile * (p.shares + p.G) + g) * 128 + kl) * p.NT + c;
+#pragma unroll 4
+      for (int s = s0 + sl; s <= s1; s += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src + (int64_t)s * 128 * p.NT);
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
+      }
+    }
+    part[sl][lane] = acc;
+    __syncthreads();
+    if (sl != 0) return;
+#pragma unroll
+    for (int q = 1; q < 4; ++q) {
+      acc.x += part[q][lane].x;
+      acc.y += part[q][lane].y;
+      acc.z += part[q][lane].z;
+      acc.w += part[q][lane].w;
+    }
+  } else if (sl != 0) {
+    return;
+  }
+  if (!in) return;
+  const float v[4] = {p.alpha * acc.x, p.alpha * acc.y, p.alpha * acc.z, p.alpha * acc.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (n0 + c + k < p.N) dst[k] = from_f32<T>(v[k]);
+}
+
+// ------------------------------------------------------------------ host side
 bool bad_sizes(int32_t dtype, int64_t n, int32_t d, int32_t G, int32_t K, int32_t M) {
   return (dtype != MACE_F32 && dtype != MACE_BF16) || n < 0 || n > INT32_MAX || d < 1 || d > 1024 || G < 1 ||
-         G > MACE_SPECIES_MAX_GROUPS || K < 1 || K > 65536 || M < 1 || M > 65536;
+         G > MACE_SPECIES_MAX_GROUPS || K < 1 || K > 65536 || M < 1 || M > 65536 ||
+         (n * d + 63) / 64 + G > INT32_MAX / ((M + 31) / 32);
+}
+
+int sm_count() {
+  static int count[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 64) return 148;
+  if (count[dev] == 0) {
+    int v = 0;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) v = 148;
+    count[dev] = v;
+  }
+  return count[dev];
+}
+
+// columns of a tile: an even split of `cols` into multiples of 32, at most `most`
+int tile_cols(int cols, int most) {
+  const int tiles = (cols + most - 1) / most;
+  return std::min(most, ((cols + tiles - 1) / tiles + 31) / 32 * 32);
+}
+
+int vector_bytes(const void* ptr, int64_t s0, int64_t s1, int64_t s2) {
+  for (int v : {32, 16})
+    if (reinterpret_cast<uintptr_t>(ptr) % v == 0 && s0 % v == 0 && s1 % v == 0 && s2 % v == 0) return v;
+  return 0;
+}
+
+bool aligned_rows(const RowView& v, int64_t n, int d) {
+  return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && (n <= 1 || v.sn % 16 == 0) && (d <= 1 || v.sm % 16 == 0);
+}
+
+template <typename TA, typename T, bool WG, bool VEC>
+int launch_gemm(const SlParams& p, int grid, cudaStream_t s) {
+  constexpr int BYTES = Sl<TA, T, WG, VEC>::BYTES;
+  static bool attr_set[64] = {};  // per device: the attribute call is slow on the host
+  int dev = 0;
+  MACE_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !attr_set[dev]) {
+    MACE_CUDA_TRY(cudaFuncSetAttribute(k_species_gemm<TA, T, WG, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
+    if (dev < 64) attr_set[dev] = true;
+  }
+  k_species_gemm<TA, T, WG, VEC><<<grid, SL_THREADS, BYTES, s>>>(p);
+  MACE_LAUNCH_CHECK("species_gemm");
+  return MACE_OK;
+}
+
+// shares (CTAs along the rows) and tiles of a weight gradient
+void wgrad_split(int64_t n, int32_t d, int32_t G, int32_t K, int32_t M, SlParams* p) {
+  p->NT = tile_cols(M, 128);
+  p->n_ct = (M + p->NT - 1) / p->NT;
+  p->n_kt = (K + 127) / 128;
+  const int64_t units = (n * d + SL_KC - 1) / SL_KC + std::min<int64_t>(G, n);
+  const int tiles = p->n_ct * p->n_kt;
+  p->shares = (int)std::max<int64_t>(1, std::min<int64_t>(units, (sm_count() + tiles - 1) / tiles));
 }
 
 }  // namespace
@@ -157,27 +1010,46 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
       (n > 0 && (!x || !y || !order)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_linear: bad arguments");
   if (n == 0) return MACE_OK;
-  const int64_t tiles = (n * d + ST - 1) / ST + G + 1;
-  if (tiles > INT32_MAX) return fail(MACE_ERR_BAD_ARG, "mace_species_linear: too many rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)tiles, (M + ST - 1) / ST);
+  const int es = dtype == MACE_F32 ? 4 : 2;
+  SlParams p{};
+  p.a = {static_cast<const char*>(x), xn * es, xm * es, K};
+  p.w = w;
+  p.transposed = transpose;
+  p.out = y;
+  p.out_sn = yn;
+  p.out_sm = ym;
+  p.vst = vector_bytes(y, n > 1 ? yn * es : 0, d > 1 ? ym * es : 0, 0);
+  p.order = order;
+  p.offsets = offsets;
+  p.n = n;
+  p.d = d;
+  p.G = G;
+  p.K = K;
+  p.N = M;
+  p.alpha = alpha;
+  const int sms = sm_count();
+  const int64_t row_tiles = (n * d + 127) / 128;
+  // narrower column tiles while the row tiles leave SMs idle
+  int most = 128;
+  while (most > 32 && row_tiles * ((M + most - 1) / most) * 2 <= sms) most /= 2;
+  p.NT = tile_cols(M, most);
+  p.n_ct = (M + p.NT - 1) / p.NT;
+  p.n_kt = 1;
+  const int grid = (int)std::min<int64_t>(sms, (row_tiles + std::min<int64_t>(G, n)) * p.n_ct);
+  const bool vec = aligned_rows(p.a, n, d);
   if (dtype == MACE_F32)
-    k_species_linear<float><<<grid, 256, 0, s>>>(static_cast<const float*>(x), xn, xm, static_cast<const float*>(w),
-                                                 transpose, G, K, M, order, offsets, n, d, alpha,
-                                                 static_cast<float*>(y), yn, ym);
-  else
-    k_species_linear<bf16><<<grid, 256, 0, s>>>(static_cast<const bf16*>(x), xn, xm, static_cast<const bf16*>(w),
-                                                transpose, G, K, M, order, offsets, n, d, alpha,
-                                                static_cast<bf16*>(y), yn, ym);
-  MACE_LAUNCH_CHECK("species_linear");
-  return MACE_OK;
+    return vec ? launch_gemm<float, float, false, true>(p, grid, s) : launch_gemm<float, float, false, false>(p, grid, s);
+  return vec ? launch_gemm<bf16, bf16, false, true>(p, grid, s) : launch_gemm<bf16, bf16, false, false>(p, grid, s);
 }
 
 extern "C" int mace_species_linear_wgrad_workspace(int64_t n, int32_t d, int32_t G, int32_t K, int32_t M,
                                                    int64_t* bytes) {
   if (bad_sizes(MACE_F32, n, d, G, K, M) || !bytes)
     return fail(MACE_ERR_BAD_ARG, "mace_species_linear_wgrad_workspace: bad arguments");
-  *bytes = 0;
+  SlParams p{};
+  wgrad_split(n, d, G, K, M, &p);
+  *bytes = (int64_t)p.n_ct * p.n_kt * (p.shares + G) * 128 * p.NT * 4;
   return MACE_OK;
 }
 
@@ -188,25 +1060,50 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   if (bad_sizes(dtype, n, d, G, K, M) || xn < 0 || xm < 0 || yn < 0 || ym < 0 || !dw || !offsets ||
       (n > 0 && (!x || !dy || !order)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_linear_wgrad: bad arguments");
-  (void)ws;
-  (void)ws_bytes;
+  int64_t need = 0;
+  mace_species_linear_wgrad_workspace(n, d, G, K, M, &need);
+  if (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 31) != 0)
+    return fail(MACE_ERR_BAD_ARG, "mace_species_linear_wgrad: workspace too small or not 32-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const dim3 grid(G, (K + ST - 1) / ST, (M + ST - 1) / ST);
-  auto go = [&](auto tx, auto ty) {
-    using TX = decltype(tx);
-    using T = decltype(ty);
-    k_species_wgrad<TX, T><<<grid, 256, 0, s>>>(static_cast<const TX*>(x), xn, xm, xs, static_cast<const T*>(dy), yn,
-                                                ym, K, M, order, offsets, n, d, alpha, static_cast<T*>(dw));
-  };
-  if (xs && dtype == MACE_F32)
-    go(int8_t{}, float{});
-  else if (xs)
-    go(int8_t{}, bf16{});
-  else if (dtype == MACE_F32)
-    go(float{}, float{});
+  const int es = dtype == MACE_F32 ? 4 : 2, xe = xs ? 1 : es;
+  SlParams p{};
+  p.a = {static_cast<const char*>(x), xn * xe, xm * xe, K};
+  p.b = {static_cast<const char*>(dy), yn * es, ym * es, M};
+  p.a_scale = xs;
+  p.ka_blocks = (K + MACE_CHECKPOINT_BLOCK - 1) / MACE_CHECKPOINT_BLOCK;
+  p.out = dw;
+  p.vst = vector_bytes(dw, (int64_t)M * es, 0, 0);
+  p.part = static_cast<float*>(ws);
+  p.order = order;
+  p.offsets = offsets;
+  p.n = n;
+  p.d = d;
+  p.G = G;
+  p.K = K;
+  p.N = M;
+  p.alpha = alpha;
+  wgrad_split(n, d, G, K, M, &p);
+  const int grid = p.shares * p.n_ct * p.n_kt;
+  int rc = MACE_OK;
+  if (n > 0) {
+    const bool vec = aligned_rows(p.a, n, d) && aligned_rows(p.b, n, d);
+    auto go = [&](auto ta, auto t) {
+      using TA = decltype(ta);
+      using T = decltype(t);
+      return vec ? launch_gemm<TA, T, true, true>(p, grid, s) : launch_gemm<TA, T, true, false>(p, grid, s);
+    };
+    if (xs)
+      rc = dtype == MACE_F32 ? go(int8_t{}, float{}) : go(int8_t{}, bf16{});
+    else
+      rc = dtype == MACE_F32 ? go(float{}, float{}) : go(bf16{}, bf16{});
+    if (rc) return rc;
+  }
+  const dim3 jg(G, (128 * p.NT + 255) / 256, p.n_ct * p.n_kt);
+  if (dtype == MACE_F32)
+    k_species_wgrad_join<float><<<jg, 256, 0, s>>>(p);
   else
-    go(bf16{}, bf16{});
-  MACE_LAUNCH_CHECK("species_wgrad");
+    k_species_wgrad_join<bf16><<<jg, 256, 0, s>>>(p);
+  MACE_LAUNCH_CHECK("species_wgrad_join");
   return MACE_OK;
 }
 
