@@ -441,6 +441,7 @@ int mace_ctx_error_flag(mace_ctx* ctx, int32_t* flag);
 #define MACE_BF16 1
 #define MACE_SPECIES_MAX_GROUPS 512      /* of the species-indexed linear map */
 #define MACE_SPECIES_MAX_INDEX 1048575   /* num_groups of grouping and embedding */
+#define MACE_SPECIES_MAX_CHANNELS 32768
 #define MACE_CHECKPOINT_BLOCK 128        /* channels that share one 8-bit scale */
 
 /*

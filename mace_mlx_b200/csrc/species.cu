@@ -13,10 +13,32 @@ namespace mace {
 
 namespace {
 
+// row movers: threads of a CTA and vectors per thread (loads in flight)
+constexpr int RW_THREADS = 256;
+constexpr int RW_UNROLL = 4;
+
+// x / C for x < 2^32 / C by multiplication: the row of a CTA's local element
+// (x < RW_THREADS RW_UNROLL 8 + C and C <= 32768 stay below the limit)
+struct RowDiv {
+  uint32_t mul, one;
+  __device__ __forceinline__ uint32_t quotient(uint32_t x) const { return one ? x : __umulhi(x, mul); }
+};
+RowDiv row_div(int C) { return {(uint32_t)((((uint64_t)1 << 32) + C - 1) / C), C == 1 ? 1u : 0u}; }
+
+// Grouping is a stable counting sort by the key (species, or num_groups for
+// padding rows), with one digit of the key per pass.  A pass counts the digits
+// of every CTA's tile, scans the counts, and scatters: each warp ranks its rows
+// among equal digits with match_any, the tile is put in digit order in shared
+// memory, and runs of equal digits are written together.  Ranks follow the
+// list order everywhere, so the order of atomics plays no part.
 constexpr int GR_THREADS = 256;
 constexpr int GR_WARPS = GR_THREADS / 32;
-constexpr int GR_TILE = 4096;     // rows of one block of a counting pass
-constexpr int GR_MAX_BINS = 1024;  // bins of one counting pass
+constexpr int GR_TILE = 4096;      // rows of one CTA of a counting pass
+constexpr int GR_MAX_BINS = 1024;  // digits of one pass
+// short lists: one CTA does the whole sort in one launch
+constexpr int GS_THREADS = 1024;
+constexpr int GS_MAX_ROWS = 8192;
+constexpr int GS_MAX_BINS = 256;
 
 // key of a row: its species, or num_groups for padding rows
 __device__ __forceinline__ int row_key(int32_t z, int G) { return (z >= 0 && z < G) ? z : G; }
@@ -26,108 +48,257 @@ struct GroupPass {
   const int32_t* row;   // null in the first pass: row i is i
   int64_t n;
   int G;
-  int shift, bins;
-  int nb;               // blocks
-  int32_t* counts;      // (bins, nb)
+  int shift, bits;
+  int nb;               // CTAs
+  int32_t* counts;      // (bins, nb), after the scan exclusive within a digit
+  int32_t* totals;      // (bins)
   int32_t* key_out;     // null in a single pass
   int32_t* row_out;
+  int32_t* offsets;     // single pass: the group offsets; else null
 };
 
-__device__ __forceinline__ int digit_of(const GroupPass& p, int32_t z) { return (row_key(z, p.G) >> p.shift) % p.bins; }
+__device__ __forceinline__ int digit_of(const GroupPass& p, int32_t z) {
+  return (row_key(z, p.G) >> p.shift) & ((1 << p.bits) - 1);
+}
 
 __global__ void __launch_bounds__(GR_THREADS) k_group_count(GroupPass p) {
   __shared__ int hist[GR_MAX_BINS];
-  for (int b = threadIdx.x; b < p.bins; b += GR_THREADS) hist[b] = 0;
+  const int bins = 1 << p.bits;
+  for (int b = threadIdx.x; b < bins; b += GR_THREADS) hist[b] = 0;
   __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * GR_TILE, i1 = imin64(p.n, i0 + GR_TILE);
-  for (int64_t i = i0 + threadIdx.x; i < i1; i += GR_THREADS) atomicAdd(&hist[digit_of(p, p.key[i])], 1);
+  const int64_t i0 = (int64_t)blockIdx.x * GR_TILE;
+#pragma unroll
+  for (int j = 0; j < GR_TILE / GR_THREADS; ++j) {
+    const int64_t i = i0 + j * GR_THREADS + threadIdx.x;
+    if (i < p.n) atomicAdd(&hist[digit_of(p, p.key[i])], 1);
+  }
   __syncthreads();
-  for (int b = threadIdx.x; b < p.bins; b += GR_THREADS) p.counts[(int64_t)b * p.nb + blockIdx.x] = hist[b];
+  for (int b = threadIdx.x; b < bins; b += GR_THREADS) p.counts[(int64_t)b * p.nb + blockIdx.x] = hist[b];
 }
 
-// exclusive sums of m counts, in place, by one block
-__global__ void __launch_bounds__(1024) k_group_scan(int32_t* c, int64_t m) {
-  __shared__ int part[1024];
-  __shared__ int carry;
-  const int t = threadIdx.x;
-  if (t == 0) carry = 0;
-  __syncthreads();
-  for (int64_t base = 0; base < m; base += 1024) {
-    const int v = base + t < m ? c[base + t] : 0;
-    part[t] = v;
-    __syncthreads();
-    for (int o = 1; o < 1024; o <<= 1) {
-      const int a = t >= o ? part[t - o] : 0;
-      __syncthreads();
-      part[t] += a;
-      __syncthreads();
+// exclusive sums of one digit's counts over the CTAs, in place, and their total: a CTA per digit
+__global__ void __launch_bounds__(GR_THREADS) k_group_scan(GroupPass p) {
+  __shared__ int sums[GR_WARPS];
+  int32_t* c = p.counts + (int64_t)blockIdx.x * p.nb;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int carry = 0;
+  for (int base = 0; base < p.nb; base += GR_THREADS) {
+    const int i = base + threadIdx.x;
+    const int v = i < p.nb ? c[i] : 0;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
     }
-    if (base + t < m) c[base + t] = carry + part[t] - v;
+    if (lane == 31) sums[warp] = s;
     __syncthreads();
-    if (t == 0) carry += part[1023];
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < GR_WARPS; ++w) {
+      if (w < warp) before += sums[w];
+      all += sums[w];
+    }
+    if (i < p.nb) c[i] = carry + before + s - v;
+    carry += all;
     __syncthreads();
   }
+  if (threadIdx.x == 0) p.totals[blockIdx.x] = carry;
 }
 
+// exclusive sums over `count` values of a CTA's threads, thread by thread: value v, result returned
+template <int THREADS>
+__device__ __forceinline__ int cta_exclusive(int v, int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) warp_sums[warp] = s;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < warp; ++w) before += warp_sums[w];
+  __syncthreads();
+  return before + s - v;
+}
+
+// rank of this lane's digit among the equal digits of lower lanes; `mine`: next
+// position of each digit for this warp, moved past the rows placed here
+__device__ __forceinline__ int place(int* mine, int digit, bool in, int lane) {
+  const unsigned same = __match_any_sync(0xffffffffu, in ? digit : -1);
+  const int rank = __popc(same & ((1u << lane) - 1));
+  const int at = in ? mine[digit] + rank : 0;
+  __syncwarp();
+  if (in && rank == 0) mine[digit] += __popc(same);
+  __syncwarp();
+  return at;
+}
+
+struct ScatterSmem {
+  int32_t key[GR_TILE], row[GR_TILE];
+  int sums[GR_WARPS];
+};
+int scatter_bytes(int bins) { return (int)sizeof(ScatterSmem) + (GR_WARPS + 2) * bins * 4; }
+
 __global__ void __launch_bounds__(GR_THREADS) k_group_scatter(GroupPass p) {
-  extern __shared__ int whist[];  // (GR_WARPS, bins): next output position of a warp's rows of a digit
+  extern __shared__ int32_t dyn[];
+  ScatterSmem& sm = *reinterpret_cast<ScatterSmem*>(dyn);
+  const int bins = 1 << p.bits;
+  int* const whist = dyn + sizeof(ScatterSmem) / 4;  // (GR_WARPS, bins): counts, then next local positions
+  int* const lstart = whist + GR_WARPS * bins;       // first local position of a digit
+  int* const gstart = lstart + bins;                 // its first position in the result
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  for (int b = tid; b < GR_WARPS * p.bins; b += GR_THREADS) whist[b] = 0;
+  for (int b = tid; b < GR_WARPS * bins; b += GR_THREADS) whist[b] = 0;
   __syncthreads();
   constexpr int SEG = GR_TILE / GR_WARPS;  // consecutive rows of one warp
   const int64_t i0 = (int64_t)blockIdx.x * GR_TILE + warp * SEG, i1 = imin64(p.n, i0 + SEG);
-  int* mine = whist + warp * p.bins;
-  for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&mine[digit_of(p, p.key[i])], 1);
+  int* const mine = whist + warp * bins;
+  int32_t z[SEG / 32];
+#pragma unroll
+  for (int j = 0; j < SEG / 32; ++j) {
+    const int64_t i = i0 + j * 32 + lane;
+    z[j] = i < i1 ? row_key(p.key[i], p.G) : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < SEG / 32; ++j)
+    if (i0 + j * 32 + lane < i1) atomicAdd(&mine[digit_of(p, z[j])], 1);
   __syncthreads();
-  for (int b = tid; b < p.bins; b += GR_THREADS) {
-    int at = p.counts[(int64_t)b * p.nb + blockIdx.x];
+  // digits in runs of bins / GR_THREADS per thread: local starts and starts in the result
+  const int per = (bins + GR_THREADS - 1) / GR_THREADS;
+  int local = 0, global = 0;
+  for (int k = 0; k < per; ++k) {
+    const int b = tid * per + k;
+    if (b >= bins) break;
+    for (int w = 0; w < GR_WARPS; ++w) local += whist[w * bins + b];
+    global += p.totals[b];
+  }
+  int ls = cta_exclusive<GR_THREADS>(local, sm.sums);
+  int gs = cta_exclusive<GR_THREADS>(global, sm.sums);
+  for (int k = 0; k < per; ++k) {
+    const int b = tid * per + k;
+    if (b >= bins) break;
+    if (p.offsets && blockIdx.x == 0 && b <= p.G) p.offsets[b] = gs;
+    lstart[b] = ls;
+    gstart[b] = gs + p.counts[(int64_t)b * p.nb + blockIdx.x];
     for (int w = 0; w < GR_WARPS; ++w) {
-      const int c = whist[w * p.bins + b];
-      whist[w * p.bins + b] = at;
+      const int c = whist[w * bins + b];
+      whist[w * bins + b] = ls;
+      ls += c;
+    }
+    gs += p.totals[b];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < SEG / 32; ++j) {
+    const int64_t i = i0 + j * 32 + lane;
+    const bool in = i < i1;
+    const int at = place(mine, digit_of(p, z[j]), in, lane);
+    if (in) {
+      sm.key[at] = z[j];
+      sm.row[at] = p.row ? p.row[i] : (int32_t)i;
+    }
+  }
+  __syncthreads();
+  const int rows = (int)imin64(GR_TILE, p.n - (int64_t)blockIdx.x * GR_TILE);
+  for (int i = tid; i < rows; i += GR_THREADS) {
+    const int32_t key = sm.key[i];
+    const int dg = digit_of(p, key);
+    const int64_t at = gstart[dg] + (i - lstart[dg]);
+    p.row_out[at] = sm.row[i];
+    if (p.key_out) p.key_out[at] = key;
+  }
+}
+
+__global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __restrict__ species, int n, int G,
+                                                            int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
+  __shared__ int whist[32][GS_MAX_BINS];
+  __shared__ int sums[32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int bins = G + 1;
+  for (int b = lane; b < bins; b += 32) whist[warp][b] = 0;
+  __syncwarp();
+  const int seg = ((n + GS_THREADS - 1) / GS_THREADS) * 32;  // consecutive rows of one warp
+  const int i0 = warp * seg, i1 = min(n, i0 + seg);
+  for (int i = i0 + lane; i < i1; i += 32) atomicAdd(&whist[warp][row_key(species[i], G)], 1);
+  __syncthreads();
+  int total = 0;
+  if (tid < bins)
+    for (int w = 0; w < 32; ++w) total += whist[w][tid];
+  int at = cta_exclusive<GS_THREADS>(total, sums);
+  if (tid < bins) {
+    offsets[tid] = at;
+    for (int w = 0; w < 32; ++w) {
+      const int c = whist[w][tid];
+      whist[w][tid] = at;
       at += c;
     }
   }
   __syncthreads();
-  for (int64_t base = i0; base < i1; base += 32) {
-    const int64_t i = base + lane;
+  for (int base = i0; base < i1; base += 32) {
+    const int i = base + lane;
     const bool in = i < i1;
-    const int32_t z = in ? p.key[i] : 0;
-    const int dg = in ? digit_of(p, z) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, dg);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    int at = 0;
-    if (in) at = mine[dg] + rank;
-    __syncwarp();
-    if (in && rank == 0) mine[dg] += __popc(same);
-    __syncwarp();
-    if (in) {
-      p.row_out[at] = p.row ? p.row[i] : (int32_t)i;
-      if (p.key_out) p.key_out[at] = row_key(z, p.G);
-    }
+    const int key = in ? row_key(species[i], G) : 0;
+    const int to = place(whist[warp], key, in, lane);
+    if (in) order[to] = i;
   }
 }
 
 // offsets[v] = first position whose key is >= v
-__global__ void k_group_offsets(const int32_t* __restrict__ order, const int32_t* __restrict__ species, int64_t n, int G,
-                                int32_t* __restrict__ offsets) {
+__global__ void k_group_offsets(const int32_t* __restrict__ key, int64_t n, int G, int32_t* __restrict__ offsets) {
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i <= n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int prev = i > 0 ? row_key(species[order[i - 1]], G) : -1;
-    const int cur = i < n ? row_key(species[order[i]], G) : G;
+    const int prev = i > 0 ? key[i - 1] : -1;
+    const int cur = i < n ? key[i] : G;
     for (int v = prev + 1; v <= cur; ++v) offsets[v] = (int32_t)i;
   }
 }
 
-template <typename T>
-__global__ void k_embed(const T* __restrict__ table, int64_t ts, int G, int C, const int32_t* __restrict__ species,
-                        int64_t n, float scale, T* __restrict__ out, int64_t os) {
+// Consecutive vectors of V elements of the (n, C) result, CTA by CTA.
+// FLAT = 0: C is a multiple of V and every row is vector-aligned, so a vector
+// lies in one row; FLAT = 1: the result is contiguous and a vector may pass a
+// row's end (any C); V = 1 serves everything else.
+template <typename T, int V, bool FLAT>
+__global__ void __launch_bounds__(RW_THREADS) k_embed(const T* __restrict__ table, int64_t ts, int G, int C,
+                                                      const int32_t* __restrict__ species, int64_t n, float scale,
+                                                      T* __restrict__ out, int64_t os, RowDiv div) {
+  const int64_t v0 = blockIdx.x * (int64_t)(RW_THREADS * RW_UNROLL);  // first vector of this CTA
   const int64_t total = n * C;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / C;
-    const int c = (int)(i - r * C);
-    const int z = species[r];
-    float v = 0.f;
-    if (z >= 0 && z < G) v = scale * to_f32(table[z * ts + c]);
-    out[r * os + c] = from_f32<T>(v);
+  const int64_t row0 = (v0 * V) / C;
+  const uint32_t first = (uint32_t)(v0 * V - row0 * C);
+#pragma unroll
+  for (int j = 0; j < RW_UNROLL; ++j) {
+    const uint32_t local = first + (threadIdx.x + j * RW_THREADS) * V;
+    uint32_t r = div.quotient(local), c = local - r * C;
+    const int64_t at = v0 * V + (threadIdx.x + j * RW_THREADS) * V;
+    if (at >= total) continue;
+    float v[V];
+    int z = species[row0 + r];
+    if constexpr (!FLAT) {
+      if (z >= 0 && z < G)
+        load_channels<T, V>(table + z * ts + c, v);
+      else
+        for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] *= scale;
+      store_channels<T, V>(out + (row0 + r) * os + c, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        v[k] = z >= 0 && z < G ? scale * to_f32(table[z * ts + c]) : 0.f;
+        if (++c == (uint32_t)C) {
+          c = 0;
+          ++r;
+          z = row0 + r < n ? species[row0 + r] : -1;
+        }
+      }
+      if (at + V <= total)
+        store_channels<T, V>(out + at, v);
+      else
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (at + k < total) out[at + k] = from_f32<T>(v[k]);
+    }
   }
 }
 
@@ -169,13 +340,15 @@ constexpr int EG_THREADS = 256;
 template <typename T, int V, int RL>
 __global__ void __launch_bounds__(EG_THREADS) k_embed_grad(EmbedGrad p) {
   constexpr int CL = 32 / RL;  // channel lanes
+  constexpr int UN = 8;        // row loads in flight per lane
   const int lane = threadIdx.x & 31, cl = lane % CL, rl = lane / CL;
   const int64_t share = blockIdx.x * (int64_t)(EG_THREADS / 32) + (threadIdx.x >> 5);
   if (share >= p.shares) return;
   const int c0 = (blockIdx.y * CL + cl) * V;
+  const bool in = c0 < p.C;
   const int64_t i1 = imin64(p.n, (share + 1) * p.share);
   int64_t i = share * p.share;
-  const T* dy = static_cast<const T*>(p.dy);
+  const T* dy = static_cast<const T*>(p.dy) + (in ? c0 : 0);
   bool first = true;
   while (i < i1) {
     const int g = group_at(p.offsets, p.G, i);
@@ -183,30 +356,46 @@ __global__ void __launch_bounds__(EG_THREADS) k_embed_grad(EmbedGrad p) {
     const int64_t lo = p.offsets[g], hi = p.offsets[g + 1];
     const int64_t end = imin64(i1, hi);
     float acc[V] = {};
-    if (c0 < p.C) {
-#pragma unroll 4
-      for (int64_t r = i + rl; r < end; r += RL) {
-        const int64_t row = p.order[r];
-        if (row < 0 || row >= p.n) continue;
-        float v[V];
-        load_channels<T, V>(dy + row * p.ds + c0, v);
+    // 32 rows of the list at a time; a row outside the tensor counts as none
+    int32_t next = i + lane < end ? p.order[i + lane] : -1;
+    for (int64_t b = i; b < end; b += 32) {
+      const int32_t mine = next;
+      next = b + 32 + lane < end ? p.order[b + 32 + lane] : -1;
+      const int rows = (int)imin64(32, end - b);
+#pragma unroll 1
+      for (int j0 = 0; j0 < rows; j0 += UN * RL) {
+        float v[UN][V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += v[k];
+        for (int u = 0; u < UN; ++u) {
+          const int j = j0 + u * RL + rl;
+          const int64_t row = __shfl_sync(0xffffffffu, mine, j & 31);
+          if (j < 32 && row >= 0 && row < p.n && in) {
+            load_channels<T, V>(dy + row * p.ds, v[u]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[u][k] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[k] += v[u][k];
       }
     }
 #pragma unroll
     for (int o = CL; o < 32; o <<= 1)
 #pragma unroll
       for (int k = 0; k < V; ++k) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], o);
-    if (rl == 0 && c0 < p.C) {
+    if (rl == 0 && in) {
       const bool whole = lo >= share * p.share && hi <= i1;
-      float* part = p.part + (share * 2 + (first ? 0 : 1)) * p.C;
+      if (whole) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        if (whole)
-          static_cast<T*>(p.out)[(int64_t)g * p.C + c0 + k] = from_f32<T>(p.scale * acc[k]);
-        else
-          part[c0 + k] = acc[k];
+        for (int k = 0; k < V; ++k) acc[k] *= p.scale;
+        store_channels<T, V>(static_cast<T*>(p.out) + (int64_t)g * p.C + c0, acc);
+      } else {
+        float* part = p.part + (share * 2 + (first ? 0 : 1)) * p.C + c0;
+#pragma unroll
+        for (int k = 0; k < V; ++k) part[k] = acc[k];
       }
     }
     first = false;
@@ -214,79 +403,197 @@ __global__ void __launch_bounds__(EG_THREADS) k_embed_grad(EmbedGrad p) {
   }
 }
 
-// groups that several shares hold: their partial rows, in share order; empty groups: zero
+// Groups that several shares hold: their partial rows, in share order; empty
+// groups: zero.  A warp takes a group of few shares by itself; the CTA's 32
+// warps take the others together.  32 channels per CTA.
+constexpr int EJ_ALONE = 16;
+
 template <typename T>
 __global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p) {
   __shared__ float sums[32][33];
-  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+  __shared__ uint32_t many;
+  const int cl = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.y * 32 + cl;
   T* out = static_cast<T*>(p.out);
-  for (int g = blockIdx.x; g < p.G; g += gridDim.x) {
+  auto span = [&](int g, int64_t* s0, int64_t* s1) -> bool {  // shares of group g; false: empty
     const Range r = group_range(p.offsets, g, p.n);
-    if (r.lo >= r.hi) {
-      if (rl == 0 && c < p.C) out[(int64_t)g * p.C + c] = from_f32<T>(0.f);
-      continue;
-    }
-    const int64_t s0 = r.lo / p.share, s1 = (r.hi - 1) / p.share;
-    if (s0 == s1) continue;  // final already
+    if (r.lo >= r.hi) return false;
+    *s0 = r.lo / p.share;
+    *s1 = (r.hi - 1) / p.share;
+    return true;
+  };
+  auto partial = [&](int g, int64_t from, int64_t s0, int64_t s1, int step) -> float {
     float acc = 0.f;
     if (c < p.C) {
-#pragma unroll 4
-      for (int64_t s = s0 + rl; s <= s1; s += 32) {
-        // a share that the group enters from before it holds its first row there
-        const int which = s > s0 || r.lo == s * p.share ? 0 : 1;
+#pragma unroll 8
+      for (int64_t s = from; s <= s1; s += step) {
+        // the group is the second of its first share's partial rows unless the share begins with it
+        const int which = s > s0 || (int64_t)p.offsets[g] <= s * p.share ? 0 : 1;
         acc += p.part[(s * 2 + which) * p.C + c];
       }
     }
-    sums[rl][cl] = acc;
+    return acc;
+  };
+  for (int g0 = blockIdx.x * 32; g0 < p.G; g0 += gridDim.x * 32) {
+    if (threadIdx.x == 0) many = 0;
     __syncthreads();
-    if (rl == 0 && c < p.C) {
-      float t = 0.f;
-#pragma unroll
-      for (int k = 0; k < 32; ++k) t += sums[k][cl];
-      out[(int64_t)g * p.C + c] = from_f32<T>(p.scale * t);
+    const int g = g0 + warp;
+    int64_t s0 = 0, s1 = 0;
+    if (g < p.G) {
+      if (!span(g, &s0, &s1)) {
+        if (c < p.C) out[(int64_t)g * p.C + c] = from_f32<T>(0.f);
+      } else if (s1 - s0 >= EJ_ALONE) {
+        if (cl == 0) atomicOr(&many, 1u << warp);
+      } else if (s1 > s0 && c < p.C) {  // one share: final already
+        out[(int64_t)g * p.C + c] = from_f32<T>(p.scale * partial(g, s0, s0, s1, 1));
+      }
     }
     __syncthreads();
+    for (uint32_t left = many; left; left &= left - 1) {
+      const int h = g0 + __ffs(left) - 1;
+      span(h, &s0, &s1);
+      sums[warp][cl] = partial(h, s0 + warp, s0, s1, 32);
+      __syncthreads();
+      if (warp == 0 && c < p.C) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) t += sums[k][cl];
+        out[(int64_t)h * p.C + c] = from_f32<T>(p.scale * t);
+      }
+      __syncthreads();
+    }
   }
 }
 
-template <typename T>
-__global__ void k_checkpoint(const T* __restrict__ x, int64_t xn, int64_t xm, int64_t rows, int d, int C, int nb,
-                             int8_t* __restrict__ q, float* __restrict__ scale) {
+// A warp quantises CK_ROWS consecutive (row, block) items; VEC: lane l holds
+// channels 4 l .. 4 l + 3 of the block (rows aligned to four channels), else
+// channels l, l + 32, l + 64, l + 96.
+constexpr int CK_ROWS = 4;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* __restrict__ x, int64_t xn, int64_t xm, int64_t rows,
+                                                           int d, int C, int nb, int8_t* __restrict__ q,
+                                                           float* __restrict__ scale) {
   const int lane = threadIdx.x & 31;
-  const int64_t item = blockIdx.x * (int64_t)(blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (item >= rows * nb) return;
-  const int64_t r = item / nb;
-  const int b = (int)(item - r * nb);
-  const T* src = x + (r / d) * xn + (r % d) * xm;
-  float v[4], top = 0.f;
-  bool bad = false;
+  const int64_t items = rows * nb;
+  const int64_t i0 = (blockIdx.x * (int64_t)(RW_THREADS / 32) + (threadIdx.x >> 5)) * CK_ROWS;
+  if (i0 >= items) return;
+  // node, component and block of the first item; the others follow by counting
+  int64_t r = nb == 1 ? i0 : i0 / nb;
+  int b = (int)(i0 - r * nb);
+  int64_t node = d == 1 ? r : r / d;
+  int m = (int)(r - node * d);
+  const int64_t row0 = r;
+  const int b0 = b;
+  float v[CK_ROWS][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = b * MACE_CHECKPOINT_BLOCK + j * 32 + lane;
-    v[j] = c < C ? to_f32(src[c]) : 0.f;
-    bad |= v[j] != v[j];
-    top = fmaxf(top, fabsf(v[j]));
-  }
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (__any_sync(0xffffffffu, bad)) top = __int_as_float(0x7fc00000);
-  const float s = __fmul_rn(top, 1.0f / 127.0f);
-  if (lane == 0) scale[item] = s;
+  for (int u = 0; u < CK_ROWS; ++u) {
+    const int c0 = b * MACE_CHECKPOINT_BLOCK + (VEC ? 4 * lane : lane);
+    const bool in = i0 + u < items;
+    const T* src = x + node * xn + m * xm;
+    if constexpr (VEC) {
+      if (in && c0 < C) {
+        load4(src + c0, v[u]);
+      } else {
+        v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.f;
+      }
+    } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = b * MACE_CHECKPOINT_BLOCK + j * 32 + lane;
-    if (c < C) q[r * C + c] = quantise8(v[j], s);
+      for (int j = 0; j < 4; ++j) v[u][j] = in && c0 + 32 * j < C ? to_f32(src[c0 + 32 * j]) : 0.f;
+    }
+    if (++b == nb) {
+      b = 0;
+      if (++m == d) {
+        m = 0;
+        ++node;
+      }
+    }
   }
+  r = row0;
+  b = b0;
+  float mine = 0.f;  // lane u's scale
+#pragma unroll
+  for (int u = 0; u < CK_ROWS; ++u) {
+    // the largest magnitude by its bits: order of floats, with NaN above infinity
+    int top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, __float_as_int(v[u][j]) & 0x7fffffff);
+    top = __reduce_max_sync(0xffffffffu, top);
+    const float s = __fmul_rn(__int_as_float(top), 1.0f / 127.0f);
+    if (lane == u) mine = s;
+    const int c0 = b * MACE_CHECKPOINT_BLOCK + (VEC ? 4 * lane : lane);
+    if (i0 + u < items) {
+      int8_t* dst = q + r * C + c0;
+      if constexpr (VEC) {
+        if (c0 < C)
+          *reinterpret_cast<char4*>(dst) = make_char4(quantise8(v[u][0], s), quantise8(v[u][1], s),
+                                                      quantise8(v[u][2], s), quantise8(v[u][3], s));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c0 + 32 * j < C) dst[32 * j] = quantise8(v[u][j], s);
+      }
+    }
+    if (++b == nb) {
+      b = 0;
+      ++r;
+    }
+  }
+  if (lane < CK_ROWS && i0 + lane < items) scale[i0 + lane] = mine;
 }
 
+// Four consecutive elements of the contiguous (rows, C) result per thread and step; a vector may pass a row's end.
 template <typename T>
-__global__ void k_restore(const int8_t* __restrict__ q, const float* __restrict__ scale, int64_t rows, int C, int nb,
-                          T* __restrict__ x) {
-  const int64_t total = rows * C;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / C;
-    const int c = (int)(i - r * C);
-    x[i] = from_f32<T>((float)q[i] * scale[r * nb + c / MACE_CHECKPOINT_BLOCK]);
+__global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* __restrict__ q, const float* __restrict__ scale,
+                                                        int64_t total, int C, int nb, T* __restrict__ x, RowDiv div,
+                                                        int vec) {
+  const int64_t e0 = blockIdx.x * (int64_t)(RW_THREADS * RW_UNROLL * 4);
+  const int64_t row0 = e0 / C;
+  const uint32_t first = (uint32_t)(e0 - row0 * C);
+  char4 w[RW_UNROLL];
+#pragma unroll
+  for (int j = 0; j < RW_UNROLL; ++j) {
+    const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
+    if (vec && at + 4 <= total) {
+      w[j] = *reinterpret_cast<const char4*>(q + at);
+    } else {
+      w[j].x = at < total ? q[at] : 0;
+      w[j].y = at + 1 < total ? q[at + 1] : 0;
+      w[j].z = at + 2 < total ? q[at + 2] : 0;
+      w[j].w = at + 3 < total ? q[at + 3] : 0;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < RW_UNROLL; ++j) {
+    const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
+    if (at >= total) break;
+    const uint32_t local = first + (threadIdx.x + j * RW_THREADS) * 4;
+    const uint32_t r = div.quotient(local), c = local - r * C;
+    const float* sc = scale + (row0 + r) * nb;
+    const float qv[4] = {(float)w[j].x, (float)w[j].y, (float)w[j].z, (float)w[j].w};
+    float v[4];
+    if (c + 4 <= (uint32_t)C && c / MACE_CHECKPOINT_BLOCK == (c + 3) / MACE_CHECKPOINT_BLOCK) {
+      const float s = sc[c / MACE_CHECKPOINT_BLOCK];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = qv[k] * s;
+    } else {
+      uint32_t ck = c;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = at + k < total ? qv[k] * sc[ck / MACE_CHECKPOINT_BLOCK] : 0.f;
+        if (++ck == (uint32_t)C) {
+          ck = 0;
+          sc += nb;
+        }
+      }
+    }
+    if (vec && at + 4 <= total) {
+      store4(x + at, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (at + k < total) x[at + k] = from_f32<T>(v[k]);
+    }
   }
 }
 
@@ -315,53 +622,90 @@ int64_t align16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 
 using namespace mace;
 
+namespace {
+
+struct GroupPlan {
+  int bits, passes, nb;
+  int64_t counts, keys, bytes;  // bytes of the count tables, of one key or row array, and of the whole workspace
+};
+bool group_plan(int64_t n, int32_t G, GroupPlan* p) {
+  if (n < 0 || n > INT32_MAX || G < 1 || G > MACE_SPECIES_MAX_INDEX) return false;
+  group_passes(G, &p->bits, &p->passes);
+  p->nb = (int)((n + GR_TILE - 1) / GR_TILE);
+  p->counts = align16(((int64_t)p->nb + 1) * (1 << p->bits) * 4);
+  p->keys = align16(n * 4);
+  // two passes: keys and rows after the first, keys after the second
+  p->bytes = p->counts + (p->passes > 1 ? 3 * p->keys : 0);
+  return true;
+}
+
+}  // namespace
+
 extern "C" int mace_species_group_workspace(int64_t n, int32_t G, int64_t* bytes) {
-  if (n < 0 || n > INT32_MAX || G < 1 || G > MACE_SPECIES_MAX_INDEX || !bytes)
+  GroupPlan plan;
+  if (!group_plan(n, G, &plan) || !bytes)
     return fail(MACE_ERR_BAD_ARG, "mace_species_group_workspace: bad arguments");
-  int bits, passes;
-  group_passes(G, &bits, &passes);
-  const int64_t nb = (n + GR_TILE - 1) / GR_TILE;
-  *bytes = align16(((int64_t)1 << bits) * nb * 4) + (passes > 1 ? 2 * align16(n * 4) : 0);
+  *bytes = plan.bytes;
   return MACE_OK;
 }
 
 extern "C" int mace_species_group(const int32_t* species, int64_t n, int32_t G, int32_t* order, int32_t* offsets,
                                   void* ws, int64_t ws_bytes, void* stream) {
-  int64_t need = 0;
-  if (mace_species_group_workspace(n, G, &need) != MACE_OK || !offsets || (n > 0 && (!species || !order)))
+  GroupPlan plan;
+  if (!group_plan(n, G, &plan) || !offsets || (n > 0 && (!species || !order)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_group: bad arguments");
-  if (n > 0 && (!ws || ws_bytes < need)) return fail(MACE_ERR_BAD_ARG, "mace_species_group: workspace too small");
+  if (n > 0 && (!ws || ws_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(ws) & 15) != 0))
+    return fail(MACE_ERR_BAD_ARG, "mace_species_group: workspace too small or not 16-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (n == 0) {
     MACE_CUDA_TRY(cudaMemsetAsync(offsets, 0, (size_t)(G + 1) * 4, s));
     return MACE_OK;
   }
-  int bits, passes;
-  group_passes(G, &bits, &passes);
+  if (n <= GS_MAX_ROWS && G < GS_MAX_BINS) {
+    k_group_small<<<1, GS_THREADS, 0, s>>>(species, (int)n, G, order, offsets);
+    MACE_LAUNCH_CHECK("group_small");
+    return MACE_OK;
+  }
   GroupPass p{};
   p.n = n;
   p.G = G;
-  p.bins = 1 << bits;
-  p.nb = (int)((n + GR_TILE - 1) / GR_TILE);
-  p.counts = static_cast<int32_t*>(ws);
-  int32_t* key2 = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + align16((int64_t)p.bins * p.nb * 4));
-  int32_t* row2 = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(key2) + align16(n * 4));
-  for (int q = 0; q < passes; ++q) {
-    p.shift = q * bits;
-    p.key = q == 0 ? species : key2;
-    p.row = q == 0 ? nullptr : row2;
-    const bool last = q == passes - 1;
-    p.key_out = last ? nullptr : key2;
-    p.row_out = last ? order : row2;
+  p.bits = plan.bits;
+  p.nb = plan.nb;
+  const int bins = 1 << plan.bits;
+  char* at = static_cast<char*>(ws);
+  p.counts = reinterpret_cast<int32_t*>(at);
+  p.totals = p.counts + (int64_t)bins * p.nb;
+  int32_t* key1 = reinterpret_cast<int32_t*>(at + plan.counts);
+  int32_t* row1 = reinterpret_cast<int32_t*>(at + plan.counts + plan.keys);
+  int32_t* key2 = reinterpret_cast<int32_t*>(at + plan.counts + 2 * plan.keys);
+  const int smem = scatter_bytes(bins);
+  static bool attr_set[64] = {};  // per device: the attribute call is slow on the host
+  int dev = 0;
+  MACE_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !attr_set[dev]) {
+    MACE_CUDA_TRY(cudaFuncSetAttribute(k_group_scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       scatter_bytes(GR_MAX_BINS)));
+    if (dev < 64) attr_set[dev] = true;
+  }
+  for (int q = 0; q < plan.passes; ++q) {
+    const bool last = q == plan.passes - 1;
+    p.shift = q * plan.bits;
+    p.key = q == 0 ? species : key1;
+    p.row = q == 0 ? nullptr : row1;
+    p.key_out = plan.passes == 1 ? nullptr : (last ? key2 : key1);
+    p.row_out = last ? order : row1;
+    p.offsets = plan.passes == 1 ? offsets : nullptr;
     k_group_count<<<p.nb, GR_THREADS, 0, s>>>(p);
     MACE_LAUNCH_CHECK("group_count");
-    k_group_scan<<<1, 1024, 0, s>>>(p.counts, (int64_t)p.bins * p.nb);
+    k_group_scan<<<bins, GR_THREADS, 0, s>>>(p);
     MACE_LAUNCH_CHECK("group_scan");
-    k_group_scatter<<<p.nb, GR_THREADS, GR_WARPS * p.bins * 4, s>>>(p);
+    k_group_scatter<<<p.nb, GR_THREADS, smem, s>>>(p);
     MACE_LAUNCH_CHECK("group_scatter");
   }
-  k_group_offsets<<<(int)blocks_for(n + 1, 256, 148 * 8), 256, 0, s>>>(order, species, n, G, offsets);
-  MACE_LAUNCH_CHECK("group_offsets");
+  if (plan.passes > 1) {
+    k_group_offsets<<<(int)blocks_for(n + 1, 256, 148 * 8), 256, 0, s>>>(key2, n, G, offsets);
+    MACE_LAUNCH_CHECK("group_offsets");
+  }
   return MACE_OK;
 }
 
@@ -369,27 +713,48 @@ namespace {
 bool bad_dtype(int32_t t) { return t != MACE_F32 && t != MACE_BF16; }
 }  // namespace
 
-extern "C" int mace_species_embed(int32_t dtype, const void* table, int64_t ts, int32_t G, int32_t C,
-                                  const int32_t* species, int64_t n, float scale, void* out, int64_t os,
-                                  void* stream) {
-  if (bad_dtype(dtype) || G < 1 || G > MACE_SPECIES_MAX_INDEX || C < 1 || n < 0 || n > INT32_MAX || ts < 0 ||
-      !table || (n > 0 && (!species || !out || os < C)))
-    return fail(MACE_ERR_BAD_ARG, "mace_species_embed: bad arguments");
-  if (n == 0) return MACE_OK;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int grid = (int)blocks_for(n * C, 256, 148 * 16);
-  if (dtype == MACE_F32)
-    k_embed<float><<<grid, 256, 0, s>>>(static_cast<const float*>(table), ts, G, C, species, n, scale,
-                                        static_cast<float*>(out), os);
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T>
+int embed(const void* table, int64_t ts, int G, int C, const int32_t* species, int64_t n, float scale, void* out,
+          int64_t os, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const T* t = static_cast<const T*>(table);
+  T* o = static_cast<T*>(out);
+  auto grid = [&](int v) {
+    const int64_t per = (int64_t)RW_THREADS * RW_UNROLL * v;
+    return (unsigned)((n * C + per - 1) / per);
+  };
+  if (C % V == 0 && ts % V == 0 && os % V == 0 && aligned16(table) && aligned16(out))
+    k_embed<T, V, false><<<grid(V), RW_THREADS, 0, s>>>(t, ts, G, C, species, n, scale, o, os, row_div(C));
+  else if (os == C && aligned16(out))
+    k_embed<T, V, true><<<grid(V), RW_THREADS, 0, s>>>(t, ts, G, C, species, n, scale, o, os, row_div(C));
   else
-    k_embed<bf16><<<grid, 256, 0, s>>>(static_cast<const bf16*>(table), ts, G, C, species, n, scale,
-                                       static_cast<bf16*>(out), os);
+    k_embed<T, 1, false><<<grid(1), RW_THREADS, 0, s>>>(t, ts, G, C, species, n, scale, o, os, row_div(C));
   MACE_LAUNCH_CHECK("species_embed");
   return MACE_OK;
 }
 
+}  // namespace
+
+extern "C" int mace_species_embed(int32_t dtype, const void* table, int64_t ts, int32_t G, int32_t C,
+                                  const int32_t* species, int64_t n, float scale, void* out, int64_t os,
+                                  void* stream) {
+  if (bad_dtype(dtype) || G < 1 || G > MACE_SPECIES_MAX_INDEX || C < 1 || C > MACE_SPECIES_MAX_CHANNELS ||
+      n < 0 || n > INT32_MAX || ts < 0 ||
+      !table || (n > 0 && (!species || !out || os < C)))
+    return fail(MACE_ERR_BAD_ARG, "mace_species_embed: bad arguments");
+  if (n == 0) return MACE_OK;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == MACE_F32 ? embed<float>(table, ts, G, C, species, n, scale, out, os, s)
+                           : embed<bf16>(table, ts, G, C, species, n, scale, out, os, s);
+}
+
 extern "C" int mace_species_embed_grad_workspace(int64_t n, int32_t G, int32_t C, int64_t* bytes) {
-  if (n < 0 || n > INT32_MAX || G < 1 || G > MACE_SPECIES_MAX_INDEX || C < 1 || !bytes)
+  if (n < 0 || n > INT32_MAX || G < 1 || G > MACE_SPECIES_MAX_INDEX || C < 1 ||
+      C > MACE_SPECIES_MAX_CHANNELS || !bytes)
     return fail(MACE_ERR_BAD_ARG, "mace_species_embed_grad_workspace: bad arguments");
   *bytes = eg_shares(n, eg_share(n)) * 2 * C * 4;
   return MACE_OK;
@@ -416,13 +781,13 @@ template <typename T>
 int embed_grad(const EmbedGrad& p, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   if (p.n > 0) {
-    if (p.C % V == 0 && p.ds % V == 0 && (reinterpret_cast<uintptr_t>(p.dy) & 15) == 0)
+    if (p.C % V == 0 && p.ds % V == 0 && aligned16(p.dy) && aligned16(p.out))
       launch_embed_grad<T, V>(p, s);
     else
       launch_embed_grad<T, 1>(p, s);
     MACE_LAUNCH_CHECK("species_embed_grad");
   }
-  k_embed_grad_join<T><<<dim3((unsigned)std::min(p.G, 148 * 8), (p.C + 31) / 32), 1024, 0, s>>>(p);
+  k_embed_grad_join<T><<<dim3((unsigned)std::min((p.G + 31) / 32, 148 * 2), (p.C + 31) / 32), 1024, 0, s>>>(p);
   MACE_LAUNCH_CHECK("species_embed_grad_join");
   return MACE_OK;
 }
@@ -432,7 +797,8 @@ int embed_grad(const EmbedGrad& p, cudaStream_t s) {
 extern "C" int mace_species_embed_grad(int32_t dtype, const void* grad, int64_t gs, const int32_t* order,
                                        const int32_t* offsets, int64_t n, int32_t G, int32_t C, float scale,
                                        void* out, void* ws, int64_t ws_bytes, void* stream) {
-  if (bad_dtype(dtype) || n < 0 || n > INT32_MAX || G < 1 || G > MACE_SPECIES_MAX_INDEX || C < 1 || gs < 0 || !out ||
+  if (bad_dtype(dtype) || n < 0 || n > INT32_MAX || G < 1 || G > MACE_SPECIES_MAX_INDEX || C < 1 ||
+      C > MACE_SPECIES_MAX_CHANNELS || gs < 0 || !out ||
       !offsets || (n > 0 && (!grad || !order)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_embed_grad: bad arguments");
   int64_t need = 0;
@@ -447,34 +813,49 @@ extern "C" int mace_species_embed_grad(int32_t dtype, const void* grad, int64_t 
 
 extern "C" int mace_rows_checkpoint(int32_t dtype, const void* x, int64_t xn, int64_t xm, int64_t n, int32_t d,
                                     int32_t C, int8_t* q, float* scale, void* stream) {
-  if (bad_dtype(dtype) || n < 0 || n > INT32_MAX || d < 1 || d > 1024 || C < 1 || xn < 0 || xm < 0 ||
+  if (bad_dtype(dtype) || n < 0 || n > INT32_MAX || d < 1 || d > 1024 || C < 1 || C > MACE_SPECIES_MAX_CHANNELS || xn < 0 || xm < 0 ||
       (n > 0 && (!x || !q || !scale)))
     return fail(MACE_ERR_BAD_ARG, "mace_rows_checkpoint: bad arguments");
   if (n == 0) return MACE_OK;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int nb = (C + MACE_CHECKPOINT_BLOCK - 1) / MACE_CHECKPOINT_BLOCK;
-  const int64_t grid = (n * d * nb + 7) / 8;
+  const int64_t per = RW_THREADS / 32 * CK_ROWS;
+  const int64_t grid = (n * d * nb + per - 1) / per;
   if (grid > INT32_MAX) return fail(MACE_ERR_BAD_ARG, "mace_rows_checkpoint: too many rows");
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    const T* src = static_cast<const T*>(x);
+    const bool vec = C % 4 == 0 && (n <= 1 || xn % 4 == 0) && (d <= 1 || xm % 4 == 0) &&
+                     reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(q) % 4 == 0;
+    if (vec)
+      k_checkpoint<T, true><<<(int)grid, RW_THREADS, 0, s>>>(src, xn, xm, n * d, d, C, nb, q, scale);
+    else
+      k_checkpoint<T, false><<<(int)grid, RW_THREADS, 0, s>>>(src, xn, xm, n * d, d, C, nb, q, scale);
+  };
   if (dtype == MACE_F32)
-    k_checkpoint<float><<<(int)grid, 256, 0, s>>>(static_cast<const float*>(x), xn, xm, n * d, d, C, nb, q, scale);
+    go(float{});
   else
-    k_checkpoint<bf16><<<(int)grid, 256, 0, s>>>(static_cast<const bf16*>(x), xn, xm, n * d, d, C, nb, q, scale);
+    go(bf16{});
   MACE_LAUNCH_CHECK("rows_checkpoint");
   return MACE_OK;
 }
 
 extern "C" int mace_rows_restore(int32_t dtype, const int8_t* q, const float* scale, int64_t n, int32_t d, int32_t C,
                                  void* x, void* stream) {
-  if (bad_dtype(dtype) || n < 0 || n > INT32_MAX || d < 1 || d > 1024 || C < 1 || (n > 0 && (!x || !q || !scale)))
+  if (bad_dtype(dtype) || n < 0 || n > INT32_MAX || d < 1 || d > 1024 || C < 1 ||
+      C > MACE_SPECIES_MAX_CHANNELS || (n > 0 && (!x || !q || !scale)))
     return fail(MACE_ERR_BAD_ARG, "mace_rows_restore: bad arguments");
   if (n == 0) return MACE_OK;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int nb = (C + MACE_CHECKPOINT_BLOCK - 1) / MACE_CHECKPOINT_BLOCK;
-  const int grid = (int)blocks_for(n * d * C, 256, 148 * 16);
+  const int64_t total = n * d * C, per = RW_THREADS * RW_UNROLL * 4;
+  if ((total + per - 1) / per > INT32_MAX) return fail(MACE_ERR_BAD_ARG, "mace_rows_restore: too many rows");
+  const unsigned grid = (unsigned)((total + per - 1) / per);
+  const int vec = reinterpret_cast<uintptr_t>(q) % 4 == 0 && aligned16(x);
   if (dtype == MACE_F32)
-    k_restore<float><<<grid, 256, 0, s>>>(q, scale, n * d, C, nb, static_cast<float*>(x));
+    k_restore<float><<<grid, RW_THREADS, 0, s>>>(q, scale, total, C, nb, static_cast<float*>(x), row_div(C), vec);
   else
-    k_restore<bf16><<<grid, 256, 0, s>>>(q, scale, n * d, C, nb, static_cast<bf16*>(x));
+    k_restore<bf16><<<grid, RW_THREADS, 0, s>>>(q, scale, total, C, nb, static_cast<bf16*>(x), row_div(C), vec);
   MACE_LAUNCH_CHECK("rows_restore");
   return MACE_OK;
 }

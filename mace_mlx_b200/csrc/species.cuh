@@ -32,6 +32,40 @@ __device__ __forceinline__ void load_channels(const T* __restrict__ src, float* 
   }
 }
 
+template <typename T, int V>
+__device__ __forceinline__ void store_channels(T* __restrict__ dst, const float* v) {
+  if constexpr (V * sizeof(T) == 16) {
+    uint4 u;
+    T* t = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int k = 0; k < V; ++k) t[k] = from_f32<T>(v[k]);
+    *reinterpret_cast<uint4*>(dst) = u;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) dst[k] = from_f32<T>(v[k]);
+  }
+}
+
+// four consecutive values, aligned to four
+__device__ __forceinline__ void load4(const float* src, float* v) {
+  const float4 u = __ldg(reinterpret_cast<const float4*>(src));
+  v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+}
+__device__ __forceinline__ void load4(const bf16* src, float* v) {
+  const uint2 u = __ldg(reinterpret_cast<const uint2*>(src));
+  v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
+  v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float* dst, const float* v) {
+  *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(bf16* dst, const float* v) {
+  bf16 t[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) t[k] = from_f32<bf16>(v[k]);
+  *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t);
+}
+
 // 8-bit value of x at scale s = max |x| / 127 (0 where s is 0, infinite or NaN);
 // the clamp only acts where s is subnormal and the quotient may pass 127
 __device__ __forceinline__ int8_t quantise8(float x, float s) {

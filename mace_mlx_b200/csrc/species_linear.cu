@@ -938,7 +938,8 @@ __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constan
 // ------------------------------------------------------------------ host side
 bool bad_sizes(int32_t dtype, int64_t n, int32_t d, int32_t G, int32_t K, int32_t M) {
   return (dtype != MACE_F32 && dtype != MACE_BF16) || n < 0 || n > INT32_MAX || d < 1 || d > 1024 || G < 1 ||
-         G > MACE_SPECIES_MAX_GROUPS || K < 1 || K > 65536 || M < 1 || M > 65536 ||
+         G > MACE_SPECIES_MAX_GROUPS || K < 1 || K > MACE_SPECIES_MAX_CHANNELS || M < 1 ||
+         M > MACE_SPECIES_MAX_CHANNELS ||
          (n * d + 63) / 64 + G > INT32_MAX / ((M + 31) / 32);
 }
 

@@ -144,6 +144,7 @@ DTYPE_F32 = 0
 DTYPE_BF16 = 1
 SPECIES_MAX_GROUPS = 512
 SPECIES_MAX_INDEX = 1048575
+SPECIES_MAX_CHANNELS = 32768
 CHECKPOINT_BLOCK = 128
 
 _lib = None

@@ -106,8 +106,9 @@ def _rows(name: str, t: torch.Tensor) -> tuple[int, int, int, int, int]:
         sm = c
     else:
         raise ValueError(f"{name} must be (N, d, C) or (N, C), got {tuple(shape)}")
-    if c < 1 or not 1 <= d <= 1024:
-        raise ValueError(f"{name}: need at least one channel and 1..1024 components, got {tuple(shape)}")
+    if not 1 <= c <= nv.SPECIES_MAX_CHANNELS or not 1 <= d <= 1024:
+        raise ValueError(f"{name}: need 1..{nv.SPECIES_MAX_CHANNELS} channels and 1..1024 components, "
+                         f"got {tuple(shape)}")
     if sc != 1 and c > 1:
         raise ValueError(f"{name}: channels must be contiguous (stride 1), got strides {t.stride()}")
     return n, d, c, sn, sm
