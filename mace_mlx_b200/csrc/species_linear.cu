@@ -72,7 +72,9 @@ struct SlParams {
   const int32_t* offsets;
   int64_t n;
   int d, G;
+  int small;            // n d < 2^32: row numbers divide in 32 bits
   int K, N;             // map: K summed channels, N outputs; weight gradient: K x N of dW
+  int w_vec;            // map: 8 consecutive weights load as vectors
   int NT;               // tile columns: 32, 64, 96 or 128
   int n_ct, n_kt;       // column tiles; weight gradient: row (channel) tiles
   int shares;           // weight gradient: CTAs along the rows
@@ -95,8 +97,22 @@ __device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a, uint64_t bde
       : "memory");
 }
 
+// true on one lane of a converged warp; the compiler knows the branch is uniform
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -230,7 +246,7 @@ struct Sl {
   static constexpr int SEG_B = 32 * (int)sizeof(T);
   static constexpr int PITCH_A = SEG_A + (VEC ? 0 : 16), PITCH_B = SEG_B + (VEC ? 0 : 16);
   static constexpr int UPC = WG ? 2 : SL_KC * (int)sizeof(TA) / 128;  // ring units per step of 64
-  static constexpr int NU = WG ? (VEC ? 4 : 3) : (sizeof(TA) == 4 ? 7 : 6);
+  static constexpr int NU = WG ? (VEC ? 4 : 3) : (VEC ? 6 : 5);
   static constexpr int UNIT_A = 32 * PITCH_A, UNIT_B = 32 * PITCH_B;
   static constexpr int IMG = 128 * 128;  // one piece of a B image: NT <= 128 rows of 64 bf16
   static constexpr int NSLOT = !WG && PB == 1 ? 4 : 2;
@@ -239,7 +255,9 @@ struct Sl {
   static constexpr int OFF_MIS = OFF_B + (WG ? 4 * NU * UNIT_B : 0);        // per ring unit and row: misalignment
   static constexpr int OFF_SCALE = OFF_MIS + (VEC ? 0 : (WG ? 8 : 4) * NU * 32);  // per B ring unit and row: A's scale
   static constexpr int OFF_PRE = OFF_SCALE + (sizeof(TA) == 1 ? 4 * NU * 32 * 4 : 0);
-  static constexpr int OFF_BAR = OFF_PRE + ((MACE_SPECIES_MAX_GROUPS + 2) * 4 + 7) / 8 * 8;
+  static constexpr int STG = 32 * 17 * 4;  // map: 32 rows x 16 columns of an epilogue warp, for unaligned results
+  static constexpr int OFF_STG = OFF_PRE + ((MACE_SPECIES_MAX_GROUPS + 2) * 4 + 7) / 8 * 8;
+  static constexpr int OFF_BAR = OFF_STG + (WG ? 0 : 8 * STG);
   static constexpr int NBAR = 8 + 2 * NSLOT + 1;
   static constexpr int BYTES = OFF_BAR + NBAR * 8 + 32;
   static_assert(BYTES <= 232448, "shared memory of a CTA");
@@ -288,85 +306,126 @@ __device__ __forceinline__ int group_of_unit(const int* pre, int G, int t) {
 template <bool WG>
 struct Walk {
   int t, t0, t1, g;
-  int first, last;  // units of group g: [first, last)
-  int64_t lo, rows; // group's first grouped row (in components) and its row count
+  int first, last;   // units of group g: [first, last)
+  int ct, rt, n_rt;  // map: column tile, row tile, row tiles of the group
+  int64_t lo, rows;  // group's first grouped row (components counted) and its row count
   __device__ __forceinline__ void load(const SlParams& p, const int* pre) {
     const Range r = group_range(p.offsets, g, p.n);
     first = pre[g];
     last = pre[g + 1];
     lo = r.lo * p.d;
     rows = (r.hi - r.lo) * p.d;
+    if (!WG) n_rt = (int)((rows + 127) >> 7);
   }
   __device__ __forceinline__ void init(const SlParams& p, const int* pre, int t0_, int t1_) {
     t = t0 = t0_;
     t1 = t1_;
     g = group_of_unit(pre, p.G, t);
     load(p, pre);
+    if (!WG) {
+      ct = (t - first) / n_rt;
+      rt = (t - first) - ct * n_rt;
+    }
   }
   __device__ __forceinline__ bool done() const { return t >= t1; }
   __device__ __forceinline__ void next(const SlParams& p, const int* pre) {
-    if (++t < last || t >= t1) return;
+    ++t;
+    if (!WG && ++rt == n_rt) {
+      rt = 0;
+      ++ct;
+    }
+    if (t < last || t >= t1) return;
     do ++g;
     while (pre[g + 1] <= t);
     load(p, pre);
+    ct = rt = 0;
   }
-  // map: row tiles of the group, this tile's column tile and row tile
-  __device__ __forceinline__ int row_tiles() const { return (int)((rows + 127) >> 7); }
-  __device__ __forceinline__ int col_tile() const { return (t - first) / row_tiles(); }
-  __device__ __forceinline__ int64_t row0() const { return (int64_t)((t - first) % row_tiles()) * 128; }
+  // first row of the tile or unit, within its group
+  __device__ __forceinline__ int64_t row0() const {
+    return WG ? (int64_t)(t - first) * SL_KC : (int64_t)rt * 128;
+  }
   // map: first / last tile of its (group, column tile) in this CTA: the weight images are new / free after it
-  __device__ __forceinline__ bool new_weights() const { return t == t0 || (t - first) % row_tiles() == 0; }
-  __device__ __forceinline__ bool last_of_weights() const {
-    return t + 1 == t1 || (t + 1 - first) % row_tiles() == 0;
-  }
+  __device__ __forceinline__ bool new_weights() const { return t == t0 || rt == 0; }
+  __device__ __forceinline__ bool last_of_weights() const { return t + 1 == t1 || rt + 1 == n_rt; }
 };
 
-// this lane's row of a 32-row unit: bytes (node, m) of view v, or null outside the group
-__device__ __forceinline__ const char* row_pointer(const SlParams& p, const RowView& v, int64_t lo, int64_t rows,
-                                                   int64_t r, int64_t* scale_row) {
-  if (r >= rows) return nullptr;
-  const int64_t at = lo + r;
-  const int64_t i = p.d == 1 ? at : at / p.d;
-  const int m = (int)(at - i * p.d);
-  const int64_t node = p.order[i];
-  if (node < 0 || node >= p.n) return nullptr;
-  if (scale_row) *scale_row = node * p.d + m;
-  return v.data + node * v.sn + m * v.sm;
+// A lane's row of the grouped list: its atom is loaded ahead of use (`node`
+// stays in flight until offset() reads it).
+struct RowRef {
+  int node, m;  // node < 0: no row
+  __device__ __forceinline__ void load(const SlParams& p, int64_t lo, int64_t rows, int64_t r) {
+    node = -1;
+    m = 0;
+    if (r >= rows) return;
+    const int64_t at = lo + r;
+    int64_t i = at;
+    if (p.d > 1) {
+      i = p.small ? (int64_t)((uint32_t)at / (uint32_t)p.d) : at / p.d;
+      m = (int)(at - i * p.d);
+    }
+    node = p.order[i];
+  }
+  __device__ __forceinline__ bool valid(const SlParams& p) const { return node >= 0 && node < p.n; }
+  __device__ __forceinline__ int64_t offset(const RowView& v) const { return node * v.sn + m * v.sm; }
+};
+
+// One ring unit: 32 row segments of SEG bytes.  VEC: lane l copies 16-byte piece
+// l % PPR of rows l / PPR + i RPI, whose offsets (in 16 bytes, NO_ROW: zeros) it
+// holds in off[i]; SWZ stores piece j of row r at j ^ (r & 7).
+constexpr uint32_t NO_ROW = 0xffffffffu;
+
+template <int SEG>
+struct Pieces {
+  static constexpr int PPR = SEG / 16, RPI = 32 / PPR, N = PPR;
+};
+
+template <int SEG>
+__device__ __forceinline__ void spread_rows(uint32_t mine, uint32_t* off) {
+  using P = Pieces<SEG>;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < P::N; ++i) off[i] = __shfl_sync(0xffffffffu, mine, i * P::RPI + lane / P::PPR);
 }
 
-// 32 row segments of SEG bytes at byte `off` of each lane's row, into ring unit `dst`
-template <int SEG, int PITCH, bool VEC, bool SWZ>
-__device__ __forceinline__ void fetch_unit(uint32_t dst, const char* row, int64_t off, int64_t row_bytes,
-                                           const char* data, uint8_t* mis) {
+// `at`: first byte of the segment within its row; ZERO: rows may be NO_ROW
+template <int SEG, int PITCH, bool SWZ, bool ZERO>
+__device__ __forceinline__ void fetch_vec(uint32_t dst, const char* data, const uint32_t* off, int64_t at,
+                                          int64_t row_bytes) {
+  using P = Pieces<SEG>;
+  const int lane = threadIdx.x & 31, j = lane % P::PPR, r0 = lane / P::PPR;
+  const int64_t left = row_bytes - at - 16 * j;
+  const uint32_t bytes = left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
+  const char* const src = bytes ? data + at + 16 * j : data;
+#pragma unroll
+  for (int i = 0; i < P::N; ++i) {
+    const int r = i * P::RPI + r0;
+    const int pos = SWZ ? (j ^ (r & 7)) : j;
+    const bool none = ZERO && off[i] == NO_ROW;
+    cp_async16(dst + r * PITCH + pos * 16, none ? src : src + (uint64_t)off[i] * 16, none ? 0u : bytes);
+  }
+}
+
+// Rows of any alignment: the 16-byte units that contain the segment; mis[r]:
+// where it starts in the first.  row: this lane's row (null: zeros).
+template <int SEG, int PITCH>
+__device__ __forceinline__ void fetch_any(uint32_t dst, const char* data, const char* row, int64_t at,
+                                          int64_t row_bytes, uint8_t* mis) {
+  constexpr int PPR = SEG / 16 + 1;
   const int lane = threadIdx.x & 31;
   // copies of no bytes still name an aligned address
   const char* const dummy = reinterpret_cast<const char*>(reinterpret_cast<uint64_t>(data) & ~(uint64_t)15);
-  if constexpr (VEC) {
-    constexpr int PPR = SEG / 16, RPI = 32 / PPR;  // pieces per row, rows per instruction
+  const int seg = (int)max(min(row_bytes - at, (int64_t)SEG), (int64_t)0);  // bytes of a row in this segment
+  const uint64_t from = row ? reinterpret_cast<uint64_t>(row + at) : 0;
+  mis[lane] = (uint8_t)(from & 15);
 #pragma unroll
-    for (int i = 0; i < PPR; ++i) {
-      const int r = i * RPI + lane / PPR, j = lane % PPR;
-      const char* base = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row), r));
-      const int64_t left = row_bytes - off - 16 * j;
-      const uint32_t bytes = base == nullptr || left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
-      const int pos = SWZ ? (j ^ (r & 7)) : j;
-      cp_async16(dst + r * PITCH + pos * 16, bytes ? base + off + 16 * j : dummy, bytes);
-    }
-  } else {
-    constexpr int PPR = SEG / 16 + 1;
-    const int shift = row ? (int)(reinterpret_cast<uint64_t>(row + off) & 15) : 0;
-    mis[lane] = (uint8_t)shift;
-#pragma unroll
-    for (int i = 0; i < PPR; ++i) {
-      const int q = i * 32 + lane;
-      const int r = q / PPR, j = q - r * PPR;
-      const char* base = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row), r));
-      const int64_t seg = min(row_bytes - off, (int64_t)SEG);  // bytes of the row in this segment
-      const char* src = reinterpret_cast<const char*>(reinterpret_cast<uint64_t>(base + off) & ~(uint64_t)15) + 16 * j;
-      const int64_t left = base + off + seg - src;
-      const uint32_t bytes = base == nullptr || seg <= 0 || left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
-      cp_async16(dst + r * PITCH + j * 16, bytes ? src : dummy, bytes);
-    }
+  for (int i = 0; i < PPR; ++i) {
+    const int q = i * 32 + lane;
+    const int r = q / PPR, j = q - r * PPR;
+    const uint64_t f = __shfl_sync(0xffffffffu, from, r);
+    const int left = (int)(f & 15) + seg - 16 * j;
+    const uint32_t bytes = f == 0 || seg == 0 || left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
+    cp_async16(dst + r * PITCH + j * 16, bytes ? reinterpret_cast<const char*>((f & ~(uint64_t)15) + 16 * j) : dummy,
+               bytes);
   }
 }
 
@@ -404,7 +463,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   auto B_FULL = [&](int s) { return bar(8 + s); };
   auto B_FREE = [&](int s) { return bar(8 + S::NSLOT + s); };
   const uint32_t DONE = bar(8 + 2 * S::NSLOT);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be uniform
 
   if (base & 1023u) {  // the images need 1024-byte alignment
     if (tid == 0) atomicExch(&g_species_error, TC_ERR_ALIGN);
@@ -452,7 +512,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         tc::mbar_init(D_FREE(s), 256);
       }
       for (int s = 0; s < S::NSLOT; ++s) {
-        tc::mbar_init(B_FULL(s), NT);
+        tc::mbar_init(B_FULL(s), WG ? NT : 128);
         tc::mbar_init(B_FREE(s), 1);
       }
       tc::mbar_init(DONE, 1);
@@ -465,33 +525,43 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = *tslot;
+  const uint32_t tmem = SL_D;  // an allocation of all 512 columns starts at column 0
 
-  // MMAs of step `it` with the images of slot bs (one thread); `use`: how often
-  // the slot was filled before, or -1 when its images were there already
+  // MMAs of step `it` with the images of slot bs, by a whole warp with warp-uniform
+  // operands (one elected lane issues); `use`: how often the slot was filled
+  // before, or -1 when its images were there already
   auto issue = [&](int it, int bs, int use, bool release) -> bool {
     using PR = Products<PA, PB>;
-    const uint32_t idesc = idesc_bf16(NT);
     const int s = it & 1;
-    if (use >= 0 && !tc::mbar_wait_or_abort(B_FULL(bs), use & 1, abort)) return false;
-    if (!tc::mbar_wait_or_abort(A_FULL(s), (it >> 1) & 1, abort)) return false;
-    if (it >= 2 && !tc::mbar_wait_or_abort(D_FREE(s), ((it >> 1) - 1) & 1, abort)) return false;
+    bool ok = use < 0 || tc::mbar_wait_or_abort(B_FULL(bs), use & 1, abort);
+    ok = ok && tc::mbar_wait_or_abort(A_FULL(s), (it >> 1) & 1, abort);
+    if (ok && it >= 2) ok = tc::mbar_wait_or_abort(D_FREE(s), ((it >> 1) - 1) & 1, abort);
+    if (!__all_sync(0xffffffffu, ok)) return false;
     tc::fence_after_sync();
-    const uint32_t img = base + bs * PB * S::IMG;
+    const uint32_t us = __shfl_sync(0xffffffffu, s, 0), ub = __shfl_sync(0xffffffffu, bs, 0);
+    const uint32_t idesc = idesc_bf16(p.NT);
+    const uint64_t desc = tc::sw128_desc(base + ub * (PB * S::IMG));
+    const uint32_t d = SL_D + us * 128, a = SL_A + us * (PA * 32);
+    if (elect_one()) {
 #pragma unroll
-    for (int q = 0; q < PR::n; ++q)
+      for (int q = 0; q < PR::n; ++q)
 #pragma unroll
-      for (int ks = 0; ks < SL_KC / 16; ++ks)
-        mma_bf16_ta(tmem + SL_D + s * 128, tmem + SL_A + s * (PA * 32) + PR::a(q) * 32 + ks * 8,
-                    tc::sw128_desc(img + PR::b(q) * NT * 128 + ks * 32), idesc, q > 0 || ks > 0);
-    tc::mma_commit(A_FREE(s));
-    if (release) tc::mma_commit(B_FREE(bs));
-    tc::mma_commit(D_FULL(s));
+        for (int ks = 0; ks < SL_KC / 16; ++ks)
+          mma_bf16_ta(d, a + PR::a(q) * 32 + ks * 8, desc + (uint32_t)(PR::b(q) * p.NT * 8 + ks * 2), idesc,
+                      q > 0 || ks > 0);
+      tc::mma_commit(A_FREE(s));
+      if (release) tc::mma_commit(B_FREE(bs));
+      tc::mma_commit(D_FULL(s));
+    }
+    __syncwarp();
     return true;
   };
   auto drain = [&]() {  // every MMA issued is complete (bounded)
-    tc::mma_commit(DONE);
-    tc::mbar_wait(DONE, 0);
+    if (elect_one()) {
+      tc::mma_commit(DONE);
+      tc::mbar_wait(DONE, 0);
+    }
+    __syncwarp();
   };
 
   if (warp < 4) {
@@ -500,55 +570,61 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     uint8_t* const mis = smem + S::OFF_MIS + warp * NU * 32;
     const int64_t row_bytes = (int64_t)p.a.width * sizeof(TA);
     const uint32_t tq = tmem + ((uint32_t)(warp * 32) << 16) + SL_A;
-    // the fetching side runs NU - 1 units ahead
+    // the fetching side runs NU - 1 units ahead; atoms of the rows after it are loaded one (map: tile, else: unit) earlier
     Walk<WG> f;
     f.init(p, pre, t0, t1);
     int fk = 0, fu = 0, slot_f = 0;  // step of the tile, unit of the step, ring slot
-    const char *row = nullptr, *row_next = nullptr;
-    auto pointer = [&](const Walk<WG>& w, int u) -> const char* {
-      const int64_t r = WG ? (int64_t)(w.t - w.first) * SL_KC + u * 32 + lane : w.row0() + warp * 32 + lane;
-      return row_pointer(p, p.a, w.lo, w.rows, r, nullptr);
+    RowRef ref;
+    uint32_t off[Pieces<S::SEG_A>::N];
+    const char* row = nullptr;
+    auto load_rows = [&]() {
+      ref.load(p, f.lo, f.rows, WG ? f.row0() + fu * 32 + lane : f.row0() + warp * 32 + lane);
     };
-    if constexpr (!WG) row = pointer(f, 0);
+    // the loaded rows become the fetched ones.  Map: a row outside the tile may hold anything (its
+    // TMEM lane is never stored), so it stands for row 0; weight gradient: it must be zero
+    auto take_rows = [&]() {
+      const bool ok = ref.valid(p);
+      const int64_t o = ok ? ref.offset(p.a) : 0;
+      if constexpr (VEC)
+        spread_rows<S::SEG_A>(WG && !ok ? NO_ROW : (uint32_t)(o >> 4), off);
+      else
+        row = WG && !ok ? nullptr : p.a.data + o;
+    };
     auto fetch = [&]() {
       if (!f.done()) {
-        int64_t off;
+        const bool fresh = WG || (fk == 0 && fu == 0);
+        if (fresh) take_rows();
+        const int64_t at = WG ? (int64_t)(wg_k0 + warp * 32) * sizeof(TA) : (int64_t)fk * SL_KC * sizeof(TA) + fu * 128;
+        const uint32_t dst = ring + slot_f * S::UNIT_A;
+        if constexpr (VEC)
+          fetch_vec<S::SEG_A, S::PITCH_A, !WG, WG>(dst, p.a.data, off, at, row_bytes);
+        else
+          fetch_any<S::SEG_A, S::PITCH_A>(dst, p.a.data, row, at, row_bytes, mis + slot_f * 32);
+        slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
         if constexpr (WG) {
-          row = fu == 0 && f.t == t0 ? pointer(f, 0) : row_next;
-          off = (int64_t)(wg_k0 + warp * 32) * sizeof(TA);
-        } else {
-          off = (int64_t)fk * SL_KC * sizeof(TA) + fu * 128;
-        }
-        fetch_unit<S::SEG_A, S::PITCH_A, VEC, !WG>(ring + slot_f * S::UNIT_A, row, off, row_bytes, p.a.data,
-                                                   mis + slot_f * 32);
-        // pointers of the next unit (map: of the next tile), ahead of their use
-        if (++fu == S::UPC) {
-          fu = 0;
-          if (++fk == n_k) {
-            fk = 0;
+          if (++fu == S::UPC) {
+            fu = 0;
             f.next(p, pre);
-            if constexpr (!WG) {
-              row = row_next;
+          }
+          if (!f.done()) load_rows();
+        } else {
+          if (fresh) {  // the next tile's rows
+            Walk<WG> nx = f;
+            nx.next(p, pre);
+            if (!nx.done()) ref.load(p, nx.lo, nx.rows, nx.row0() + warp * 32 + lane);
+          }
+          if (++fu == S::UPC) {
+            fu = 0;
+            if (++fk == n_k) {
+              fk = 0;
+              f.next(p, pre);
             }
           }
         }
-        if constexpr (WG) {
-          if (!f.done()) row_next = pointer(f, fu);
-        } else if (fk == 0 && fu == 0) {
-          // the tile after the one whose fetch starts now
-          Walk<WG> nx = f;
-          if (!nx.done()) nx.next(p, pre);
-          row_next = nx.done() ? nullptr : pointer(nx, 0);
-        }
-        slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
       }
       cp_commit();
     };
-    if constexpr (!WG) {
-      Walk<WG> nx = f;
-      nx.next(p, pre);
-      row_next = nx.done() ? nullptr : pointer(nx, 0);
-    }
+    load_rows();
     for (int i = 0; i < NU - 1; ++i) fetch();
     const int steps = (t1 - t0) * n_k;
     int slot = 0;
@@ -637,92 +713,135 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     cp_wait<0>();
   } else if (warp < 8) {
     // ---------------- operand B: 64-wide images, one column n per thread ----------------
-    const int w4 = warp - 4, n = w4 * 32 + lane;
-    if (w4 * 32 < NT) {
-      auto put = [&](uint32_t img, int chunk, const float* v) {  // 8 K-values of column n
-        uint32_t t[4][3];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) split2<PB>(v[2 * q], v[2 * q + 1], t[q]);
-#pragma unroll
-        for (int b = 0; b < PB; ++b)
-          sts128(img + b * NT * 128 + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
-      };
-      bool ok = true;
+    const int w4 = warp - 4;
+    bool ok = true;
+    {
       if constexpr (!WG) {
-        Walk<WG> w;
-        int it = 0, fills = 0;  // steps; weight images written (slot fills % NSLOT, or the step's own when resident)
-        for (w.init(p, pre, t0, t1); !w.done() && ok; w.next(p, pre)) {
-          const bool fill = !resident || w.new_weights();
-          const bool release = !resident || w.last_of_weights();
-          const T* wt = static_cast<const T*>(p.w) + (int64_t)w.g * p.K * p.N;
-          const int col = fill ? w.col_tile() * NT + n : 0;
-          for (int k = 0; k < n_k && ok; ++k, ++it) {
-            const int s = resident ? k : fills % S::NSLOT;
-            const int use = resident ? fills / n_k : fills / S::NSLOT;
-            if (fill) {
-              ++fills;
-              float v[32];
+        // 8 K-values of image row n
+        auto put = [&](uint32_t img, int n, int chunk, const float* v) {
+          uint32_t t[4][3];
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const int k0 = k * SL_KC + half * 32;
-                if (!p.transposed) {
+          for (int q = 0; q < 4; ++q) split2<PB>(v[2 * q], v[2 * q + 1], t[q]);
 #pragma unroll
-                  for (int j = 0; j < 32; ++j)
-                    v[j] = col < p.N && k0 + j < p.K ? to_f32(wt[(int64_t)(k0 + j) * p.N + col]) : 0.f;
+          for (int b = 0; b < PB; ++b)
+            sts128(img + b * NT * 128 + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
+        };
+        // the images of steps [k0, k0 + nk): items of 32 (image row, K octet) pairs, taken in turn by the
+        // four warps, four at a time so that 32 values per lane are in flight.  Weights (K, N): lanes are 32
+        // neighbouring columns; transposed (N, K): 4 rows x 8 octets, 256 contiguous bytes of each row
+        auto fill = [&](int g, int ct, int k0, int nk, int slot0) {
+          const T* wt = static_cast<const T*>(p.w) + (int64_t)g * p.K * p.N;
+          const int per = NT / 4;  // items of a step: NT / 32 blocks of columns x 8 octets, or NT / 4 blocks of rows
+          for (int i0 = w4; i0 < nk * per; i0 += 16) {
+            float v[4][8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int i = i0 + 4 * u;
+              const int step = i / per, j = i - step * per;
+              const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane;
+              const int chunk = p.transposed ? lane & 7 : j & 7;
+              const int col = ct * NT + n, k = (k0 + step) * SL_KC + chunk * 8;
+              const bool in = i < nk * per && col < p.N;
+              if (p.transposed) {
+                const T* src = wt + (int64_t)col * p.K + k;
+                if (p.w_vec && in && k + 8 <= p.K) {
+                  load_eight(src, v[u]);
                 } else {
 #pragma unroll
-                  for (int j = 0; j < 32; ++j)
-                    v[j] = col < p.N && k0 + j < p.K ? to_f32(wt[(int64_t)col * p.K + k0 + j]) : 0.f;
+                  for (int e = 0; e < 8; ++e) v[u][e] = in && k + e < p.K ? to_f32(src[e]) : 0.f;
                 }
-                if (half == 0 && use > 0) {
-                  ok = __all_sync(0xffffffffu, tc::mbar_wait_or_abort(B_FREE(s), (use - 1) & 1, abort));
-                  if (!ok) break;
-                }
-                const uint32_t img = base + s * PB * S::IMG;
+              } else {
+                const T* src = wt + (int64_t)k * p.N + col;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) put(img, half * 4 + q, v + 8 * q);
+                for (int e = 0; e < 8; ++e) v[u][e] = in && k + e < p.K ? to_f32(src[(int64_t)e * p.N]) : 0.f;
               }
-              if (!ok) break;
-              tc::fence_proxy_async();
-              tc::mbar_arrive(B_FULL(s));
             }
-            if (warp == 4) {
-              if (lane == 0) ok = issue(it, s, fill ? use : -1, release);
-              ok = __shfl_sync(0xffffffffu, ok, 0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int i = i0 + 4 * u;
+              if (i >= nk * per) break;
+              const int step = i / per, j = i - step * per;
+              const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane;
+              put(base + (slot0 + step) * PB * S::IMG, n, p.transposed ? lane & 7 : j & 7, v[u]);
             }
           }
+          tc::fence_proxy_async();
+        };
+        Walk<WG> w;
+        int it = 0, fills = 0;  // steps; image sets (resident) or images written
+        for (w.init(p, pre, t0, t1); !w.done() && ok; w.next(p, pre)) {
+          const bool renew = !resident || w.new_weights();
+          const bool release = !resident || w.last_of_weights();
+          if (resident && renew) {
+            for (int k = 0; k < n_k && ok && fills > 0; ++k)
+              ok = tc::mbar_wait_or_abort(B_FREE(k), (fills - 1) & 1, abort);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fill(w.g, w.ct, 0, n_k, 0);
+            for (int k = 0; k < n_k; ++k) tc::mbar_arrive(B_FULL(k));
+            ++fills;
+          }
+          for (int k = 0; k < n_k && ok; ++k, ++it) {
+            int s = k, use = renew ? fills - 1 : -1;
+            if (!resident) {
+              s = fills % S::NSLOT;
+              use = fills / S::NSLOT;
+              ++fills;
+              ok = use == 0 || tc::mbar_wait_or_abort(B_FREE(s), (use - 1) & 1, abort);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              fill(w.g, w.ct, k, 1, s);
+              tc::mbar_arrive(B_FULL(s));
+            }
+            if (warp == 4) ok = issue(it, s, use, release);
+          }
         }
-        if (warp == 4 && lane == 0) drain();
-      } else {
+        if (warp == 4) drain();
+      } else if (w4 * 32 < NT) {
+        const int n = w4 * 32 + lane;
+        auto put = [&](uint32_t img, int chunk, const float* v) {  // 8 K-values of image row n
+          uint32_t t[4][3];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) split2<PB>(v[2 * q], v[2 * q + 1], t[q]);
+#pragma unroll
+          for (int b = 0; b < PB; ++b)
+            sts128(img + b * NT * 128 + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
+        };
         const uint32_t ring = base + S::OFF_B + w4 * NU * S::UNIT_B;
         uint8_t* const mis = smem + S::OFF_MIS + (4 + w4) * NU * 32;
         float* const sc = reinterpret_cast<float*>(smem + S::OFF_SCALE) + w4 * NU * 32;
         const int64_t row_bytes = (int64_t)p.b.width * sizeof(T);
-        const int64_t off = (int64_t)(wg_n0 + w4 * 32) * sizeof(T);
+        const int64_t at = (int64_t)(wg_n0 + w4 * 32) * sizeof(T);
         Walk<WG> f;
         f.init(p, pre, t0, t1);
         int fu = 0, slot_f = 0;
-        const char* row_next = nullptr;
-        float sc_next = 0.f;
-        auto pointer = [&]() {
-          const int64_t r = (int64_t)(f.t - f.first) * SL_KC + fu * 32 + lane;
-          int64_t srow = 0;
-          row_next = row_pointer(p, p.b, f.lo, f.rows, r, &srow);
-          if constexpr (sizeof(TA) == 1)
-            sc_next = row_next ? p.a_scale[srow * p.ka_blocks + wg_k0 / MACE_CHECKPOINT_BLOCK] : 0.f;
-        };
-        pointer();
+        RowRef ref;
+        ref.load(p, f.lo, f.rows, f.row0() + lane);
         auto fetch = [&]() {
           if (!f.done()) {
-            fetch_unit<S::SEG_B, S::PITCH_B, VEC, false>(ring + slot_f * S::UNIT_B, row_next, off, row_bytes, p.b.data,
-                                                         mis + slot_f * 32);
-            if constexpr (sizeof(TA) == 1) sc[slot_f * 32 + lane] = sc_next;
+            const bool in = ref.valid(p);
+            const int64_t o = in ? ref.offset(p.b) : 0;
+            const uint32_t dst = ring + slot_f * S::UNIT_B;
+            if constexpr (VEC) {
+              uint32_t off[Pieces<S::SEG_B>::N];
+              spread_rows<S::SEG_B>(in ? (uint32_t)(o >> 4) : NO_ROW, off);
+              fetch_vec<S::SEG_B, S::PITCH_B, false, true>(dst, p.b.data, off, at, row_bytes);
+            } else {
+              fetch_any<S::SEG_B, S::PITCH_B>(dst, p.b.data, in ? p.b.data + o : nullptr, at, row_bytes,
+                                              mis + slot_f * 32);
+            }
+            if constexpr (sizeof(TA) == 1) {
+              const float* src = in ? p.a_scale + ((int64_t)ref.node * p.d + ref.m) * p.ka_blocks +
+                                          wg_k0 / MACE_CHECKPOINT_BLOCK
+                                    : p.a_scale;
+              cp_async4(tc::smem_u32(sc + slot_f * 32 + lane), src, in ? 4u : 0u);
+            }
+            slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
             if (++fu == 2) {
               fu = 0;
               f.next(p, pre);
             }
-            if (!f.done()) pointer();
-            slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
+            if (!f.done()) ref.load(p, f.lo, f.rows, f.row0() + fu * 32 + lane);
           }
           cp_commit();
         };
@@ -774,16 +893,17 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     float acc[64];
     bool ok = true;
     bool fresh = true;  // acc holds nothing yet
+    RowRef ref{-1, 0};  // map: this lane's row of the tile, loaded while the tile is computed
     // weight gradient: warp 8 issues the next step's MMAs before it takes this step's result
     auto issue_wg = [&](int it) {
-      if (WG && warp == 8 && it < t1 - t0) {
-        if (lane == 0) ok = issue(it, it & 1, it >> 1, true);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-      }
+      if (WG && warp == 8 && it < t1 - t0) ok = issue(it, it & 1, it >> 1, true);
     };
     issue_wg(0);
     for (int it = 0; !w.done() && ok; ++it) {
       const int s = it & 1;
+      if constexpr (!WG) {
+        if (fresh) ref.load(p, w.lo, w.rows, w.row0() + quad * 32 + lane);
+      }
       issue_wg(it + 1);
       if (!ok) break;
       ok = tc::mbar_wait_or_abort(D_FULL(s), (it >> 1) & 1, abort);
@@ -808,21 +928,30 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
       fresh = false;
       if constexpr (!WG) {
         if ((it + 1) % n_k != 0) continue;
-        const int64_t r = w.row0() + quad * 32 + lane;
-        const int c0 = w.col_tile() * NT + half * CW;
-        if (r < w.rows) {
-          const int64_t at = w.lo + r;
-          const int64_t i = at / p.d;
-          const int64_t node = p.order[i];
-          if (node >= 0 && node < p.n) {
-            T* dst = static_cast<T*>(p.out) + node * p.out_sn + (at - i * p.d) * p.out_sm + c0;
+        const int c0 = w.ct * NT + half * CW;
+        T* dst = nullptr;
+        if (ref.valid(p)) dst = static_cast<T*>(p.out) + ref.node * p.out_sn + ref.m * p.out_sm + c0;
+        float* const stage = reinterpret_cast<float*>(smem + S::OFF_STG + (warp - 8) * S::STG);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              if (b * 16 >= CW) break;
+        for (int b = 0; b < 4; ++b) {
+          const int left = p.N - c0 - b * 16;
+          if (b * 16 >= CW || left <= 0) break;
 #pragma unroll
-              for (int k = 0; k < 16; ++k) acc[b * 16 + k] *= p.alpha;
-              if (p.N - c0 - b * 16 > 0) store16<T>(dst + b * 16, acc + b * 16, p.N - c0 - b * 16, p.vst);
+          for (int k = 0; k < 16; ++k) acc[b * 16 + k] *= p.alpha;
+          if (p.vst && left >= 16) {
+            if (dst) store16<T>(dst + b * 16, acc + b * 16, 16, p.vst);
+          } else {
+            // unaligned rows: two rows of 16 columns per store instruction
+#pragma unroll
+            for (int k = 0; k < 16; ++k) stage[lane * 17 + k] = acc[b * 16 + k];
+            __syncwarp();
+#pragma unroll 4
+            for (int r = 0; r < 32; r += 2) {
+              const int rr = r + (lane >> 4), k = lane & 15;
+              T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), rr));
+              if (to && k < left) to[b * 16 + k] = from_f32<T>(stage[rr * 17 + k]);
             }
+            __syncwarp();
           }
         }
         fresh = true;
@@ -856,7 +985,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         w.next(p, pre);
       }
     }
-    if (WG && warp == 8 && lane == 0) drain();
+    if (WG && warp == 8) drain();
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -872,11 +1001,9 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
 // four columns x 4 share lanes).
 template <typename T>
 __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constant__ SlParams p) {
-  __shared__ unsigned long long sum[2];
+  __shared__ int64_t sum[2][8];
   __shared__ float4 part[4][64];
   const int g = blockIdx.x, tid = threadIdx.x;
-  if (tid < 2) sum[tid] = 0;
-  __syncthreads();
   int64_t before = 0, all = 0;
   for (int i = tid; i < p.G; i += 256) {
     const int64_t c = group_units(p, i, SL_KC);
@@ -884,12 +1011,25 @@ __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constan
     if (i < g) before += c;
   }
   const int64_t mine = group_units(p, g, SL_KC);
-  atomicAdd(&sum[0], (unsigned long long)before);  // whole numbers: any order gives the same sum
-  atomicAdd(&sum[1], (unsigned long long)all);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if ((tid & 31) == 0) {
+    sum[0][tid >> 5] = before;
+    sum[1][tid >> 5] = all;
+  }
   __syncthreads();
+  before = all = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    before += sum[0][w];
+    all += sum[1][w];
+  }
   // as in group_prefix
-  before = min((int64_t)sum[0], (int64_t)INT32_MAX);
-  all = min((int64_t)sum[1], (int64_t)INT32_MAX);
+  before = min(before, (int64_t)INT32_MAX);
+  all = min(all, (int64_t)INT32_MAX);
   const int tile = blockIdx.z;
   const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
   const int lane = tid & 63, sl = tid >> 6;
@@ -969,7 +1109,9 @@ int vector_bytes(const void* ptr, int64_t s0, int64_t s1, int64_t s2) {
 }
 
 bool aligned_rows(const RowView& v, int64_t n, int d) {
-  return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && (n <= 1 || v.sn % 16 == 0) && (d <= 1 || v.sm % 16 == 0);
+  // (row offsets in 16 bytes fit 32 bits)
+  return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && (n <= 1 || v.sn % 16 == 0) && (d <= 1 || v.sm % 16 == 0) &&
+         ((n - 1) * v.sn + (d - 1) * v.sm) / 16 < (int64_t)NO_ROW;
 }
 
 template <typename TA, typename T, bool WG, bool VEC>
@@ -1028,6 +1170,8 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.G = G;
   p.K = K;
   p.N = M;
+  p.small = n * d < ((int64_t)1 << 32);
+  p.w_vec = transpose && K % 8 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
   p.alpha = alpha;
   const int sms = sm_count();
   const int64_t row_tiles = (n * d + 127) / 128;
@@ -1082,6 +1226,7 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   p.G = G;
   p.K = K;
   p.N = M;
+  p.small = n * d < ((int64_t)1 << 32);
   p.alpha = alpha;
   wgrad_split(n, d, G, K, M, &p);
   const int grid = p.shares * p.n_ct * p.n_kt;
