@@ -56,12 +56,6 @@ __device__ __forceinline__ void load4(const bf16* src, float* v) {
   v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
   v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
 }
-// eight consecutive values, 16-byte aligned
-__device__ __forceinline__ void load_eight(const float* src, float* v) {
-  load4(src, v);
-  load4(src + 4, v + 4);
-}
-__device__ __forceinline__ void load_eight(const bf16* src, float* v) { load_channels<bf16, 8>(src, v); }
 __device__ __forceinline__ void store4(float* dst, const float* v) {
   *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
 }

@@ -5,9 +5,9 @@
 //   dW[g] = alpha sum over r in g of x[r]^T dy[r]  (128 input channels x NT columns per tile, K = rows)
 //
 // Arithmetic.  An fp32 operand is split into three bf16 pieces x = h + m + l
-// (h truncated, m rounded: the 24 bits of x exactly) and six of the nine
-// products are kept (h h, h m, m h, m m, h l, l h; the dropped ones are below
-// 2^-23 of x w), all kind::f16 MMAs: the instruction count of a 3xTF32 split
+// (8 bits each: the 24 bits of x exactly) and six of the nine products are
+// kept (h h, h m, m h, m m, h l, l h; the dropped ones are below 2^-21 of
+// x w, 2^-24 on average), all kind::f16 MMAs: the instruction count of a 3xTF32 split
 // with 3/4 of its operand bytes.  bf16 data is one piece; 8-bit checkpoint
 // values are exact in one bf16 piece and their row scale is folded into dy.
 // The tensor core truncates when it accumulates, so an accumulator takes one
@@ -66,7 +66,7 @@ struct SlParams {
   int transposed;
   void* out;            // map: y; weight gradient: dW (G, K, N)
   int64_t out_sn, out_sm;  // map: elements
-  int vst;              // bytes of one vector store of `out` (32, 16), 0: element by element
+  int vst;              // map: rows of `out` are whole 16-byte pieces; weight gradient: bytes of a vector store (32, 16, 0)
   float* part;          // weight gradient: partial tiles
   const int32_t* order;
   const int32_t* offsets;
@@ -74,7 +74,7 @@ struct SlParams {
   int d, G;
   int small;            // n d < 2^32: row numbers divide in 32 bits
   int K, N;             // map: K summed channels, N outputs; weight gradient: K x N of dW
-  int w_vec;            // map: 8 consecutive weights load as vectors
+  int w_vec;            // map: rows of the weights are 16-byte aligned
   int NT;               // tile columns: 32, 64, 96 or 128
   int n_ct, n_kt;       // column tiles; weight gradient: row (channel) tiles
   int shares;           // weight gradient: CTAs along the rows
@@ -97,6 +97,25 @@ __device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a, uint64_t bde
       : "memory");
 }
 
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t phase, uint32_t suspend_ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(phase), "r"(suspend_ns)
+      : "memory");
+  return ok != 0;
+}
+
+// Bounded wait for a phase; false once the CTA's abort flag is up (a wait that gives up raises it).  A phase that
+// is complete costs one try: reading the abort flag and the global timer before it would cost more than the hand-over.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t phase, volatile int* abort) {
+  if (mbar_try(bar, phase, 0)) return true;
+  return tc::mbar_wait_or_abort(bar, phase, abort);
+}
+
 // true on one lane of a converged warp; the compiler knows the branch is uniform
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -110,6 +129,15 @@ __device__ __forceinline__ bool elect_one() {
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// 16 bytes, or zeros
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool zero) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %2, 0;\n\t"
+      "cp.async.cg.shared.global [%0], [%1], 16, p;\n\t}" ::"r"(dst),
+      "l"(src), "r"((uint32_t)zero)
+      : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -138,6 +166,27 @@ __device__ __forceinline__ float lds_as(uint32_t a, bf16) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
   return __uint_as_float((uint32_t)v << 16);
 }
+__device__ __forceinline__ float lds_raw(uint32_t a, float) { return lds_as(a, 0.f); }
+__device__ __forceinline__ bf16 lds_raw(uint32_t a, bf16) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+  return __ushort_as_bfloat16(v);
+}
+__device__ __forceinline__ void lds_eight(uint32_t a, float* v, float) {
+  const uint4 x = lds128(a), y = lds128(a + 16);
+  const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(w[k]);
+}
+__device__ __forceinline__ void lds_eight(uint32_t a, float* v, bf16) {
+  const uint4 x = lds128(a);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[2 * k] = __uint_as_float(w[k] << 16);
+    v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+  }
+}
 __device__ __forceinline__ float lds_as(uint32_t a, int8_t) {
   int v;
   asm volatile("ld.shared.s8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -151,18 +200,31 @@ __device__ __forceinline__ uint32_t pack_bf16(float x0, float x1) {
   return r;
 }
 
-// the bf16 pieces of two values, packed: P = 3: h (truncated, so that no finite
-// value becomes infinite), m, l with x = h + m + l; P = 1: x rounded (exact here)
+// (x0 - y0, x1 - y1)
+__device__ __forceinline__ void sub2(float& x0, float& x1, uint32_t y0, uint32_t y1) {
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%0, %1};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "sub.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "r"(y0), "r"(y1));
+}
+
+// the bf16 pieces of two values, packed: P = 3: x = h + m + l, each the leading
+// 8 bits of what is left (exact, and no finite value becomes infinite);
+// P = 1: x rounded (exact where it is used)
 template <int P>
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t* out) {
   if constexpr (P == 1) {
     out[0] = pack_bf16(x0, x1);
   } else {
-    out[0] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
-    const float r0 = x0 - __uint_as_float(__float_as_uint(x0) & 0xffff0000u);
-    const float r1 = x1 - __uint_as_float(__float_as_uint(x1) & 0xffff0000u);
-    out[1] = pack_bf16(r0, r1);
-    out[2] = pack_bf16(r0 - __uint_as_float(out[1] << 16), r1 - __uint_as_float(out[1] & 0xffff0000u));
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+      out[k] = __byte_perm(u0, u1, 0x7632);
+      if (k < 2) sub2(x0, x1, u0 & 0xffff0000u, u1 & 0xffff0000u);
+    }
   }
 }
 
@@ -246,19 +308,19 @@ struct Sl {
   static constexpr int SEG_B = 32 * (int)sizeof(T);
   static constexpr int PITCH_A = SEG_A + (VEC ? 0 : 16), PITCH_B = SEG_B + (VEC ? 0 : 16);
   static constexpr int UPC = WG ? 2 : SL_KC * (int)sizeof(TA) / 128;  // ring units per step of 64
-  static constexpr int NU = WG ? (VEC ? 4 : 3) : (VEC ? 6 : 5);
+  static constexpr int NU = WG ? (VEC ? 4 : 3) : 5;
+  static constexpr int NU_B = VEC && PA == 3 ? 3 : NU;  // (a fourth unit of fp32 rows would not fit)
   static constexpr int UNIT_A = 32 * PITCH_A, UNIT_B = 32 * PITCH_B;
-  static constexpr int IMG = 128 * 128;  // one piece of a B image: NT <= 128 rows of 64 bf16
   static constexpr int NSLOT = !WG && PB == 1 ? 4 : 2;
-  static constexpr int OFF_A = NSLOT * PB * IMG;
+  static constexpr int OFF_A = NSLOT * PB * 128 * 128;
   static constexpr int OFF_B = OFF_A + 4 * NU * UNIT_A;
-  static constexpr int OFF_MIS = OFF_B + (WG ? 4 * NU * UNIT_B : 0);        // per ring unit and row: misalignment
+  static constexpr int STG = 32 * 128;  // map: an epilogue warp's staging, 32 rows x 128 bytes
+  static constexpr int OFF_STG = OFF_B + (WG ? 4 * NU_B * UNIT_B : 0);
+  static constexpr int OFF_MIS = OFF_STG + (WG ? 0 : 8 * STG);        // per ring unit and row: misalignment
   static constexpr int OFF_SCALE = OFF_MIS + (VEC ? 0 : (WG ? 8 : 4) * NU * 32);  // per B ring unit and row: A's scale
   static constexpr int OFF_PRE = OFF_SCALE + (sizeof(TA) == 1 ? 4 * NU * 32 * 4 : 0);
-  static constexpr int STG = 32 * 17 * 4;  // map: 32 rows x 16 columns of an epilogue warp, for unaligned results
-  static constexpr int OFF_STG = OFF_PRE + ((MACE_SPECIES_MAX_GROUPS + 2) * 4 + 7) / 8 * 8;
-  static constexpr int OFF_BAR = OFF_STG + (WG ? 0 : 8 * STG);
-  static constexpr int NBAR = 8 + 2 * NSLOT + 1;
+  static constexpr int OFF_BAR = OFF_PRE + (3 * MACE_SPECIES_MAX_GROUPS + 2) * 4;
+  static constexpr int NBAR = 8 + 2 * NSLOT + 2;
   static constexpr int BYTES = OFF_BAR + NBAR * 8 + 32;
   static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
@@ -268,12 +330,22 @@ __device__ __forceinline__ int64_t group_units(const SlParams& p, int g, int uni
   return ((r.hi - r.lo) * p.d + unit_rows - 1) / unit_rows;
 }
 
-// exclusive prefix of per-group tile counts into pre[0..G], by the whole CTA (G <= 512 = SL_THREADS)
-__device__ __forceinline__ void group_prefix(const SlParams& p, int unit_rows, int per_unit, int* pre,
-                                             int64_t* warp_sums) {
+// The groups in shared memory: units of group g are [pre[g], pre[g + 1]), its rows [lo[g], hi[g]) of `order`.
+struct Groups {
+  int *pre, *lo, *hi;
+};
+
+// fills them, by the whole CTA (G <= 512 = SL_THREADS)
+__device__ __forceinline__ void load_groups(const SlParams& p, int unit_rows, int per_unit, const Groups& q,
+                                            int64_t* warp_sums) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t s = 0;
-  if (tid < p.G) s = group_units(p, tid, unit_rows) * per_unit;
+  if (tid < p.G) {
+    const Range r = group_range(p.offsets, tid, p.n);
+    q.lo[tid] = (int)r.lo;
+    q.hi[tid] = (int)r.hi;
+    s = ((r.hi - r.lo) * p.d + unit_rows - 1) / unit_rows * per_unit;
+  }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
@@ -282,91 +354,88 @@ __device__ __forceinline__ void group_prefix(const SlParams& p, int unit_rows, i
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
   for (int w = 0; w < warp; ++w) s += warp_sums[w];
-  if (tid < p.G) pre[tid + 1] = (int)min(s, (int64_t)INT32_MAX);  // beyond it: offsets that overlap
-  if (tid == 0) pre[0] = 0;
+  if (tid < p.G) q.pre[tid + 1] = (int)min(s, (int64_t)INT32_MAX);  // beyond it: offsets that overlap
+  if (tid == 0) q.pre[0] = 0;
   __syncthreads();
 }
 
-// largest g < G with pre[g] <= t (a group that holds unit t: empty groups have pre[g] == pre[g + 1])
-__device__ __forceinline__ int group_of_unit(const int* pre, int G, int t) {
-  int lo = 0, hi = G - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (pre[mid] <= t)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
-}
-
-// The steps of a CTA, in order; every role walks the same ones.
-// Map: tiles [t, t1) of (group, column tile, row tile), n_k steps each.
-// Weight gradient: 64-row units [t, t1) of the groups, one step each.
-template <bool WG>
+// The steps of a CTA, in order; every role walks the same ones, holding little (the rest is in shared memory).
+// Map: tiles t of (group, column tile, row tile).  Weight gradient: 64-row units t of the groups.
 struct Walk {
-  int t, t0, t1, g;
-  int first, last;   // units of group g: [first, last)
-  int ct, rt, n_rt;  // map: column tile, row tile, row tiles of the group
-  int64_t lo, rows;  // group's first grouped row (components counted) and its row count
-  __device__ __forceinline__ void load(const SlParams& p, const int* pre) {
-    const Range r = group_range(p.offsets, g, p.n);
-    first = pre[g];
-    last = pre[g + 1];
-    lo = r.lo * p.d;
-    rows = (r.hi - r.lo) * p.d;
-    if (!WG) n_rt = (int)((rows + 127) >> 7);
-  }
-  __device__ __forceinline__ void init(const SlParams& p, const int* pre, int t0_, int t1_) {
-    t = t0 = t0_;
-    t1 = t1_;
-    g = group_of_unit(pre, p.G, t);
-    load(p, pre);
-    if (!WG) {
-      ct = (t - first) / n_rt;
-      rt = (t - first) - ct * n_rt;
+  int t, g;
+  __device__ __forceinline__ void init(const SlParams& p, const Groups& q, int t0) {
+    t = t0;
+    int lo = 0, hi = p.G - 1;  // the largest g with pre[g] <= t: empty groups have pre[g] == pre[g + 1]
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (q.pre[mid] <= t)
+        lo = mid;
+      else
+        hi = mid - 1;
     }
+    g = lo;
   }
-  __device__ __forceinline__ bool done() const { return t >= t1; }
-  __device__ __forceinline__ void next(const SlParams& p, const int* pre) {
-    ++t;
-    if (!WG && ++rt == n_rt) {
-      rt = 0;
-      ++ct;
-    }
-    if (t < last || t >= t1) return;
-    do ++g;
-    while (pre[g + 1] <= t);
-    load(p, pre);
-    ct = rt = 0;
+  __device__ __forceinline__ void next(const Groups& q, int t1) {
+    if (++t < t1)
+      while (q.pre[g + 1] <= t) ++g;
   }
-  // first row of the tile or unit, within its group
-  __device__ __forceinline__ int64_t row0() const {
-    return WG ? (int64_t)(t - first) * SL_KC : (int64_t)rt * 128;
-  }
-  // map: first / last tile of its (group, column tile) in this CTA: the weight images are new / free after it
-  __device__ __forceinline__ bool new_weights() const { return t == t0 || rt == 0; }
-  __device__ __forceinline__ bool last_of_weights() const { return t + 1 == t1 || rt + 1 == n_rt; }
 };
 
-// A lane's row of the grouped list: its atom is loaded ahead of use (`node`
-// stays in flight until offset() reads it).
+// Map: a tile's rows [at, end) of the grouped list (components counted), its column tile, and whether it is the
+// first or the last row tile of its (group, column tile).
+struct Tile {
+  int64_t at, end;
+  int ct;
+  bool first, last;
+  __device__ __forceinline__ Tile(const SlParams& p, const Groups& q, const Walk& w) {
+    at = (int64_t)q.lo[w.g] * p.d;
+    end = (int64_t)q.hi[w.g] * p.d;
+    const int n_rt = (int)((end - at + 127) >> 7);
+    int rt = w.t - q.pre[w.g];
+    ct = 0;
+    if (p.n_ct > 1) {
+      ct = rt / n_rt;
+      rt -= ct * n_rt;
+    }
+    at += (int64_t)rt * 128;
+    first = rt == 0;
+    last = rt + 1 == n_rt;
+  }
+};
+
+// A lane's row of the grouped list, loaded ahead of use.  The load is issued for every lane (from a clamped place)
+// and its result first read by valid(): selecting a default right after the load would wait for it.
 struct RowRef {
-  int node, m;  // node < 0: no row
-  __device__ __forceinline__ void load(const SlParams& p, int64_t lo, int64_t rows, int64_t r) {
-    node = -1;
-    m = 0;
-    if (r >= rows) return;
-    const int64_t at = lo + r;
+  int node, m;  // m < 0: no such row
+  __device__ __forceinline__ void load(const SlParams& p, int64_t at, int64_t end) {
+    const bool in = at < end;
+    at = min(at, end - 1);
     int64_t i = at;
+    m = 0;
     if (p.d > 1) {
       i = p.small ? (int64_t)((uint32_t)at / (uint32_t)p.d) : at / p.d;
       m = (int)(at - i * p.d);
     }
-    node = p.order[i];
+    if (!in) m = -1;
+    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(node) : "l"(p.order + i));
   }
-  __device__ __forceinline__ bool valid(const SlParams& p) const { return node >= 0 && node < p.n; }
+  __device__ __forceinline__ bool valid(const SlParams& p) const { return m >= 0 && node >= 0 && node < p.n; }
   __device__ __forceinline__ int64_t offset(const RowView& v) const { return node * v.sn + m * v.sm; }
+};
+
+// Weight gradient: the atoms of consecutive 32-row units, one row per lane.
+struct WalkRows {
+  Walk w;
+  int u;
+  __device__ __forceinline__ void load(const SlParams& p, const Groups& q, int t1, RowRef& ref) {
+    if (w.t >= t1) return;
+    ref.load(p, (int64_t)q.lo[w.g] * p.d + (int64_t)(w.t - q.pre[w.g]) * SL_KC + u * 32 + (threadIdx.x & 31),
+             (int64_t)q.hi[w.g] * p.d);
+    if (++u == 2) {
+      u = 0;
+      w.next(q, t1);
+    }
+  }
 };
 
 // One ring unit: 32 row segments of SEG bytes.  VEC: lane l copies 16-byte piece
@@ -387,34 +456,33 @@ __device__ __forceinline__ void spread_rows(uint32_t mine, uint32_t* off) {
   for (int i = 0; i < P::N; ++i) off[i] = __shfl_sync(0xffffffffu, mine, i * P::RPI + lane / P::PPR);
 }
 
-// `at`: first byte of the segment within its row; ZERO: rows may be NO_ROW
+// `at`: first byte of the segment within its row; ZERO: rows may be NO_ROW.  Rows are whole 16-byte pieces here:
+// a copy whose source size is a register costs several instructions more than one that is all or nothing.
 template <int SEG, int PITCH, bool SWZ, bool ZERO>
-__device__ __forceinline__ void fetch_vec(uint32_t dst, const char* data, const uint32_t* off, int64_t at,
-                                          int64_t row_bytes) {
+__device__ __forceinline__ void fetch_vec(uint32_t dst, const char* data, const uint32_t* off, int at, int row_bytes) {
   using P = Pieces<SEG>;
   const int lane = threadIdx.x & 31, j = lane % P::PPR, r0 = lane / P::PPR;
-  const int64_t left = row_bytes - at - 16 * j;
-  const uint32_t bytes = left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
-  const char* const src = bytes ? data + at + 16 * j : data;
+  const bool past = at + 16 * j >= row_bytes;
+  const char* const src = past ? data : data + at + 16 * j;
 #pragma unroll
   for (int i = 0; i < P::N; ++i) {
     const int r = i * P::RPI + r0;
     const int pos = SWZ ? (j ^ (r & 7)) : j;
     const bool none = ZERO && off[i] == NO_ROW;
-    cp_async16(dst + r * PITCH + pos * 16, none ? src : src + (uint64_t)off[i] * 16, none ? 0u : bytes);
+    cp_async16_or_zero(dst + r * PITCH + pos * 16, none ? data : src + (uint64_t)off[i] * 16, past || none);
   }
 }
 
 // Rows of any alignment: the 16-byte units that contain the segment; mis[r]:
 // where it starts in the first.  row: this lane's row (null: zeros).
 template <int SEG, int PITCH>
-__device__ __forceinline__ void fetch_any(uint32_t dst, const char* data, const char* row, int64_t at,
-                                          int64_t row_bytes, uint8_t* mis) {
+__device__ __forceinline__ void fetch_any(uint32_t dst, const char* data, const char* row, int at, int row_bytes,
+                                          uint8_t* mis) {
   constexpr int PPR = SEG / 16 + 1;
   const int lane = threadIdx.x & 31;
   // copies of no bytes still name an aligned address
   const char* const dummy = reinterpret_cast<const char*>(reinterpret_cast<uint64_t>(data) & ~(uint64_t)15);
-  const int seg = (int)max(min(row_bytes - at, (int64_t)SEG), (int64_t)0);  // bytes of a row in this segment
+  const int seg = max(min(row_bytes - at, SEG), 0);  // bytes of a row in this segment
   const uint64_t from = row ? reinterpret_cast<uint64_t>(row + at) : 0;
   mis[lane] = (uint8_t)(from & 15);
 #pragma unroll
@@ -445,6 +513,109 @@ __device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int s) {
                     __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }
 
+constexpr int SL_IMG = 128 * 128;  // bytes of one piece of a B image: up to 128 rows of 64 bf16
+
+// 8 K-values of row n of a B image: their bf16 pieces
+template <int P>
+__device__ __forceinline__ void put_eight(uint32_t img, int n, int chunk, const float* v) {
+  uint32_t t[4][3];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) split2<P>(v[2 * q], v[2 * q + 1], t[q]);
+#pragma unroll
+  for (int b = 0; b < P; ++b)
+    sts128(img + b * SL_IMG + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
+}
+
+// Where weight (k, n) of a step waits, as it is, in its own image slot: 64 columns (one round of the rewriting)
+// apart from the other 64, where the images of the first round are not written.
+template <typename T>
+__device__ __forceinline__ uint32_t raw_place(int k, int n, bool transposed) {
+  if (sizeof(T) == 2) return transposed ? n * 128 + k * 2 : (n >> 6) * 8192 + k * 128 + (n & 63) * 2;
+  return transposed ? ((n >> 5) & 1) * 16384 + (n >> 6) * 8192 + (n & 31) * 256 + k * 4
+                    : (k >> 5) * 16384 + (n >> 6) * 8192 + (k & 31) * 256 + (n & 63) * 4;
+}
+
+// Map: the weight images of steps [k0, k0 + nk) of (group g, column tile ct), at img0 + step * stride, by warps
+// 4 to 7; full: the first step's barrier (arrived on as each step is done).  Weights of whole 16-byte pieces come
+// as they are by cp.async into their own image slots, all steps at once (one memory latency for the whole set),
+// and are rewritten in place through registers, 64 image rows at a time; others are loaded value by value.  A
+// round is 16 items of 32 (image row, K octet) pairs, one per lane, four items per warp.  Weights (K, N): an item
+// is one octet of 32 neighbouring columns; transposed (N, K): 8 octets of 4 rows.
+template <typename T, int PB>
+__device__ __forceinline__ bool fill_weights(const SlParams& p, uint32_t img0, uint32_t stride, int g, int ct, int k0,
+                                             int nk, uint32_t full, uint32_t w_sync_bar, int& syncs,
+                                             volatile int* abort) {
+  const int lane = threadIdx.x & 31, w4 = (threadIdx.x >> 5) & 3;
+  const int NT = p.NT;
+  auto w_sync = [&]() -> bool {  // the four warps meet (a bounded wait, unlike a barrier)
+    tc::mbar_arrive(w_sync_bar);
+    return __all_sync(0xffffffffu, wait_phase(w_sync_bar, syncs++ & 1, abort));
+  };
+  const T* wt = static_cast<const T*>(p.w) + (int64_t)g * p.K * p.N;
+  if (p.w_vec) {
+    constexpr int E = 16 / sizeof(T);  // elements of a piece
+    // 64 x NT (transposed: NT x 64) elements of a step, the columns (K) in 64 / E or fewer pieces
+    const int width = p.transposed ? SL_KC : NT, ppr = width / E, pieces = (p.transposed ? NT : SL_KC) * ppr;
+#pragma unroll 1
+    for (int s = 0; s < nk; ++s) {
+      const uint32_t raw = img0 + s * stride;
+#pragma unroll 4
+      for (int i = w4 * 32 + lane; i < pieces; i += 128) {
+        const int r = (uint32_t)i / (uint32_t)ppr, c = (i - r * ppr) * E;
+        const int kk = p.transposed ? c : r, nn = p.transposed ? r : c;
+        const int k = (k0 + s) * SL_KC + kk, n = ct * NT + nn;
+        const bool in = k < p.K && n < p.N;
+        const T* src = p.transposed ? wt + (int64_t)n * p.K + k : wt + (int64_t)k * p.N + n;
+        cp_async16_or_zero(raw + raw_place<T>(kk, nn, p.transposed), in ? src : wt, !in);
+      }
+    }
+    cp_commit();
+    cp_wait<0>();
+    if (!w_sync()) return false;
+  }
+#pragma unroll 1
+  for (int s = 0; s < nk; ++s) {
+    const uint32_t img = img0 + s * stride;
+#pragma unroll 1
+    for (int h = 0; h * 64 < NT; ++h) {
+      float v[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = h * 16 + u * 4 + w4;
+        const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane, kk = (p.transposed ? lane & 7 : j & 7) * 8;
+        if (p.w_vec) {
+          if (p.transposed) {
+            lds_eight(img + raw_place<T>(kk, n, true), v[u], T{});
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[u][e] = lds_as(img + raw_place<T>(kk + e, n, false), T{});
+          }
+        } else {
+          const int col = ct * NT + n, k = (k0 + s) * SL_KC + kk;
+          const T* src = p.transposed ? wt + (int64_t)col * p.K + k : wt + (int64_t)k * p.N + col;
+          const int64_t step = p.transposed ? 1 : p.N;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[u][e] = n < NT && col < p.N && k + e < p.K ? to_f32(src[e * step]) : 0.f;
+        }
+      }
+      if (p.w_vec && !w_sync()) return false;  // every raw value of the round is in registers
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = h * 16 + u * 4 + w4;
+        const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane;
+        if constexpr (PB == 3) {  // alpha rides on the split weights
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[u][e] *= p.alpha;
+        }
+        if (n < NT) put_eight<PB>(img, n, p.transposed ? lane & 7 : j & 7, v[u]);
+      }
+    }
+    tc::fence_proxy_async();
+    tc::mbar_arrive(full + 8 * s);
+  }
+  return true;
+}
+
 template <typename TA, typename T, bool WG, bool VEC>
 __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_constant__ SlParams p) {
   using S = Sl<TA, T, WG, VEC>;
@@ -452,6 +623,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = tc::smem_u32(smem);
   int* const pre = reinterpret_cast<int*>(smem + S::OFF_PRE);
+  const Groups q{pre, pre + MACE_SPECIES_MAX_GROUPS + 2, pre + 2 * MACE_SPECIES_MAX_GROUPS + 2};
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + S::NBAR);
   volatile int* const abort = reinterpret_cast<int*>(tslot + 1);
@@ -462,7 +634,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   auto D_FREE = [&](int s) { return bar(6 + s); };
   auto B_FULL = [&](int s) { return bar(8 + s); };
   auto B_FREE = [&](int s) { return bar(8 + S::NSLOT + s); };
-  const uint32_t DONE = bar(8 + 2 * S::NSLOT);
+  const uint32_t DONE = bar(8 + 2 * S::NSLOT), W_SYNC = bar(9 + 2 * S::NSLOT);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be uniform
 
@@ -471,13 +643,14 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     return;
   }
 
-  if constexpr (!WG) {
-    // rows outside every group: zero
+  // map: zeros in the rows outside every group, shared by warps 5 to 7 of every CTA
+  auto zero_rows = [&]() {
+    constexpr int w0 = 5, nw = 3;
     const int64_t b0 = min(max((int64_t)p.offsets[0], (int64_t)0), p.n);
     const int64_t b1 = max(min(max((int64_t)p.offsets[p.G], (int64_t)0), p.n), b0);
     const int64_t outside = (p.n - (b1 - b0)) * p.d;
     T* out = static_cast<T*>(p.out);
-    for (int64_t r = blockIdx.x * (int64_t)(SL_THREADS / 32) + warp; r < outside; r += (int64_t)gridDim.x * (SL_THREADS / 32)) {
+    for (int64_t r = blockIdx.x * (int64_t)nw + warp - w0; r < outside; r += (int64_t)gridDim.x * nw) {
       int64_t i = r / p.d;
       const int m = (int)(r - i * p.d);
       if (i >= b0) i += b1 - b0;
@@ -485,26 +658,12 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
       if (node < 0 || node >= p.n) continue;
       for (int c = lane; c < p.N; c += 32) out[node * p.out_sn + m * p.out_sm + c] = from_f32<T>(0.f);
     }
-  }
+  };
 
-  if (tid == 0) *abort = 0;
-  group_prefix(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, pre, reinterpret_cast<int64_t*>(smem));
-  // this CTA's share of the units; weight gradient: blockIdx.x = share * tiles + tile
-  const int total = pre[p.G];
-  const int tiles = WG ? p.n_ct * p.n_kt : 1;
-  const int nshare = WG ? min(p.shares, total) : gridDim.x;  // no share without a unit between two that have some
-  const int share = WG ? blockIdx.x / tiles : blockIdx.x;
-  if (share >= nshare) return;
-  const int tile = WG ? blockIdx.x % tiles : 0;
-  const int t0 = (int)((int64_t)share * total / nshare), t1 = (int)((int64_t)(share + 1) * total / nshare);
-  if (t0 >= t1) return;
-  const int wg_k0 = WG ? (tile / p.n_ct) * 128 : 0, wg_n0 = WG ? (tile % p.n_ct) * p.NT : 0;
-  const int n_k = WG ? 1 : (p.K + SL_KC - 1) / SL_KC;  // steps of a tile
-  const bool resident = n_k <= S::NSLOT;               // map: the weight images of a tile stay for the next row tile
   const int NT = p.NT;
-
-  if (warp == 8) {
+  if (warp == 15) {  // while the others wait for the offsets
     if (lane == 0) {
+      *abort = 0;
       for (int s = 0; s < 2; ++s) {
         tc::mbar_init(A_FULL(s), 128);
         tc::mbar_init(A_FREE(s), 1);
@@ -516,6 +675,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         tc::mbar_init(B_FREE(s), 1);
       }
       tc::mbar_init(DONE, 1);
+      tc::mbar_init(W_SYNC, 128);
       tc::fence_barrier_init();
     }
     __syncwarp();
@@ -523,8 +683,24 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     tc::tmem_relinquish();
   }
   tc::fence_before_sync();
-  __syncthreads();
+  load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, q, reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
+  // this CTA's share of the units; weight gradient: blockIdx.x = share * tiles + tile
+  const int total = pre[p.G];
+  const int tiles = WG ? p.n_ct * p.n_kt : 1;
+  const int nshare = WG ? min(p.shares, total) : gridDim.x;  // no share without a unit between two that have some
+  const int share = WG ? blockIdx.x / tiles : blockIdx.x;
+  const int tile = WG ? blockIdx.x % tiles : 0;
+  const int t0 = share < nshare ? (int)((int64_t)share * total / nshare) : 0;
+  const int t1 = share < nshare ? (int)((int64_t)(share + 1) * total / nshare) : 0;
+  if (t0 >= t1) {
+    if (!WG && warp >= 5 && warp < 8) zero_rows();
+    if (warp == 15) tc::tmem_dealloc(SL_D, SL_TMEM);
+    return;
+  }
+  const int wg_k0 = WG ? (tile / p.n_ct) * 128 : 0, wg_n0 = WG ? (tile % p.n_ct) * p.NT : 0;
+  const int n_k = WG ? 1 : (p.K + SL_KC - 1) / SL_KC;  // steps of a tile
+  const bool resident = n_k <= S::NSLOT;               // map: the weight images of a tile stay for the next row tile
   const uint32_t tmem = SL_D;  // an allocation of all 512 columns starts at column 0
 
   // MMAs of step `it` with the images of slot bs, by a whole warp with warp-uniform
@@ -533,21 +709,21 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   auto issue = [&](int it, int bs, int use, bool release) -> bool {
     using PR = Products<PA, PB>;
     const int s = it & 1;
-    bool ok = use < 0 || tc::mbar_wait_or_abort(B_FULL(bs), use & 1, abort);
-    ok = ok && tc::mbar_wait_or_abort(A_FULL(s), (it >> 1) & 1, abort);
-    if (ok && it >= 2) ok = tc::mbar_wait_or_abort(D_FREE(s), ((it >> 1) - 1) & 1, abort);
+    bool ok = use < 0 || wait_phase(B_FULL(bs), use & 1, abort);
+    ok = ok && wait_phase(A_FULL(s), (it >> 1) & 1, abort);
+    if (ok && it >= 2) ok = wait_phase(D_FREE(s), ((it >> 1) - 1) & 1, abort);
     if (!__all_sync(0xffffffffu, ok)) return false;
     tc::fence_after_sync();
     const uint32_t us = __shfl_sync(0xffffffffu, s, 0), ub = __shfl_sync(0xffffffffu, bs, 0);
     const uint32_t idesc = idesc_bf16(p.NT);
-    const uint64_t desc = tc::sw128_desc(base + ub * (PB * S::IMG));
+    const uint64_t desc = tc::sw128_desc(base + ub * (PB * SL_IMG));
     const uint32_t d = SL_D + us * 128, a = SL_A + us * (PA * 32);
     if (elect_one()) {
 #pragma unroll
       for (int q = 0; q < PR::n; ++q)
 #pragma unroll
         for (int ks = 0; ks < SL_KC / 16; ++ks)
-          mma_bf16_ta(d, a + PR::a(q) * 32 + ks * 8, desc + (uint32_t)(PR::b(q) * p.NT * 8 + ks * 2), idesc,
+          mma_bf16_ta(d, a + PR::a(q) * 32 + ks * 8, desc + (uint32_t)(PR::b(q) * (SL_IMG / 16) + ks * 2), idesc,
                       q > 0 || ks > 0);
       tc::mma_commit(A_FREE(s));
       if (release) tc::mma_commit(B_FREE(bs));
@@ -568,17 +744,21 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     // ---------------- operand A: memory -> ring -> registers -> TMEM ----------------
     const uint32_t ring = base + S::OFF_A + warp * NU * S::UNIT_A;
     uint8_t* const mis = smem + S::OFF_MIS + warp * NU * 32;
-    const int64_t row_bytes = (int64_t)p.a.width * sizeof(TA);
+    const int row_bytes = p.a.width * (int)sizeof(TA);
     const uint32_t tq = tmem + ((uint32_t)(warp * 32) << 16) + SL_A;
-    // the fetching side runs NU - 1 units ahead; atoms of the rows after it are loaded one (map: tile, else: unit) earlier
-    Walk<WG> f;
-    f.init(p, pre, t0, t1);
-    int fk = 0, fu = 0, slot_f = 0;  // step of the tile, unit of the step, ring slot
-    RowRef ref;
+    // the fetching side runs NU - 1 units ahead; the atoms of its rows are loaded one tile (weight gradient: two
+    // units) before
+    const int tile_units = n_k * S::UPC;  // ring units of a tile
+    const int units = (t1 - t0) * tile_units;
+    int left = units, fu = 0, slot_f = 0;  // units to fetch, unit within the tile, ring slot
+    RowRef ref, ahead;
+    WalkRows rows{};
+    rows.w.init(p, q, t0);
     uint32_t off[Pieces<S::SEG_A>::N];
     const char* row = nullptr;
-    auto load_rows = [&]() {
-      ref.load(p, f.lo, f.rows, WG ? f.row0() + fu * 32 + lane : f.row0() + warp * 32 + lane);
+    auto load_tile = [&]() {
+      const Tile t(p, q, rows.w);
+      ref.load(p, t.at + warp * 32 + lane, t.end);
     };
     // the loaded rows become the fetched ones.  Map: a row outside the tile may hold anything (its
     // TMEM lane is never stored), so it stands for row 0; weight gradient: it must be zero
@@ -591,56 +771,51 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         row = WG && !ok ? nullptr : p.a.data + o;
     };
     auto fetch = [&]() {
-      if (!f.done()) {
-        const bool fresh = WG || (fk == 0 && fu == 0);
-        if (fresh) take_rows();
-        const int64_t at = WG ? (int64_t)(wg_k0 + warp * 32) * sizeof(TA) : (int64_t)fk * SL_KC * sizeof(TA) + fu * 128;
+      if (left > 0) {
+        --left;
+        if (fu == 0) {
+          take_rows();
+          if constexpr (WG) {
+            ref = ahead;
+            rows.load(p, q, t1, ahead);
+          } else {
+            rows.w.next(q, t1);
+            if (rows.w.t < t1) load_tile();
+          }
+        }
         const uint32_t dst = ring + slot_f * S::UNIT_A;
+        const int at = WG ? (wg_k0 + warp * 32) * (int)sizeof(TA) : fu * 128;
         if constexpr (VEC)
           fetch_vec<S::SEG_A, S::PITCH_A, !WG, WG>(dst, p.a.data, off, at, row_bytes);
         else
           fetch_any<S::SEG_A, S::PITCH_A>(dst, p.a.data, row, at, row_bytes, mis + slot_f * 32);
         slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
-        if constexpr (WG) {
-          if (++fu == S::UPC) {
-            fu = 0;
-            f.next(p, pre);
-          }
-          if (!f.done()) load_rows();
-        } else {
-          if (fresh) {  // the next tile's rows
-            Walk<WG> nx = f;
-            nx.next(p, pre);
-            if (!nx.done()) ref.load(p, nx.lo, nx.rows, nx.row0() + warp * 32 + lane);
-          }
-          if (++fu == S::UPC) {
-            fu = 0;
-            if (++fk == n_k) {
-              fk = 0;
-              f.next(p, pre);
-            }
-          }
-        }
+        if (!WG && ++fu == tile_units) fu = 0;
       }
       cp_commit();
     };
-    load_rows();
-    for (int i = 0; i < NU - 1; ++i) fetch();
-    const int steps = (t1 - t0) * n_k;
+    if constexpr (WG) {
+      rows.load(p, q, t1, ref);
+      rows.load(p, q, t1, ahead);
+    } else {
+      load_tile();
+    }
+    // (one loop, so that the code of a unit exists once: the roles' loops together fill the instruction cache)
     int slot = 0;
     bool ok = true;
-    for (int it = 0; it < steps && ok; ++it) {
-      const int s = it & 1;
-#pragma unroll
-      for (int u = 0; u < S::UPC; ++u) {
-        cp_wait<NU - 2>();
+#pragma unroll 1
+    for (int i = 1 - NU; i < units && ok; ++i) {
+      const int it = i / S::UPC, u = i - it * S::UPC, s = it & 1;
+      {
+        if (i >= 0) cp_wait<NU - 2>();
         __syncwarp();
         fetch();
+        if (i < 0) continue;
         const uint32_t src = ring + slot * S::UNIT_A;
         const uint8_t* const ms = mis + slot * 32;
         slot = slot + 1 == NU ? 0 : slot + 1;
         if (u == 0) {
-          if (it >= 2) ok = tc::mbar_wait_or_abort(A_FREE(s), ((it >> 1) - 1) & 1, abort);
+          ok = it < 2 || wait_phase(A_FREE(s), ((it >> 1) - 1) & 1, abort);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc::fence_after_sync();
@@ -704,7 +879,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
           for (int a = 0; a < PA; ++a) tmem_st16u(ta + a * 32 + u * 16, out[a]);
         }
       }
-      if (ok) {
+      if (u == S::UPC - 1) {
         tc::tmem_wait_st();
         tc::fence_before_sync();
         tc::mbar_arrive(A_FULL(s));
@@ -717,68 +892,24 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     bool ok = true;
     {
       if constexpr (!WG) {
-        // 8 K-values of image row n
-        auto put = [&](uint32_t img, int n, int chunk, const float* v) {
-          uint32_t t[4][3];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) split2<PB>(v[2 * q], v[2 * q + 1], t[q]);
-#pragma unroll
-          for (int b = 0; b < PB; ++b)
-            sts128(img + b * NT * 128 + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
+        int syncs = 0;
+        auto fill = [&](int g, int ct, int k0, int nk, int slot0) -> bool {
+          return fill_weights<T, PB>(p, base + slot0 * PB * SL_IMG, PB * SL_IMG, g, ct, k0, nk, bar(8 + slot0), W_SYNC,
+                                     syncs, abort);
         };
-        // the images of steps [k0, k0 + nk): items of 32 (image row, K octet) pairs, taken in turn by the
-        // four warps, four at a time so that 32 values per lane are in flight.  Weights (K, N): lanes are 32
-        // neighbouring columns; transposed (N, K): 4 rows x 8 octets, 256 contiguous bytes of each row
-        auto fill = [&](int g, int ct, int k0, int nk, int slot0) {
-          const T* wt = static_cast<const T*>(p.w) + (int64_t)g * p.K * p.N;
-          const int per = NT / 4;  // items of a step: NT / 32 blocks of columns x 8 octets, or NT / 4 blocks of rows
-          for (int i0 = w4; i0 < nk * per; i0 += 16) {
-            float v[4][8];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int i = i0 + 4 * u;
-              const int step = i / per, j = i - step * per;
-              const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane;
-              const int chunk = p.transposed ? lane & 7 : j & 7;
-              const int col = ct * NT + n, k = (k0 + step) * SL_KC + chunk * 8;
-              const bool in = i < nk * per && col < p.N;
-              if (p.transposed) {
-                const T* src = wt + (int64_t)col * p.K + k;
-                if (p.w_vec && in && k + 8 <= p.K) {
-                  load_eight(src, v[u]);
-                } else {
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) v[u][e] = in && k + e < p.K ? to_f32(src[e]) : 0.f;
-                }
-              } else {
-                const T* src = wt + (int64_t)k * p.N + col;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[u][e] = in && k + e < p.K ? to_f32(src[(int64_t)e * p.N]) : 0.f;
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int i = i0 + 4 * u;
-              if (i >= nk * per) break;
-              const int step = i / per, j = i - step * per;
-              const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane;
-              put(base + (slot0 + step) * PB * S::IMG, n, p.transposed ? lane & 7 : j & 7, v[u]);
-            }
-          }
-          tc::fence_proxy_async();
-        };
-        Walk<WG> w;
+        Walk w;
         int it = 0, fills = 0;  // steps; image sets (resident) or images written
-        for (w.init(p, pre, t0, t1); !w.done() && ok; w.next(p, pre)) {
-          const bool renew = !resident || w.new_weights();
-          const bool release = !resident || w.last_of_weights();
+        for (w.init(p, q, t0); w.t < t1 && ok; w.next(q, t1)) {
+          const Tile t(p, q, w);
+          const bool renew = !resident || t.first || w.t == t0;      // the images are new
+          const bool release = !resident || t.last || w.t + 1 == t1;  // and free after this tile
           if (resident && renew) {
             for (int k = 0; k < n_k && ok && fills > 0; ++k)
-              ok = tc::mbar_wait_or_abort(B_FREE(k), (fills - 1) & 1, abort);
+              ok = wait_phase(B_FREE(k), (fills - 1) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            fill(w.g, w.ct, 0, n_k, 0);
-            for (int k = 0; k < n_k; ++k) tc::mbar_arrive(B_FULL(k));
+            ok = fill(w.g, t.ct, 0, n_k, 0);
+            if (!ok) break;
             ++fills;
           }
           for (int k = 0; k < n_k && ok; ++k, ++it) {
@@ -787,38 +918,35 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
               s = fills % S::NSLOT;
               use = fills / S::NSLOT;
               ++fills;
-              ok = use == 0 || tc::mbar_wait_or_abort(B_FREE(s), (use - 1) & 1, abort);
+              ok = use == 0 || wait_phase(B_FREE(s), (use - 1) & 1, abort);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
-              fill(w.g, w.ct, k, 1, s);
-              tc::mbar_arrive(B_FULL(s));
+              ok = fill(w.g, t.ct, k, 1, s);
+              if (!ok) break;
             }
             if (warp == 4) ok = issue(it, s, use, release);
           }
         }
-        if (warp == 4) drain();
+        if (warp == 4)
+          drain();
+        else
+          zero_rows();
       } else if (w4 * 32 < NT) {
         const int n = w4 * 32 + lane;
-        auto put = [&](uint32_t img, int chunk, const float* v) {  // 8 K-values of image row n
-          uint32_t t[4][3];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) split2<PB>(v[2 * q], v[2 * q + 1], t[q]);
-#pragma unroll
-          for (int b = 0; b < PB; ++b)
-            sts128(img + b * NT * 128 + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
-        };
-        const uint32_t ring = base + S::OFF_B + w4 * NU * S::UNIT_B;
+        const uint32_t ring = base + S::OFF_B + w4 * S::NU_B * S::UNIT_B;
         uint8_t* const mis = smem + S::OFF_MIS + (4 + w4) * NU * 32;
+        constexpr int NU_B = S::NU_B;
         float* const sc = reinterpret_cast<float*>(smem + S::OFF_SCALE) + w4 * NU * 32;
-        const int64_t row_bytes = (int64_t)p.b.width * sizeof(T);
-        const int64_t at = (int64_t)(wg_n0 + w4 * 32) * sizeof(T);
-        Walk<WG> f;
-        f.init(p, pre, t0, t1);
-        int fu = 0, slot_f = 0;
-        RowRef ref;
-        ref.load(p, f.lo, f.rows, f.row0() + lane);
+        const int row_bytes = p.b.width * (int)sizeof(T), at = (wg_n0 + w4 * 32) * (int)sizeof(T);
+        int left = 2 * (t1 - t0), slot_f = 0;
+        RowRef ref, ahead;
+        WalkRows rows{};
+        rows.w.init(p, q, t0);
+        rows.load(p, q, t1, ref);
+        rows.load(p, q, t1, ahead);
         auto fetch = [&]() {
-          if (!f.done()) {
+          if (left > 0) {
+            --left;
             const bool in = ref.valid(p);
             const int64_t o = in ? ref.offset(p.b) : 0;
             const uint32_t dst = ring + slot_f * S::UNIT_B;
@@ -836,46 +964,41 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
                                     : p.a_scale;
               cp_async4(tc::smem_u32(sc + slot_f * 32 + lane), src, in ? 4u : 0u);
             }
-            slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
-            if (++fu == 2) {
-              fu = 0;
-              f.next(p, pre);
-            }
-            if (!f.done()) ref.load(p, f.lo, f.rows, f.row0() + fu * 32 + lane);
+            slot_f = slot_f + 1 == NU_B ? 0 : slot_f + 1;
+            ref = ahead;
+            rows.load(p, q, t1, ahead);
           }
           cp_commit();
         };
-        for (int i = 0; i < NU - 1; ++i) fetch();
         int slot = 0;
-        for (int it = 0; it < t1 - t0 && ok; ++it) {
-          const int s = it & 1;
 #pragma unroll 1
-          for (int u = 0; u < 2; ++u) {
-            cp_wait<NU - 2>();
-            __syncwarp();
-            fetch();
-            const uint32_t src = ring + slot * S::UNIT_B;
-            const uint8_t* const ms = mis + slot * 32;
-            const float* const ss = sc + slot * 32;
-            slot = slot + 1 == NU ? 0 : slot + 1;
-            if (u == 0 && it >= 2) {
-              ok = __all_sync(0xffffffffu, tc::mbar_wait_or_abort(B_FREE(s), ((it >> 1) - 1) & 1, abort));
-              if (!ok) break;
-            }
-            const uint32_t img = base + s * PB * S::IMG;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float v[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int r = 8 * q + j;
-                v[j] = lds_as(src + r * S::PITCH_B + lane * (int)sizeof(T) + (VEC ? 0 : ms[r]), T{});
-                if constexpr (sizeof(TA) == 1) v[j] *= ss[r];
-              }
-              put(img, u * 4 + q, v);
-            }
+        for (int i = 1 - NU_B; i < 2 * (t1 - t0) && ok; ++i) {
+          const int it = i >> 1, u = i & 1, s = it & 1;
+          if (i >= 0) cp_wait<NU_B - 2>();
+          __syncwarp();
+          fetch();
+          if (i < 0) continue;
+          const uint32_t src = ring + slot * S::UNIT_B;
+          const uint8_t* const ms = mis + slot * 32;
+          const float* const ss = sc + slot * 32;
+          slot = slot + 1 == NU_B ? 0 : slot + 1;
+          if (u == 0 && it >= 2) {
+            ok = __all_sync(0xffffffffu, wait_phase(B_FREE(s), ((it >> 1) - 1) & 1, abort));
+            if (!ok) break;
           }
-          if (ok) {
+          const uint32_t img = base + s * PB * SL_IMG;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int r = 8 * q + j;
+              v[j] = lds_as(src + r * S::PITCH_B + lane * (int)sizeof(T) + (VEC ? 0 : ms[r]), T{});
+              if constexpr (sizeof(TA) == 1) v[j] *= ss[r];
+            }
+            put_eight<PB>(img, n, u * 4 + q, v);
+          }
+          if (u == 1) {
             tc::fence_proxy_async();
             tc::mbar_arrive(B_FULL(s));
           }
@@ -888,78 +1011,129 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     const int quad = warp & 3, half = (warp - 8) >> 2;
     const int CW = NT / 2;  // columns of this warp: 16, 32, 48 or 64
     const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16) + SL_D + half * CW;
-    Walk<WG> w;
-    w.init(p, pre, t0, t1);
+    Walk w;
+    w.init(p, q, t0);
     float acc[64];
     bool ok = true;
     bool fresh = true;  // acc holds nothing yet
-    RowRef ref{-1, 0};  // map: this lane's row of the tile, loaded while the tile is computed
+    RowRef ref{-1, -1};  // map: this lane's row of the tile, loaded while the tile is computed
+    int ct = 0, k = 0;   // map: the tile's column tile, the step
     // weight gradient: warp 8 issues the next step's MMAs before it takes this step's result
     auto issue_wg = [&](int it) {
       if (WG && warp == 8 && it < t1 - t0) ok = issue(it, it & 1, it >> 1, true);
     };
     issue_wg(0);
-    for (int it = 0; !w.done() && ok; ++it) {
+    for (int it = 0; w.t < t1 && ok; ++it) {
       const int s = it & 1;
       if constexpr (!WG) {
-        if (fresh) ref.load(p, w.lo, w.rows, w.row0() + quad * 32 + lane);
+        if (fresh) {
+          const Tile t(p, q, w);
+          ref.load(p, t.at + quad * 32 + lane, t.end);
+          ct = t.ct;
+        }
       }
       issue_wg(it + 1);
       if (!ok) break;
-      ok = tc::mbar_wait_or_abort(D_FULL(s), (it >> 1) & 1, abort);
+      ok = wait_phase(D_FULL(s), (it >> 1) & 1, abort);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc::fence_after_sync();
       const uint32_t td = tq + s * 128;
+      if (fresh) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t v[32];
-        if (h * 32 < CW) tmem_ld16u(td + h * 32, v);
-        if (h * 32 + 16 < CW) tmem_ld16u(td + h * 32 + 16, v + 16);
+        for (int k = 0; k < 64; ++k) acc[k] = 0.f;
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        uint32_t v[16];
+        if (h * 16 < CW) tmem_ld16u(td + h * 16, v);
         tc::tmem_wait_ld();
-        if (h == 1) {
+        if (h == 3) {
           tc::fence_before_sync();
           tc::mbar_arrive(D_FREE(s));
         }
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
-          acc[h * 32 + k] = fresh ? __uint_as_float(v[k]) : acc[h * 32 + k] + __uint_as_float(v[k]);
+        for (int k = 0; k < 16; ++k) acc[h * 16 + k] += __uint_as_float(v[k]);
       }
       fresh = false;
       if constexpr (!WG) {
-        if ((it + 1) % n_k != 0) continue;
-        const int c0 = w.ct * NT + half * CW;
-        T* dst = nullptr;
-        if (ref.valid(p)) dst = static_cast<T*>(p.out) + ref.node * p.out_sn + ref.m * p.out_sm + c0;
-        float* const stage = reinterpret_cast<float*>(smem + S::OFF_STG + (warp - 8) * S::STG);
+        if (++k < n_k) continue;
+        k = 0;
+        const int c0 = ct * NT + half * CW;
+        // Rows leave through shared memory, CB columns at a time: a thread holds one row, so stores straight from
+        // registers would touch 32 rows per instruction (measured 3600 cycles of the load/store unit per tile
+        // against 1500 staged).
+        constexpr int CB = 128 / sizeof(T);  // columns of a 128-byte row segment
+        const bool mine = ref.valid(p);
+        const int64_t o = mine ? ref.node * p.out_sn + ref.m * p.out_sm : -1;
+        // aligned rows: offsets in 16 bytes
+        const uint32_t o16 = mine ? (uint32_t)((uint64_t)o * sizeof(T) >> 4) : NO_ROW;
+        const uint32_t stage = base + S::OFF_STG + (warp - 8) * S::STG;
+        if constexpr (PB == 1) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int left = p.N - c0 - b * 16;
-          if (b * 16 >= CW || left <= 0) break;
+          for (int k = 0; k < 64; ++k) acc[k] *= p.alpha;
+        }
 #pragma unroll
-          for (int k = 0; k < 16; ++k) acc[b * 16 + k] *= p.alpha;
-          if (p.vst && left >= 16) {
-            if (dst) store16<T>(dst + b * 16, acc + b * 16, 16, p.vst);
-          } else {
-            // unaligned rows: two rows of 16 columns per store instruction
+        for (int b = 0; b < 64; b += CB) {
+          const int left = min(p.N - c0 - b, CW - b);  // columns of this segment
+          if (left <= 0) break;
+          // piece j of row r at j ^ (r & 7); the addresses are made here each time: held across the tiles they
+          // would push the accumulators to memory
+          int row = lane;
+          asm volatile("" : "+r"(row));
 #pragma unroll
-            for (int k = 0; k < 16; ++k) stage[lane * 17 + k] = acc[b * 16 + k];
-            __syncwarp();
-#pragma unroll 4
-            for (int r = 0; r < 32; r += 2) {
-              const int rr = r + (lane >> 4), k = lane & 15;
-              T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), rr));
-              if (to && k < left) to[b * 16 + k] = from_f32<T>(stage[rr * 17 + k]);
+          for (int j = 0; j < 8; ++j) {
+            uint32_t w4[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              if constexpr (sizeof(T) == 4)
+                w4[q] = __float_as_uint(acc[b + 4 * j + q]);
+              else
+                w4[q] = pack_bf16(acc[b + 8 * j + 2 * q], acc[b + 8 * j + 2 * q + 1]);
             }
-            __syncwarp();
+            sts128(stage + row * 128 + ((j ^ (row & 7)) << 4), w4[0], w4[1], w4[2], w4[3]);
           }
+          __syncwarp();
+          if (p.vst) {
+            // 4 rows x 128 bytes per instruction
+            const int j = row & 7;
+            const bool have = left * (int)sizeof(T) > 16 * j;
+            char* const to = static_cast<char*>(p.out) + (c0 + b) * (int)sizeof(T) + 16 * j;
+            const uint32_t src = stage + (row >> 3) * 128;
+#pragma unroll
+            for (int i0 = 0; i0 < 8; i0 += 4) {
+              uint4 v[4];
+              uint32_t ro[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {  // (r & 7 alternates between lane / 8 and lane / 8 + 4)
+                v[i] = lds128(src + (i0 + i) * 512 + ((j ^ ((row >> 3) + (i & 1) * 4)) << 4));
+                ro[i] = __shfl_sync(0xffffffffu, o16, (i0 + i) * 4 + (row >> 3));
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (ro[i] != NO_ROW && have) *reinterpret_cast<uint4*>(to + (uint64_t)ro[i] * 16) = v[i];
+            }
+          } else {
+            // unaligned rows: element by element, neighbouring lanes on neighbouring columns
+#pragma unroll 4
+            for (int r = 0; r < 32; ++r) {
+              const int64_t ro = __shfl_sync(0xffffffffu, o, r);
+#pragma unroll
+              for (int c = 0; c < CB; c += 32) {
+                const int byte = (c + lane) * (int)sizeof(T);
+                const T v = lds_raw(stage + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15)), T{});
+                if (ro >= 0 && c + lane < left) (static_cast<T*>(p.out) + ro + c0 + b)[c + lane] = v;
+              }
+            }
+          }
+          __syncwarp();
         }
         fresh = true;
-        w.next(p, pre);
+        w.next(q, t1);
       } else {
-        const bool group_ends = w.t + 1 == w.last;
-        if (group_ends || w.t + 1 == w.t1) {
-          const bool whole = group_ends && w.first >= t0;
+        const bool group_ends = w.t + 1 == pre[w.g + 1];
+        if (group_ends || w.t + 1 == t1) {
+          const bool whole = group_ends && pre[w.g] >= t0;
           const int kl = quad * 32 + lane, c0 = half * CW;
           if (whole) {
             if (wg_k0 + kl < p.K) {
@@ -982,7 +1156,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
           }
           fresh = true;
         }
-        w.next(p, pre);
+        w.next(q, t1);
       }
     }
     if (WG && warp == 8) drain();
@@ -990,7 +1164,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   tc::fence_before_sync();
   __syncthreads();
   if (tid == 0 && *abort) atomicExch(&g_species_error, TC_ERR_TIMEOUT);
-  if (warp == 8) {
+  if (warp == 15) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, SL_TMEM);
   }
@@ -1027,7 +1201,7 @@ __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constan
     before += sum[0][w];
     all += sum[1][w];
   }
-  // as in group_prefix
+  // as in load_groups
   before = min(before, (int64_t)INT32_MAX);
   all = min(all, (int64_t)INT32_MAX);
   const int tile = blockIdx.z;
@@ -1108,9 +1282,9 @@ int vector_bytes(const void* ptr, int64_t s0, int64_t s1, int64_t s2) {
   return 0;
 }
 
-bool aligned_rows(const RowView& v, int64_t n, int d) {
+bool aligned_rows(const RowView& v, int64_t n, int d, int size) {
   // (row offsets in 16 bytes fit 32 bits)
-  return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && (n <= 1 || v.sn % 16 == 0) && (d <= 1 || v.sm % 16 == 0) &&
+  return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && v.width * size % 16 == 0 && (n <= 1 || v.sn % 16 == 0) && (d <= 1 || v.sm % 16 == 0) &&
          ((n - 1) * v.sn + (d - 1) * v.sm) / 16 < (int64_t)NO_ROW;
 }
 
@@ -1162,7 +1336,8 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.out = y;
   p.out_sn = yn;
   p.out_sm = ym;
-  p.vst = vector_bytes(y, n > 1 ? yn * es : 0, d > 1 ? ym * es : 0, 0);
+  // (as for the input: whole 16-byte pieces, offsets in 32 bits)
+  p.vst = aligned_rows({static_cast<const char*>(y), yn * es, ym * es, M}, n, d, es);
   p.order = order;
   p.offsets = offsets;
   p.n = n;
@@ -1171,7 +1346,7 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.K = K;
   p.N = M;
   p.small = n * d < ((int64_t)1 << 32);
-  p.w_vec = transpose && K % 8 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
+  p.w_vec = (transpose ? K : M) * es % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
   p.alpha = alpha;
   const int sms = sm_count();
   const int64_t row_tiles = (n * d + 127) / 128;
@@ -1182,7 +1357,7 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.n_ct = (M + p.NT - 1) / p.NT;
   p.n_kt = 1;
   const int grid = (int)std::min<int64_t>(sms, (row_tiles + std::min<int64_t>(G, n)) * p.n_ct);
-  const bool vec = aligned_rows(p.a, n, d);
+  const bool vec = aligned_rows(p.a, n, d, es);
   if (dtype == MACE_F32)
     return vec ? launch_gemm<float, float, false, true>(p, grid, s) : launch_gemm<float, float, false, false>(p, grid, s);
   return vec ? launch_gemm<bf16, bf16, false, true>(p, grid, s) : launch_gemm<bf16, bf16, false, false>(p, grid, s);
@@ -1232,7 +1407,7 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   const int grid = p.shares * p.n_ct * p.n_kt;
   int rc = MACE_OK;
   if (n > 0) {
-    const bool vec = aligned_rows(p.a, n, d) && aligned_rows(p.b, n, d);
+    const bool vec = aligned_rows(p.a, n, d, xe) && aligned_rows(p.b, n, d, es);
     auto go = [&](auto ta, auto t) {
       using TA = decltype(ta);
       using T = decltype(t);
