@@ -440,6 +440,7 @@ int mace_ctx_error_flag(mace_ctx* ctx, int32_t* flag);
 #define MACE_F32 0
 #define MACE_BF16 1
 #define MACE_SPECIES_MAX_GROUPS 512      /* of the species-indexed linear map */
+#define MACE_SPECIES_MAX_ROWS 2147483136 /* n * d of the map: row numbers are 32-bit (a tile may end 511 past them) */
 #define MACE_SPECIES_MAX_INDEX 1048575   /* num_groups of grouping and embedding */
 #define MACE_SPECIES_MAX_CHANNELS 32768
 #define MACE_CHECKPOINT_BLOCK 128        /* channels that share one 8-bit scale */

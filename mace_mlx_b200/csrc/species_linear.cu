@@ -33,6 +33,7 @@
 // it is read from shared memory (template VEC = 0; VEC = 1 when every row is
 // 16-byte aligned).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "species.cuh"
@@ -72,7 +73,6 @@ struct SlParams {
   const int32_t* offsets;
   int64_t n;
   int d, G;
-  int small;            // n d < 2^32: row numbers divide in 32 bits
   int K, N;             // map: K summed channels, N outputs; weight gradient: K x N of dW
   int w_vec;            // map: rows of the weights are 16-byte aligned
   int NT;               // tile columns: 32, 64, 96 or 128
@@ -87,13 +87,15 @@ __device__ __forceinline__ constexpr uint32_t idesc_bf16(int N) {
 }
 
 // D[tmem] (+)= A[tmem] . B[smem]^T in bf16: A's M rows are the TMEM lanes, two
-// consecutive K elements per 32-bit column
-__device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+// consecutive K elements per 32-bit column; B's descriptor as its two halves
+__device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a, uint32_t blo, uint32_t bhi, uint32_t idesc,
+                                            bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, {%6, %6, %6, %6}, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(blo), "r"(bhi), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
       : "memory");
 }
 
@@ -206,6 +208,16 @@ __device__ __forceinline__ void sub2(float& x0, float& x1, uint32_t y0, uint32_t
       "mov.b64 a, {%0, %1};\n\t"
       "mov.b64 b, {%2, %3};\n\t"
       "sub.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "r"(y0), "r"(y1));
+}
+
+__device__ __forceinline__ void add2(float& x0, float& x1, uint32_t y0, uint32_t y1) {
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%0, %1};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\t"
       "mov.b64 {%0, %1}, a;\n\t}"
       : "+f"(x0), "+f"(x1)
       : "r"(y0), "r"(y1));
@@ -381,25 +393,23 @@ struct Walk {
   }
 };
 
-// Map: a tile's rows [at, end) of the grouped list (components counted), its column tile, and whether it is the
-// first or the last row tile of its (group, column tile).
+// Map: a tile's rows [at, end) of the grouped list (components counted), its column tile, and how many tiles of the
+// same (group, column tile) are left with it.
 struct Tile {
-  int64_t at, end;
-  int ct;
-  bool first, last;
+  int at, end;
+  int ct, run;
   __device__ __forceinline__ Tile(const SlParams& p, const Groups& q, const Walk& w) {
-    at = (int64_t)q.lo[w.g] * p.d;
-    end = (int64_t)q.hi[w.g] * p.d;
-    const int n_rt = (int)((end - at + 127) >> 7);
+    at = q.lo[w.g] * p.d;
+    end = q.hi[w.g] * p.d;
+    const int n_rt = (end - at + 127) >> 7;
     int rt = w.t - q.pre[w.g];
     ct = 0;
     if (p.n_ct > 1) {
       ct = rt / n_rt;
       rt -= ct * n_rt;
     }
-    at += (int64_t)rt * 128;
-    first = rt == 0;
-    last = rt + 1 == n_rt;
+    at += rt * 128;
+    run = n_rt - rt;
   }
 };
 
@@ -407,14 +417,14 @@ struct Tile {
 // and its result first read by valid(): selecting a default right after the load would wait for it.
 struct RowRef {
   int node, m;  // m < 0: no such row
-  __device__ __forceinline__ void load(const SlParams& p, int64_t at, int64_t end) {
+  __device__ __forceinline__ void load(const SlParams& p, int at, int end) {
     const bool in = at < end;
     at = min(at, end - 1);
-    int64_t i = at;
+    int i = at;
     m = 0;
     if (p.d > 1) {
-      i = p.small ? (int64_t)((uint32_t)at / (uint32_t)p.d) : at / p.d;
-      m = (int)(at - i * p.d);
+      i = (uint32_t)at / (uint32_t)p.d;
+      m = at - i * p.d;
     }
     if (!in) m = -1;
     asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(node) : "l"(p.order + i));
@@ -423,18 +433,26 @@ struct RowRef {
   __device__ __forceinline__ int64_t offset(const RowView& v) const { return node * v.sn + m * v.sm; }
 };
 
-// Weight gradient: the atoms of consecutive 32-row units, one row per lane.
-struct WalkRows {
+// Weight gradient: a lane's rows of the two 32-row ring units of a step, loaded a step ahead (moving a loaded value
+// waits for it, so the distance between load and move is what hides the latency).
+struct StepRows {
+  RowRef now[2], next[2];
   Walk w;
-  int u;
-  __device__ __forceinline__ void load(const SlParams& p, const Groups& q, int t1, RowRef& ref) {
+  __device__ __forceinline__ void load(const SlParams& p, const Groups& q, int t1) {
     if (w.t >= t1) return;
-    ref.load(p, (int64_t)q.lo[w.g] * p.d + (int64_t)(w.t - q.pre[w.g]) * SL_KC + u * 32 + (threadIdx.x & 31),
-             (int64_t)q.hi[w.g] * p.d);
-    if (++u == 2) {
-      u = 0;
-      w.next(q, t1);
-    }
+    const int at = q.lo[w.g] * p.d + (w.t - q.pre[w.g]) * SL_KC + (threadIdx.x & 31), end = q.hi[w.g] * p.d;
+    next[0].load(p, at, end);
+    next[1].load(p, at + 32, end);
+    w.next(q, t1);
+  }
+  __device__ __forceinline__ void init(const SlParams& p, const Groups& q, int t0, int t1) {
+    w.init(p, q, t0);
+    load(p, q, t1);
+  }
+  __device__ __forceinline__ void step(const SlParams& p, const Groups& q, int t1) {
+    now[0] = next[0];
+    now[1] = next[1];
+    load(p, q, t1);
   }
 };
 
@@ -554,19 +572,25 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint32_t img0, u
   const T* wt = static_cast<const T*>(p.w) + (int64_t)g * p.K * p.N;
   if (p.w_vec) {
     constexpr int E = 16 / sizeof(T);  // elements of a piece
-    // 64 x NT (transposed: NT x 64) elements of a step, the columns (K) in 64 / E or fewer pieces
-    const int width = p.transposed ? SL_KC : NT, ppr = width / E, pieces = (p.transposed ? NT : SL_KC) * ppr;
+    // rows of a step: 64 of NT weights, transposed NT of 64; a warp takes as many as its lanes hold pieces of
+    const int ppr = (p.transposed ? SL_KC : NT) / E, rpi = 32 / ppr;
+    const int rows = p.transposed ? NT : SL_KC, pitch = p.transposed ? p.K : p.N;
+    const int sub = lane / ppr, c = (lane - sub * ppr) * E;
+    const bool on = sub < rpi;
 #pragma unroll 1
     for (int s = 0; s < nk; ++s) {
       const uint32_t raw = img0 + s * stride;
-#pragma unroll 4
-      for (int i = w4 * 32 + lane; i < pieces; i += 128) {
-        const int r = (uint32_t)i / (uint32_t)ppr, c = (i - r * ppr) * E;
-        const int kk = p.transposed ? c : r, nn = p.transposed ? r : c;
-        const int k = (k0 + s) * SL_KC + kk, n = ct * NT + nn;
-        const bool in = k < p.K && n < p.N;
-        const T* src = p.transposed ? wt + (int64_t)n * p.K + k : wt + (int64_t)k * p.N + n;
-        cp_async16_or_zero(raw + raw_place<T>(kk, nn, p.transposed), in ? src : wt, !in);
+      const int k = (k0 + s) * SL_KC, n = ct * NT;
+      const int r0 = p.transposed ? n : k, c0 = (p.transposed ? k : n) + c;  // in the whole matrix
+      const int r_end = p.transposed ? p.N : p.K, c_end = p.transposed ? p.K : p.N;
+      int r = w4 * rpi + sub;
+      const T* src = wt + (int64_t)(r0 + r) * pitch + c0;
+      const int64_t hop = (int64_t)(4 * rpi) * pitch;
+#pragma unroll 8
+      for (; r < rows && on; r += 4 * rpi, src += hop) {
+        const bool in = r0 + r < r_end && c0 < c_end;
+        cp_async16_or_zero(raw + raw_place<T>(p.transposed ? c : r, p.transposed ? r : c, p.transposed), in ? src : wt,
+                           !in);
       }
     }
     cp_commit();
@@ -703,33 +727,35 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   const bool resident = n_k <= S::NSLOT;               // map: the weight images of a tile stay for the next row tile
   const uint32_t tmem = SL_D;  // an allocation of all 512 columns starts at column 0
 
-  // MMAs of step `it` with the images of slot bs, by a whole warp with warp-uniform
-  // operands (one elected lane issues); `use`: how often the slot was filled
-  // before, or -1 when its images were there already
+  // MMAs of step `it` with the images of slot bs, by one elected thread; `use`: how often the slot was filled
+  // before, or -1 when its images were there already.  The queue of issued MMAs is a few hundred cycles deep, so the
+  // path from one step's last to the next step's first is kept short: two waits, no warp-wide operation
+  const uint32_t idesc = idesc_bf16(NT), bhi = (uint32_t)(tc::sw128_desc(base) >> 32);
   auto issue = [&](int it, int bs, int use, bool release) -> bool {
     using PR = Products<PA, PB>;
     const int s = it & 1;
-    bool ok = use < 0 || wait_phase(B_FULL(bs), use & 1, abort);
-    ok = ok && wait_phase(A_FULL(s), (it >> 1) & 1, abort);
-    if (ok && it >= 2) ok = wait_phase(D_FREE(s), ((it >> 1) - 1) & 1, abort);
-    if (!__all_sync(0xffffffffu, ok)) return false;
+    if (use >= 0 && !wait_phase(B_FULL(bs), use & 1, abort)) return false;
+    if (!wait_phase(A_FULL(s), (it >> 1) & 1, abort)) return false;
+    if (it >= 2 && !wait_phase(D_FREE(s), ((it >> 1) - 1) & 1, abort)) return false;
     tc::fence_after_sync();
-    const uint32_t us = __shfl_sync(0xffffffffu, s, 0), ub = __shfl_sync(0xffffffffu, bs, 0);
-    const uint32_t idesc = idesc_bf16(p.NT);
-    const uint64_t desc = tc::sw128_desc(base + ub * (PB * SL_IMG));
-    const uint32_t d = SL_D + us * 128, a = SL_A + us * (PA * 32);
-    if (elect_one()) {
+    const uint32_t blo = (uint32_t)tc::sw128_desc(base + bs * (PB * SL_IMG));
+    // the stage as a constant: the only operand left to compute is the low half of B's descriptor
+    auto emit = [&](auto stage) {
+      constexpr uint32_t st = decltype(stage)::value;
 #pragma unroll
       for (int q = 0; q < PR::n; ++q)
 #pragma unroll
         for (int ks = 0; ks < SL_KC / 16; ++ks)
-          mma_bf16_ta(d, a + PR::a(q) * 32 + ks * 8, desc + (uint32_t)(PR::b(q) * (SL_IMG / 16) + ks * 2), idesc,
-                      q > 0 || ks > 0);
-      tc::mma_commit(A_FREE(s));
-      if (release) tc::mma_commit(B_FREE(bs));
-      tc::mma_commit(D_FULL(s));
-    }
-    __syncwarp();
+          mma_bf16_ta(SL_D + st * 128, SL_A + st * (PA * 32) + PR::a(q) * 32 + ks * 8,
+                      blo + PR::b(q) * (SL_IMG / 16) + ks * 2, bhi, idesc, q > 0 || ks > 0);
+    };
+    if (s)
+      emit(std::integral_constant<uint32_t, 1>{});
+    else
+      emit(std::integral_constant<uint32_t, 0>{});
+    tc::mma_commit(A_FREE(s));
+    tc::mma_commit(D_FULL(s));
+    if (release) tc::mma_commit(B_FREE(bs));
     return true;
   };
   auto drain = [&]() {  // every MMA issued is complete (bounded)
@@ -751,13 +777,13 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     const int tile_units = n_k * S::UPC;  // ring units of a tile
     const int units = (t1 - t0) * tile_units;
     int left = units, fu = 0, slot_f = 0;  // units to fetch, unit within the tile, ring slot
-    RowRef ref, ahead;
-    WalkRows rows{};
-    rows.w.init(p, q, t0);
+    RowRef ref;      // map: this lane's row of the next tile
+    Walk w_tile;
+    StepRows rows;   // weight gradient
     uint32_t off[Pieces<S::SEG_A>::N];
     const char* row = nullptr;
     auto load_tile = [&]() {
-      const Tile t(p, q, rows.w);
+      const Tile t(p, q, w_tile);
       ref.load(p, t.at + warp * 32 + lane, t.end);
     };
     // the loaded rows become the fetched ones.  Map: a row outside the tile may hold anything (its
@@ -773,15 +799,14 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     auto fetch = [&]() {
       if (left > 0) {
         --left;
-        if (fu == 0) {
+        if constexpr (WG) {
+          if (fu == 0) rows.step(p, q, t1);
+          ref = fu == 0 ? rows.now[0] : rows.now[1];
           take_rows();
-          if constexpr (WG) {
-            ref = ahead;
-            rows.load(p, q, t1, ahead);
-          } else {
-            rows.w.next(q, t1);
-            if (rows.w.t < t1) load_tile();
-          }
+        } else if (fu == 0) {
+          take_rows();
+          w_tile.next(q, t1);
+          if (w_tile.t < t1) load_tile();
         }
         const uint32_t dst = ring + slot_f * S::UNIT_A;
         const int at = WG ? (wg_k0 + warp * 32) * (int)sizeof(TA) : fu * 128;
@@ -790,14 +815,14 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         else
           fetch_any<S::SEG_A, S::PITCH_A>(dst, p.a.data, row, at, row_bytes, mis + slot_f * 32);
         slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
-        if (!WG && ++fu == tile_units) fu = 0;
+        if (++fu == tile_units) fu = 0;
       }
       cp_commit();
     };
     if constexpr (WG) {
-      rows.load(p, q, t1, ref);
-      rows.load(p, q, t1, ahead);
+      rows.init(p, q, t0, t1);
     } else {
+      w_tile.init(p, q, t0);
       load_tile();
     }
     // (one loop, so that the code of a unit exists once: the roles' loops together fill the instruction cache)
@@ -898,34 +923,33 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
                                      syncs, abort);
         };
         Walk w;
+        w.init(p, q, t0);
         int it = 0, fills = 0;  // steps; image sets (resident) or images written
-        for (w.init(p, q, t0); w.t < t1 && ok; w.next(q, t1)) {
+        while (w.t < t1 && ok) {
           const Tile t(p, q, w);
-          const bool renew = !resident || t.first || w.t == t0;      // the images are new
-          const bool release = !resident || t.last || w.t + 1 == t1;  // and free after this tile
-          if (resident && renew) {
-            for (int k = 0; k < n_k && ok && fills > 0; ++k)
-              ok = wait_phase(B_FREE(k), (fills - 1) & 1, abort);
-            ok = __all_sync(0xffffffffu, ok);
+          if (resident) {
+            // the tiles of this CTA that share the weights
+            const int run = min(t.run, t1 - w.t);
+            for (int k = 0; k < n_k && ok && fills > 0; ++k) ok = wait_phase(B_FREE(k), (fills - 1) & 1, abort);
+            ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, 0, n_k, 0);
             if (!ok) break;
-            ok = fill(w.g, t.ct, 0, n_k, 0);
-            if (!ok) break;
+            if (warp == 4 && elect_one())
+              for (int i = 0; i < run && ok; ++i)
+                for (int k = 0; k < n_k && ok; ++k) ok = issue(it + i * n_k + k, k, i == 0 ? fills : -1, i + 1 == run);
+            it += run * n_k;
             ++fills;
-          }
-          for (int k = 0; k < n_k && ok; ++k, ++it) {
-            int s = k, use = renew ? fills - 1 : -1;
-            if (!resident) {
-              s = fills % S::NSLOT;
-              use = fills / S::NSLOT;
-              ++fills;
+            w.t += run - 1;
+          } else {
+            for (int k = 0; k < n_k && ok; ++k, ++it, ++fills) {
+              const int s = fills % S::NSLOT, use = fills / S::NSLOT;
               ok = use == 0 || wait_phase(B_FREE(s), (use - 1) & 1, abort);
+              ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, k, 1, s);
+              if (ok && warp == 4 && elect_one()) ok = issue(it, s, use, true);
               ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              ok = fill(w.g, t.ct, k, 1, s);
-              if (!ok) break;
             }
-            if (warp == 4) ok = issue(it, s, use, release);
           }
+          ok = __all_sync(0xffffffffu, ok);
+          w.next(q, t1);
         }
         if (warp == 4)
           drain();
@@ -939,14 +963,14 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         float* const sc = reinterpret_cast<float*>(smem + S::OFF_SCALE) + w4 * NU * 32;
         const int row_bytes = p.b.width * (int)sizeof(T), at = (wg_n0 + w4 * 32) * (int)sizeof(T);
         int left = 2 * (t1 - t0), slot_f = 0;
-        RowRef ref, ahead;
-        WalkRows rows{};
-        rows.w.init(p, q, t0);
-        rows.load(p, q, t1, ref);
-        rows.load(p, q, t1, ahead);
+        StepRows rows;
+        rows.init(p, q, t0, t1);
         auto fetch = [&]() {
           if (left > 0) {
+            const bool second = left & 1;
             --left;
+            if (!second) rows.step(p, q, t1);
+            const RowRef ref = second ? rows.now[1] : rows.now[0];
             const bool in = ref.valid(p);
             const int64_t o = in ? ref.offset(p.b) : 0;
             const uint32_t dst = ring + slot_f * S::UNIT_B;
@@ -965,8 +989,6 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
               cp_async4(tc::smem_u32(sc + slot_f * 32 + lane), src, in ? 4u : 0u);
             }
             slot_f = slot_f + 1 == NU_B ? 0 : slot_f + 1;
-            ref = ahead;
-            rows.load(p, q, t1, ahead);
           }
           cp_commit();
         };
@@ -1020,7 +1042,10 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     int ct = 0, k = 0;   // map: the tile's column tile, the step
     // weight gradient: warp 8 issues the next step's MMAs before it takes this step's result
     auto issue_wg = [&](int it) {
-      if (WG && warp == 8 && it < t1 - t0) ok = issue(it, it & 1, it >> 1, true);
+      if (WG && warp == 8 && it < t1 - t0) {
+        if (elect_one()) ok = issue(it, it & 1, it >> 1, true);
+        ok = __all_sync(0xffffffffu, ok);
+      }
     };
     issue_wg(0);
     for (int it = 0; w.t < t1 && ok; ++it) {
@@ -1053,7 +1078,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
           tc::mbar_arrive(D_FREE(s));
         }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) acc[h * 16 + k] += __uint_as_float(v[k]);
+        for (int k = 0; k < 16; k += 2) add2(acc[h * 16 + k], acc[h * 16 + k + 1], v[k], v[k + 1]);
       }
       fresh = false;
       if constexpr (!WG) {
@@ -1148,11 +1173,13 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
               }
             }
           } else {
-            // (share, group) pairs of one tile are a staircase: share + g numbers them
-            float* dst = p.part + (((int64_t)tile * (p.shares + p.G) + share + w.g) * 128 + kl) * NT + c0;
+            // (share, group) pairs of one tile are a staircase: share + g numbers them.  A partial tile is stored
+            // as [column quad][row]: a warp's 32 rows are one line per instruction
+            float4* dst = reinterpret_cast<float4*>(p.part) +
+                          ((int64_t)tile * (p.shares + p.G) + share + w.g) * 32 * NT + c0 / 4 * 128 + kl;
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-              if (b * 16 < CW) store16<float>(dst + b * 16, acc + b * 16, 16, 32);
+            for (int b = 0; b < 16; ++b)
+              if (b * 4 < CW) dst[b * 128] = make_float4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
           }
           fresh = true;
         }
@@ -1170,9 +1197,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   }
 }
 
-// dW of the groups that several shares hold, in share order, and of empty groups (zero).
-// One CTA: group blockIdx.x, 256 consecutive elements of tile blockIdx.z (64 lanes of
-// four columns x 4 share lanes).
+// dW of the groups that several shares hold, in share order, and of empty groups (zero).  One CTA: group blockIdx.x,
+// 8 rows x 8 column quads (one per lane of 64) of tile blockIdx.z, four threads of each taking every fourth share.
 template <typename T>
 __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constant__ SlParams p) {
   __shared__ int64_t sum[2][8];
@@ -1207,9 +1233,8 @@ __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constan
   const int tile = blockIdx.z;
   const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
   const int lane = tid & 63, sl = tid >> 6;
-  const int e = blockIdx.y * 256 + lane * 4;  // element of the 128 x NT tile
-  const int kl = e / p.NT, c = e % p.NT;
-  const bool in = e < 128 * p.NT && k0 + kl < p.K;
+  const int kl = (blockIdx.y & 15) * 8 + (lane & 7), cq = (blockIdx.y >> 4) * 8 + (lane >> 3), c = cq * 4;
+  const bool in = k0 + kl < p.K && n0 + c < p.N;
   T* dst = static_cast<T*>(p.out) + ((int64_t)g * p.K + k0 + kl) * p.N + n0 + c;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (mine > 0) {
@@ -1219,10 +1244,11 @@ __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constan
     const int s1 = (int)min(((before + mine) * shares - 1) / all, shares - 1);
     if (s0 == s1) return;  // written by its only share
     if (in) {
-      const float* src = p.part + (((int64_t)tile * (p.shares + p.G) + g) * 128 + kl) * p.NT + c;
+      const float4* src = reinterpret_cast<const float4*>(p.part) +
+                          ((int64_t)tile * (p.shares + p.G) + g) * 32 * p.NT + cq * 128 + kl;
 #pragma unroll 4
       for (int s = s0 + sl; s <= s1; s += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src + (int64_t)s * 128 * p.NT);
+        const float4 v = src[(int64_t)s * 32 * p.NT];
         acc.x += v.x;
         acc.y += v.y;
         acc.z += v.z;
@@ -1254,7 +1280,7 @@ bool bad_sizes(int32_t dtype, int64_t n, int32_t d, int32_t G, int32_t K, int32_
   return (dtype != MACE_F32 && dtype != MACE_BF16) || n < 0 || n > INT32_MAX || d < 1 || d > 1024 || G < 1 ||
          G > MACE_SPECIES_MAX_GROUPS || K < 1 || K > MACE_SPECIES_MAX_CHANNELS || M < 1 ||
          M > MACE_SPECIES_MAX_CHANNELS ||
-         (n * d + 63) / 64 + G > INT32_MAX / ((M + 31) / 32);
+         n * d > MACE_SPECIES_MAX_ROWS || (n * d + 63) / 64 + G > INT32_MAX / ((M + 31) / 32);
 }
 
 int sm_count() {
@@ -1345,7 +1371,6 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.G = G;
   p.K = K;
   p.N = M;
-  p.small = n * d < ((int64_t)1 << 32);
   p.w_vec = (transpose ? K : M) * es % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
   p.alpha = alpha;
   const int sms = sm_count();
@@ -1401,7 +1426,6 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   p.G = G;
   p.K = K;
   p.N = M;
-  p.small = n * d < ((int64_t)1 << 32);
   p.alpha = alpha;
   wgrad_split(n, d, G, K, M, &p);
   const int grid = p.shares * p.n_ct * p.n_kt;
@@ -1419,7 +1443,7 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
       rc = dtype == MACE_F32 ? go(float{}, float{}) : go(bf16{}, bf16{});
     if (rc) return rc;
   }
-  const dim3 jg(G, (128 * p.NT + 255) / 256, p.n_ct * p.n_kt);
+  const dim3 jg(G, 16 * (p.NT / 32), p.n_ct * p.n_kt);
   if (dtype == MACE_F32)
     k_species_wgrad_join<float><<<jg, 256, 0, s>>>(p);
   else

@@ -143,6 +143,7 @@ NOALLOC_MAX_GRAPH_ATOMS = 16384
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 SPECIES_MAX_GROUPS = 512
+SPECIES_MAX_ROWS = 2147483136
 SPECIES_MAX_INDEX = 1048575
 SPECIES_MAX_CHANNELS = 32768
 CHECKPOINT_BLOCK = 128
