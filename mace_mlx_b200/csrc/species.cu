@@ -16,6 +16,7 @@ namespace {
 // row movers: threads of a CTA and vectors per thread (loads in flight)
 constexpr int RW_THREADS = 256;
 constexpr int RW_UNROLL = 4;
+constexpr int RS_UNROLL = 8;  // of the restore, whose loads are 4 bytes
 
 // x / C for x < 2^32 / C by multiplication: the row of a CTA's local element
 // (x < RW_THREADS RW_UNROLL 8 + C and C <= 32768 stay below the limit)
@@ -124,10 +125,16 @@ __device__ __forceinline__ int cta_exclusive(int v, int* warp_sums) {
   return before + s - v;
 }
 
-// rank of this lane's digit among the equal digits of lower lanes; `mine`: next
-// position of each digit for this warp, moved past the rows placed here
-__device__ __forceinline__ int place(int* mine, int digit, bool in, int lane) {
-  const unsigned same = __match_any_sync(0xffffffffu, in ? digit : -1);
+// Position of this lane's row: `mine` holds the next position of each digit for this warp and is moved past the rows
+// placed here.  Lanes of equal digit find one another bit by bit with ballots (match_any on spread digits costs
+// several times as much: the pass over 4M rows took 56 us with it).
+__device__ __forceinline__ int place(int* mine, int digit, int bits, bool in, int lane) {
+  unsigned same = __ballot_sync(0xffffffffu, in);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1;
+    const unsigned m = __ballot_sync(0xffffffffu, one);
+    same &= one ? m : ~m;
+  }
   const int rank = __popc(same & ((1u << lane) - 1));
   const int at = in ? mine[digit] + rank : 0;
   __syncwarp();
@@ -194,7 +201,7 @@ __global__ void __launch_bounds__(GR_THREADS) k_group_scatter(GroupPass p) {
   for (int j = 0; j < SEG / 32; ++j) {
     const int64_t i = i0 + j * 32 + lane;
     const bool in = i < i1;
-    const int at = place(mine, digit_of(p, z[j]), in, lane);
+    const int at = place(mine, digit_of(p, z[j]), p.bits, in, lane);
     if (in) {
       sm.key[at] = z[j];
       sm.row[at] = p.row ? p.row[i] : (int32_t)i;
@@ -212,7 +219,7 @@ __global__ void __launch_bounds__(GR_THREADS) k_group_scatter(GroupPass p) {
 }
 
 __global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __restrict__ species, int n, int G,
-                                                            int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
+                                                            int bits, int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
   __shared__ int whist[32][GS_MAX_BINS];
   __shared__ int sums[32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -240,7 +247,7 @@ __global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __res
     const int i = base + lane;
     const bool in = i < i1;
     const int key = in ? row_key(species[i], G) : 0;
-    const int to = place(whist[warp], key, in, lane);
+    const int to = place(whist[warp], key, bits, in, lane);
     if (in) order[to] = i;
   }
 }
@@ -338,9 +345,9 @@ __device__ __forceinline__ int group_at(const int32_t* __restrict__ offsets, int
 constexpr int EG_THREADS = 256;
 
 template <typename T, int V, int RL>
-__global__ void __launch_bounds__(EG_THREADS) k_embed_grad(EmbedGrad p) {
-  constexpr int CL = 32 / RL;  // channel lanes
-  constexpr int UN = 8;        // row loads in flight per lane
+__global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad(EmbedGrad p) {
+  constexpr int CL = 32 / RL;             // channel lanes
+  constexpr int UN = RL == 8 ? 4 : 8;     // row loads in flight per lane (UN RL <= 32)
   const int lane = threadIdx.x & 31, cl = lane % CL, rl = lane / CL;
   const int64_t share = blockIdx.x * (int64_t)(EG_THREADS / 32) + (threadIdx.x >> 5);
   if (share >= p.shares) return;
@@ -350,9 +357,8 @@ __global__ void __launch_bounds__(EG_THREADS) k_embed_grad(EmbedGrad p) {
   int64_t i = share * p.share;
   const T* dy = static_cast<const T*>(p.dy) + (in ? c0 : 0);
   bool first = true;
-  while (i < i1) {
-    const int g = group_at(p.offsets, p.G, i);
-    if (g >= p.G) break;  // padding rows are last
+  int g = group_at(p.offsets, p.G, i);
+  while (i < i1 && g < p.G) {  // (padding rows are last)
     const int64_t lo = p.offsets[g], hi = p.offsets[g + 1];
     const int64_t end = imin64(i1, hi);
     float acc[V] = {};
@@ -364,22 +370,16 @@ __global__ void __launch_bounds__(EG_THREADS) k_embed_grad(EmbedGrad p) {
       const int rows = (int)imin64(32, end - b);
 #pragma unroll 1
       for (int j0 = 0; j0 < rows; j0 += UN * RL) {
-        float v[UN][V];
+        Raw<T, V> v[UN];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
           const int j = j0 + u * RL + rl;
-          const int64_t row = __shfl_sync(0xffffffffu, mine, j & 31);
-          if (j < 32 && row >= 0 && row < p.n && in) {
-            load_channels<T, V>(dy + row * p.ds, v[u]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[u][k] = 0.f;
-          }
+          const int64_t row = __shfl_sync(0xffffffffu, mine, j);
+          v[u].zero();
+          if (row >= 0 && row < p.n && in) v[u].load(dy + row * p.ds);
         }
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
-#pragma unroll
-          for (int k = 0; k < V; ++k) acc[k] += v[u][k];
+        for (int u = 0; u < UN; ++u) v[u].add_to(acc);
       }
     }
 #pragma unroll
@@ -400,16 +400,19 @@ __global__ void __launch_bounds__(EG_THREADS) k_embed_grad(EmbedGrad p) {
     }
     first = false;
     i = end > i ? end : i1;  // offsets that do not rise end the walk
+    // the next group with rows: mostly the next one
+    if (++g < p.G && !(p.offsets[g + 1] > i)) g = group_at(p.offsets, p.G, i);
   }
 }
 
 // Groups that several shares hold: their partial rows, in share order; empty
 // groups: zero.  A warp takes a group of few shares by itself; the CTA's 32
-// warps take the others together.  32 channels per CTA.
+// warps take the others together.  32 channels and per_cta groups per CTA and round (few groups: one each, so
+// that they are joined side by side).
 constexpr int EJ_ALONE = 16;
 
 template <typename T>
-__global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p) {
+__global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p, int per_cta) {
   __shared__ float sums[32][33];
   __shared__ uint32_t many;
   const int cl = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -434,12 +437,12 @@ __global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p) {
     }
     return acc;
   };
-  for (int g0 = blockIdx.x * 32; g0 < p.G; g0 += gridDim.x * 32) {
+  for (int g0 = blockIdx.x * per_cta; g0 < p.G; g0 += gridDim.x * per_cta) {
     if (threadIdx.x == 0) many = 0;
     __syncthreads();
     const int g = g0 + warp;
     int64_t s0 = 0, s1 = 0;
-    if (g < p.G) {
+    if (warp < per_cta && g < p.G) {
       if (!span(g, &s0, &s1)) {
         if (c < p.C) out[(int64_t)g * p.C + c] = from_f32<T>(0.f);
       } else if (s1 - s0 >= EJ_ALONE) {
@@ -521,17 +524,16 @@ __global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* __restrict__
     top = __reduce_max_sync(0xffffffffu, top);
     const float s = __fmul_rn(__int_as_float(top), 1.0f / 127.0f);
     if (lane == u) mine = s;
+    const uint32_t packed = quantise8x4(v[u], s);
     const int c0 = b * MACE_CHECKPOINT_BLOCK + (VEC ? 4 * lane : lane);
     if (i0 + u < items) {
       int8_t* dst = q + r * C + c0;
       if constexpr (VEC) {
-        if (c0 < C)
-          *reinterpret_cast<char4*>(dst) = make_char4(quantise8(v[u][0], s), quantise8(v[u][1], s),
-                                                      quantise8(v[u][2], s), quantise8(v[u][3], s));
+        if (c0 < C) *reinterpret_cast<uint32_t*>(dst) = packed;
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (c0 + 32 * j < C) dst[32 * j] = quantise8(v[u][j], s);
+          if (c0 + 32 * j < C) dst[32 * j] = (int8_t)(packed >> (8 * j));
       }
     }
     if (++b == nb) {
@@ -547,12 +549,12 @@ template <typename T>
 __global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* __restrict__ q, const float* __restrict__ scale,
                                                         int64_t total, int C, int nb, T* __restrict__ x, RowDiv div,
                                                         int vec) {
-  const int64_t e0 = blockIdx.x * (int64_t)(RW_THREADS * RW_UNROLL * 4);
+  const int64_t e0 = blockIdx.x * (int64_t)(RW_THREADS * RS_UNROLL * 4);
   const int64_t row0 = e0 / C;
   const uint32_t first = (uint32_t)(e0 - row0 * C);
-  char4 w[RW_UNROLL];
+  char4 w[RS_UNROLL];
 #pragma unroll
-  for (int j = 0; j < RW_UNROLL; ++j) {
+  for (int j = 0; j < RS_UNROLL; ++j) {
     const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
     if (vec && at + 4 <= total) {
       w[j] = *reinterpret_cast<const char4*>(q + at);
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* __restrict
     }
   }
 #pragma unroll
-  for (int j = 0; j < RW_UNROLL; ++j) {
+  for (int j = 0; j < RS_UNROLL; ++j) {
     const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
     if (at >= total) break;
     const uint32_t local = first + (threadIdx.x + j * RW_THREADS) * 4;
@@ -610,8 +612,8 @@ void group_passes(int G, int* bits, int* passes) {
 }
 
 // rows of one warp's share of the table gradient: enough warps to fill the
-// GPU (148 SMs x 4 CTAs x 8 warps), but shares of at least 16 rows
-int64_t eg_share(int64_t n) { return std::max<int64_t>(16, (n + 148 * 32 - 1) / (148 * 32)); }
+// GPU once (148 SMs x 3 CTAs x 8 warps), but shares of at least 16 rows
+int64_t eg_share(int64_t n) { return std::max<int64_t>(16, (n + 148 * 24 - 1) / (148 * 24)); }
 int64_t eg_shares(int64_t n, int64_t share) { return (n + share - 1) / share; }
 
 int64_t align16(int64_t b) { return (b + 15) & ~(int64_t)15; }
@@ -626,6 +628,7 @@ namespace {
 
 struct GroupPlan {
   int bits, passes, nb;
+  bool small;  // one CTA, one launch, no workspace
   int64_t counts, keys, bytes;  // bytes of the count tables, of one key or row array, and of the whole workspace
 };
 bool group_plan(int64_t n, int32_t G, GroupPlan* p) {
@@ -636,6 +639,8 @@ bool group_plan(int64_t n, int32_t G, GroupPlan* p) {
   p->keys = align16(n * 4);
   // two passes: keys and rows after the first, keys after the second
   p->bytes = p->counts + (p->passes > 1 ? 3 * p->keys : 0);
+  p->small = n <= GS_MAX_ROWS && G < GS_MAX_BINS;
+  if (p->small) p->bytes = 0;
   return true;
 }
 
@@ -654,15 +659,15 @@ extern "C" int mace_species_group(const int32_t* species, int64_t n, int32_t G, 
   GroupPlan plan;
   if (!group_plan(n, G, &plan) || !offsets || (n > 0 && (!species || !order)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_group: bad arguments");
-  if (n > 0 && (!ws || ws_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(ws) & 15) != 0))
+  if (plan.bytes > 0 && (!ws || ws_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(ws) & 15) != 0))
     return fail(MACE_ERR_BAD_ARG, "mace_species_group: workspace too small or not 16-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (n == 0) {
     MACE_CUDA_TRY(cudaMemsetAsync(offsets, 0, (size_t)(G + 1) * 4, s));
     return MACE_OK;
   }
-  if (n <= GS_MAX_ROWS && G < GS_MAX_BINS) {
-    k_group_small<<<1, GS_THREADS, 0, s>>>(species, (int)n, G, order, offsets);
+  if (plan.small) {
+    k_group_small<<<1, GS_THREADS, 0, s>>>(species, (int)n, G, plan.bits, order, offsets);
     MACE_LAUNCH_CHECK("group_small");
     return MACE_OK;
   }
@@ -787,7 +792,9 @@ int embed_grad(const EmbedGrad& p, cudaStream_t s) {
       launch_embed_grad<T, 1>(p, s);
     MACE_LAUNCH_CHECK("species_embed_grad");
   }
-  k_embed_grad_join<T><<<dim3((unsigned)std::min((p.G + 31) / 32, 148 * 2), (p.C + 31) / 32), 1024, 0, s>>>(p);
+  const int per_cta = std::max(1, std::min(32, (p.G + 147) / 148));
+  k_embed_grad_join<T><<<dim3((unsigned)std::min((p.G + per_cta - 1) / per_cta, 148 * 2), (p.C + 31) / 32), 1024, 0,
+                         s>>>(p, per_cta);
   MACE_LAUNCH_CHECK("species_embed_grad_join");
   return MACE_OK;
 }
@@ -848,7 +855,7 @@ extern "C" int mace_rows_restore(int32_t dtype, const int8_t* q, const float* sc
   if (n == 0) return MACE_OK;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int nb = (C + MACE_CHECKPOINT_BLOCK - 1) / MACE_CHECKPOINT_BLOCK;
-  const int64_t total = n * d * C, per = RW_THREADS * RW_UNROLL * 4;
+  const int64_t total = n * d * C, per = RW_THREADS * RS_UNROLL * 4;
   if ((total + per - 1) / per > INT32_MAX) return fail(MACE_ERR_BAD_ARG, "mace_rows_restore: too many rows");
   const unsigned grid = (unsigned)((total + per - 1) / per);
   const int vec = reinterpret_cast<uintptr_t>(q) % 4 == 0 && aligned16(x);

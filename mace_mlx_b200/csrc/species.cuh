@@ -66,12 +66,67 @@ __device__ __forceinline__ void store4(bf16* dst, const float* v) {
   *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t);
 }
 
-// 8-bit value of x at scale s = max |x| / 127 (0 where s is 0, infinite or NaN);
-// the clamp only acts where s is subnormal and the quotient may pass 127
-__device__ __forceinline__ int8_t quantise8(float x, float s) {
+// V channels as loaded: one 16-byte piece where they fill it, else single values
+template <typename T, int V>
+struct Raw {
+  static constexpr bool PIECE = V * sizeof(T) == 16;
+  uint4 piece;
+  T one[PIECE ? 1 : V];
+  __device__ __forceinline__ void zero() {
+    if constexpr (PIECE)
+      piece = make_uint4(0, 0, 0, 0);
+    else
+      for (int k = 0; k < V; ++k) one[k] = from_f32<T>(0.f);
+  }
+  __device__ __forceinline__ void load(const T* __restrict__ src) {
+    if constexpr (PIECE)
+      piece = __ldg(reinterpret_cast<const uint4*>(src));
+    else
+      for (int k = 0; k < V; ++k) one[k] = src[k];
+  }
+  __device__ __forceinline__ void add_to(float* acc) const {
+    if constexpr (!PIECE) {
+      for (int k = 0; k < V; ++k) acc[k] += to_f32(one[k]);
+    } else {
+      const uint32_t w[4] = {piece.x, piece.y, piece.z, piece.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) {
+          acc[k] += __uint_as_float(w[k]);
+        } else {
+          acc[2 * k] += __uint_as_float(w[k] << 16);
+          acc[2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+        }
+      }
+    }
+  }
+};
+
+// 8-bit value of x at scale s = max |x| / 127 (0 where s is 0, infinite or NaN): the IEEE quotient rounded to
+// the nearest, half to even; the clamp only acts where s is subnormal and the quotient may pass 127
+__device__ __forceinline__ int quantise8(float x, float s) {
   if (!(s > 0.f) || s > 3.4028234e38f) return 0;
-  const float r = rintf(__fdiv_rn(x, s));
-  return (int8_t)fminf(fmaxf(r, -127.f), 127.f);
+  return (int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f);
+}
+
+// Four of them, one per byte.  x * (1 / s) is within 2^-15 of the quotient (|quotient| <= 127, two roundings and one
+// of 1 / s), so it rounds to the same number unless it lies within 2^-14 of a tie; only then are the four divided.
+// Adding 1.5 2^23 rounds to a whole number, half to even, and leaves it in the low bits.
+__device__ __forceinline__ uint32_t quantise8x4(const float* x, float s) {
+  const float inv = __frcp_rn(s);
+  uint32_t w[4];
+  bool tie = !(s > 1e-30f && s < 1e30f);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float r = x[k] * inv, t = r + 12582912.f;
+    w[k] = __float_as_uint(t);
+    tie |= fabsf(r - (t - 12582912.f)) > 0.5f - 6.2e-5f;
+  }
+  if (tie) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (uint32_t)quantise8(x[k], s);
+  }
+  return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
 }
 
 // rows [lo, hi) of `order` that belong to group g, kept inside [0, n] whatever offsets holds

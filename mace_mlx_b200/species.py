@@ -30,6 +30,7 @@ Reference: node embedding ``mace_mlx/model.py:373-438``, skip tensor product
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple
 
 import torch
@@ -63,38 +64,47 @@ class RowCheckpoint(NamedTuple):
 
 
 # ---------------------------------------------------------------- checks
-def _cuda(name: str, t: torch.Tensor) -> torch.Tensor:
+# These run before every call and small calls are bound by them: device
+# indices and raw streams, which cost a tenth of device and stream objects.
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _cuda(name: str, t: torch.Tensor) -> int:
+    """Device index of a CUDA tensor."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path), got device {t.device}")
-    return t
+    return t.get_device()
 
 
-def _index(name: str, t: torch.Tensor) -> torch.Tensor:
-    _cuda(name, t)
+def _on(name: str, t: torch.Tensor, dev: int) -> None:
+    if _cuda(name, t) != dev:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
+
+
+def _index(name: str, t: torch.Tensor) -> int:
+    dev = _cuda(name, t)
     if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D int32 tensor, got {t.dtype} {tuple(t.shape)}")
-    return t
+    return dev
 
 
-def _dtype(name: str, t: torch.Tensor) -> int:
-    code = _DTYPES.get(t.dtype)
+def _dtype(name: str, dtype: torch.dtype) -> int:
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise ValueError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+        raise ValueError(f"{name} must be float32 or bfloat16, got {dtype}")
     return code
 
 
-def _same(name: str, t: torch.Tensor, other: torch.Tensor, dtype: bool = True) -> None:
-    if t.device != other.device:
-        raise ValueError(f"{name} is on {t.device}, expected {other.device}")
-    if dtype and t.dtype != other.dtype:
+def _same_dtype(name: str, t: torch.Tensor, other: torch.Tensor) -> None:
+    if t.dtype != other.dtype:
         raise ValueError(f"{name} is {t.dtype}, expected {other.dtype}")
 
 
 def _rows(name: str, t: torch.Tensor) -> tuple[int, int, int, int, int]:
     """(N, d, C, node stride, component stride) of (N, d, C) or (N, C) feature rows."""
-    _cuda(name, t)
     shape = t.shape
     if len(shape) == 3:
         n, d, c = shape
@@ -114,39 +124,33 @@ def _rows(name: str, t: torch.Tensor) -> tuple[int, int, int, int, int]:
     return n, d, c, sn, sm
 
 
-def _groups(groups: SpeciesGroups, n: int, like: torch.Tensor) -> int:
-    """Checks a grouping of n rows and returns its number of groups."""
+def _groups(groups: SpeciesGroups, n: int, dev: int) -> tuple[int, int, int]:
+    """(number of groups, pointers of order and offsets) of a grouping of n rows."""
     order, offsets = groups
-    _index("groups.order", order)
-    _index("groups.offsets", offsets)
-    _same("groups.order", order, like, False)
-    _same("groups.offsets", offsets, like, False)
+    if _index("groups.order", order) != dev or _index("groups.offsets", offsets) != dev:
+        raise ValueError(f"the grouping is on {order.device} and {offsets.device}, expected cuda:{dev}")
     if order.shape[0] != n:
         raise ValueError(f"groups.order lists {order.shape[0]} rows, expected {n}")
-    if offsets.shape[0] < 2:
+    g = offsets.shape[0] - 1
+    if g < 1:
         raise ValueError("groups.offsets needs num_elements + 1 entries")
-    return offsets.shape[0] - 1
+    return g, order.data_ptr(), offsets.data_ptr()
 
 
-def _weight(weight: torch.Tensor, num_groups: int) -> tuple[int, int]:
-    _cuda("weight", weight)
-    if weight.dim() != 3 or not weight.is_contiguous():
-        raise ValueError(f"weight must be a contiguous (num_elements, K, M) tensor, got {tuple(weight.shape)} "
-                         f"with strides {weight.stride()}")
-    if weight.shape[0] != num_groups:
-        raise ValueError(f"weight has {weight.shape[0]} elements, the grouping {num_groups}")
+def _map_limits(n: int, d: int, num_groups: int) -> None:
     if num_groups > MAX_GROUPS:
         raise ValueError(f"species_linear takes at most {MAX_GROUPS} elements, got {num_groups}")
-    return weight.shape[1], weight.shape[2]
+    if n * d > nv.SPECIES_MAX_ROWS:
+        raise ValueError(f"species_linear takes at most {nv.SPECIES_MAX_ROWS} rows, got {n} x {d}")
 
 
-def _out(out: torch.Tensor | None, shape: tuple[int, ...], like: torch.Tensor) -> torch.Tensor:
+def _out(out: torch.Tensor | None, shape, like: torch.Tensor, dev: int) -> torch.Tensor:
     """The result tensor: a new one, or ``out`` (a view into a wider table is fine)."""
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    _cuda("out", out)
-    _same("out", out, like)
-    if tuple(out.shape) != tuple(shape):
+        return like.new_empty(shape)
+    _on("out", out, dev)
+    _same_dtype("out", out, like)
+    if out.shape != shape:
         raise ValueError(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
     n, d, c, sn, sm = _rows("out", out)
     apart = d == 1 or sm >= c
@@ -157,29 +161,32 @@ def _out(out: torch.Tensor | None, shape: tuple[int, ...], like: torch.Tensor) -
     return out
 
 
-class _on:
-    """The device of a call: makes it current if it is not, and gives its stream."""
-
-    __slots__ = ("guard", "index")
-
-    def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
-        self.guard = None if self.index == torch.cuda.current_device() else torch.cuda.device(self.index)
-
-    def __enter__(self) -> int:
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(dev: int, fn, *args) -> None:
+    """Calls a C entry on the current stream of device ``dev``."""
+    if _current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        nv.check(rc)
 
 
-def _workspace(size_fn, args: tuple, like: torch.Tensor) -> tuple[torch.Tensor, int]:
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(entry: str, dev: int, *sizes: int) -> int:
+    """Workspace of a C entry: it depends on the sizes and the device's SM count only."""
     need = C.c_int64()
-    nv.check(size_fn(*args, C.byref(need)))
-    return torch.empty(max(need.value, 16), dtype=torch.uint8, device=like.device), need.value
+    with torch.cuda.device(dev):
+        nv.check(getattr(nv.load_library(), entry)(*sizes, C.byref(need)))
+    return need.value
+
+
+def _workspace(entry: str, dev: int, like: torch.Tensor, *sizes: int) -> tuple[torch.Tensor | None, int | None, int]:
+    nbytes = _workspace_bytes(entry, dev, *sizes)
+    if nbytes == 0:
+        return None, None, 0
+    ws = like.new_empty(nbytes, dtype=torch.uint8)
+    return ws, ws.data_ptr(), nbytes
 
 
 # ------------------------------------------------------------- operators
@@ -188,34 +195,30 @@ def group_species(species: torch.Tensor, num_elements: int) -> SpeciesGroups:
 
     Pairs are grouped the same way: ``species[sender] * E + species[receiver]``.
     """
-    _index("species", species)
+    dev = _index("species", species)
     if not 1 <= num_elements <= MAX_INDEX:
         raise ValueError(f"num_elements must be 1..{MAX_INDEX}, got {num_elements}")
     n = species.shape[0]
-    lib = nv.load_library()
-    order = torch.empty(n, dtype=torch.int32, device=species.device)
-    offsets = torch.empty(num_elements + 1, dtype=torch.int32, device=species.device)
-    with _on(species) as stream:
-        ws, nbytes = _workspace(lib.mace_species_group_workspace, (n, num_elements), species)
-        nv.check(lib.mace_species_group(species.data_ptr(), n, num_elements, order.data_ptr(), offsets.data_ptr(),
-                                        ws.data_ptr(), nbytes, stream))
+    order = torch.empty_like(species)
+    offsets = species.new_empty(num_elements + 1)
+    ws, ptr, nbytes = _workspace("mace_species_group_workspace", dev, species, n, num_elements)
+    _launch(dev, nv.load_library().mace_species_group, species.data_ptr(), n, num_elements, order.data_ptr(),
+            offsets.data_ptr(), ptr, nbytes)
     return SpeciesGroups(order, offsets)
 
 
 def _embedding(table, species, scale, out):
-    _cuda("table", table)
-    _index("species", species)
-    _same("species", species, table, False)
-    code = _dtype("table", table)
+    dev = _cuda("table", table)
+    if _index("species", species) != dev:
+        raise ValueError(f"species is on {species.device}, expected cuda:{dev}")
+    code = _dtype("table", table.dtype)
     g, _, c, ts, _ = _rows("table", table)
     if table.dim() != 2 or not 1 <= g <= MAX_INDEX:
         raise ValueError(f"table must be (num_elements, C) with 1..{MAX_INDEX} rows, got {tuple(table.shape)}")
     n = species.shape[0]
-    out = _out(out, (n, c), table)
-    with _on(table) as stream:
-        lib = nv.load_library()
-        nv.check(lib.mace_species_embed(code, table.data_ptr(), ts, g, c, species.data_ptr(), n, scale,
-                                        out.data_ptr(), max(out.stride(0), c), stream))
+    out = _out(out, (n, c), table, dev)
+    _launch(dev, nv.load_library().mace_species_embed, code, table.data_ptr(), ts, g, c, species.data_ptr(), n, scale,
+            out.data_ptr(), max(out.stride(0), c))
     return out
 
 
@@ -226,7 +229,7 @@ def species_embedding(table: torch.Tensor, species: torch.Tensor, *, scale: floa
     When ``table`` requires a gradient, its backward sums over ``groups``
     (made from ``species`` when not given).
     """
-    if table.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and table.requires_grad:
         if out is not None:
             raise ValueError("out= cannot take part in autograd")
         return _EmbeddingFn.apply(table, species, scale, groups)
@@ -235,38 +238,46 @@ def species_embedding(table: torch.Tensor, species: torch.Tensor, *, scale: floa
 
 def species_embedding_grad(grad: torch.Tensor, groups: SpeciesGroups, *, scale: float = 1.0) -> torch.Tensor:
     """Table gradient ``scale * sum of grad over each group`` (num_elements, C)."""
-    code = _dtype("grad", grad)
+    dev = _cuda("grad", grad)
+    code = _dtype("grad", grad.dtype)
     n, _, c, gs, _ = _rows("grad", grad)
     if grad.dim() != 2:
         raise ValueError(f"grad must be (N, C), got {tuple(grad.shape)}")
-    g = _groups(groups, n, grad)
-    lib = nv.load_library()
-    out = torch.empty((g, c), dtype=grad.dtype, device=grad.device)
-    with _on(grad) as stream:
-        ws, nbytes = _workspace(lib.mace_species_embed_grad_workspace, (n, g, c), grad)
-        nv.check(lib.mace_species_embed_grad(code, grad.data_ptr(), gs, groups.order.data_ptr(),
-                                             groups.offsets.data_ptr(), n, g, c, scale, out.data_ptr(),
-                                             ws.data_ptr(), nbytes, stream))
+    g, order, offsets = _groups(groups, n, dev)
+    out = grad.new_empty((g, c))
+    ws, ptr, nbytes = _workspace("mace_species_embed_grad_workspace", dev, grad, n, g, c)
+    _launch(dev, nv.load_library().mace_species_embed_grad, code, grad.data_ptr(), gs, order, offsets, n, g, c, scale,
+            out.data_ptr(), ptr, nbytes)
     return out
 
 
 def _linear(x, weight, groups, alpha, transpose, out):
-    code = _dtype("x", x)
+    dev = _cuda("x", x)
+    code = _dtype("x", x.dtype)
     n, d, k, sn, sm = _rows("x", x)
-    g = _groups(groups, n, x)
-    k_in, k_out = _weight(weight, g)
-    _same("weight", weight, x)
+    g, order, offsets = _groups(groups, n, dev)
+    _on("weight", weight, dev)
+    if weight.dim() != 3 or not weight.is_contiguous():
+        raise ValueError(f"weight must be a contiguous (num_elements, K, M) tensor, got {tuple(weight.shape)} "
+                         f"with strides {weight.stride()}")
+    wg, k_in, k_out = weight.shape
+    if wg != g:
+        raise ValueError(f"weight has {wg} elements, the grouping {g}")
+    _map_limits(n, d, g)
+    _same_dtype("weight", weight, x)
     if transpose:
         k_in, k_out = k_out, k_in
     if k != k_in:
         raise ValueError(f"x has {k} channels, the weight takes {k_in}")
-    y = _out(out, x.shape[:-1] + (k_out,), x)
-    ys = y.stride()
-    with _on(x) as stream:
-        lib = nv.load_library()
-        nv.check(lib.mace_species_linear(code, x.data_ptr(), sn, sm, weight.data_ptr(), int(transpose), g, k_in, k_out,
-                                         groups.order.data_ptr(), groups.offsets.data_ptr(), n, d, alpha,
-                                         y.data_ptr(), ys[0], ys[1] if len(ys) == 3 else k_out, stream))
+    shape = (n, d, k_out) if x.dim() == 3 else (n, k_out)
+    if out is None:
+        y = x.new_empty(shape)
+        yn, ym = d * k_out, k_out
+    else:
+        y = _out(out, shape, x, dev)
+        yn, ym = y.stride()[0], y.stride()[1] if d > 1 else k_out
+    _launch(dev, nv.load_library().mace_species_linear, code, x.data_ptr(), sn, sm, weight.data_ptr(), transpose, g,
+            k_in, k_out, order, offsets, n, d, alpha, y.data_ptr(), yn, ym)
     return y
 
 
@@ -281,6 +292,9 @@ def species_linear(x: torch.Tensor, weight: torch.Tensor, groups: SpeciesGroups,
     and so may ``out``, which must not overlap x.  In autograd,
     ``checkpoint`` keeps x for the weight gradient in 8 bits
     (``checkpoint_rows``) instead of x itself.
+
+    float32 products keep fp32 accuracy; an infinity in a float32 row or
+    matrix gives infinities or NaN in the results it enters.
     """
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         if out is not None or transpose:
@@ -292,29 +306,26 @@ def species_linear(x: torch.Tensor, weight: torch.Tensor, groups: SpeciesGroups,
 def species_linear_grad_weight(x: torch.Tensor | RowCheckpoint, grad: torch.Tensor, groups: SpeciesGroups, *,
                                alpha: float = 1.0) -> torch.Tensor:
     """Weight gradient (num_elements, K, M) from the rows x, or from their 8-bit checkpoint."""
-    code = _dtype("grad", grad)
+    dev = _cuda("grad", grad)
+    code = _dtype("grad", grad.dtype)
     n, d, m, gn, gm = _rows("grad", grad)
     scale = None
     if isinstance(x, RowCheckpoint):
         x, scale = _checkpoint(x)
-        _same("x.q", x, grad, False)
+        scale = scale.data_ptr()
+        _on("x.q", x, dev)
     else:
-        _dtype("x", x)
-        _same("x", x, grad)
+        _on("x", x, dev)
+        _same_dtype("x", x, grad)
     xn, xd, k, sn, sm = _rows("x", x)
-    if (xn, xd) != (n, d):
+    if xn != n or xd != d:
         raise ValueError(f"x rows {tuple(x.shape)} do not match grad rows {tuple(grad.shape)}")
-    g = _groups(groups, n, grad)
-    if g > MAX_GROUPS:
-        raise ValueError(f"species_linear takes at most {MAX_GROUPS} elements, got {g}")
-    lib = nv.load_library()
-    dw = torch.empty((g, k, m), dtype=grad.dtype, device=grad.device)
-    with _on(grad) as stream:
-        ws, nbytes = _workspace(lib.mace_species_linear_wgrad_workspace, (n, d, g, k, m), grad)
-        nv.check(lib.mace_species_linear_wgrad(
-            code, x.data_ptr(), sn, sm, None if scale is None else scale.data_ptr(), grad.data_ptr(), gn, gm, g, k, m,
-            groups.order.data_ptr(), groups.offsets.data_ptr(), n, d, alpha, dw.data_ptr(), ws.data_ptr(), nbytes,
-            stream))
+    g, order, offsets = _groups(groups, n, dev)
+    _map_limits(n, d, g)
+    dw = grad.new_empty((g, k, m))
+    ws, ptr, nbytes = _workspace("mace_species_linear_wgrad_workspace", dev, grad, n, d, g, k, m)
+    _launch(dev, nv.load_library().mace_species_linear_wgrad, code, x.data_ptr(), sn, sm, scale, grad.data_ptr(), gn,
+            gm, g, k, m, order, offsets, n, d, alpha, dw.data_ptr(), ptr, nbytes)
     return dw
 
 
@@ -327,14 +338,13 @@ def species_linear_grad(x: torch.Tensor | RowCheckpoint, grad: torch.Tensor, wei
 
 def _checkpoint(ck: RowCheckpoint) -> tuple[torch.Tensor, torch.Tensor]:
     q, scale = ck
-    _cuda("q", q)
-    _cuda("scale", scale)
+    dev = _cuda("q", q)
+    _on("scale", scale, dev)
     if q.dtype != torch.int8 or not q.is_contiguous() or q.dim() not in (2, 3):
         raise ValueError(f"q must be contiguous int8 (N, d, C) or (N, C), got {q.dtype} {tuple(q.shape)}")
-    want = tuple(q.shape[:-1]) + (-(-q.shape[-1] // CHECKPOINT_BLOCK),)
-    if scale.dtype != torch.float32 or not scale.is_contiguous() or tuple(scale.shape) != want:
+    want = (*q.shape[:-1], -(-q.shape[-1] // CHECKPOINT_BLOCK))
+    if scale.dtype != torch.float32 or not scale.is_contiguous() or scale.shape != want:
         raise ValueError(f"scale must be contiguous float32 {want}, got {scale.dtype} {tuple(scale.shape)}")
-    _same("scale", scale, q, False)
     return q, scale
 
 
@@ -345,28 +355,24 @@ def checkpoint_rows(x: torch.Tensor) -> RowCheckpoint:
     The error of a value is at most half a scale.  A block that holds an
     infinity or NaN is restored as NaN.
     """
-    code = _dtype("x", x)
+    dev = _cuda("x", x)
+    code = _dtype("x", x.dtype)
     n, d, c, sn, sm = _rows("x", x)
-    lib = nv.load_library()
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1] + (-(-c // CHECKPOINT_BLOCK),), dtype=torch.float32, device=x.device)
-    with _on(x) as stream:
-        nv.check(lib.mace_rows_checkpoint(code, x.data_ptr(), sn, sm, n, d, c, q.data_ptr(), scale.data_ptr(),
-                                          stream))
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty((*x.shape[:-1], -(-c // CHECKPOINT_BLOCK)), dtype=torch.float32)
+    _launch(dev, nv.load_library().mace_rows_checkpoint, code, x.data_ptr(), sn, sm, n, d, c, q.data_ptr(),
+            scale.data_ptr())
     return RowCheckpoint(q, scale)
 
 
 def restore_rows(checkpoint: RowCheckpoint, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values ``q * scale`` an 8-bit checkpoint stands for, rounded to ``dtype``."""
     q, scale = _checkpoint(checkpoint)
-    code = _DTYPES.get(dtype)
-    if code is None:
-        raise ValueError(f"dtype must be float32 or bfloat16, got {dtype}")
+    code = _dtype("dtype", dtype)
     n, d, c, _, _ = _rows("q", q)
-    x = torch.empty(q.shape, dtype=dtype, device=q.device)
-    with _on(q) as stream:
-        lib = nv.load_library()
-        nv.check(lib.mace_rows_restore(code, q.data_ptr(), scale.data_ptr(), n, d, c, x.data_ptr(), stream))
+    x = q.new_empty(q.shape, dtype=dtype)
+    _launch(q.get_device(), nv.load_library().mace_rows_restore, code, q.data_ptr(), scale.data_ptr(), n, d, c,
+            x.data_ptr())
     return x
 
 

@@ -34,14 +34,15 @@ def test_c_entries_check_their_arguments():
     lib = nv.load_library()
     need = C.c_int64(-1)
     one = C.c_void_p(16)  # never dereferenced: every call below is refused on the host
-    assert lib.mace_species_group_workspace(1000, 89, C.byref(need)) == nv.MACE_OK and need.value > 0
+    assert lib.mace_species_group_workspace(1000, 89, C.byref(need)) == nv.MACE_OK and need.value == 0  # one CTA
+    assert lib.mace_species_group_workspace(100000, 89, C.byref(need)) == nv.MACE_OK and need.value > 0
     assert lib.mace_species_group_workspace(-1, 89, C.byref(need)) == nv.MACE_ERR_BAD_ARG
     assert lib.mace_species_group_workspace(1, 0, C.byref(need)) == nv.MACE_ERR_BAD_ARG
     assert lib.mace_species_group_workspace(1, nv.SPECIES_MAX_INDEX + 1, C.byref(need)) == nv.MACE_ERR_BAD_ARG
     assert lib.mace_species_group_workspace(2**31, 1, C.byref(need)) == nv.MACE_ERR_BAD_ARG
     assert lib.mace_species_group_workspace(1, 1, None) == nv.MACE_ERR_BAD_ARG
     assert lib.mace_species_group(one, 5, 2, one, None, one, 1 << 20, None) == nv.MACE_ERR_BAD_ARG
-    assert lib.mace_species_group(one, 5, 2, one, one, one, 3, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_species_group(one, 100000, 2, one, one, one, 3, None) == nv.MACE_ERR_BAD_ARG
     assert "workspace" in nv.last_error(lib)
     assert lib.mace_species_embed(2, one, 8, 1, 8, one, 1, 1.0, one, 8, None) == nv.MACE_ERR_BAD_ARG
     assert lib.mace_species_embed(0, one, 8, 1, 8, one, 1, 1.0, one, 7, None) == nv.MACE_ERR_BAD_ARG
