@@ -16,7 +16,7 @@ namespace {
 // row movers: threads of a CTA and vectors per thread (loads in flight)
 constexpr int RW_THREADS = 256;
 constexpr int RW_UNROLL = 4;
-constexpr int RS_UNROLL = 8;  // of the restore, whose loads are 4 bytes
+constexpr int RS_UNROLL = 4;  // of the restore
 
 // x / C for x < 2^32 / C by multiplication: the row of a CTA's local element
 // (x < RW_THREADS RW_UNROLL 8 + C and C <= 32768 stay below the limit)
@@ -60,6 +60,11 @@ struct GroupPass {
 
 __device__ __forceinline__ int digit_of(const GroupPass& p, int32_t z) {
   return (row_key(z, p.G) >> p.shift) & ((1 << p.bits) - 1);
+}
+
+// digit of what is a key already
+__device__ __forceinline__ int digit_of_key(const GroupPass& p, int32_t key) {
+  return (key >> p.shift) & ((1 << p.bits) - 1);
 }
 
 __global__ void __launch_bounds__(GR_THREADS) k_group_count(GroupPass p) {
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(GR_THREADS) k_group_scatter(GroupPass p) {
   }
 #pragma unroll
   for (int j = 0; j < SEG / 32; ++j)
-    if (i0 + j * 32 + lane < i1) atomicAdd(&mine[digit_of(p, z[j])], 1);
+    if (i0 + j * 32 + lane < i1) atomicAdd(&mine[digit_of_key(p, z[j])], 1);
   __syncthreads();
   // digits in runs of bins / GR_THREADS per thread: local starts and starts in the result
   const int per = (bins + GR_THREADS - 1) / GR_THREADS;
@@ -201,7 +206,7 @@ __global__ void __launch_bounds__(GR_THREADS) k_group_scatter(GroupPass p) {
   for (int j = 0; j < SEG / 32; ++j) {
     const int64_t i = i0 + j * 32 + lane;
     const bool in = i < i1;
-    const int at = place(mine, digit_of(p, z[j]), p.bits, in, lane);
+    const int at = place(mine, digit_of_key(p, z[j]), p.bits, in, lane);
     if (in) {
       sm.key[at] = z[j];
       sm.row[at] = p.row ? p.row[i] : (int32_t)i;
@@ -211,7 +216,7 @@ __global__ void __launch_bounds__(GR_THREADS) k_group_scatter(GroupPass p) {
   const int rows = (int)imin64(GR_TILE, p.n - (int64_t)blockIdx.x * GR_TILE);
   for (int i = tid; i < rows; i += GR_THREADS) {
     const int32_t key = sm.key[i];
-    const int dg = digit_of(p, key);
+    const int dg = digit_of_key(p, key);
     const int64_t at = gstart[dg] + (i - lstart[dg]);
     p.row_out[at] = sm.row[i];
     if (p.key_out) p.key_out[at] = key;
@@ -425,10 +430,11 @@ __global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p, int per_c
     *s1 = (r.hi - 1) / p.share;
     return true;
   };
+  // sum of a group's partial rows from, from + step, ...: this lane's channel
   auto partial = [&](int g, int64_t from, int64_t s0, int64_t s1, int step) -> float {
     float acc = 0.f;
     if (c < p.C) {
-#pragma unroll 8
+#pragma unroll 4
       for (int64_t s = from; s <= s1; s += step) {
         // the group is the second of its first share's partial rows unless the share begins with it
         const int which = s > s0 || (int64_t)p.offsets[g] <= s * p.share ? 0 : 1;
@@ -455,7 +461,37 @@ __global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p, int per_c
     for (uint32_t left = many; left; left &= left - 1) {
       const int h = g0 + __ffs(left) - 1;
       span(h, &s0, &s1);
-      sums[warp][cl] = partial(h, s0 + warp, s0, s1, 32);
+      if (p.C % 4 == 0) {
+        // four rows of 32 channels at once, 16 bytes per lane
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int quad = blockIdx.y * 32 + (cl & 7) * 4;
+        if (quad < p.C) {
+#pragma unroll 4
+          for (int64_t s = s0 + warp * 4 + (cl >> 3); s <= s1; s += 128) {
+            const int which = s > s0 || (int64_t)p.offsets[h] <= s * p.share ? 0 : 1;
+            const float4 v = *reinterpret_cast<const float4*>(p.part + (s * 2 + which) * p.C + quad);
+            acc.x += v.x;
+            acc.y += v.y;
+            acc.z += v.z;
+            acc.w += v.w;
+          }
+        }
+#pragma unroll
+        for (int o = 8; o < 32; o <<= 1) {
+          acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o);
+          acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+          acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o);
+          acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+        }
+        if (cl < 8) {
+          sums[warp][cl * 4] = acc.x;
+          sums[warp][cl * 4 + 1] = acc.y;
+          sums[warp][cl * 4 + 2] = acc.z;
+          sums[warp][cl * 4 + 3] = acc.w;
+        }
+      } else {
+        sums[warp][cl] = partial(h, s0 + warp, s0, s1, 32);
+      }
       __syncthreads();
       if (warp == 0 && c < p.C) {
         float t = 0.f;
@@ -481,39 +517,41 @@ __global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* __restrict__
   const int64_t items = rows * nb;
   const int64_t i0 = (blockIdx.x * (int64_t)(RW_THREADS / 32) + (threadIdx.x >> 5)) * CK_ROWS;
   if (i0 >= items) return;
-  // node, component and block of the first item; the others follow by counting
-  int64_t r = nb == 1 ? i0 : i0 / nb;
-  int b = (int)(i0 - r * nb);
-  int64_t node = d == 1 ? r : r / d;
-  int m = (int)(r - node * d);
-  const int64_t row0 = r;
-  const int b0 = b;
+  const int here = (int)imin64(CK_ROWS, items - i0);
+  // row, node and component of the first item; the others follow by counting
+  const int64_t r0 = nb == 1 ? i0 : i0 / nb;
+  const int b0 = (int)(i0 - r0 * nb);
+  const int64_t node = d == 1 ? r0 : r0 / d;
+  const int m0 = (int)(r0 - node * d);
+  const int mine_c = VEC ? 4 * lane : lane;  // this lane's first channel of a block
   float v[CK_ROWS][4];
+  {
+    const T* src = x + node * xn + m0 * xm + mine_c;
+    const int64_t wrap = xn - (d - 1) * xm;
+    int b = b0, m = m0;
 #pragma unroll
-  for (int u = 0; u < CK_ROWS; ++u) {
-    const int c0 = b * MACE_CHECKPOINT_BLOCK + (VEC ? 4 * lane : lane);
-    const bool in = i0 + u < items;
-    const T* src = x + node * xn + m * xm;
-    if constexpr (VEC) {
-      if (in && c0 < C) {
-        load4(src + c0, v[u]);
-      } else {
+    for (int u = 0; u < CK_ROWS; ++u) {
+      const int c = b * MACE_CHECKPOINT_BLOCK;
+      if constexpr (VEC) {
         v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.f;
-      }
-    } else {
+        if (u < here && c + mine_c < C) load4(src + c, v[u]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[u][j] = in && c0 + 32 * j < C ? to_f32(src[c0 + 32 * j]) : 0.f;
-    }
-    if (++b == nb) {
-      b = 0;
-      if (++m == d) {
-        m = 0;
-        ++node;
+        for (int j = 0; j < 4; ++j) v[u][j] = u < here && c + mine_c + 32 * j < C ? to_f32(src[c + 32 * j]) : 0.f;
+      }
+      if (++b == nb) {
+        b = 0;
+        if (++m == d) {
+          m = 0;
+          src += wrap;
+        } else {
+          src += xm;
+        }
       }
     }
   }
-  r = row0;
-  b = b0;
+  int8_t* dst = q + r0 * C + mine_c;
+  int b = b0;
   float mine = 0.f;  // lane u's scale
 #pragma unroll
   for (int u = 0; u < CK_ROWS; ++u) {
@@ -525,20 +563,17 @@ __global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* __restrict__
     const float s = __fmul_rn(__int_as_float(top), 1.0f / 127.0f);
     if (lane == u) mine = s;
     const uint32_t packed = quantise8x4(v[u], s);
-    const int c0 = b * MACE_CHECKPOINT_BLOCK + (VEC ? 4 * lane : lane);
-    if (i0 + u < items) {
-      int8_t* dst = q + r * C + c0;
-      if constexpr (VEC) {
-        if (c0 < C) *reinterpret_cast<uint32_t*>(dst) = packed;
-      } else {
+    const int c = b * MACE_CHECKPOINT_BLOCK;
+    if constexpr (VEC) {
+      if (u < here && c + mine_c < C) *reinterpret_cast<uint32_t*>(dst + c) = packed;
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c0 + 32 * j < C) dst[32 * j] = (int8_t)(packed >> (8 * j));
-      }
+      for (int j = 0; j < 4; ++j)
+        if (u < here && c + mine_c + 32 * j < C) dst[c + 32 * j] = (int8_t)(packed >> (8 * j));
     }
     if (++b == nb) {
       b = 0;
-      ++r;
+      dst += C;
     }
   }
   if (lane < CK_ROWS && i0 + lane < items) scale[i0 + lane] = mine;
@@ -552,40 +587,42 @@ __global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* __restrict
   const int64_t e0 = blockIdx.x * (int64_t)(RW_THREADS * RS_UNROLL * 4);
   const int64_t row0 = e0 / C;
   const uint32_t first = (uint32_t)(e0 - row0 * C);
-  char4 w[RS_UNROLL];
+  uint32_t w[RS_UNROLL];
+  float sc[RS_UNROLL];  // scale of the vector's first element
 #pragma unroll
   for (int j = 0; j < RS_UNROLL; ++j) {
     const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
+    const uint32_t local = first + (threadIdx.x + j * RW_THREADS) * 4;
+    const uint32_t r = div.quotient(local), c = local - r * C;
+    w[j] = 0;
+    sc[j] = 0.f;
+    if (at < total) sc[j] = scale[(row0 + r) * nb + c / MACE_CHECKPOINT_BLOCK];
     if (vec && at + 4 <= total) {
-      w[j] = *reinterpret_cast<const char4*>(q + at);
+      w[j] = *reinterpret_cast<const uint32_t*>(q + at);
     } else {
-      w[j].x = at < total ? q[at] : 0;
-      w[j].y = at + 1 < total ? q[at + 1] : 0;
-      w[j].z = at + 2 < total ? q[at + 2] : 0;
-      w[j].w = at + 3 < total ? q[at + 3] : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (at + k < total) w[j] |= (uint32_t)(uint8_t)q[at + k] << (8 * k);
     }
   }
 #pragma unroll
   for (int j = 0; j < RS_UNROLL; ++j) {
     const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
-    if (at >= total) break;
-    const uint32_t local = first + (threadIdx.x + j * RW_THREADS) * 4;
-    const uint32_t r = div.quotient(local), c = local - r * C;
-    const float* sc = scale + (row0 + r) * nb;
-    const float qv[4] = {(float)w[j].x, (float)w[j].y, (float)w[j].z, (float)w[j].w};
     float v[4];
-    if (c + 4 <= (uint32_t)C && c / MACE_CHECKPOINT_BLOCK == (c + 3) / MACE_CHECKPOINT_BLOCK) {
-      const float s = sc[c / MACE_CHECKPOINT_BLOCK];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = qv[k] * s;
+    for (int k = 0; k < 4; ++k) v[k] = (float)(int8_t)(w[j] >> (8 * k));
+    const uint32_t local = first + (threadIdx.x + j * RW_THREADS) * 4;
+    uint32_t r = div.quotient(local), c = local - r * C;
+    if (c + 4 <= (uint32_t)C && (C & 3) == 0) {  // (a block boundary is a multiple of 4)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] *= sc[j];
     } else {
-      uint32_t ck = c;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        v[k] = at + k < total ? qv[k] * sc[ck / MACE_CHECKPOINT_BLOCK] : 0.f;
-        if (++ck == (uint32_t)C) {
-          ck = 0;
-          sc += nb;
+        if (at + k < total) v[k] *= scale[(row0 + r) * nb + c / MACE_CHECKPOINT_BLOCK];
+        if (++c == (uint32_t)C) {
+          c = 0;
+          ++r;
         }
       }
     }

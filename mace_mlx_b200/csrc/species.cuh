@@ -109,11 +109,11 @@ __device__ __forceinline__ int quantise8(float x, float s) {
   return (int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f);
 }
 
-// Four of them, one per byte.  x * (1 / s) is within 2^-15 of the quotient (|quotient| <= 127, two roundings and one
-// of 1 / s), so it rounds to the same number unless it lies within 2^-14 of a tie; only then are the four divided.
+// Four of them, one per byte.  x times the hardware's 1 / s (2^-23 relative) is within 2^-15 of the quotient, which
+// is at most 127 in magnitude, so it rounds to the same number unless it lies within 2^-14 of a tie; only then are the four divided.
 // Adding 1.5 2^23 rounds to a whole number, half to even, and leaves it in the low bits.
 __device__ __forceinline__ uint32_t quantise8x4(const float* x, float s) {
-  const float inv = __frcp_rn(s);
+  const float inv = __fdividef(1.0f, s);
   uint32_t w[4];
   bool tie = !(s > 1e-30f && s < 1e30f);
 #pragma unroll

@@ -69,6 +69,7 @@ struct SlParams {
   int64_t out_sn, out_sm;  // map: elements
   int vst;              // map: rows of `out` are whole 16-byte pieces; weight gradient: bytes of a vector store (32, 16, 0)
   float* part;          // weight gradient: partial tiles
+  int* units;           // weight gradient: first unit of each group, written by CTA 0 for the join (G + 1)
   const int32_t* order;
   const int32_t* offsets;
   int64_t n;
@@ -336,11 +337,6 @@ struct Sl {
   static constexpr int BYTES = OFF_BAR + NBAR * 8 + 32;
   static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
-
-__device__ __forceinline__ int64_t group_units(const SlParams& p, int g, int unit_rows) {
-  const Range r = group_range(p.offsets, g, p.n);
-  return ((r.hi - r.lo) * p.d + unit_rows - 1) / unit_rows;
-}
 
 // The groups in shared memory: units of group g are [pre[g], pre[g + 1]), its rows [lo[g], hi[g]) of `order`.
 struct Groups {
@@ -709,6 +705,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   tc::fence_before_sync();
   load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, q, reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
+  if (WG && blockIdx.x == 0)
+    for (int i = tid; i <= p.G; i += SL_THREADS) p.units[i] = pre[i];
   // this CTA's share of the units; weight gradient: blockIdx.x = share * tiles + tile
   const int total = pre[p.G];
   const int tiles = WG ? p.n_ct * p.n_kt : 1;
@@ -1201,35 +1199,9 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
 // 8 rows x 8 column quads (one per lane of 64) of tile blockIdx.z, four threads of each taking every fourth share.
 template <typename T>
 __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constant__ SlParams p) {
-  __shared__ int64_t sum[2][8];
   __shared__ float4 part[4][64];
   const int g = blockIdx.x, tid = threadIdx.x;
-  int64_t before = 0, all = 0;
-  for (int i = tid; i < p.G; i += 256) {
-    const int64_t c = group_units(p, i, SL_KC);
-    all += c;
-    if (i < g) before += c;
-  }
-  const int64_t mine = group_units(p, g, SL_KC);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  if ((tid & 31) == 0) {
-    sum[0][tid >> 5] = before;
-    sum[1][tid >> 5] = all;
-  }
-  __syncthreads();
-  before = all = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    before += sum[0][w];
-    all += sum[1][w];
-  }
-  // as in load_groups
-  before = min(before, (int64_t)INT32_MAX);
-  all = min(all, (int64_t)INT32_MAX);
+  const int64_t before = p.units[g], mine = p.units[g + 1] - before, all = p.units[p.G];
   const int tile = blockIdx.z;
   const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
   const int lane = tid & 63, sl = tid >> 6;
@@ -1329,6 +1301,10 @@ int launch_gemm(const SlParams& p, int grid, cudaStream_t s) {
   return MACE_OK;
 }
 
+int64_t partial_bytes(const SlParams& p, int G) {
+  return (int64_t)p.n_ct * p.n_kt * (p.shares + G) * 128 * p.NT * 4;
+}
+
 // shares (CTAs along the rows) and tiles of a weight gradient
 void wgrad_split(int64_t n, int32_t d, int32_t G, int32_t K, int32_t M, SlParams* p) {
   p->NT = tile_cols(M, 128);
@@ -1394,7 +1370,7 @@ extern "C" int mace_species_linear_wgrad_workspace(int64_t n, int32_t d, int32_t
     return fail(MACE_ERR_BAD_ARG, "mace_species_linear_wgrad_workspace: bad arguments");
   SlParams p{};
   wgrad_split(n, d, G, K, M, &p);
-  *bytes = (int64_t)p.n_ct * p.n_kt * (p.shares + G) * 128 * p.NT * 4;
+  *bytes = partial_bytes(p, G) + (int64_t)(G + 1) * 4;
   return MACE_OK;
 }
 
@@ -1428,21 +1404,24 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   p.N = M;
   p.alpha = alpha;
   wgrad_split(n, d, G, K, M, &p);
-  const int grid = p.shares * p.n_ct * p.n_kt;
-  int rc = MACE_OK;
-  if (n > 0) {
-    const bool vec = aligned_rows(p.a, n, d, xe) && aligned_rows(p.b, n, d, es);
-    auto go = [&](auto ta, auto t) {
-      using TA = decltype(ta);
-      using T = decltype(t);
-      return vec ? launch_gemm<TA, T, true, true>(p, grid, s) : launch_gemm<TA, T, true, false>(p, grid, s);
-    };
-    if (xs)
-      rc = dtype == MACE_F32 ? go(int8_t{}, float{}) : go(int8_t{}, bf16{});
-    else
-      rc = dtype == MACE_F32 ? go(float{}, float{}) : go(bf16{}, bf16{});
-    if (rc) return rc;
+  if (n == 0) {
+    MACE_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)G * K * M * es, s));
+    return MACE_OK;
   }
+  p.units = reinterpret_cast<int*>(static_cast<char*>(ws) + partial_bytes(p, G));
+  const int grid = p.shares * p.n_ct * p.n_kt;
+  const bool vec = aligned_rows(p.a, n, d, xe) && aligned_rows(p.b, n, d, es);
+  auto go = [&](auto ta, auto t) {
+    using TA = decltype(ta);
+    using T = decltype(t);
+    return vec ? launch_gemm<TA, T, true, true>(p, grid, s) : launch_gemm<TA, T, true, false>(p, grid, s);
+  };
+  int rc;
+  if (xs)
+    rc = dtype == MACE_F32 ? go(int8_t{}, float{}) : go(int8_t{}, bf16{});
+  else
+    rc = dtype == MACE_F32 ? go(float{}, float{}) : go(bf16{}, bf16{});
+  if (rc) return rc;
   const dim3 jg(G, 16 * (p.NT / 32), p.n_ct * p.n_kt);
   if (dtype == MACE_F32)
     k_species_wgrad_join<float><<<jg, 256, 0, s>>>(p);
