@@ -12,7 +12,8 @@
 // values are exact in one bf16 piece and their row scale is folded into dy.
 // The tensor core truncates when it accumulates, so an accumulator takes one
 // 64-wide step of K, smallest products first, and the epilogue warps add the
-// steps in fp32 registers.
+// steps in fp32 registers (bf16 alone, whose result is rounded to 2^-9, takes
+// several steps).
 //
 // Roles of a CTA (16 warps, one CTA per SM, a contiguous share of the tiles):
 //   warps 0-3   operand A: own 32 TMEM lanes each, fetch their rows with 16-byte
@@ -45,6 +46,7 @@ namespace {
 
 constexpr int SL_THREADS = 16 * 32;
 constexpr int SL_KC = 64;              // K of one accumulation step
+constexpr int SL_LONG = 8;             // weight gradient of bf16: steps accumulated in TMEM
 constexpr int SL_D = 0;                // TMEM columns: two accumulators of 128
 constexpr int SL_A = 256;              // then two A stages
 constexpr uint32_t SL_TMEM = 512;
@@ -317,6 +319,7 @@ template <typename TA, typename T, bool WG, bool VEC>
 struct Sl {
   static constexpr int PA = sizeof(TA) == 4 ? 3 : 1;
   static constexpr int PB = sizeof(TA) == 2 ? 1 : 3;
+  static constexpr bool LONG = PA == 1 && PB == 1;  // sums of several steps (the result is rounded to 2^-9)
   static constexpr int SEG_A = WG ? 32 * (int)sizeof(TA) : 128;  // bytes of a row in one ring unit of 32 rows
   static constexpr int SEG_B = 32 * (int)sizeof(T);
   static constexpr int PITCH_A = SEG_A + (VEC ? 0 : 16), PITCH_B = SEG_B + (VEC ? 0 : 16);
@@ -511,6 +514,93 @@ __device__ __forceinline__ void fetch_any(uint32_t dst, const char* data, const 
   }
 }
 
+// Map: 32 staged row segments of 128 bytes (piece j of row r at j ^ (r & 7)) to columns c0 .. c0 + left - 1 of the
+// rows at element offset o (< 0: none; o16: in 16 bytes for aligned rows), one row per lane.
+template <typename T>
+__device__ __forceinline__ void copy_out(const SlParams& p, uint32_t stage, int64_t o, uint32_t o16, int c0, int left) {
+  int row = threadIdx.x & 31;
+  asm volatile("" : "+r"(row));  // addresses are made here each time: held across the tiles they crowd the registers
+  __syncwarp();
+  if (p.vst) {
+    // 4 rows x 128 bytes per instruction
+    const int j = row & 7;
+    const bool have = left * (int)sizeof(T) > 16 * j;
+    char* const to = static_cast<char*>(p.out) + (int64_t)c0 * sizeof(T) + 16 * j;
+    const uint32_t src = stage + (row >> 3) * 128;
+#pragma unroll
+    for (int i0 = 0; i0 < 8; i0 += 4) {
+      uint4 v[4];
+      uint32_t ro[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // (r & 7 alternates between lane / 8 and lane / 8 + 4)
+        v[i] = lds128(src + (i0 + i) * 512 + ((j ^ ((row >> 3) + (i & 1) * 4)) << 4));
+        ro[i] = __shfl_sync(0xffffffffu, o16, (i0 + i) * 4 + (row >> 3));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (ro[i] != NO_ROW && have) *reinterpret_cast<uint4*>(to + (uint64_t)ro[i] * 16) = v[i];
+    }
+  } else {
+    // unaligned rows: element by element, neighbouring lanes on neighbouring columns
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r) {
+      const int64_t ro = __shfl_sync(0xffffffffu, o, r);
+#pragma unroll
+      for (int c = 0; c < 128 / (int)sizeof(T); c += 32) {
+        const int byte = (c + row) * (int)sizeof(T);
+        const T v = lds_raw(stage + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15)), T{});
+        if (ro >= 0 && c + row < left) (static_cast<T*>(p.out) + ro + c0)[c + row] = v;
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// Weight gradient: a lane's NT / 2 sums of row kl of a 128 x NT tile (columns c0 ..), done with group g: dW itself
+// where this share held the whole group, else a partial tile.  (share, group) pairs of one tile are a staircase:
+// share + g numbers them; a partial tile is stored as [column quad][row], so that a warp's 32 rows are one line per
+// instruction.
+template <typename T>
+__device__ __forceinline__ void finish_wgrad(const SlParams& p, float* acc, int g, bool whole, int tile, int share, int k0,
+                                             int n0, int kl, int c0) {
+  const int CW = p.NT / 2;
+  if (!whole) {
+    float4* dst = reinterpret_cast<float4*>(p.part) + ((int64_t)tile * (p.shares + p.G) + share + g) * 32 * p.NT +
+                  c0 / 4 * 128 + kl;
+#pragma unroll
+    for (int b = 0; b < 16; ++b)
+      if (b * 4 < CW) dst[b * 128] = make_float4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
+  } else if (k0 + kl < p.K) {
+    T* dst = static_cast<T*>(p.out) + ((int64_t)g * p.K + k0 + kl) * p.N + n0 + c0;
+    const int left = p.N - n0 - c0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      if (b * 16 >= CW) break;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) acc[b * 16 + k] *= p.alpha;
+      if (left - b * 16 > 0) store16<T>(dst + b * 16, acc + b * 16, left - b * 16, p.vst);
+    }
+  }
+}
+
+// Map: zeros in the rows outside every group, shared by warps 5 to 7 of every CTA.
+template <typename T>
+__device__ __forceinline__ void zero_rows(const SlParams& p) {
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - 5;
+  const int64_t b0 = min(max((int64_t)p.offsets[0], (int64_t)0), p.n);
+  const int64_t b1 = max(min(max((int64_t)p.offsets[p.G], (int64_t)0), p.n), b0);
+  const int64_t outside = (p.n - (b1 - b0)) * p.d;
+  T* out = static_cast<T*>(p.out);
+  for (int64_t r = blockIdx.x * (int64_t)3 + w; r < outside; r += (int64_t)gridDim.x * 3) {
+    int64_t i = r / p.d;
+    const int m = (int)(r - i * p.d);
+    if (i >= b0) i += b1 - b0;
+    const int64_t node = p.order[i];
+    if (node < 0 || node >= p.n) continue;
+    for (int c = lane; c < p.N; c += 32) out[node * p.out_sn + m * p.out_sm + c] = from_f32<T>(0.f);
+  }
+}
+
 // 16 bytes at byte offset s of the 32 bytes (a, b)
 __device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int s) {
   uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -663,23 +753,6 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     return;
   }
 
-  // map: zeros in the rows outside every group, shared by warps 5 to 7 of every CTA
-  auto zero_rows = [&]() {
-    constexpr int w0 = 5, nw = 3;
-    const int64_t b0 = min(max((int64_t)p.offsets[0], (int64_t)0), p.n);
-    const int64_t b1 = max(min(max((int64_t)p.offsets[p.G], (int64_t)0), p.n), b0);
-    const int64_t outside = (p.n - (b1 - b0)) * p.d;
-    T* out = static_cast<T*>(p.out);
-    for (int64_t r = blockIdx.x * (int64_t)nw + warp - w0; r < outside; r += (int64_t)gridDim.x * nw) {
-      int64_t i = r / p.d;
-      const int m = (int)(r - i * p.d);
-      if (i >= b0) i += b1 - b0;
-      const int64_t node = p.order[i];
-      if (node < 0 || node >= p.n) continue;
-      for (int c = lane; c < p.N; c += 32) out[node * p.out_sn + m * p.out_sm + c] = from_f32<T>(0.f);
-    }
-  };
-
   const int NT = p.NT;
   if (warp == 15) {  // while the others wait for the offsets
     if (lane == 0) {
@@ -716,7 +789,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   const int t0 = share < nshare ? (int)((int64_t)share * total / nshare) : 0;
   const int t1 = share < nshare ? (int)((int64_t)(share + 1) * total / nshare) : 0;
   if (t0 >= t1) {
-    if (!WG && warp >= 5 && warp < 8) zero_rows();
+    if (!WG && warp >= 5 && warp < 8) zero_rows<T>(p);
     if (warp == 15) tc::tmem_dealloc(SL_D, SL_TMEM);
     return;
   }
@@ -729,30 +802,33 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   // before, or -1 when its images were there already.  The queue of issued MMAs is a few hundred cycles deep, so the
   // path from one step's last to the next step's first is kept short: two waits, no warp-wide operation
   const uint32_t idesc = idesc_bf16(NT), bhi = (uint32_t)(tc::sw128_desc(base) >> 32);
-  auto issue = [&](int it, int bs, int use, bool release) -> bool {
+  // The accumulator takes the sn-th sum: one step, or for bf16 (S::LONG) a whole tile or SL_LONG steps, of which this
+  // is the first / last.
+  auto issue = [&](int it, int bs, int use, bool release, int sn, bool first, bool last) -> bool {
     using PR = Products<PA, PB>;
     const int s = it & 1;
     if (use >= 0 && !wait_phase(B_FULL(bs), use & 1, abort)) return false;
     if (!wait_phase(A_FULL(s), (it >> 1) & 1, abort)) return false;
-    if (it >= 2 && !wait_phase(D_FREE(s), ((it >> 1) - 1) & 1, abort)) return false;
+    if (first && sn >= 2 && !wait_phase(D_FREE(sn & 1), ((sn >> 1) - 1) & 1, abort)) return false;
     tc::fence_after_sync();
+    const uint32_t dcol = SL_D + (sn & 1) * 128;
     const uint32_t blo = (uint32_t)tc::sw128_desc(base + bs * (PB * SL_IMG));
-    // the stage as a constant: the only operand left to compute is the low half of B's descriptor
+    // (the stage as a constant: little is left to compute)
     auto emit = [&](auto stage) {
       constexpr uint32_t st = decltype(stage)::value;
 #pragma unroll
       for (int q = 0; q < PR::n; ++q)
 #pragma unroll
         for (int ks = 0; ks < SL_KC / 16; ++ks)
-          mma_bf16_ta(SL_D + st * 128, SL_A + st * (PA * 32) + PR::a(q) * 32 + ks * 8,
-                      blo + PR::b(q) * (SL_IMG / 16) + ks * 2, bhi, idesc, q > 0 || ks > 0);
+          mma_bf16_ta(dcol, SL_A + st * (PA * 32) + PR::a(q) * 32 + ks * 8, blo + PR::b(q) * (SL_IMG / 16) + ks * 2, bhi,
+                      idesc, !first || q > 0 || ks > 0);
     };
     if (s)
       emit(std::integral_constant<uint32_t, 1>{});
     else
       emit(std::integral_constant<uint32_t, 0>{});
     tc::mma_commit(A_FREE(s));
-    tc::mma_commit(D_FULL(s));
+    if (last) tc::mma_commit(D_FULL(sn & 1));
     if (release) tc::mma_commit(B_FREE(bs));
     return true;
   };
@@ -922,7 +998,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         };
         Walk w;
         w.init(p, q, t0);
-        int it = 0, fills = 0;  // steps; image sets (resident) or images written
+        int it = 0, tile_no = 0, fills = 0;  // steps, tiles; image sets (resident) or images written
         while (w.t < t1 && ok) {
           const Tile t(p, q, w);
           if (resident) {
@@ -933,8 +1009,11 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
             if (!ok) break;
             if (warp == 4 && elect_one())
               for (int i = 0; i < run && ok; ++i)
-                for (int k = 0; k < n_k && ok; ++k) ok = issue(it + i * n_k + k, k, i == 0 ? fills : -1, i + 1 == run);
+                for (int k = 0; k < n_k && ok; ++k)
+                  ok = issue(it + i * n_k + k, k, i == 0 ? fills : -1, i + 1 == run,
+                             S::LONG ? tile_no + i : it + i * n_k + k, !S::LONG || k == 0, !S::LONG || k + 1 == n_k);
             it += run * n_k;
+            tile_no += run;
             ++fills;
             w.t += run - 1;
           } else {
@@ -942,9 +1021,11 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
               const int s = fills % S::NSLOT, use = fills / S::NSLOT;
               ok = use == 0 || wait_phase(B_FREE(s), (use - 1) & 1, abort);
               ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, k, 1, s);
-              if (ok && warp == 4 && elect_one()) ok = issue(it, s, use, true);
+              if (ok && warp == 4 && elect_one())
+                ok = issue(it, s, use, true, S::LONG ? tile_no : it, !S::LONG || k == 0, !S::LONG || k + 1 == n_k);
               ok = __all_sync(0xffffffffu, ok);
             }
+            ++tile_no;
           }
           ok = __all_sync(0xffffffffu, ok);
           w.next(q, t1);
@@ -952,7 +1033,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         if (warp == 4)
           drain();
         else
-          zero_rows();
+          zero_rows<T>(p);
       } else if (w4 * 32 < NT) {
         const int n = w4 * 32 + lane;
         const uint32_t ring = base + S::OFF_B + w4 * S::NU_B * S::UNIT_B;
@@ -1038,16 +1119,27 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     bool fresh = true;  // acc holds nothing yet
     RowRef ref{-1, -1};  // map: this lane's row of the tile, loaded while the tile is computed
     int ct = 0, k = 0;   // map: the tile's column tile, the step
-    // weight gradient: warp 8 issues the next step's MMAs before it takes this step's result
-    auto issue_wg = [&](int it) {
-      if (WG && warp == 8 && it < t1 - t0) {
-        if (elect_one()) ok = issue(it, it & 1, it >> 1, true);
-        ok = __all_sync(0xffffffffu, ok);
-      }
+    // weight gradient: the steps of one sum, within a group; warp 8 issues the next sum's MMAs before it takes this one's
+    auto sum_steps = [&](const Walk& x) { return S::LONG ? min(min(SL_LONG, pre[x.g + 1] - x.t), t1 - x.t) : 1; };
+    auto advance = [&](Walk& x, int n) {
+      x.t += n - 1;
+      x.next(q, t1);
     };
-    issue_wg(0);
-    for (int it = 0; w.t < t1 && ok; ++it) {
-      const int s = it & 1;
+    Walk m = w;
+    int mi = 0, ms = 0;  // the issuing side: step, sum
+    auto issue_wg = [&]() {
+      if (!WG || warp != 8 || m.t >= t1) return;
+      const int n = sum_steps(m);
+      if (elect_one())
+        for (int i = 0; i < n && ok; ++i) ok = issue(mi + i, (mi + i) & 1, (mi + i) >> 1, true, ms, i == 0, i + 1 == n);
+      ok = __all_sync(0xffffffffu, ok);
+      mi += n;
+      ++ms;
+      advance(m, n);
+    };
+    issue_wg();
+    for (int sn = 0; w.t < t1 && ok; ++sn) {
+      const int s = sn & 1;
       if constexpr (!WG) {
         if (fresh) {
           const Tile t(p, q, w);
@@ -1055,9 +1147,9 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
           ct = t.ct;
         }
       }
-      issue_wg(it + 1);
+      issue_wg();
       if (!ok) break;
-      ok = wait_phase(D_FULL(s), (it >> 1) & 1, abort);
+      ok = wait_phase(D_FULL(s), (sn >> 1) & 1, abort);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc::fence_after_sync();
@@ -1080,7 +1172,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
       }
       fresh = false;
       if constexpr (!WG) {
-        if (++k < n_k) continue;
+        k += S::LONG ? n_k : 1;
+        if (k < n_k) continue;
         k = 0;
         const int c0 = ct * NT + half * CW;
         // Rows leave through shared memory, CB columns at a time: a thread holds one row, so stores straight from
@@ -1117,71 +1210,19 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
             sts128(stage + row * 128 + ((j ^ (row & 7)) << 4), w4[0], w4[1], w4[2], w4[3]);
           }
           __syncwarp();
-          if (p.vst) {
-            // 4 rows x 128 bytes per instruction
-            const int j = row & 7;
-            const bool have = left * (int)sizeof(T) > 16 * j;
-            char* const to = static_cast<char*>(p.out) + (c0 + b) * (int)sizeof(T) + 16 * j;
-            const uint32_t src = stage + (row >> 3) * 128;
-#pragma unroll
-            for (int i0 = 0; i0 < 8; i0 += 4) {
-              uint4 v[4];
-              uint32_t ro[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {  // (r & 7 alternates between lane / 8 and lane / 8 + 4)
-                v[i] = lds128(src + (i0 + i) * 512 + ((j ^ ((row >> 3) + (i & 1) * 4)) << 4));
-                ro[i] = __shfl_sync(0xffffffffu, o16, (i0 + i) * 4 + (row >> 3));
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (ro[i] != NO_ROW && have) *reinterpret_cast<uint4*>(to + (uint64_t)ro[i] * 16) = v[i];
-            }
-          } else {
-            // unaligned rows: element by element, neighbouring lanes on neighbouring columns
-#pragma unroll 4
-            for (int r = 0; r < 32; ++r) {
-              const int64_t ro = __shfl_sync(0xffffffffu, o, r);
-#pragma unroll
-              for (int c = 0; c < CB; c += 32) {
-                const int byte = (c + lane) * (int)sizeof(T);
-                const T v = lds_raw(stage + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15)), T{});
-                if (ro >= 0 && c + lane < left) (static_cast<T*>(p.out) + ro + c0 + b)[c + lane] = v;
-              }
-            }
-          }
+          copy_out<T>(p, stage, o, o16, c0 + b, left);
           __syncwarp();
         }
         fresh = true;
         w.next(q, t1);
       } else {
-        const bool group_ends = w.t + 1 == pre[w.g + 1];
-        if (group_ends || w.t + 1 == t1) {
-          const bool whole = group_ends && pre[w.g] >= t0;
-          const int kl = quad * 32 + lane, c0 = half * CW;
-          if (whole) {
-            if (wg_k0 + kl < p.K) {
-              T* dst = static_cast<T*>(p.out) + ((int64_t)w.g * p.K + wg_k0 + kl) * p.N + wg_n0 + c0;
-              const int left = p.N - wg_n0 - c0;
-#pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                if (b * 16 >= CW) break;
-#pragma unroll
-                for (int k = 0; k < 16; ++k) acc[b * 16 + k] *= p.alpha;
-                if (left - b * 16 > 0) store16<T>(dst + b * 16, acc + b * 16, left - b * 16, p.vst);
-              }
-            }
-          } else {
-            // (share, group) pairs of one tile are a staircase: share + g numbers them.  A partial tile is stored
-            // as [column quad][row]: a warp's 32 rows are one line per instruction
-            float4* dst = reinterpret_cast<float4*>(p.part) +
-                          ((int64_t)tile * (p.shares + p.G) + share + w.g) * 32 * NT + c0 / 4 * 128 + kl;
-#pragma unroll
-            for (int b = 0; b < 16; ++b)
-              if (b * 4 < CW) dst[b * 128] = make_float4(acc[4 * b], acc[4 * b + 1], acc[4 * b + 2], acc[4 * b + 3]);
-          }
+        const int len = sum_steps(w);
+        const bool group_ends = w.t + len == pre[w.g + 1];
+        if (group_ends || w.t + len == t1) {
+          finish_wgrad<T>(p, acc, w.g, group_ends && pre[w.g] >= t0, tile, share, wg_k0, wg_n0, quad * 32 + lane, half * CW);
           fresh = true;
         }
-        w.next(q, t1);
+        advance(w, len);
       }
     }
     if (WG && warp == 8) drain();
@@ -1194,6 +1235,16 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     tc::tmem_dealloc(tmem, SL_TMEM);
   }
 }
+
+}  // namespace
+
+}  // namespace mace
+
+#include "species_direct.cuh"
+
+namespace mace {
+
+namespace {
 
 // dW of the groups that several shares hold, in share order, and of empty groups (zero).  One CTA: group blockIdx.x,
 // 8 rows x 8 column quads (one per lane of 64) of tile blockIdx.z, four threads of each taking every fourth share.
@@ -1361,7 +1412,8 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   const bool vec = aligned_rows(p.a, n, d, es);
   if (dtype == MACE_F32)
     return vec ? launch_gemm<float, float, false, true>(p, grid, s) : launch_gemm<float, float, false, false>(p, grid, s);
-  return vec ? launch_gemm<bf16, bf16, false, true>(p, grid, s) : launch_gemm<bf16, bf16, false, false>(p, grid, s);
+  // bf16 in whole pieces: nothing to convert
+  return vec && p.w_vec ? launch_direct<false>(p, grid, s) : launch_gemm<bf16, bf16, false, false>(p, grid, s);
 }
 
 extern "C" int mace_species_linear_wgrad_workspace(int64_t n, int32_t d, int32_t G, int32_t K, int32_t M,
@@ -1419,8 +1471,10 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   int rc;
   if (xs)
     rc = dtype == MACE_F32 ? go(int8_t{}, float{}) : go(int8_t{}, bf16{});
-  else
-    rc = dtype == MACE_F32 ? go(float{}, float{}) : go(bf16{}, bf16{});
+  else if (dtype == MACE_F32)
+    rc = go(float{}, float{});
+  else  // bf16 in whole pieces: nothing to convert
+    rc = vec ? launch_direct<true>(p, grid, s) : launch_gemm<bf16, bf16, true, false>(p, grid, s);
   if (rc) return rc;
   const dim3 jg(G, 16 * (p.NT / 32), p.n_ct * p.n_kt);
   if (dtype == MACE_F32)
