@@ -5,6 +5,7 @@
 // What they restate (paths in the reference project):
 //   node embedding (one-hot linear)  mace_mlx/model.py:373-438
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "species.cuh"
@@ -34,12 +35,12 @@ RowDiv row_div(int C) { return {(uint32_t)((((uint64_t)1 << 32) + C - 1) / C), C
 // list order everywhere, so the order of atomics plays no part.
 constexpr int GR_THREADS = 256;
 constexpr int GR_WARPS = GR_THREADS / 32;
-constexpr int GR_TILE = 4096;      // rows of one CTA of a counting pass
+constexpr int GR_TILE = 2048;      // rows of one CTA of a counting pass (a pass is a chain of latencies: many small CTAs)
 constexpr int GR_MAX_BINS = 1024;  // digits of one pass
 // short lists: one CTA does the whole sort in one launch
 constexpr int GS_THREADS = 1024;
 constexpr int GS_MAX_ROWS = 8192;
-constexpr int GS_MAX_BINS = 256;
+constexpr int GS_MAX_BINS = 256;  // (shared memory of a static size)
 
 // key of a row: its species, or num_groups for padding rows
 __device__ __forceinline__ int row_key(int32_t z, int G) { return (z >= 0 && z < G) ? z : G; }
@@ -62,12 +63,8 @@ __device__ __forceinline__ int digit_of(const GroupPass& p, int32_t z) {
   return (row_key(z, p.G) >> p.shift) & ((1 << p.bits) - 1);
 }
 
-// digit of what is a key already
-__device__ __forceinline__ int digit_of_key(const GroupPass& p, int32_t key) {
-  return (key >> p.shift) & ((1 << p.bits) - 1);
-}
-
 __global__ void __launch_bounds__(GR_THREADS) k_group_count(GroupPass p) {
+  pdl_wait();
   __shared__ int hist[GR_MAX_BINS];
   const int bins = 1 << p.bits;
   for (int b = threadIdx.x; b < bins; b += GR_THREADS) hist[b] = 0;
@@ -84,6 +81,7 @@ __global__ void __launch_bounds__(GR_THREADS) k_group_count(GroupPass p) {
 
 // exclusive sums of one digit's counts over the CTAs, in place, and their total: a CTA per digit
 __global__ void __launch_bounds__(GR_THREADS) k_group_scan(GroupPass p) {
+  pdl_wait();
   __shared__ int sums[GR_WARPS];
   int32_t* c = p.counts + (int64_t)blockIdx.x * p.nb;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -130,22 +128,24 @@ __device__ __forceinline__ int cta_exclusive(int v, int* warp_sums) {
   return before + s - v;
 }
 
-// Position of this lane's row: `mine` holds the next position of each digit for this warp and is moved past the rows
-// placed here.  Lanes of equal digit find one another bit by bit with ballots (match_any on spread digits costs
-// several times as much: the pass over 4M rows took 56 us with it).
-__device__ __forceinline__ int place(int* mine, int digit, int bits, bool in, int lane) {
+// Place of this lane's row among its warp's rows of the same digit: `count` holds how many came before, and is moved
+// on.  Lanes of equal digit find one another bit by bit with ballots (match_any on spread digits costs several times
+// as much: a pass over 4M rows took 56 us with it).
+template <int BITS>
+__device__ __forceinline__ int place(int* count, int digit, bool in, int lane) {
   unsigned same = __ballot_sync(0xffffffffu, in);
-  for (int b = 0; b < bits; ++b) {
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
     const bool one = (digit >> b) & 1;
     const unsigned m = __ballot_sync(0xffffffffu, one);
     same &= one ? m : ~m;
   }
   const int rank = __popc(same & ((1u << lane) - 1));
-  const int at = in ? mine[digit] + rank : 0;
+  const int before = in ? count[digit] : 0;
   __syncwarp();
-  if (in && rank == 0) mine[digit] += __popc(same);
+  if (in && rank == 0) count[digit] = before + __popc(same);
   __syncwarp();
-  return at;
+  return before + rank;
 }
 
 struct ScatterSmem {
@@ -154,93 +154,114 @@ struct ScatterSmem {
 };
 int scatter_bytes(int bins) { return (int)sizeof(ScatterSmem) + (GR_WARPS + 2) * bins * 4; }
 
-__global__ void __launch_bounds__(GR_THREADS) k_group_scatter(GroupPass p) {
+template <int BITS>
+__global__ void __launch_bounds__(GR_THREADS, 5) k_group_scatter(GroupPass p) {
+  pdl_wait();
   extern __shared__ int32_t dyn[];
   ScatterSmem& sm = *reinterpret_cast<ScatterSmem*>(dyn);
-  const int bins = 1 << p.bits;
-  int* const whist = dyn + sizeof(ScatterSmem) / 4;  // (GR_WARPS, bins): counts, then next local positions
-  int* const lstart = whist + GR_WARPS * bins;       // first local position of a digit
-  int* const gstart = lstart + bins;                 // its first position in the result
+  constexpr int BINS = 1 << BITS;
+  int* const whist = dyn + sizeof(ScatterSmem) / 4;  // (GR_WARPS, BINS): a warp's counts, then its first local positions
+  int* const lstart = whist + GR_WARPS * BINS;       // digit totals
+  int* const gstart = lstart + BINS;                 // a digit's first position in the result, less its first local one
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  for (int b = tid; b < GR_WARPS * bins; b += GR_THREADS) whist[b] = 0;
-  __syncthreads();
   constexpr int SEG = GR_TILE / GR_WARPS;  // consecutive rows of one warp
   const int64_t i0 = (int64_t)blockIdx.x * GR_TILE + warp * SEG, i1 = imin64(p.n, i0 + SEG);
-  int* const mine = whist + warp * bins;
-  int32_t z[SEG / 32];
+  int* const mine = whist + warp * BINS;
+  auto digit = [&](int32_t key) { return (key >> p.shift) & (BINS - 1); };
+  // every global load of the CTA's input first
+  int32_t z[SEG / 32], row[SEG / 32];
 #pragma unroll
   for (int j = 0; j < SEG / 32; ++j) {
     const int64_t i = i0 + j * 32 + lane;
     z[j] = i < i1 ? row_key(p.key[i], p.G) : 0;
+    row[j] = p.row && i < i1 ? p.row[i] : (int32_t)i;
   }
-#pragma unroll
-  for (int j = 0; j < SEG / 32; ++j)
-    if (i0 + j * 32 + lane < i1) atomicAdd(&mine[digit_of_key(p, z[j])], 1);
+  for (int b = tid; b < BINS; b += GR_THREADS) {
+    lstart[b] = p.totals[b];
+    gstart[b] = p.counts[(int64_t)b * p.nb + blockIdx.x];
+  }
+  for (int b = tid; b < GR_WARPS * BINS; b += GR_THREADS) whist[b] = 0;
   __syncthreads();
-  // digits in runs of bins / GR_THREADS per thread: local starts and starts in the result
-  const int per = (bins + GR_THREADS - 1) / GR_THREADS;
+  int rel[SEG / 32];  // place within the warp's rows of the digit
+#pragma unroll
+  for (int j = 0; j < SEG / 32; ++j) rel[j] = place<BITS>(mine, digit(z[j]), i0 + j * 32 + lane < i1, lane);
+  __syncthreads();
+  // digits in runs of PER per thread: local starts and starts in the result
+  constexpr int PER = (BINS + GR_THREADS - 1) / GR_THREADS;
   int local = 0, global = 0;
-  for (int k = 0; k < per; ++k) {
-    const int b = tid * per + k;
-    if (b >= bins) break;
-    for (int w = 0; w < GR_WARPS; ++w) local += whist[w * bins + b];
-    global += p.totals[b];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int b = tid * PER + k;
+    if (b >= BINS) break;
+#pragma unroll
+    for (int w = 0; w < GR_WARPS; ++w) local += whist[w * BINS + b];
+    global += lstart[b];
   }
   int ls = cta_exclusive<GR_THREADS>(local, sm.sums);
   int gs = cta_exclusive<GR_THREADS>(global, sm.sums);
-  for (int k = 0; k < per; ++k) {
-    const int b = tid * per + k;
-    if (b >= bins) break;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int b = tid * PER + k;
+    if (b >= BINS) break;
     if (p.offsets && blockIdx.x == 0 && b <= p.G) p.offsets[b] = gs;
-    lstart[b] = ls;
-    gstart[b] = gs + p.counts[(int64_t)b * p.nb + blockIdx.x];
+    gstart[b] += gs - ls;
+    gs += lstart[b];
+#pragma unroll
     for (int w = 0; w < GR_WARPS; ++w) {
-      const int c = whist[w * bins + b];
-      whist[w * bins + b] = ls;
+      const int c = whist[w * BINS + b];
+      whist[w * BINS + b] = ls;
       ls += c;
     }
-    gs += p.totals[b];
   }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < SEG / 32; ++j) {
-    const int64_t i = i0 + j * 32 + lane;
-    const bool in = i < i1;
-    const int at = place(mine, digit_of_key(p, z[j]), p.bits, in, lane);
-    if (in) {
+    if (i0 + j * 32 + lane < i1) {
+      const int at = mine[digit(z[j])] + rel[j];
       sm.key[at] = z[j];
-      sm.row[at] = p.row ? p.row[i] : (int32_t)i;
+      sm.row[at] = row[j];
     }
   }
   __syncthreads();
   const int rows = (int)imin64(GR_TILE, p.n - (int64_t)blockIdx.x * GR_TILE);
-  for (int i = tid; i < rows; i += GR_THREADS) {
+#pragma unroll
+  for (int j = 0; j < GR_TILE / GR_THREADS; ++j) {
+    const int i = j * GR_THREADS + tid;
+    if (i >= rows) break;
     const int32_t key = sm.key[i];
-    const int dg = digit_of_key(p, key);
-    const int64_t at = gstart[dg] + (i - lstart[dg]);
+    const int at = gstart[digit(key)] + i;
     p.row_out[at] = sm.row[i];
     if (p.key_out) p.key_out[at] = key;
   }
 }
 
+template <int BITS>
 __global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __restrict__ species, int n, int G,
-                                                            int bits, int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
-  __shared__ int whist[32][GS_MAX_BINS];
+                                                            int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
+  pdl_wait();
+  __shared__ int whist[32][1 << BITS];
   __shared__ int sums[32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int bins = G + 1;
-  for (int b = lane; b < bins; b += 32) whist[warp][b] = 0;
+  constexpr int MOST = GS_MAX_ROWS / GS_THREADS;  // rounds of 32 rows of one warp
+  const int rounds = (n + GS_THREADS - 1) / GS_THREADS;
+  const int i0 = warp * rounds * 32, i1 = min(n, i0 + rounds * 32);  // consecutive rows of one warp
+  int key[MOST], rel[MOST];
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) key[j] = i0 + j * 32 + lane < i1 ? row_key(species[i0 + j * 32 + lane], G) : 0;
+  for (int b = lane; b < (1 << BITS); b += 32) whist[warp][b] = 0;
   __syncwarp();
-  const int seg = ((n + GS_THREADS - 1) / GS_THREADS) * 32;  // consecutive rows of one warp
-  const int i0 = warp * seg, i1 = min(n, i0 + seg);
-  for (int i = i0 + lane; i < i1; i += 32) atomicAdd(&whist[warp][row_key(species[i], G)], 1);
+#pragma unroll
+  for (int j = 0; j < MOST; ++j)
+    if (j < rounds) rel[j] = place<BITS>(whist[warp], key[j], i0 + j * 32 + lane < i1, lane);
   __syncthreads();
   int total = 0;
-  if (tid < bins)
+  if (tid < (1 << BITS))
+#pragma unroll 8
     for (int w = 0; w < 32; ++w) total += whist[w][tid];
   int at = cta_exclusive<GS_THREADS>(total, sums);
-  if (tid < bins) {
-    offsets[tid] = at;
+  if (tid < (1 << BITS)) {
+    if (tid <= G) offsets[tid] = at;
+#pragma unroll 8
     for (int w = 0; w < 32; ++w) {
       const int c = whist[w][tid];
       whist[w][tid] = at;
@@ -248,22 +269,32 @@ __global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __res
     }
   }
   __syncthreads();
-  for (int base = i0; base < i1; base += 32) {
-    const int i = base + lane;
-    const bool in = i < i1;
-    const int key = in ? row_key(species[i], G) : 0;
-    const int to = place(whist[warp], key, bits, in, lane);
-    if (in) order[to] = i;
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) {
+    const int i = i0 + j * 32 + lane;
+    if (j < rounds && i < i1) order[whist[warp][key[j]] + rel[j]] = i;
   }
 }
 
-// offsets[v] = first position whose key is >= v
-__global__ void k_group_offsets(const int32_t* __restrict__ key, int64_t n, int G, int32_t* __restrict__ offsets) {
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i <= n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int prev = i > 0 ? key[i - 1] : -1;
-    const int cur = i < n ? key[i] : G;
-    for (int v = prev + 1; v <= cur; ++v) offsets[v] = (int32_t)i;
+// offsets[v] = first position whose key is >= v; four positions per thread (key is 16-byte aligned)
+__global__ void __launch_bounds__(256) k_group_offsets(const int32_t* __restrict__ key, int64_t n, int G,
+                                                       int32_t* __restrict__ offsets) {
+  pdl_wait();
+  const int64_t i0 = (blockIdx.x * (int64_t)256 + threadIdx.x) * 4;
+  if (i0 > n) return;
+  int k[5];
+  k[0] = i0 > 0 ? key[i0 - 1] : -1;
+  if (i0 + 4 <= n) {
+    const int4 v = *reinterpret_cast<const int4*>(key + i0);
+    k[1] = v.x, k[2] = v.y, k[3] = v.z, k[4] = v.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) k[j + 1] = i0 + j < n ? key[i0 + j] : G;
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (i0 + j <= n)
+      for (int v = k[j] + 1; v <= k[j + 1]; ++v) offsets[v] = (int32_t)(i0 + j);
 }
 
 // Consecutive vectors of V elements of the (n, C) result, CTA by CTA.
@@ -274,6 +305,7 @@ template <typename T, int V, bool FLAT>
 __global__ void __launch_bounds__(RW_THREADS) k_embed(const T* __restrict__ table, int64_t ts, int G, int C,
                                                       const int32_t* __restrict__ species, int64_t n, float scale,
                                                       T* __restrict__ out, int64_t os, RowDiv div) {
+  pdl_wait();
   const int64_t v0 = blockIdx.x * (int64_t)(RW_THREADS * RW_UNROLL);  // first vector of this CTA
   const int64_t total = n * C;
   const int64_t row0 = (v0 * V) / C;
@@ -351,6 +383,7 @@ constexpr int EG_THREADS = 256;
 
 template <typename T, int V, int RL>
 __global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad(EmbedGrad p) {
+  pdl_wait();
   constexpr int CL = 32 / RL;             // channel lanes
   constexpr int UN = RL == 8 ? 4 : 8;     // row loads in flight per lane (UN RL <= 32)
   const int lane = threadIdx.x & 31, cl = lane % CL, rl = lane / CL;
@@ -418,6 +451,7 @@ constexpr int EJ_ALONE = 16;
 
 template <typename T>
 __global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p, int per_cta) {
+  pdl_wait();
   __shared__ float sums[32][33];
   __shared__ uint32_t many;
   const int cl = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -513,6 +547,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* __restrict__ x, int64_t xn, int64_t xm, int64_t rows,
                                                            int d, int C, int nb, int8_t* __restrict__ q,
                                                            float* __restrict__ scale) {
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t items = rows * nb;
   const int64_t i0 = (blockIdx.x * (int64_t)(RW_THREADS / 32) + (threadIdx.x >> 5)) * CK_ROWS;
@@ -584,6 +619,7 @@ template <typename T>
 __global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* __restrict__ q, const float* __restrict__ scale,
                                                         int64_t total, int C, int nb, T* __restrict__ x, RowDiv div,
                                                         int vec) {
+  pdl_wait();
   const int64_t e0 = blockIdx.x * (int64_t)(RW_THREADS * RS_UNROLL * 4);
   const int64_t row0 = e0 / C;
   const uint32_t first = (uint32_t)(e0 - row0 * C);
@@ -636,10 +672,6 @@ __global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* __restrict
   }
 }
 
-int64_t blocks_for(int64_t items, int per_block, int64_t most) {
-  return std::max<int64_t>(1, std::min<int64_t>((items + per_block - 1) / per_block, most));
-}
-
 // bits of one counting pass and passes for G + 1 keys
 void group_passes(int G, int* bits, int* passes) {
   int b = 1;
@@ -662,6 +694,14 @@ int64_t align16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 using namespace mace;
 
 namespace {
+
+// f(std::integral_constant<int, bits>) for 1 <= bits <= MOST
+template <int MOST, typename F>
+int with_bits(int bits, F&& f) {
+  if constexpr (MOST > 1)
+    if (bits < MOST) return with_bits<MOST - 1>(bits, f);
+  return f(std::integral_constant<int, MOST>{});
+}
 
 struct GroupPlan {
   int bits, passes, nb;
@@ -703,11 +743,11 @@ extern "C" int mace_species_group(const int32_t* species, int64_t n, int32_t G, 
     MACE_CUDA_TRY(cudaMemsetAsync(offsets, 0, (size_t)(G + 1) * 4, s));
     return MACE_OK;
   }
-  if (plan.small) {
-    k_group_small<<<1, GS_THREADS, 0, s>>>(species, (int)n, G, plan.bits, order, offsets);
-    MACE_LAUNCH_CHECK("group_small");
-    return MACE_OK;
-  }
+  if (plan.small)
+    return with_bits<8>(plan.bits, [&](auto bits) {
+      return launch("group_small", k_group_small<decltype(bits)::value>, 1, GS_THREADS, 0, s, species, (int)n, G, order,
+                    offsets);
+    });
   GroupPass p{};
   p.n = n;
   p.G = G;
@@ -720,15 +760,6 @@ extern "C" int mace_species_group(const int32_t* species, int64_t n, int32_t G, 
   int32_t* key1 = reinterpret_cast<int32_t*>(at + plan.counts);
   int32_t* row1 = reinterpret_cast<int32_t*>(at + plan.counts + plan.keys);
   int32_t* key2 = reinterpret_cast<int32_t*>(at + plan.counts + 2 * plan.keys);
-  const int smem = scatter_bytes(bins);
-  static bool attr_set[64] = {};  // per device: the attribute call is slow on the host
-  int dev = 0;
-  MACE_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev >= 64 || !attr_set[dev]) {
-    MACE_CUDA_TRY(cudaFuncSetAttribute(k_group_scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       scatter_bytes(GR_MAX_BINS)));
-    if (dev < 64) attr_set[dev] = true;
-  }
   for (int q = 0; q < plan.passes; ++q) {
     const bool last = q == plan.passes - 1;
     p.shift = q * plan.bits;
@@ -737,18 +768,25 @@ extern "C" int mace_species_group(const int32_t* species, int64_t n, int32_t G, 
     p.key_out = plan.passes == 1 ? nullptr : (last ? key2 : key1);
     p.row_out = last ? order : row1;
     p.offsets = plan.passes == 1 ? offsets : nullptr;
-    k_group_count<<<p.nb, GR_THREADS, 0, s>>>(p);
-    MACE_LAUNCH_CHECK("group_count");
-    k_group_scan<<<bins, GR_THREADS, 0, s>>>(p);
-    MACE_LAUNCH_CHECK("group_scan");
-    k_group_scatter<<<p.nb, GR_THREADS, smem, s>>>(p);
-    MACE_LAUNCH_CHECK("group_scatter");
+    int rc = launch("group_count", k_group_count, p.nb, GR_THREADS, 0, s, p);
+    if (!rc) rc = launch("group_scan", k_group_scan, bins, GR_THREADS, 0, s, p);
+    if (!rc)
+      rc = with_bits<10>(plan.bits, [&](auto bits) {
+        constexpr int B = decltype(bits)::value;
+        static bool attr_set[64] = {};  // per device: the attribute call is slow on the host
+        int dev = 0;
+        MACE_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev >= 64 || !attr_set[dev]) {
+          MACE_CUDA_TRY(cudaFuncSetAttribute(k_group_scatter<B>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             scatter_bytes(1 << B)));
+          if (dev < 64) attr_set[dev] = true;
+        }
+        return launch("group_scatter", k_group_scatter<B>, p.nb, GR_THREADS, scatter_bytes(1 << B), s, p);
+      });
+    if (rc) return rc;
   }
-  if (plan.passes > 1) {
-    k_group_offsets<<<(int)blocks_for(n + 1, 256, 148 * 8), 256, 0, s>>>(key2, n, G, offsets);
-    MACE_LAUNCH_CHECK("group_offsets");
-  }
-  return MACE_OK;
+  if (plan.passes == 1) return MACE_OK;
+  return launch("group_offsets", k_group_offsets, (unsigned)((n + 1024) / 1024), 256, 0, s, key2, n, G, offsets);
 }
 
 namespace {
@@ -769,14 +807,12 @@ int embed(const void* table, int64_t ts, int G, int C, const int32_t* species, i
     const int64_t per = (int64_t)RW_THREADS * RW_UNROLL * v;
     return (unsigned)((n * C + per - 1) / per);
   };
-  if (C % V == 0 && ts % V == 0 && os % V == 0 && aligned16(table) && aligned16(out))
-    k_embed<T, V, false><<<grid(V), RW_THREADS, 0, s>>>(t, ts, G, C, species, n, scale, o, os, row_div(C));
-  else if (os == C && aligned16(out))
-    k_embed<T, V, true><<<grid(V), RW_THREADS, 0, s>>>(t, ts, G, C, species, n, scale, o, os, row_div(C));
-  else
-    k_embed<T, 1, false><<<grid(1), RW_THREADS, 0, s>>>(t, ts, G, C, species, n, scale, o, os, row_div(C));
-  MACE_LAUNCH_CHECK("species_embed");
-  return MACE_OK;
+  auto go = [&](auto kernel, int v) {
+    return launch("species_embed", kernel, grid(v), RW_THREADS, 0, s, t, ts, G, C, species, n, scale, o, os, row_div(C));
+  };
+  if (C % V == 0 && ts % V == 0 && os % V == 0 && aligned16(table) && aligned16(out)) return go(k_embed<T, V, false>, V);
+  if (os == C && aligned16(out)) return go(k_embed<T, V, true>, V);
+  return go(k_embed<T, 1, false>, 1);
 }
 
 }  // namespace
@@ -805,35 +841,30 @@ extern "C" int mace_species_embed_grad_workspace(int64_t n, int32_t G, int32_t C
 namespace {
 
 template <typename T, int V>
-void launch_embed_grad(const EmbedGrad& p, cudaStream_t s) {
+int launch_embed_grad(const EmbedGrad& p, cudaStream_t s) {
   // row lanes: the most that still leave V channels per lane for one row
   const int cl = (p.C + V - 1) / V;
   const unsigned gx = (unsigned)((p.shares + EG_THREADS / 32 - 1) / (EG_THREADS / 32));
-  if (cl <= 4)
-    k_embed_grad<T, V, 8><<<dim3(gx, 1), EG_THREADS, 0, s>>>(p);
-  else if (cl <= 8)
-    k_embed_grad<T, V, 4><<<dim3(gx, 1), EG_THREADS, 0, s>>>(p);
-  else if (cl <= 16)
-    k_embed_grad<T, V, 2><<<dim3(gx, 1), EG_THREADS, 0, s>>>(p);
-  else
-    k_embed_grad<T, V, 1><<<dim3(gx, (cl + 31) / 32), EG_THREADS, 0, s>>>(p);
+  auto go = [&](auto kernel, int lanes) {
+    return launch("species_embed_grad", kernel, dim3(gx, (cl + lanes - 1) / lanes), EG_THREADS, 0, s, p);
+  };
+  if (cl <= 4) return go(k_embed_grad<T, V, 8>, 4);
+  if (cl <= 8) return go(k_embed_grad<T, V, 4>, 8);
+  if (cl <= 16) return go(k_embed_grad<T, V, 2>, 16);
+  return go(k_embed_grad<T, V, 1>, 32);
 }
 
 template <typename T>
 int embed_grad(const EmbedGrad& p, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   if (p.n > 0) {
-    if (p.C % V == 0 && p.ds % V == 0 && aligned16(p.dy) && aligned16(p.out))
-      launch_embed_grad<T, V>(p, s);
-    else
-      launch_embed_grad<T, 1>(p, s);
-    MACE_LAUNCH_CHECK("species_embed_grad");
+    const bool vec = p.C % V == 0 && p.ds % V == 0 && aligned16(p.dy) && aligned16(p.out);
+    const int rc = vec ? launch_embed_grad<T, V>(p, s) : launch_embed_grad<T, 1>(p, s);
+    if (rc) return rc;
   }
   const int per_cta = std::max(1, std::min(32, (p.G + 147) / 148));
-  k_embed_grad_join<T><<<dim3((unsigned)std::min((p.G + per_cta - 1) / per_cta, 148 * 2), (p.C + 31) / 32), 1024, 0,
-                         s>>>(p, per_cta);
-  MACE_LAUNCH_CHECK("species_embed_grad_join");
-  return MACE_OK;
+  const dim3 grid(std::min((p.G + per_cta - 1) / per_cta, 148 * 2), (p.C + 31) / 32);
+  return launch("species_embed_grad_join", k_embed_grad_join<T>, grid, 1024, 0, s, p, per_cta);
 }
 
 }  // namespace
@@ -871,17 +902,10 @@ extern "C" int mace_rows_checkpoint(int32_t dtype, const void* x, int64_t xn, in
     const T* src = static_cast<const T*>(x);
     const bool vec = C % 4 == 0 && (n <= 1 || xn % 4 == 0) && (d <= 1 || xm % 4 == 0) &&
                      reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(q) % 4 == 0;
-    if (vec)
-      k_checkpoint<T, true><<<(int)grid, RW_THREADS, 0, s>>>(src, xn, xm, n * d, d, C, nb, q, scale);
-    else
-      k_checkpoint<T, false><<<(int)grid, RW_THREADS, 0, s>>>(src, xn, xm, n * d, d, C, nb, q, scale);
+    return launch("rows_checkpoint", vec ? k_checkpoint<T, true> : k_checkpoint<T, false>, (unsigned)grid, RW_THREADS, 0,
+                  s, src, xn, xm, n * d, d, C, nb, q, scale);
   };
-  if (dtype == MACE_F32)
-    go(float{});
-  else
-    go(bf16{});
-  MACE_LAUNCH_CHECK("rows_checkpoint");
-  return MACE_OK;
+  return dtype == MACE_F32 ? go(float{}) : go(bf16{});
 }
 
 extern "C" int mace_rows_restore(int32_t dtype, const int8_t* q, const float* scale, int64_t n, int32_t d, int32_t C,
@@ -896,10 +920,10 @@ extern "C" int mace_rows_restore(int32_t dtype, const int8_t* q, const float* sc
   if ((total + per - 1) / per > INT32_MAX) return fail(MACE_ERR_BAD_ARG, "mace_rows_restore: too many rows");
   const unsigned grid = (unsigned)((total + per - 1) / per);
   const int vec = reinterpret_cast<uintptr_t>(q) % 4 == 0 && aligned16(x);
-  if (dtype == MACE_F32)
-    k_restore<float><<<grid, RW_THREADS, 0, s>>>(q, scale, total, C, nb, static_cast<float*>(x), row_div(C), vec);
-  else
-    k_restore<bf16><<<grid, RW_THREADS, 0, s>>>(q, scale, total, C, nb, static_cast<bf16*>(x), row_div(C), vec);
-  MACE_LAUNCH_CHECK("rows_restore");
-  return MACE_OK;
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    return launch("rows_restore", k_restore<T>, grid, RW_THREADS, 0, s, q, scale, total, C, nb, static_cast<T*>(x),
+                  row_div(C), vec);
+  };
+  return dtype == MACE_F32 ? go(float{}) : go(bf16{});
 }

@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
     tc::tmem_alloc(tc::smem_u32(tslot), DR_TMEM);
     tc::tmem_relinquish();
   }
+  pdl_wait();  // nothing of the caller's is read or written before
   tc::fence_before_sync();
   load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, q, reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
     Walk w;
     w.init(p, q, t0);
     if constexpr (!WG) {
-      const uint32_t stage = base + S::OFF_STG + (warp - 8) * S::STG;
+      uint8_t* const stage = smem + S::OFF_STG + (warp - 8) * S::STG;
       RowRef ref;  // this lane's row of the next tile, loaded while the tile before it is stored
       int ct = 0;
       auto load_tile = [&]() {
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
               o[k] = pack_bf16(p.alpha * __uint_as_float(v[2 * k]), p.alpha * __uint_as_float(v[2 * k + 1]));
 #pragma unroll
             for (int k = 0; k < 2; ++k)
-              sts128(stage + row * 128 + (((2 * h + k) ^ (row & 7)) << 4), o[4 * k], o[4 * k + 1], o[4 * k + 2],
+              store_piece(stage + row * 128 + (((2 * h + k) ^ (row & 7)) << 4), o[4 * k], o[4 * k + 1], o[4 * k + 2],
                      o[4 * k + 3]);
           }
         }
@@ -472,9 +473,7 @@ int launch_direct(const SlParams& p, int grid, cudaStream_t s) {
     MACE_CUDA_TRY(cudaFuncSetAttribute(k_species_direct<WG>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
     if (dev < 64) attr_set[dev] = true;
   }
-  k_species_direct<WG><<<grid, SL_THREADS, BYTES, s>>>(p);
-  MACE_LAUNCH_CHECK("species_direct");
-  return MACE_OK;
+  return launch("species_direct", k_species_direct<WG>, grid, SL_THREADS, BYTES, s, p);
 }
 
 }  // namespace

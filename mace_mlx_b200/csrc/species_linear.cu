@@ -153,49 +153,29 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
+// Shared memory through pointers, so that constant offsets become part of the instruction
+template <typename T>
+__device__ __forceinline__ T load_as(const uint8_t* a) { return *reinterpret_cast<const T*>(a); }
+template <typename T>
+__device__ __forceinline__ float load_f32(const uint8_t* a) { return to_f32(load_as<T>(a)); }
+__device__ __forceinline__ void store_piece(uint8_t* a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  *reinterpret_cast<uint4*>(a) = make_uint4(x, y, z, w);
 }
-__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-__device__ __forceinline__ float lds_as(uint32_t a, float) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ float lds_as(uint32_t a, bf16) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
-  return __uint_as_float((uint32_t)v << 16);
-}
-__device__ __forceinline__ float lds_raw(uint32_t a, float) { return lds_as(a, 0.f); }
-__device__ __forceinline__ bf16 lds_raw(uint32_t a, bf16) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
-  return __ushort_as_bfloat16(v);
-}
-__device__ __forceinline__ void lds_eight(uint32_t a, float* v, float) {
-  const uint4 x = lds128(a), y = lds128(a + 16);
+// eight consecutive values
+__device__ __forceinline__ void load_eight(const uint8_t* a, float* v, float) {
+  const uint4 x = load_as<uint4>(a), y = load_as<uint4>(a + 16);
   const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(w[k]);
 }
-__device__ __forceinline__ void lds_eight(uint32_t a, float* v, bf16) {
-  const uint4 x = lds128(a);
+__device__ __forceinline__ void load_eight(const uint8_t* a, float* v, bf16) {
+  const uint4 x = load_as<uint4>(a);
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     v[2 * k] = __uint_as_float(w[k] << 16);
     v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
   }
-}
-__device__ __forceinline__ float lds_as(uint32_t a, int8_t) {
-  int v;
-  asm volatile("ld.shared.s8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return (float)v;
 }
 
 // two values rounded to bf16, x0 in the low half
@@ -517,7 +497,7 @@ __device__ __forceinline__ void fetch_any(uint32_t dst, const char* data, const 
 // Map: 32 staged row segments of 128 bytes (piece j of row r at j ^ (r & 7)) to columns c0 .. c0 + left - 1 of the
 // rows at element offset o (< 0: none; o16: in 16 bytes for aligned rows), one row per lane.
 template <typename T>
-__device__ __forceinline__ void copy_out(const SlParams& p, uint32_t stage, int64_t o, uint32_t o16, int c0, int left) {
+__device__ __forceinline__ void copy_out(const SlParams& p, const uint8_t* stage, int64_t o, uint32_t o16, int c0, int left) {
   int row = threadIdx.x & 31;
   asm volatile("" : "+r"(row));  // addresses are made here each time: held across the tiles they crowd the registers
   __syncwarp();
@@ -526,14 +506,14 @@ __device__ __forceinline__ void copy_out(const SlParams& p, uint32_t stage, int6
     const int j = row & 7;
     const bool have = left * (int)sizeof(T) > 16 * j;
     char* const to = static_cast<char*>(p.out) + (int64_t)c0 * sizeof(T) + 16 * j;
-    const uint32_t src = stage + (row >> 3) * 128;
+    const uint8_t* const src = stage + (row >> 3) * 128;
 #pragma unroll
     for (int i0 = 0; i0 < 8; i0 += 4) {
       uint4 v[4];
       uint32_t ro[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // (r & 7 alternates between lane / 8 and lane / 8 + 4)
-        v[i] = lds128(src + (i0 + i) * 512 + ((j ^ ((row >> 3) + (i & 1) * 4)) << 4));
+        v[i] = load_as<uint4>(src + (i0 + i) * 512 + ((j ^ ((row >> 3) + (i & 1) * 4)) << 4));
         ro[i] = __shfl_sync(0xffffffffu, o16, (i0 + i) * 4 + (row >> 3));
       }
 #pragma unroll
@@ -548,7 +528,7 @@ __device__ __forceinline__ void copy_out(const SlParams& p, uint32_t stage, int6
 #pragma unroll
       for (int c = 0; c < 128 / (int)sizeof(T); c += 32) {
         const int byte = (c + row) * (int)sizeof(T);
-        const T v = lds_raw(stage + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15)), T{});
+        const T v = load_as<T>(stage + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15)));
         if (ro >= 0 && c + row < left) (static_cast<T*>(p.out) + ro + c0)[c + row] = v;
       }
     }
@@ -621,13 +601,13 @@ constexpr int SL_IMG = 128 * 128;  // bytes of one piece of a B image: up to 128
 
 // 8 K-values of row n of a B image: their bf16 pieces
 template <int P>
-__device__ __forceinline__ void put_eight(uint32_t img, int n, int chunk, const float* v) {
+__device__ __forceinline__ void put_eight(uint8_t* img, int n, int chunk, const float* v) {
   uint32_t t[4][3];
 #pragma unroll
   for (int q = 0; q < 4; ++q) split2<P>(v[2 * q], v[2 * q + 1], t[q]);
 #pragma unroll
   for (int b = 0; b < P; ++b)
-    sts128(img + b * SL_IMG + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
+    store_piece(img + b * SL_IMG + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
 }
 
 // Where weight (k, n) of a step waits, as it is, in its own image slot: 64 columns (one round of the rewriting)
@@ -646,7 +626,7 @@ __device__ __forceinline__ uint32_t raw_place(int k, int n, bool transposed) {
 // round is 16 items of 32 (image row, K octet) pairs, one per lane, four items per warp.  Weights (K, N): an item
 // is one octet of 32 neighbouring columns; transposed (N, K): 8 octets of 4 rows.
 template <typename T, int PB>
-__device__ __forceinline__ bool fill_weights(const SlParams& p, uint32_t img0, uint32_t stride, int g, int ct, int k0,
+__device__ __forceinline__ bool fill_weights(const SlParams& p, uint8_t* img0, int stride, int g, int ct, int k0,
                                              int nk, uint32_t full, uint32_t w_sync_bar, int& syncs,
                                              volatile int* abort) {
   const int lane = threadIdx.x & 31, w4 = (threadIdx.x >> 5) & 3;
@@ -665,7 +645,7 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint32_t img0, u
     const bool on = sub < rpi;
 #pragma unroll 1
     for (int s = 0; s < nk; ++s) {
-      const uint32_t raw = img0 + s * stride;
+      const uint32_t raw = tc::smem_u32(img0) + s * stride;
       const int k = (k0 + s) * SL_KC, n = ct * NT;
       const int r0 = p.transposed ? n : k, c0 = (p.transposed ? k : n) + c;  // in the whole matrix
       const int r_end = p.transposed ? p.N : p.K, c_end = p.transposed ? p.K : p.N;
@@ -685,7 +665,7 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint32_t img0, u
   }
 #pragma unroll 1
   for (int s = 0; s < nk; ++s) {
-    const uint32_t img = img0 + s * stride;
+    uint8_t* const img = img0 + s * stride;
 #pragma unroll 1
     for (int h = 0; h * 64 < NT; ++h) {
       float v[4][8];
@@ -695,10 +675,10 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint32_t img0, u
         const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane, kk = (p.transposed ? lane & 7 : j & 7) * 8;
         if (p.w_vec) {
           if (p.transposed) {
-            lds_eight(img + raw_place<T>(kk, n, true), v[u], T{});
+            load_eight(img + raw_place<T>(kk, n, true), v[u], T{});
           } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[u][e] = lds_as(img + raw_place<T>(kk + e, n, false), T{});
+            for (int e = 0; e < 8; ++e) v[u][e] = load_f32<T>(img + raw_place<T>(kk + e, n, false));
           }
         } else {
           const int col = ct * NT + n, k = (k0 + s) * SL_KC + kk;
@@ -775,6 +755,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     tc::tmem_alloc(tc::smem_u32(tslot), SL_TMEM);
     tc::tmem_relinquish();
   }
+  pdl_wait();  // nothing of the caller's is read or written before
   tc::fence_before_sync();
   load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, q, reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
@@ -910,7 +891,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         __syncwarp();
         fetch();
         if (i < 0) continue;
-        const uint32_t src = ring + slot * S::UNIT_A;
+        const uint8_t* const src = smem + S::OFF_A + (warp * NU + slot) * S::UNIT_A;
         const uint8_t* const ms = mis + slot * 32;
         slot = slot + 1 == NU ? 0 : slot + 1;
         if (u == 0) {
@@ -924,7 +905,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
           // this lane's row: 128 bytes of it
           const int sh = VEC ? 0 : ms[lane];
           auto piece = [&](int j) {
-            return lds128(src + lane * S::PITCH_A + (VEC ? (j ^ (lane & 7)) : j) * 16);
+            return load_as<uint4>(src + lane * S::PITCH_A + (VEC ? (j ^ (lane & 7)) : j) * 16);
           };
           uint32_t out[PA][16];
           uint4 cur = piece(0);
@@ -967,10 +948,10 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
           uint32_t out[PA][16];
 #pragma unroll
           for (int r = 0; r < 32; r += 2) {
-            const uint32_t a0 = src + r * S::PITCH_A + lane * (int)sizeof(TA) + (VEC ? 0 : ms[r]);
-            const uint32_t a1 = src + (r + 1) * S::PITCH_A + lane * (int)sizeof(TA) + (VEC ? 0 : ms[r + 1]);
+            const uint8_t* const mine = src + lane * (int)sizeof(TA);
             uint32_t t[3];
-            split2<PA>(lds_as(a0, TA{}), lds_as(a1, TA{}), t);
+            split2<PA>(load_f32<TA>(mine + r * S::PITCH_A + (VEC ? 0 : ms[r])),
+                       load_f32<TA>(mine + (r + 1) * S::PITCH_A + (VEC ? 0 : ms[r + 1])), t);
 #pragma unroll
             for (int a = 0; a < PA; ++a) out[a][r / 2] = t[a];
           }
@@ -993,7 +974,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
       if constexpr (!WG) {
         int syncs = 0;
         auto fill = [&](int g, int ct, int k0, int nk, int slot0) -> bool {
-          return fill_weights<T, PB>(p, base + slot0 * PB * SL_IMG, PB * SL_IMG, g, ct, k0, nk, bar(8 + slot0), W_SYNC,
+          return fill_weights<T, PB>(p, smem + slot0 * PB * SL_IMG, PB * SL_IMG, g, ct, k0, nk, bar(8 + slot0), W_SYNC,
                                      syncs, abort);
         };
         Walk w;
@@ -1079,7 +1060,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
           __syncwarp();
           fetch();
           if (i < 0) continue;
-          const uint32_t src = ring + slot * S::UNIT_B;
+          const uint8_t* const src = smem + S::OFF_B + (w4 * NU_B + slot) * S::UNIT_B + lane * (int)sizeof(T);
           const uint8_t* const ms = mis + slot * 32;
           const float* const ss = sc + slot * 32;
           slot = slot + 1 == NU_B ? 0 : slot + 1;
@@ -1087,14 +1068,14 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
             ok = __all_sync(0xffffffffu, wait_phase(B_FREE(s), ((it >> 1) - 1) & 1, abort));
             if (!ok) break;
           }
-          const uint32_t img = base + s * PB * SL_IMG;
+          uint8_t* const img = smem + s * PB * SL_IMG;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const int r = 8 * q + j;
-              v[j] = lds_as(src + r * S::PITCH_B + lane * (int)sizeof(T) + (VEC ? 0 : ms[r]), T{});
+              v[j] = load_f32<T>(src + r * S::PITCH_B + (VEC ? 0 : ms[r]));
               if constexpr (sizeof(TA) == 1) v[j] *= ss[r];
             }
             put_eight<PB>(img, n, u * 4 + q, v);
@@ -1184,7 +1165,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         const int64_t o = mine ? ref.node * p.out_sn + ref.m * p.out_sm : -1;
         // aligned rows: offsets in 16 bytes
         const uint32_t o16 = mine ? (uint32_t)((uint64_t)o * sizeof(T) >> 4) : NO_ROW;
-        const uint32_t stage = base + S::OFF_STG + (warp - 8) * S::STG;
+        uint8_t* const stage = smem + S::OFF_STG + (warp - 8) * S::STG;
         if constexpr (PB == 1) {
 #pragma unroll
           for (int k = 0; k < 64; ++k) acc[k] *= p.alpha;
@@ -1207,7 +1188,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
               else
                 w4[q] = pack_bf16(acc[b + 8 * j + 2 * q], acc[b + 8 * j + 2 * q + 1]);
             }
-            sts128(stage + row * 128 + ((j ^ (row & 7)) << 4), w4[0], w4[1], w4[2], w4[3]);
+            store_piece(stage + row * 128 + ((j ^ (row & 7)) << 4), w4[0], w4[1], w4[2], w4[3]);
           }
           __syncwarp();
           copy_out<T>(p, stage, o, o16, c0 + b, left);
@@ -1246,56 +1227,71 @@ namespace mace {
 
 namespace {
 
-// dW of the groups that several shares hold, in share order, and of empty groups (zero).  One CTA: group blockIdx.x,
-// 8 rows x 8 column quads (one per lane of 64) of tile blockIdx.z, four threads of each taking every fourth share.
+// dW of the groups that several shares hold, in share order, and of empty groups (zero).  CTA (g, y, tile): group g,
+// rows 8 (y % 16) .. of the tile, in blocks of 8 rows x 8 column quads (64 lanes).  Few shares: the four sets of 64
+// threads of the CTAs with y < 16 take a block each; many: CTA y takes block y / 16, each set every fourth share.
 template <typename T>
 __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constant__ SlParams p) {
+  pdl_wait();
   __shared__ float4 part[4][64];
   const int g = blockIdx.x, tid = threadIdx.x;
   const int64_t before = p.units[g], mine = p.units[g + 1] - before, all = p.units[p.G];
   const int tile = blockIdx.z;
   const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
   const int lane = tid & 63, sl = tid >> 6;
-  const int kl = (blockIdx.y & 15) * 8 + (lane & 7), cq = (blockIdx.y >> 4) * 8 + (lane >> 3), c = cq * 4;
-  const bool in = k0 + kl < p.K && n0 + c < p.N;
-  T* dst = static_cast<T*>(p.out) + ((int64_t)g * p.K + k0 + kl) * p.N + n0 + c;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int kl = (blockIdx.y & 15) * 8 + (lane & 7), block = blockIdx.y >> 4;
+  int s0 = 0, s1 = -1;  // shares of the group
   if (mine > 0) {
     // share of unit u: the largest s with floor(s all / shares) <= u
     const int64_t shares = min((int64_t)p.shares, all);
-    const int s0 = (int)min(((before + 1) * shares - 1) / all, shares - 1);
-    const int s1 = (int)min(((before + mine) * shares - 1) / all, shares - 1);
+    s0 = (int)min(((before + 1) * shares - 1) / all, shares - 1);
+    s1 = (int)min(((before + mine) * shares - 1) / all, shares - 1);
     if (s0 == s1) return;  // written by its only share
-    if (in) {
-      const float4* src = reinterpret_cast<const float4*>(p.part) +
-                          ((int64_t)tile * (p.shares + p.G) + g) * 32 * p.NT + cq * 128 + kl;
-#pragma unroll 4
-      for (int s = s0 + sl; s <= s1; s += 4) {
-        const float4 v = src[(int64_t)s * 32 * p.NT];
-        acc.x += v.x;
-        acc.y += v.y;
-        acc.z += v.z;
-        acc.w += v.w;
-      }
+  }
+  const float4* const first = reinterpret_cast<const float4*>(p.part) +
+                              ((int64_t)tile * (p.shares + p.G) + g) * 32 * p.NT + kl;
+  T* const row = static_cast<T*>(p.out) + ((int64_t)g * p.K + k0 + kl) * p.N + n0;
+  auto sum = [&](int cq, int from, int step) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = from; s <= s1; s += step) {
+      const float4 v = first[(int64_t)s * 32 * p.NT + cq * 128];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
     }
-    part[sl][lane] = acc;
-    __syncthreads();
-    if (sl != 0) return;
+    return acc;
+  };
+  auto write = [&](int cq, float4 a) {
+    if (k0 + kl >= p.K) return;
+    const float v[4] = {p.alpha * a.x, p.alpha * a.y, p.alpha * a.z, p.alpha * a.w};
+    if (p.vst && n0 + cq * 4 + 4 <= p.N) {
+      store4(row + cq * 4, v);
+    } else {
 #pragma unroll
-    for (int q = 1; q < 4; ++q) {
-      acc.x += part[q][lane].x;
-      acc.y += part[q][lane].y;
-      acc.z += part[q][lane].z;
-      acc.w += part[q][lane].w;
+      for (int k = 0; k < 4; ++k)
+        if (n0 + cq * 4 + k < p.N) row[cq * 4 + k] = from_f32<T>(v[k]);
     }
-  } else if (sl != 0) {
+  };
+  if (s1 - s0 < 8) {
+    const int cq = sl * 8 + (lane >> 3);
+    if (block == 0 && cq * 4 < p.NT) write(cq, sum(cq, s0, 1));
     return;
   }
-  if (!in) return;
-  const float v[4] = {p.alpha * acc.x, p.alpha * acc.y, p.alpha * acc.z, p.alpha * acc.w};
+  const int cq = block * 8 + (lane >> 3);
+  part[sl][lane] = sum(cq, s0 + sl, 4);
+  __syncthreads();
+  if (sl != 0) return;
+  float4 a = part[0][lane];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (n0 + c + k < p.N) dst[k] = from_f32<T>(v[k]);
+  for (int q = 1; q < 4; ++q) {
+    a.x += part[q][lane].x;
+    a.y += part[q][lane].y;
+    a.z += part[q][lane].z;
+    a.w += part[q][lane].w;
+  }
+  write(cq, a);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1347,9 +1343,7 @@ int launch_gemm(const SlParams& p, int grid, cudaStream_t s) {
     MACE_CUDA_TRY(cudaFuncSetAttribute(k_species_gemm<TA, T, WG, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
     if (dev < 64) attr_set[dev] = true;
   }
-  k_species_gemm<TA, T, WG, VEC><<<grid, SL_THREADS, BYTES, s>>>(p);
-  MACE_LAUNCH_CHECK("species_gemm");
-  return MACE_OK;
+  return launch("species_gemm", k_species_gemm<TA, T, WG, VEC>, grid, SL_THREADS, BYTES, s, p);
 }
 
 int64_t partial_bytes(const SlParams& p, int G) {
@@ -1477,12 +1471,8 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
     rc = vec ? launch_direct<true>(p, grid, s) : launch_gemm<bf16, bf16, true, false>(p, grid, s);
   if (rc) return rc;
   const dim3 jg(G, 16 * (p.NT / 32), p.n_ct * p.n_kt);
-  if (dtype == MACE_F32)
-    k_species_wgrad_join<float><<<jg, 256, 0, s>>>(p);
-  else
-    k_species_wgrad_join<bf16><<<jg, 256, 0, s>>>(p);
-  MACE_LAUNCH_CHECK("species_wgrad_join");
-  return MACE_OK;
+  return launch("species_wgrad_join", dtype == MACE_F32 ? k_species_wgrad_join<float> : k_species_wgrad_join<bf16>, jg, 256,
+                0, s, p);
 }
 
 extern "C" int mace_species_error_flag(int32_t* flag) {
