@@ -171,11 +171,11 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
       ring_loop([&](uint32_t dst) {
         if (k == 0) {
           // (a row outside the tile may hold anything: its TMEM lane is never stored)
-          spread_rows<128>(ref.valid(p) ? (uint32_t)(ref.offset(p.a) >> 4) : 0u, off);
+          spread_rows<128>(ref.valid(p) ? ref.pieces(p.a) : 0u, off);
           w.next(q, t1);
           if (w.t < t1) load_tile();
         }
-        fetch_vec<128, 128, true, false>(dst + w4 * 4096, p.a.data, off, k * 128, p.a.width * 2);
+        fetch_vec<128, 128, true, false>(dst + w4 * 4096, p.a.data, off, 0, k * 128, p.a.width * 2);
         if (++k == n_k) k = 0;
       });
     } else {
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
       ring_loop([&](uint32_t dst) {
         if (!second) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) now[u] = next[u].valid(p) ? (uint32_t)(next[u].offset(v) >> 4) : NO_ROW;
+          for (int u = 0; u < 2; ++u) now[u] = next[u].valid(p) ? next[u].pieces(v) : NO_ROW;
           load_pair();
         }
         const uint32_t mine = second ? now[1] : now[0];
@@ -367,12 +367,11 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
                      o[4 * k + 3]);
           }
         }
-        const bool mine = ref.valid(p);
-        const int64_t o = mine ? ref.node * p.out_sn + ref.m * p.out_sm : -1;
+        const RowRef here = ref;
         const int c0 = ct * NT + half * CW, left = min(p.N - c0, CW);
         w.next(q, t1);
         if (w.t < t1) load_tile();
-        if (left > 0) copy_out<bf16>(p, stage, o, mine ? (uint32_t)((uint64_t)o >> 3) : NO_ROW, c0, left);
+        if (left > 0) copy_out<bf16>(p, stage, here, here.valid(p), c0, left);
         __syncwarp();
       }
     } else {

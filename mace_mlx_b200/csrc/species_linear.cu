@@ -56,8 +56,9 @@ __device__ int g_species_error;  // TC_ERR_TIMEOUT once a bounded wait gave up
 // feature rows: element (node, m, c) at data + node * node_stride + m * comp_stride + c
 struct RowView {
   const char* data;
-  int64_t sn, sm;  // bytes
-  int width;       // channels
+  int64_t sn, sm;       // bytes
+  int width;            // channels
+  uint32_t sn16, sm16;  // aligned rows: 16 bytes
 };
 
 struct SlParams {
@@ -68,7 +69,9 @@ struct SlParams {
   const void* w;        // map: weights (G, K, N), or (G, N, K) when transposed
   int transposed;
   void* out;            // map: y; weight gradient: dW (G, K, N)
-  int64_t out_sn, out_sm;  // map: elements
+  int64_t out_sn, out_sm;     // map: elements
+  uint32_t out_n32, out_m32;  // map: the same in 16 bytes (vst) or, where all offsets fit 32 bits (out32), elements
+  int out32;
   int vst;              // map: rows of `out` are whole 16-byte pieces; weight gradient: bytes of a vector store (32, 16, 0)
   float* part;          // weight gradient: partial tiles
   int* units;           // weight gradient: first unit of each group, written by CTA 0 for the join (G + 1)
@@ -76,9 +79,11 @@ struct SlParams {
   const int32_t* offsets;
   int64_t n;
   int d, G;
+  uint32_t div_mul, div_shift;  // x / d for x < 2^31, d > 1: the high word of x div_mul, shifted
   int K, N;             // map: K summed channels, N outputs; weight gradient: K x N of dW
   int w_vec;            // map: rows of the weights are 16-byte aligned
   int NT;               // tile columns: 32, 64, 96 or 128
+  int img, slots;       // map: bytes of one piece of a weight image, slots for the images of a step
   int n_ct, n_kt;       // column tiles; weight gradient: row (channel) tiles
   int shares;           // weight gradient: CTAs along the rows
   float alpha;
@@ -307,8 +312,9 @@ struct Sl {
   static constexpr int NU = WG ? (VEC ? 4 : 3) : 5;
   static constexpr int NU_B = VEC && PA == 3 ? 3 : NU;  // (a fourth unit of fp32 rows would not fit)
   static constexpr int UNIT_A = 32 * PITCH_A, UNIT_B = 32 * PITCH_B;
-  static constexpr int NSLOT = !WG && PB == 1 ? 4 : 2;
-  static constexpr int OFF_A = NSLOT * PB * 128 * 128;
+  static constexpr int IMAGES = (!WG && PB == 1 ? 4 : 2) * PB * 128 * 128;  // bytes of all B images
+  static constexpr int MAX_SLOTS = WG ? 2 : 8;
+  static constexpr int OFF_A = IMAGES;
   static constexpr int OFF_B = OFF_A + 4 * NU * UNIT_A;
   static constexpr int STG = 32 * 128;  // map: an epilogue warp's staging, 32 rows x 128 bytes
   static constexpr int OFF_STG = OFF_B + (WG ? 4 * NU_B * UNIT_B : 0);
@@ -316,7 +322,7 @@ struct Sl {
   static constexpr int OFF_SCALE = OFF_MIS + (VEC ? 0 : (WG ? 8 : 4) * NU * 32);  // per B ring unit and row: A's scale
   static constexpr int OFF_PRE = OFF_SCALE + (sizeof(TA) == 1 ? 4 * NU * 32 * 4 : 0);
   static constexpr int OFF_BAR = OFF_PRE + (3 * MACE_SPECIES_MAX_GROUPS + 2) * 4;
-  static constexpr int NBAR = 8 + 2 * NSLOT + 2;
+  static constexpr int NBAR = 8 + 2 * MAX_SLOTS + 2;
   static constexpr int BYTES = OFF_BAR + NBAR * 8 + 32;
   static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
@@ -402,7 +408,7 @@ struct RowRef {
     int i = at;
     m = 0;
     if (p.d > 1) {
-      i = (uint32_t)at / (uint32_t)p.d;
+      i = __umulhi((uint32_t)at, p.div_mul) >> p.div_shift;
       m = at - i * p.d;
     }
     if (!in) m = -1;
@@ -410,6 +416,7 @@ struct RowRef {
   }
   __device__ __forceinline__ bool valid(const SlParams& p) const { return m >= 0 && node >= 0 && node < p.n; }
   __device__ __forceinline__ int64_t offset(const RowView& v) const { return node * v.sn + m * v.sm; }
+  __device__ __forceinline__ uint32_t pieces(const RowView& v) const { return node * v.sn16 + m * v.sm16; }
 };
 
 // Weight gradient: a lane's rows of the two 32-row ring units of a step, loaded a step ahead (moving a loaded value
@@ -435,11 +442,10 @@ struct StepRows {
   }
 };
 
-// One ring unit: 32 row segments of SEG bytes.  VEC: lane l copies 16-byte piece
-// l % PPR of rows l / PPR + i RPI, whose offsets (in 16 bytes, NO_ROW: zeros) it
-// holds in off[i]; SWZ stores piece j of row r at j ^ (r & 7).
 constexpr uint32_t NO_ROW = 0xffffffffu;
 
+// One ring unit: 32 row segments of SEG bytes.  Aligned rows (VEC): lane l copies 16-byte piece l % PPR of rows
+// l / PPR + i RPI, whose offsets (in 16 bytes) it holds in off[i]; SWZ stores piece j of row r at j ^ (r & 7).
 template <int SEG>
 struct Pieces {
   static constexpr int PPR = SEG / 16, RPI = 32 / PPR, N = PPR;
@@ -453,20 +459,23 @@ __device__ __forceinline__ void spread_rows(uint32_t mine, uint32_t* off) {
   for (int i = 0; i < P::N; ++i) off[i] = __shfl_sync(0xffffffffu, mine, i * P::RPI + lane / P::PPR);
 }
 
-// `at`: first byte of the segment within its row; ZERO: rows may be NO_ROW.  Rows are whole 16-byte pieces here:
-// a copy whose source size is a register costs several instructions more than one that is all or nothing.
-template <int SEG, int PITCH, bool SWZ, bool ZERO>
-__device__ __forceinline__ void fetch_vec(uint32_t dst, const char* data, const uint32_t* off, int at, int row_bytes) {
+// `at`: first byte of the segment within its row; MASK: bit r of `rows` says whether row r exists (else zeros; its
+// offset is 0).  Rows are whole 16-byte pieces here: a copy whose source size is a register costs several
+// instructions more than one that is all or nothing.
+template <int SEG, int PITCH, bool SWZ, bool MASK>
+__device__ __forceinline__ void fetch_vec(uint32_t dst, const char* data, const uint32_t* off, uint32_t rows, int at,
+                                          int row_bytes) {
   using P = Pieces<SEG>;
   const int lane = threadIdx.x & 31, j = lane % P::PPR, r0 = lane / P::PPR;
   const bool past = at + 16 * j >= row_bytes;
   const char* const src = past ? data : data + at + 16 * j;
+  rows = past ? 0u : rows >> r0;
 #pragma unroll
   for (int i = 0; i < P::N; ++i) {
     const int r = i * P::RPI + r0;
     const int pos = SWZ ? (j ^ (r & 7)) : j;
-    const bool none = ZERO && off[i] == NO_ROW;
-    cp_async16_or_zero(dst + r * PITCH + pos * 16, none ? data : src + (uint64_t)off[i] * 16, past || none);
+    cp_async16_or_zero(dst + r * PITCH + pos * 16, src + (uint64_t)off[i] * 16,
+                       MASK ? !((rows >> (i * P::RPI)) & 1u) : past);
   }
 }
 
@@ -494,15 +503,55 @@ __device__ __forceinline__ void fetch_any(uint32_t dst, const char* data, const 
   }
 }
 
-// Map: 32 staged row segments of 128 bytes (piece j of row r at j ^ (r & 7)) to columns c0 .. c0 + left - 1 of the
-// rows at element offset o (< 0: none; o16: in 16 bytes for aligned rows), one row per lane.
+// Map: 32 staged row segments of 128 bytes (piece j of row r at j ^ (r & 7)) to columns c0 .. c0 + left - 1 of their
+// rows, one row per lane (mine: it exists).  Rows of any alignment: a row at a time, neighbouring lanes on
+// neighbouring columns (not inlined: its registers would crowd the aligned path's).
 template <typename T>
-__device__ __forceinline__ void copy_out(const SlParams& p, const uint8_t* stage, int64_t o, uint32_t o16, int c0, int left) {
+__device__ __noinline__ void copy_out_any(const SlParams& p, uint32_t stage_addr, int node, int m, bool mine, int c0,
+                                          int left) {
+  // (a shared-memory address: the compiler cannot see through the call that a pointer would be one)
+  const uint8_t* const stage = static_cast<const uint8_t*>(__cvta_shared_to_generic(stage_addr));
+  const int lane = threadIdx.x & 31;
+  constexpr int CB = 128 / sizeof(T);  // columns of a segment
+  if (p.out32) {
+    const uint32_t o = mine ? node * p.out_n32 + m * p.out_m32 : NO_ROW;
+    T* const to = static_cast<T*>(p.out) + c0 + lane;
+    // (unrolled whole: the values of many rows are read before the first is stored.  600 000 bf16 rows of 97 -> 61,
+    // fwd: 103 us, by 8 rows 134; fp32 dx: 135, by 8 146)
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+      const uint32_t ro = __shfl_sync(0xffffffffu, o, r);
+#pragma unroll
+      for (int c = 0; c < CB; c += 32) {
+        const int byte = (c + lane) * (int)sizeof(T);
+        const T v = load_as<T>(stage + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15)));
+        if (ro != NO_ROW && c + lane < left) to[ro + (uint32_t)c] = v;
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int r = 0; r < 32; ++r) {
+      const bool in = __shfl_sync(0xffffffffu, mine, r);
+      const int64_t ro = __shfl_sync(0xffffffffu, node, r) * p.out_sn + __shfl_sync(0xffffffffu, m, r) * p.out_sm;
+      for (int c = lane; c < left && c < CB; c += 32) {
+        const int byte = c * (int)sizeof(T);
+        if (in)
+          (static_cast<T*>(p.out) + ro + c0)[c] =
+              load_as<T>(stage + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15)));
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void copy_out(const SlParams& p, const uint8_t* stage, const RowRef& ref, bool mine, int c0,
+                                         int left) {
   int row = threadIdx.x & 31;
   asm volatile("" : "+r"(row));  // addresses are made here each time: held across the tiles they crowd the registers
   __syncwarp();
   if (p.vst) {
     // 4 rows x 128 bytes per instruction
+    const uint32_t o = mine ? ref.node * p.out_n32 + ref.m * p.out_m32 : NO_ROW;
     const int j = row & 7;
     const bool have = left * (int)sizeof(T) > 16 * j;
     char* const to = static_cast<char*>(p.out) + (int64_t)c0 * sizeof(T) + 16 * j;
@@ -514,24 +563,14 @@ __device__ __forceinline__ void copy_out(const SlParams& p, const uint8_t* stage
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // (r & 7 alternates between lane / 8 and lane / 8 + 4)
         v[i] = load_as<uint4>(src + (i0 + i) * 512 + ((j ^ ((row >> 3) + (i & 1) * 4)) << 4));
-        ro[i] = __shfl_sync(0xffffffffu, o16, (i0 + i) * 4 + (row >> 3));
+        ro[i] = __shfl_sync(0xffffffffu, o, (i0 + i) * 4 + (row >> 3));
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (ro[i] != NO_ROW && have) *reinterpret_cast<uint4*>(to + (uint64_t)ro[i] * 16) = v[i];
     }
   } else {
-    // unaligned rows: element by element, neighbouring lanes on neighbouring columns
-#pragma unroll 4
-    for (int r = 0; r < 32; ++r) {
-      const int64_t ro = __shfl_sync(0xffffffffu, o, r);
-#pragma unroll
-      for (int c = 0; c < 128 / (int)sizeof(T); c += 32) {
-        const int byte = (c + row) * (int)sizeof(T);
-        const T v = load_as<T>(stage + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15)));
-        if (ro >= 0 && c + row < left) (static_cast<T*>(p.out) + ro + c0)[c + row] = v;
-      }
-    }
+    copy_out_any<T>(p, tc::smem_u32(stage), ref.node, ref.m, mine, c0, left);
   }
   __syncwarp();
 }
@@ -597,23 +636,24 @@ __device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int s) {
                     __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }
 
-constexpr int SL_IMG = 128 * 128;  // bytes of one piece of a B image: up to 128 rows of 64 bf16
+constexpr int SL_IMG = 128 * 128;  // bytes of one piece of a B image of up to 128 rows of 64 bf16
 
-// 8 K-values of row n of a B image: their bf16 pieces
+// 8 K-values of row n of a B image: their bf16 pieces, `piece` bytes apart
 template <int P>
-__device__ __forceinline__ void put_eight(uint8_t* img, int n, int chunk, const float* v) {
+__device__ __forceinline__ void put_eight(uint8_t* img, int piece, int n, int chunk, const float* v) {
   uint32_t t[4][3];
 #pragma unroll
   for (int q = 0; q < 4; ++q) split2<P>(v[2 * q], v[2 * q + 1], t[q]);
 #pragma unroll
   for (int b = 0; b < P; ++b)
-    store_piece(img + b * SL_IMG + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
+    store_piece(img + b * piece + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
 }
 
-// Where weight (k, n) of a step waits, as it is, in its own image slot: 64 columns (one round of the rewriting)
-// apart from the other 64, where the images of the first round are not written.
+// Where weight (k, n) of a step waits, as it is, in its own image slot.  More than 64 columns are rewritten in two
+// rounds of 64: the second 64 wait where the images of the first are not written.
 template <typename T>
-__device__ __forceinline__ uint32_t raw_place(int k, int n, bool transposed) {
+__device__ __forceinline__ uint32_t raw_place(int k, int n, bool transposed, int NT) {
+  if (NT <= 64) return (transposed ? n * SL_KC + k : k * NT + n) * (int)sizeof(T);
   if (sizeof(T) == 2) return transposed ? n * 128 + k * 2 : (n >> 6) * 8192 + k * 128 + (n & 63) * 2;
   return transposed ? ((n >> 5) & 1) * 16384 + (n >> 6) * 8192 + (n & 31) * 256 + k * 4
                     : (k >> 5) * 16384 + (n >> 6) * 8192 + (k & 31) * 256 + (n & 63) * 4;
@@ -655,7 +695,7 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint8_t* img0, i
 #pragma unroll 8
       for (; r < rows && on; r += 4 * rpi, src += hop) {
         const bool in = r0 + r < r_end && c0 < c_end;
-        cp_async16_or_zero(raw + raw_place<T>(p.transposed ? c : r, p.transposed ? r : c, p.transposed), in ? src : wt,
+        cp_async16_or_zero(raw + raw_place<T>(p.transposed ? c : r, p.transposed ? r : c, p.transposed, NT), in ? src : wt,
                            !in);
       }
     }
@@ -673,12 +713,13 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint8_t* img0, i
       for (int u = 0; u < 4; ++u) {
         const int j = h * 16 + u * 4 + w4;
         const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane, kk = (p.transposed ? lane & 7 : j & 7) * 8;
+        if (n >= NT) continue;
         if (p.w_vec) {
           if (p.transposed) {
-            load_eight(img + raw_place<T>(kk, n, true), v[u], T{});
+            load_eight(img + raw_place<T>(kk, n, true, NT), v[u], T{});
           } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[u][e] = load_f32<T>(img + raw_place<T>(kk + e, n, false));
+            for (int e = 0; e < 8; ++e) v[u][e] = load_f32<T>(img + raw_place<T>(kk + e, n, false, NT));
           }
         } else {
           const int col = ct * NT + n, k = (k0 + s) * SL_KC + kk;
@@ -697,7 +738,7 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint8_t* img0, i
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[u][e] *= p.alpha;
         }
-        if (n < NT) put_eight<PB>(img, n, p.transposed ? lane & 7 : j & 7, v[u]);
+        if (n < NT) put_eight<PB>(img, p.img, n, p.transposed ? lane & 7 : j & 7, v[u]);
       }
     }
     tc::fence_proxy_async();
@@ -723,8 +764,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   auto D_FULL = [&](int s) { return bar(4 + s); };
   auto D_FREE = [&](int s) { return bar(6 + s); };
   auto B_FULL = [&](int s) { return bar(8 + s); };
-  auto B_FREE = [&](int s) { return bar(8 + S::NSLOT + s); };
-  const uint32_t DONE = bar(8 + 2 * S::NSLOT), W_SYNC = bar(9 + 2 * S::NSLOT);
+  auto B_FREE = [&](int s) { return bar(8 + S::MAX_SLOTS + s); };
+  const uint32_t DONE = bar(8 + 2 * S::MAX_SLOTS), W_SYNC = bar(9 + 2 * S::MAX_SLOTS);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be uniform
 
@@ -743,7 +784,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         tc::mbar_init(D_FULL(s), 1);
         tc::mbar_init(D_FREE(s), 256);
       }
-      for (int s = 0; s < S::NSLOT; ++s) {
+      for (int s = 0; s < S::MAX_SLOTS; ++s) {
         tc::mbar_init(B_FULL(s), WG ? NT : 128);
         tc::mbar_init(B_FREE(s), 1);
       }
@@ -776,7 +817,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   }
   const int wg_k0 = WG ? (tile / p.n_ct) * 128 : 0, wg_n0 = WG ? (tile % p.n_ct) * p.NT : 0;
   const int n_k = WG ? 1 : (p.K + SL_KC - 1) / SL_KC;  // steps of a tile
-  const bool resident = n_k <= S::NSLOT;               // map: the weight images of a tile stay for the next row tile
+  const int img = WG ? SL_IMG : p.img, slots = WG ? 2 : p.slots;
+  const bool resident = n_k <= slots;               // map: the weight images of a tile stay for the next row tile
   const uint32_t tmem = SL_D;  // an allocation of all 512 columns starts at column 0
 
   // MMAs of step `it` with the images of slot bs, by one elected thread; `use`: how often the slot was filled
@@ -793,7 +835,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     if (first && sn >= 2 && !wait_phase(D_FREE(sn & 1), ((sn >> 1) - 1) & 1, abort)) return false;
     tc::fence_after_sync();
     const uint32_t dcol = SL_D + (sn & 1) * 128;
-    const uint32_t blo = (uint32_t)tc::sw128_desc(base + bs * (PB * SL_IMG));
+    const uint32_t blo = (uint32_t)tc::sw128_desc(base + bs * (PB * img));
     // (the stage as a constant: little is left to compute)
     auto emit = [&](auto stage) {
       constexpr uint32_t st = decltype(stage)::value;
@@ -801,7 +843,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
       for (int q = 0; q < PR::n; ++q)
 #pragma unroll
         for (int ks = 0; ks < SL_KC / 16; ++ks)
-          mma_bf16_ta(dcol, SL_A + st * (PA * 32) + PR::a(q) * 32 + ks * 8, blo + PR::b(q) * (SL_IMG / 16) + ks * 2, bhi,
+          mma_bf16_ta(dcol, SL_A + st * (PA * 32) + PR::a(q) * 32 + ks * 8, blo + PR::b(q) * (img / 16) + ks * 2, bhi,
                       idesc, !first || q > 0 || ks > 0);
     };
     if (s)
@@ -843,13 +885,16 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     };
     // the loaded rows become the fetched ones.  Map: a row outside the tile may hold anything (its
     // TMEM lane is never stored), so it stands for row 0; weight gradient: it must be zero
+    uint32_t here = 0;  // weight gradient: which rows of the unit exist
     auto take_rows = [&]() {
       const bool ok = ref.valid(p);
-      const int64_t o = ok ? ref.offset(p.a) : 0;
-      if constexpr (VEC)
-        spread_rows<S::SEG_A>(WG && !ok ? NO_ROW : (uint32_t)(o >> 4), off);
-      else
+      if constexpr (VEC) {
+        if constexpr (WG) here = __ballot_sync(0xffffffffu, ok);
+        spread_rows<S::SEG_A>(ok ? ref.pieces(p.a) : 0u, off);
+      } else {
+        const int64_t o = ok ? ref.offset(p.a) : 0;
         row = WG && !ok ? nullptr : p.a.data + o;
+      }
     };
     auto fetch = [&]() {
       if (left > 0) {
@@ -866,7 +911,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         const uint32_t dst = ring + slot_f * S::UNIT_A;
         const int at = WG ? (wg_k0 + warp * 32) * (int)sizeof(TA) : fu * 128;
         if constexpr (VEC)
-          fetch_vec<S::SEG_A, S::PITCH_A, !WG, WG>(dst, p.a.data, off, at, row_bytes);
+          fetch_vec<S::SEG_A, S::PITCH_A, !WG, WG>(dst, p.a.data, off, here, at, row_bytes);
         else
           fetch_any<S::SEG_A, S::PITCH_A>(dst, p.a.data, row, at, row_bytes, mis + slot_f * 32);
         slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
@@ -974,7 +1019,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
       if constexpr (!WG) {
         int syncs = 0;
         auto fill = [&](int g, int ct, int k0, int nk, int slot0) -> bool {
-          return fill_weights<T, PB>(p, smem + slot0 * PB * SL_IMG, PB * SL_IMG, g, ct, k0, nk, bar(8 + slot0), W_SYNC,
+          return fill_weights<T, PB>(p, smem + slot0 * PB * img, PB * img, g, ct, k0, nk, bar(8 + slot0), W_SYNC,
                                      syncs, abort);
         };
         Walk w;
@@ -999,7 +1044,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
             w.t += run - 1;
           } else {
             for (int k = 0; k < n_k && ok; ++k, ++it, ++fills) {
-              const int s = fills % S::NSLOT, use = fills / S::NSLOT;
+              const int s = fills % slots, use = fills / slots;
               ok = use == 0 || wait_phase(B_FREE(s), (use - 1) & 1, abort);
               ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, k, 1, s);
               if (ok && warp == 4 && elect_one())
@@ -1032,14 +1077,14 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
             if (!second) rows.step(p, q, t1);
             const RowRef ref = second ? rows.now[1] : rows.now[0];
             const bool in = ref.valid(p);
-            const int64_t o = in ? ref.offset(p.b) : 0;
             const uint32_t dst = ring + slot_f * S::UNIT_B;
             if constexpr (VEC) {
               uint32_t off[Pieces<S::SEG_B>::N];
-              spread_rows<S::SEG_B>(in ? (uint32_t)(o >> 4) : NO_ROW, off);
-              fetch_vec<S::SEG_B, S::PITCH_B, false, true>(dst, p.b.data, off, at, row_bytes);
+              spread_rows<S::SEG_B>(in ? ref.pieces(p.b) : 0u, off);
+              fetch_vec<S::SEG_B, S::PITCH_B, false, true>(dst, p.b.data, off, __ballot_sync(0xffffffffu, in), at,
+                                                           row_bytes);
             } else {
-              fetch_any<S::SEG_B, S::PITCH_B>(dst, p.b.data, in ? p.b.data + o : nullptr, at, row_bytes,
+              fetch_any<S::SEG_B, S::PITCH_B>(dst, p.b.data, in ? p.b.data + ref.offset(p.b) : nullptr, at, row_bytes,
                                               mis + slot_f * 32);
             }
             if constexpr (sizeof(TA) == 1) {
@@ -1078,7 +1123,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
               v[j] = load_f32<T>(src + r * S::PITCH_B + (VEC ? 0 : ms[r]));
               if constexpr (sizeof(TA) == 1) v[j] *= ss[r];
             }
-            put_eight<PB>(img, n, u * 4 + q, v);
+            put_eight<PB>(img, SL_IMG, n, u * 4 + q, v);
           }
           if (u == 1) {
             tc::fence_proxy_async();
@@ -1162,9 +1207,6 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         // against 1500 staged).
         constexpr int CB = 128 / sizeof(T);  // columns of a 128-byte row segment
         const bool mine = ref.valid(p);
-        const int64_t o = mine ? ref.node * p.out_sn + ref.m * p.out_sm : -1;
-        // aligned rows: offsets in 16 bytes
-        const uint32_t o16 = mine ? (uint32_t)((uint64_t)o * sizeof(T) >> 4) : NO_ROW;
         uint8_t* const stage = smem + S::OFF_STG + (warp - 8) * S::STG;
         if constexpr (PB == 1) {
 #pragma unroll
@@ -1191,7 +1233,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
             store_piece(stage + row * 128 + ((j ^ (row & 7)) << 4), w4[0], w4[1], w4[2], w4[3]);
           }
           __syncwarp();
-          copy_out<T>(p, stage, o, o16, c0 + b, left);
+          copy_out<T>(p, stage, ref, mine, c0 + b, left);
           __syncwarp();
         }
         fresh = true;
@@ -1327,6 +1369,25 @@ int vector_bytes(const void* ptr, int64_t s0, int64_t s1, int64_t s2) {
   return 0;
 }
 
+RowView row_view(const void* data, int64_t sn, int64_t sm, int width, int size) {
+  return {static_cast<const char*>(data), sn * size, sm * size, width, (uint32_t)(sn * size / 16),
+          (uint32_t)(sm * size / 16)};
+}
+
+// x / d for x < 2^31: x times ceil(2^(31 + s) / d), 2^(s - 1) < d <= 2^s, shifted by 31 + s
+void set_divisor(SlParams* p, int d) {
+  int s = 1;
+  while ((1 << s) < d) ++s;
+  p->div_mul = (uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d);
+  p->div_shift = s - 1;
+}
+
+// weight images of a step that fit the map's shared memory at NT columns and `pieces` pieces, and a piece's bytes
+int image_slots(int NT, int pieces, int* img) {
+  *img = NT > 64 ? SL_IMG : NT * 128;
+  return std::min(8, (pieces == 3 ? 2 * 3 : 4) * SL_IMG / (pieces * *img));
+}
+
 bool aligned_rows(const RowView& v, int64_t n, int d, int size) {
   // (row offsets in 16 bytes fit 32 bits)
   return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && v.width * size % 16 == 0 && (n <= 1 || v.sn % 16 == 0) && (d <= 1 || v.sm % 16 == 0) &&
@@ -1377,37 +1438,51 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int es = dtype == MACE_F32 ? 4 : 2;
   SlParams p{};
-  p.a = {static_cast<const char*>(x), xn * es, xm * es, K};
+  p.a = row_view(x, xn, xm, K, es);
   p.w = w;
   p.transposed = transpose;
   p.out = y;
   p.out_sn = yn;
   p.out_sm = ym;
   // (as for the input: whole 16-byte pieces, offsets in 32 bits)
-  p.vst = aligned_rows({static_cast<const char*>(y), yn * es, ym * es, M}, n, d, es);
+  const RowView out = row_view(y, yn, ym, M, es);
+  p.vst = aligned_rows(out, n, d, es);
+  p.out32 = (n - 1) * yn + (d - 1) * ym + M < (int64_t)NO_ROW;
+  p.out_n32 = p.vst ? out.sn16 : (uint32_t)yn;
+  p.out_m32 = p.vst ? out.sm16 : (uint32_t)ym;
   p.order = order;
   p.offsets = offsets;
   p.n = n;
   p.d = d;
   p.G = G;
+  set_divisor(&p, d);
   p.K = K;
   p.N = M;
   p.w_vec = (transpose ? K : M) * es % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
   p.alpha = alpha;
+  const bool vec = aligned_rows(p.a, n, d, es), direct = dtype == MACE_BF16 && vec && p.w_vec;
   const int sms = sm_count();
   const int64_t row_tiles = (n * d + 127) / 128;
   // narrower column tiles while the row tiles leave SMs idle
   int most = 128;
   while (most > 32 && row_tiles * ((M + most - 1) / most) * 2 <= sms) most /= 2;
+  // and so narrow that the weight images of the whole K stay in shared memory (K <= 512), rather than being made
+  // anew for every tile (256 -> 256 fp32 channels, 300k rows: 646 us)
+  const int n_k = (K + SL_KC - 1) / SL_KC, pieces = dtype == MACE_F32 ? 3 : 1;
+  if (!direct) {
+    int fit = most;
+    while (fit > 32 && n_k > image_slots(tile_cols(M, fit), pieces, &p.img)) fit /= 2;
+    if (n_k <= image_slots(tile_cols(M, fit), pieces, &p.img)) most = fit;
+  }
   p.NT = tile_cols(M, most);
+  p.slots = image_slots(p.NT, pieces, &p.img);
   p.n_ct = (M + p.NT - 1) / p.NT;
   p.n_kt = 1;
   const int grid = (int)std::min<int64_t>(sms, (row_tiles + std::min<int64_t>(G, n)) * p.n_ct);
-  const bool vec = aligned_rows(p.a, n, d, es);
+  if (direct) return launch_direct<false>(p, grid, s);  // bf16 in whole pieces: nothing to convert
   if (dtype == MACE_F32)
     return vec ? launch_gemm<float, float, false, true>(p, grid, s) : launch_gemm<float, float, false, false>(p, grid, s);
-  // bf16 in whole pieces: nothing to convert
-  return vec && p.w_vec ? launch_direct<false>(p, grid, s) : launch_gemm<bf16, bf16, false, false>(p, grid, s);
+  return launch_gemm<bf16, bf16, false, false>(p, grid, s);
 }
 
 extern "C" int mace_species_linear_wgrad_workspace(int64_t n, int32_t d, int32_t G, int32_t K, int32_t M,
@@ -1434,8 +1509,9 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int es = dtype == MACE_F32 ? 4 : 2, xe = xs ? 1 : es;
   SlParams p{};
-  p.a = {static_cast<const char*>(x), xn * xe, xm * xe, K};
-  p.b = {static_cast<const char*>(dy), yn * es, ym * es, M};
+  p.a = row_view(x, xn, xm, K, xe);
+  p.b = row_view(dy, yn, ym, M, es);
+  set_divisor(&p, d);
   p.a_scale = xs;
   p.ka_blocks = (K + MACE_CHECKPOINT_BLOCK - 1) / MACE_CHECKPOINT_BLOCK;
   p.out = dw;
