@@ -28,15 +28,29 @@ struct RowDiv {
 RowDiv row_div(int C) { return {(uint32_t)((((uint64_t)1 << 32) + C - 1) / C), C == 1 ? 1u : 0u}; }
 
 // Grouping is a stable counting sort by the key (species, or num_groups for
-// padding rows), with one digit of the key per pass.  A pass counts the digits
-// of every CTA's tile, scans the counts, and scatters: each warp ranks its rows
-// among equal digits with match_any, the tile is put in digit order in shared
-// memory, and runs of equal digits are written together.  Ranks follow the
-// list order everywhere, so the order of atomics plays no part.
-constexpr int GR_THREADS = 256;
-constexpr int GR_WARPS = GR_THREADS / 32;
-constexpr int GR_TILE = 2048;      // rows of one CTA of a counting pass (a pass is a chain of latencies: many small CTAs)
-constexpr int GR_MAX_BINS = 1024;  // digits of one pass
+// padding rows): one pass for keys of up to 13 bits, else two passes over half
+// the bits each.  A pass counts the digits of every CTA's share of the list,
+// scans the counts over the CTAs, and scatters: a warp takes consecutive rows,
+// ranks them among equal digits with ballots and moves its own counter of the
+// digit on (16 bits in shared memory: a share has fewer rows).  Ranks follow
+// the list order everywhere, so the order of atomics plays no part.
+//
+// 4M rows, 7921 groups: 49 us, of which the scatter is two thirds, bound by its
+// 4-byte stores (a sector each) and the chain from counter to counter; in two
+// passes of 7 bits, put in digit order in shared memory before they are
+// stored, 98 us.  1000 groups: 38 us (89 in two passes); 89 groups: 36 us (40).
+// 16 000 groups take two passes (101 us): the counters of 14 bits would leave
+// shared memory for 5 warps.
+constexpr int GR_THREADS = 1024;  // of the counting and scanning CTAs
+constexpr int GR_MAX_BITS = 13;   // digit of one pass: the counters of 12 warps fill the shared memory
+constexpr int GR_CTAS = 148;      // one per SM
+template <int BITS>
+struct GroupCfg {
+  static constexpr int BINS = 1 << BITS, WORDS = BINS / 2;
+  static constexpr int WARPS = BITS == 13 ? 12 : (BITS == 12 ? 24 : 32), THREADS = WARPS * 32;
+  static constexpr int BYTES = (BINS + WARPS * WORDS + 32) * 4;
+  static_assert(BYTES <= 232448, "shared memory of a CTA");
+};
 // short lists: one CTA does the whole sort in one launch
 constexpr int GS_THREADS = 1024;
 constexpr int GS_MAX_ROWS = 8192;
@@ -46,68 +60,63 @@ constexpr int GS_MAX_BINS = 256;  // (shared memory of a static size)
 __device__ __forceinline__ int row_key(int32_t z, int G) { return (z >= 0 && z < G) ? z : G; }
 
 struct GroupPass {
-  const int32_t* key;   // species (first pass) or keys sorted by the lower digit
-  const int32_t* row;   // null in the first pass: row i is i
+  const int32_t* species;
+  const int2* in;       // second pass: (key, row) sorted by the lower digit; null in the first: row i is i
   int64_t n;
   int G;
   int shift, bits;
-  int nb;               // CTAs
-  int32_t* counts;      // (bins, nb), after the scan exclusive within a digit
+  int share, nb;        // rows of a CTA (a multiple of its threads, below 2^16), CTAs
+  int32_t* counts;      // (nb, bins), after the scan exclusive within a digit
   int32_t* totals;      // (bins)
-  int32_t* key_out;     // null in a single pass
-  int32_t* row_out;
+  int2* out;            // first pass of two: (key, row), one scattered store; else null
+  int32_t* order;
   int32_t* offsets;     // single pass: the group offsets; else null
 };
 
-__device__ __forceinline__ int digit_of(const GroupPass& p, int32_t z) {
-  return (row_key(z, p.G) >> p.shift) & ((1 << p.bits) - 1);
+__device__ __forceinline__ int key_of(const GroupPass& p, int64_t i) {
+  return p.in ? p.in[i].x : row_key(p.species[i], p.G);
 }
+__device__ __forceinline__ int digit_of(const GroupPass& p, int key) { return (key >> p.shift) & ((1 << p.bits) - 1); }
 
 __global__ void __launch_bounds__(GR_THREADS) k_group_count(GroupPass p) {
-  pdl_wait();
-  __shared__ int hist[GR_MAX_BINS];
+  __shared__ int hist[1 << GR_MAX_BITS];
   const int bins = 1 << p.bits;
   for (int b = threadIdx.x; b < bins; b += GR_THREADS) hist[b] = 0;
+  pdl_wait();
   __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * GR_TILE;
-#pragma unroll
-  for (int j = 0; j < GR_TILE / GR_THREADS; ++j) {
-    const int64_t i = i0 + j * GR_THREADS + threadIdx.x;
-    if (i < p.n) atomicAdd(&hist[digit_of(p, p.key[i])], 1);
-  }
+  const int64_t i0 = blockIdx.x * (int64_t)p.share;
+  const int rows = (int)imin64(p.share, p.n - i0);
+#pragma unroll 8
+  for (int i = threadIdx.x; i < rows; i += GR_THREADS) atomicAdd(&hist[digit_of(p, key_of(p, i0 + i))], 1);
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += GR_THREADS) p.counts[(int64_t)b * p.nb + blockIdx.x] = hist[b];
+  for (int b = threadIdx.x; b < bins; b += GR_THREADS) p.counts[(int64_t)blockIdx.x * bins + b] = hist[b];
 }
 
-// exclusive sums of one digit's counts over the CTAs, in place, and their total: a CTA per digit
+// exclusive sums of the counts of 32 digits over the CTAs, in place, and their totals: a lane per digit, each warp a
+// run of CTAs
 __global__ void __launch_bounds__(GR_THREADS) k_group_scan(GroupPass p) {
   pdl_wait();
-  __shared__ int sums[GR_WARPS];
-  int32_t* c = p.counts + (int64_t)blockIdx.x * p.nb;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int carry = 0;
-  for (int base = 0; base < p.nb; base += GR_THREADS) {
-    const int i = base + threadIdx.x;
-    const int v = i < p.nb ? c[i] : 0;
-    int s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-    if (lane == 31) sums[warp] = s;
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < GR_WARPS; ++w) {
-      if (w < warp) before += sums[w];
-      all += sums[w];
-    }
-    if (i < p.nb) c[i] = carry + before + s - v;
-    carry += all;
-    __syncthreads();
+  __shared__ int sums[32][33];
+  const int bins = 1 << p.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.x * 32 + lane;
+  const int per = (p.nb + 31) / 32, c0 = warp * per, c1 = min(p.nb, c0 + per);
+  int32_t* const c = p.counts + b;
+  int sum = 0;
+  if (b < bins)
+#pragma unroll 8
+    for (int k = c0; k < c1; ++k) sum += c[(int64_t)k * bins];
+  sums[warp][lane] = sum;
+  __syncthreads();
+  int at = 0;
+  for (int w = 0; w < warp; ++w) at += sums[w][lane];
+  if (b >= bins) return;
+  if (warp == 31) p.totals[b] = at + sum;
+#pragma unroll 8
+  for (int k = c0; k < c1; ++k) {
+    const int v = c[(int64_t)k * bins];
+    c[(int64_t)k * bins] = at;
+    at += v;
   }
-  if (threadIdx.x == 0) p.totals[blockIdx.x] = carry;
 }
 
 // exclusive sums over `count` values of a CTA's threads, thread by thread: value v, result returned
@@ -128,11 +137,10 @@ __device__ __forceinline__ int cta_exclusive(int v, int* warp_sums) {
   return before + s - v;
 }
 
-// Place of this lane's row among its warp's rows of the same digit: `count` holds how many came before, and is moved
-// on.  Lanes of equal digit find one another bit by bit with ballots (match_any on spread digits costs several times
-// as much: a pass over 4M rows took 56 us with it).
+// The lanes (of those with `in`) whose digit is this lane's.  They find one another bit by bit with ballots (match_any
+// on spread digits costs several times as much).
 template <int BITS>
-__device__ __forceinline__ int place(int* count, int digit, bool in, int lane) {
+__device__ __forceinline__ unsigned same_digit(int digit, bool in) {
   unsigned same = __ballot_sync(0xffffffffu, in);
 #pragma unroll
   for (int b = 0; b < BITS; ++b) {
@@ -140,98 +148,139 @@ __device__ __forceinline__ int place(int* count, int digit, bool in, int lane) {
     const unsigned m = __ballot_sync(0xffffffffu, one);
     same &= one ? m : ~m;
   }
+  return same;
+}
+
+// Place of this lane's row among its warp's rows of the same digit: `count` holds how many came before, and is moved
+// on.
+template <typename C>
+__device__ __forceinline__ int place(C* count, int digit, bool in, unsigned same, int lane) {
   const int rank = __popc(same & ((1u << lane) - 1));
   const int before = in ? count[digit] : 0;
   __syncwarp();
-  if (in && rank == 0) count[digit] = before + __popc(same);
+  if (in && rank == 0) count[digit] = (C)(before + __popc(same));
   __syncwarp();
   return before + rank;
 }
 
-struct ScatterSmem {
-  int32_t key[GR_TILE], row[GR_TILE];
-  int sums[GR_WARPS];
-};
-int scatter_bytes(int bins) { return (int)sizeof(ScatterSmem) + (GR_WARPS + 2) * bins * 4; }
+// The same in a packed 16-bit counter, for digits that seldom meet within a warp: every row counts itself, and only
+// where two met (a counter is then further on than its own addition) are the lanes of equal digit found.
+template <int BITS>
+__device__ __forceinline__ int place_spread(uint32_t* pos, int digit, bool in, int lane) {
+  const int half = 16 * (digit & 1);
+  uint32_t before = 0, after = 0;
+  if (in) before = atomicAdd(&pos[digit >> 1], 1u << half) >> half & 0xffffu;
+  __syncwarp();
+  if (in) after = *reinterpret_cast<volatile uint32_t*>(&pos[digit >> 1]) >> half & 0xffffu;
+  __syncwarp();
+  if (!__any_sync(0xffffffffu, in && after != before + 1)) return before;
+  const unsigned same = same_digit<BITS>(digit, in);
+  return after - __popc(same) + __popc(same & ((1u << lane) - 1));
+}
 
 template <int BITS>
-__global__ void __launch_bounds__(GR_THREADS, 5) k_group_scatter(GroupPass p) {
-  pdl_wait();
+__global__ void __launch_bounds__(GroupCfg<BITS>::THREADS, 1) k_group_scatter(GroupPass p) {
+  using Cfg = GroupCfg<BITS>;
+  constexpr int BINS = Cfg::BINS, WORDS = Cfg::WORDS, WARPS = Cfg::WARPS, THREADS = Cfg::THREADS;
   extern __shared__ int32_t dyn[];
-  ScatterSmem& sm = *reinterpret_cast<ScatterSmem*>(dyn);
-  constexpr int BINS = 1 << BITS;
-  int* const whist = dyn + sizeof(ScatterSmem) / 4;  // (GR_WARPS, BINS): a warp's counts, then its first local positions
-  int* const lstart = whist + GR_WARPS * BINS;       // digit totals
-  int* const gstart = lstart + BINS;                 // a digit's first position in the result, less its first local one
+  int* const base = dyn;                                           // a digit's first position of this CTA
+  uint32_t* const pos = reinterpret_cast<uint32_t*>(dyn + BINS);   // (WARPS, BINS) of 16 bits: counts, then positions
+  int* const sums = dyn + BINS + WARPS * WORDS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int SEG = GR_TILE / GR_WARPS;  // consecutive rows of one warp
-  const int64_t i0 = (int64_t)blockIdx.x * GR_TILE + warp * SEG, i1 = imin64(p.n, i0 + SEG);
-  int* const mine = whist + warp * BINS;
-  auto digit = [&](int32_t key) { return (key >> p.shift) & (BINS - 1); };
-  // every global load of the CTA's input first
-  int32_t z[SEG / 32], row[SEG / 32];
+  for (int k = tid; k < WARPS * WORDS; k += THREADS) pos[k] = 0;
+  pdl_wait();
+  // totals and this CTA's counts of a run of PER digits per thread
+  constexpr int PER = (BINS + THREADS - 1) / THREADS;
+  int total[PER], before[PER];
 #pragma unroll
-  for (int j = 0; j < SEG / 32; ++j) {
-    const int64_t i = i0 + j * 32 + lane;
-    z[j] = i < i1 ? row_key(p.key[i], p.G) : 0;
-    row[j] = p.row && i < i1 ? p.row[i] : (int32_t)i;
+  for (int k = 0; k < PER; ++k) {
+    const int b = tid * PER + k;
+    total[k] = b < BINS ? p.totals[b] : 0;
+    before[k] = b < BINS ? p.counts[(int64_t)blockIdx.x * BINS + b] : 0;
   }
-  for (int b = tid; b < BINS; b += GR_THREADS) {
-    lstart[b] = p.totals[b];
-    gstart[b] = p.counts[(int64_t)b * p.nb + blockIdx.x];
-  }
-  for (int b = tid; b < GR_WARPS * BINS; b += GR_THREADS) whist[b] = 0;
   __syncthreads();
-  int rel[SEG / 32];  // place within the warp's rows of the digit
+  const int seg = p.share / WARPS;  // consecutive rows of one warp
+  const int64_t i0 = blockIdx.x * (int64_t)p.share + warp * seg;
+  const int rows = (int)max(imin64(seg, p.n - i0), (int64_t)0);
+  uint32_t* const mine = pos + warp * WORDS;
+#pragma unroll 8
+  for (int i = lane; i < rows; i += 32) {
+    const int d = digit_of(p, key_of(p, i0 + i));
+    atomicAdd(&mine[d >> 1], 1u << (16 * (d & 1)));
+  }
+  int sum = 0;
 #pragma unroll
-  for (int j = 0; j < SEG / 32; ++j) rel[j] = place<BITS>(mine, digit(z[j]), i0 + j * 32 + lane < i1, lane);
-  __syncthreads();
-  // digits in runs of PER per thread: local starts and starts in the result
-  constexpr int PER = (BINS + GR_THREADS - 1) / GR_THREADS;
-  int local = 0, global = 0;
+  for (int k = 0; k < PER; ++k) sum += total[k];
+  sum = cta_exclusive<THREADS>(sum, sums);
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int b = tid * PER + k;
     if (b >= BINS) break;
-#pragma unroll
-    for (int w = 0; w < GR_WARPS; ++w) local += whist[w * BINS + b];
-    global += lstart[b];
+    if (p.offsets && blockIdx.x == 0 && b <= p.G) p.offsets[b] = sum;
+    base[b] = sum + before[k];
+    sum += total[k];
   }
-  int ls = cta_exclusive<GR_THREADS>(local, sm.sums);
-  int gs = cta_exclusive<GR_THREADS>(global, sm.sums);
+  // (cta_exclusive's barriers stand between the counts and this)
+  for (int k = tid; k < WORDS; k += THREADS) {  // two digits at a time: neither half overflows
+    uint32_t at = 0;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int b = tid * PER + k;
-    if (b >= BINS) break;
-    if (p.offsets && blockIdx.x == 0 && b <= p.G) p.offsets[b] = gs;
-    gstart[b] += gs - ls;
-    gs += lstart[b];
-#pragma unroll
-    for (int w = 0; w < GR_WARPS; ++w) {
-      const int c = whist[w * BINS + b];
-      whist[w * BINS + b] = ls;
-      ls += c;
+    for (int w = 0; w < WARPS; ++w) {
+      const uint32_t c = pos[w * WORDS + k];
+      pos[w * WORDS + k] = at;
+      at += c;
     }
   }
   __syncthreads();
+  constexpr int U = 4;  // rounds of 32 rows in flight
+  // (4M rows of 7921 groups 49 us, by ballots alone 55; of 4000 39 against 42, of 1000 no difference)
+  constexpr bool SPREAD = BITS >= 12;
+  uint16_t* const mine16 = reinterpret_cast<uint16_t*>(mine);
+  int z[U], r[U];
+  auto load = [&](int i) {
 #pragma unroll
-  for (int j = 0; j < SEG / 32; ++j) {
-    if (i0 + j * 32 + lane < i1) {
-      const int at = mine[digit(z[j])] + rel[j];
-      sm.key[at] = z[j];
-      sm.row[at] = row[j];
+    for (int u = 0; u < U; ++u) {
+      const int k = i + u * 32 + lane;
+      int2 v = make_int2(0, (int)(i0 + k));
+      if (k < rows) {
+        if (p.in)
+          v = p.in[i0 + k];
+        else
+          v.x = p.species[i0 + k];  // (its key is taken when it is used: nothing waits for the load here)
+      }
+      z[u] = v.x, r[u] = v.y;
     }
-  }
-  __syncthreads();
-  const int rows = (int)imin64(GR_TILE, p.n - (int64_t)blockIdx.x * GR_TILE);
+  };
+  load(0);
+#pragma unroll 1
+  for (int i = 0; i < rows; i += U * 32) {
+    int k0[U], r0[U];
 #pragma unroll
-  for (int j = 0; j < GR_TILE / GR_THREADS; ++j) {
-    const int i = j * GR_THREADS + tid;
-    if (i >= rows) break;
-    const int32_t key = sm.key[i];
-    const int at = gstart[digit(key)] + i;
-    p.row_out[at] = sm.row[i];
-    if (p.key_out) p.key_out[at] = key;
+    for (int u = 0; u < U; ++u) {
+      k0[u] = p.in ? z[u] : row_key(z[u], p.G);
+      r0[u] = r[u];
+    }
+    load(i + U * 32);
+    unsigned same[U];
+    if constexpr (!SPREAD) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) same[u] = same_digit<BITS>(digit_of(p, k0[u]), i + u * 32 + lane < rows);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = i + u * 32 + lane < rows;
+      const int d = digit_of(p, k0[u]);
+      int at = base[d];
+      if constexpr (SPREAD)
+        at += place_spread<BITS>(mine, d, in, lane);
+      else
+        at += place(mine16, d, in, same[u], lane);
+      if (in) {
+        if (p.out)
+          p.out[at] = make_int2(k0[u], r0[u]);
+        else
+          p.order[at] = r0[u];
+      }
+    }
   }
 }
 
@@ -252,7 +301,10 @@ __global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __res
   __syncwarp();
 #pragma unroll
   for (int j = 0; j < MOST; ++j)
-    if (j < rounds) rel[j] = place<BITS>(whist[warp], key[j], i0 + j * 32 + lane < i1, lane);
+    if (j < rounds) {
+      const bool in = i0 + j * 32 + lane < i1;
+      rel[j] = place(whist[warp], key[j], in, same_digit<BITS>(key[j], in), lane);
+    }
   __syncthreads();
   int total = 0;
   if (tid < (1 << BITS))
@@ -276,25 +328,23 @@ __global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __res
   }
 }
 
-// offsets[v] = first position whose key is >= v; four positions per thread (key is 16-byte aligned)
-__global__ void __launch_bounds__(256) k_group_offsets(const int32_t* __restrict__ key, int64_t n, int G,
+// Two passes: offsets[v] = first position of the order whose key is >= v, a thread per offset (a pass over the keys that writes an offset where
+// the key changes leaves one thread all the writes of a long run of empty groups)
+__global__ void __launch_bounds__(256) k_group_offsets(const int32_t* __restrict__ species,
+                                                       const int32_t* __restrict__ order, int64_t n, int G,
                                                        int32_t* __restrict__ offsets) {
   pdl_wait();
-  const int64_t i0 = (blockIdx.x * (int64_t)256 + threadIdx.x) * 4;
-  if (i0 > n) return;
-  int k[5];
-  k[0] = i0 > 0 ? key[i0 - 1] : -1;
-  if (i0 + 4 <= n) {
-    const int4 v = *reinterpret_cast<const int4*>(key + i0);
-    k[1] = v.x, k[2] = v.y, k[3] = v.z, k[4] = v.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) k[j + 1] = i0 + j < n ? key[i0 + j] : G;
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v > G) return;
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (row_key(species[order[mid]], G) < v)
+      lo = mid + 1;
+    else
+      hi = mid;
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (i0 + j <= n)
-      for (int v = k[j] + 1; v <= k[j + 1]; ++v) offsets[v] = (int32_t)(i0 + j);
+  offsets[v] = (int32_t)lo;
 }
 
 // Consecutive vectors of V elements of the (n, C) result, CTA by CTA.
@@ -676,7 +726,7 @@ __global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* __restrict
 void group_passes(int G, int* bits, int* passes) {
   int b = 1;
   while ((1 << b) < G + 1) ++b;
-  *passes = b <= 10 ? 1 : 2;
+  *passes = b <= GR_MAX_BITS ? 1 : 2;
   *bits = (b + *passes - 1) / *passes;
 }
 
@@ -704,18 +754,24 @@ int with_bits(int bits, F&& f) {
 }
 
 struct GroupPlan {
-  int bits, passes, nb;
+  int bits, passes, share, nb;
   bool small;  // one CTA, one launch, no workspace
-  int64_t counts, keys, bytes;  // bytes of the count tables, of one key or row array, and of the whole workspace
+  int64_t counts, pairs, bytes;  // bytes of the count tables, of the (key, row) pairs between two passes, and of the whole
 };
 bool group_plan(int64_t n, int32_t G, GroupPlan* p) {
   if (n < 0 || n > INT32_MAX || G < 1 || G > MACE_SPECIES_MAX_INDEX) return false;
   group_passes(G, &p->bits, &p->passes);
-  p->nb = (int)((n + GR_TILE - 1) / GR_TILE);
+  // two rounds of a CTA's warps at least, and no counter of 16 bits overflows
+  int64_t step = 0;
+  with_bits<GR_MAX_BITS>(p->bits, [&](auto bits) {
+    step = GroupCfg<decltype(bits)::value>::THREADS;
+    return 0;
+  });
+  p->share = (int)(std::min(std::max((n + GR_CTAS * step - 1) / (GR_CTAS * step), (int64_t)2), 65535 / step) * step);
+  p->nb = (int)((n + p->share - 1) / p->share);
   p->counts = align16(((int64_t)p->nb + 1) * (1 << p->bits) * 4);
-  p->keys = align16(n * 4);
-  // two passes: keys and rows after the first, keys after the second
-  p->bytes = p->counts + (p->passes > 1 ? 3 * p->keys : 0);
+  p->pairs = align16(n * 8);
+  p->bytes = p->counts + (p->passes > 1 ? p->pairs : 0);
   p->small = n <= GS_MAX_ROWS && G < GS_MAX_BINS;
   if (p->small) p->bytes = 0;
   return true;
@@ -752,41 +808,40 @@ extern "C" int mace_species_group(const int32_t* species, int64_t n, int32_t G, 
   p.n = n;
   p.G = G;
   p.bits = plan.bits;
+  p.share = plan.share;
   p.nb = plan.nb;
   const int bins = 1 << plan.bits;
   char* at = static_cast<char*>(ws);
   p.counts = reinterpret_cast<int32_t*>(at);
   p.totals = p.counts + (int64_t)bins * p.nb;
-  int32_t* key1 = reinterpret_cast<int32_t*>(at + plan.counts);
-  int32_t* row1 = reinterpret_cast<int32_t*>(at + plan.counts + plan.keys);
-  int32_t* key2 = reinterpret_cast<int32_t*>(at + plan.counts + 2 * plan.keys);
+  int2* const pairs = reinterpret_cast<int2*>(at + plan.counts);
+  p.species = species;
+  p.order = order;
   for (int q = 0; q < plan.passes; ++q) {
     const bool last = q == plan.passes - 1;
     p.shift = q * plan.bits;
-    p.key = q == 0 ? species : key1;
-    p.row = q == 0 ? nullptr : row1;
-    p.key_out = plan.passes == 1 ? nullptr : (last ? key2 : key1);
-    p.row_out = last ? order : row1;
+    p.in = q == 0 ? nullptr : pairs;
+    p.out = last ? nullptr : pairs;
     p.offsets = plan.passes == 1 ? offsets : nullptr;
     int rc = launch("group_count", k_group_count, p.nb, GR_THREADS, 0, s, p);
-    if (!rc) rc = launch("group_scan", k_group_scan, bins, GR_THREADS, 0, s, p);
+    if (!rc) rc = launch("group_scan", k_group_scan, (bins + 31) / 32, GR_THREADS, 0, s, p);
     if (!rc)
-      rc = with_bits<10>(plan.bits, [&](auto bits) {
+      rc = with_bits<GR_MAX_BITS>(plan.bits, [&](auto bits) {
         constexpr int B = decltype(bits)::value;
         static bool attr_set[64] = {};  // per device: the attribute call is slow on the host
         int dev = 0;
         MACE_CUDA_TRY(cudaGetDevice(&dev));
         if (dev >= 64 || !attr_set[dev]) {
           MACE_CUDA_TRY(cudaFuncSetAttribute(k_group_scatter<B>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             scatter_bytes(1 << B)));
+                                             GroupCfg<B>::BYTES));
           if (dev < 64) attr_set[dev] = true;
         }
-        return launch("group_scatter", k_group_scatter<B>, p.nb, GR_THREADS, scatter_bytes(1 << B), s, p);
+        return launch("group_scatter", k_group_scatter<B>, p.nb, GroupCfg<B>::THREADS, GroupCfg<B>::BYTES, s, p);
       });
     if (rc) return rc;
   }
   if (plan.passes == 1) return MACE_OK;
-  return launch("group_offsets", k_group_offsets, (unsigned)((n + 1024) / 1024), 256, 0, s, key2, n, G, offsets);
+  return launch("group_offsets", k_group_offsets, (unsigned)(G / 256 + 1), 256, 0, s, species, order, n, G, offsets);
 }
 
 namespace {

@@ -107,6 +107,26 @@ def test_grouping_of_many_rows(sp):
                                                        out_int32=True))
 
 
+@pytest.mark.parametrize("n,g,used", [
+    (30_001, 4095, 4095),    # the last group count of a 12-bit pass
+    (30_001, 4096, 4096),    # the first of 13 bits
+    (50_001, 8191, 8191),    # the last count of one pass
+    (50_001, 8192, 8192),    # the first of two
+    (50_001, 8191, 3),       # equal digits in every warp where they are expected to differ
+    (50_001, 5000, 1),
+    (9, 8191, 8191),         # fewer rows than a warp
+    (10_000_019, 8191, 8191),  # the longest share of a CTA
+    (10_000_019, 2, 1),
+])  # fmt: skip
+def test_grouping_at_the_limits_of_a_pass(sp, n, g, used):
+    z = draw_species(n, g, n, pad=0.05, only=None if used == g else list(range(g - used, g)))
+    got = sp.group_species(z, g)
+    key, order = torch.sort(torch.where(valid(z, g), z, g), stable=True)
+    assert torch.equal(got.order, order.int())
+    assert torch.equal(got.offsets, torch.searchsorted(key, torch.arange(g + 1, device="cuda", dtype=torch.int32),
+                                                       out_int32=True))
+
+
 # ----------------------------------------------------------------- embedding
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,c", [(1, 1), (7, 3), (1000, 128), (333, 97), (65, 256), (130, 300), (2000, 8)])
