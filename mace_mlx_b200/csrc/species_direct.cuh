@@ -31,7 +31,7 @@ struct Dr {
   static constexpr int STG = 32 * 128;             // map: an epilogue warp's staging
   static constexpr int OFF_STG = OFF_W + NW * A;
   static constexpr int OFF_PRE = OFF_STG + (WG ? 0 : 8 * STG);
-  static constexpr int OFF_BAR = OFF_PRE + (3 * MACE_SPECIES_MAX_GROUPS + 2) * 4;
+  static constexpr int OFF_BAR = OFF_PRE + Groups::INTS * 4;
   static constexpr int NBAR = 2 * DR_NS + 4 + 8 + 1;
   static constexpr int BYTES = OFF_BAR + NBAR * 8 + 16;
   static_assert(BYTES <= 232448, "shared memory of a CTA");
@@ -61,8 +61,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
   using S = Dr<WG>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = tc::smem_u32(smem);
-  int* const pre = reinterpret_cast<int*>(smem + S::OFF_PRE);
-  const Groups q{pre, pre + MACE_SPECIES_MAX_GROUPS + 2, pre + 2 * MACE_SPECIES_MAX_GROUPS + 2};
+  const Groups q(smem + S::OFF_PRE);
+  const int* const pre = q.pre;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + S::NBAR);
   volatile int* const abort = reinterpret_cast<int*>(tslot + 1);
@@ -106,19 +106,16 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
   }
   pdl_wait();  // nothing of the caller's is read or written before
   tc::fence_before_sync();
-  load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, q, reinterpret_cast<int64_t*>(smem));
+  const int tiles = WG ? p.n_ct * p.n_kt : 1;  // units and shares as in k_species_gemm
+  const int share = WG ? blockIdx.x / tiles : blockIdx.x;
+  const int tile = WG ? blockIdx.x % tiles : 0;
+  load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, WG ? 0 : p.start, share, WG ? p.shares : gridDim.x, WG, q,
+              reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
   const uint32_t tmem = *tslot;
   if (WG && blockIdx.x == 0)
     for (int i = tid; i <= p.G; i += SL_THREADS) p.units[i] = pre[i];
-  // this CTA's share of the units, as in k_species_gemm
-  const int total = pre[p.G];
-  const int tiles = WG ? p.n_ct * p.n_kt : 1;
-  const int nshare = WG ? min(p.shares, total) : gridDim.x;
-  const int share = WG ? blockIdx.x / tiles : blockIdx.x;
-  const int tile = WG ? blockIdx.x % tiles : 0;
-  const int t0 = share < nshare ? (int)((int64_t)share * total / nshare) : 0;
-  const int t1 = share < nshare ? (int)((int64_t)(share + 1) * total / nshare) : 0;
+  const int t0 = q.bounds[0], t1 = q.bounds[1];
   if (t0 >= t1) {
     if (!WG && warp >= 5 && warp < 8) zero_rows<bf16>(p);
     if (warp == 15) tc::tmem_dealloc(tmem, DR_TMEM);

@@ -83,6 +83,7 @@ struct SlParams {
   int K, N;             // map: K summed channels, N outputs; weight gradient: K x N of dW
   int w_vec;            // map: rows of the weights are 16-byte aligned
   int NT;               // tile columns: 32, 64, 96 or 128
+  int start;            // map: what the weight images of a group cost, in half row tiles
   int img, slots;       // map: bytes of one piece of a weight image, slots for the images of a step
   int n_ct, n_kt;       // column tiles; weight gradient: row (channel) tiles
   int shares;           // weight gradient: CTAs along the rows
@@ -298,6 +299,18 @@ struct Products<1, 1> {
   __device__ static constexpr int b(int) { return 0; }
 };
 
+// The groups in shared memory: units of group g are [pre[g], pre[g + 1]), its rows [lo[g], hi[g]) of `order`.
+struct Groups {
+  int *pre, *lo, *hi;
+  int* bounds;  // this CTA's units
+  static constexpr int INTS = 3 * MACE_SPECIES_MAX_GROUPS + 4;
+  __device__ __forceinline__ explicit Groups(void* at)
+      : pre(static_cast<int*>(at)),
+        lo(pre + MACE_SPECIES_MAX_GROUPS + 2),
+        hi(lo + MACE_SPECIES_MAX_GROUPS),
+        bounds(hi + MACE_SPECIES_MAX_GROUPS) {}
+};
+
 // ------------------------------------------------------------------ layout
 // TA: stored type of A's rows, T: type of the parameters and of B, WG: weight gradient
 template <typename TA, typename T, bool WG, bool VEC>
@@ -321,38 +334,74 @@ struct Sl {
   static constexpr int OFF_MIS = OFF_STG + (WG ? 0 : 8 * STG);        // per ring unit and row: misalignment
   static constexpr int OFF_SCALE = OFF_MIS + (VEC ? 0 : (WG ? 8 : 4) * NU * 32);  // per B ring unit and row: A's scale
   static constexpr int OFF_PRE = OFF_SCALE + (sizeof(TA) == 1 ? 4 * NU * 32 * 4 : 0);
-  static constexpr int OFF_BAR = OFF_PRE + (3 * MACE_SPECIES_MAX_GROUPS + 2) * 4;
+  static constexpr int OFF_BAR = OFF_PRE + Groups::INTS * 4;
   static constexpr int NBAR = 8 + 2 * MAX_SLOTS + 2;
   static constexpr int BYTES = OFF_BAR + NBAR * 8 + 32;
   static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
 
-// The groups in shared memory: units of group g are [pre[g], pre[g + 1]), its rows [lo[g], hi[g]) of `order`.
-struct Groups {
-  int *pre, *lo, *hi;
-};
+// x k / n; 64-bit division is slow
+__device__ __forceinline__ int64_t part(int64_t x, int k, int n) {
+  return x < (1 << 22) && n < (1 << 10) ? (int64_t)((uint32_t)x * (uint32_t)k / (uint32_t)n) : x * k / n;
+}
 
-// fills them, by the whole CTA (G <= 512 = SL_THREADS)
-__device__ __forceinline__ void load_groups(const SlParams& p, int unit_rows, int per_unit, const Groups& q,
-                                            int64_t* warp_sums) {
+// Fills them, by the whole CTA (G <= 512 = SL_THREADS), and finds this CTA's units [t0, t1): the share-th of `shares`
+// of the whole, or of min(shares, units) with `each` (no share without a unit between two that have some).  `start`:
+// what a group costs beside its units, in half units (once for each of `runs` equal runs of its units); shares are
+// equal in that sum, floor(share * sum / shares) on.
+__device__ __forceinline__ void load_groups(const SlParams& p, int unit_rows, int runs, int start, int share,
+                                            int shares, bool each, const Groups& q, int64_t* warp_sums) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t s = 0;
+  int64_t s = 0, mine = 0, per = 0;  // units of the groups up to this one, its own, those of a run
+  int some = 0;  // groups up to this one that have rows
   if (tid < p.G) {
     const Range r = group_range(p.offsets, tid, p.n);
     q.lo[tid] = (int)r.lo;
     q.hi[tid] = (int)r.hi;
-    s = ((r.hi - r.lo) * p.d + unit_rows - 1) / unit_rows * per_unit;
+    per = ((r.hi - r.lo) * p.d + unit_rows - 1) / unit_rows;
+    s = mine = per * runs;
   }
+  const unsigned have = __ballot_sync(0xffffffffu, mine > 0);
+  some = __popc(have & (0xffffffffu >> (31 - lane)));
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
     if (lane >= o) s += u;
   }
   if (lane == 31) warp_sums[warp] = s;
+  if (lane == 31) warp_sums[16 + warp] = some;
+  if (tid < 2) q.bounds[tid] = 0;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) s += warp_sums[w];
+  int64_t all = 0, all_some = 0;
+#pragma unroll
+  for (int w = 0; w < SL_THREADS / 32; ++w) {
+    if (w < warp) {
+      s += warp_sums[w];
+      some += (int)warp_sums[16 + w];
+    }
+    all += warp_sums[w];
+    all_some += warp_sums[16 + w];
+  }
   if (tid < p.G) q.pre[tid + 1] = (int)min(s, (int64_t)INT32_MAX);  // beyond it: offsets that overlap
   if (tid == 0) q.pre[0] = 0;
+  const int scale = start ? 2 : 1;
+  const int64_t cost = scale * all + (int64_t)start * runs * all_some;
+  if (each) shares = (int)min((int64_t)shares, all);
+  if (mine > 0 && share < shares) {
+    // the group in which a bound lies says which unit it is
+    const int64_t c0 = scale * (s - mine) + (int64_t)start * runs * (some - 1);  // where the group starts
+    const int64_t len = scale * per + start;                                      // of a run
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t x = part(cost, share + k, shares) - c0;
+      if (x >= 0 && x < len * runs) {
+        const int run = runs == 1 ? 0 : (int)(x / len);
+        const int64_t unit = s - mine + run * per + (max(x - run * len - start, (int64_t)0) + scale - 1) / scale;
+        q.bounds[k] = (int)min(unit, (int64_t)INT32_MAX);
+      }
+    }
+    if (share + 1 == shares && s == all) q.bounds[1] = (int)min(all, (int64_t)INT32_MAX);
+  }
   __syncthreads();
 }
 
@@ -753,8 +802,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   constexpr int PA = S::PA, PB = S::PB, NU = S::NU;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = tc::smem_u32(smem);
-  int* const pre = reinterpret_cast<int*>(smem + S::OFF_PRE);
-  const Groups q{pre, pre + MACE_SPECIES_MAX_GROUPS + 2, pre + 2 * MACE_SPECIES_MAX_GROUPS + 2};
+  const Groups q(smem + S::OFF_PRE);
+  const int* const pre = q.pre;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + S::NBAR);
   volatile int* const abort = reinterpret_cast<int*>(tslot + 1);
@@ -798,18 +847,17 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   }
   pdl_wait();  // nothing of the caller's is read or written before
   tc::fence_before_sync();
-  load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, q, reinterpret_cast<int64_t*>(smem));
+  // unit: map: a row tile of a (group, column tile); weight gradient: 64 rows.  blockIdx.x of the weight gradient:
+  // share * tiles + tile
+  const int tiles = WG ? p.n_ct * p.n_kt : 1;
+  const int share = WG ? blockIdx.x / tiles : blockIdx.x;
+  const int tile = WG ? blockIdx.x % tiles : 0;
+  load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, WG ? 0 : p.start, share, WG ? p.shares : gridDim.x, WG, q,
+              reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
   if (WG && blockIdx.x == 0)
     for (int i = tid; i <= p.G; i += SL_THREADS) p.units[i] = pre[i];
-  // this CTA's share of the units; weight gradient: blockIdx.x = share * tiles + tile
-  const int total = pre[p.G];
-  const int tiles = WG ? p.n_ct * p.n_kt : 1;
-  const int nshare = WG ? min(p.shares, total) : gridDim.x;  // no share without a unit between two that have some
-  const int share = WG ? blockIdx.x / tiles : blockIdx.x;
-  const int tile = WG ? blockIdx.x % tiles : 0;
-  const int t0 = share < nshare ? (int)((int64_t)share * total / nshare) : 0;
-  const int t1 = share < nshare ? (int)((int64_t)(share + 1) * total / nshare) : 0;
+  const int t0 = q.bounds[0], t1 = q.bounds[1];
   if (t0 >= t1) {
     if (!WG && warp >= 5 && warp < 8) zero_rows<T>(p);
     if (warp == 15) tc::tmem_dealloc(SL_D, SL_TMEM);
@@ -1478,6 +1526,10 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.slots = image_slots(p.NT, pieces, &p.img);
   p.n_ct = (M + p.NT - 1) / p.NT;
   p.n_kt = 1;
+  // Making a group's images (9 000 cycles) costs about as much as 1.5 row tiles.  40 000 rows of 4 species 128 -> 128
+  // fp32 26.5 us without it, 20.7 with 2 to 6; 600 000 rows 133, 130.4 with 4, 129.1 with 6.  bf16 rows copied as they
+  // lie (direct): no difference.
+  p.start = !direct && n_k <= p.slots ? 4 : 0;
   const int grid = (int)std::min<int64_t>(sms, (row_tiles + std::min<int64_t>(G, n)) * p.n_ct);
   if (direct) return launch_direct<false>(p, grid, s);  // bf16 in whole pieces: nothing to convert
   if (dtype == MACE_F32)
