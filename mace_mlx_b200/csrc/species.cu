@@ -792,6 +792,8 @@ extern "C" int mace_species_group(const int32_t* species, int64_t n, int32_t G, 
   GroupPlan plan;
   if (!group_plan(n, G, &plan) || !offsets || (n > 0 && (!species || !order)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_group: bad arguments");
+  if (unaligned(4, species, order, offsets))
+    return fail(MACE_ERR_BAD_ARG, "mace_species_group: an address is not a multiple of its values' size");
   if (plan.bytes > 0 && (!ws || ws_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(ws) & 15) != 0))
     return fail(MACE_ERR_BAD_ARG, "mace_species_group: workspace too small or not 16-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -879,6 +881,8 @@ extern "C" int mace_species_embed(int32_t dtype, const void* table, int64_t ts, 
       n < 0 || n > INT32_MAX || ts < 0 ||
       !table || (n > 0 && (!species || !out || os < C)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_embed: bad arguments");
+  if (unaligned(value_size(dtype), table, out) || unaligned(4, species))
+    return fail(MACE_ERR_BAD_ARG, "mace_species_embed: an address is not a multiple of its values' size");
   if (n == 0) return MACE_OK;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return dtype == MACE_F32 ? embed<float>(table, ts, G, C, species, n, scale, out, os, s)
@@ -931,6 +935,8 @@ extern "C" int mace_species_embed_grad(int32_t dtype, const void* grad, int64_t 
       C > MACE_SPECIES_MAX_CHANNELS || gs < 0 || !out ||
       !offsets || (n > 0 && (!grad || !order)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_embed_grad: bad arguments");
+  if (unaligned(value_size(dtype), grad, out) || unaligned(4, order, offsets, ws))
+    return fail(MACE_ERR_BAD_ARG, "mace_species_embed_grad: an address is not a multiple of its values' size");
   int64_t need = 0;
   mace_species_embed_grad_workspace(n, G, C, &need);
   if (need > 0 && (!ws || ws_bytes < need))
@@ -946,6 +952,8 @@ extern "C" int mace_rows_checkpoint(int32_t dtype, const void* x, int64_t xn, in
   if (bad_dtype(dtype) || n < 0 || n > INT32_MAX || d < 1 || d > 1024 || C < 1 || C > MACE_SPECIES_MAX_CHANNELS || xn < 0 || xm < 0 ||
       (n > 0 && (!x || !q || !scale)))
     return fail(MACE_ERR_BAD_ARG, "mace_rows_checkpoint: bad arguments");
+  if (unaligned(value_size(dtype), x) || unaligned(4, scale))
+    return fail(MACE_ERR_BAD_ARG, "mace_rows_checkpoint: an address is not a multiple of its values' size");
   if (n == 0) return MACE_OK;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int nb = (C + MACE_CHECKPOINT_BLOCK - 1) / MACE_CHECKPOINT_BLOCK;
@@ -968,6 +976,8 @@ extern "C" int mace_rows_restore(int32_t dtype, const int8_t* q, const float* sc
   if (bad_dtype(dtype) || n < 0 || n > INT32_MAX || d < 1 || d > 1024 || C < 1 ||
       C > MACE_SPECIES_MAX_CHANNELS || (n > 0 && (!x || !q || !scale)))
     return fail(MACE_ERR_BAD_ARG, "mace_rows_restore: bad arguments");
+  if (unaligned(value_size(dtype), x) || unaligned(4, scale))
+    return fail(MACE_ERR_BAD_ARG, "mace_rows_restore: an address is not a multiple of its values' size");
   if (n == 0) return MACE_OK;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int nb = (C + MACE_CHECKPOINT_BLOCK - 1) / MACE_CHECKPOINT_BLOCK;

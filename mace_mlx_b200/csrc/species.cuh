@@ -18,6 +18,11 @@ __device__ __forceinline__ void pdl_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// an address that is not a multiple of its values' size
+template <typename... P>
+bool unaligned(int size, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) % size != 0) || ...); }
+inline int value_size(int32_t dtype) { return dtype == MACE_F32 ? 4 : 2; }
+
 template <typename... P, typename... A>
 int launch(const char* name, void (*kernel)(P...), dim3 grid, unsigned threads, unsigned smem, cudaStream_t s, A... args) {
   cudaLaunchConfig_t cfg{};

@@ -86,15 +86,15 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
     if (lane == 0) {
       *abort = 0;
       for (int s = 0; s < DR_NS; ++s) {
-        tc::mbar_init(FULL(s), WG ? 256 : 128);
+        tc::mbar_init(FULL(s), WG ? 8 : 4);
         tc::mbar_init(FREE(s), 1);
       }
       for (int s = 0; s < 2; ++s) {
         tc::mbar_init(D_FULL(s), 1);
-        tc::mbar_init(D_FREE(s), 256);
+        tc::mbar_init(D_FREE(s), 8);
       }
       for (int s = 0; s < 4; ++s) {
-        tc::mbar_init(W_FULL(s), 128);
+        tc::mbar_init(W_FULL(s), 4);
         tc::mbar_init(W_FREE(s), 1);
       }
       tc::mbar_init(DONE, 1);
@@ -106,10 +106,10 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
   }
   pdl_wait();  // nothing of the caller's is read or written before
   tc::fence_before_sync();
-  const int tiles = WG ? p.n_ct * p.n_kt : 1;  // units and shares as in k_species_gemm
+  const int tiles = WG ? p.n_ct * p.n_kt : 1;  // units and shares as in k_species_map and k_species_wgrad
   const int share = WG ? blockIdx.x / tiles : blockIdx.x;
   const int tile = WG ? blockIdx.x % tiles : 0;
-  load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, WG ? 0 : p.start, share, WG ? p.shares : gridDim.x, WG, q,
+  load_groups<SL_THREADS>(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, WG ? 0 : p.start, share, WG ? p.shares : gridDim.x, WG, q,
               reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
   const uint32_t tmem = *tslot;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
   // copies of step i were issued in the i-th commit group of this thread: hand the step on once they have landed
   auto hand_on = [&](int i) {
     tc::fence_proxy_async();
-    tc::mbar_arrive(FULL(i % DR_NS));
+    warp_arrive(FULL(i % DR_NS));
   };
   auto ring_loop = [&](auto&& copy) {
     bool ok = true;
@@ -168,11 +168,11 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
       ring_loop([&](uint32_t dst) {
         if (k == 0) {
           // (a row outside the tile may hold anything: its TMEM lane is never stored)
-          spread_rows<128>(ref.valid(p) ? ref.pieces(p.a) : 0u, off);
+          spread_rows(ref.valid(p) ? ref.pieces(p.a) : 0u, off);
           w.next(q, t1);
           if (w.t < t1) load_tile();
         }
-        fetch_vec<128, 128, true, false>(dst + w4 * 4096, p.a.data, off, 0, k * 128, p.a.width * 2);
+        fetch_vec(dst + w4 * 4096, p.a.data, off, k * 128, p.a.width * 2);
         if (++k == n_k) k = 0;
       });
     } else {
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
       }
     };
     const uint32_t idesc = idesc_bf16(NT) | (p.transposed ? 0u : 1u << 16);  // B's major
-    // step `it`, the first (and last) of its tile or not, with the weights of slot ws; use: as in k_species_gemm
+    // step `it`, the first (and last) of its tile or not, with the weights of slot ws; use: as in k_species_map
     auto issue = [&](int it, int tile_no, bool first, bool last, int ws, int use, bool release) -> bool {
       const int s = it % DR_NS, ds = tile_no & 1;
       if (use >= 0 && !wait_phase(W_FULL(ws), use & 1, abort)) return false;
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
         cp_commit();
         cp_wait<0>();
         tc::fence_proxy_async();
-        for (int k = 0; k < n_k; ++k) tc::mbar_arrive(W_FULL(k));
+        for (int k = 0; k < n_k; ++k) warp_arrive(W_FULL(k));
         if (warp == 4 && elect_one())
           for (int i = 0; i < run && ok; ++i)
             for (int k = 0; k < n_k && ok; ++k)
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
           cp_commit();
           cp_wait<0>();
           tc::fence_proxy_async();
-          tc::mbar_arrive(W_FULL(s));
+          warp_arrive(W_FULL(s));
           if (warp == 4 && elect_one()) ok = issue(it, tile_no, k == 0, k + 1 == n_k, s, use, true);
           ok = __all_sync(0xffffffffu, ok);
         }
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
           tc::tmem_wait_ld();
           if (h == 3) {
             tc::fence_before_sync();
-            tc::mbar_arrive(D_FREE(s));
+            warp_arrive(D_FREE(s));
           }
           if (h * 16 < CW) {
             uint32_t o[8];
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
           tc::tmem_wait_ld();
           if (h == 3) {
             tc::fence_before_sync();
-            tc::mbar_arrive(D_FREE(s));
+            warp_arrive(D_FREE(s));
           }
 #pragma unroll
           for (int k = 0; k < 16; k += 2) add2(acc[h * 16 + k], acc[h * 16 + k + 1], v[k], v[k + 1]);
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
         const bool group_ends = w.t + len == pre[w.g + 1];
         if (group_ends || w.t + len == t1) {
           finish_wgrad<bf16>(p, acc, w.g, group_ends && pre[w.g] >= t0, tile, share, wg_k0, wg_n0, quad * 32 + lane,
-                             half * CW);
+                             half * CW, CW);
           fresh = true;
         }
         advance(w, len);
@@ -461,15 +461,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
 
 template <bool WG>
 int launch_direct(const SlParams& p, int grid, cudaStream_t s) {
-  constexpr int BYTES = Dr<WG>::BYTES;
-  static bool attr_set[64] = {};  // per device: the attribute call is slow on the host
-  int dev = 0;
-  MACE_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev >= 64 || !attr_set[dev]) {
-    MACE_CUDA_TRY(cudaFuncSetAttribute(k_species_direct<WG>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
-    if (dev < 64) attr_set[dev] = true;
-  }
-  return launch("species_direct", k_species_direct<WG>, grid, SL_THREADS, BYTES, s, p);
+  static bool attr_set[64] = {};
+  return launch_big("species_direct", k_species_direct<WG>, attr_set, grid, SL_THREADS, Dr<WG>::BYTES, s, p);
 }
 
 }  // namespace

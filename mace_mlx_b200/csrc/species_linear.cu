@@ -15,19 +15,18 @@
 // steps in fp32 registers (bf16 alone, whose result is rounded to 2^-9, takes
 // several steps).
 //
-// Roles of a CTA (16 warps, one CTA per SM, a contiguous share of the tiles):
+// Roles of a CTA of the map (16 warps, one CTA per SM, a share of the tiles of equal cost):
 //   warps 0-3   operand A: own 32 TMEM lanes each, fetch their rows with 16-byte
 //               cp.async through a private ring (gathered by `order`), split
 //               them in registers and store them to TMEM
-//   warps 4-7   operand B: weights (map) or dy rows (weight gradient) into
-//               128B-swizzled K-major shared-memory images
+//   warps 4-7   operand B: the weights into 128B-swizzled K-major shared-memory
+//               images, kept while the tiles share them; warp 4 issues the MMAs
+//               (a 17th warp would cut every thread to 96 registers)
 //   warps 8-15  epilogue: TMEM -> fp32 registers -> memory
-//   the MMAs are issued by warp 4 (map: its weight images rarely change) or
-//   warp 8 (weight gradient: it stores only at a group's end); a 17th warp
-//   would cut every thread to 96 registers
 // handing over through mbarriers only.  Every wait is bounded (about 2 s): one
 // that gives up raises the CTA's abort flag, which ends every other wait, and
-// TC_ERR_TIMEOUT in g_species_error.
+// TC_ERR_TIMEOUT in g_species_error.  species_wgrad.cuh has the weight
+// gradient, species_direct.cuh both for bf16 rows that need no conversion.
 //
 // Rows may start at any alignment: a segment is fetched as the 16-byte units
 // that contain it (its end clipped by the copy's source size) and shifted when
@@ -46,6 +45,7 @@ namespace {
 
 constexpr int SL_THREADS = 16 * 32;
 constexpr int SL_KC = 64;              // K of one accumulation step
+constexpr int SL_IMG = 128 * 128;      // bytes of one piece of a B image of up to 128 rows of 64 bf16
 constexpr int SL_LONG = 8;             // weight gradient of bf16: steps accumulated in TMEM
 constexpr int SL_D = 0;                // TMEM columns: two accumulators of 128
 constexpr int SL_A = 256;              // then two A stages
@@ -127,6 +127,13 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t phase, volatil
   return tc::mbar_wait_or_abort(bar, phase, abort);
 }
 
+// One arrival for what the lanes of a warp have done (each behind its own fence where another proxy reads it).  An
+// arrival by every thread queues on the barrier.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) tc::mbar_arrive(bar);
+}
+
 // true on one lane of a converged warp; the compiler knows the branch is uniform
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -141,6 +148,9 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // 16 bytes, or zeros
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool zero) {
   asm volatile(
@@ -152,6 +162,9 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -224,7 +237,8 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t* out) {
     for (int k = 0; k < 3; ++k) {
       const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
       out[k] = __byte_perm(u0, u1, 0x7632);
-      if (k < 2) sub2(x0, x1, u0 & 0xffff0000u, u1 & 0xffff0000u);
+      // (the first value's piece back by a multiplication: masks and permutes share one pipe, half as wide)
+      if (k < 2) sub2(x0, x1, out[k] * 65536u, u1 & 0xffff0000u);
     }
   }
 }
@@ -312,28 +326,20 @@ struct Groups {
 };
 
 // ------------------------------------------------------------------ layout
-// TA: stored type of A's rows, T: type of the parameters and of B, WG: weight gradient
-template <typename TA, typename T, bool WG, bool VEC>
+template <typename T, bool VEC>
 struct Sl {
-  static constexpr int PA = sizeof(TA) == 4 ? 3 : 1;
-  static constexpr int PB = sizeof(TA) == 2 ? 1 : 3;
-  static constexpr bool LONG = PA == 1 && PB == 1;  // sums of several steps (the result is rounded to 2^-9)
-  static constexpr int SEG_A = WG ? 32 * (int)sizeof(TA) : 128;  // bytes of a row in one ring unit of 32 rows
-  static constexpr int SEG_B = 32 * (int)sizeof(T);
-  static constexpr int PITCH_A = SEG_A + (VEC ? 0 : 16), PITCH_B = SEG_B + (VEC ? 0 : 16);
-  static constexpr int UPC = WG ? 2 : SL_KC * (int)sizeof(TA) / 128;  // ring units per step of 64
-  static constexpr int NU = WG ? (VEC ? 4 : 3) : 5;
-  static constexpr int NU_B = VEC && PA == 3 ? 3 : NU;  // (a fourth unit of fp32 rows would not fit)
-  static constexpr int UNIT_A = 32 * PITCH_A, UNIT_B = 32 * PITCH_B;
-  static constexpr int IMAGES = (!WG && PB == 1 ? 4 : 2) * PB * 128 * 128;  // bytes of all B images
-  static constexpr int MAX_SLOTS = WG ? 2 : 8;
-  static constexpr int OFF_A = IMAGES;
-  static constexpr int OFF_B = OFF_A + 4 * NU * UNIT_A;
-  static constexpr int STG = 32 * 128;  // map: an epilogue warp's staging, 32 rows x 128 bytes
-  static constexpr int OFF_STG = OFF_B + (WG ? 4 * NU_B * UNIT_B : 0);
-  static constexpr int OFF_MIS = OFF_STG + (WG ? 0 : 8 * STG);        // per ring unit and row: misalignment
-  static constexpr int OFF_SCALE = OFF_MIS + (VEC ? 0 : (WG ? 8 : 4) * NU * 32);  // per B ring unit and row: A's scale
-  static constexpr int OFF_PRE = OFF_SCALE + (sizeof(TA) == 1 ? 4 * NU * 32 * 4 : 0);
+  static constexpr int P = sizeof(T) == 4 ? 3 : 1;  // pieces of a value
+  static constexpr bool LONG = P == 1;              // sums of a whole tile (the result is rounded to 2^-9)
+  static constexpr int PITCH = 128 + (VEC ? 0 : 16);  // of a ring unit: 32 rows x 128 bytes
+  static constexpr int UPC = SL_KC * (int)sizeof(T) / 128;  // ring units per step of 64
+  static constexpr int NU = 5;
+  static constexpr int UNIT = 32 * PITCH;
+  static constexpr int MAX_SLOTS = 8;
+  static constexpr int OFF_A = (P == 3 ? 6 : 4) * SL_IMG;  // after the weight images
+  static constexpr int STG = 32 * 128;                     // an epilogue warp's staging, 32 rows x 128 bytes
+  static constexpr int OFF_STG = OFF_A + 4 * NU * UNIT;
+  static constexpr int OFF_MIS = OFF_STG + 8 * STG;  // per ring unit and row: misalignment
+  static constexpr int OFF_PRE = OFF_MIS + (VEC ? 0 : 4 * NU * 32);
   static constexpr int OFF_BAR = OFF_PRE + Groups::INTS * 4;
   static constexpr int NBAR = 8 + 2 * MAX_SLOTS + 2;
   static constexpr int BYTES = OFF_BAR + NBAR * 8 + 32;
@@ -345,10 +351,11 @@ __device__ __forceinline__ int64_t part(int64_t x, int k, int n) {
   return x < (1 << 22) && n < (1 << 10) ? (int64_t)((uint32_t)x * (uint32_t)k / (uint32_t)n) : x * k / n;
 }
 
-// Fills them, by the whole CTA (G <= 512 = SL_THREADS), and finds this CTA's units [t0, t1): the share-th of `shares`
+// Fills them, by the whole CTA (G <= 512 threads), and finds this CTA's units [t0, t1): the share-th of `shares`
 // of the whole, or of min(shares, units) with `each` (no share without a unit between two that have some).  `start`:
 // what a group costs beside its units, in half units (once for each of `runs` equal runs of its units); shares are
 // equal in that sum, floor(share * sum / shares) on.
+template <int THREADS>
 __device__ __forceinline__ void load_groups(const SlParams& p, int unit_rows, int runs, int start, int share,
                                             int shares, bool each, const Groups& q, int64_t* warp_sums) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -369,18 +376,18 @@ __device__ __forceinline__ void load_groups(const SlParams& p, int unit_rows, in
     if (lane >= o) s += u;
   }
   if (lane == 31) warp_sums[warp] = s;
-  if (lane == 31) warp_sums[16 + warp] = some;
+  if (lane == 31) warp_sums[32 + warp] = some;
   if (tid < 2) q.bounds[tid] = 0;
   __syncthreads();
   int64_t all = 0, all_some = 0;
 #pragma unroll
-  for (int w = 0; w < SL_THREADS / 32; ++w) {
+  for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) {
       s += warp_sums[w];
-      some += (int)warp_sums[16 + w];
+      some += (int)warp_sums[32 + w];
     }
     all += warp_sums[w];
-    all_some += warp_sums[16 + w];
+    all_some += warp_sums[32 + w];
   }
   if (tid < p.G) q.pre[tid + 1] = (int)min(s, (int64_t)INT32_MAX);  // beyond it: offsets that overlap
   if (tid == 0) q.pre[0] = 0;
@@ -468,85 +475,48 @@ struct RowRef {
   __device__ __forceinline__ uint32_t pieces(const RowView& v) const { return node * v.sn16 + m * v.sm16; }
 };
 
-// Weight gradient: a lane's rows of the two 32-row ring units of a step, loaded a step ahead (moving a loaded value
-// waits for it, so the distance between load and move is what hides the latency).
-struct StepRows {
-  RowRef now[2], next[2];
-  Walk w;
-  __device__ __forceinline__ void load(const SlParams& p, const Groups& q, int t1) {
-    if (w.t >= t1) return;
-    const int at = q.lo[w.g] * p.d + (w.t - q.pre[w.g]) * SL_KC + (threadIdx.x & 31), end = q.hi[w.g] * p.d;
-    next[0].load(p, at, end);
-    next[1].load(p, at + 32, end);
-    w.next(q, t1);
-  }
-  __device__ __forceinline__ void init(const SlParams& p, const Groups& q, int t0, int t1) {
-    w.init(p, q, t0);
-    load(p, q, t1);
-  }
-  __device__ __forceinline__ void step(const SlParams& p, const Groups& q, int t1) {
-    now[0] = next[0];
-    now[1] = next[1];
-    load(p, q, t1);
-  }
-};
-
 constexpr uint32_t NO_ROW = 0xffffffffu;
 
-// One ring unit: 32 row segments of SEG bytes.  Aligned rows (VEC): lane l copies 16-byte piece l % PPR of rows
-// l / PPR + i RPI, whose offsets (in 16 bytes) it holds in off[i]; SWZ stores piece j of row r at j ^ (r & 7).
-template <int SEG>
-struct Pieces {
-  static constexpr int PPR = SEG / 16, RPI = 32 / PPR, N = PPR;
-};
-
-template <int SEG>
+// 32 row segments of 128 bytes.  Aligned rows: lane l copies 16-byte piece l % 8 of rows l / 8 + 4 i, whose offsets
+// (in 16 bytes) it holds in off[i], piece j of row r to j ^ (r & 7).
 __device__ __forceinline__ void spread_rows(uint32_t mine, uint32_t* off) {
-  using P = Pieces<SEG>;
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < P::N; ++i) off[i] = __shfl_sync(0xffffffffu, mine, i * P::RPI + lane / P::PPR);
+  for (int i = 0; i < 8; ++i) off[i] = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
 }
 
-// `at`: first byte of the segment within its row; MASK: bit r of `rows` says whether row r exists (else zeros; its
-// offset is 0).  Rows are whole 16-byte pieces here: a copy whose source size is a register costs several
-// instructions more than one that is all or nothing.
-template <int SEG, int PITCH, bool SWZ, bool MASK>
-__device__ __forceinline__ void fetch_vec(uint32_t dst, const char* data, const uint32_t* off, uint32_t rows, int at,
-                                          int row_bytes) {
-  using P = Pieces<SEG>;
-  const int lane = threadIdx.x & 31, j = lane % P::PPR, r0 = lane / P::PPR;
+// `at`: first byte of the segment within its row.  Rows are whole 16-byte pieces here: a copy whose source size is a
+// register costs several instructions more than one that is all or nothing.
+__device__ __forceinline__ void fetch_vec(uint32_t dst, const char* data, const uint32_t* off, int at, int row_bytes) {
+  const int lane = threadIdx.x & 31, j = lane & 7, r0 = lane >> 3;
   const bool past = at + 16 * j >= row_bytes;
   const char* const src = past ? data : data + at + 16 * j;
-  rows = past ? 0u : rows >> r0;
 #pragma unroll
-  for (int i = 0; i < P::N; ++i) {
-    const int r = i * P::RPI + r0;
-    const int pos = SWZ ? (j ^ (r & 7)) : j;
-    cp_async16_or_zero(dst + r * PITCH + pos * 16, src + (uint64_t)off[i] * 16,
-                       MASK ? !((rows >> (i * P::RPI)) & 1u) : past);
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + r0;
+    cp_async16_or_zero(dst + r * 128 + ((j ^ (r & 7)) << 4), src + (uint64_t)off[i] * 16, past);
   }
 }
 
-// Rows of any alignment: the 16-byte units that contain the segment; mis[r]:
-// where it starts in the first.  row: this lane's row (null: zeros).
-template <int SEG, int PITCH>
+// Rows of any alignment: the 16-byte pieces that contain the segment; mis[r]: where it starts in the first.  (Value by
+// value, as the weight gradient takes rows of 4-byte values, costs the four warps here more than the shifting: 600 000
+// fp32 rows 97 -> 61 164 us against 136.)  row: this lane's row.
+template <int PITCH>
 __device__ __forceinline__ void fetch_any(uint32_t dst, const char* data, const char* row, int at, int row_bytes,
                                           uint8_t* mis) {
-  constexpr int PPR = SEG / 16 + 1;
   const int lane = threadIdx.x & 31;
   // copies of no bytes still name an aligned address
   const char* const dummy = reinterpret_cast<const char*>(reinterpret_cast<uint64_t>(data) & ~(uint64_t)15);
-  const int seg = max(min(row_bytes - at, SEG), 0);  // bytes of a row in this segment
-  const uint64_t from = row ? reinterpret_cast<uint64_t>(row + at) : 0;
+  const int seg = max(min(row_bytes - at, 128), 0);  // bytes of a row in this segment
+  const uint64_t from = reinterpret_cast<uint64_t>(row + at);
   mis[lane] = (uint8_t)(from & 15);
 #pragma unroll
-  for (int i = 0; i < PPR; ++i) {
+  for (int i = 0; i < 9; ++i) {
     const int q = i * 32 + lane;
-    const int r = q / PPR, j = q - r * PPR;
+    const int r = q / 9, j = q - r * 9;
     const uint64_t f = __shfl_sync(0xffffffffu, from, r);
     const int left = (int)(f & 15) + seg - 16 * j;
-    const uint32_t bytes = f == 0 || seg == 0 || left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
+    const uint32_t bytes = seg == 0 || left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
     cp_async16(dst + r * PITCH + j * 16, bytes ? reinterpret_cast<const char*>((f & ~(uint64_t)15) + 16 * j) : dummy,
                bytes);
   }
@@ -630,8 +600,7 @@ __device__ __forceinline__ void copy_out(const SlParams& p, const uint8_t* stage
 // instruction.
 template <typename T>
 __device__ __forceinline__ void finish_wgrad(const SlParams& p, float* acc, int g, bool whole, int tile, int share, int k0,
-                                             int n0, int kl, int c0) {
-  const int CW = p.NT / 2;
+                                             int n0, int kl, int c0, int CW) {
   if (!whole) {
     float4* dst = reinterpret_cast<float4*>(p.part) + ((int64_t)tile * (p.shares + p.G) + share + g) * 32 * p.NT +
                   c0 / 4 * 128 + kl;
@@ -685,8 +654,6 @@ __device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int s) {
                     __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }
 
-constexpr int SL_IMG = 128 * 128;  // bytes of one piece of a B image of up to 128 rows of 64 bf16
-
 // 8 K-values of row n of a B image: their bf16 pieces, `piece` bytes apart
 template <int P>
 __device__ __forceinline__ void put_eight(uint8_t* img, int piece, int n, int chunk, const float* v) {
@@ -721,7 +688,7 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint8_t* img0, i
   const int lane = threadIdx.x & 31, w4 = (threadIdx.x >> 5) & 3;
   const int NT = p.NT;
   auto w_sync = [&]() -> bool {  // the four warps meet (a bounded wait, unlike a barrier)
-    tc::mbar_arrive(w_sync_bar);
+    warp_arrive(w_sync_bar);
     return __all_sync(0xffffffffu, wait_phase(w_sync_bar, syncs++ & 1, abort));
   };
   const T* wt = static_cast<const T*>(p.w) + (int64_t)g * p.K * p.N;
@@ -791,19 +758,18 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint8_t* img0, i
       }
     }
     tc::fence_proxy_async();
-    tc::mbar_arrive(full + 8 * s);
+    warp_arrive(full + 8 * s);
   }
   return true;
 }
 
-template <typename TA, typename T, bool WG, bool VEC>
-__global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_constant__ SlParams p) {
-  using S = Sl<TA, T, WG, VEC>;
-  constexpr int PA = S::PA, PB = S::PB, NU = S::NU;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_constant__ SlParams p) {
+  using S = Sl<T, VEC>;
+  constexpr int P = S::P, NU = S::NU;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = tc::smem_u32(smem);
   const Groups q(smem + S::OFF_PRE);
-  const int* const pre = q.pre;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + S::NBAR);
   volatile int* const abort = reinterpret_cast<int*>(tslot + 1);
@@ -828,17 +794,17 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
     if (lane == 0) {
       *abort = 0;
       for (int s = 0; s < 2; ++s) {
-        tc::mbar_init(A_FULL(s), 128);
+        tc::mbar_init(A_FULL(s), 4);
         tc::mbar_init(A_FREE(s), 1);
         tc::mbar_init(D_FULL(s), 1);
-        tc::mbar_init(D_FREE(s), 256);
+        tc::mbar_init(D_FREE(s), 8);
       }
       for (int s = 0; s < S::MAX_SLOTS; ++s) {
-        tc::mbar_init(B_FULL(s), WG ? NT : 128);
+        tc::mbar_init(B_FULL(s), 4);
         tc::mbar_init(B_FREE(s), 1);
       }
       tc::mbar_init(DONE, 1);
-      tc::mbar_init(W_SYNC, 128);
+      tc::mbar_init(W_SYNC, 4);
       tc::fence_barrier_init();
     }
     __syncwarp();
@@ -847,382 +813,233 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   }
   pdl_wait();  // nothing of the caller's is read or written before
   tc::fence_before_sync();
-  // unit: map: a row tile of a (group, column tile); weight gradient: 64 rows.  blockIdx.x of the weight gradient:
-  // share * tiles + tile
-  const int tiles = WG ? p.n_ct * p.n_kt : 1;
-  const int share = WG ? blockIdx.x / tiles : blockIdx.x;
-  const int tile = WG ? blockIdx.x % tiles : 0;
-  load_groups(p, WG ? SL_KC : 128, WG ? 1 : p.n_ct, WG ? 0 : p.start, share, WG ? p.shares : gridDim.x, WG, q,
-              reinterpret_cast<int64_t*>(smem));
+  // unit: a row tile of a (group, column tile)
+  load_groups<SL_THREADS>(p, 128, p.n_ct, p.start, blockIdx.x, gridDim.x, false, q, reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
-  if (WG && blockIdx.x == 0)
-    for (int i = tid; i <= p.G; i += SL_THREADS) p.units[i] = pre[i];
   const int t0 = q.bounds[0], t1 = q.bounds[1];
   if (t0 >= t1) {
-    if (!WG && warp >= 5 && warp < 8) zero_rows<T>(p);
+    if (warp >= 5 && warp < 8) zero_rows<T>(p);
     if (warp == 15) tc::tmem_dealloc(SL_D, SL_TMEM);
     return;
   }
-  const int wg_k0 = WG ? (tile / p.n_ct) * 128 : 0, wg_n0 = WG ? (tile % p.n_ct) * p.NT : 0;
-  const int n_k = WG ? 1 : (p.K + SL_KC - 1) / SL_KC;  // steps of a tile
-  const int img = WG ? SL_IMG : p.img, slots = WG ? 2 : p.slots;
-  const bool resident = n_k <= slots;               // map: the weight images of a tile stay for the next row tile
+  const int n_k = (p.K + SL_KC - 1) / SL_KC;  // steps of a tile
+  const bool resident = n_k <= p.slots;       // the weight images of a tile stay for the next row tile
   const uint32_t tmem = SL_D;  // an allocation of all 512 columns starts at column 0
-
-  // MMAs of step `it` with the images of slot bs, by one elected thread; `use`: how often the slot was filled
-  // before, or -1 when its images were there already.  The queue of issued MMAs is a few hundred cycles deep, so the
-  // path from one step's last to the next step's first is kept short: two waits, no warp-wide operation
-  const uint32_t idesc = idesc_bf16(NT), bhi = (uint32_t)(tc::sw128_desc(base) >> 32);
-  // The accumulator takes the sn-th sum: one step, or for bf16 (S::LONG) a whole tile or SL_LONG steps, of which this
-  // is the first / last.
-  auto issue = [&](int it, int bs, int use, bool release, int sn, bool first, bool last) -> bool {
-    using PR = Products<PA, PB>;
-    const int s = it & 1;
-    if (use >= 0 && !wait_phase(B_FULL(bs), use & 1, abort)) return false;
-    if (!wait_phase(A_FULL(s), (it >> 1) & 1, abort)) return false;
-    if (first && sn >= 2 && !wait_phase(D_FREE(sn & 1), ((sn >> 1) - 1) & 1, abort)) return false;
-    tc::fence_after_sync();
-    const uint32_t dcol = SL_D + (sn & 1) * 128;
-    const uint32_t blo = (uint32_t)tc::sw128_desc(base + bs * (PB * img));
-    // (the stage as a constant: little is left to compute)
-    auto emit = [&](auto stage) {
-      constexpr uint32_t st = decltype(stage)::value;
-#pragma unroll
-      for (int q = 0; q < PR::n; ++q)
-#pragma unroll
-        for (int ks = 0; ks < SL_KC / 16; ++ks)
-          mma_bf16_ta(dcol, SL_A + st * (PA * 32) + PR::a(q) * 32 + ks * 8, blo + PR::b(q) * (img / 16) + ks * 2, bhi,
-                      idesc, !first || q > 0 || ks > 0);
-    };
-    if (s)
-      emit(std::integral_constant<uint32_t, 1>{});
-    else
-      emit(std::integral_constant<uint32_t, 0>{});
-    tc::mma_commit(A_FREE(s));
-    if (last) tc::mma_commit(D_FULL(sn & 1));
-    if (release) tc::mma_commit(B_FREE(bs));
-    return true;
-  };
-  auto drain = [&]() {  // every MMA issued is complete (bounded)
-    if (elect_one()) {
-      tc::mma_commit(DONE);
-      tc::mbar_wait(DONE, 0);
-    }
-    __syncwarp();
-  };
 
   if (warp < 4) {
     // ---------------- operand A: memory -> ring -> registers -> TMEM ----------------
-    const uint32_t ring = base + S::OFF_A + warp * NU * S::UNIT_A;
+    const uint32_t ring = base + S::OFF_A + warp * NU * S::UNIT;
     uint8_t* const mis = smem + S::OFF_MIS + warp * NU * 32;
-    const int row_bytes = p.a.width * (int)sizeof(TA);
+    const int row_bytes = p.a.width * (int)sizeof(T);
     const uint32_t tq = tmem + ((uint32_t)(warp * 32) << 16) + SL_A;
-    // the fetching side runs NU - 1 units ahead; the atoms of its rows are loaded one tile (weight gradient: two
-    // units) before
+    // the fetching side runs NU - 1 units ahead; the atoms of its rows are loaded one tile before
     const int tile_units = n_k * S::UPC;  // ring units of a tile
     const int units = (t1 - t0) * tile_units;
     int left = units, fu = 0, slot_f = 0;  // units to fetch, unit within the tile, ring slot
-    RowRef ref;      // map: this lane's row of the next tile
+    RowRef ref;  // this lane's row of the next tile
     Walk w_tile;
-    StepRows rows;   // weight gradient
-    uint32_t off[Pieces<S::SEG_A>::N];
+    uint32_t off[8];
     const char* row = nullptr;
     auto load_tile = [&]() {
       const Tile t(p, q, w_tile);
       ref.load(p, t.at + warp * 32 + lane, t.end);
     };
-    // the loaded rows become the fetched ones.  Map: a row outside the tile may hold anything (its
-    // TMEM lane is never stored), so it stands for row 0; weight gradient: it must be zero
-    uint32_t here = 0;  // weight gradient: which rows of the unit exist
-    auto take_rows = [&]() {
-      const bool ok = ref.valid(p);
-      if constexpr (VEC) {
-        if constexpr (WG) here = __ballot_sync(0xffffffffu, ok);
-        spread_rows<S::SEG_A>(ok ? ref.pieces(p.a) : 0u, off);
-      } else {
-        const int64_t o = ok ? ref.offset(p.a) : 0;
-        row = WG && !ok ? nullptr : p.a.data + o;
-      }
-    };
     auto fetch = [&]() {
       if (left > 0) {
         --left;
-        if constexpr (WG) {
-          if (fu == 0) rows.step(p, q, t1);
-          ref = fu == 0 ? rows.now[0] : rows.now[1];
-          take_rows();
-        } else if (fu == 0) {
-          take_rows();
+        if (fu == 0) {
+          // (a row outside the tile may hold anything, as its TMEM lane is never stored: it stands for row 0)
+          const bool ok = ref.valid(p);
+          if constexpr (VEC)
+            spread_rows(ok ? ref.pieces(p.a) : 0u, off);
+          else
+            row = p.a.data + (ok ? ref.offset(p.a) : 0);
           w_tile.next(q, t1);
           if (w_tile.t < t1) load_tile();
         }
-        const uint32_t dst = ring + slot_f * S::UNIT_A;
-        const int at = WG ? (wg_k0 + warp * 32) * (int)sizeof(TA) : fu * 128;
+        const uint32_t dst = ring + slot_f * S::UNIT;
         if constexpr (VEC)
-          fetch_vec<S::SEG_A, S::PITCH_A, !WG, WG>(dst, p.a.data, off, here, at, row_bytes);
+          fetch_vec(dst, p.a.data, off, fu * 128, row_bytes);
         else
-          fetch_any<S::SEG_A, S::PITCH_A>(dst, p.a.data, row, at, row_bytes, mis + slot_f * 32);
+          fetch_any<S::PITCH>(dst, p.a.data, row, fu * 128, row_bytes, mis + slot_f * 32);
         slot_f = slot_f + 1 == NU ? 0 : slot_f + 1;
         if (++fu == tile_units) fu = 0;
       }
       cp_commit();
     };
-    if constexpr (WG) {
-      rows.init(p, q, t0, t1);
-    } else {
-      w_tile.init(p, q, t0);
-      load_tile();
-    }
+    w_tile.init(p, q, t0);
+    load_tile();
     // (one loop, so that the code of a unit exists once: the roles' loops together fill the instruction cache)
     int slot = 0;
     bool ok = true;
 #pragma unroll 1
     for (int i = 1 - NU; i < units && ok; ++i) {
       const int it = i / S::UPC, u = i - it * S::UPC, s = it & 1;
-      {
-        if (i >= 0) cp_wait<NU - 2>();
-        __syncwarp();
-        fetch();
-        if (i < 0) continue;
-        const uint8_t* const src = smem + S::OFF_A + (warp * NU + slot) * S::UNIT_A;
-        const uint8_t* const ms = mis + slot * 32;
-        slot = slot + 1 == NU ? 0 : slot + 1;
-        if (u == 0) {
-          ok = it < 2 || wait_phase(A_FREE(s), ((it >> 1) - 1) & 1, abort);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc::fence_after_sync();
-        }
-        const uint32_t ta = tq + s * (PA * 32);
-        if constexpr (!WG) {
-          // this lane's row: 128 bytes of it
-          const int sh = VEC ? 0 : ms[lane];
-          auto piece = [&](int j) {
-            return load_as<uint4>(src + lane * S::PITCH_A + (VEC ? (j ^ (lane & 7)) : j) * 16);
-          };
-          uint32_t out[PA][16];
-          uint4 cur = piece(0);
+      if (i >= 0) cp_wait<NU - 2>();
+      __syncwarp();
+      fetch();
+      if (i < 0) continue;
+      const uint8_t* const src = smem + S::OFF_A + (warp * NU + slot) * S::UNIT;
+      const uint8_t* const ms = mis + slot * 32;
+      slot = slot + 1 == NU ? 0 : slot + 1;
+      if (u == 0) {
+        ok = it < 2 || wait_phase(A_FREE(s), ((it >> 1) - 1) & 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::fence_after_sync();
+      }
+      const uint32_t ta = tq + s * (P * 32);
+      // this lane's row: 128 bytes of it
+      const int sh = VEC ? 0 : ms[lane];
+      auto piece = [&](int j) { return load_as<uint4>(src + lane * S::PITCH + (VEC ? j ^ (lane & 7) : j) * 16); };
+      uint32_t out[P][16];
+      uint4 cur = piece(0);
 #pragma unroll
-          for (int h = 0; h < 8 / (sizeof(TA) == 4 ? 8 : 4); ++h) {
+      for (int h = 0; h < 8 / (P == 3 ? 8 : 4); ++h) {
 #pragma unroll
-            for (int q = 0; q < (sizeof(TA) == 4 ? 8 : 4); ++q) {
-              const int j = h * 4 + q;
-              uint4 v = cur;
-              if constexpr (VEC) {
-                if (j < 7) cur = piece(j + 1);
-              } else {
-                const uint4 nx = piece(j + 1);
-                v = shifted(cur, nx, sh);
-                cur = nx;
-              }
-              if constexpr (sizeof(TA) == 4) {
-                uint32_t t[3];
-                split2<PA>(__uint_as_float(v.x), __uint_as_float(v.y), t);
-#pragma unroll
-                for (int a = 0; a < PA; ++a) out[a][2 * q] = t[a];
-                split2<PA>(__uint_as_float(v.z), __uint_as_float(v.w), t);
-#pragma unroll
-                for (int a = 0; a < PA; ++a) out[a][2 * q + 1] = t[a];
-              } else {
-                out[0][4 * q] = v.x;
-                out[0][4 * q + 1] = v.y;
-                out[0][4 * q + 2] = v.z;
-                out[0][4 * q + 3] = v.w;
-              }
-            }
-            if constexpr (sizeof(TA) == 2) tmem_st16u(ta + h * 16, out[0]);
+        for (int q = 0; q < (P == 3 ? 8 : 4); ++q) {
+          const int j = h * 4 + q;
+          uint4 v = cur;
+          if constexpr (VEC) {
+            if (j < 7) cur = piece(j + 1);
+          } else {
+            const uint4 nx = piece(j + 1);
+            v = shifted(cur, nx, sh);
+            cur = nx;
           }
-          if constexpr (sizeof(TA) == 4) {
-#pragma unroll
-            for (int a = 0; a < PA; ++a) tmem_st16u(ta + a * 32 + u * 16, out[a]);
-          }
-        } else {
-          // this lane's channel of 32 rows
-          uint32_t out[PA][16];
-#pragma unroll
-          for (int r = 0; r < 32; r += 2) {
-            const uint8_t* const mine = src + lane * (int)sizeof(TA);
+          if constexpr (P == 3) {
             uint32_t t[3];
-            split2<PA>(load_f32<TA>(mine + r * S::PITCH_A + (VEC ? 0 : ms[r])),
-                       load_f32<TA>(mine + (r + 1) * S::PITCH_A + (VEC ? 0 : ms[r + 1])), t);
+            split2<P>(__uint_as_float(v.x), __uint_as_float(v.y), t);
 #pragma unroll
-            for (int a = 0; a < PA; ++a) out[a][r / 2] = t[a];
+            for (int a = 0; a < P; ++a) out[a][2 * q] = t[a];
+            split2<P>(__uint_as_float(v.z), __uint_as_float(v.w), t);
+#pragma unroll
+            for (int a = 0; a < P; ++a) out[a][2 * q + 1] = t[a];
+          } else {
+            out[0][4 * q] = v.x;
+            out[0][4 * q + 1] = v.y;
+            out[0][4 * q + 2] = v.z;
+            out[0][4 * q + 3] = v.w;
           }
-#pragma unroll
-          for (int a = 0; a < PA; ++a) tmem_st16u(ta + a * 32 + u * 16, out[a]);
         }
+        if constexpr (P == 1) tmem_st16u(ta + h * 16, out[0]);
+      }
+      if constexpr (P == 3) {
+#pragma unroll
+        for (int a = 0; a < P; ++a) tmem_st16u(ta + a * 32 + u * 16, out[a]);
       }
       if (u == S::UPC - 1) {
         tc::tmem_wait_st();
         tc::fence_before_sync();
-        tc::mbar_arrive(A_FULL(s));
+        warp_arrive(A_FULL(s));
       }
     }
     cp_wait<0>();
   } else if (warp < 8) {
-    // ---------------- operand B: 64-wide images, one column n per thread ----------------
-    const int w4 = warp - 4;
+    // ---------------- operand B: the weight images, and the MMAs ----------------
+    // MMAs of step `it` with the images of slot bs, by one elected thread; `use`: how often the slot was filled
+    // before, or -1 when its images were there already.  The queue of issued MMAs is a few hundred cycles deep, so
+    // the path from one step's last to the next step's first is kept short: two waits, no warp-wide operation.
+    const uint32_t idesc = idesc_bf16(NT), bhi = (uint32_t)(tc::sw128_desc(base) >> 32);
+    // The accumulator takes the sn-th sum: one step, or for bf16 (S::LONG) a whole tile, of which this is the first /
+    // last.
+    auto issue = [&](int it, int bs, int use, bool release, int sn, bool first, bool last) -> bool {
+      using PR = Products<P, P>;
+      const int s = it & 1;
+      if (use >= 0 && !wait_phase(B_FULL(bs), use & 1, abort)) return false;
+      if (!wait_phase(A_FULL(s), (it >> 1) & 1, abort)) return false;
+      if (first && sn >= 2 && !wait_phase(D_FREE(sn & 1), ((sn >> 1) - 1) & 1, abort)) return false;
+      tc::fence_after_sync();
+      const uint32_t dcol = SL_D + (sn & 1) * 128;
+      const uint32_t blo = (uint32_t)tc::sw128_desc(base + bs * (P * p.img));
+      // (the stage as a constant: little is left to compute)
+      auto emit = [&](auto stage) {
+        constexpr uint32_t st = decltype(stage)::value;
+#pragma unroll
+        for (int q = 0; q < PR::n; ++q)
+#pragma unroll
+          for (int ks = 0; ks < SL_KC / 16; ++ks)
+            mma_bf16_ta(dcol, SL_A + st * (P * 32) + PR::a(q) * 32 + ks * 8, blo + PR::b(q) * (p.img / 16) + ks * 2, bhi,
+                        idesc, !first || q > 0 || ks > 0);
+      };
+      if (s)
+        emit(std::integral_constant<uint32_t, 1>{});
+      else
+        emit(std::integral_constant<uint32_t, 0>{});
+      tc::mma_commit(A_FREE(s));
+      if (last) tc::mma_commit(D_FULL(sn & 1));
+      if (release) tc::mma_commit(B_FREE(bs));
+      return true;
+    };
     bool ok = true;
-    {
-      if constexpr (!WG) {
-        int syncs = 0;
-        auto fill = [&](int g, int ct, int k0, int nk, int slot0) -> bool {
-          return fill_weights<T, PB>(p, smem + slot0 * PB * img, PB * img, g, ct, k0, nk, bar(8 + slot0), W_SYNC,
-                                     syncs, abort);
-        };
-        Walk w;
-        w.init(p, q, t0);
-        int it = 0, tile_no = 0, fills = 0;  // steps, tiles; image sets (resident) or images written
-        while (w.t < t1 && ok) {
-          const Tile t(p, q, w);
-          if (resident) {
-            // the tiles of this CTA that share the weights
-            const int run = min(t.run, t1 - w.t);
-            for (int k = 0; k < n_k && ok && fills > 0; ++k) ok = wait_phase(B_FREE(k), (fills - 1) & 1, abort);
-            ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, 0, n_k, 0);
-            if (!ok) break;
-            if (warp == 4 && elect_one())
-              for (int i = 0; i < run && ok; ++i)
-                for (int k = 0; k < n_k && ok; ++k)
-                  ok = issue(it + i * n_k + k, k, i == 0 ? fills : -1, i + 1 == run,
-                             S::LONG ? tile_no + i : it + i * n_k + k, !S::LONG || k == 0, !S::LONG || k + 1 == n_k);
-            it += run * n_k;
-            tile_no += run;
-            ++fills;
-            w.t += run - 1;
-          } else {
-            for (int k = 0; k < n_k && ok; ++k, ++it, ++fills) {
-              const int s = fills % slots, use = fills / slots;
-              ok = use == 0 || wait_phase(B_FREE(s), (use - 1) & 1, abort);
-              ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, k, 1, s);
-              if (ok && warp == 4 && elect_one())
-                ok = issue(it, s, use, true, S::LONG ? tile_no : it, !S::LONG || k == 0, !S::LONG || k + 1 == n_k);
-              ok = __all_sync(0xffffffffu, ok);
-            }
-            ++tile_no;
-          }
+    int syncs = 0;
+    auto fill = [&](int g, int ct, int k0, int nk, int slot0) -> bool {
+      return fill_weights<T, P>(p, smem + slot0 * P * p.img, P * p.img, g, ct, k0, nk, bar(8 + slot0), W_SYNC, syncs,
+                                abort);
+    };
+    Walk w;
+    w.init(p, q, t0);
+    int it = 0, tile_no = 0, fills = 0;  // steps, tiles; image sets (resident) or images written
+    while (w.t < t1 && ok) {
+      const Tile t(p, q, w);
+      if (resident) {
+        // the tiles of this CTA that share the weights
+        const int run = min(t.run, t1 - w.t);
+        for (int k = 0; k < n_k && ok && fills > 0; ++k) ok = wait_phase(B_FREE(k), (fills - 1) & 1, abort);
+        ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, 0, n_k, 0);
+        if (!ok) break;
+        if (warp == 4 && elect_one())
+          for (int i = 0; i < run && ok; ++i)
+            for (int k = 0; k < n_k && ok; ++k)
+              ok = issue(it + i * n_k + k, k, i == 0 ? fills : -1, i + 1 == run,
+                         S::LONG ? tile_no + i : it + i * n_k + k, !S::LONG || k == 0, !S::LONG || k + 1 == n_k);
+        it += run * n_k;
+        tile_no += run;
+        ++fills;
+        w.t += run - 1;
+      } else {
+        for (int k = 0; k < n_k && ok; ++k, ++it, ++fills) {
+          const int s = fills % p.slots, use = fills / p.slots;
+          ok = use == 0 || wait_phase(B_FREE(s), (use - 1) & 1, abort);
+          ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, k, 1, s);
+          if (ok && warp == 4 && elect_one())
+            ok = issue(it, s, use, true, S::LONG ? tile_no : it, !S::LONG || k == 0, !S::LONG || k + 1 == n_k);
           ok = __all_sync(0xffffffffu, ok);
-          w.next(q, t1);
         }
-        if (warp == 4)
-          drain();
-        else
-          zero_rows<T>(p);
-      } else if (w4 * 32 < NT) {
-        const int n = w4 * 32 + lane;
-        const uint32_t ring = base + S::OFF_B + w4 * S::NU_B * S::UNIT_B;
-        uint8_t* const mis = smem + S::OFF_MIS + (4 + w4) * NU * 32;
-        constexpr int NU_B = S::NU_B;
-        float* const sc = reinterpret_cast<float*>(smem + S::OFF_SCALE) + w4 * NU * 32;
-        const int row_bytes = p.b.width * (int)sizeof(T), at = (wg_n0 + w4 * 32) * (int)sizeof(T);
-        int left = 2 * (t1 - t0), slot_f = 0;
-        StepRows rows;
-        rows.init(p, q, t0, t1);
-        auto fetch = [&]() {
-          if (left > 0) {
-            const bool second = left & 1;
-            --left;
-            if (!second) rows.step(p, q, t1);
-            const RowRef ref = second ? rows.now[1] : rows.now[0];
-            const bool in = ref.valid(p);
-            const uint32_t dst = ring + slot_f * S::UNIT_B;
-            if constexpr (VEC) {
-              uint32_t off[Pieces<S::SEG_B>::N];
-              spread_rows<S::SEG_B>(in ? ref.pieces(p.b) : 0u, off);
-              fetch_vec<S::SEG_B, S::PITCH_B, false, true>(dst, p.b.data, off, __ballot_sync(0xffffffffu, in), at,
-                                                           row_bytes);
-            } else {
-              fetch_any<S::SEG_B, S::PITCH_B>(dst, p.b.data, in ? p.b.data + ref.offset(p.b) : nullptr, at, row_bytes,
-                                              mis + slot_f * 32);
-            }
-            if constexpr (sizeof(TA) == 1) {
-              const float* src = in ? p.a_scale + ((int64_t)ref.node * p.d + ref.m) * p.ka_blocks +
-                                          wg_k0 / MACE_CHECKPOINT_BLOCK
-                                    : p.a_scale;
-              cp_async4(tc::smem_u32(sc + slot_f * 32 + lane), src, in ? 4u : 0u);
-            }
-            slot_f = slot_f + 1 == NU_B ? 0 : slot_f + 1;
-          }
-          cp_commit();
-        };
-        int slot = 0;
-#pragma unroll 1
-        for (int i = 1 - NU_B; i < 2 * (t1 - t0) && ok; ++i) {
-          const int it = i >> 1, u = i & 1, s = it & 1;
-          if (i >= 0) cp_wait<NU_B - 2>();
-          __syncwarp();
-          fetch();
-          if (i < 0) continue;
-          const uint8_t* const src = smem + S::OFF_B + (w4 * NU_B + slot) * S::UNIT_B + lane * (int)sizeof(T);
-          const uint8_t* const ms = mis + slot * 32;
-          const float* const ss = sc + slot * 32;
-          slot = slot + 1 == NU_B ? 0 : slot + 1;
-          if (u == 0 && it >= 2) {
-            ok = __all_sync(0xffffffffu, wait_phase(B_FREE(s), ((it >> 1) - 1) & 1, abort));
-            if (!ok) break;
-          }
-          uint8_t* const img = smem + s * PB * SL_IMG;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int r = 8 * q + j;
-              v[j] = load_f32<T>(src + r * S::PITCH_B + (VEC ? 0 : ms[r]));
-              if constexpr (sizeof(TA) == 1) v[j] *= ss[r];
-            }
-            put_eight<PB>(img, SL_IMG, n, u * 4 + q, v);
-          }
-          if (u == 1) {
-            tc::fence_proxy_async();
-            tc::mbar_arrive(B_FULL(s));
-          }
-        }
-        cp_wait<0>();
+        ++tile_no;
       }
+      ok = __all_sync(0xffffffffu, ok);
+      w.next(q, t1);
+    }
+    if (warp == 4) {
+      if (elect_one()) {  // every MMA issued is complete (bounded)
+        tc::mma_commit(DONE);
+        tc::mbar_wait(DONE, 0);
+      }
+      __syncwarp();
+    } else {
+      zero_rows<T>(p);
     }
   } else {
     // ---------------- epilogue ----------------
     const int quad = warp & 3, half = (warp - 8) >> 2;
     const int CW = NT / 2;  // columns of this warp: 16, 32, 48 or 64
     const uint32_t tq = tmem + ((uint32_t)(quad * 32) << 16) + SL_D + half * CW;
+    uint8_t* const stage = smem + S::OFF_STG + (warp - 8) * S::STG;
     Walk w;
     w.init(p, q, t0);
     float acc[64];
     bool ok = true;
-    bool fresh = true;  // acc holds nothing yet
-    RowRef ref{-1, -1};  // map: this lane's row of the tile, loaded while the tile is computed
-    int ct = 0, k = 0;   // map: the tile's column tile, the step
-    // weight gradient: the steps of one sum, within a group; warp 8 issues the next sum's MMAs before it takes this one's
-    auto sum_steps = [&](const Walk& x) { return S::LONG ? min(min(SL_LONG, pre[x.g + 1] - x.t), t1 - x.t) : 1; };
-    auto advance = [&](Walk& x, int n) {
-      x.t += n - 1;
-      x.next(q, t1);
-    };
-    Walk m = w;
-    int mi = 0, ms = 0;  // the issuing side: step, sum
-    auto issue_wg = [&]() {
-      if (!WG || warp != 8 || m.t >= t1) return;
-      const int n = sum_steps(m);
-      if (elect_one())
-        for (int i = 0; i < n && ok; ++i) ok = issue(mi + i, (mi + i) & 1, (mi + i) >> 1, true, ms, i == 0, i + 1 == n);
-      ok = __all_sync(0xffffffffu, ok);
-      mi += n;
-      ++ms;
-      advance(m, n);
-    };
-    issue_wg();
+    bool fresh = true;   // acc holds nothing yet
+    RowRef ref{-1, -1};  // this lane's row of the tile, loaded while the tile is computed
+    int ct = 0, k = 0;   // the tile's column tile, the step
     for (int sn = 0; w.t < t1 && ok; ++sn) {
       const int s = sn & 1;
-      if constexpr (!WG) {
-        if (fresh) {
-          const Tile t(p, q, w);
-          ref.load(p, t.at + quad * 32 + lane, t.end);
-          ct = t.ct;
-        }
+      if (fresh) {
+        const Tile t(p, q, w);
+        ref.load(p, t.at + quad * 32 + lane, t.end);
+        ct = t.ct;
       }
-      issue_wg();
-      if (!ok) break;
       ok = wait_phase(D_FULL(s), (sn >> 1) & 1, abort);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -1239,64 +1056,51 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
         tc::tmem_wait_ld();
         if (h == 3) {
           tc::fence_before_sync();
-          tc::mbar_arrive(D_FREE(s));
+          warp_arrive(D_FREE(s));
         }
 #pragma unroll
         for (int k = 0; k < 16; k += 2) add2(acc[h * 16 + k], acc[h * 16 + k + 1], v[k], v[k + 1]);
       }
       fresh = false;
-      if constexpr (!WG) {
-        k += S::LONG ? n_k : 1;
-        if (k < n_k) continue;
-        k = 0;
-        const int c0 = ct * NT + half * CW;
-        // Rows leave through shared memory, CB columns at a time: a thread holds one row, so stores straight from
-        // registers would touch 32 rows per instruction (measured 3600 cycles of the load/store unit per tile
-        // against 1500 staged).
-        constexpr int CB = 128 / sizeof(T);  // columns of a 128-byte row segment
-        const bool mine = ref.valid(p);
-        uint8_t* const stage = smem + S::OFF_STG + (warp - 8) * S::STG;
-        if constexpr (PB == 1) {
+      k += S::LONG ? n_k : 1;
+      if (k < n_k) continue;
+      k = 0;
+      const int c0 = ct * NT + half * CW;
+      // Rows leave through shared memory, CB columns at a time: a thread holds one row, and 32-byte stores of it
+      // touch 32 rows per instruction (600 000 rows 128 -> 128 fp32: 149 us with them, 130 staged).
+      constexpr int CB = 128 / sizeof(T);  // columns of a 128-byte row segment
+      const bool mine = ref.valid(p);
+      if constexpr (P == 1) {
 #pragma unroll
-          for (int k = 0; k < 64; ++k) acc[k] *= p.alpha;
-        }
-#pragma unroll
-        for (int b = 0; b < 64; b += CB) {
-          const int left = min(p.N - c0 - b, CW - b);  // columns of this segment
-          if (left <= 0) break;
-          // piece j of row r at j ^ (r & 7); the addresses are made here each time: held across the tiles they
-          // would push the accumulators to memory
-          int row = lane;
-          asm volatile("" : "+r"(row));
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            uint32_t w4[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if constexpr (sizeof(T) == 4)
-                w4[q] = __float_as_uint(acc[b + 4 * j + q]);
-              else
-                w4[q] = pack_bf16(acc[b + 8 * j + 2 * q], acc[b + 8 * j + 2 * q + 1]);
-            }
-            store_piece(stage + row * 128 + ((j ^ (row & 7)) << 4), w4[0], w4[1], w4[2], w4[3]);
-          }
-          __syncwarp();
-          copy_out<T>(p, stage, ref, mine, c0 + b, left);
-          __syncwarp();
-        }
-        fresh = true;
-        w.next(q, t1);
-      } else {
-        const int len = sum_steps(w);
-        const bool group_ends = w.t + len == pre[w.g + 1];
-        if (group_ends || w.t + len == t1) {
-          finish_wgrad<T>(p, acc, w.g, group_ends && pre[w.g] >= t0, tile, share, wg_k0, wg_n0, quad * 32 + lane, half * CW);
-          fresh = true;
-        }
-        advance(w, len);
+        for (int k = 0; k < 64; ++k) acc[k] *= p.alpha;
       }
+#pragma unroll
+      for (int b = 0; b < 64; b += CB) {
+        const int left = min(p.N - c0 - b, CW - b);  // columns of this segment
+        if (left <= 0) break;
+        // piece j of row r at j ^ (r & 7); the addresses are made here each time: held across the tiles they
+        // would push the accumulators to memory
+        int row = lane;
+        asm volatile("" : "+r"(row));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t w4[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if constexpr (sizeof(T) == 4)
+              w4[q] = __float_as_uint(acc[b + 4 * j + q]);
+            else
+              w4[q] = pack_bf16(acc[b + 8 * j + 2 * q], acc[b + 8 * j + 2 * q + 1]);
+          }
+          store_piece(stage + row * 128 + ((j ^ (row & 7)) << 4), w4[0], w4[1], w4[2], w4[3]);
+        }
+        __syncwarp();
+        copy_out<T>(p, stage, ref, mine, c0 + b, left);
+        __syncwarp();
+      }
+      fresh = true;
+      w.next(q, t1);
     }
-    if (WG && warp == 8) drain();
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -1307,11 +1111,26 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_gemm(const __grid_con
   }
 }
 
+// launches a kernel with `smem` bytes of dynamic shared memory; attr_set: of this kernel, per device (the attribute
+// call is slow on the host)
+template <typename K>
+int launch_big(const char* name, K kernel, bool* attr_set, int grid, int threads, int smem, cudaStream_t s,
+               const SlParams& p) {
+  int dev = 0;
+  MACE_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !attr_set[dev]) {
+    MACE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev < 64) attr_set[dev] = true;
+  }
+  return launch(name, kernel, grid, threads, smem, s, p);
+}
+
 }  // namespace
 
 }  // namespace mace
 
 #include "species_direct.cuh"
+#include "species_wgrad.cuh"
 
 namespace mace {
 
@@ -1442,17 +1261,23 @@ bool aligned_rows(const RowView& v, int64_t n, int d, int size) {
          ((n - 1) * v.sn + (d - 1) * v.sm) / 16 < (int64_t)NO_ROW;
 }
 
-template <typename TA, typename T, bool WG, bool VEC>
-int launch_gemm(const SlParams& p, int grid, cudaStream_t s) {
-  constexpr int BYTES = Sl<TA, T, WG, VEC>::BYTES;
-  static bool attr_set[64] = {};  // per device: the attribute call is slow on the host
-  int dev = 0;
-  MACE_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev >= 64 || !attr_set[dev]) {
-    MACE_CUDA_TRY(cudaFuncSetAttribute(k_species_gemm<TA, T, WG, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
-    if (dev < 64) attr_set[dev] = true;
+template <typename T, bool VEC>
+int launch_map(const SlParams& p, int grid, cudaStream_t s) {
+  static bool attr_set[64] = {};
+  return launch_big("species_map", k_species_map<T, VEC>, attr_set, grid, SL_THREADS, Sl<T, VEC>::BYTES, s, p);
+}
+
+template <typename TA, typename T, bool VEC>
+int launch_wgrad(const SlParams& p, int grid, cudaStream_t s) {
+  static bool attr_set[64] = {};
+  static int regs = 0;  // the shares that the kernel deals out are taken from what it is launched with
+  if (regs == 0) {
+    cudaFuncAttributes a;
+    MACE_CUDA_TRY(cudaFuncGetAttributes(&a, k_species_wgrad<TA, T, VEC>));
+    regs = a.numRegs;
   }
-  return launch("species_gemm", k_species_gemm<TA, T, WG, VEC>, grid, SL_THREADS, BYTES, s, p);
+  if (regs != WG_REGS) return fail(MACE_ERR_CUDA, "species_wgrad: built with other than 80 registers a thread");
+  return launch_big("species_wgrad", k_species_wgrad<TA, T, VEC>, attr_set, grid, WG_THREADS, Wg<TA, T, VEC>::BYTES, s, p);
 }
 
 int64_t partial_bytes(const SlParams& p, int G) {
@@ -1482,6 +1307,8 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   if (bad_sizes(dtype, n, d, G, K, M) || xn < 0 || xm < 0 || yn < 0 || ym < 0 || !w || !offsets ||
       (n > 0 && (!x || !y || !order)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_linear: bad arguments");
+  if (unaligned(value_size(dtype), x, w, y) || unaligned(4, order, offsets))
+    return fail(MACE_ERR_BAD_ARG, "mace_species_linear: an address is not a multiple of its values' size");
   if (n == 0) return MACE_OK;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int es = dtype == MACE_F32 ? 4 : 2;
@@ -1533,8 +1360,8 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   const int grid = (int)std::min<int64_t>(sms, (row_tiles + std::min<int64_t>(G, n)) * p.n_ct);
   if (direct) return launch_direct<false>(p, grid, s);  // bf16 in whole pieces: nothing to convert
   if (dtype == MACE_F32)
-    return vec ? launch_gemm<float, float, false, true>(p, grid, s) : launch_gemm<float, float, false, false>(p, grid, s);
-  return launch_gemm<bf16, bf16, false, false>(p, grid, s);
+    return vec ? launch_map<float, true>(p, grid, s) : launch_map<float, false>(p, grid, s);
+  return launch_map<bf16, false>(p, grid, s);
 }
 
 extern "C" int mace_species_linear_wgrad_workspace(int64_t n, int32_t d, int32_t G, int32_t K, int32_t M,
@@ -1554,6 +1381,8 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   if (bad_sizes(dtype, n, d, G, K, M) || xn < 0 || xm < 0 || yn < 0 || ym < 0 || !dw || !offsets ||
       (n > 0 && (!x || !dy || !order)))
     return fail(MACE_ERR_BAD_ARG, "mace_species_linear_wgrad: bad arguments");
+  if (unaligned(xs ? 1 : value_size(dtype), x) || unaligned(value_size(dtype), dy, dw) || unaligned(4, xs, order, offsets))
+    return fail(MACE_ERR_BAD_ARG, "mace_species_linear_wgrad: an address is not a multiple of its values' size");
   int64_t need = 0;
   mace_species_linear_wgrad_workspace(n, d, G, K, M, &need);
   if (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 31) != 0)
@@ -1588,7 +1417,7 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   auto go = [&](auto ta, auto t) {
     using TA = decltype(ta);
     using T = decltype(t);
-    return vec ? launch_gemm<TA, T, true, true>(p, grid, s) : launch_gemm<TA, T, true, false>(p, grid, s);
+    return vec ? launch_wgrad<TA, T, true>(p, grid, s) : launch_wgrad<TA, T, false>(p, grid, s);
   };
   int rc;
   if (xs)
@@ -1596,7 +1425,7 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   else if (dtype == MACE_F32)
     rc = go(float{}, float{});
   else  // bf16 in whole pieces: nothing to convert
-    rc = vec ? launch_direct<true>(p, grid, s) : launch_gemm<bf16, bf16, true, false>(p, grid, s);
+    rc = vec ? launch_direct<true>(p, grid, s) : launch_wgrad<bf16, bf16, false>(p, grid, s);
   if (rc) return rc;
   const dim3 jg(G, 16 * (p.NT / 32), p.n_ct * p.n_kt);
   return launch("species_wgrad_join", dtype == MACE_F32 ? k_species_wgrad_join<float> : k_species_wgrad_join<bf16>, jg, 256,

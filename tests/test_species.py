@@ -67,3 +67,27 @@ def test_c_entries_check_their_arguments():
     assert lib.mace_rows_restore(0, one, None, 1, 1, 8, one, None) == nv.MACE_ERR_BAD_ARG
     assert lib.mace_rows_restore(0, one, one, 1, 0, 8, one, None) == nv.MACE_ERR_BAD_ARG
     assert lib.mace_species_error_flag(None) == nv.MACE_ERR_BAD_ARG
+
+
+def test_c_entries_refuse_addresses_off_their_values():
+    lib = nv.load_library()
+    one, odd, half = C.c_void_p(32), C.c_void_p(33), C.c_void_p(34)  # never dereferenced
+
+    def refused(f, args, *at):
+        for k in at:
+            for address in (odd, half) if k >= 0 else (odd,):
+                call = list(args)
+                call[abs(k)] = address
+                assert f(*call) == nv.MACE_ERR_BAD_ARG and "values' size" in nv.last_error(lib), (f, k)
+
+    # (0: fp32; a negative place may be any multiple of two)
+    refused(lib.mace_species_group, (one, 5, 2, one, one, None, 0, None), 0, 3, 4)
+    refused(lib.mace_species_embed, (0, one, 8, 1, 8, one, 1, 1.0, one, 8, None), 1, 5, 8)
+    refused(lib.mace_species_embed, (1, one, 8, 1, 8, one, 1, 1.0, one, 8, None), -1, 5, -8)
+    refused(lib.mace_species_embed_grad, (0, one, 8, one, one, 4, 1, 8, 1.0, one, one, 1 << 20, None), 1, 3, 4, 9, 10)
+    refused(lib.mace_species_linear, (0, one, 8, 8, one, 0, 1, 8, 8, one, one, 4, 1, 1.0, one, 8, 8, None), 1, 4, 9, 10, 14)
+    refused(lib.mace_species_linear, (1, one, 8, 8, one, 0, 1, 8, 8, one, one, 4, 1, 1.0, one, 8, 8, None), -1, -4, -14)
+    refused(lib.mace_species_linear_wgrad, (0, one, 8, 8, None, one, 8, 8, 1, 8, 8, one, one, 4, 1, 1.0, one, one, 1 << 30,
+                                            None), 1, 4, 5, 11, 12, 16)
+    refused(lib.mace_rows_checkpoint, (0, one, 8, 8, 1, 1, 8, one, one, None), 1, 8)
+    refused(lib.mace_rows_restore, (0, one, one, 1, 1, 8, one, None), 2, 6)
