@@ -428,6 +428,8 @@ int mace_ctx_error_flag(mace_ctx* ctx, int32_t* flag);
  * the caller owns every buffer, workspaces included; nothing here allocates or
  * synchronises, so every call can be captured into a CUDA graph.  Calls use
  * the current device, which must own the pointers.
+ * Addresses are multiples of their values' size (checked); a workspace aligned
+ * to 32 bytes serves every entry.
  *
  * A species index outside [0, num_groups) marks a padding row (NaN features
  * there are never read): it belongs to no group, its outputs are zero and it

@@ -562,3 +562,49 @@ def test_groupings_that_are_not_permutations_stay_in_bounds(sp):
         sp.species_embedding_grad(dy[:, 0], bad)
     torch.cuda.synchronize()
     assert sp.error_flag() == 0
+
+
+# ------------------------------------------------------------------- together
+@pytest.fixture(scope="module")
+def head_example():
+    import importlib.util
+    import pathlib
+
+    path = pathlib.Path(__file__).resolve().parents[1] / "examples" / "species_head.py"
+    spec = importlib.util.spec_from_file_location("species_head", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_head_on_model_features_has_the_plain_gradients(sp, head_example):
+    n = 6
+    h, z, graph = head_example.frozen_features(n, seed=1)
+    groups = sp.group_species(z, 4)
+    head = head_example.SpeciesHead(4, h.shape[2], 48, gen(5))
+    energy = head(h, z, groups, graph, n)
+    energy.square().sum().backward()
+    # the same in 64 bits; the weight gradient of what the 8-bit rows stand for, by exchanging them behind the forward
+    p = {k: v.detach().double().requires_grad_() for k, v in head.named_parameters()}
+    kept = sp.restore_rows(sp.checkpoint_rows(h)).double()
+
+    def plain(rows):
+        y = torch.einsum("ndk,nkm->ndm", rows, p["weight"][z.long()]) * h.shape[2]**-0.5
+        return y
+
+    y = plain(h.double())
+    y = y + (plain(kept) - plain(kept).detach()) - (y - y.detach())  # the value of h, the gradient of `kept`
+    y0 = y[:, 0] + p["table"][z.long()]
+    atom = torch.tanh(y0) @ p["scalar"] + y[:, 1:].square().sum(1) @ p["vector"]
+    want = torch.zeros(n, device="cuda", dtype=torch.float64).index_add(0, graph, atom) / graph.bincount(minlength=n)
+    want.square().sum().backward()
+    # fp32 sums of a few thousand terms each way: 2^-16 of the largest value covers their roundings and torch's
+    assert (energy.double() - want).abs().max() <= 2.0**-16 * want.abs().max()
+    for name, q in p.items():
+        got = getattr(head, name).grad.double()
+        assert (got - q.grad).abs().max() <= 2.0**-16 * q.grad.abs().max(), name
+
+
+def test_head_example_learns(head_example):
+    losses = head_example.train(n_structures=8, steps=60)
+    assert losses[-1] < 0.2 * losses[0]
