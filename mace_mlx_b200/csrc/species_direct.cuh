@@ -113,8 +113,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
               reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
   const uint32_t tmem = *tslot;
-  if (WG && blockIdx.x == 0)
-    for (int i = tid; i <= p.G; i += SL_THREADS) p.units[i] = pre[i];
+  if (WG && blockIdx.x == 0) write_spans<SL_THREADS>(p, q);
   const int t0 = q.bounds[0], t1 = q.bounds[1];
   if (t0 >= t1) {
     if (!WG && warp >= 5 && warp < 8) zero_rows<bf16>(p);

@@ -74,7 +74,8 @@ struct SlParams {
   int out32;
   int vst;              // map: rows of `out` are whole 16-byte pieces; weight gradient: bytes of a vector store (32, 16, 0)
   float* part;          // weight gradient: partial tiles
-  int* units;           // weight gradient: first unit of each group, written by CTA 0 for the join (G + 1)
+  int* spans;           // weight gradient: a group's first share, and its last in the upper 16 bits (-1: no rows),
+                        // written by CTA 0 for the join
   const int32_t* order;
   const int32_t* offsets;
   int64_t n;
@@ -410,6 +411,22 @@ __device__ __forceinline__ void load_groups(const SlParams& p, int unit_rows, in
     if (share + 1 == shares && s == all) q.bounds[1] = (int)min(all, (int64_t)INT32_MAX);
   }
   __syncthreads();
+}
+
+// Weight gradient: the shares of every group, for the join.  Share of unit u: the largest s with
+// floor(s all / shares) <= u.
+template <int THREADS>
+__device__ __forceinline__ void write_spans(const SlParams& p, const Groups& q) {
+  const int64_t all = q.pre[p.G];
+  const int shares = (int)min((int64_t)p.shares, all);
+  auto share_of = [&](int64_t u) -> int {
+    const int64_t x = (u + 1) * shares - 1;
+    return min(x <= UINT32_MAX ? (int)((uint32_t)x / (uint32_t)all) : (int)(x / all), shares - 1);
+  };
+  for (int g = threadIdx.x; g < p.G; g += THREADS) {
+    const int64_t u0 = q.pre[g], u1 = q.pre[g + 1];
+    p.spans[g] = u0 < u1 ? share_of(u0) | share_of(u1 - 1) << 16 : -1;
+  }
 }
 
 // The steps of a CTA, in order; every role walks the same ones, holding little (the rest is in shared memory).
@@ -1144,19 +1161,13 @@ __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constan
   pdl_wait();
   __shared__ float4 part[4][64];
   const int g = blockIdx.x, tid = threadIdx.x;
-  const int64_t before = p.units[g], mine = p.units[g + 1] - before, all = p.units[p.G];
+  const int span = p.spans[g];
+  const int s0 = span & 0xffff, s1 = span >> 16;  // shares of the group; none: s1 = -1
+  if (s0 == s1) return;                           // written by its only share
   const int tile = blockIdx.z;
   const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
   const int lane = tid & 63, sl = tid >> 6;
   const int kl = (blockIdx.y & 15) * 8 + (lane & 7), block = blockIdx.y >> 4;
-  int s0 = 0, s1 = -1;  // shares of the group
-  if (mine > 0) {
-    // share of unit u: the largest s with floor(s all / shares) <= u
-    const int64_t shares = min((int64_t)p.shares, all);
-    s0 = (int)min(((before + 1) * shares - 1) / all, shares - 1);
-    s1 = (int)min(((before + mine) * shares - 1) / all, shares - 1);
-    if (s0 == s1) return;  // written by its only share
-  }
   const float4* const first = reinterpret_cast<const float4*>(p.part) +
                               ((int64_t)tile * (p.shares + p.G) + g) * 32 * p.NT + kl;
   T* const row = static_cast<T*>(p.out) + ((int64_t)g * p.K + k0 + kl) * p.N + n0;
@@ -1370,7 +1381,7 @@ extern "C" int mace_species_linear_wgrad_workspace(int64_t n, int32_t d, int32_t
     return fail(MACE_ERR_BAD_ARG, "mace_species_linear_wgrad_workspace: bad arguments");
   SlParams p{};
   wgrad_split(n, d, G, K, M, &p);
-  *bytes = partial_bytes(p, G) + (int64_t)(G + 1) * 4;
+  *bytes = partial_bytes(p, G) + (int64_t)G * 4;
   return MACE_OK;
 }
 
@@ -1411,7 +1422,7 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
     MACE_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)G * K * M * es, s));
     return MACE_OK;
   }
-  p.units = reinterpret_cast<int*>(static_cast<char*>(ws) + partial_bytes(p, G));
+  p.spans = reinterpret_cast<int*>(static_cast<char*>(ws) + partial_bytes(p, G));
   const int grid = p.shares * p.n_ct * p.n_kt;
   const bool vec = aligned_rows(p.a, n, d, xe) && aligned_rows(p.b, n, d, es);
   auto go = [&](auto ta, auto t) {

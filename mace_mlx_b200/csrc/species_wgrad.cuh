@@ -239,8 +239,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_co
   const int tiles = p.n_ct * p.n_kt, share = blockIdx.x / tiles, tile = blockIdx.x % tiles;
   load_groups<WG_THREADS>(p, SL_KC, 1, 0, share, p.shares, true, q, reinterpret_cast<int64_t*>(smem));
   tc::fence_after_sync();
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= p.G; i += WG_THREADS) p.units[i] = pre[i];
+  if (blockIdx.x == 0) write_spans<WG_THREADS>(p, q);
   const int t0 = q.bounds[0], t1 = q.bounds[1];
   if (t0 >= t1) {
     if (warp == 20) tc::tmem_dealloc(SL_D, SL_TMEM);
