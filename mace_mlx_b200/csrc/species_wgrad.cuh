@@ -99,7 +99,7 @@ struct Wg {
   static constexpr int OFF_BAR = OFF_PRE + Groups::INTS * 4;
   static constexpr int NBAR = 13;
   static constexpr int BYTES = OFF_BAR + NBAR * 8 + 16;
-  static_assert(BYTES <= 232448 && OFF_PRE % 8 == 0, "shared memory of a CTA");
+  static_assert(BYTES <= 232448 && OFF_MIS % 16 == 0 && OFF_SCALE % 16 == 0 && OFF_PRE % 8 == 0, "shared memory of a CTA");
   // the rows of the units fetched before the first wait come from TeamRows::init, and later waits cover later ones
   static_assert(NU_A <= 2 * TeamRows::AHEAD && NU_B <= 2 * TeamRows::AHEAD, "units in flight");
 };
@@ -114,6 +114,7 @@ __device__ __forceinline__ void tmem_st8u(uint32_t a, const uint32_t* v) {
 // h * 16 .. h * 16 + 15 of `rows` (zeros for a row that does not exist or past its end).  Aligned rows (VEC) come in
 // 16-byte pieces, other rows of 4-byte values value by value, and those of smaller ones as the 16-byte pieces that
 // contain the segment, mis[r] saying where it starts in the first.
+// (600 000 rows 97 x 61: fp32 156 us, 8-bit x 147; with the 4-byte values in pieces too 163 and 162.)
 template <bool VEC>
 struct UnitRows {
   uint32_t mine, have;  // this lane's row in 16 bytes (aligned), which rows exist
@@ -169,22 +170,31 @@ __device__ __forceinline__ void fetch_unit(uint32_t dst, const RowView& v, const
       }
     }
   } else {
-    constexpr int PPR = SEG / 16 + 1;
+    // lane l: piece l % PPR of rows l / PPR + i RPI, then the last piece of row l
+    constexpr int PPR = SEG / 16, RPI = 32 / PPR;
     const char* const dummy = reinterpret_cast<const char*>(reinterpret_cast<uint64_t>(v.data) & ~(uint64_t)15);
     const int seg = max(min(row_bytes - at, SEG), 0);  // bytes of a row in this segment
     if ((lane >> 4) == h) mis[lane & 15] = (uint8_t)(rows.from & 15);
+    // (the segment and 16 bytes more are inside the rows: every piece is whole)
+    const bool inside = rows.have == 0xffffffffu && at + SEG + 16 <= row_bytes;
+    auto copy = [&](uint64_t f, int r, int j) {
+      const char* const src = reinterpret_cast<const char*>((f & ~(uint64_t)15) + 16 * j);
+      if (inside) {
+        cp_async16(dst + r * PITCH + j * 16, src);
+      } else {
+        const int left = (int)(f & 15) + seg - 16 * j;
+        const uint32_t bytes = f == 0 || seg == 0 || left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
+        // (a copy of no bytes still names an aligned address)
+        cp_async16(dst + r * PITCH + j * 16, bytes ? src : dummy, bytes);
+      }
+    };
 #pragma unroll
-    for (int i = 0; i < (WG_UNIT * PPR + 31) / 32; ++i) {
-      const int k = i * 32 + lane;
-      const int r = k / PPR, j = k - r * PPR;
-      const uint64_t f = __shfl_sync(0xffffffffu, rows.from, (h * 16 + r) & 31);
-      if (r >= WG_UNIT) continue;
-      const int left = (int)(f & 15) + seg - 16 * j;
-      const uint32_t bytes = f == 0 || seg == 0 || left <= 0 ? 0u : (left < 16 ? (uint32_t)left : 16u);
-      // (a copy of no bytes still names an aligned address)
-      cp_async16(dst + r * PITCH + j * 16, bytes ? reinterpret_cast<const char*>((f & ~(uint64_t)15) + 16 * j) : dummy,
-                 bytes);
+    for (int i = 0; i < WG_UNIT / RPI; ++i) {
+      const int r = i * RPI + lane / PPR;
+      copy(__shfl_sync(0xffffffffu, rows.from, h * 16 + r), r, lane % PPR);
     }
+    const uint64_t f = __shfl_sync(0xffffffffu, rows.from, h * 16 + (lane & 15));
+    if (lane < WG_UNIT) copy(f, lane, PPR);
   }
 }
 
@@ -295,11 +305,13 @@ __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_co
         }
         // this lane's channel of 16 rows
         uint32_t out[PA][WG_UNIT / 2];
+        const uint4 off = ANY ? load_as<uint4>(ms) : make_uint4(0, 0, 0, 0);
+        const uint32_t skip[4] = {off.x, off.y, off.z, off.w};  // a byte per row
 #pragma unroll
         for (int r = 0; r < WG_UNIT; r += 2) {
           uint32_t t[3];
-          split2<PA>(load_f32<TA>(src + r * S::PITCH_A + (ANY ? ms[r] : 0)),
-                     load_f32<TA>(src + (r + 1) * S::PITCH_A + (ANY ? ms[r + 1] : 0)), t);
+          split2<PA>(load_f32<TA>(src + r * S::PITCH_A + (skip[r >> 2] >> (8 * (r & 3)) & 0xff)),
+                     load_f32<TA>(src + (r + 1) * S::PITCH_A + (skip[r >> 2] >> (8 * (r & 3) + 8) & 0xff)), t);
 #pragma unroll
           for (int a = 0; a < PA; ++a) out[a][r / 2] = t[a];
         }
@@ -352,7 +364,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_co
         if (i < 0) continue;
         const uint8_t* const src = smem + S::OFF_B + (w8 * NU + slot) * S::UNIT_B + lane * (int)sizeof(T);
         const uint8_t* const ms = mis + slot * WG_UNIT;
-        const float* const ss = sc + slot * WG_UNIT;
+        const uint8_t* const ss = reinterpret_cast<const uint8_t*>(sc + slot * WG_UNIT);
         slot = slot + 1 == NU ? 0 : slot + 1;
         const int it = i >> 1, half = i & 1, s = it & 1;
         if (!half) {
@@ -362,12 +374,13 @@ __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_co
         }
 #pragma unroll
         for (int h = 0; h < WG_UNIT / 8; ++h) {
-          float v[8];
+          float v[8], scale[8];
+          const uint2 off = ANY ? load_as<uint2>(ms + 8 * h) : make_uint2(0, 0);
+          if constexpr (sizeof(TA) == 1) load_eight(ss + 32 * h, scale, float{});
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const int r = 8 * h + j;
-            v[j] = load_f32<T>(src + r * S::PITCH_B + (ANY ? ms[r] : 0));
-            if constexpr (sizeof(TA) == 1) v[j] *= ss[r];
+            v[j] = load_f32<T>(src + (8 * h + j) * S::PITCH_B + ((j < 4 ? off.x : off.y) >> (8 * (j & 3)) & 0xff));
+            if constexpr (sizeof(TA) == 1) v[j] *= scale[j];
           }
           put_eight<PB>(img + s * (PB * SL_IMG), SL_IMG, n, team * 4 + half * 2 + h, v);
         }
