@@ -51,9 +51,10 @@ struct GroupCfg {
   static constexpr int BYTES = (BINS + WARPS * WORDS + 32) * 4;
   static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
-// short lists: one CTA does the whole sort in one launch
+// short lists: one CTA does the whole sort in one launch (89 groups: 1000 rows 3.5 us against 6.3 in three launches, 4096
+// 6.2 against 7.9, 8192 10.1 against 8.3)
 constexpr int GS_THREADS = 1024;
-constexpr int GS_MAX_ROWS = 8192;
+constexpr int GS_MAX_ROWS = 6144;
 constexpr int GS_MAX_BINS = 256;  // (shared memory of a static size)
 
 // key of a row: its species, or num_groups for padding rows
@@ -437,17 +438,20 @@ constexpr int EG_THREADS = 256;
 // A warp sums its share of the grouped list, V channels per lane and RL rows side by side.  The list is read and its
 // rows are loaded UN RL at a time whatever groups they belong to; a group's end only cuts the additions, so that no
 // load waits for a group before it.  1M fp32 rows of 128 channels: 4 groups 88 us with the join, 7921 groups 104 (79 is
-// what HBM needs; group by group 92 and 112); 300 000 rows of 97: 67 (73).
-template <typename T, int V, int RL>
+// what HBM needs; group by group 92 and 112).  APART: rows that are not whole 16-byte pieces, a lane's channels 32
+// apart, so that a warp still has 128 channels of 8 rows in flight: 1M rows of 97 channels fp32 87 us, bf16 76 (with
+// one channel per lane 212 and 178).
+template <typename T, int V, int RL, bool APART = false>
 __global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad(EmbedGrad p) {
   pdl_wait();
   constexpr int CL = 32 / RL;          // channel lanes
   constexpr int UN = RL == 8 ? 4 : 8;  // row loads in flight per lane
+  constexpr int HOP = APART ? CL : 1;  // from one channel of a lane to the next
   constexpr int R = UN * RL;           // rows at a time (at most 32)
   const int lane = threadIdx.x & 31, cl = lane % CL, rl = lane / CL;
   const int64_t share = blockIdx.x * (int64_t)(EG_THREADS / 32) + (threadIdx.x >> 5);
   if (share >= p.shares) return;
-  const int c0 = (blockIdx.y * CL + cl) * V;
+  const int c0 = APART ? blockIdx.y * CL * V + cl : (blockIdx.y * CL + cl) * V;
   const bool in = c0 < p.C;
   // (positions in 32 bits: n < 2^31, and none passes n by more than 64)
   const uint32_t i0 = (uint32_t)(share * p.share), i1 = (uint32_t)imin64(p.n, share * p.share + p.share);
@@ -478,25 +482,38 @@ __global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad(EmbedGrad p) {
       if (lo >= i0 && hi <= i1) {
 #pragma unroll
         for (int k = 0; k < V; ++k) acc[k] *= p.scale;
-        store_channels<T, V>(static_cast<T*>(p.out) + (int64_t)g * p.C + c0, acc);
+        T* const out = static_cast<T*>(p.out) + (int64_t)g * p.C + c0;
+        if constexpr (APART) {
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            if (k * HOP < p.C - c0) out[k * HOP] = from_f32<T>(acc[k]);
+        } else {
+          store_channels<T, V>(out, acc);
+        }
       } else {
         float* part = p.part + (share * 2 + (first ? 0 : 1)) * p.C + c0;
 #pragma unroll
-        for (int k = 0; k < V; ++k) part[k] = acc[k];
+        for (int k = 0; k < V; ++k)
+          if (!APART || k * HOP < p.C - c0) part[k * HOP] = acc[k];
       }
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) acc[k] = 0.f;
     first = false;
   };
-  Raw<T, V> v[UN];
+  Raw<T, V, APART> v[UN];
   int32_t mine = 0;
   auto load = [&](int j) {  // rows j .. j + R - 1 of the 32
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int64_t row = __shfl_sync(0xffffffffu, mine, j + u * RL + rl);
       v[u].zero();
-      if (row >= 0 && row < p.n && in) v[u].load(dy + row * p.ds);  // a row outside the tensor counts as none
+      if (row >= 0 && row < p.n && in) {
+        if constexpr (APART)
+          v[u].load(dy + row * p.ds, HOP, p.C - c0);
+        else
+          v[u].load(dy + row * p.ds);
+      }  // a row outside the tensor counts as none
     }
   };
   uint32_t b32 = i0;
@@ -613,6 +630,7 @@ __global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad_by_group(EmbedGrad
 // groups: zero.  A warp takes a group of few shares by itself; the CTA's 32
 // warps take the others together.  32 channels and per_cta groups per CTA and round (few groups: one each, so
 // that they are joined side by side).
+// (1M rows of 128 channels, 4 groups: 87 us, 157 with a warp to each; 89 groups 91 and 98)
 constexpr int EJ_ALONE = 16;
 
 template <typename T>
@@ -983,6 +1001,7 @@ int embed(const void* table, int64_t ts, int G, int C, const int32_t* species, i
   auto go = [&](auto kernel, int v) {
     return launch("species_embed", kernel, grid(v), RW_THREADS, 0, s, t, ts, G, C, species, n, scale, o, os, row_div(C));
   };
+  // 1M rows of 128 fp32 channels 79 us (114 as a FLAT result, 215 one by one); of 97 channels 94 FLAT, 164 one by one
   if (C % V == 0 && ts % V == 0 && os % V == 0 && aligned16(table) && aligned16(out)) return go(k_embed<T, V, false>, V);
   if (os == C && aligned16(out)) return go(k_embed<T, V, true>, V);
   return go(k_embed<T, 1, false>, 1);
@@ -1029,6 +1048,12 @@ int launch_embed_grad(const EmbedGrad& p, cudaStream_t s) {
     if (cl <= 16) return go(k_embed_grad_by_group<T, V, 2>, 16);
     return go(k_embed_grad_by_group<T, V, 1>, 32);
   } else {
+    // (rows that are not whole pieces: four channels per lane, 32 apart, so that a warp has the row)
+    if constexpr (V == 1)
+      if (p.C > 32) {
+        const dim3 grid(gx, (p.C + 127) / 128);
+        return launch("species_embed_grad", k_embed_grad<T, 4, 1, true>, grid, EG_THREADS, 0, s, p);
+      }
     if (cl <= 4) return go(k_embed_grad<T, V, 8>, 4);
     if (cl <= 8) return go(k_embed_grad<T, V, 4>, 8);
     if (cl <= 16) return go(k_embed_grad<T, V, 2>, 16);

@@ -98,10 +98,10 @@ __device__ __forceinline__ void store4(bf16* dst, const float* v) {
   *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t);
 }
 
-// V channels as loaded: one 16-byte piece where they fill it, else single values
-template <typename T, int V>
+// V channels as loaded: one 16-byte piece where they fill it, else single values; APART: never neighbours
+template <typename T, int V, bool APART = false>
 struct Raw {
-  static constexpr bool PIECE = V * sizeof(T) == 16;
+  static constexpr bool PIECE = !APART && V * sizeof(T) == 16;
   uint4 piece;
   T one[PIECE ? 1 : V];
   __device__ __forceinline__ void zero() {
@@ -115,6 +115,12 @@ struct Raw {
       piece = __ldg(reinterpret_cast<const uint4*>(src));
     else
       for (int k = 0; k < V; ++k) one[k] = src[k];
+  }
+  // channels `hop` apart, those below `left`
+  __device__ __forceinline__ void load(const T* __restrict__ src, int hop, int left) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k * hop < left) one[k] = src[k * hop];
   }
   __device__ __forceinline__ void add_to(float* acc) const {
     if constexpr (!PIECE) {

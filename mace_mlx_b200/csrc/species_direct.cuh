@@ -8,7 +8,7 @@
 //
 // all in the 128-byte swizzled layout (piece j of line l at j ^ (l & 7)), from a ring of DR_NS steps of 64.
 // Accumulation stays in TMEM over a whole tile (map) or SL_LONG steps (weight gradient; the truncation of each
-// addition is 2^-24 of the sum, the result is rounded to 2^-9).  Roles of a CTA (16 warps, one CTA per SM):
+// addition is 2^-24 of the sum, the result is rounded to 8 bits).  Roles of a CTA (16 warps, one CTA per SM):
 //   warps 0-3   rows of x;  warps 4-7  map: weights (kept while the tiles share them) and the MMAs, zero rows;
 //               weight gradient: rows of dy;  warps 8-15  epilogue (weight gradient: warp 8 issues the MMAs)
 // Waits are bounded as in species_linear.cu.

@@ -12,7 +12,7 @@
 // values are exact in one bf16 piece and their row scale is folded into dy.
 // The tensor core truncates when it accumulates, so an accumulator takes one
 // 64-wide step of K, smallest products first, and the epilogue warps add the
-// steps in fp32 registers (bf16 alone, whose result is rounded to 2^-9, takes
+// steps in fp32 registers (bf16 alone, whose result is rounded to 8 bits, takes
 // several steps).
 //
 // Roles of a CTA of the map (16 warps, one CTA per SM, a share of the tiles of equal cost):
@@ -330,7 +330,7 @@ struct Groups {
 template <typename T, bool VEC>
 struct Sl {
   static constexpr int P = sizeof(T) == 4 ? 3 : 1;  // pieces of a value
-  static constexpr bool LONG = P == 1;              // sums of a whole tile (the result is rounded to 2^-9)
+  static constexpr bool LONG = P == 1;              // sums of a whole tile (the result is rounded to 8 bits)
   static constexpr int PITCH = 128 + (VEC ? 0 : 16);  // of a ring unit: 32 rows x 128 bytes
   static constexpr int UPC = SL_KC * (int)sizeof(T) / 128;  // ring units per step of 64
   static constexpr int NU = 5;
@@ -342,7 +342,7 @@ struct Sl {
   static constexpr int OFF_MIS = OFF_STG + 8 * STG;  // per ring unit and row: misalignment
   static constexpr int OFF_PRE = OFF_MIS + (VEC ? 0 : 4 * NU * 32);
   static constexpr int OFF_BAR = OFF_PRE + Groups::INTS * 4;
-  static constexpr int NBAR = 8 + 2 * MAX_SLOTS + 2;
+  static constexpr int NBAR = 8 + 2 * MAX_SLOTS + 1;
   static constexpr int BYTES = OFF_BAR + NBAR * 8 + 32;
   static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
@@ -682,60 +682,17 @@ __device__ __forceinline__ void put_eight(uint8_t* img, int piece, int n, int ch
     store_piece(img + b * piece + n * 128 + ((chunk ^ (n & 7)) << 4), t[0][b], t[1][b], t[2][b], t[3][b]);
 }
 
-// Where weight (k, n) of a step waits, as it is, in its own image slot.  More than 64 columns are rewritten in two
-// rounds of 64: the second 64 wait where the images of the first are not written.
-template <typename T>
-__device__ __forceinline__ uint32_t raw_place(int k, int n, bool transposed, int NT) {
-  if (NT <= 64) return (transposed ? n * SL_KC + k : k * NT + n) * (int)sizeof(T);
-  if (sizeof(T) == 2) return transposed ? n * 128 + k * 2 : (n >> 6) * 8192 + k * 128 + (n & 63) * 2;
-  return transposed ? ((n >> 5) & 1) * 16384 + (n >> 6) * 8192 + (n & 31) * 256 + k * 4
-                    : (k >> 5) * 16384 + (n >> 6) * 8192 + (k & 31) * 256 + (n & 63) * 4;
-}
-
 // Map: the weight images of steps [k0, k0 + nk) of (group g, column tile ct), at img0 + step * stride, by warps
-// 4 to 7; full: the first step's barrier (arrived on as each step is done).  Weights of whole 16-byte pieces come
-// as they are by cp.async into their own image slots, all steps at once (one memory latency for the whole set),
-// and are rewritten in place through registers, 64 image rows at a time; others are loaded value by value.  A
-// round is 16 items of 32 (image row, K octet) pairs, one per lane, four items per warp.  Weights (K, N): an item
-// is one octet of 32 neighbouring columns; transposed (N, K): 8 octets of 4 rows.
+// 4 to 7; full: the first step's barrier (arrived on as each step is done).  A round is 64 image rows of a step:
+// 16 items of 32 (image row, K octet) pairs, one per lane, four items per warp, with all of their loads in flight
+// (through shared memory by cp.async, rewritten in place, was slower: 40 000 fp32 rows 128 -> 128 20.6 us, 19.0 so).
+// Weights (K, N): an item is one octet of 32 neighbouring columns; transposed (N, K): 8 octets of 4 rows.
 template <typename T, int PB>
-__device__ __forceinline__ bool fill_weights(const SlParams& p, uint8_t* img0, int stride, int g, int ct, int k0,
-                                             int nk, uint32_t full, uint32_t w_sync_bar, int& syncs,
-                                             volatile int* abort) {
+__device__ __forceinline__ void fill_weights(const SlParams& p, uint8_t* img0, int stride, int g, int ct, int k0,
+                                             int nk, uint32_t full) {
   const int lane = threadIdx.x & 31, w4 = (threadIdx.x >> 5) & 3;
   const int NT = p.NT;
-  auto w_sync = [&]() -> bool {  // the four warps meet (a bounded wait, unlike a barrier)
-    warp_arrive(w_sync_bar);
-    return __all_sync(0xffffffffu, wait_phase(w_sync_bar, syncs++ & 1, abort));
-  };
   const T* wt = static_cast<const T*>(p.w) + (int64_t)g * p.K * p.N;
-  if (p.w_vec) {
-    constexpr int E = 16 / sizeof(T);  // elements of a piece
-    // rows of a step: 64 of NT weights, transposed NT of 64; a warp takes as many as its lanes hold pieces of
-    const int ppr = (p.transposed ? SL_KC : NT) / E, rpi = 32 / ppr;
-    const int rows = p.transposed ? NT : SL_KC, pitch = p.transposed ? p.K : p.N;
-    const int sub = lane / ppr, c = (lane - sub * ppr) * E;
-    const bool on = sub < rpi;
-#pragma unroll 1
-    for (int s = 0; s < nk; ++s) {
-      const uint32_t raw = tc::smem_u32(img0) + s * stride;
-      const int k = (k0 + s) * SL_KC, n = ct * NT;
-      const int r0 = p.transposed ? n : k, c0 = (p.transposed ? k : n) + c;  // in the whole matrix
-      const int r_end = p.transposed ? p.N : p.K, c_end = p.transposed ? p.K : p.N;
-      int r = w4 * rpi + sub;
-      const T* src = wt + (int64_t)(r0 + r) * pitch + c0;
-      const int64_t hop = (int64_t)(4 * rpi) * pitch;
-#pragma unroll 8
-      for (; r < rows && on; r += 4 * rpi, src += hop) {
-        const bool in = r0 + r < r_end && c0 < c_end;
-        cp_async16_or_zero(raw + raw_place<T>(p.transposed ? c : r, p.transposed ? r : c, p.transposed, NT), in ? src : wt,
-                           !in);
-      }
-    }
-    cp_commit();
-    cp_wait<0>();
-    if (!w_sync()) return false;
-  }
 #pragma unroll 1
   for (int s = 0; s < nk; ++s) {
     uint8_t* const img = img0 + s * stride;
@@ -746,23 +703,22 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint8_t* img0, i
       for (int u = 0; u < 4; ++u) {
         const int j = h * 16 + u * 4 + w4;
         const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane, kk = (p.transposed ? lane & 7 : j & 7) * 8;
-        if (n >= NT) continue;
-        if (p.w_vec) {
-          if (p.transposed) {
-            load_eight(img + raw_place<T>(kk, n, true, NT), v[u], T{});
+        const int col = ct * NT + n, k = (k0 + s) * SL_KC + kk;
+        const bool in = n < NT && col < p.N;
+        if (p.transposed && p.w_vec) {
+          if (in && k + 8 <= p.K) {
+            load_eight(reinterpret_cast<const uint8_t*>(wt + (int64_t)col * p.K + k), v[u], T{});
           } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[u][e] = load_f32<T>(img + raw_place<T>(kk + e, n, false, NT));
+            for (int e = 0; e < 8; ++e) v[u][e] = in && k + e < p.K ? to_f32(wt[(int64_t)col * p.K + k + e]) : 0.f;
           }
         } else {
-          const int col = ct * NT + n, k = (k0 + s) * SL_KC + kk;
           const T* src = p.transposed ? wt + (int64_t)col * p.K + k : wt + (int64_t)k * p.N + col;
           const int64_t step = p.transposed ? 1 : p.N;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[u][e] = n < NT && col < p.N && k + e < p.K ? to_f32(src[e * step]) : 0.f;
+          for (int e = 0; e < 8; ++e) v[u][e] = in && k + e < p.K ? to_f32(src[e * step]) : 0.f;
         }
       }
-      if (p.w_vec && !w_sync()) return false;  // every raw value of the round is in registers
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int j = h * 16 + u * 4 + w4;
@@ -777,7 +733,6 @@ __device__ __forceinline__ bool fill_weights(const SlParams& p, uint8_t* img0, i
     tc::fence_proxy_async();
     warp_arrive(full + 8 * s);
   }
-  return true;
 }
 
 template <typename T, bool VEC>
@@ -797,7 +752,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
   auto D_FREE = [&](int s) { return bar(6 + s); };
   auto B_FULL = [&](int s) { return bar(8 + s); };
   auto B_FREE = [&](int s) { return bar(8 + S::MAX_SLOTS + s); };
-  const uint32_t DONE = bar(8 + 2 * S::MAX_SLOTS), W_SYNC = bar(9 + 2 * S::MAX_SLOTS);
+  const uint32_t DONE = bar(8 + 2 * S::MAX_SLOTS);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be uniform
 
@@ -821,7 +776,6 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
         tc::mbar_init(B_FREE(s), 1);
       }
       tc::mbar_init(DONE, 1);
-      tc::mbar_init(W_SYNC, 4);
       tc::fence_barrier_init();
     }
     __syncwarp();
@@ -989,10 +943,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
       return true;
     };
     bool ok = true;
-    int syncs = 0;
-    auto fill = [&](int g, int ct, int k0, int nk, int slot0) -> bool {
-      return fill_weights<T, P>(p, smem + slot0 * P * p.img, P * p.img, g, ct, k0, nk, bar(8 + slot0), W_SYNC, syncs,
-                                abort);
+    auto fill = [&](int g, int ct, int k0, int nk, int slot0) {
+      fill_weights<T, P>(p, smem + slot0 * P * p.img, P * p.img, g, ct, k0, nk, bar(8 + slot0));
     };
     Walk w;
     w.init(p, q, t0);
@@ -1003,8 +955,9 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
         // the tiles of this CTA that share the weights
         const int run = min(t.run, t1 - w.t);
         for (int k = 0; k < n_k && ok && fills > 0; ++k) ok = wait_phase(B_FREE(k), (fills - 1) & 1, abort);
-        ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, 0, n_k, 0);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        fill(w.g, t.ct, 0, n_k, 0);
         if (warp == 4 && elect_one())
           for (int i = 0; i < run && ok; ++i)
             for (int k = 0; k < n_k && ok; ++k)
@@ -1018,7 +971,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
         for (int k = 0; k < n_k && ok; ++k, ++it, ++fills) {
           const int s = fills % p.slots, use = fills / p.slots;
           ok = use == 0 || wait_phase(B_FREE(s), (use - 1) & 1, abort);
-          ok = __all_sync(0xffffffffu, ok) && fill(w.g, t.ct, k, 1, s);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) fill(w.g, t.ct, k, 1, s);
           if (ok && warp == 4 && elect_one())
             ok = issue(it, s, use, true, S::LONG ? tile_no : it, !S::LONG || k == 0, !S::LONG || k + 1 == n_k);
           ok = __all_sync(0xffffffffu, ok);
@@ -1155,7 +1109,9 @@ namespace {
 
 // dW of the groups that several shares hold, in share order, and of empty groups (zero).  CTA (g, y, tile): group g,
 // rows 8 (y % 16) .. of the tile, in blocks of 8 rows x 8 column quads (64 lanes).  Few shares: the four sets of 64
-// threads of the CTAs with y < 16 take a block each; many: CTA y takes block y / 16, each set every fourth share.
+// threads of the CTAs with y < 16 take a block each; many: CTA y takes block y / 16, each set every fourth share
+// (gradients of 40 000 rows 128 x 128 in 4 groups: 19.1 us, 32.6 with one set per block; 300 000 rows in 89: no
+// difference).
 template <typename T>
 __global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constant__ SlParams p) {
   pdl_wait();
@@ -1346,10 +1302,12 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.N = M;
   p.w_vec = (transpose ? K : M) * es % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
   p.alpha = alpha;
+  // direct: bf16 in whole pieces, nothing to convert (600 000 rows 128 -> 128: 57 us, 82 by the general kernel)
   const bool vec = aligned_rows(p.a, n, d, es), direct = dtype == MACE_BF16 && vec && p.w_vec;
   const int sms = sm_count();
   const int64_t row_tiles = (n * d + 127) / 128;
-  // narrower column tiles while the row tiles leave SMs idle
+  // narrower column tiles while the row tiles leave SMs idle (3000 fp32 rows 128 -> 128: 11.1 us, 16.5 with tiles of
+  // 128 columns; bf16 no difference)
   int most = 128;
   while (most > 32 && row_tiles * ((M + most - 1) / most) * 2 <= sms) most /= 2;
   // and so narrow that the weight images of the whole K stay in shared memory (K <= 512), rather than being made
@@ -1364,12 +1322,12 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.slots = image_slots(p.NT, pieces, &p.img);
   p.n_ct = (M + p.NT - 1) / p.NT;
   p.n_kt = 1;
-  // Making a group's images (9 000 cycles) costs about as much as 1.5 row tiles.  40 000 rows of 4 species 128 -> 128
+  // Making a group's images costs about as much as 1.5 row tiles.  40 000 rows of 4 species 128 -> 128
   // fp32 26.5 us without it, 20.7 with 2 to 6; 600 000 rows 133, 130.4 with 4, 129.1 with 6.  bf16 rows copied as they
   // lie (direct): no difference.
   p.start = !direct && n_k <= p.slots ? 4 : 0;
   const int grid = (int)std::min<int64_t>(sms, (row_tiles + std::min<int64_t>(G, n)) * p.n_ct);
-  if (direct) return launch_direct<false>(p, grid, s);  // bf16 in whole pieces: nothing to convert
+  if (direct) return launch_direct<false>(p, grid, s);
   if (dtype == MACE_F32)
     return vec ? launch_map<float, true>(p, grid, s) : launch_map<float, false>(p, grid, s);
   return launch_map<bf16, false>(p, grid, s);

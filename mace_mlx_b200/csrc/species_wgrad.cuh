@@ -84,7 +84,7 @@ template <typename TA, typename T, bool VEC>
 struct Wg {
   static constexpr int PA = sizeof(TA) == 4 ? 3 : 1;
   static constexpr int PB = sizeof(TA) == 2 ? 1 : 3;
-  static constexpr bool LONG = PA == 1 && PB == 1;  // sums of several steps (the result is rounded to 2^-9)
+  static constexpr bool LONG = PA == 1 && PB == 1;  // sums of several steps (the result is rounded to 8 bits)
   static constexpr int SEG_A = 32 * (int)sizeof(TA), SEG_B = 32 * (int)sizeof(T);  // bytes of a row in a unit
   static constexpr bool ANY_A = !VEC && sizeof(TA) < 4, ANY_B = !VEC && sizeof(T) < 4;  // see fetch_unit
   static constexpr int PITCH_A = SEG_A + (ANY_A ? 16 : 0), PITCH_B = SEG_B + (ANY_B ? 16 : 0);
