@@ -564,6 +564,44 @@ def test_groupings_that_are_not_permutations_stay_in_bounds(sp):
     assert sp.error_flag() == 0
 
 
+# ------------------------------------------------------------- ends and repeats
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [1, 8, 33, 61, 64, 128, 129, 250])
+def test_embedding_gradient_at_group_ends(sp, dtype, c):
+    # groups that end with, before and after the 8, 16 or 32 rows read at a time, empty ones between them, one over many
+    # warps' shares, padding last
+    sizes = [0, 1, 31, 32, 33, 0, 0, 64, 7, 8, 9, 16, 0, 1, 1, 1, 4096, 32, 128, 0, 5, 27, 0]
+    z = torch.cat([torch.full((k,), i, dtype=torch.int32) for i, k in enumerate(sizes)] + [torch.full((40,), -1, dtype=torch.int32)])
+    z = z[torch.randperm(len(z), generator=torch.Generator().manual_seed(c))].cuda()
+    g = len(sizes)
+    dy = randn(len(z), c, seed=c, dtype=dtype)
+    dy[z < 0] = float("nan")
+    got = sp.species_embedding_grad(dy, sp.group_species(z, g))
+    ok = z >= 0
+    want = torch.zeros(g, c, device="cuda", dtype=torch.float64).index_add_(0, z[ok].long(), dy[ok].double())
+    mass = torch.zeros_like(want).index_add_(0, z[ok].long(), dy[ok].double().abs())
+    assert_sum(got, want, mass, max(sizes))
+
+
+@pytest.mark.parametrize("dtype,k,m", [(torch.float32, 128, 128), (torch.float32, 97, 61), (torch.bfloat16, 96, 96),
+                                       (torch.bfloat16, 97, 61)])
+def test_equal_calls_give_equal_bits(sp, dtype, k, m):
+    n, d, g = 30_011, 3, 7
+    z = draw_species(n, g, 4, pad=0.01)
+    x, dy, w = randn(n, d, k, seed=1, dtype=dtype), randn(n, d, m, seed=2, dtype=dtype), randn(g, k, m, seed=3, dtype=dtype)
+
+    def everything():
+        groups = sp.group_species(z, g)
+        ck = sp.checkpoint_rows(x)
+        return [*groups, sp.species_linear(x, w, groups), *sp.species_linear_grad(x, dy, w, groups),
+                sp.species_linear_grad_weight(ck, dy, groups), sp.species_embedding_grad(x[:, 0], groups), *ck]
+
+    first = everything()
+    for _ in range(5):
+        for a, b in zip(first, everything(), strict=True):
+            assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------- together
 @pytest.fixture(scope="module")
 def head_example():
