@@ -35,8 +35,8 @@ RowDiv row_div(int C) { return {(uint32_t)((((uint64_t)1 << 32) + C - 1) / C), C
 // digit on (16 bits in shared memory: a share has fewer rows).  Ranks follow
 // the list order everywhere, so the order of atomics plays no part.
 //
-// 4M rows, 7921 groups: 49 us, of which the scatter is two thirds, bound by its
-// 4-byte stores (a sector each) and the chain from counter to counter; in two
+// 4M rows, 7921 groups: 45 us, of which the scatter is two thirds, bound by its
+// 4-byte stores (a sector each) and the latency of its few warps; in two
 // passes of 7 bits, put in digit order in shared memory before they are
 // stored, 98 us.  1000 groups: 38 us (89 in two passes); 89 groups: 36 us (40).
 // 16 000 groups take two passes (101 us): the counters of 14 bits would leave
@@ -164,21 +164,6 @@ __device__ __forceinline__ int place(C* count, int digit, bool in, unsigned same
   return before + rank;
 }
 
-// The same in a packed 16-bit counter, for digits that seldom meet within a warp: every row counts itself, and only
-// where two met (a counter is then further on than its own addition) are the lanes of equal digit found.
-template <int BITS>
-__device__ __forceinline__ int place_spread(uint32_t* pos, int digit, bool in, int lane) {
-  const int half = 16 * (digit & 1);
-  uint32_t before = 0, after = 0;
-  if (in) before = atomicAdd(&pos[digit >> 1], 1u << half) >> half & 0xffffu;
-  __syncwarp();
-  if (in) after = *reinterpret_cast<volatile uint32_t*>(&pos[digit >> 1]) >> half & 0xffffu;
-  __syncwarp();
-  if (!__any_sync(0xffffffffu, in && after != before + 1)) return before;
-  const unsigned same = same_digit<BITS>(digit, in);
-  return after - __popc(same) + __popc(same & ((1u << lane) - 1));
-}
-
 template <int BITS>
 __global__ void __launch_bounds__(GroupCfg<BITS>::THREADS, 1) k_group_scatter(GroupPass p) {
   using Cfg = GroupCfg<BITS>;
@@ -190,13 +175,12 @@ __global__ void __launch_bounds__(GroupCfg<BITS>::THREADS, 1) k_group_scatter(Gr
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   for (int k = tid; k < WARPS * WORDS; k += THREADS) pos[k] = 0;
   pdl_wait();
-  // totals and this CTA's counts of a run of PER digits per thread
   constexpr int PER = (BINS + THREADS - 1) / THREADS;
-  int total[PER], before[PER];
+  int before[PER];  // this CTA's counts of digits tid + k THREADS
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int b = tid * PER + k;
-    total[k] = b < BINS ? p.totals[b] : 0;
+    const int b = tid + k * THREADS;
+    if (b < BINS) base[b] = p.totals[b];
     before[k] = b < BINS ? p.counts[(int64_t)blockIdx.x * BINS + b] : 0;
   }
   __syncthreads();
@@ -209,17 +193,27 @@ __global__ void __launch_bounds__(GroupCfg<BITS>::THREADS, 1) k_group_scatter(Gr
     const int d = digit_of(p, key_of(p, i0 + i));
     atomicAdd(&mine[d >> 1], 1u << (16 * (d & 1)));
   }
+  // exclusive sums over the digits, PER neighbours per thread
   int sum = 0;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) sum += total[k];
+  for (int k = 0; k < PER; ++k) sum += tid * PER + k < BINS ? base[tid * PER + k] : 0;
   sum = cta_exclusive<THREADS>(sum, sums);
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int b = tid * PER + k;
     if (b >= BINS) break;
-    if (p.offsets && blockIdx.x == 0 && b <= p.G) p.offsets[b] = sum;
-    base[b] = sum + before[k];
-    sum += total[k];
+    const int total = base[b];
+    base[b] = sum;
+    sum += total;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int b = tid + k * THREADS;
+    if (b >= BINS) break;
+    const int at = base[b];
+    if (p.offsets && blockIdx.x == 0 && b <= p.G) p.offsets[b] = at;
+    base[b] = at + before[k];
   }
   // (cta_exclusive's barriers stand between the counts and this)
   for (int k = tid; k < WORDS; k += THREADS) {  // two digits at a time: neither half overflows
@@ -233,9 +227,8 @@ __global__ void __launch_bounds__(GroupCfg<BITS>::THREADS, 1) k_group_scatter(Gr
   }
   __syncthreads();
   constexpr int U = 4;  // rounds of 32 rows in flight
-  // (4M rows of 7921 groups 49 us, by ballots alone 55; of 4000 39 against 42, of 1000 no difference)
+  // (4M rows of 4000 groups 40 us, 49 by ballots; of 1000 no difference)
   constexpr bool SPREAD = BITS >= 12;
-  uint16_t* const mine16 = reinterpret_cast<uint16_t*>(mine);
   int z[U], r[U];
   auto load = [&](int i) {
 #pragma unroll
@@ -261,20 +254,43 @@ __global__ void __launch_bounds__(GroupCfg<BITS>::THREADS, 1) k_group_scatter(Gr
       r0[u] = r[u];
     }
     load(i + U * 32);
+    // The counters of U rounds in order, none waiting for the one before.  Spread digits: every row counts itself, and
+    // where two met (a counter is further on than its own addition) the lanes of equal digit are found afterwards;
+    // else they are found first and one of them counts them all.
     unsigned same[U];
-    if constexpr (!SPREAD) {
+    uint32_t first[U], last[U];  // rows of the digit before this one (before its lanes); SPREAD: after the round
 #pragma unroll
-      for (int u = 0; u < U; ++u) same[u] = same_digit<BITS>(digit_of(p, k0[u]), i + u * 32 + lane < rows);
+    for (int u = 0; u < U; ++u) {
+      const bool in = i + u * 32 + lane < rows;
+      const int d = digit_of(p, k0[u]), half = 16 * (d & 1);
+      volatile uint32_t* const word = mine + (d >> 1);
+      first[u] = last[u] = 0;
+      if constexpr (SPREAD) {
+        if (in) first[u] = atomicAdd(const_cast<uint32_t*>(word), 1u << half) >> half & 0xffffu;
+        __syncwarp();
+        if (in) last[u] = *word >> half & 0xffffu;
+        __syncwarp();
+      } else {
+        same[u] = same_digit<BITS>(d, in);
+        if (in) first[u] = *word >> half & 0xffffu;
+        __syncwarp();
+        if (in && (same[u] & ((1u << lane) - 1)) == 0) atomicAdd(const_cast<uint32_t*>(word), (uint32_t)__popc(same[u]) << half);
+        __syncwarp();
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool in = i + u * 32 + lane < rows;
       const int d = digit_of(p, k0[u]);
-      int at = base[d];
-      if constexpr (SPREAD)
-        at += place_spread<BITS>(mine, d, in, lane);
-      else
-        at += place(mine16, d, in, same[u], lane);
+      int at = base[d] + (int)first[u];
+      if constexpr (SPREAD) {
+        if (__any_sync(0xffffffffu, in && last[u] != first[u] + 1)) {
+          same[u] = same_digit<BITS>(d, in);
+          at = base[d] + (int)last[u] - __popc(same[u]) + __popc(same[u] & ((1u << lane) - 1));
+        }
+      } else {
+        at += __popc(same[u] & ((1u << lane) - 1));
+      }
       if (in) {
         if (p.out)
           p.out[at] = make_int2(k0[u], r0[u]);
