@@ -1326,9 +1326,9 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.slots = image_slots(p.NT, pieces, &p.img);
   p.n_ct = (M + p.NT - 1) / p.NT;
   p.n_kt = 1;
-  // Making a group's images costs about as much as 1.5 row tiles.  40 000 rows of 4 species 128 -> 128
-  // fp32 26.5 us without it, 20.7 with 2 to 6; 600 000 rows 133, 130.4 with 4, 129.1 with 6.  bf16 rows copied as they
-  // lie (direct): no difference.
+  // Making a group's images costs about as much as 1.5 row tiles.  40 000 fp32 rows of 4 species 128 -> 128 20.7 us
+  // without it, 17.4 with 1 to 6; 600 000 rows 130.8, 127.6 with 4, 126.3 with 6; 60 000 rows of 89 species 27.4, 24.5
+  // with 4, 26.2 with 6.  bf16 rows copied as they lie (direct): no difference.
   p.start = !direct && n_k <= p.slots ? 4 : 0;
   const int grid = (int)std::min<int64_t>(sms, (row_tiles + std::min<int64_t>(G, n)) * p.n_ct);
   if (direct) return launch_direct<false>(p, grid, s);
