@@ -51,8 +51,8 @@ struct GroupCfg {
   static constexpr int BYTES = (BINS + WARPS * WORDS + 32) * 4;
   static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
-// short lists: one CTA does the whole sort in one launch (89 groups: 1000 rows 3.5 us against 6.3 in three launches, 4096
-// 6.2 against 7.9, 8192 10.1 against 8.3)
+// short lists: one CTA does the whole sort in one launch (89 groups: 1000 rows 3.5 us against 6.3 in three launches,
+// 4096 rows 6.2 against 7.9, 8192 rows 10.1 against 8.3)
 constexpr int GS_THREADS = 1024;
 constexpr int GS_MAX_ROWS = 6144;
 constexpr int GS_MAX_BINS = 256;  // (shared memory of a static size)
@@ -274,7 +274,8 @@ __global__ void __launch_bounds__(GroupCfg<BITS>::THREADS, 1) k_group_scatter(Gr
         same[u] = same_digit<BITS>(d, in);
         if (in) first[u] = *word >> half & 0xffffu;
         __syncwarp();
-        if (in && (same[u] & ((1u << lane) - 1)) == 0) atomicAdd(const_cast<uint32_t*>(word), (uint32_t)__popc(same[u]) << half);
+        if (in && (same[u] & ((1u << lane) - 1)) == 0)
+          atomicAdd(const_cast<uint32_t*>(word), (uint32_t)__popc(same[u]) << half);
         __syncwarp();
       }
     }
@@ -912,7 +913,7 @@ int with_bits(int bits, F&& f) {
 struct GroupPlan {
   int bits, passes, share, nb;
   bool small;  // one CTA, one launch, no workspace
-  int64_t counts, pairs, bytes;  // bytes of the count tables, of the (key, row) pairs between two passes, and of the whole
+  int64_t counts, pairs, bytes;  // of the count tables, of the (key, row) pairs between two passes, of all
 };
 bool group_plan(int64_t n, int32_t G, GroupPlan* p) {
   if (n < 0 || n > INT32_MAX || G < 1 || G > MACE_SPECIES_MAX_INDEX) return false;
