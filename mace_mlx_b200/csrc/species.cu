@@ -1110,8 +1110,9 @@ extern "C" int mace_species_embed_grad(int32_t dtype, const void* grad, int64_t 
     return fail(MACE_ERR_BAD_ARG, "mace_species_embed_grad: an address is not a multiple of its values' size");
   int64_t need = 0;
   mace_species_embed_grad_workspace(n, G, C, &need);
-  if (need > 0 && (!ws || ws_bytes < need))
-    return fail(MACE_ERR_BAD_ARG, "mace_species_embed_grad: workspace too small");
+  // (the join reads partial rows four channels at a time)
+  if (need > 0 && (!ws || ws_bytes < need || !aligned16(ws)))
+    return fail(MACE_ERR_BAD_ARG, "mace_species_embed_grad: workspace too small or not 16-byte aligned");
   EmbedGrad p{grad, gs, order, offsets, n, G, C, eg_share(n), 0, scale, out, static_cast<float*>(ws)};
   p.shares = eg_shares(n, p.share);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -91,3 +91,20 @@ def test_c_entries_refuse_addresses_off_their_values():
                                             None), 1, 4, 5, 11, 12, 16)
     refused(lib.mace_rows_checkpoint, (0, one, 8, 8, 1, 1, 8, one, one, None), 1, 8)
     refused(lib.mace_rows_restore, (0, one, one, 1, 1, 8, one, None), 2, 6)
+
+
+def test_c_entries_refuse_workspaces_off_their_alignment():
+    """Every kernel that reads its workspace in 16-byte pieces (the weight gradient's is held to 32)."""
+    lib = nv.load_library()
+    one, size = C.c_void_p(32), 1 << 20  # never dereferenced
+    # a list of one row leaves one share with partial rows: the smallest call that has a workspace
+    grad = [0, one, 8, one, one, 1, 1, 8, 1.0, one, None, size, None]
+    group = [one, 100000, 2, one, one, None, size, None]
+    wgrad = [0, one, 8, 8, None, one, 8, 8, 1, 8, 8, one, one, 4, 1, 1.0, one, None, 1 << 30, None]
+    for f, args, at, offsets in ((lib.mace_species_embed_grad, grad, 10, (4, 8, 12)),
+                                 (lib.mace_species_group, group, 5, (4, 8, 12)),
+                                 (lib.mace_species_linear_wgrad, wgrad, 17, (4, 8, 16))):
+        for offset in offsets:
+            call = list(args)
+            call[at] = C.c_void_p(64 + offset)
+            assert f(*call) == nv.MACE_ERR_BAD_ARG and "aligned" in nv.last_error(lib), (f, offset)
