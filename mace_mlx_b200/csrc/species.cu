@@ -303,8 +303,8 @@ __global__ void __launch_bounds__(GroupCfg<BITS>::THREADS, 1) k_group_scatter(Gr
 }
 
 template <int BITS>
-__global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __restrict__ species, int n, int G,
-                                                            int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
+__global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* species, int n, int G, int32_t* order,
+                                                            int32_t* offsets) {
   pdl_wait();
   __shared__ int whist[32][1 << BITS];
   __shared__ int sums[32];
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __res
   const int i0 = warp * rounds * 32, i1 = min(n, i0 + rounds * 32);  // consecutive rows of one warp
   int key[MOST], rel[MOST];
 #pragma unroll
-  for (int j = 0; j < MOST; ++j) key[j] = i0 + j * 32 + lane < i1 ? row_key(species[i0 + j * 32 + lane], G) : 0;
+  for (int j = 0; j < MOST; ++j) key[j] = i0 + j * 32 + lane < i1 ? row_key(load_in(species + i0 + j * 32 + lane), G) : 0;
   for (int b = lane; b < (1 << BITS); b += 32) whist[warp][b] = 0;
   __syncwarp();
 #pragma unroll
@@ -349,16 +349,15 @@ __global__ void __launch_bounds__(GS_THREADS) k_group_small(const int32_t* __res
 // Two passes: offsets[v] = first position of the order whose key is >= v, a thread per offset (a pass over the keys
 // that writes an offset where the key changes leaves one thread all the writes of a long run of empty groups: 4M rows
 // that use 3 of 1M groups 3685 us, 115 so)
-__global__ void __launch_bounds__(256) k_group_offsets(const int32_t* __restrict__ species,
-                                                       const int32_t* __restrict__ order, int64_t n, int G,
-                                                       int32_t* __restrict__ offsets) {
+__global__ void __launch_bounds__(256) k_group_offsets(const int32_t* species, const int32_t* order, int64_t n, int G,
+                                                       int32_t* offsets) {
   pdl_wait();
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v > G) return;
   int64_t lo = 0, hi = n;
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
-    if (row_key(species[order[mid]], G) < v)
+    if (row_key(load_in(species + load_in(order + mid)), G) < v)
       lo = mid + 1;
     else
       hi = mid;
@@ -367,52 +366,69 @@ __global__ void __launch_bounds__(256) k_group_offsets(const int32_t* __restrict
 }
 
 // out[i] = scale table[species[i]].  The table stays in L2 and the result's stores are the bound: 1M rows of 128 fp32
-// channels 79 us, 6.5 TB/s.
+// channels 77 us, 6.7 TB/s (90 with 5 or 6 CTAs of 256 threads on an SM instead of 7); of 128 bf16 channels 45.
 // Consecutive vectors of V elements of the (n, C) result, CTA by CTA.
 // FLAT = 0: C is a multiple of V and every row is vector-aligned, so a vector
 // lies in one row; FLAT = 1: the result is contiguous and a vector may pass a
 // row's end (any C); V = 1 serves everything else.
 template <typename T, int V, bool FLAT>
-__global__ void __launch_bounds__(RW_THREADS) k_embed(const T* __restrict__ table, int64_t ts, int G, int C,
-                                                      const int32_t* __restrict__ species, int64_t n, float scale,
-                                                      T* __restrict__ out, int64_t os, RowDiv div) {
+__global__ void __launch_bounds__(RW_THREADS, V == 8 && FLAT ? 5 : 7)
+    k_embed(const T* table, int64_t ts, int G, int C, const int32_t* species, int64_t n, float scale, T* out, int64_t os,
+            RowDiv div) {
   pdl_wait();
   const int64_t v0 = blockIdx.x * (int64_t)(RW_THREADS * RW_UNROLL);  // first vector of this CTA
   const int64_t total = n * C;
   const int64_t row0 = (v0 * V) / C;
   const uint32_t first = (uint32_t)(v0 * V - row0 * C);
+  uint32_t row[RW_UNROLL], col[RW_UNROLL];
+  int z[RW_UNROLL];
+  Raw<T, V> x[RW_UNROLL];  // !FLAT: as loaded
+  float v[FLAT ? RW_UNROLL : 1][FLAT ? V : 1];
 #pragma unroll
   for (int j = 0; j < RW_UNROLL; ++j) {
     const uint32_t local = first + (threadIdx.x + j * RW_THREADS) * V;
-    uint32_t r = div.quotient(local), c = local - r * C;
-    const int64_t at = v0 * V + (threadIdx.x + j * RW_THREADS) * V;
-    if (at >= total) continue;
-    float v[V];
-    int z = species[row0 + r];
-    if constexpr (!FLAT) {
-      if (z >= 0 && z < G)
-        load_channels<T, V>(table + z * ts + c, v);
-      else
-        for (int k = 0; k < V; ++k) v[k] = 0.f;
+    row[j] = div.quotient(local), col[j] = local - row[j] * C;
+    z[j] = v0 * V + (threadIdx.x + j * RW_THREADS) * V < total ? load_in(species + row0 + row[j]) : -1;
+  }
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] *= scale;
-      store_channels<T, V>(out + (row0 + r) * os + c, v);
-    } else {
+  for (int j = 0; j < RW_UNROLL; ++j) {
+    const int64_t at = v0 * V + (threadIdx.x + j * RW_THREADS) * V;
+    if constexpr (!FLAT) {
+      if (z[j] >= 0 && z[j] < G)
+        x[j].load(table + z[j] * ts + col[j]);
+      else
+        x[j].zero();
+    } else if (at < total) {
+      uint32_t r = row[j], c = col[j];
+      int t = z[j];
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        v[k] = z >= 0 && z < G ? scale * to_f32(table[z * ts + c]) : 0.f;
+        v[j][k] = t >= 0 && t < G ? scale * to_f32(load_in(table + t * ts + c)) : 0.f;
         if (++c == (uint32_t)C) {
           c = 0;
           ++r;
-          z = row0 + r < n ? species[row0 + r] : -1;
+          t = row0 + r < n ? load_in(species + row0 + r) : -1;
         }
       }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < RW_UNROLL; ++j) {
+    const int64_t at = v0 * V + (threadIdx.x + j * RW_THREADS) * V;
+    if (at >= total) continue;
+    if constexpr (!FLAT) {
+      float u[V];
+      x[j].values(u);
+#pragma unroll
+      for (int k = 0; k < V; ++k) u[k] *= scale;
+      store_channels<T, V>(out + (row0 + row[j]) * os + col[j], u);
+    } else {
       if (at + V <= total)
-        store_channels<T, V>(out + at, v);
+        store_channels<T, V>(out + at, v[j]);
       else
 #pragma unroll
         for (int k = 0; k < V; ++k)
-          if (at + k < total) out[at + k] = from_f32<T>(v[k]);
+          if (at + k < total) out[at + k] = from_f32<T>(v[j][k]);
     }
   }
 }
@@ -439,7 +455,7 @@ struct EmbedGrad {
 
 // group of grouped position i: the largest g with offsets[g] <= i (G: past the last group); by a whole warp, 32 places
 // at a time
-__device__ __forceinline__ int group_at(const int32_t* __restrict__ offsets, int G, int64_t i) {
+__device__ __forceinline__ int group_at(const int32_t* offsets, int G, int64_t i) {
   const int lane = threadIdx.x & 31;
   int lo = 0, count = G + 1;  // the group is one of lo .. lo + count - 1
   while (count > 1) {
@@ -750,9 +766,8 @@ __global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p, int per_c
 constexpr int CK_ROWS = 4;
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* __restrict__ x, int64_t xn, int64_t xm, int64_t rows,
-                                                           int d, int C, int nb, int8_t* __restrict__ q,
-                                                           float* __restrict__ scale) {
+__global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* x, int64_t xn, int64_t xm, int64_t rows, int d,
+                                                           int C, int nb, int8_t* q, float* scale) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t items = rows * nb;
@@ -778,7 +793,7 @@ __global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* __restrict__
         if (u < here && c + mine_c < C) load4(src + c, v[u]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[u][j] = u < here && c + mine_c + 32 * j < C ? to_f32(src[c + 32 * j]) : 0.f;
+        for (int j = 0; j < 4; ++j) v[u][j] = u < here && c + mine_c + 32 * j < C ? to_f32(load_in(src + c + 32 * j)) : 0.f;
       }
       if (++b == nb) {
         b = 0;
@@ -823,9 +838,8 @@ __global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* __restrict__
 // x = q scale, bound by HBM (1.6M rows of 128 fp32 channels 163 us, 6.3 TB/s).
 // Four consecutive elements of the contiguous (rows, C) result per thread and step; a vector may pass a row's end.
 template <typename T>
-__global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* __restrict__ q, const float* __restrict__ scale,
-                                                        int64_t total, int C, int nb, T* __restrict__ x, RowDiv div,
-                                                        int vec) {
+__global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* q, const float* scale, int64_t total, int C, int nb,
+                                                        T* x, RowDiv div, int vec) {
   pdl_wait();
   const int64_t e0 = blockIdx.x * (int64_t)(RW_THREADS * RS_UNROLL * 4);
   const int64_t row0 = e0 / C;
@@ -839,42 +853,46 @@ __global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* __restrict
     const uint32_t r = div.quotient(local), c = local - r * C;
     w[j] = 0;
     sc[j] = 0.f;
-    if (at < total) sc[j] = scale[(row0 + r) * nb + c / MACE_CHECKPOINT_BLOCK];
+    if (at < total) sc[j] = load_in(scale + (row0 + r) * nb + c / MACE_CHECKPOINT_BLOCK);
     if (vec && at + 4 <= total) {
-      w[j] = *reinterpret_cast<const uint32_t*>(q + at);
+      w[j] = load_in(reinterpret_cast<const uint32_t*>(q + at));
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (at + k < total) w[j] |= (uint32_t)(uint8_t)q[at + k] << (8 * k);
+        if (at + k < total) w[j] |= (uint32_t)(uint8_t)load_in(q + at + k) << (8 * k);
     }
   }
+  float v[RS_UNROLL][4];
 #pragma unroll
   for (int j = 0; j < RS_UNROLL; ++j) {
     const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
-    float v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = (float)(int8_t)(w[j] >> (8 * k));
+    for (int k = 0; k < 4; ++k) v[j][k] = (float)(int8_t)(w[j] >> (8 * k));
     const uint32_t local = first + (threadIdx.x + j * RW_THREADS) * 4;
     uint32_t r = div.quotient(local), c = local - r * C;
     if (c + 4 <= (uint32_t)C && (C & 3) == 0) {  // (a block boundary is a multiple of 4)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] *= sc[j];
+      for (int k = 0; k < 4; ++k) v[j][k] *= sc[j];
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (at + k < total) v[k] *= scale[(row0 + r) * nb + c / MACE_CHECKPOINT_BLOCK];
+        if (at + k < total) v[j][k] *= load_in(scale + (row0 + r) * nb + c / MACE_CHECKPOINT_BLOCK);
         if (++c == (uint32_t)C) {
           c = 0;
           ++r;
         }
       }
     }
+  }
+#pragma unroll
+  for (int j = 0; j < RS_UNROLL; ++j) {
+    const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
     if (vec && at + 4 <= total) {
-      store4(x + at, v);
+      store4(x + at, v[j]);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (at + k < total) x[at + k] = from_f32<T>(v[k]);
+        if (at + k < total) x[at + k] = from_f32<T>(v[j][k]);
     }
   }
 }
@@ -1024,7 +1042,7 @@ int embed(const void* table, int64_t ts, int G, int C, const int32_t* species, i
   auto go = [&](auto kernel, int v) {
     return launch("species_embed", kernel, grid(v), RW_THREADS, 0, s, t, ts, G, C, species, n, scale, o, os, row_div(C));
   };
-  // 1M rows of 128 fp32 channels 79 us (114 as a FLAT result, 215 one by one); of 97 channels 94 FLAT, 164 one by one
+  // 1M rows of 128 fp32 channels 77 us (114 as a FLAT result, 215 one by one); of 97 channels 95 FLAT, 164 one by one
   if (C % V == 0 && ts % V == 0 && os % V == 0 && aligned16(table) && aligned16(out)) return go(k_embed<T, V, false>, V);
   if (os == C && aligned16(out)) return go(k_embed<T, V, true>, V);
   return go(k_embed<T, 1, false>, 1);

@@ -50,22 +50,45 @@ __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ bf16 from_f32<bf16>(float x) { return __float2bfloat16_rn(x); }
 
-// V consecutive channels as fp32: one 16-byte load where V channels fill it, else one by one
-template <typename T, int V>
-__device__ __forceinline__ void load_channels(const T* __restrict__ src, float* v) {
-  if constexpr (V * sizeof(T) == 16) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
-    const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = to_f32(t[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = to_f32(src[k]);
-  }
+// Loads of what a kernel gets.  The kernel before it may have written it, and with a dependent launch that one still
+// runs when this one starts: so these are plain loads (the read-only path is for data that nothing writes while the
+// kernel lives), and volatile, which keeps them behind pdl_wait().  They depend on no store in the compiler's eyes, but
+// the assembler keeps them behind the stores that come before them: load first, store afterwards.
+__device__ __forceinline__ uint4 load_in(const uint4* a) {
+  uint4 v;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 load_in(const uint2* a) {
+  uint2 v;
+  asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t load_in(const uint32_t* a) {
+  uint32_t v;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(a));
+  return v;
+}
+__device__ __forceinline__ int32_t load_in(const int32_t* a) {
+  return (int32_t)load_in(reinterpret_cast<const uint32_t*>(a));
+}
+__device__ __forceinline__ float load_in(const float* a) {
+  return __uint_as_float(load_in(reinterpret_cast<const uint32_t*>(a)));
+}
+__device__ __forceinline__ bf16 load_in(const bf16* a) {
+  uint16_t v;
+  asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(a));
+  return __ushort_as_bfloat16(v);
+}
+__device__ __forceinline__ int8_t load_in(const int8_t* a) {
+  int32_t v;
+  asm volatile("ld.global.s8 %0, [%1];" : "=r"(v) : "l"(a));
+  return (int8_t)v;
 }
 
+// V consecutive channels: one 16-byte store where they fill it, else one by one
 template <typename T, int V>
-__device__ __forceinline__ void store_channels(T* __restrict__ dst, const float* v) {
+__device__ __forceinline__ void store_channels(T* dst, const float* v) {
   if constexpr (V * sizeof(T) == 16) {
     uint4 u;
     T* t = reinterpret_cast<T*>(&u);
@@ -80,11 +103,11 @@ __device__ __forceinline__ void store_channels(T* __restrict__ dst, const float*
 
 // four consecutive values, aligned to four
 __device__ __forceinline__ void load4(const float* src, float* v) {
-  const float4 u = __ldg(reinterpret_cast<const float4*>(src));
-  v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+  const uint4 u = load_in(reinterpret_cast<const uint4*>(src));
+  v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
 }
 __device__ __forceinline__ void load4(const bf16* src, float* v) {
-  const uint2 u = __ldg(reinterpret_cast<const uint2*>(src));
+  const uint2 u = load_in(reinterpret_cast<const uint2*>(src));
   v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
   v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
 }
@@ -110,33 +133,39 @@ struct Raw {
     else
       for (int k = 0; k < V; ++k) one[k] = from_f32<T>(0.f);
   }
-  __device__ __forceinline__ void load(const T* __restrict__ src) {
+  __device__ __forceinline__ void load(const T* src) {
     if constexpr (PIECE)
-      piece = __ldg(reinterpret_cast<const uint4*>(src));
+      piece = load_in(reinterpret_cast<const uint4*>(src));
     else
-      for (int k = 0; k < V; ++k) one[k] = src[k];
+      for (int k = 0; k < V; ++k) one[k] = load_in(src + k);
   }
   // channels `hop` apart, those below `left`
-  __device__ __forceinline__ void load(const T* __restrict__ src, int hop, int left) {
+  __device__ __forceinline__ void load(const T* src, int hop, int left) {
 #pragma unroll
     for (int k = 0; k < V; ++k)
-      if (k * hop < left) one[k] = src[k * hop];
+      if (k * hop < left) one[k] = load_in(src + k * hop);
   }
-  __device__ __forceinline__ void add_to(float* acc) const {
+  __device__ __forceinline__ void values(float* v) const {
     if constexpr (!PIECE) {
-      for (int k = 0; k < V; ++k) acc[k] += to_f32(one[k]);
+      for (int k = 0; k < V; ++k) v[k] = to_f32(one[k]);
     } else {
       const uint32_t w[4] = {piece.x, piece.y, piece.z, piece.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if constexpr (sizeof(T) == 4) {
-          acc[k] += __uint_as_float(w[k]);
+          v[k] = __uint_as_float(w[k]);
         } else {
-          acc[2 * k] += __uint_as_float(w[k] << 16);
-          acc[2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+          v[2 * k] = __uint_as_float(w[k] << 16);
+          v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
         }
       }
     }
+  }
+  __device__ __forceinline__ void add_to(float* acc) const {
+    float v[V];
+    values(v);
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] += v[k];
   }
 };
 
@@ -171,7 +200,7 @@ __device__ __forceinline__ uint32_t quantise8x4(const float* x, float s) {
 struct Range {
   int64_t lo, hi;
 };
-__device__ __forceinline__ Range group_range(const int32_t* __restrict__ offsets, int g, int64_t n) {
+__device__ __forceinline__ Range group_range(const int32_t* offsets, int g, int64_t n) {
   Range r;
   r.lo = min(max((int64_t)offsets[g], (int64_t)0), n);
   r.hi = min(max((int64_t)offsets[g + 1], r.lo), n);

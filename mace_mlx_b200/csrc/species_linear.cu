@@ -489,7 +489,7 @@ struct RowRef {
       m = at - i * p.d;
     }
     if (!in) m = -1;
-    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(node) : "l"(p.order + i));
+    node = load_in(p.order + i);
   }
   __device__ __forceinline__ bool valid(const SlParams& p) const { return m >= 0 && node >= 0 && node < p.n; }
   __device__ __forceinline__ int64_t offset(const RowView& v) const { return node * v.sn + m * v.sm; }

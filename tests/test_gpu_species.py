@@ -564,6 +564,33 @@ def test_groupings_that_are_not_permutations_stay_in_bounds(sp):
     assert sp.error_flag() == 0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_calls_in_a_row_on_buffers_used_again(sp, dtype):
+    """Each call reads what the call before it has just written to memory that earlier calls had read."""
+    n, g, c = 700, 5, 64
+    tables, w = randn(6, g, c, seed=140, dtype=dtype), randn(g, c, c, seed=141, dtype=dtype)
+    lists = [draw_species(n, g, 142 + k, pad=0.1) for k in range(6)]
+
+    def chain(k, rows, y):
+        groups = sp.group_species(lists[k], g)
+        sp.species_embedding(tables[k], lists[k], out=rows)
+        sp.species_linear(rows, w, groups, out=y)
+        ck = sp.checkpoint_rows(y)
+        return [*groups, y.clone(), sp.restore_rows(ck), sp.species_embedding_grad(y, groups),
+                sp.species_linear_grad_weight(ck, y, groups)]
+
+    want = []
+    for k in range(6):
+        rows, y = torch.empty(n, c, dtype=dtype, device="cuda"), torch.empty(n, c, dtype=dtype, device="cuda")
+        want.append(chain(k, rows, y))
+        torch.cuda.synchronize()
+    rows, y = torch.empty(n, c, dtype=dtype, device="cuda"), torch.empty(n, c, dtype=dtype, device="cuda")
+    for _ in range(10):
+        got = [chain(k, rows, y) for k in range(6)]
+        for a, b in zip(sum(got, []), sum(want, []), strict=True):
+            assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------- ends and repeats
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("c", [1, 8, 33, 61, 64, 128, 129, 250])

@@ -108,3 +108,16 @@ def test_c_entries_refuse_workspaces_off_their_alignment():
             call = list(args)
             call[at] = C.c_void_p(64 + offset)
             assert f(*call) == nv.MACE_ERR_BAD_ARG and "aligned" in nv.last_error(lib), (f, offset)
+
+
+def test_kernels_read_their_inputs_by_plain_loads():
+    """A kernel of these operators may start while the one before it still writes its inputs, so none goes through the
+    read-only path, which is for data that nothing writes while a kernel lives."""
+    from pathlib import Path
+
+    sources = sorted((Path(mace_mlx_b200.__file__).parent / "csrc").glob("species*.cu*"))
+    assert len(sources) == 5
+    for path in sources:
+        text = path.read_text()
+        for form in ("__ldg(", "global.nc", "__restrict__"):
+            assert form not in text, (path.name, form)
