@@ -727,10 +727,6 @@ __device__ __forceinline__ void fill_weights(const SlParams& p, uint8_t* img0, i
       for (int u = 0; u < 4; ++u) {
         const int j = h * 16 + u * 4 + w4;
         const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane;
-        if constexpr (PB == 3) {  // alpha rides on the split weights
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[u][e] *= p.alpha;
-        }
         if (n < NT) put_eight<PB>(img, p.img, n, p.transposed ? lane & 7 : j & 7, v[u]);
       }
     }
@@ -1045,10 +1041,9 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
       // touch 32 rows per instruction (600 000 rows 128 -> 128 fp32: 149 us with them, 130 staged).
       constexpr int CB = 128 / sizeof(T);  // columns of a 128-byte row segment
       const bool mine = ref.valid(p);
-      if constexpr (P == 1) {
+      // (alpha times the weights instead, before they are split, left the range of fp32 where the result does not)
 #pragma unroll
-        for (int k = 0; k < 64; ++k) acc[k] *= p.alpha;
-      }
+      for (int k = 0; k < 64; ++k) acc[k] *= p.alpha;
 #pragma unroll
       for (int b = 0; b < 64; b += CB) {
         const int left = min(p.N - c0 - b, CW - b);  // columns of this segment

@@ -349,6 +349,21 @@ def test_large_and_small_magnitudes(sp):
         assert_sum(sp.species_linear(x, w, groups), y, mass, k, f"{sx} {sw}")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sx,sw,alpha", [(1e30, 1e-12, 1e-30), (1e-25, 1e25, 1e20), (1e-12, 1e20, 1e27), (1e4, 1e-30, 1e-9)])
+def test_alpha_meets_the_sum(sp, dtype, sx, sw, alpha):
+    """alpha x W is in range where alpha W (or alpha x) is not."""
+    n, k, m, g = 130, 64, 32, 2
+    z = draw_species(n, g, 65)
+    groups = sp.group_species(z, g)
+    x, dy = (randn(n, 1, k, seed=66) * sx).to(dtype), (randn(n, 1, m, seed=67) * sx).to(dtype)
+    w = (randn(g, k, m, seed=68) * sw).to(dtype)
+    y, mass = linear64(x, w, z, alpha)
+    assert_sum(sp.species_linear(x, w, groups, alpha=alpha), y, mass, k, "forward")
+    dx, mass = linear64(dy, w.transpose(1, 2), z, alpha)
+    assert_sum(sp.species_linear(dy, w, groups, alpha=alpha, transpose=True), dx, mass, m, "input gradient")
+
+
 def test_linear_past_32_bit_offsets(sp):
     """Rows whose element offsets pass 2^31."""
     n, k, m, g = 1000, 64, 32, 2
