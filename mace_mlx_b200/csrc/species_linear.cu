@@ -1112,61 +1112,65 @@ namespace {
 // (gradients of 40 000 rows 128 x 128 in 4 groups: 19.1 us, 32.6 with one set per block; 300 000 rows in 89: no
 // difference).
 template <typename T>
-__global__ void __launch_bounds__(256) k_species_wgrad_join(const __grid_constant__ SlParams p) {
+__global__ void __launch_bounds__(256, 6) k_species_wgrad_join(const __grid_constant__ SlParams p) {
   pdl_wait();
   __shared__ float4 part[4][64];
   const int g = blockIdx.x, tid = threadIdx.x;
   const int span = p.spans[g];
   const int s0 = span & 0xffff, s1 = span >> 16;  // shares of the group; none: s1 = -1
   if (s0 == s1) return;                           // written by its only share
-  const int tile = blockIdx.z;
-  const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
   const int lane = tid & 63, sl = tid >> 6;
   const int kl = (blockIdx.y & 15) * 8 + (lane & 7), block = blockIdx.y >> 4;
-  const float4* const first = reinterpret_cast<const float4*>(p.part) +
-                              ((int64_t)tile * (p.shares + p.G) + g) * 32 * p.NT + kl;
-  T* const row = static_cast<T*>(p.out) + ((int64_t)g * p.K + k0 + kl) * p.N + n0;
-  auto sum = [&](int cq, int from, int step) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int tiles = p.n_ct * p.n_kt;
+  for (int tile = blockIdx.z; tile < tiles; tile += gridDim.z) {
+    const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
+    const float4* const first = reinterpret_cast<const float4*>(p.part) +
+                                ((int64_t)tile * (p.shares + p.G) + g) * 32 * p.NT + kl;
+    T* const row = static_cast<T*>(p.out) + ((int64_t)g * p.K + k0 + kl) * p.N + n0;
+    auto sum = [&](int cq, int from, int step) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-    for (int s = from; s <= s1; s += step) {
-      const float4 v = first[(int64_t)s * 32 * p.NT + cq * 128];
-      acc.x += v.x;
-      acc.y += v.y;
-      acc.z += v.z;
-      acc.w += v.w;
-    }
-    return acc;
-  };
-  auto write = [&](int cq, float4 a) {
-    if (k0 + kl >= p.K) return;
-    const float v[4] = {p.alpha * a.x, p.alpha * a.y, p.alpha * a.z, p.alpha * a.w};
-    if (p.vst && n0 + cq * 4 + 4 <= p.N) {
-      store4(row + cq * 4, v);
-    } else {
+      for (int s = from; s <= s1; s += step) {
+        const float4 v = first[(int64_t)s * 32 * p.NT + cq * 128];
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
+      }
+      return acc;
+    };
+    auto write = [&](int cq, float4 a) {
+      if (k0 + kl >= p.K) return;
+      const float v[4] = {p.alpha * a.x, p.alpha * a.y, p.alpha * a.z, p.alpha * a.w};
+      if (p.vst && n0 + cq * 4 + 4 <= p.N) {
+        store4(row + cq * 4, v);
+      } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n0 + cq * 4 + k < p.N) row[cq * 4 + k] = from_f32<T>(v[k]);
+        for (int k = 0; k < 4; ++k)
+          if (n0 + cq * 4 + k < p.N) row[cq * 4 + k] = from_f32<T>(v[k]);
+      }
+    };
+    if (s1 - s0 < 8) {
+      const int cq = sl * 8 + (lane >> 3);
+      if (block == 0 && cq * 4 < p.NT) write(cq, sum(cq, s0, 1));
+      continue;
     }
-  };
-  if (s1 - s0 < 8) {
-    const int cq = sl * 8 + (lane >> 3);
-    if (block == 0 && cq * 4 < p.NT) write(cq, sum(cq, s0, 1));
-    return;
-  }
-  const int cq = block * 8 + (lane >> 3);
-  part[sl][lane] = sum(cq, s0 + sl, 4);
-  __syncthreads();
-  if (sl != 0) return;
-  float4 a = part[0][lane];
+    const int cq = block * 8 + (lane >> 3);
+    part[sl][lane] = sum(cq, s0 + sl, 4);
+    __syncthreads();
+    if (sl == 0) {
+      float4 a = part[0][lane];
 #pragma unroll
-  for (int q = 1; q < 4; ++q) {
-    a.x += part[q][lane].x;
-    a.y += part[q][lane].y;
-    a.z += part[q][lane].z;
-    a.w += part[q][lane].w;
+      for (int q = 1; q < 4; ++q) {
+        a.x += part[q][lane].x;
+        a.y += part[q][lane].y;
+        a.z += part[q][lane].z;
+        a.w += part[q][lane].w;
+      }
+      write(cq, a);
+    }
+    __syncthreads();  // (the next tile's)
   }
-  write(cq, a);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1395,7 +1399,7 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   else  // bf16 in whole pieces: nothing to convert
     rc = vec ? launch_direct<true>(p, grid, s) : launch_wgrad<bf16, bf16, false>(p, grid, s);
   if (rc) return rc;
-  const dim3 jg(G, 16 * (p.NT / 32), p.n_ct * p.n_kt);
+  const dim3 jg(G, 16 * (p.NT / 32), std::min(p.n_ct * p.n_kt, 65535));  // (a grid's z; there may be one tile more)
   return launch("species_wgrad_join", dtype == MACE_F32 ? k_species_wgrad_join<float> : k_species_wgrad_join<bf16>, jg, 256,
                 0, s, p);
 }

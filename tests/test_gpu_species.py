@@ -272,6 +272,20 @@ def test_linear_over_many_tiles(sp, dtype, mix):
     assert torch.equal(got, sp.species_linear_grad_weight(x, dy, groups, alpha=0.5))
 
 
+def test_weight_gradient_of_the_widest_matrices(sp):
+    """65 536 tiles of a matrix, and a group without rows."""
+    n, k, g = 3, 32768, 2
+    z = torch.zeros(n, dtype=torch.int32, device="cuda")
+    x, dy = randn(n, k, seed=25, dtype=torch.bfloat16), randn(n, k, seed=26, dtype=torch.bfloat16)
+    junk = torch.full((g, k, k), 7.0, dtype=torch.bfloat16, device="cuda")
+    del junk  # (what the result is likely to be made in)
+    dw = sp.species_linear_grad_weight(x, dy, sp.group_species(z, g))
+    assert not dw[1].any()
+    for c in range(0, k, 4096):
+        part = x[:, c:c + 4096].double()
+        assert_sum(dw[0, c:c + 4096], part.T @ dy.double(), part.abs().T @ dy.double().abs(), n)
+
+
 def _views(x):
     """x (n, d, k) in other layouts of the same values."""
     n, d, k = x.shape
