@@ -436,8 +436,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_direct(const __grid_c
         const int len = segment(w);
         const bool group_ends = w.t + len == pre[w.g + 1];
         if (group_ends || w.t + len == t1) {
-          finish_wgrad<bf16>(p, acc, w.g, group_ends && pre[w.g] >= t0, tile, share, wg_k0, wg_n0, quad * 32 + lane,
-                             half * CW, CW);
+          finish_wgrad<bf16>(p, acc, w.g, group_ends && pre[w.g] >= t0, pre[w.g] > t0, tile, share, wg_k0, wg_n0,
+                             quad * 32 + lane, half * CW, CW);
           fresh = true;
         }
         advance(w, len);

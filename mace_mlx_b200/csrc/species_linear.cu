@@ -78,8 +78,8 @@ struct SlParams {
   int out32;
   int vst;              // map: rows of `out` are whole 16-byte pieces; weight gradient: bytes of a vector store (32, 16, 0)
   float* part;          // weight gradient: partial tiles
-  int* spans;           // weight gradient: a group's first share, and its last in the upper 16 bits (-1: no rows),
-                        // written by CTA 0 for the join
+  int* spans;           // weight gradient: a group's first share, bit 15 if it begins inside it, and its last in the
+                        // upper 16 bits (-1: no rows), written by CTA 0 for the join
   const int32_t* order;
   const int32_t* offsets;
   int64_t n;
@@ -429,7 +429,12 @@ __device__ __forceinline__ void write_spans(const SlParams& p, const Groups& q) 
   };
   for (int g = threadIdx.x; g < p.G; g += THREADS) {
     const int64_t u0 = q.pre[g], u1 = q.pre[g + 1];
-    p.spans[g] = u0 < u1 ? share_of(u0) | share_of(u1 - 1) << 16 : -1;
+    int span = -1;
+    if (u0 < u1) {
+      const int s0 = share_of(u0);
+      span = s0 | (u0 > s0 * all / shares) << 15 | share_of(u1 - 1) << 16;
+    }
+    p.spans[g] = span;
   }
 }
 
@@ -616,14 +621,14 @@ __device__ __forceinline__ void copy_out(const SlParams& p, const uint8_t* stage
 }
 
 // Weight gradient: a lane's NT / 2 sums of row kl of a 128 x NT tile (columns c0 ..), done with group g: dW itself
-// where this share held the whole group, else a partial tile.  (share, group) pairs of one tile are a staircase:
-// share + g numbers them; a partial tile is stored as [column quad][row], so that a warp's 32 rows are one line per
-// instruction.
+// where this share held the whole group, else a partial tile: a share has two for each tile of the matrix, one for a
+// group that begins with it or before it, one for a group that begins inside it (`inside`) and goes on.  A partial tile
+// is stored as [column quad][row], so that a warp's 32 rows are one line per instruction.
 template <typename T>
-__device__ __forceinline__ void finish_wgrad(const SlParams& p, float* acc, int g, bool whole, int tile, int share, int k0,
-                                             int n0, int kl, int c0, int CW) {
+__device__ __forceinline__ void finish_wgrad(const SlParams& p, float* acc, int g, bool whole, bool inside, int tile,
+                                             int share, int k0, int n0, int kl, int c0, int CW) {
   if (!whole) {
-    float4* dst = reinterpret_cast<float4*>(p.part) + ((int64_t)tile * (p.shares + p.G) + share + g) * 32 * p.NT +
+    float4* dst = reinterpret_cast<float4*>(p.part) + (((int64_t)tile * p.shares + share) * 2 + inside) * 32 * p.NT +
                   c0 / 4 * 128 + kl;
 #pragma unroll
     for (int b = 0; b < 16; ++b)
@@ -1117,21 +1122,23 @@ __global__ void __launch_bounds__(256, 6) k_species_wgrad_join(const __grid_cons
   __shared__ float4 part[4][64];
   const int g = blockIdx.x, tid = threadIdx.x;
   const int span = p.spans[g];
-  const int s0 = span & 0xffff, s1 = span >> 16;  // shares of the group; none: s1 = -1
+  const int s0 = span & 0x7fff, s1 = span >> 16;  // shares of the group; none: s1 = -1
   if (s0 == s1) return;                           // written by its only share
   const int lane = tid & 63, sl = tid >> 6;
   const int kl = (blockIdx.y & 15) * 8 + (lane & 7), block = blockIdx.y >> 4;
   const int tiles = p.n_ct * p.n_kt;
   for (int tile = blockIdx.z; tile < tiles; tile += gridDim.z) {
     const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
-    const float4* const first = reinterpret_cast<const float4*>(p.part) +
-                                ((int64_t)tile * (p.shares + p.G) + g) * 32 * p.NT + kl;
+    const float4* const first = reinterpret_cast<const float4*>(p.part) + (int64_t)tile * p.shares * 64 * p.NT + kl;
+    const int inside = span & 0x8000 ? 32 * p.NT : 0;  // where its partial tile of share s0 is the second
     T* const row = static_cast<T*>(p.out) + ((int64_t)g * p.K + k0 + kl) * p.N + n0;
     auto sum = [&](int cq, int from, int step) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4* at = first + (int64_t)from * 64 * p.NT + cq * 128;
+      int skip = from == s0 ? inside : 0;
 #pragma unroll 8
-      for (int s = from; s <= s1; s += step) {
-        const float4 v = first[(int64_t)s * 32 * p.NT + cq * 128];
+      for (int s = from; s <= s1; s += step, at += step * 64 * p.NT, skip = 0) {
+        const float4 v = at[skip];
         acc.x += v.x;
         acc.y += v.y;
         acc.z += v.z;
@@ -1250,8 +1257,9 @@ int launch_wgrad(const SlParams& p, int grid, cudaStream_t s) {
   return launch_big("species_wgrad", k_species_wgrad<TA, T, VEC>, attr_set, grid, WG_THREADS, Wg<TA, T, VEC>::BYTES, s, p);
 }
 
-int64_t partial_bytes(const SlParams& p, int G) {
-  return (int64_t)p.n_ct * p.n_kt * (p.shares + G) * 128 * p.NT * 4;
+// (one share has every group whole)
+int64_t partial_bytes(const SlParams& p) {
+  return p.shares > 1 ? (int64_t)p.n_ct * p.n_kt * p.shares * 2 * 128 * p.NT * 4 : 0;
 }
 
 // shares (CTAs along the rows) and tiles of a weight gradient
@@ -1342,7 +1350,7 @@ extern "C" int mace_species_linear_wgrad_workspace(int64_t n, int32_t d, int32_t
     return fail(MACE_ERR_BAD_ARG, "mace_species_linear_wgrad_workspace: bad arguments");
   SlParams p{};
   wgrad_split(n, d, G, K, M, &p);
-  *bytes = partial_bytes(p, G) + (int64_t)G * 4;
+  *bytes = partial_bytes(p) + (int64_t)G * 4;
   return MACE_OK;
 }
 
@@ -1383,7 +1391,7 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
     MACE_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)G * K * M * es, s));
     return MACE_OK;
   }
-  p.spans = reinterpret_cast<int*>(static_cast<char*>(ws) + partial_bytes(p, G));
+  p.spans = reinterpret_cast<int*>(static_cast<char*>(ws) + partial_bytes(p));
   const int grid = p.shares * p.n_ct * p.n_kt;
   const bool vec = aligned_rows(p.a, n, d, xe) && aligned_rows(p.b, n, d, es);
   auto go = [&](auto ta, auto t) {

@@ -477,9 +477,9 @@ __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_co
         const int len = sum_steps(w);
         const bool group_ends = w.t + len == pre[w.g + 1];
         if (group_ends || w.t + len == t1) {
-          const bool whole = group_ends && pre[w.g] >= t0;
-          finish_wgrad<T>(p, acc, w.g, whole, tile, share, k0, n0, quad * 32 + lane, 0, min(NT, 64));
-          if (NT > 64) finish_wgrad<T>(p, acc + 64, w.g, whole, tile, share, k0, n0, quad * 32 + lane, 64, NT - 64);
+          const bool whole = group_ends && pre[w.g] >= t0, inside = pre[w.g] > t0;
+          finish_wgrad<T>(p, acc, w.g, whole, inside, tile, share, k0, n0, quad * 32 + lane, 0, min(NT, 64));
+          if (NT > 64) finish_wgrad<T>(p, acc + 64, w.g, whole, inside, tile, share, k0, n0, quad * 32 + lane, 64, NT - 64);
           fresh = true;
         }
         advance(w, len);

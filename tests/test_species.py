@@ -121,3 +121,20 @@ def test_kernels_read_their_inputs_by_plain_loads():
         text = path.read_text()
         for form in ("__ldg(", "global.nc", "__restrict__"):
             assert form not in text, (path.name, form)
+
+
+def test_weight_gradient_workspace_follows_its_shares():
+    """Two partial tiles a share and none for one share, however many groups there are."""
+    lib, need = nv.load_library(), C.c_int64()
+
+    def bytes_of(n, d, g, k, m):
+        assert lib.mace_species_linear_wgrad_workspace(n, d, g, k, m, C.byref(need)) == nv.MACE_OK
+        return need.value
+
+    for g, k, m in ((89, 4096, 4096), (512, 2048, 2048), (1, 32768, 32768)):  # a tile to every SM: one share
+        assert bytes_of(10_000, 3, g, k, m) <= 4 * g
+    tile = 4 * 128 * 128
+    for n, g, k, m in ((1_000_000, 512, 512, 512), (1000, 4, 128, 128), (100, 300, 128, 128), (5, 512, 300, 257)):
+        tiles = -(-k // 128) * -(-m // 128)
+        units = n // 64 + 1 + min(g, n)
+        assert bytes_of(n, 1, g, k, m) <= 4 * g + tiles * 2 * min(units, -(-148 // tiles)) * tile
