@@ -51,6 +51,7 @@ constexpr int SL_THREADS = 16 * 32;
 constexpr int SL_KC = 64;              // K of one accumulation step
 constexpr int SL_IMG = 128 * 128;      // bytes of one piece of a B image of up to 128 rows of 64 bf16
 constexpr int SL_LONG = 8;             // weight gradient of bf16: steps accumulated in TMEM
+constexpr int SL_STEPS = 2048;         // weight gradient: steps that a share may add into one fp32 sum
 constexpr int SL_D = 0;                // TMEM columns: two accumulators of 128
 constexpr int SL_A = 256;              // then two A stages
 constexpr uint32_t SL_TMEM = 512;
@@ -1270,6 +1271,9 @@ void wgrad_split(int64_t n, int32_t d, int32_t G, int32_t K, int32_t M, SlParams
   const int64_t units = (n * d + SL_KC - 1) / SL_KC + std::min<int64_t>(G, n);
   const int tiles = p->n_ct * p->n_kt;
   p->shares = (int)std::max<int64_t>(1, std::min<int64_t>(units, (sm_count() + tiles - 1) / tiles));
+  // The error of a sum grows with the square root of its steps, so long lists take more shares, each SM as many as the
+  // others.  (MACE_SPECIES_MAX_ROWS rows make at most 16 533 shares; the join's table holds 32 767.)
+  p->shares *= (int)std::max<int64_t>(1, (units + (int64_t)p->shares * SL_STEPS - 1) / ((int64_t)p->shares * SL_STEPS));
 }
 
 }  // namespace

@@ -272,6 +272,21 @@ def test_linear_over_many_tiles(sp, dtype, mix):
     assert torch.equal(got, sp.species_linear_grad_weight(x, dy, groups, alpha=0.5))
 
 
+def test_weight_gradient_of_very_long_groups(sp):
+    """The error stays where it is as the rows grow: no fp32 sum takes more than a stated number of steps."""
+    n, k = 300_000_000, 8
+    groups = sp.SpeciesGroups(torch.arange(n, dtype=torch.int32, device="cuda"),
+                              torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    x, dy = randn(n, k, seed=27), randn(1, k, seed=28)
+    want = torch.zeros(k, dtype=torch.float64, device="cuda")
+    mass = torch.zeros_like(want)
+    for part in x.split(1 << 24):
+        want += part.double().sum(0)
+        mass += part.double().abs().sum(0)
+    dw = sp.species_linear_grad_weight(x, dy.expand(n, k), groups)[0]  # (one row of dy, shared)
+    assert_sum(dw, want[:, None] * dy.double(), mass[:, None] * dy.double().abs(), n)
+
+
 def test_weight_gradient_of_the_widest_matrices(sp):
     """65 536 tiles of a matrix, and a group without rows."""
     n, k, g = 3, 32768, 2
