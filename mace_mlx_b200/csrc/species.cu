@@ -473,10 +473,11 @@ constexpr int EG_THREADS = 256;
 
 // A warp sums its share of the grouped list, V channels per lane and RL rows side by side.  The list is read and its
 // rows are loaded UN RL at a time whatever groups they belong to; a group's end only cuts the additions, so that no
-// load waits for a group before it.  1M fp32 rows of 128 channels: 4 groups 88 us with the join, 7921 groups 104 (79 is
+// load waits for a group before it.  1M fp32 rows of 128 channels: 4 groups 86 us with the join, 7921 groups 103 (79 is
 // what HBM needs; group by group 92 and 112).  APART: rows that are not whole 16-byte pieces, a lane's channels 32
-// apart, so that a warp still has 128 channels of 8 rows in flight: 1M rows of 97 channels fp32 87 us, bf16 76 (with
-// one channel per lane 212 and 178).
+// apart, so that a warp still has 128 channels of 8 rows in flight: 1M rows of 97 channels fp32 87 us, bf16 78 (with
+// one channel per lane 212 and 178).  A lane sums 32 rows of the list and then those sums: in one sum of its share the
+// error at 1e8 rows of 17 channels was past 2.6e-6 of the result (3e-7 so, at no cost).
 template <typename T, int V, int RL, bool APART = false>
 __global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad(EmbedGrad p) {
   pdl_wait();
@@ -508,8 +509,10 @@ __global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad(EmbedGrad p) {
   };
   uint32_t lo = offset(g), hi = offset(g + 1);
   bool first = true;
-  float acc[V] = {};
+  float acc[V] = {}, sum[V] = {};  // of the last 32 rows (at most), of those before them
   auto flush = [&]() {
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] += sum[k];
 #pragma unroll
     for (int o = CL; o < 32; o <<= 1)
 #pragma unroll
@@ -534,7 +537,7 @@ __global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad(EmbedGrad p) {
       }
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] = 0.f;
+    for (int k = 0; k < V; ++k) acc[k] = sum[k] = 0.f;
     first = false;
   };
   Raw<T, V, APART> v[UN];
@@ -554,6 +557,11 @@ __global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad(EmbedGrad p) {
   };
   uint32_t b32 = i0;
   auto take = [&](uint32_t b) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      sum[k] += acc[k];
+      acc[k] = 0.f;
+    }
     mine = next;
     next = b + 32 + lane < stop ? p.order[b + 32 + lane] : -1;
   };
@@ -686,16 +694,19 @@ __global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p, int per_c
   };
   // sum of a group's partial rows from, from + step, ...: this lane's channel
   auto partial = [&](int g, int64_t from, int64_t s0, int64_t s1, int step) -> float {
-    float acc = 0.f;
-    if (c < p.C) {
+    float sum = 0.f;
+    if (c < p.C)
+      for (int64_t s = from; s <= s1;) {
+        float acc = 0.f;
 #pragma unroll 4
-      for (int64_t s = from; s <= s1; s += step) {
-        // the group is the second of its first share's partial rows unless the share begins with it
-        const int which = s > s0 || (int64_t)p.offsets[g] <= s * p.share ? 0 : 1;
-        acc += p.part[(s * 2 + which) * p.C + c];
+        for (const int64_t e = min(s + 64 * step, s1 + 1); s < e; s += step) {
+          // the group is the second of its first share's partial rows unless the share begins with it
+          const int which = s > s0 || (int64_t)p.offsets[g] <= s * p.share ? 0 : 1;
+          acc += p.part[(s * 2 + which) * p.C + c];
+        }
+        sum += acc;
       }
-    }
-    return acc;
+    return sum;
   };
   for (int g0 = blockIdx.x * per_cta; g0 < p.G; g0 += gridDim.x * per_cta) {
     if (threadIdx.x == 0) many = 0;
@@ -905,9 +916,15 @@ void group_passes(int G, int* bits, int* passes) {
   *bits = (b + *passes - 1) / *passes;
 }
 
-// rows of one warp's share of the table gradient: enough warps to fill the
-// GPU once (148 SMs x 3 CTAs x 8 warps), but shares of at least 16 rows
-int64_t eg_share(int64_t n) { return std::max<int64_t>(16, (n + 148 * 24 - 1) / (148 * 24)); }
+// rows of one warp's share of the table gradient: enough warps to fill the GPU
+// (148 SMs x 3 CTAs x 8 warps) once, or several times over where a share would
+// pass 4096 rows (the error of a sum grows with the square root of its terms;
+// 20M rows in 1.4 fills instead of 2 take 20 % longer), but at least 16 rows
+int64_t eg_share(int64_t n) {
+  constexpr int64_t WARPS = 148 * 24;
+  const int64_t fills = std::max<int64_t>(1, (n + WARPS * 4096 - 1) / (WARPS * 4096));
+  return std::max<int64_t>(16, (n + WARPS * fills - 1) / (WARPS * fills));
+}
 int64_t eg_shares(int64_t n, int64_t share) { return (n + share - 1) / share; }
 
 int64_t align16(int64_t b) { return (b + 15) & ~(int64_t)15; }

@@ -193,6 +193,21 @@ def test_embedding_gradient_of_long_groups_and_strides(sp):
     assert torch.equal(sp.species_embedding_grad(ones, sp.group_species(z, g)), counts[:, None].expand(g, c))
 
 
+@pytest.mark.parametrize("c", [8, 17])
+def test_embedding_gradient_of_very_long_groups(sp, c):
+    """The error stays where it is as the rows grow: no fp32 sum takes more than a stated number of rows."""
+    n = 100_000_000
+    groups = sp.SpeciesGroups(torch.arange(n, dtype=torch.int32, device="cuda"),
+                              torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    dy = randn(n, c, seed=15)
+    want = torch.zeros(c, dtype=torch.float64, device="cuda")
+    mass = torch.zeros_like(want)
+    for part in dy.split(1 << 23):
+        want += part.double().sum(0)
+        mass += part.double().abs().sum(0)
+    assert_sum(sp.species_embedding_grad(dy, groups)[0], want, mass, n)
+
+
 # -------------------------------------------------------------------- linear
 def linear64(x, w, z, alpha):
     """Output and product magnitudes of the map in 64 bits; x (n, d, k)."""
