@@ -231,6 +231,16 @@ __device__ __forceinline__ void add2(float& x0, float& x1, uint32_t y0, uint32_t
       : "r"(y0), "r"(y1));
 }
 
+__device__ __forceinline__ void mul2(float& x0, float& x1, float y) {
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%0, %1};\n\t"
+      "mov.b64 b, {%2, %2};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(y));
+}
+
 // the bf16 pieces of two values, packed: P = 3: x = h + m + l, each the leading
 // 8 bits of what is left (exact, and no finite value becomes infinite);
 // P = 1: x rounded (exact where it is used)
@@ -621,6 +631,60 @@ __device__ __forceinline__ void copy_out(const SlParams& p, const uint8_t* stage
   __syncwarp();
 }
 
+// Infinities and NaN among split operands: a piece of an infinity is inf - inf, so whatever it enters is NaN, and an
+// infinite piece times a zero one is too: a whole row of results, or a column of them.  So a CTA that has met such a row,
+// or weights that are not finite, goes over its results once more when it is done, and makes those that are NaN from
+// the operands as they are, in fp32.  (A look at every result, or the call within the epilogue, cost 2 to 3 us of 125.)
+
+// Map: this CTA's tiles, each by the epilogue warps that stored it
+template <typename S>
+__device__ __noinline__ void redo_map(const SlParams& p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const Groups q(smem + S::OFF_PRE);
+  const int t0 = q.bounds[0], t1 = q.bounds[1];
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, half = (threadIdx.x >> 7) & 1, CW = p.NT / 2;
+  const int64_t wk = p.transposed ? 1 : p.N, wc = p.transposed ? p.K : 1;
+  Walk w;
+  w.init(p, q, t0);
+#pragma unroll 1
+  for (; w.t < t1; w.next(q, t1)) {
+    const Tile t(p, q, w);
+    const int c0 = t.ct * p.NT + half * CW, c1 = min(c0 + CW, p.N);
+    const float* const wt = static_cast<const float*>(p.w) + (int64_t)w.g * p.K * p.N;
+    RowRef ref;  // lane r: row 32 quad + r
+    ref.load(p, t.at + quad * 32 + lane, t.end);
+    const bool mine = ref.valid(p);
+    const int64_t at = mine ? ref.node * p.out_sn + ref.m * p.out_sm : -1;
+    unsigned left = 0;  // rows with a NaN in these columns
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      const int64_t to = __shfl_sync(0xffffffffu, at, r);
+      const float* const y = static_cast<const float*>(p.out) + to;
+      bool nan = false;
+#pragma unroll
+      for (int c = c0 + lane; c < c0 + 64; c += 32)
+        if (to >= 0 && c < c1) nan |= y[c] != y[c];
+      left |= (unsigned)__any_sync(0xffffffffu, nan) << r;
+    }
+    for (; left; left &= left - 1) {
+      const int r = __ffs(left) - 1;
+      const int64_t from = __shfl_sync(0xffffffffu, mine ? ref.offset(p.a) : 0, r);
+      const float* const x = reinterpret_cast<const float*>(p.a.data + from);
+      float* const y = static_cast<float*>(p.out) + __shfl_sync(0xffffffffu, at, r);
+      bool nan = false;  // a NaN in the row: every result is one
+      for (int k = lane; k < p.K; k += 32) nan |= x[k] != x[k];
+      if (__any_sync(0xffffffffu, nan)) continue;
+      for (int c = c0 + lane; c < c1; c += 32) {
+        if (y[c] == y[c]) continue;
+        float sum = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < p.K; ++k) sum = __fmaf_rn(x[k], wt[k * wk + c * wc], sum);
+        y[c] = p.alpha * sum;
+      }
+    }
+  }
+}
+
 // Weight gradient: a lane's NT / 2 sums of row kl of a 128 x NT tile (columns c0 ..), done with group g: dW itself
 // where this share held the whole group, else a partial tile: a share has two for each tile of the matrix, one for a
 // group that begins with it or before it, one for a group that begins inside it (`inside`) and goes on.  A partial tile
@@ -699,10 +763,11 @@ __device__ __forceinline__ void put_eight(uint8_t* img, int piece, int n, int ch
 // Weights (K, N): an item is one octet of 32 neighbouring columns; transposed (N, K): 8 octets of 4 rows.
 template <typename T, int PB>
 __device__ __forceinline__ void fill_weights(const SlParams& p, uint8_t* img0, int stride, int g, int ct, int k0,
-                                             int nk, uint32_t full) {
+                                             int nk, uint32_t full, volatile int* odd) {
   const int lane = threadIdx.x & 31, w4 = (threadIdx.x >> 5) & 3;
   const int NT = p.NT;
   const T* wt = static_cast<const T*>(p.w) + (int64_t)g * p.K * p.N;
+  float probe = 0.f;
 #pragma unroll 1
   for (int s = 0; s < nk; ++s) {
     uint8_t* const img = img0 + s * stride;
@@ -733,9 +798,14 @@ __device__ __forceinline__ void fill_weights(const SlParams& p, uint8_t* img0, i
       for (int u = 0; u < 4; ++u) {
         const int j = h * 16 + u * 4 + w4;
         const int n = p.transposed ? j * 4 + (lane >> 3) : (j >> 3) * 32 + lane;
+        if constexpr (PB == 3) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) probe = __fmaf_rn(v[u][e], 0.f, probe);
+        }
         if (n < NT) put_eight<PB>(img, p.img, n, p.transposed ? lane & 7 : j & 7, v[u]);
       }
     }
+    if (PB == 3 && probe != 0.f) *odd = 1;
     tc::fence_proxy_async();
     warp_arrive(full + 8 * s);
   }
@@ -751,6 +821,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + S::NBAR);
   volatile int* const abort = reinterpret_cast<int*>(tslot + 1);
+  volatile int* const odd = reinterpret_cast<int*>(tslot + 2);  // a weight or a row is not finite
   auto bar = [&](int i) { return tc::smem_u32(bars + i); };
   auto A_FULL = [&](int s) { return bar(s); };
   auto A_FREE = [&](int s) { return bar(2 + s); };
@@ -770,7 +841,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
   const int NT = p.NT;
   if (warp == 15) {  // while the others wait for the offsets
     if (lane == 0) {
-      *abort = 0;
+      *abort = *odd = 0;
       for (int s = 0; s < 2; ++s) {
         tc::mbar_init(A_FULL(s), 4);
         tc::mbar_init(A_FREE(s), 1);
@@ -950,7 +1021,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
     };
     bool ok = true;
     auto fill = [&](int g, int ct, int k0, int nk, int slot0) {
-      fill_weights<T, P>(p, smem + slot0 * P * p.img, P * p.img, g, ct, k0, nk, bar(8 + slot0));
+      fill_weights<T, P>(p, smem + slot0 * P * p.img, P * p.img, g, ct, k0, nk, bar(8 + slot0), odd);
     };
     Walk w;
     w.init(p, q, t0);
@@ -1008,6 +1079,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
     float acc[64];
     bool ok = true;
     bool fresh = true;   // acc holds nothing yet
+    float probe = 0.f;   // NaN once a row was not finite (its first result tells)
     RowRef ref{-1, -1};  // this lane's row of the tile, loaded while the tile is computed
     int ct = 0, k = 0;   // the tile's column tile, the step
     for (int sn = 0; w.t < t1 && ok; ++sn) {
@@ -1047,9 +1119,10 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
       // touch 32 rows per instruction (600 000 rows 128 -> 128 fp32: 149 us with them, 130 staged).
       constexpr int CB = 128 / sizeof(T);  // columns of a 128-byte row segment
       const bool mine = ref.valid(p);
+      if (P == 3 && mine) probe = __fmaf_rn(acc[0], 0.f, probe);
       // (alpha times the weights instead, before they are split, left the range of fp32 where the result does not)
 #pragma unroll
-      for (int k = 0; k < 64; ++k) acc[k] *= p.alpha;
+      for (int k = 0; k < 64; k += 2) mul2(acc[k], acc[k + 1], p.alpha);
 #pragma unroll
       for (int b = 0; b < 64; b += CB) {
         const int left = min(p.N - c0 - b, CW - b);  // columns of this segment
@@ -1077,10 +1150,13 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
       fresh = true;
       w.next(q, t1);
     }
+    if (P == 3 && probe != 0.f) *odd = 1;
   }
   tc::fence_before_sync();
   __syncthreads();
   if (tid == 0 && *abort) atomicExch(&g_species_error, TC_ERR_TIMEOUT);
+  if constexpr (P == 3)
+    if (*odd && !*abort && threadIdx.x >= 256) redo_map<S>(p);
   if (warp == 15) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, SL_TMEM);

@@ -198,6 +198,67 @@ __device__ __forceinline__ void fetch_unit(uint32_t dst, const RowView& v, const
   }
 }
 
+// As redo_map: rows 32 quad .. of this share's results and partial tiles of matrix tile (k0, n0), by the warp that stored
+// them.  The values of an 8-bit checkpoint are those that restoring gives.
+template <typename TA, typename T>
+__device__ __noinline__ void redo_wgrad(const SlParams& p, const Groups& q, int t0, int t1, int tile, int share, int k0,
+                                        int n0, int quad) {
+  constexpr int CB = 16;  // columns at a time
+  const int kl = quad * 32 + (threadIdx.x & 31), k = k0 + kl;
+  __syncwarp();
+  Walk w;
+  w.init(p, q, t0);
+#pragma unroll 1
+  while (w.t < t1) {
+    const int begin = q.pre[w.g], end = min(q.pre[w.g + 1], t1), d = p.d;
+    const bool whole = begin >= t0 && q.pre[w.g + 1] <= t1;
+    const int64_t first = (int64_t)q.lo[w.g] * d;
+    const int a0 = (int)(first + (int64_t)(w.t - begin) * SL_KC);
+    const int a1 = (int)min(first + (int64_t)(end - begin) * SL_KC, (int64_t)q.hi[w.g] * d);
+    T* const out = static_cast<T*>(p.out) + ((int64_t)w.g * p.K + k) * p.N + n0;
+    float* const part = p.part + ((((int64_t)tile * p.shares + share) * 2 + (begin > t0)) * 32 * p.NT + kl) * 4;
+#pragma unroll 1
+    for (int c = 0; c < min(p.NT, p.N - n0); c += CB) {
+      unsigned left = 0;  // columns that are NaN
+      if (k < p.K)
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+          if (c + j < p.NT && n0 + c + j < p.N) {
+            const float v = whole ? to_f32(out[c + j]) : part[(c + j) / 4 * 512 + (c + j) % 4];
+            left |= (unsigned)(v != v) << j;
+          }
+      if (!__any_sync(0xffffffffu, left != 0)) continue;
+      float sum[CB] = {};
+      unsigned open = left;  // those whose sum is not NaN yet
+#pragma unroll 1
+      for (int a = a0; a < a1 && __any_sync(0xffffffffu, open != 0); ++a) {
+        const int i = d > 1 ? (int)(__umulhi((uint32_t)a, p.div_mul) >> p.div_shift) : a, m = a - i * d;
+        const int64_t node = p.order[i];
+        if (node < 0 || node >= p.n) continue;
+        const T* const dy = reinterpret_cast<const T*>(p.b.data + node * p.b.sn + m * p.b.sm) + n0 + c;
+        float x = 0.f;
+        if (k < p.K) x = to_f32(reinterpret_cast<const TA*>(p.a.data + node * p.a.sn + m * p.a.sm)[k]);
+        if constexpr (sizeof(TA) == 1) x *= p.a_scale[(node * d + m) * p.ka_blocks + k0 / MACE_CHECKPOINT_BLOCK];
+#pragma unroll
+        for (int j = 0; j < CB; ++j) {
+          if (n0 + c + j < p.N) sum[j] = __fmaf_rn(x, to_f32(dy[j]), sum[j]);
+          if (sum[j] != sum[j]) open &= ~(1u << j);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < CB; ++j)
+        if ((left >> j) & 1u) {
+          if (whole)
+            out[c + j] = from_f32<T>(p.alpha * sum[j]);
+          else
+            part[(c + j) / 4 * 512 + (c + j) % 4] = sum[j];
+        }
+    }
+    w.t = end - 1;
+    w.next(q, t1);
+  }
+}
+
 template <typename TA, typename T, bool VEC>
 __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_constant__ SlParams p) {
   using S = Wg<TA, T, VEC>;
@@ -209,6 +270,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_co
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + S::NBAR);
   volatile int* const abort = reinterpret_cast<int*>(tslot + 1);
+  volatile int* const odd = reinterpret_cast<int*>(tslot + 2);  // something that entered the sums is not finite
   auto bar = [&](int i) { return tc::smem_u32(bars + i); };
   auto A_FULL = [&](int s) { return bar(s); };
   auto A_FREE = [&](int s) { return bar(2 + s); };
@@ -227,7 +289,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_co
   }
   if (warp == 20) {  // while the others wait for the offsets
     if (lane == 0) {
-      *abort = 0;
+      *abort = *odd = 0;
       for (int s = 0; s < 2; ++s) {
         tc::mbar_init(A_FULL(s), 8);
         tc::mbar_init(A_FREE(s), 1);
@@ -449,6 +511,9 @@ __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_co
       const uint32_t tq = SL_D + ((uint32_t)(quad * 32) << 16);
       float acc[128];
       bool fresh = true;  // acc holds nothing yet
+      // NaN once a value of x or of dy was not finite: what it enters is a row of this lane, or a column of every lane, of
+      // which each warp watches a quarter
+      float probe = 0.f;
       for (int sn = 0; w.t < t1 && ok; ++sn) {
         const int s = sn & 1;
         ok = __all_sync(0xffffffffu, wait_phase(D_FULL(s), (sn >> 1) & 1, abort));
@@ -478,11 +543,27 @@ __global__ void __launch_bounds__(WG_THREADS, 1) k_species_wgrad(const __grid_co
         const bool group_ends = w.t + len == pre[w.g + 1];
         if (group_ends || w.t + len == t1) {
           const bool whole = group_ends && pre[w.g] >= t0, inside = pre[w.g] > t0;
+          if constexpr (PB == 3) {
+            probe = __fmaf_rn(acc[0], 0.f, probe);
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              if (b == quad && b * 32 < NT) {
+                float t[2] = {};
+#pragma unroll
+                for (int k = 0; k < 32; ++k) t[k & 1] = __fmaf_rn(acc[b * 32 + k], 0.f, t[k & 1]);
+                probe += t[0] + t[1];
+              }
+          }
           finish_wgrad<T>(p, acc, w.g, whole, inside, tile, share, k0, n0, quad * 32 + lane, 0, min(NT, 64));
           if (NT > 64) finish_wgrad<T>(p, acc + 64, w.g, whole, inside, tile, share, k0, n0, quad * 32 + lane, 64, NT - 64);
           fresh = true;
         }
         advance(w, len);
+      }
+      if constexpr (PB == 3) {
+        if (probe != 0.f) *odd = 1;
+        tc::named_sync(1, 128);
+        if (ok && *odd) redo_wgrad<TA, T>(p, q, t0, t1, tile, share, k0, n0, quad);
       }
     }
   }

@@ -293,8 +293,8 @@ def species_linear(x: torch.Tensor, weight: torch.Tensor, groups: SpeciesGroups,
     ``checkpoint`` keeps x for the weight gradient in 8 bits
     (``checkpoint_rows``) instead of x itself.
 
-    float32 products keep fp32 accuracy; an infinity in a float32 row or
-    matrix gives infinities or NaN in the results it enters.
+    float32 products keep fp32 accuracy, here and in the gradients; infinities
+    and NaN enter the results as they enter fp32 sums.
     """
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         if out is not None or transpose:

@@ -381,6 +381,63 @@ def test_rows_with_infinities_and_nan_stay_apart(sp):
     assert not got[17].isfinite().any() and got[200].isnan().all()
 
 
+def assert_ieee(got, want, mass, n, what=""):
+    """Infinities and NaN where the 64-bit result has them (rounded to the type), and the other values within bounds."""
+    want = torch.where(want.to(got.dtype).isinf(), want.sign() * torch.inf, want)
+    assert torch.equal(got.isnan(), want.isnan()), f"{what}: NaN at other places"
+    odd = ~want.isfinite()
+    assert torch.equal(got[odd & ~want.isnan()].double(), want[odd & ~want.isnan()]), f"{what}: other infinities"
+    assert odd.any() and not odd.all()
+    assert_sum(got.where(~odd, 0.0), want.where(~odd, 0.0), mass.where(~odd, 0.0), n, what)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,k,m,g", [(300, 1, 128, 64, 2), (300, 3, 33, 70, 5), (9001, 3, 150, 40, 3)])
+def test_infinities_enter_sums_as_in_the_definition(sp, dtype, n, d, k, m, g):
+    z = draw_species(n, g, 53, pad=0.1)
+    z[:8] = torch.arange(8, device="cuda") % g
+    x, w, dy = randn(n, d, k, seed=54, dtype=dtype), randn(g, k, m, seed=55, dtype=dtype), \
+        randn(n, d, m, seed=56, dtype=dtype)
+    groups = sp.group_species(z, g)
+
+    def both(inf_x, inf_w, inf_dy, what):
+        y, mass = linear64(x, w, z, 0.5)
+        assert_ieee(sp.species_linear(x, w, groups, alpha=0.5), y, mass, k, what + ": forward")
+        dx, mass = linear64(dy, w.transpose(1, 2), z, 0.5)
+        dw, wmass = wgrad64(x, dy, z, g, 0.5)
+        got_x, got_w = sp.species_linear_grad(x, dy, w, groups, alpha=0.5)
+        if inf_w or inf_dy:
+            assert_ieee(got_x, dx, mass, m, what + ": input gradient")
+        if inf_x or inf_dy:
+            assert_ieee(got_w, dw, wmass, n * d, what + ": weight gradient")
+
+    x[3, 0, 5], x[4, 0, 7], x[4, 0, 8] = torch.inf, -torch.inf, -torch.inf
+    both(True, False, False, "rows of x")
+    x[5, 0, 2] = torch.nan
+    both(True, False, False, "a NaN beside them")
+    dy[6, 0, 3], dy[2, 0, 4] = -torch.inf, torch.inf
+    both(True, False, True, "rows of dy")
+    w[1, 2, 6] = torch.inf
+    both(True, True, True, "a matrix")
+    assert sp.error_flag() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_checkpoint_whose_scale_times_the_gradient_overflows(sp, dtype):
+    """q = 0 adds nothing, the others what the restored values give."""
+    n, k, m, g = 5000, 130, 48, 3
+    z = draw_species(n, g, 93)
+    x, dy = randn(n, 1, k, seed=94), randn(n, 1, m, seed=95, dtype=dtype)
+    x[7], dy[7] = x[7] * 1e25, 1e20
+    x[7, 0, ::3] = 0.0
+    ck = sp.checkpoint_rows(x)
+    values = sp.restore_rows(ck).double()
+    dw, mass = wgrad64(values, dy, z, g, 1.0)
+    got = sp.species_linear_grad_weight(ck, dy, sp.group_species(z, g))
+    assert_ieee(got, dw, mass, n)
+    assert got[z[7], ::3].isfinite().all()
+
+
 def test_large_and_small_magnitudes(sp):
     """The split operands keep fp32's range: nothing overflows or is lost near its ends."""
     n, k, m = 130, 64, 32
