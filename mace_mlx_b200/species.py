@@ -11,7 +11,8 @@ train them.
   the forward and the backward, which ``species_linear_grad_weight`` reads
 
 ``species_embedding`` and ``species_linear`` take part in autograd when an
-argument requires a gradient (once differentiable).
+argument requires a gradient (once differentiable, in reverse mode: a tensor
+with a forward-mode tangent is refused).
 
 Every call runs hand-written kernels of ``libmace_b200`` on the current stream
 of the tensors' device, allocates only its results and workspace through
@@ -34,6 +35,7 @@ import functools
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native as nv
 
@@ -76,6 +78,8 @@ def _cuda(name: str, t: torch.Tensor) -> int:
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path), got device {t.device}")
+    if forward_ad._current_level >= 0 and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a tangent: the species operators have no forward-mode derivative")
     return t.get_device()
 
 
@@ -232,6 +236,7 @@ def species_embedding(table: torch.Tensor, species: torch.Tensor, *, scale: floa
     if torch.is_grad_enabled() and table.requires_grad:
         if out is not None:
             raise ValueError("out= cannot take part in autograd")
+        _cuda("table", table)
         return _EmbeddingFn.apply(table, species, scale, groups)
     return _embedding(table, species, scale, out)
 
@@ -299,6 +304,7 @@ def species_linear(x: torch.Tensor, weight: torch.Tensor, groups: SpeciesGroups,
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         if out is not None or transpose:
             raise ValueError("out= and transpose= cannot take part in autograd")
+        _cuda("x", x), _cuda("weight", weight)
         return _LinearFn.apply(x, weight, groups.order, groups.offsets, alpha, checkpoint)
     return _linear(x, weight, groups, alpha, transpose, out)
 

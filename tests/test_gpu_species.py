@@ -665,6 +665,36 @@ def test_refusals(sp):
     assert sp.error_flag() == 0
 
 
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_tangents_are_refused(sp, requires_grad):
+    """A forward-mode tangent would be dropped: every entry that takes features refuses it."""
+    from torch.autograd import forward_ad
+
+    z = torch.zeros(8, dtype=torch.int32, device="cuda")
+    groups = sp.group_species(z, 2)
+    plain = {"x": torch.zeros(8, 3, 16), "w": torch.zeros(2, 16, 4), "dy": torch.zeros(8, 3, 4), "t": torch.zeros(2, 16)}
+    plain = {k: v.cuda() for k, v in plain.items()}
+    ck = sp.checkpoint_rows(plain["x"])
+    with forward_ad.dual_level():
+        dual = {k: forward_ad.make_dual(v.clone().requires_grad_(requires_grad), torch.ones_like(v))
+                for k, v in plain.items()}
+        scale = forward_ad.make_dual(ck.scale, torch.ones_like(ck.scale))
+        for i, call in enumerate((
+            lambda: sp.species_linear(dual["x"], plain["w"], groups), lambda: sp.species_linear(plain["x"], dual["w"], groups),
+            lambda: sp.species_linear_grad(dual["x"], plain["dy"], plain["w"], groups),
+            lambda: sp.species_linear_grad(plain["x"], dual["dy"], plain["w"], groups),
+            lambda: sp.species_linear_grad(plain["x"], plain["dy"], dual["w"], groups),
+            lambda: sp.species_linear_grad_weight(dual["x"], plain["dy"], groups),
+            lambda: sp.species_linear_grad_weight(plain["x"], dual["dy"], groups),
+            lambda: sp.species_embedding(dual["t"], z), lambda: sp.species_embedding_grad(dual["x"][:, 0], groups),
+            lambda: sp.checkpoint_rows(dual["x"]), lambda: sp.restore_rows(sp.RowCheckpoint(ck.q, scale)),
+        )):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+                pytest.fail(f"call {i} was accepted")
+        sp.species_linear(plain["x"], plain["w"], groups)  # without a tangent: as ever
+
+
 def test_groupings_that_are_not_permutations_stay_in_bounds(sp):
     """order and offsets come from the caller: whatever they hold, no row outside the tensors is touched."""
     n, k, g = 300, 32, 3
