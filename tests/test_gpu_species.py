@@ -139,6 +139,18 @@ def test_embedding_lookup(sp, dtype, n, c):
     assert torch.equal(sp.species_embedding(table, z, scale=scale), want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c,pitch", [(64, 64), (33, 33), (33, 40)])
+def test_embedding_of_padding_is_zero_whatever_the_scale(sp, dtype, c, pitch):
+    n, g = 500, 7
+    table, z = randn(g, c, seed=3, dtype=dtype), draw_species(n, g, 5, pad=0.3)
+    for scale in (float("inf"), float("nan"), -2.0):
+        out = torch.ones(n, pitch, dtype=dtype, device="cuda")[:, :c]
+        got = sp.species_embedding(table, z, scale=scale, out=out)
+        assert not got[~valid(z, g)].any()
+        assert torch.equal(got[valid(z, g)].isfinite(), torch.full_like(got[valid(z, g)], scale == -2.0, dtype=torch.bool))
+
+
 def test_embedding_of_strided_tables_and_outputs(sp):
     g, n = 5, 257
     z = draw_species(n, g, 4, pad=0.1)
