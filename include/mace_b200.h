@@ -462,7 +462,7 @@ int mace_species_embed(int32_t dtype, const void* table, int64_t table_stride, i
 
 /* grad_table[g] = scale * sum of grad[order[i]] over offsets[g] <= i < offsets[g + 1]
  * (grad_table is (num_groups, C) contiguous; rows of empty groups are zero).
- * The summation order depends on the sizes only. */
+ * The summation order depends on the sizes and on whether rows are whole 16-byte pieces, nothing else. */
 int mace_species_embed_grad_workspace(int64_t n, int32_t num_groups, int32_t C, int64_t* bytes);
 int mace_species_embed_grad(int32_t dtype, const void* grad, int64_t grad_stride, const int32_t* order,
                             const int32_t* offsets, int64_t n, int32_t num_groups, int32_t C, float scale,

@@ -496,6 +496,54 @@ def test_linear_past_32_bit_offsets(sp):
     assert torch.equal(sp.species_linear(dense, w, groups, out=out), sp.species_linear(dense, w, groups))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,m", [(64, 32), (33, 21)])
+def test_unaligned_rows_past_32_bit_offsets(sp, dtype, k, m):
+    """Rows at any address and results whose element offsets pass 2^32, in every operator."""
+    n, g = 500, 3
+    pitch = 9_000_000
+    table = torch.empty(n, pitch, dtype=dtype, device="cuda")  # 4.5e9 elements, 9 or 18 GB
+    z = draw_species(n, g, 74, pad=0.1)
+    groups = sp.group_species(z, g)
+    x, dy, w = randn(n, k, seed=75, dtype=dtype), randn(n, m, seed=76, dtype=dtype), randn(g, k, m, seed=77, dtype=dtype)
+    far_x, far_dy = table[:, -k - 1:-1], table[:, pitch // 2 + 1:pitch // 2 + 1 + m]
+    far_x.copy_(x), far_dy.copy_(dy)
+    y, mass = linear64(x[:, None], w, z, 1.0)
+    far = table[:, pitch - 2000 + 1:pitch - 2000 + 1 + m]
+    for source in (x, far_x):
+        table[:, pitch - 2000:pitch - 2000 + m + 2] = 7.0
+        assert_sum(sp.species_linear(source, w, groups, out=far)[:, None], y, mass, k, "forward")
+        assert (table[:, pitch - 2000] == 7.0).all() and (table[:, pitch - 2000 + 1 + m] == 7.0).all()
+    dw, mass = wgrad64(x[:, None], dy[:, None], z, g, 1.0)
+    assert_sum(sp.species_linear_grad_weight(far_x, far_dy, groups), dw, mass, n, "weight gradient")
+    ck = sp.checkpoint_rows(x)
+    far_ck = sp.checkpoint_rows(far_x)
+    assert torch.equal(far_ck.q, ck.q) and torch.equal(far_ck.scale, ck.scale)
+    assert torch.equal(sp.species_linear_grad_weight(ck, far_dy, groups), sp.species_linear_grad_weight(ck, dy, groups))
+    ok = valid(z, g)
+    want = torch.zeros(g, k, dtype=torch.float64, device="cuda").index_add_(0, z[ok].long(), x[ok].double())
+    mass = torch.zeros_like(want).index_add_(0, z[ok].long(), x[ok].double().abs())
+    assert_sum(sp.species_embedding_grad(far_x, groups), want, mass, n, "embedding gradient")
+    assert torch.equal(sp.species_embedding(w[0], z, out=far), sp.species_embedding(w[0], z))
+    assert sp.error_flag() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,m", [(64, 128), (40, 24), (33, 7)])
+def test_weights_at_any_address(sp, dtype, k, m):
+    n, d, g = 400, 3, 5
+    z = draw_species(n, g, 34, pad=0.1)
+    x, dy = randn(n, d, k, seed=35, dtype=dtype), randn(n, d, m, seed=36, dtype=dtype)
+    groups = sp.group_species(z, g)
+    for off in (1, 3):
+        w = randn(g * k * m + off, seed=37, dtype=dtype)[off:].view(g, k, m)
+        assert w.is_contiguous() and w.data_ptr() % 16
+        y, mass = linear64(x, w, z, 0.3)
+        assert_sum(sp.species_linear(x, w, groups, alpha=0.3), y, mass, k, "forward")
+        dx, mass = linear64(dy, w.transpose(1, 2), z, 0.3)
+        assert_sum(sp.species_linear_grad(x, dy, w, groups, alpha=0.3)[0], dx, mass, m, "input gradient")
+
+
 # ---------------------------------------------------------------- checkpoint
 def quantise(x):
     """The checkpoint's definition in fp32 (each operation rounded once)."""
@@ -581,6 +629,31 @@ def test_autograd_matches_differences(sp, checkpoint):
             assert abs(diff - dot) <= bound, (diff, dot, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_autograd_through_a_checkpoint_is_that_of_the_restored_rows(sp, dtype):
+    """The weight gradient against its formula and against differences of the map on the rows that the checkpoint holds."""
+    n, d, k, m, g = 150, 3, 48, 40, 5
+    z = draw_species(n, g, 106, pad=0.1)
+    groups = sp.group_species(z, g)
+    x, w, v = randn(n, d, k, seed=107, dtype=dtype), randn(g, k, m, seed=108, dtype=dtype), randn(n, d, m, seed=109, dtype=dtype)
+    x.requires_grad_(), w.requires_grad_()
+    sp.species_linear(x, w, groups, alpha=0.2, checkpoint=True).backward(v)
+    kept = sp.restore_rows(sp.checkpoint_rows(x.detach())).double()
+    dw, mass = wgrad64(kept, v, z, g, 0.2)
+    assert_sum(w.grad, dw, mass, n * d, "weight gradient")
+    dx, mass = linear64(v, w.detach().transpose(1, 2), z, 0.2)
+    assert_sum(x.grad, dx, mass, m, "input gradient")
+    if dtype == torch.float32:
+        # the map is linear in w: the difference over any step, in 64 bits, is the gradient's product with the step
+        step = randn(g, k, m, seed=110)
+        diff = float(((linear64(kept, w.detach() + step, z, 0.2)[0] - linear64(kept, w.detach(), z, 0.2)[0]) * v.double()).sum())
+        dot = float((w.grad.double() * step.double()).sum())
+        # every entry of the gradient within assert_sum's bound, and w + step rounded once
+        bound = float(((n * d + 16) * 2 * U * wgrad64(kept, v, z, g, 0.2)[1] * step.abs().double()).sum())
+        bound += float((U * (w.detach() + step).abs().double() * wgrad64(kept, v, z, g, 0.2)[1]).sum())
+        assert abs(diff - dot) <= bound < 0.05 * abs(diff), (diff, dot, bound)
+
+
 def test_embedding_autograd_and_expanded_gradients(sp):
     n, g, c = 500, 7, 24
     z = draw_species(n, g, 110, pad=0.1)
@@ -628,6 +701,42 @@ def test_other_streams_and_cuda_graphs(sp):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_from_two_host_threads(sp):
+    import threading
+
+    n, d, k, g = 3000, 3, 64, 6
+
+    def work(seed):
+        z = draw_species(n, g, seed, pad=0.05)
+        x, w = randn(n, d, k, seed=seed + 1), randn(g, k, k, seed=seed + 2)
+        groups = sp.group_species(z, g)
+        y = sp.species_linear(x, w, groups)
+        return [*groups, y, *sp.species_linear_grad(x, y, w, groups),
+                sp.species_linear_grad_weight(sp.checkpoint_rows(x), y, groups), sp.species_embedding_grad(y[:, 0], groups)]
+
+    want = {seed: work(seed) for seed in (150, 160)}
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def thread(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[seed] = work(seed)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=thread, args=(seed,)) for seed in want]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for seed, values in want.items():
+        assert all(torch.equal(a, b) for a, b in zip(got[seed], values, strict=True))
 
 
 # ------------------------------------------------------------------ refusals
