@@ -443,7 +443,7 @@ __device__ __forceinline__ void write_spans(const SlParams& p, const Groups& q) 
     int span = -1;
     if (u0 < u1) {
       const int s0 = share_of(u0);
-      span = s0 | (u0 > s0 * all / shares) << 15 | share_of(u1 - 1) << 16;
+      span = s0 | (s0 * all < u0 * shares) << 15 | share_of(u1 - 1) << 16;  // (u0 > floor(s0 all / shares))
     }
     p.spans[g] = span;
   }
