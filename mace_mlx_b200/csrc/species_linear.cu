@@ -1190,11 +1190,12 @@ namespace {
 
 // dW of the groups that several shares hold, in share order, and of empty groups (zero).  CTA (g, y, tile): group g,
 // rows 8 (y % 16) .. of the tile, in blocks of 8 rows x 8 column quads (64 lanes).  Few shares: the four sets of 64
-// threads of the CTAs with y < 16 take a block each; many: CTA y takes block y / 16, each set every fourth share
-// (gradients of 40 000 rows 128 x 128 in 4 groups: 19.1 us, 32.6 with one set per block; 300 000 rows in 89: no
-// difference).
+// threads of the CTAs with y < 16 take a block each; many: CTA y takes block y / 16 (of more than 16 groups, which mostly
+// have few shares, all blocks), each set every fourth share.  Eight loads in flight per thread need its 64 registers
+// (weight gradients of 40 000 rows 128 x 128 in 4 groups: 20.8 us, 21.8 with 40 registers, 32.6 with one set per block;
+// of 60 000 rows in 89 groups 28.4, 29.8 with a CTA per block).
 template <typename T>
-__global__ void __launch_bounds__(256, 6) k_species_wgrad_join(const __grid_constant__ SlParams p) {
+__global__ void __launch_bounds__(256, 4) k_species_wgrad_join(const __grid_constant__ SlParams p) {
   pdl_wait();
   __shared__ float4 part[4][64];
   const int g = blockIdx.x, tid = threadIdx.x;
@@ -1202,7 +1203,7 @@ __global__ void __launch_bounds__(256, 6) k_species_wgrad_join(const __grid_cons
   const int s0 = span & 0x7fff, s1 = span >> 16;  // shares of the group; none: s1 = -1
   if (s0 == s1) return;                           // written by its only share
   const int lane = tid & 63, sl = tid >> 6;
-  const int kl = (blockIdx.y & 15) * 8 + (lane & 7), block = blockIdx.y >> 4;
+  const int kl = (blockIdx.y & 15) * 8 + (lane & 7), block = blockIdx.y >> 4, blocks = gridDim.y >> 4;
   const int tiles = p.n_ct * p.n_kt;
   for (int tile = blockIdx.z; tile < tiles; tile += gridDim.z) {
     const int k0 = (tile / p.n_ct) * 128, n0 = (tile % p.n_ct) * p.NT;
@@ -1239,21 +1240,23 @@ __global__ void __launch_bounds__(256, 6) k_species_wgrad_join(const __grid_cons
       if (block == 0 && cq * 4 < p.NT) write(cq, sum(cq, s0, 1));
       continue;
     }
-    const int cq = block * 8 + (lane >> 3);
-    part[sl][lane] = sum(cq, s0 + sl, 4);
-    __syncthreads();
-    if (sl == 0) {
-      float4 a = part[0][lane];
+    for (int b = block; b * 32 < p.NT; b += blocks) {
+      const int cq = b * 8 + (lane >> 3);
+      part[sl][lane] = sum(cq, s0 + sl, 4);
+      __syncthreads();
+      if (sl == 0) {
+        float4 a = part[0][lane];
 #pragma unroll
-      for (int q = 1; q < 4; ++q) {
-        a.x += part[q][lane].x;
-        a.y += part[q][lane].y;
-        a.z += part[q][lane].z;
-        a.w += part[q][lane].w;
+        for (int q = 1; q < 4; ++q) {
+          a.x += part[q][lane].x;
+          a.y += part[q][lane].y;
+          a.z += part[q][lane].z;
+          a.w += part[q][lane].w;
+        }
+        write(cq, a);
       }
-      write(cq, a);
+      __syncthreads();
     }
-    __syncthreads();  // (the next tile's)
   }
 }
 
@@ -1487,7 +1490,7 @@ extern "C" int mace_species_linear_wgrad(int32_t dtype, const void* x, int64_t x
   else  // bf16 in whole pieces: nothing to convert
     rc = vec ? launch_direct<true>(p, grid, s) : launch_wgrad<bf16, bf16, false>(p, grid, s);
   if (rc) return rc;
-  const dim3 jg(G, 16 * (p.NT / 32), std::min(p.n_ct * p.n_kt, 65535));  // (a grid's z; there may be one tile more)
+  const dim3 jg(G, 16 * (G > 16 ? 1 : p.NT / 32), std::min(p.n_ct * p.n_kt, 65535));  // (a grid's z; there may be one tile more)
   return launch("species_wgrad_join", dtype == MACE_F32 ? k_species_wgrad_join<float> : k_species_wgrad_join<bf16>, jg, 256,
                 0, s, p);
 }
