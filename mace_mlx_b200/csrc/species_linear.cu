@@ -231,14 +231,16 @@ __device__ __forceinline__ void add2(float& x0, float& x1, uint32_t y0, uint32_t
       : "r"(y0), "r"(y1));
 }
 
-__device__ __forceinline__ void mul2(float& x0, float& x1, float y) {
-  asm("{\n\t.reg .b64 a, b;\n\t"
+// (x0 + z y0, x1 + z y1)
+__device__ __forceinline__ void fma2(float& x0, float& x1, uint32_t y0, uint32_t y1, float z) {
+  asm("{\n\t.reg .b64 a, b, c;\n\t"
       "mov.b64 a, {%0, %1};\n\t"
-      "mov.b64 b, {%2, %2};\n\t"
-      "mul.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "mov.b64 c, {%4, %4};\n\t"
+      "fma.rn.f32x2 a, b, c, a;\n\t"
       "mov.b64 {%0, %1}, a;\n\t}"
       : "+f"(x0), "+f"(x1)
-      : "f"(y));
+      : "r"(y0), "r"(y1), "f"(z));
 }
 
 // the bf16 pieces of two values, packed: P = 3: x = h + m + l, each the leading
@@ -1098,6 +1100,8 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
 #pragma unroll
         for (int k = 0; k < 64; ++k) acc[k] = 0.f;
       }
+      // (alpha meets the sums of a step: with the weights, before they are split, it left the range of fp32 where the
+      // result does not)
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         uint32_t v[16];
@@ -1108,7 +1112,7 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
           warp_arrive(D_FREE(s));
         }
 #pragma unroll
-        for (int k = 0; k < 16; k += 2) add2(acc[h * 16 + k], acc[h * 16 + k + 1], v[k], v[k + 1]);
+        for (int k = 0; k < 16; k += 2) fma2(acc[h * 16 + k], acc[h * 16 + k + 1], v[k], v[k + 1], p.alpha);
       }
       fresh = false;
       k += S::LONG ? n_k : 1;
@@ -1120,9 +1124,6 @@ __global__ void __launch_bounds__(SL_THREADS, 1) k_species_map(const __grid_cons
       constexpr int CB = 128 / sizeof(T);  // columns of a 128-byte row segment
       const bool mine = ref.valid(p);
       if (P == 3 && mine) probe = __fmaf_rn(acc[0], 0.f, probe);
-      // (alpha times the weights instead, before they are split, left the range of fp32 where the result does not)
-#pragma unroll
-      for (int k = 0; k < 64; k += 2) mul2(acc[k], acc[k + 1], p.alpha);
 #pragma unroll
       for (int b = 0; b < 64; b += CB) {
         const int left = min(p.N - c0 - b, CW - b);  // columns of this segment
