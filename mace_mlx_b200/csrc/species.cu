@@ -849,10 +849,11 @@ __global__ void __launch_bounds__(RW_THREADS) k_checkpoint(const T* x, int64_t x
   if (lane < CK_ROWS && i0 + lane < items) scale[i0 + lane] = mine;
 }
 
-// x = q scale, bound by HBM (1.6M rows of 128 fp32 channels 163 us, 6.3 TB/s).
+// x = q scale, bound by HBM (1.6M rows of 128 fp32 channels 162 us, 6.4 TB/s; bf16 109, 5.7; of 97 channels 166 and 166;
+// with 5 CTAs on an SM instead of 8 fp32 183, bf16 151).
 // Four consecutive elements of the contiguous (rows, C) result per thread and step; a vector may pass a row's end.
 template <typename T>
-__global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* q, const float* scale, int64_t total, int C, int nb,
+__global__ void __launch_bounds__(RW_THREADS, 8) k_restore(const int8_t* q, const float* scale, int64_t total, int C, int nb,
                                                         T* x, RowDiv div, int vec) {
   pdl_wait();
   const int64_t e0 = blockIdx.x * (int64_t)(RW_THREADS * RS_UNROLL * 4);
@@ -876,39 +877,49 @@ __global__ void __launch_bounds__(RW_THREADS) k_restore(const int8_t* q, const f
         if (at + k < total) w[j] |= (uint32_t)(uint8_t)load_in(q + at + k) << (8 * k);
     }
   }
+  auto values = [&](int j, float* v) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (float)(int8_t)(w[j] >> (8 * k));
+  };
+  auto store = [&](int j, const float* v) {
+    const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
+    if (vec && at + 4 <= total) {
+      store4(x + at, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (at + k < total) x[at + k] = from_f32<T>(v[k]);
+    }
+  };
+  if ((C & 3) == 0) {  // a vector has one scale: rows and blocks are multiples of 4
+#pragma unroll
+    for (int j = 0; j < RS_UNROLL; ++j) {
+      float v[4];
+      values(j, v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] *= sc[j];
+      store(j, v);
+    }
+    return;
+  }
   float v[RS_UNROLL][4];
 #pragma unroll
   for (int j = 0; j < RS_UNROLL; ++j) {
     const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[j][k] = (float)(int8_t)(w[j] >> (8 * k));
+    values(j, v[j]);
     const uint32_t local = first + (threadIdx.x + j * RW_THREADS) * 4;
     uint32_t r = div.quotient(local), c = local - r * C;
-    if (c + 4 <= (uint32_t)C && (C & 3) == 0) {  // (a block boundary is a multiple of 4)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[j][k] *= sc[j];
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (at + k < total) v[j][k] *= load_in(scale + (row0 + r) * nb + c / MACE_CHECKPOINT_BLOCK);
-        if (++c == (uint32_t)C) {
-          c = 0;
-          ++r;
-        }
+    for (int k = 0; k < 4; ++k) {
+      if (at + k < total) v[j][k] *= load_in(scale + (row0 + r) * nb + c / MACE_CHECKPOINT_BLOCK);
+      if (++c == (uint32_t)C) {
+        c = 0;
+        ++r;
       }
     }
   }
 #pragma unroll
-  for (int j = 0; j < RS_UNROLL; ++j) {
-    const int64_t at = e0 + (threadIdx.x + j * RW_THREADS) * 4;
-    if (vec && at + 4 <= total) {
-      store4(x + at, v[j]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (at + k < total) x[at + k] = from_f32<T>(v[j][k]);
-    }
-  }
+  for (int j = 0; j < RS_UNROLL; ++j) store(j, v[j]);
 }
 
 // bits of one counting pass and passes for G + 1 keys
