@@ -424,10 +424,10 @@ int mace_ctx_error_flag(mace_ctx* ctx, int32_t* flag);
  * Species operators: the parts of the model whose parameters are indexed by an
  * atom's species (the node embedding, reference model.py:373-438, and the skip
  * tensor product, reference tensor_product.py:1046-1305), by themselves and
- * with their parameter gradients, for callers that train them.  No context:
- * the caller owns every buffer, workspaces included; nothing here allocates or
- * synchronises, so every call can be captured into a CUDA graph.  Calls use
- * the current device, which must own the pointers.
+ * with their parameter gradients, for callers that train parts of this form.
+ * No context: the caller owns every buffer, workspaces included; nothing here
+ * allocates or synchronises, so every call can be captured into a CUDA graph.
+ * Calls use the current device, which must own the pointers.
  * Addresses are multiples of their values' size (checked); a workspace aligned
  * to 32 bytes serves every entry.
  *

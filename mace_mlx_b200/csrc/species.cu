@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(EG_THREADS, 3) k_embed_grad_by_group(EmbedGrad
 // groups: zero.  A warp takes a group of few shares by itself; the CTA's 32
 // warps take the others together.  32 channels and per_cta groups per CTA and round (few groups: one each, so
 // that they are joined side by side).
-// (1M rows of 128 channels, 4 groups: 87 us, 157 with a warp to each; 89 groups 91 and 98)
+// (1M rows of 128 channels, 4 groups: 86 us, 157 with a warp to each; 89 groups 91 and 98)
 constexpr int EJ_ALONE = 16;
 
 template <typename T>
@@ -772,8 +772,8 @@ __global__ void __launch_bounds__(1024) k_embed_grad_join(EmbedGrad p, int per_c
   }
 }
 
-// scale = max |x| / 127 of a row's block, q = x / scale rounded to the nearest: one pass, bound by HBM (1.6M rows of
-// 128 fp32 channels 197 us, 5.2 TB/s; the issue slots are 75 % used, the IEEE quotients among them).
+// scale = max |x| fl(1 / 127) of a row's block, q = x / scale rounded to the nearest: one pass, bound by HBM and by its
+// instructions (1.6M rows of 128 fp32 channels 199 us, 5.2 TB/s, with the issue slots 75 % used; bf16 217 us).
 // A warp quantises CK_ROWS consecutive (row, block) items, all of their loads in flight; VEC: lane l holds
 // channels 4 l .. 4 l + 3 of the block (rows aligned to four channels), else
 // channels l, l + 32, l + 64, l + 96.

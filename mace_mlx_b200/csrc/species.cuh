@@ -169,15 +169,16 @@ struct Raw {
   }
 };
 
-// 8-bit value of x at scale s = max |x| / 127 (0 where s is 0, infinite or NaN): the IEEE quotient rounded to
+// 8-bit value of x at scale s = max |x| fl(1 / 127) (0 where s is 0, infinite or NaN): the IEEE quotient rounded to
 // the nearest, half to even; the clamp only acts where s is subnormal and the quotient may pass 127
 __device__ __forceinline__ int quantise8(float x, float s) {
   if (!(s > 0.f) || s > 3.4028234e38f) return 0;
   return (int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f);
 }
 
-// Four of them, one per byte.  x times the hardware's 1 / s (2^-23 relative) is within 2^-15 of the quotient, which
-// is at most 127 in magnitude, so it rounds to the same number unless it lies within 2^-14 of a tie; only then are the four divided.
+// Four of them, one per byte.  x times the hardware's 1 / s (2 units in the last place, 2^-22 relative) is within 3.8e-5
+// of the quotient, which is at most 127 in magnitude, so it rounds to the same number unless it lies within 6.2e-5 of a
+// tie; only then are the four divided.
 // Adding 1.5 2^23 rounds to a whole number, half to even, and leaves it in the low bits.
 __device__ __forceinline__ uint32_t quantise8x4(const float* x, float s) {
   const float inv = __fdividef(1.0f, s);

@@ -11,9 +11,9 @@
 // addition is 2^-24 of the sum, the result is rounded to 8 bits).  Roles of a CTA (16 warps, one CTA per SM):
 //   warps 0-3   rows of x;  warps 4-7  map: weights (kept while the tiles share them) and the MMAs, zero rows;
 //               weight gradient: rows of dy;  warps 8-15  epilogue (weight gradient: warp 8 issues the MMAs)
-// 600 000 rows 128 -> 128: map 57 us (5.4 TB/s; 47 is what HBM needs), weight gradient 47 to 52 (general kernel 135);
-// 300 007 rows 96 -> 96 in 89 groups 31 and 31 (17.6): 8 to 10 us of each are the start of the pipeline, weights and
-// the join, the rest copies and hand-over.  Waits are bounded as in species_linear.cu.
+// 600 000 rows 128 -> 128: map 58 us (5.3 TB/s; 47 is what HBM needs), weight gradient with the join 61 (general kernel
+// 135); 300 007 rows 96 -> 96 in 89 groups 32 and 36 (17.6): 8 to 14 us of each are the start of the pipeline, weights
+// and the join, the rest copies and hand-over.  Waits are bounded as in species_linear.cu.
 #pragma once
 
 namespace mace {

@@ -23,8 +23,8 @@
 //               images, kept while the tiles share them; warp 4 issues the MMAs
 //               (a 17th warp would cut every thread to 96 registers)
 //   warps 8-15  epilogue: TMEM -> fp32 registers -> memory
-// handing over through mbarriers only.  600 000 fp32 rows 128 -> 128 take 126 us
-// (4.9 TB/s; 94 is what HBM needs): no role is busy all the time, the hand-over
+// handing over through mbarriers only.  600 000 fp32 rows 128 -> 128 take 124 us
+// (5.0 TB/s; 94 is what HBM needs): no role is busy all the time, the hand-over
 // between them is what is left.  A tile's 128 rows by NT columns are what TMEM
 // holds twice beside two stages of A; K goes in steps of 64, what an
 // accumulator may take.  Every wait is bounded (about 2 s): one
@@ -539,7 +539,7 @@ __device__ __forceinline__ void fetch_vec(uint32_t dst, const char* data, const 
 
 // Rows of any alignment: the 16-byte pieces that contain the segment; mis[r]: where it starts in the first.  (Value by
 // value, as the weight gradient takes rows of 4-byte values, costs the four warps here more than the shifting: 600 000
-// fp32 rows 97 -> 61 164 us against 136.)  row: this lane's row.
+// fp32 rows 97 -> 61 164 us against 139.)  row: this lane's row.
 template <int PITCH>
 __device__ __forceinline__ void fetch_any(uint32_t dst, const char* data, const char* row, int at, int row_bytes,
                                           uint8_t* mis) {
@@ -575,7 +575,7 @@ __device__ __noinline__ void copy_out_any(const SlParams& p, uint32_t stage_addr
     const uint32_t o = mine ? node * p.out_n32 + m * p.out_m32 : NO_ROW;
     T* const to = static_cast<T*>(p.out) + c0 + lane;
     // (unrolled whole: the values of many rows are read before the first is stored.  600 000 bf16 rows of 97 -> 61,
-    // fwd: 103 us, by 8 rows 134; fp32 dx: 135, by 8 146)
+    // fwd: 102 us, by 8 rows 134; fp32 dx: 138, by 8 146)
 #pragma unroll
     for (int r = 0; r < 32; ++r) {
       const uint32_t ro = __shfl_sync(0xffffffffu, o, r);
@@ -1401,12 +1401,12 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   const bool vec = aligned_rows(p.a, n, d, es), direct = dtype == MACE_BF16 && vec && p.w_vec;
   const int sms = sm_count();
   const int64_t row_tiles = (n * d + 127) / 128;
-  // narrower column tiles while the row tiles leave SMs idle (3000 fp32 rows 128 -> 128: 11.1 us, 16.5 with tiles of
+  // narrower column tiles while the row tiles leave SMs idle (3000 fp32 rows 128 -> 128: 9.3 us, 12.6 with tiles of
   // 128 columns; bf16 no difference)
   int most = 128;
   while (most > 32 && row_tiles * ((M + most - 1) / most) * 2 <= sms) most /= 2;
   // and so narrow that the weight images of the whole K stay in shared memory (K <= 512), rather than being made
-  // anew for every tile (256 -> 256 fp32 channels, 300k rows: 646 us)
+  // anew for every tile (256 -> 256 fp32 channels, 300k rows: 326 us, 580 so)
   const int n_k = (K + SL_KC - 1) / SL_KC, pieces = dtype == MACE_F32 ? 3 : 1;
   if (!direct) {
     int fit = most;
@@ -1417,9 +1417,9 @@ extern "C" int mace_species_linear(int32_t dtype, const void* x, int64_t xn, int
   p.slots = image_slots(p.NT, pieces, &p.img);
   p.n_ct = (M + p.NT - 1) / p.NT;
   p.n_kt = 1;
-  // Making a group's images costs about as much as 1.5 row tiles.  40 000 fp32 rows of 4 species 128 -> 128 20.7 us
-  // without it, 17.4 with 1 to 6; 600 000 rows 130.8, 127.6 with 4, 126.3 with 6; 60 000 rows of 89 species 27.4, 24.5
-  // with 4, 26.2 with 6.  bf16 rows copied as they lie (direct): no difference.
+  // Making a group's images costs about as much as 1.5 row tiles.  40 000 fp32 rows of 4 species 128 -> 128 21.2 us
+  // without it, 18.5 with 4 or 6; 600 000 rows 128.5, 125.0 with 4, 124.6 with 6; 60 000 rows of 89 species 29.1, 26.5
+  // with 4, 27.4 with 6.  bf16 rows copied as they lie (direct): no difference.
   p.start = !direct && n_k <= p.slots ? 4 : 0;
   const int grid = (int)std::min<int64_t>(sms, (row_tiles + std::min<int64_t>(G, n)) * p.n_ct);
   if (direct) return launch_direct<false>(p, grid, s);

@@ -3,7 +3,8 @@
 // parts, and described there.
 //
 // A step is 64 rows: A = their 128 channels of x (a TMEM lane per channel), B = NT columns of dy.  600 000 fp32 rows
-// 128 x 128 take 133 us with the join (94 is what HBM needs; 8-bit x 116, of 59; 64 x 64 105, of 47): the schedulers
+// 128 x 128 take 131 us with the join (94 is what HBM needs; 8-bit x 121, of 59, with bf16 dy 121, of 36; 64 x 64 108,
+// of 47): the schedulers
 // issue in 70 % of the cycles, masks and permutes of the split keep their pipe busy in 64 %, HBM is at 4.7 TB/s.  With
 // four warps for each operand a step took as long as a warp needs from its rows in shared memory to their pieces in
 // the operand (147, 127 and 131 us), so each operand has two teams of four warps with 32 rows of every step each, and
@@ -114,7 +115,7 @@ __device__ __forceinline__ void tmem_st8u(uint32_t a, const uint32_t* v) {
 // h * 16 .. h * 16 + 15 of `rows` (zeros for a row that does not exist or past its end).  Aligned rows (VEC) come in
 // 16-byte pieces, other rows of 4-byte values value by value, and those of smaller ones as the 16-byte pieces that
 // contain the segment, mis[r] saying where it starts in the first.
-// (600 000 rows 97 x 61: fp32 156 us, 8-bit x 147; with the 4-byte values in pieces too 163 and 162.)
+// (600 000 rows 97 x 61: fp32 158 us, 8-bit x 151; with the 4-byte values in pieces too 163 and 162.)
 template <bool VEC>
 struct UnitRows {
   uint32_t mine, have;  // this lane's row in 16 bytes (aligned), which rows exist

@@ -1,6 +1,7 @@
 """Species operators: the parts of a MACE model whose parameters are indexed by
 an atom's species, by themselves and with their gradients, for programs that
-train them.
+train parts of this form (a head on a frozen model's features, a layer of their
+own).
 
 * ``group_species``               -- stable grouping of atoms (or edges) by species
 * ``species_embedding``           -- ``scale * table[species]`` (the node embedding)
