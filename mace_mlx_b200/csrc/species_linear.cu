@@ -636,7 +636,9 @@ __device__ __forceinline__ void copy_out(const SlParams& p, const uint8_t* stage
 // Infinities and NaN among split operands: a piece of an infinity is inf - inf, so whatever it enters is NaN, and an
 // infinite piece times a zero one is too: a whole row of results, or a column of them.  So a CTA that has met such a row,
 // or weights that are not finite, goes over its results once more when it is done, and makes those that are NaN from
-// the operands as they are, in fp32.  (A look at every result, or the call within the epilogue, cost 2 to 3 us of 125.)
+// the operands as they are, in fp32.  (A look at every result, or the call within the epilogue, cost 2 to 3 us of 125.
+// 600 000 rows 128 -> 128 with one infinity among them take 0.7 ms, all of them NaN 1.5, all infinite 13, with a NaN or
+// an infinity among the weights up to 11 and 39; the weight gradient up to 16, 0.4 and 24.)
 
 // Map: this CTA's tiles, each by the epilogue warps that stored it
 template <typename S>
@@ -679,8 +681,9 @@ __device__ __noinline__ void redo_map(const SlParams& p) {
       for (int c = c0 + lane; c < c1; c += 32) {
         if (y[c] == y[c]) continue;
         float sum = 0.f;
+        for (int k = 0; k < p.K && sum == sum;)
 #pragma unroll 8
-        for (int k = 0; k < p.K; ++k) sum = __fmaf_rn(x[k], wt[k * wk + c * wc], sum);
+          for (const int e = min(k + 32, p.K); k < e; ++k) sum = __fmaf_rn(x[k], wt[k * wk + c * wc], sum);
         y[c] = p.alpha * sum;
       }
     }

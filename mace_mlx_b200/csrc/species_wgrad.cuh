@@ -205,17 +205,17 @@ template <typename TA, typename T>
 __device__ __noinline__ void redo_wgrad(const SlParams& p, const Groups& q, int t0, int t1, int tile, int share, int k0,
                                         int n0, int quad) {
   constexpr int CB = 16;  // columns at a time
-  const int kl = quad * 32 + (threadIdx.x & 31), k = k0 + kl;
+  const int lane = threadIdx.x & 31, kl = quad * 32 + lane, k = k0 + kl;
   __syncwarp();
   Walk w;
   w.init(p, q, t0);
 #pragma unroll 1
   while (w.t < t1) {
-    const int begin = q.pre[w.g], end = min(q.pre[w.g + 1], t1), d = p.d;
+    const int begin = q.pre[w.g], end = min(q.pre[w.g + 1], t1);
     const bool whole = begin >= t0 && q.pre[w.g + 1] <= t1;
-    const int64_t first = (int64_t)q.lo[w.g] * d;
+    const int64_t first = (int64_t)q.lo[w.g] * p.d;
     const int a0 = (int)(first + (int64_t)(w.t - begin) * SL_KC);
-    const int a1 = (int)min(first + (int64_t)(end - begin) * SL_KC, (int64_t)q.hi[w.g] * d);
+    const int a1 = (int)min(first + (int64_t)(end - begin) * SL_KC, (int64_t)q.hi[w.g] * p.d);
     T* const out = static_cast<T*>(p.out) + ((int64_t)w.g * p.K + k) * p.N + n0;
     float* const part = p.part + ((((int64_t)tile * p.shares + share) * 2 + (begin > t0)) * 32 * p.NT + kl) * 4;
 #pragma unroll 1
@@ -232,19 +232,25 @@ __device__ __noinline__ void redo_wgrad(const SlParams& p, const Groups& q, int 
       float sum[CB] = {};
       unsigned open = left;  // those whose sum is not NaN yet
 #pragma unroll 1
-      for (int a = a0; a < a1 && __any_sync(0xffffffffu, open != 0); ++a) {
-        const int i = d > 1 ? (int)(__umulhi((uint32_t)a, p.div_mul) >> p.div_shift) : a, m = a - i * d;
-        const int64_t node = p.order[i];
-        if (node < 0 || node >= p.n) continue;
-        const T* const dy = reinterpret_cast<const T*>(p.b.data + node * p.b.sn + m * p.b.sm) + n0 + c;
-        float x = 0.f;
-        if (k < p.K) x = to_f32(reinterpret_cast<const TA*>(p.a.data + node * p.a.sn + m * p.a.sm)[k]);
-        if constexpr (sizeof(TA) == 1) x *= p.a_scale[(node * d + m) * p.ka_blocks + k0 / MACE_CHECKPOINT_BLOCK];
+      for (int a = a0; a < a1 && __any_sync(0xffffffffu, open != 0); a += 32) {
+        RowRef ref;  // lane r: row a + r
+        ref.load(p, a + lane, a1);
+        const int valid = ref.valid(p);
+#pragma unroll 2
+        for (int r = 0; r < 32; ++r) {
+          const int64_t node = __shfl_sync(0xffffffffu, ref.node, r), m = __shfl_sync(0xffffffffu, ref.m, r);
+          if (!__shfl_sync(0xffffffffu, valid, r)) continue;
+          const T* const dy = reinterpret_cast<const T*>(p.b.data + node * p.b.sn + m * p.b.sm) + n0 + c;
+          float x = 0.f;
+          if (k < p.K) x = to_f32(reinterpret_cast<const TA*>(p.a.data + node * p.a.sn + m * p.a.sm)[k]);
+          if constexpr (sizeof(TA) == 1) x *= p.a_scale[(node * p.d + m) * p.ka_blocks + k0 / MACE_CHECKPOINT_BLOCK];
 #pragma unroll
-        for (int j = 0; j < CB; ++j) {
-          if (n0 + c + j < p.N) sum[j] = __fmaf_rn(x, to_f32(dy[j]), sum[j]);
-          if (sum[j] != sum[j]) open &= ~(1u << j);
+          for (int j = 0; j < CB; ++j)
+            if (n0 + c + j < p.N) sum[j] = __fmaf_rn(x, to_f32(dy[j]), sum[j]);
         }
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+          if (sum[j] != sum[j]) open &= ~(1u << j);
       }
 #pragma unroll
       for (int j = 0; j < CB; ++j)
