@@ -403,8 +403,10 @@ class _EmbeddingFn(torch.autograd.Function):
     def forward(ctx, table, species, scale, groups):
         if groups is None:
             groups = group_species(species, table.shape[0])
-        elif groups.offsets.shape[0] != table.shape[0] + 1:
-            raise ValueError(f"the grouping has {groups.offsets.shape[0] - 1} elements, the table {table.shape[0]}")
+        else:
+            g, _, _ = _groups(groups, species.shape[0], table.get_device())
+            if g != table.shape[0]:
+                raise ValueError(f"the grouping has {g} elements, the table {table.shape[0]}")
         ctx.save_for_backward(groups.order, groups.offsets)
         ctx.scale = scale
         return _embedding(table, species, scale, None)

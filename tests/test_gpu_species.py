@@ -786,6 +786,17 @@ def test_refusals(sp):
     assert sp.error_flag() == 0
 
 
+def test_a_grouping_of_other_rows_is_refused_in_the_forward(sp):
+    z = torch.zeros(8, dtype=torch.int32, device="cuda")
+    table = torch.zeros(2, 4, device="cuda", requires_grad=True)
+    groups = sp.group_species(z, 2)
+    for bad in (sp.group_species(z[:5], 2), sp.group_species(z, 3), sp.SpeciesGroups(groups.order.cpu(), groups.offsets),
+                sp.SpeciesGroups(groups.order.long(), groups.offsets)):
+        with pytest.raises(ValueError):
+            sp.species_embedding(table, z, groups=bad)
+    assert sp.species_embedding(table, z, groups=groups).requires_grad
+
+
 @pytest.mark.parametrize("requires_grad", [False, True])
 def test_tangents_are_refused(sp, requires_grad):
     """A forward-mode tangent would be dropped: every entry that takes features refuses it."""
