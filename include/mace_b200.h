@@ -509,6 +509,63 @@ int mace_rows_restore(int32_t dtype, const int8_t* q, const float* scale, int64_
  * are incomplete). */
 int mace_species_error_flag(int32_t* flag);
 
+/*
+ * Normalisation operators of training: layer norm of feature rows (followed by
+ * SiLU in the radial MLPs of the non-linear interaction block, reference
+ * radial.py:344-357; the reference has no training path) with its gradients,
+ * and the norm and the clipping of a model's gradients.  As above: no context,
+ * the caller owns every buffer, nothing allocates or synchronises, and sums
+ * are kept in fp32 or wider and rounded once.
+ */
+#define MACE_ACT_NONE 0
+#define MACE_ACT_SILU 1
+#define MACE_LAYER_NORM_MAX_CHANNELS 8192
+
+/*
+ * y[i] = f(weight * (x[i] - mean) / sqrt(var + eps) + bias) for n rows of C
+ * channels (strides in elements; x rows may overlap or repeat, y rows must not,
+ * and y must not overlap x), f the identity or SiLU.  weight and bias hold
+ * param_dtype; NULL stands for ones and zeros.
+ */
+int mace_layer_norm(int32_t dtype, const void* x, int64_t x_stride, int32_t param_dtype, const void* weight,
+                    const void* bias, int64_t n, int32_t C, float eps, int32_t activation, void* y, int64_t y_stride,
+                    void* stream);
+
+/*
+ * Gradients of mace_layer_norm for the output gradient dy: dx (n rows of C),
+ * dweight and dbias (C values of param_dtype); any may be NULL (not wanted).
+ * The workspace serves dweight and dbias.  The order of their sums depends on
+ * n and C alone.
+ */
+int mace_layer_norm_grad_workspace(int64_t n, int32_t C, int64_t* bytes);
+int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride,
+                         int32_t param_dtype, const void* weight, const void* bias, int64_t n, int32_t C, float eps,
+                         int32_t activation, void* dx, int64_t dx_stride, void* dweight, void* dbias, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/*
+ * norm = the 2-norm of `count` tensors taken as one vector, in device memory.
+ * Tensor t is sizes[t] values of dtypes[t] at grads[t] (host arrays, read
+ * before the call returns, so a captured call keeps their contents).  Squares
+ * are summed in fp64, in an order that depends on the sizes, types and
+ * addresses modulo 16 alone.
+ */
+int mace_grad_norm_workspace(int32_t count, int64_t* bytes);
+int mace_grad_norm(int32_t count, const void* const* grads, const int64_t* sizes, const int32_t* dtypes, float* norm,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The same, and out[t] = grads[t] * min(1, max_norm / (norm + 1e-6)) as values
+ * of out_dtypes[t].  A tensor is clipped in place where out[t] is grads[t]
+ * (then the dtypes must agree), and left untouched where the factor is 1.
+ * Apart from that no output may overlap another tensor of the call (checked).
+ * A norm that is NaN makes every value NaN, an infinite one the finite values
+ * zero.  The workspace is that of mace_grad_norm.
+ */
+int mace_grad_clip(int32_t count, const void* const* grads, const int64_t* sizes, const int32_t* dtypes,
+                   void* const* out, const int32_t* out_dtypes, double max_norm, float* norm, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -135,6 +135,8 @@ EXPORTED = (
     "mace_species_embed_grad_workspace", "mace_species_embed_grad", "mace_species_linear",
     "mace_species_linear_wgrad_workspace", "mace_species_linear_wgrad", "mace_rows_checkpoint", "mace_rows_restore",
     "mace_species_error_flag",
+    "mace_layer_norm", "mace_layer_norm_grad_workspace", "mace_layer_norm_grad", "mace_grad_norm_workspace",
+    "mace_grad_norm", "mace_grad_clip",
 )
 NOALLOC_MAX_ATOMS = 131072
 NOALLOC_MAX_GRAPH_ATOMS = 16384
@@ -147,6 +149,11 @@ SPECIES_MAX_ROWS = 2147483136
 SPECIES_MAX_INDEX = 1048575
 SPECIES_MAX_CHANNELS = 32768
 CHECKPOINT_BLOCK = 128
+
+# normalisation operators
+ACT_NONE = 0
+ACT_SILU = 1
+LAYER_NORM_MAX_CHANNELS = 8192
 
 _lib = None
 
@@ -202,6 +209,13 @@ def load_library(path: str | Path | None = None) -> C.CDLL:
         "mace_rows_checkpoint": ([i32, vp, i64, i64, i64, i32, i32, vp, vp, vp], C.c_int),
         "mace_rows_restore": ([i32, vp, vp, i64, i32, i32, vp, vp], C.c_int),
         "mace_species_error_flag": ([C.POINTER(i32)], C.c_int),
+        "mace_layer_norm": ([i32, vp, i64, i32, vp, vp, i64, i32, f32, i32, vp, i64, vp], C.c_int),
+        "mace_layer_norm_grad_workspace": ([i64, i32, C.POINTER(i64)], C.c_int),
+        "mace_layer_norm_grad": ([i32, vp, i64, vp, i64, i32, vp, vp, i64, i32, f32, i32, vp, i64, vp, vp, vp, i64, vp],
+                                 C.c_int),
+        "mace_grad_norm_workspace": ([i32, C.POINTER(i64)], C.c_int),
+        "mace_grad_norm": ([i32, vp, vp, vp, vp, vp, i64, vp], C.c_int),
+        "mace_grad_clip": ([i32, vp, vp, vp, vp, vp, C.c_double, vp, vp, i64, vp], C.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

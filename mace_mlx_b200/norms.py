@@ -1,0 +1,293 @@
+"""Normalisation operators of training, beside the species operators, for
+programs that train parts of MACE's form on the GPU.
+
+* ``layer_norm``       -- layer norm of feature rows, with the SiLU that follows
+  it in the radial MLPs of the non-linear interaction block
+* ``layer_norm_grad``  -- its input and parameter gradients
+* ``grad_norm``        -- the 2-norm of a model's gradients taken as one vector
+* ``clip_grads``       -- the same, and the gradients scaled down to a largest norm
+
+``layer_norm`` takes part in autograd when an argument requires a gradient
+(once differentiable, in reverse mode: a tensor with a forward-mode tangent is
+refused).  It keeps x for its backward, and no statistics: the backward makes
+them again from x.
+
+Every call runs hand-written kernels of ``libmace_b200`` on the current stream
+of the tensors' device, allocates only its results and workspace through
+torch, and neither synchronises nor reads device values, so it can be captured
+into a CUDA graph.  Tensors last used on another stream need the caller's
+``wait_stream``/``record_stream``, as for torch's own operators.
+
+Reference: Linear -> LayerNorm -> SiLU stacks ``mace_mlx/radial.py:344-357``;
+the reference has no training path.
+"""
+
+from __future__ import annotations
+
+import math
+from array import array
+from collections.abc import Iterable, Sequence
+
+import torch
+from torch.autograd import forward_ad
+
+from . import native as nv
+from .species import _cuda, _dtype, _launch, _on, _workspace
+
+MAX_CHANNELS = nv.LAYER_NORM_MAX_CHANNELS
+_ACTIVATIONS = {None: nv.ACT_NONE, "silu": nv.ACT_SILU}
+
+__all__ = ["layer_norm", "layer_norm_grad", "grad_norm", "clip_grads"]
+
+
+# ---------------------------------------------------------------- layer norm
+def _rows(name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    """(rows, C, row stride) of (..., C) whose leading dimensions lie one row stride apart."""
+    shape = t.shape
+    if len(shape) != 2:
+        if not shape:
+            raise ValueError(f"{name} must be (..., C), got a scalar")
+        try:
+            t = t.view(math.prod(shape[:-1]), shape[-1])
+        except RuntimeError:
+            raise ValueError(f"{name}: rows must lie at one stride, got shape {tuple(shape)} with strides "
+                             f"{t.stride()}") from None
+    n, c = t.shape
+    if not 1 <= c <= MAX_CHANNELS or n >= 2**31:
+        raise ValueError(f"{name}: need 1..{MAX_CHANNELS} channels and fewer than 2**31 rows, got {tuple(shape)}")
+    sn, sc = t.stride()
+    if sc != 1 and c > 1:
+        raise ValueError(f"{name}: channels must be contiguous (stride 1), got strides {t.stride()}")
+    return n, c, sn
+
+
+def _params(weight, bias, dev: int, c: int, dtype: torch.dtype) -> tuple[int, int | None, int | None]:
+    """(type code, pointers of weight and bias): C contiguous values, both of x's type or both float32."""
+    kind = None
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        _on(name, t, dev)
+        if t.dim() != 1 or t.shape[0] != c or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous ({c},) tensor, got {tuple(t.shape)} with strides {t.stride()}")
+        if t.dtype != dtype and t.dtype != torch.float32:
+            raise ValueError(f"{name} is {t.dtype}, expected {dtype} or float32")
+        if kind is not None and t.dtype != kind:
+            raise ValueError(f"weight is {kind}, bias {t.dtype}: they must be of one type")
+        kind = t.dtype
+    return (_dtype("weight", dtype if kind is None else kind), None if weight is None else weight.data_ptr(),
+            None if bias is None else bias.data_ptr())
+
+
+def _activation(activation: str | None) -> int:
+    code = _ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"activation must be None or 'silu', got {activation!r}")
+    return code
+
+
+def _eps(eps: float) -> float:
+    if not 0.0 <= eps < 3e38:
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    return eps
+
+
+def _layer_norm(x, weight, bias, eps, activation, out):
+    dev = _cuda("x", x)
+    code = _dtype("x", x.dtype)
+    n, c, xs = _rows("x", x)
+    pcode, w, b = _params(weight, bias, dev, c, x.dtype)
+    act = _activation(activation)
+    if out is None:
+        y = x.new_empty(x.shape)
+        ys = c
+    else:
+        y = out
+        _on("out", y, dev)
+        if y.dtype != x.dtype or y.shape != x.shape:
+            raise ValueError(f"out must be {x.dtype} {tuple(x.shape)}, got {y.dtype} {tuple(y.shape)}")
+        _, _, ys = _rows("out", y)
+        if n > 1 and ys < c:
+            raise ValueError(f"out rows overlap (strides {y.stride()})")
+    _launch(dev, nv.load_library().mace_layer_norm, code, x.data_ptr(), xs, pcode, w, b, n, c, _eps(eps), act,
+            y.data_ptr(), ys)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+    return y
+
+
+def _layer_norm_grad(x, grad, weight, bias, eps, activation, want_x, want_w, want_b):
+    dev = _cuda("x", x)
+    code = _dtype("x", x.dtype)
+    n, c, xs = _rows("x", x)
+    _on("grad", grad, dev)
+    if grad.dtype != x.dtype or grad.shape != x.shape:
+        raise ValueError(f"grad must be {x.dtype} {tuple(x.shape)}, got {grad.dtype} {tuple(grad.shape)}")
+    _, _, gs = _rows("grad", grad)
+    pcode, w, b = _params(weight, bias, dev, c, x.dtype)
+    act = _activation(activation)
+    dx = x.new_empty(x.shape) if want_x else None
+    dw = torch.empty_like(weight) if want_w else None
+    db = torch.empty_like(bias) if want_b else None
+    ws, ptr, nbytes = None, None, 0
+    if want_w or want_b:
+        ws, ptr, nbytes = _workspace("mace_layer_norm_grad_workspace", dev, x, n, c)
+    _launch(dev, nv.load_library().mace_layer_norm_grad, code, x.data_ptr(), xs, grad.data_ptr(), gs, pcode, w, b, n, c,
+            _eps(eps), act, dx.data_ptr() if want_x else None, c, dw.data_ptr() if want_w else None,
+            db.data_ptr() if want_b else None, ptr, nbytes)
+    return dx, dw, db
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
+               eps: float = 1e-5, activation: str | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``f(weight * (x - mean) / sqrt(var + eps) + bias)`` over the last dimension, of up to 8192 channels.
+
+    ``activation`` is None (f the identity) or ``"silu"``.  x is float32 or
+    bfloat16, (..., C) with contiguous channels and rows at one stride, so a
+    slot of a node-feature table is passed in place; so may ``out``, which must
+    not overlap x.  weight and bias (C,), either or both, are of x's type or
+    float32; without them they are ones and zeros.
+
+    Statistics and products are fp32, rounded once to x's type.  Deviations
+    from the mean are squared in fp32: rows whose values pass 1e18 lose them.
+    """
+    grads = [t for t in (x, weight, bias) if isinstance(t, torch.Tensor) and t.requires_grad]
+    if grads and torch.is_grad_enabled():
+        if out is not None:
+            raise ValueError("out= cannot take part in autograd")
+        _cuda("x", x)
+        for name, t in (("weight", weight), ("bias", bias)):
+            if t is not None:
+                _cuda(name, t)
+        return _LayerNormFn.apply(x, weight, bias, eps, activation)
+    return _layer_norm(x, weight, bias, eps, activation, out)
+
+
+def layer_norm_grad(x: torch.Tensor, grad: torch.Tensor, weight: torch.Tensor | None = None,
+                    bias: torch.Tensor | None = None, *, eps: float = 1e-5, activation: str | None = None
+                    ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of ``layer_norm`` at x, weight and bias for the output gradient ``grad``.
+
+    Those of weight and bias have their type (None without them); their sums
+    over the rows are fp32, in an order that depends on the sizes alone, so
+    equal calls give equal bits.
+    """
+    return _layer_norm_grad(x, grad, weight, bias, eps, activation, True, weight is not None, bias is not None)
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, activation):
+        ctx.save_for_backward(x, weight, bias)
+        ctx.more = eps, activation
+        return _layer_norm(x, weight, bias, eps, activation, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias = ctx.saved_tensors
+        if grad.dim() != 2 or grad.stride(-1) != 1:  # sums hand back expanded gradients, others any order
+            grad = grad.contiguous()
+        return (*_layer_norm_grad(x, grad, weight, bias, *ctx.more, *ctx.needs_input_grad[:3]), None, None)
+
+
+# ----------------------------------------------------------- gradient norms
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the values fill their memory without gaps or repeats, in whatever order of the dimensions."""
+    if t.layout is not torch.strided:
+        return False
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int) -> tuple[array, array, array]:
+    """Pointers, sizes and type codes of dense tensors on device ``dev``."""
+    tangents = forward_ad._current_level >= 0
+    for i, t in enumerate(tensors):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}[{i}] must be a torch.Tensor, got {type(t).__name__}")
+        if not t.is_cuda or t.get_device() != dev or tangents:
+            _on(f"{name}[{i}]", t, dev)
+        if not _dense(t):
+            raise ValueError(f"{name}[{i}] has gaps or repeated values (strides {t.stride()}); use .contiguous()"
+                             if t.layout is torch.strided else f"{name}[{i}] is not strided, got {t.layout}")
+    try:
+        codes = array("i", [_CODES[t.dtype] for t in tensors])
+    except KeyError as e:
+        raise ValueError(f"{name} must be float32 or bfloat16, got {e.args[0]}") from None
+    return array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]), codes
+
+
+_CODES = {torch.float32: nv.DTYPE_F32, torch.bfloat16: nv.DTYPE_BF16}
+
+
+def _grads(grads: Iterable[torch.Tensor | None]) -> list[torch.Tensor]:
+    if isinstance(grads, torch.Tensor):
+        raise TypeError("grads must be a sequence of tensors, got one tensor")
+    return [g for g in grads if g is not None]
+
+
+def _grad_call(grads, dev, more):
+    ptrs, sizes, codes = _flat("grads", grads, dev)
+    norm = torch.empty((), dtype=torch.float32, device=torch.device("cuda", dev))
+    ws, wptr, nbytes = _workspace("mace_grad_norm_workspace", dev, norm, len(grads))
+    fn, extra = more
+    _launch(dev, fn, len(grads), ptrs.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], *extra,
+            norm.data_ptr(), wptr, nbytes)
+    return norm
+
+
+def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
+    """The 2-norm of all gradients taken as one vector: a float32 scalar on their device.
+
+    The gradients are float32 or bfloat16 (mixed as they come), on one device,
+    without gaps in their memory; entries that are None (parameters without a
+    gradient) are passed over.  Squares are summed in fp64.
+    """
+    grads = _grads(grads)
+    dev = _cuda("grads[0]", grads[0]) if grads else torch.cuda.current_device()
+    return _grad_call(grads, dev, (nv.load_library().mace_grad_norm, ()))
+
+
+def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
+               out: Sequence[torch.Tensor | None] | None = None) -> torch.Tensor:
+    """Scales the gradients by ``min(1, max_norm / (norm + 1e-6))``, in place, and returns their ``grad_norm``.
+
+    Gradients below the bound are left untouched, and nothing waits for the
+    norm on the host.  With ``out`` (a tensor for every gradient, of its shape
+    and order of dimensions, float32 or bfloat16) the results go there and the
+    gradients stay, unless ``out`` holds the gradient itself.  No tensor that
+    is written may overlap another one of the call, so none may be listed twice.
+
+    A norm that is NaN makes every gradient NaN; an infinite one makes the
+    finite values zero and the others NaN: test the norm where that can occur.
+    """
+    if isinstance(max_norm, torch.Tensor):
+        raise TypeError("max_norm must be a number: a tensor's value would be waited for")
+    max_norm = float(max_norm)
+    if not 0.0 <= max_norm < math.inf:
+        raise ValueError(f"max_norm must be finite and not negative, got {max_norm}")
+    every = list(grads) if not isinstance(grads, torch.Tensor) else grads
+    grads = _grads(every)
+    into = grads
+    if out is not None:
+        if len(out) != len(every):
+            raise ValueError(f"out has {len(out)} tensors, grads {len(every)}")
+        into = [o for o, g in zip(out, every) if g is not None]
+    dev = _cuda("grads[0]", grads[0]) if grads else torch.cuda.current_device()
+    ptrs, _, codes = _flat("out" if out is not None else "grads", into, dev)
+    if out is not None:
+        for i, (g, o) in enumerate(zip(grads, into)):
+            if o.shape != g.shape or o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
+                raise ValueError(f"out[{i}] must be {tuple(g.shape)} with strides {g.stride()}, got {tuple(o.shape)} with "
+                                 f"strides {o.stride()}")
+    norm = _grad_call(grads, dev, (nv.load_library().mace_grad_clip,
+                                   (ptrs.buffer_info()[0], codes.buffer_info()[0], max_norm)))
+    torch.autograd.graph.increment_version(into)
+    return norm

@@ -80,7 +80,7 @@ def _cuda(name: str, t: torch.Tensor) -> int:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path), got device {t.device}")
     if forward_ad._current_level >= 0 and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
-        raise ValueError(f"{name} carries a tangent: the species operators have no forward-mode derivative")
+        raise ValueError(f"{name} carries a tangent: there is no forward-mode derivative")
     return t.get_device()
 
 

@@ -1,0 +1,787 @@
+"""Normalisation operators on the GPU against their definitions in 64 bits.
+
+Bounds (u = 2^-24, the unit roundoff of fp32; every step's rounding carried
+through to first order, with whole numbers rounded up):
+
+* forward, with R = max |x - x[0]| of a row: x - x[0] rounds by u R, its mean
+  by 24 u R (8 values of a lane, then sums of at most 2^10 lanes), so a
+  deviation from the mean is off by D = 28 u R; the sum of its squares rounds
+  by 26 u, so rstd is off by D rstd + 18 u of itself and xhat by
+  E = D rstd (1 + |xhat|) + 19 u |xhat|.
+  z = w xhat + b is one fma: |w| E + u |z|.  SiLU has a slope below 1.1, and
+  its sigmoid is off by (12 + 2.4 |z|) u of itself (exp within 2 + 1.17 |z|
+  units, a sum, a quotient within 2 units, a product) or by 1e-36.
+* backward: the slope of SiLU, f' = s (1 + z (1 - s)), is off by half of z's
+  error (|f''| <= 1/2) and by (16 + 10 |z|) u; then dz, g = w dz, and the means of
+  g and g xhat (26 u of the mean magnitude) enter dx = rstd (g - c1 - xhat c2)
+  as they stand, with 4 u for its own three operations.
+* a sum over rows adds at most 256 rows a lane, then warps, then shares: its
+  rounding stays below (min(n, 512) + 16) u of the terms' magnitudes.
+* those errors are random, so over a whole result of unit-scale inputs the
+  relative error in the 2-norm also stays below 2^-19;
+* a bf16 result adds half a unit in its last place, at most 2^-8 of it.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+F32, BF16 = torch.float32, torch.bfloat16
+DTYPES = [F32, BF16]
+
+
+@pytest.fixture(scope="module")
+def nm():
+    from mace_mlx_b200 import norms
+
+    return norms
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(*shape, seed=0, dtype=F32):
+    return torch.randn(shape, generator=gen(seed), device="cuda").to(dtype)
+
+
+def inputs(n, c, dtype, param, seed=0):
+    """x with channels of their own scale and offset, dy, weight and bias."""
+    x = (randn(n, c, seed=seed) * (0.5 + randn(c, seed=seed + 1).abs()) + randn(c, seed=seed + 2)).to(dtype)
+    return (x, randn(n, c, seed=seed + 3, dtype=dtype), (1.0 + 0.3 * randn(c, seed=seed + 4)).to(param),
+            (0.3 * randn(c, seed=seed + 5)).to(param))
+
+
+class Rows64:
+    """The definition in 64 bits, and how far fp32 may be off."""
+
+    def __init__(self, x, weight, bias, eps, silu):
+        x = x.double()
+        x = x - x[:, :1]  # (the mean of equal large ones would round in 64 bits too)
+        self.n, self.c = x.shape
+        one = torch.ones(self.c, dtype=torch.float64, device=x.device)
+        self.w = one if weight is None else weight.double()
+        b = 0 * one if bias is None else bias.double()
+        mean = x.mean(1, keepdim=True)
+        eps = float(torch.tensor(eps, dtype=F32))  # the kernel gets it in fp32
+        self.rstd = 1.0 / torch.sqrt((x - mean).square().mean(1, keepdim=True) + eps)
+        self.xhat = (x - mean) * self.rstd
+        self.D = 28 * U * x.abs().amax(1, keepdim=True) * self.rstd
+        self.E = self.D * (1 + self.xhat.abs()) + 19 * U * self.xhat.abs()
+        self.z = self.w * self.xhat + b
+        self.E_z = self.w.abs() * self.E + U * self.z.abs()
+        self.silu = silu
+        self.sig = torch.sigmoid(self.z)
+
+    def forward(self):
+        if not self.silu:
+            return self.z, self.E_z
+        y = self.z * self.sig
+        return y, 1.1 * self.E_z + (12 + 2.4 * self.z.abs()) * U * y.abs() + 1e-36 * (1 + self.z.abs())
+
+    def backward(self, dy):
+        dz, E_dz = dy.double(), torch.zeros_like(self.z)
+        if self.silu:
+            slope = self.sig * (1 + self.z * (1 - self.sig))
+            E_dz = dz.abs() * (0.5 * self.E_z + (16 + 10 * self.z.abs()) * U)
+            dz = dz * slope
+            E_dz = E_dz + U * dz.abs()
+        depth = (min(self.n, 512) + 16) * U
+        dw, mass = (dz * self.xhat).sum(0), (dz * self.xhat).abs().sum(0)
+        E_dw = (E_dz * self.xhat.abs() + dz.abs() * self.E).sum(0) + depth * mass
+        db, E_db = dz.sum(0), E_dz.sum(0) + depth * dz.abs().sum(0)
+        g = dz * self.w
+        E_g = E_dz * self.w.abs() + U * g.abs()
+        c1, c2 = g.mean(1, keepdim=True), (g * self.xhat).mean(1, keepdim=True)
+        E_c1 = E_g.mean(1, keepdim=True) + 26 * U * g.abs().mean(1, keepdim=True)
+        E_c2 = ((E_g * self.xhat.abs() + g.abs() * self.E).mean(1, keepdim=True)
+                + 27 * U * (g * self.xhat).abs().mean(1, keepdim=True))
+        dx = self.rstd * (g - c1 - self.xhat * c2)
+        E_dx = self.rstd * (E_g + E_c1 + self.E * c2.abs() + self.xhat.abs() * E_c2
+                            + 4 * U * (g.abs() + c1.abs() + (self.xhat * c2).abs()))
+        return (dx, E_dx + dx.abs() * (self.D + 18 * U)), (dw, E_dw), (db, E_db)
+
+
+def assert_close(got, want, bound, what="", norm=True):
+    bound = bound * 1.01 + 1e-37
+    if got.dtype == BF16:
+        bound = bound * (1 + 2.0**-8) + 2.0**-8 * want.abs()
+    off = (got.double() - want).abs()
+    bad = ~(off <= bound)
+    assert not bad.any(), f"{what}: {int(bad.sum())} values off, worst {float(off.max()):.3e}, {float((off / bound).max()):.2f} of its bound"
+    if norm:
+        rel, size = float(off.norm()), float(want.norm())
+        assert rel <= (2.0**-19 if got.dtype == F32 else 2.0**-8 + 2.0**-19) * size, f"{what}: relative error {rel / size:.3e}"
+
+
+def check_rows(nm, x, dy, w, b, eps=1e-5, silu=False, norm=True):
+    act = "silu" if silu else None
+    ref = Rows64(x, w, b, eps, silu)
+    y = nm.layer_norm(x, w, b, eps=eps, activation=act)
+    assert y.dtype == x.dtype and y.shape == x.shape
+    assert_close(y, *ref.forward(), "y", norm)
+    got = nm.layer_norm_grad(x, dy, w, b, eps=eps, activation=act)
+    for name, value, (want, bound), like in zip(("dx", "dw", "db"), got, ref.backward(dy), (x, w, b)):
+        if like is None:
+            assert value is None
+            continue
+        assert value.dtype == like.dtype and value.shape == like.shape
+        assert_close(value, want, bound, name, norm)
+
+
+# ----------------------------------------------------------------- layer norm
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("dtype,param", [(F32, F32), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("n,c", [(1, 1), (5, 1), (3, 2), (40, 3), (1, 8), (70, 16), (33, 31), (1000, 32), (129, 33),
+                                 (4097, 64), (1, 64), (300, 61), (1003, 97), (500, 96), (1, 128), (777, 128), (64, 130),
+                                 (100, 250), (31, 255), (1000, 256), (65, 257), (50, 264), (20, 511), (200, 512),
+                                 (7, 1000), (33, 2048), (3, 4097), (2, 8191), (5, 8192)])  # fmt: skip
+def test_layer_norm_and_its_gradients(nm, n, c, dtype, param, silu):
+    x, dy, w, b = inputs(n, c, dtype, param, seed=n + c)
+    # (two or three channels leave dx as the small difference of large terms, one none at all)
+    check_rows(nm, x, dy, w, b, silu=silu, norm=c >= 8)
+
+
+@pytest.mark.parametrize("n", [200_003, 1_500_001])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layer_norm_of_many_rows(nm, n, dtype):
+    x, dy, w, b = inputs(n, 64, dtype, F32, seed=1)
+    check_rows(nm, x, dy, w, b, silu=True)
+
+
+def test_sums_of_one_sign_over_many_rows(nm):
+    n, c = 3_000_001, 40
+    x, _, w, b = inputs(n, c, F32, F32, seed=2)
+    dy = randn(n, c, seed=3).abs_() + 0.5
+    check_rows(nm, x, dy, w, b)
+
+
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("c", [64, 97, 700])
+def test_layer_norm_without_parameters(nm, c, silu):
+    x, dy, w, b = inputs(100, c, F32, F32, seed=4)
+    for weight, bias in ((None, None), (w, None), (None, b)):
+        check_rows(nm, x, dy, weight, bias, silu=silu)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c,pitch,at", [(64, 192, 64), (64, 65, 0), (64, 72, 3), (97, 200, 5), (128, 512, 128),
+                                        (512, 1030, 1), (2048, 2052, 4), (300, 300, 0)])
+def test_rows_in_a_wider_table(nm, dtype, c, pitch, at):
+    n = 111
+    x, dy, w, b = inputs(n, pitch, dtype, F32, seed=5)
+    table, grads = x.clone(), dy.clone()
+    x, dy, w, b = x[:, at:at + c], dy[:, at:at + c], w[at:at + c].clone(), b[at:at + c].clone()
+    check_rows(nm, x, dy, w, b, silu=True)
+    node = torch.full((n + 2, pitch), 7.0, dtype=dtype, device="cuda")
+    out = node[1:n + 1, at:at + c]
+    got = nm.layer_norm(x, w, b, activation="silu", out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert_close(out, *Rows64(x, w, b, 1e-5, True).forward(), "out")
+    assert (node[0] == 7.0).all() and (node[n + 1:] == 7.0).all()
+    assert (node[:, :at] == 7.0).all() and (node[:, at + c:] == 7.0).all()
+    if pitch >= 2 * c + at:  # a table's slot into another slot of the same table
+        into = table[:, at + c:at + 2 * c]
+        before = table.clone()
+        nm.layer_norm(table[:, at:at + c], w, b, activation="silu", out=into)
+        assert torch.equal(into, out)
+        before[:, at + c:at + 2 * c] = into
+        assert torch.equal(table, before)
+    assert torch.equal(grads[:, at:at + c], dy)
+
+
+def test_repeated_rows_and_other_shapes(nm):
+    c = 64
+    x, dy, w, b = inputs(1, c, F32, F32, seed=6)
+    many = x.expand(50, c)
+    assert torch.equal(nm.layer_norm(many, w, b), nm.layer_norm(x, w, b).expand(50, c))
+    dx, dw, db = nm.layer_norm_grad(many, dy.expand(50, c), w, b)
+    one = nm.layer_norm_grad(x, dy, w, b)
+    assert torch.equal(dx, one[0].expand(50, c))
+    ref = Rows64(many, w, b, 1e-5, False).backward(dy.expand(50, c))
+    assert_close(dw, *ref[1])
+    assert_close(db, *ref[2])
+    x, dy, w, b = inputs(24, c, F32, F32, seed=7)
+    want, grads = nm.layer_norm(x, w, b), nm.layer_norm_grad(x, dy, w, b)
+    for shape in ((2, 3, 4, c), (24, 1, c), (1, 24, c)):
+        assert torch.equal(nm.layer_norm(x.view(shape), w, b), want.view(shape))
+        got = nm.layer_norm_grad(x.view(shape), dy.view(shape), w, b)
+        assert torch.equal(got[0], grads[0].view(shape)) and torch.equal(got[1], grads[1])
+    assert torch.equal(nm.layer_norm(x[0], w, b), want[0])  # one row without leading dimensions
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(0, 64), (0, 97), (0, 2048), (3, 0, 64)])
+def test_no_rows(nm, dtype, shape):
+    x, w = torch.zeros(shape, dtype=dtype, device="cuda"), torch.ones(shape[-1], device="cuda")
+    assert nm.layer_norm(x, w, w).shape == shape
+    dx, dw, db = nm.layer_norm_grad(x, x, w, w, activation="silu")
+    assert dx.shape == shape and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("c", [8, 64, 97, 300, 2048])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_equal_and_offset_rows(nm, dtype, c):
+    """A row of equal values is b (or its SiLU) exactly, whatever the value; an offset common to a row changes nothing
+    but what it rounds in x itself."""
+    _, dy, w, b = inputs(6, c, dtype, dtype, seed=8)
+    value = torch.tensor([0.0, 1.0, -3.7, 1e6 + 3, 1e-20, -2e17], device="cuda")
+    x = value[:, None].expand(6, c).to(dtype).contiguous()
+    assert torch.equal(nm.layer_norm(x, w, b), b.expand(6, c))
+    check_rows(nm, x, dy, w, b, norm=False)
+    x = (randn(6, c, seed=9) + torch.tensor([0.0, 10, 1e3, 1e4, -1e5, 3e5], device="cuda")[:, None]).to(dtype)
+    check_rows(nm, x, dy, w, b, silu=True, norm=False)
+    if dtype == F32:
+        # the bound holds for the spread of a row, which no offset enters: as accurate as without it
+        for eps in (1e-5, 0.0):
+            check_rows(nm, x, dy, w, b, eps=eps, norm=True)
+
+
+def test_scales_from_1e_minus_15_to_1e15(nm):
+    x, dy, w, b = inputs(31, 64, F32, F32, seed=10)
+    for scale in (1e-15, 1e-6, 1e6, 1e15):
+        check_rows(nm, x * scale, dy, w, b, eps=0.0)
+        check_rows(nm, x * scale, dy * scale, w, b, eps=1e-5, norm=False)
+
+
+@pytest.mark.parametrize("c", [31, 64, 97, 256, 520])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_are_not_finite_stay_by_themselves(nm, dtype, c):
+    n = 45
+    x, dy, w, b = inputs(n, c, dtype, F32, seed=11)
+    want = nm.layer_norm(x, w, b, activation="silu"), nm.layer_norm_grad(x, dy, w, b, activation="silu")[0]
+    bad = [3, 17, 18, 44]
+    x[3, 0], x[17, c - 1], x[18, c // 2], x[44] = float("nan"), float("inf"), -float("inf"), float("inf")
+    good = torch.ones(n, dtype=torch.bool, device="cuda")
+    good[bad] = False
+    y = nm.layer_norm(x, w, b, activation="silu")
+    dx, dw, db = nm.layer_norm_grad(x, dy, w, b, activation="silu")
+    for got, expected in zip((y, dx), want):
+        assert torch.equal(got[good], expected[good])
+        assert got[~good].isnan().all()
+    assert dw.isnan().all() and db.isnan().all()
+    # rows behind the last of a warp's are no rows: eps 0 leaves no trace of them
+    x, dy, w, b = inputs(5, c, dtype, F32, seed=12)
+    assert all(t.isfinite().all() for t in nm.layer_norm_grad(x, dy, w, b, eps=0.0, activation="silu"))
+
+
+def test_large_pre_activations(nm):
+    """SiLU far from zero: neither exp(-z) nor its reciprocal spoils the result."""
+    x, dy, w, b = inputs(50, 64, F32, F32, seed=13)
+    b = torch.linspace(-200, 200, 64, device="cuda")
+    check_rows(nm, x, dy, w, b, silu=True)
+    check_rows(nm, x, dy, 30 * w, b, silu=True)
+
+
+def test_offsets_past_32_bits(nm):
+    n, c = 33_600_011, 64  # 2.15e9 values of 2 bytes
+    x = torch.empty(n, c, dtype=BF16, device="cuda").normal_(generator=gen(14))
+    dy = torch.empty(n, c, dtype=BF16, device="cuda").normal_(generator=gen(15))
+    w, b = 1 + 0.1 * randn(c, seed=16), randn(c, seed=17)
+    y = nm.layer_norm(x, w, b, activation="silu")
+    for at in (0, n // 2, 2**25 - 7, n - 1001):
+        assert torch.equal(y[at:at + 1001], nm.layer_norm(x[at:at + 1001], w, b, activation="silu"))
+    del y
+    dx, dw, db = nm.layer_norm_grad(x, dy, w, b, activation="silu")
+    for at in (0, n // 2, 2**25 - 7, n - 1001):
+        want = nm.layer_norm_grad(x[at:at + 1001], dy[at:at + 1001], w, b, activation="silu")[0]
+        assert torch.equal(dx[at:at + 1001], want)
+    del dx
+    sums = torch.zeros(2, c, dtype=torch.float64, device="cuda")
+    bound = torch.zeros_like(sums)
+    for xs, ds in zip(x.split(2_000_000), dy.split(2_000_000)):
+        _, (pw, ew), (pb, eb) = Rows64(xs, w, b, 1e-5, True).backward(ds)
+        sums += torch.stack([pw, pb])
+        bound += torch.stack([ew, eb])
+    assert_close(dw, sums[0], bound[0], "dw", norm=False)
+    assert_close(db, sums[1], bound[1], "db", norm=False)
+
+
+@pytest.mark.parametrize("c", [1, 2, 13, 64, 300])
+def test_gradients_against_differences(nm, c):
+    """The gradients' product with a step is the definition's change along it, in 64 bits."""
+    n = 9
+    x, dy, w, b = inputs(n, c, F32, F32, seed=18)
+    dx, dw, db = (t.double() for t in nm.layer_norm_grad(x, dy, w, b, activation="silu", eps=1e-2))
+    step = [randn(*t.shape, seed=19 + i).double() for i, t in enumerate((x, w, b))]
+
+    def loss(h):
+        moved = [t.double() + h * s for t, s in zip((x, w, b), step)]
+        eps = float(torch.tensor(1e-2))
+        return float((Rows64(*moved, eps, True).forward()[0] * dy.double()).sum())
+
+    def slope(h):  # central differences, error of the order h^4
+        return (8 * (loss(h) - loss(-h)) - (loss(2 * h) - loss(-2 * h))) / (12 * h)
+
+    want = slope(1e-3)
+    dot = float((dx * step[0]).sum() + (dw * step[1]).sum() + (db * step[2]).sum())
+    ref = Rows64(x, w, b, 1e-2, True).backward(dy)
+    bound = sum(float((e * s.abs()).sum()) for (_, e), s in zip(ref, step)) + 10 * abs(want - slope(2e-3)) + 1e-9
+    assert abs(dot - want) <= bound, (dot, want, bound)
+    assert bound < 0.05 * abs(want) or c == 1
+
+
+# ------------------------------------------------------------------- autograd
+@pytest.mark.parametrize("dtype,param", [(F32, F32), (BF16, F32)])
+def test_autograd(nm, dtype, param):
+    n, c = 300, 96
+    x, dy, w, b = inputs(n, c, dtype, param, seed=20)
+    want = nm.layer_norm_grad(x, dy, w, b, activation="silu")
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = nm.layer_norm(*leaves, activation="silu")
+    assert torch.equal(y.detach(), nm.layer_norm(x, w, b, activation="silu"))
+    y.backward(dy)
+    assert all(torch.equal(t.grad, g) for t, g in zip(leaves, want))
+    for frozen in range(3):  # what needs no gradient gets none, the others the same bits
+        leaves = [t.clone().requires_grad_(i != frozen) for i, t in enumerate((x, w, b))]
+        nm.layer_norm(*leaves, activation="silu").backward(dy)
+        for i, (t, g) in enumerate(zip(leaves, want)):
+            assert t.grad is None if i == frozen else torch.equal(t.grad, g)
+    only = x.clone().requires_grad_()
+    nm.layer_norm(only).backward(dy)
+    assert torch.equal(only.grad, nm.layer_norm_grad(x, dy)[0])
+    with torch.no_grad():
+        assert not nm.layer_norm(leaves[0], leaves[1]).requires_grad
+
+
+def test_autograd_of_expanded_and_permuted_gradients(nm):
+    n, c = 200, 33
+    x, _, w, b = inputs(n, c, F32, F32, seed=21)
+    x, w, b = x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+    nm.layer_norm(x, w, b).sum().backward()
+    want = nm.layer_norm_grad(x.detach(), torch.ones(n, c, device="cuda"), w.detach(), b.detach())
+    assert all(torch.equal(t.grad, g) for t, g in zip((x, w, b), want))
+    x.grad = w.grad = b.grad = None
+    v = randn(c, n, seed=22)
+    (nm.layer_norm(x, w, b).T * v).sum().backward()
+    want = nm.layer_norm_grad(x.detach(), v.T.contiguous(), w.detach(), b.detach())
+    assert all(torch.equal(t.grad, g) for t, g in zip((x, w, b), want))
+    x.grad = w.grad = b.grad = None
+    # parameters shared by two uses add up
+    (nm.layer_norm(x, w, b) + nm.layer_norm(x, w, b)).sum().backward()
+    once = nm.layer_norm_grad(x.detach(), torch.ones(n, c, device="cuda"), w.detach(), b.detach())
+    assert all(torch.equal(t.grad, g + g) for t, g in zip((x, w, b), once))
+    # a slot of a table, several leading dimensions
+    table = randn(6, 7, 3 * c, seed=23).requires_grad_()
+    dy = randn(6, 7, c, seed=24)
+    nm.layer_norm(table[..., c:2 * c], w, b).backward(dy)
+    want = nm.layer_norm_grad(table.detach()[..., c:2 * c], dy, w.detach(), b.detach())[0]
+    assert torch.equal(table.grad[..., c:2 * c], want) and not table.grad[..., :c].any()
+
+
+def test_second_derivatives_are_refused(nm):
+    x = randn(4, 8, seed=25).requires_grad_()
+    (g,) = torch.autograd.grad(nm.layer_norm(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_a_changed_input_is_noticed(nm):
+    x = randn(4, 8, seed=26).requires_grad_()
+    h = x * 1.0
+    y = nm.layer_norm(h)
+    with torch.no_grad():
+        nm.layer_norm(randn(4, 8, seed=27), out=h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+# ------------------------------------------------------------- gradient norms
+def lists_of_gradients():
+    return {
+        "one": [(1,)], "scalar": [()], "empty among others": [(0,), (5, 3), (0, 7)], "odd": [(1,), (7, 3), (129,), (33, 5)],
+        "around a tile": [(4095,), (4096,), (4097,), (8191,), (8192,), (8193,)], "many small": [(3,)] * 300,
+        "large": [(1000, 1001), (17,), (3_000_001,)], "65": [(10,)] * 65, "257": [(64, 9)] * 257,
+        "thousands": [(1 + i % 50,) for i in range(2500)],
+    }  # fmt: skip
+
+
+def norm64(grads):
+    return torch.cat([g.double().flatten() for g in grads]).norm()
+
+
+def assert_norm(got, grads):
+    assert got.dtype == F32 and got.shape == ()
+    want = norm64(grads)
+    # the fp64 sum is off by far less than fp32's half unit
+    assert abs(got.double() - want) <= U * (1 + 2.0**-10) * want + 2.0**-150
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, "mixed"])
+@pytest.mark.parametrize("name", list(lists_of_gradients()))
+def test_gradient_norm(nm, name, dtype):
+    grads = [randn(*s, seed=i, dtype=(F32, BF16)[i % 2] if dtype == "mixed" else dtype)
+             for i, s in enumerate(lists_of_gradients()[name])]
+    before = [g.clone() for g in grads]
+    got = nm.grad_norm(grads)
+    assert_norm(got, grads)
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    assert torch.equal(nm.grad_norm([None, *grads, None]), got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_norm_of_every_alignment(nm, dtype):
+    flat = randn(20_000, seed=30, dtype=dtype)
+    for at in range(9):
+        for size in (1, 2, 7, 8, 9, 15, 16, 17, 4090, 4096, 4100, 8200):
+            assert_norm(nm.grad_norm([flat[at:at + size]]), [flat[at:at + size]])
+
+
+def test_gradient_norm_of_extreme_values(nm):
+    for scale in (1e-40, 1e-30, 1e-20, 1e10, 1e25, 1e35):
+        grads = [randn(1000, seed=31).clamp(-3, 3) * scale, torch.zeros(5, device="cuda")]
+        assert_norm(nm.grad_norm(grads), grads)
+    assert float(nm.grad_norm([torch.zeros(10, device="cuda")])) == 0.0
+    assert float(nm.grad_norm([])) == 0.0 and float(nm.grad_norm([None])) == 0.0
+    assert float(nm.grad_norm([torch.zeros(0, device="cuda")])) == 0.0
+    big = torch.full((4,), 3e38, device="cuda")  # the norm itself lies past fp32
+    assert float(nm.grad_norm([big])) == float("inf")
+    for value in (float("inf"), -float("inf"), float("nan")):
+        grads = [randn(100, seed=32), randn(5000, seed=33)]
+        grads[1][4321] = value
+        got = float(nm.grad_norm(grads))
+        assert got != got if value != value else got == float("inf")
+
+
+def test_gradient_norm_in_any_order_of_dimensions(nm):
+    g = randn(30, 7, 11, seed=34)
+    for t in (g.permute(2, 0, 1), g.transpose(0, 2), g[:, :, :, None], g[5:20]):
+        assert_norm(nm.grad_norm([t]), [t])
+
+
+def test_gradient_norm_past_32_bits(nm):
+    g = torch.empty(2**31 + 12345, dtype=BF16, device="cuda").normal_(generator=gen(35))
+    want = sum(float(part.double().square().sum()) for part in g.split(2**28)) ** 0.5
+    assert abs(float(nm.grad_norm([g, g[:1]])) - (want**2 + float(g[0]) ** 2) ** 0.5) <= 2 * U * want
+    guard = g[-1].clone()
+    nm.clip_grads([g[:-1]], want / 2)
+    assert g[-1] == guard
+    after = sum(float(part.double().square().sum()) for part in g[:-1].split(2**28)) ** 0.5
+    assert abs(after - want / 2) <= 2.0**-8 * want
+
+
+def clipped64(grads, max_norm):
+    norm = norm64(grads)
+    return [g.double() * torch.clamp(max_norm / (norm + 1e-6), max=1.0) for g in grads]
+
+
+def assert_clipped(got, want):
+    for a, b in zip(got, want, strict=True):
+        # the factor rounds once, the product once, a 16-bit result once more
+        bound = 2.01 * U * b.abs() + 2.0**-150 + (2.0**-8 * b.abs() if a.dtype == BF16 else 0.0)
+        assert not ((a.double() - b).abs() > bound).any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, "mixed"])
+@pytest.mark.parametrize("name", list(lists_of_gradients()))
+def test_clipping_in_place(nm, name, dtype):
+    grads = [randn(*s, seed=i, dtype=(F32, BF16)[i % 2] if dtype == "mixed" else dtype)
+             for i, s in enumerate(lists_of_gradients()[name])]
+    norm = norm64(grads)
+    before = [g.clone() for g in grads]
+    got = nm.clip_grads(grads, float(norm) * 1.5)
+    assert_norm(got, before)
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    got = nm.clip_grads([None, *grads], float(norm) * 0.3)
+    assert_norm(got, before)
+    assert_clipped(grads, clipped64(before, float(norm) * 0.3))
+
+
+@pytest.mark.parametrize("ins", DTYPES)
+@pytest.mark.parametrize("outs", DTYPES)
+def test_clipping_into_other_tensors(nm, ins, outs):
+    shapes = [(1,), (7, 3), (0,), (4097,), (64, 64), (8193,), (100_003,)]
+    sizes = [torch.Size(s).numel() for s in shapes]
+    for shift in range(9):  # outputs one behind the other, at every address relative to the inputs'
+        grads = [randn(*s, seed=i, dtype=ins) for i, s in enumerate(shapes)]
+        before = [g.clone() for g in grads]
+        buffer = torch.full((shift + sum(sizes) + 3,), 7.0, dtype=outs, device="cuda")
+        out = [part.view(s) for part, s in zip(buffer[shift:shift + sum(sizes)].split(sizes), shapes)]
+        for factor in (0.5, 2.0):
+            max_norm = float(norm64(grads)) * factor
+            assert_norm(nm.clip_grads([None, *grads], max_norm, out=[None, *out]), grads)
+            assert_clipped(out, clipped64(grads, max_norm))
+            if factor == 2.0:
+                assert all(torch.equal(o, g.to(outs)) for o, g in zip(out, grads))
+        assert all(torch.equal(a, b) for a, b in zip(grads, before))
+        assert (buffer[:shift] == 7.0).all() and (buffer[-3:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_clipping_packed_gradients(nm, dtype):
+    """Gradients one behind the other in one buffer, each at any address: the gaps keep their values."""
+    sizes = [5, 1, 4096, 33, 2, 8191, 16, 3, 1000]
+    flat = randn(sum(sizes) + 9 * len(sizes), seed=40, dtype=dtype)
+    at, grads, kept = 0, [], torch.ones(len(flat), dtype=torch.bool, device="cuda")
+    for i, size in enumerate(sizes):
+        grads.append(flat[at:at + size])
+        kept[at:at + size] = False
+        at += size + i % 3
+    before = flat.clone()
+    want = clipped64([g.clone() for g in grads], 3.0)
+    nm.clip_grads(grads, 3.0)
+    assert_clipped(grads, want)
+    assert torch.equal(flat[kept], before[kept])
+
+
+def test_clipping_of_some_in_place_and_some_elsewhere(nm):
+    a, b, c = randn(100, seed=41), randn(40, 50, seed=42).T, randn(77, seed=43, dtype=BF16)
+    into = [a, torch.empty_like(b), torch.empty(77, device="cuda")]
+    assert into[1].stride() == b.stride()
+    want = clipped64([a, b, c], 5.0)
+    nm.clip_grads([a, b, c], 5.0, out=into)
+    assert_clipped(into, want)
+    again = clipped64([a, b, c], 1e9)
+    nm.clip_grads([a, b, c], 1e9, out=into)
+    assert_clipped(into, again)
+
+
+def test_clipping_to_zero_and_of_infinities(nm):
+    g = randn(5000, seed=44)
+    nm.clip_grads([g], 0.0)
+    assert not g.any()
+    nm.clip_grads([g], 0.0)  # a zero norm: 0 / 1e-6
+    assert not g.any()
+    assert float(nm.clip_grads([], 1.0)) == 0.0 and float(nm.clip_grads([None], 1.0, out=[None])) == 0.0
+    g = randn(5000, seed=45)
+    g[17] = float("inf")
+    assert float(nm.clip_grads([g], 1.0)) == float("inf")
+    assert g[17].isnan() and not g[:17].any() and not g[18:].any()
+    g = randn(5000, seed=46)
+    g[17] = float("nan")
+    nm.clip_grads([g], 1.0)
+    assert g.isnan().all()
+
+
+def test_clipping_counts_as_a_change(nm):
+    g = randn(10, seed=47)
+    version = g._version
+    nm.grad_norm([g])
+    assert g._version == version
+    nm.clip_grads([g], 1.0)
+    assert g._version > version
+
+
+# ------------------------------------------------------------ streams, graphs
+def everything(nm, x, dy, w, b, grads, out):
+    y = nm.layer_norm(x, w, b, activation="silu")
+    more = nm.layer_norm_grad(x, dy, w, b, activation="silu")
+    wide = nm.layer_norm_grad(x.view(-1, x.numel() // 4), dy.view(-1, x.numel() // 4))[0]
+    return [y, *more, wide, nm.grad_norm([*grads, more[1]]), nm.clip_grads([*grads, more[2]], 2.0, out=out), *out]
+
+
+def step_inputs(seed):
+    x, dy, w, b = inputs(64, 96, F32, F32, seed=seed)
+    grads = [randn(5000, seed=seed + 7), randn(33, 3, seed=seed + 8, dtype=BF16)]
+    return x, dy, w, b, grads
+
+
+def outputs():
+    return [torch.empty(5000, device="cuda"), torch.empty(33, 3, device="cuda"), torch.empty(96, device="cuda")]
+
+
+def test_other_streams_and_cuda_graphs(nm):
+    x, dy, w, b, grads = step_inputs(50)
+    want = [t.clone() for t in everything(nm, x, dy, w, b, grads, outputs())]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = everything(nm, x, dy, w, b, grads, outputs())
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    graphs, results = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        out = outputs()
+        with torch.cuda.graph(graph):
+            results.append(everything(nm, x, dy, w, b, grads, out))
+    for factor in (2.0, 0.01):  # (clipped, and below the bound)
+        x.mul_(factor)
+        dy.mul_(factor)
+        for g in grads:
+            g.mul_(factor)
+        want = everything(nm, x, dy, w, b, grads, outputs())
+        for graph, got in zip(graphs, results):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_in_place_clipping_in_a_graph(nm):
+    source, g = randn(100_000, seed=60), torch.zeros(100_000, device="cuda")
+    nm.clip_grads([g], 1.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g.copy_(source)
+        norm = nm.clip_grads([g], 10.0)
+    for factor in (1.0, 1e-3, 50.0):
+        source.copy_(randn(100_000, seed=61) * factor)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert_norm(norm, [source])
+        assert_clipped([g], clipped64([source], 10.0))
+
+
+def test_training_step_in_a_graph(nm):
+    """Forward, backward and clipping captured as one step, replayed on new inputs."""
+    n, c = 500, 64
+    x, _, w, b = inputs(n, c, F32, F32, seed=62)
+    leaves = [t.clone().requires_grad_() for t in (w, b)]
+    target = randn(n, c, seed=63)
+
+    def step():
+        loss = (nm.layer_norm(x, *leaves, activation="silu") - target).square().sum()
+        got = torch.autograd.grad(loss, leaves)
+        return [*got, nm.clip_grads(got, 1.0)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    x.copy_(randn(n, c, seed=64))
+    graph.replay()
+    want = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, d) for a, d in zip(got, want))
+
+
+def test_calls_from_two_host_threads(nm):
+    import threading
+
+    data = {seed: step_inputs(seed) for seed in (70, 80)}
+    want = {seed: [t.clone() for t in everything(nm, *d, outputs())] for seed, d in data.items()}
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def thread(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[seed] = everything(nm, *data[seed], outputs())
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=thread, args=(seed,)) for seed in data]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for seed, values in want.items():
+        assert all(torch.equal(a, b) for a, b in zip(got[seed], values, strict=True))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_calls_in_a_row_on_buffers_used_again(nm, dtype):
+    """Each call reads what the call before it has just written to memory that earlier calls had read."""
+    n, c = 3000, 64
+    sources = [inputs(n, c, dtype, F32, seed=90 + 10 * k) for k in range(6)]
+
+    def chain(k, x, rows, again):
+        source, dy, w, b = sources[k]
+        x.copy_(source)
+        nm.layer_norm(x, w, b, activation="silu", out=rows)
+        nm.layer_norm(rows, w, b, out=again)
+        grads = nm.layer_norm_grad(rows, again, w, b, activation="silu")
+        norm = nm.clip_grads(list(grads), 1.0)
+        return [rows.clone(), again.clone(), *grads, norm]
+
+    def buffers():
+        return [torch.empty(n, c, dtype=dtype, device="cuda") for _ in range(3)]
+
+    want = []
+    for k in range(6):
+        want.append(chain(k, *buffers()))
+        torch.cuda.synchronize()
+    shared = buffers()
+    for _ in range(10):
+        got = [chain(k, *shared) for k in range(6)]
+        for a, b in zip(sum(got, []), sum(want, []), strict=True):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype,n,c", [(F32, 30_011, 64), (BF16, 30_011, 97), (F32, 3001, 2048), (F32, 777, 129)])
+def test_equal_calls_give_equal_bits(nm, dtype, n, c):
+    x, dy, w, b = inputs(n, c, dtype, F32, seed=100)
+    first = [nm.layer_norm(x, w, b), *nm.layer_norm_grad(x, dy, w, b), nm.grad_norm([x, dy, w])]
+    for _ in range(5):
+        again = [nm.layer_norm(x, w, b), *nm.layer_norm_grad(x, dy, w, b), nm.grad_norm([x, dy, w])]
+        assert all(torch.equal(p, q) for p, q in zip(first, again))
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals(nm):
+    x, w, b = torch.zeros(8, 16, device="cuda"), torch.ones(16, device="cuda"), torch.zeros(16, device="cuda")
+    leaf = torch.zeros(8, 16, device="cuda", requires_grad=True)
+    g, h = torch.zeros(40, device="cuda"), torch.zeros(40, device="cuda")
+    bad = [
+        lambda: nm.layer_norm(x.half(), w, b), lambda: nm.layer_norm(x.double()), lambda: nm.layer_norm(x.T, b[:8]),
+        lambda: nm.layer_norm(x[:, ::2], w[:8]), lambda: nm.layer_norm(x, w[:8]), lambda: nm.layer_norm(x, w, b[:8]),
+        lambda: nm.layer_norm(x, w[None]), lambda: nm.layer_norm(x, w.cpu(), b), lambda: nm.layer_norm(x, w, b.cpu()),
+        lambda: nm.layer_norm(x, w.bfloat16()), lambda: nm.layer_norm(x.bfloat16(), w.bfloat16(), b),
+        lambda: nm.layer_norm(x, torch.ones(32, device="cuda")[::2]), lambda: nm.layer_norm(x, w.double()),
+        lambda: nm.layer_norm(x, w, b, eps=-1.0), lambda: nm.layer_norm(x, w, b, eps=float("nan")),
+        lambda: nm.layer_norm(x, w, b, eps=float("inf")), lambda: nm.layer_norm(x, activation="relu"),
+        lambda: nm.layer_norm(x, out=torch.zeros(7, 16, device="cuda")), lambda: nm.layer_norm(x, out=x.bfloat16()),
+        lambda: nm.layer_norm(x, out=torch.zeros(16, device="cuda").expand(8, 16)),
+        lambda: nm.layer_norm(x, out=torch.zeros(8, 16)), lambda: nm.layer_norm(leaf, out=torch.zeros_like(x)),
+        lambda: nm.layer_norm(torch.zeros((), device="cuda")), lambda: nm.layer_norm(torch.zeros(4, 0, device="cuda")),
+        lambda: nm.layer_norm(torch.zeros(2, 8193, device="cuda")),
+        lambda: nm.layer_norm(torch.zeros(4, 6, 16, device="cuda")[:, :5]),  # no one stride between the rows
+        lambda: nm.layer_norm_grad(x, x[:4]), lambda: nm.layer_norm_grad(x, x.bfloat16()),
+        lambda: nm.layer_norm_grad(x, torch.ones(1, device="cuda").expand(8, 16)), lambda: nm.layer_norm_grad(x, x.cpu()),
+        lambda: nm.layer_norm_grad(x, x, w[:4]), lambda: nm.layer_norm_grad(x, x, activation="gelu"),
+        lambda: nm.grad_norm([g.half()]), lambda: nm.grad_norm([g.double()]), lambda: nm.grad_norm([g, g.cpu()]),
+        lambda: nm.grad_norm([g[::2]]), lambda: nm.grad_norm([g[:1].expand(5)]), lambda: nm.grad_norm([g.to_sparse()]),
+        lambda: nm.grad_norm([x[:, :8]]), lambda: nm.grad_norm([g.int()]),
+        lambda: nm.clip_grads([g], -1.0), lambda: nm.clip_grads([g], float("inf")),
+        lambda: nm.clip_grads([g], 1.0, out=[]), lambda: nm.clip_grads([g], 1.0, out=[h[:39]]),
+        lambda: nm.clip_grads([g], 1.0, out=[h.half()]), lambda: nm.clip_grads([g], 1.0, out=[h.cpu()]),
+        lambda: nm.clip_grads([x], 1.0, out=[torch.zeros(16, 8, device="cuda").T]),
+        lambda: nm.clip_grads([x[:, :8]], 1.0), lambda: nm.clip_grads([g, h], 1.0, out=[h[:40], None][:1]),
+    ]  # fmt: skip
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was accepted")
+    from mace_mlx_b200.native import NativeError
+
+    for call in (lambda: nm.clip_grads([g, g], 1.0), lambda: nm.clip_grads([g, g[3:7]], 1.0),
+                 lambda: nm.clip_grads([g, h], 1.0, out=[h, torch.zeros_like(h)]),
+                 lambda: nm.clip_grads([g[:39]], 1.0, out=[g[1:]]),
+                 lambda: nm.clip_grads([g, h], 1.0, out=[torch.zeros(40, device="cuda")] * 2)):
+        with pytest.raises(NativeError, match="overlaps"):
+            call()
+    for call in (lambda: nm.layer_norm([1.0]), lambda: nm.grad_norm([1.0]), lambda: nm.grad_norm(g),
+                 lambda: nm.clip_grads([g], 1.0, out=[None]), lambda: nm.clip_grads([g], torch.ones((), device="cuda"))):
+        with pytest.raises(TypeError):
+            call()
+    nm.grad_norm([g, g])  # only read: twice is twice
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_tangents_are_refused(nm, requires_grad):
+    from torch.autograd import forward_ad
+
+    plain = {"x": torch.zeros(8, 16, device="cuda"), "w": torch.ones(16, device="cuda")}
+    with forward_ad.dual_level():
+        dual = {k: forward_ad.make_dual(v.clone().requires_grad_(requires_grad), torch.ones_like(v))
+                for k, v in plain.items()}
+        for i, call in enumerate((
+            lambda: nm.layer_norm(dual["x"], plain["w"]), lambda: nm.layer_norm(plain["x"], dual["w"]),
+            lambda: nm.layer_norm(plain["x"], plain["w"], dual["w"]), lambda: nm.layer_norm_grad(dual["x"], plain["x"]),
+            lambda: nm.layer_norm_grad(plain["x"], dual["x"]), lambda: nm.layer_norm_grad(plain["x"], plain["x"], dual["w"]),
+            lambda: nm.grad_norm([plain["x"], dual["w"]]), lambda: nm.clip_grads([dual["w"]], 1.0),
+        )):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+                pytest.fail(f"call {i} was accepted")
+        nm.layer_norm(plain["x"], plain["w"])  # without a tangent: as ever
+        nm.grad_norm([plain["w"]])

@@ -1,0 +1,138 @@
+"""Normalisation operators without a GPU: refusals of the Python entry points and of
+the C ABI (host-side argument checks only, no launch)."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+import mace_mlx_b200
+from mace_mlx_b200 import native as nv
+from mace_mlx_b200 import norms
+
+
+def test_operators_are_public():
+    for name in norms.__all__:
+        assert hasattr(norms, name)
+    assert mace_mlx_b200.norms is norms
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros(4, 8), torch.ones(8)
+    for call in (lambda: norms.layer_norm(x, w, w), lambda: norms.layer_norm(x.requires_grad_(), w),
+                 lambda: norms.layer_norm_grad(x, x, w, w), lambda: norms.grad_norm([x]),
+                 lambda: norms.clip_grads([x, w], 1.0), lambda: norms.clip_grads([None, x], 1.0, out=[None, x])):
+        with pytest.raises(ValueError, match="no CPU path"):
+            call()
+
+
+def test_bounds_of_the_norm_are_checked_first():
+    for bad in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="max_norm"):
+            norms.clip_grads([torch.zeros(2)], bad)
+    with pytest.raises(TypeError, match="max_norm"):
+        norms.clip_grads([torch.zeros(2)], torch.ones(()))
+    for call in (lambda: norms.grad_norm(torch.zeros(2)), lambda: norms.clip_grads(torch.zeros(2), 1.0),
+                 lambda: norms.grad_norm([1.0])):
+        with pytest.raises(TypeError):
+            call()
+
+
+@pytest.mark.parametrize("t,dense", [
+    (torch.zeros(3, 4), True), (torch.zeros(3, 4).T, True), (torch.zeros(2, 3, 4).permute(1, 2, 0), True),
+    (torch.zeros(3, 4)[:, :2], False), (torch.zeros(3, 4)[:2], True), (torch.zeros(3, 4)[::2], False),
+    (torch.zeros(1).expand(5), False), (torch.zeros(4, 1).expand(4, 3), False), (torch.zeros(0, 4), True),
+    (torch.zeros(()), True), (torch.zeros(3, 1, 4)[:, :, :1], False), (torch.zeros(5, 2)[:, 0], False),
+    (torch.zeros(1, 9)[:, ::2][:, :1], True), (torch.zeros(3, 4).to_sparse(), False),
+])  # fmt: skip
+def test_dense_tensors_are_told_apart(t, dense):
+    assert norms._dense(t) == dense
+
+
+def test_c_entries_check_their_arguments():
+    lib = nv.load_library()
+    one, odd = C.c_void_p(32), C.c_void_p(33)  # never dereferenced: every call below is refused on the host
+
+    def refused(f, args, changes, match=""):
+        for at, value in changes:
+            call = list(args)
+            call[at] = value
+            assert f(*call) == nv.MACE_ERR_BAD_ARG and match in nv.last_error(lib), (f, at, value)
+
+    rows = (0, one, 8, 0, one, one, 4, 8, 1e-5, 0, one, 8, None)
+    refused(lib.mace_layer_norm, rows, [
+        (0, 2), (1, None), (2, -1), (3, 2), (6, -1), (6, 2**31), (7, 0), (7, nv.LAYER_NORM_MAX_CHANNELS + 1), (8, -1.0),
+        (8, float("inf")), (8, float("nan")), (9, 2), (9, -1), (10, None), (11, 7)])
+    refused(lib.mace_layer_norm, rows, [(1, odd), (4, odd), (5, odd), (10, odd)], "values' size")
+    assert lib.mace_layer_norm(0, None, 8, 0, None, None, 0, 8, 1e-5, 0, None, 8, None) == nv.MACE_OK  # no rows
+
+    need = C.c_int64(-1)
+    assert lib.mace_layer_norm_grad_workspace(1000, 128, C.byref(need)) == nv.MACE_OK and need.value > 0
+    for args in ((-1, 8), (2**31, 8), (1, 0), (1, nv.LAYER_NORM_MAX_CHANNELS + 1)):
+        assert lib.mace_layer_norm_grad_workspace(*args, C.byref(need)) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_layer_norm_grad_workspace(1, 8, None) == nv.MACE_ERR_BAD_ARG
+    grad = (0, one, 8, one, 8, 0, one, one, 4, 8, 1e-5, 0, one, 8, one, one, one, 1 << 20, None)
+    refused(lib.mace_layer_norm_grad, grad, [(0, 7), (1, None), (2, -1), (3, None), (4, -1), (5, 7), (8, -1), (9, 0),
+                                             (10, -1.0), (11, 5), (13, 7)])
+    refused(lib.mace_layer_norm_grad, grad, [(k, odd) for k in (1, 3, 6, 7, 12, 14, 15)], "values' size")
+    refused(lib.mace_layer_norm_grad, grad, [(16, None), (16, C.c_void_p(40)), (17, 3)], "workspace")
+
+
+def test_c_entries_check_lists_of_tensors():
+    lib = nv.load_library()
+    need = C.c_int64(-1)
+    assert lib.mace_grad_norm_workspace(0, C.byref(need)) == nv.MACE_OK and need.value == 0
+    assert lib.mace_grad_norm_workspace(5000, C.byref(need)) == nv.MACE_OK and need.value > 0
+    assert lib.mace_grad_norm_workspace(-1, C.byref(need)) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_grad_norm_workspace(1, None) == nv.MACE_ERR_BAD_ARG
+    one = C.c_void_p(4096)
+
+    def call(ptrs, sizes, types, out=None, out_types=None, max_norm=1.0, norm=one, ws=one, nbytes=1 << 20):
+        n = len(ptrs)
+        a = ((C.c_void_p * n)(*ptrs), (C.c_int64 * n)(*sizes), (C.c_int32 * n)(*types))
+        if out is None:
+            rc = lib.mace_grad_norm(n, *a, norm, ws, nbytes, None)
+        else:
+            rc = lib.mace_grad_clip(n, *a, (C.c_void_p * n)(*out), (C.c_int32 * n)(*(out_types or types)), max_norm, norm,
+                                    ws, nbytes, None)
+        return rc, nv.last_error(lib)
+
+    bad = [
+        call([64], [-1], [0]), call([64], [8], [2]), call([None], [8], [0]), call([66], [8], [0]), call([65], [8], [1]),
+        call([64], [8], [0], norm=None), call([64], [8], [0], ws=None), call([64], [8], [0], nbytes=8),
+        call([64], [8], [0], ws=C.c_void_p(4)), call([64], [2**41], [0]),
+        call([64], [8], [0], out=[64], max_norm=-1.0), call([64], [8], [0], out=[64], max_norm=float("inf")),
+        call([64], [8], [0], out=[64], max_norm=float("nan")), call([64], [8], [0], out=[None]),
+        call([64], [8], [0], out=[64], out_types=[1]), call([64], [8], [0], out=[63], out_types=[1]),
+    ]
+    assert [rc for rc, _ in bad] == [nv.MACE_ERR_BAD_ARG] * len(bad)
+    # outputs over other tensors: one listed twice, a later one inside an earlier, an output that begins in its own
+    # input, or reaches into another's input or output
+    overlaps = [
+        call([64, 64], [8, 8], [0, 0], out=[64, 64]), call([64, 80], [8, 2], [0, 0], out=[64, 80]),
+        call([64], [8], [0], out=[68]), call([64], [8], [0], out=[92]),
+        call([64, 256], [8, 8], [0, 0], out=[252, 512]), call([64, 256], [8, 8], [0, 0], out=[512, 528]),
+        call([64, 256], [8, 8], [1, 1], out=[1024, 1040], out_types=[0, 1]),
+        call([4096, 64, 256], [100, 4, 4], [0, 0, 0], out=[4096, 4492, 256]),
+    ]
+    for rc, text in overlaps:
+        assert rc == nv.MACE_ERR_BAD_ARG and "overlaps" in text
+
+
+def test_kernels_read_their_inputs_by_plain_loads():
+    """As the species operators' kernels: one may start while the kernel before it still writes its inputs."""
+    from pathlib import Path
+
+    for name in ("layer_norm.cu", "grad_norm.cu"):
+        text = (Path(mace_mlx_b200.__file__).parent / "csrc" / name).read_text()
+        for form in ("__ldg(", "global.nc", "__restrict__"):
+            assert form not in text, (name, form)
+
+
+def test_workspace_follows_the_shares_of_the_rows():
+    """At most a row of sums (2 C values in whole 16 bytes) for every 256 rows of a CTA, or for each CTA of a full GPU."""
+    lib, need = nv.load_library(), C.c_int64()
+    for n, c in ((0, 64), (1, 1), (1000, 128), (50_000_000, 64), (2**31 - 1, 8), (20_000, 2048), (5, 8192), (10**6, 8192)):
+        assert lib.mace_layer_norm_grad_workspace(n, c, C.byref(need)) == nv.MACE_OK
+        pitch = (2 * c + 3) // 4 * 16
+        assert need.value % pitch == 0 and need.value // pitch <= min(n, n // 256 + 148 * 32)
