@@ -21,7 +21,8 @@ namespace {
 constexpr int GN_THREADS = 256;
 constexpr int GN_UNROLL = 4;                         // pieces of a thread and tile (loads in flight)
 constexpr int GN_TILE = GN_THREADS * GN_UNROLL;      // pieces
-constexpr int GN_CTAS = 148 * 8;                     // of a launch, at most
+constexpr int GN_PER_SM = 6;                         // CTAs
+constexpr int GN_CTAS = 148 * GN_PER_SM;             // of a launch, at most
 constexpr int GN_MAX_TENSORS = 1024;                 // of a launch: kernel parameters hold 32 764 bytes
 
 constexpr uint8_t IN_BF16 = 1, OUT_BF16 = 2, OUT_PIECES = 4;  // OUT_PIECES: a piece's results are aligned to their size
@@ -116,7 +117,7 @@ __device__ __forceinline__ Run run_of(uint32_t tiles) {
 }
 
 template <int CAP>
-__global__ void __launch_bounds__(GN_THREADS) k_grad_squares(const __grid_constant__ GradList<CAP> list, double* part) {
+__global__ void __launch_bounds__(GN_THREADS, GN_PER_SM) k_grad_squares(const __grid_constant__ GradList<CAP> list, double* part) {
   __shared__ double sums[GN_THREADS / 32];
   pdl_wait();
   const Run run = run_of(list.first[list.count]);
@@ -180,7 +181,7 @@ __device__ __forceinline__ void clip_tile(const void* in, void* out, int64_t siz
 
 // A CTA goes through its run from the end: what the sums read last is still in L2.
 template <int CAP>
-__global__ void __launch_bounds__(GN_THREADS) k_grad_clip(const __grid_constant__ GradList<CAP> list, const double* part,
+__global__ void __launch_bounds__(GN_THREADS, GN_PER_SM) k_grad_clip(const __grid_constant__ GradList<CAP> list, const double* part,
                                                           int parts, double max_norm, float* norm) {
   __shared__ double sums[GN_THREADS / 32];
   pdl_wait();

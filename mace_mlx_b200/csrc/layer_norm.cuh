@@ -1,0 +1,394 @@
+// Rows of the layer norm in registers (layer_norm.cu, layer_norm_grad.cu): how a row is spread over its lanes, and the
+// arithmetic on a lane's 8 values, two at a time (the packed fp32 instructions of sm_100).
+#pragma once
+
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+
+#include "common.cuh"
+#include "species.cuh"
+
+namespace mace {
+
+constexpr int LN_THREADS = 256;  // of a CTA whose rows have up to 32 lanes
+constexpr int LN_VALUES = 8;     // of a lane
+constexpr int LN_SMS = 148;
+constexpr int LN_TURN = 8;       // rows that many apart begin at the same address modulo 16
+
+struct LayerNorm {
+  const void* x;
+  int64_t xs;
+  const void* dy;
+  int64_t ds;
+  const void* w;
+  const void* b;
+  int param_f32;
+  int64_t n;
+  int C;
+  float eps, inv_C;
+  uint32_t inner;  // rows [LN_TURN, LN_TURN + inner) have LN_TURN neighbours on either side
+  void* y;  // forward: the result; backward: dx, or null
+  int64_t ys;
+  // backward: rows of a CTA, and its sums: (shares, pitch) with dw in columns [0, C), db behind them; null: not wanted
+  int64_t share, shares;
+  float* part;
+  int pitch;
+  void* dw;
+  void* db;
+};
+
+// How a row's channels reach its lanes, 8 each:
+//   FULL    16-byte pieces, every row starts with one, and the lanes take exactly C channels
+//   PIECES  16-byte pieces at 16-byte addresses, wherever the row starts: its first and last piece may hold values of
+//           its neighbours, which are masked.  A row's start modulo 16 repeats every LN_TURN rows, so lanes that step
+//           by that many rows keep their channels.  More channels than a piece has.
+//   APART   single values, neighbouring lanes neighbouring channels: rows that start differently modulo 16 in two
+//           operands, or that are no longer than a piece
+enum Layout { FULL, PIECES, APART };
+
+// ---- two fp32 values at a time
+__device__ __forceinline__ uint64_t pack2(float2 a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t r) {
+  float2 a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+  return a;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+  return unpack2(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+  return unpack2(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)), "l"(pack2(c)));
+  return unpack2(r);
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+// A lane's channels: value j is channel at(j), and in the row where 0 <= at(j) < C.
+template <typename T, Layout LAYOUT>
+struct Lane {
+  static constexpr int V = LAYOUT == APART ? 1 : 16 / sizeof(T), K = LN_VALUES / V;
+  // values of a lane that are none of the row's come as zeros (PIECES: cut off the words as they lie in memory), and
+  // what is subtracted from the row's values is multiplied by `on` (1 or 0) for them
+  static constexpr int WORDS = LAYOUT == PIECES ? LN_VALUES * sizeof(T) / 4 : 1;
+  int first[K];             // channel of a piece's first value
+  int count[K];             // channels of the row in a piece
+  uint32_t keep[WORDS];
+  float2 on[LAYOUT == FULL ? 1 : LN_VALUES / 2];
+  // head: values between a 16-byte address and the row's start
+  __device__ __forceinline__ Lane(int lane, int lanes, int C, int head) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      first[k] = (k * lanes + lane) * V - head;
+      count[k] = LAYOUT == FULL ? V : max(0, min(first[k] + V, C) - max(first[k], 0));
+    }
+    if constexpr (LAYOUT != FULL) {
+#pragma unroll
+      for (int i = 0; i < LN_VALUES / 2; ++i)
+        on[i] = make_float2(in(2 * i, C) ? 1.f : 0.f, in(2 * i + 1, C) ? 1.f : 0.f);
+    }
+    if constexpr (LAYOUT == PIECES) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i)
+        keep[i] = sizeof(T) == 4 ? (in(i, C) ? 0xffffffffu : 0u)
+                                 : (in(2 * i, C) ? 0xffffu : 0u) | (in(2 * i + 1, C) ? 0xffff0000u : 0u);
+    }
+  }
+  __device__ __forceinline__ int at(int j) const { return first[j / V] + j % V; }
+  __device__ __forceinline__ bool in(int j, int C) const { return LAYOUT == FULL || (at(j) >= 0 && at(j) < C); }
+  __device__ __forceinline__ bool whole(int k) const { return LAYOUT == FULL || count[k] == V; }
+  __device__ __forceinline__ bool any(int k) const { return LAYOUT == FULL || count[k] > 0; }
+
+  __device__ __forceinline__ void param(const void* p, int f32, float missing, int C, float2* v) const {
+    float t[LN_VALUES];
+#pragma unroll
+    for (int j = 0; j < LN_VALUES; ++j) {
+      t[j] = 0.f;
+      if (in(j, C))
+        t[j] = !p ? missing
+                  : (f32 ? load_in(static_cast<const float*>(p) + at(j)) : to_f32(load_in(static_cast<const bf16*>(p) + at(j))));
+    }
+#pragma unroll
+    for (int i = 0; i < LN_VALUES / 2; ++i) v[i] = make_float2(t[2 * i], t[2 * i + 1]);
+  }
+};
+
+// the first (from: LAST) or last `m` values of a 16-byte piece at dst, 0 < m < 16 / size: a store for each power of two
+// in m, each aligned to its size
+template <int SIZE>
+__device__ __forceinline__ void store_some(char* dst, const uint32_t* w, int m, bool last) {
+  const int bytes = m * SIZE;
+  char* at = last ? dst + 16 - bytes : dst;
+  // from the piece's end inwards, or from its start
+  if (bytes & 8) *reinterpret_cast<uint2*>(last ? dst + 8 : dst) = last ? make_uint2(w[2], w[3]) : make_uint2(w[0], w[1]);
+  const bool far = bytes & 8;
+  if (bytes & 4)
+    *reinterpret_cast<uint32_t*>(last ? dst + (far ? 4 : 12) : dst + (far ? 8 : 0)) = last ? (far ? w[1] : w[3]) : (far ? w[2] : w[0]);
+  if constexpr (SIZE == 2)
+    if (bytes & 2) {
+      // word of the odd value: the one that holds the first (last) value kept
+      const int i = last ? (16 - bytes) / 4 : (bytes - 2) / 4;
+      const uint32_t u = i == 0 ? w[0] : (i == 1 ? w[1] : (i == 2 ? w[2] : w[3]));
+      *reinterpret_cast<uint16_t*>(last ? at : dst + bytes - 2) = (uint16_t)(last ? u >> 16 : u);
+    }
+}
+
+// A lane's part of a row as it lies in memory.
+template <typename T, Layout LAYOUT>
+struct Part {
+  using At = Lane<T, LAYOUT>;
+  static constexpr int V = At::V, K = At::K;
+  Raw<T, V> raw[K];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int k = 0; k < K; ++k) raw[k].zero();
+  }
+  // (what is not of the row stays as it was, or is a neighbour's); inner: no first or last row, whose pieces could
+  // reach out of the tensor
+  __device__ __forceinline__ void load(const At& at, const T* row, bool inner) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const T* const src = row + at.first[k];
+      if constexpr (LAYOUT == PIECES) {
+        if (at.any(k)) {
+          if (inner || at.whole(k)) {
+            raw[k].load(src);
+          } else {
+            T t[V];
+            const int from = at.first[k] < 0 ? V - at.count[k] : 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[i] = i >= from && i < from + at.count[k] ? load_in(src + i) : from_f32<T>(0.f);
+            raw[k].piece = *reinterpret_cast<const uint4*>(t);
+          }
+        }
+      } else {
+        if (at.any(k)) raw[k].load(src);
+      }
+    }
+  }
+  __device__ __forceinline__ void values(const At& at, float2* v) const {
+    float t[LN_VALUES];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      Raw<T, V> r = raw[k];
+      if constexpr (LAYOUT == PIECES) {
+        r.piece.x &= at.keep[4 * k];
+        r.piece.y &= at.keep[4 * k + 1];
+        r.piece.z &= at.keep[4 * k + 2];
+        r.piece.w &= at.keep[4 * k + 3];
+      }
+      r.values(t + k * V);
+    }
+#pragma unroll
+    for (int i = 0; i < LN_VALUES / 2; ++i) v[i] = make_float2(t[2 * i], t[2 * i + 1]);
+  }
+  static __device__ __forceinline__ void store(const At& at, T* row, const float2* v) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      T* const dst = row + at.first[k];
+      if constexpr (LAYOUT == APART) {
+        if (at.any(k)) *dst = from_f32<T>(k & 1 ? v[k / 2].y : v[k / 2].x);
+      } else {
+        uint32_t w[4];
+        if constexpr (sizeof(T) == 4) {
+          w[0] = __float_as_uint(v[2 * k].x), w[1] = __float_as_uint(v[2 * k].y);
+          w[2] = __float_as_uint(v[2 * k + 1].x), w[3] = __float_as_uint(v[2 * k + 1].y);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __float22bfloat162_rn(v[i]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+        if (at.whole(k))
+          *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if (at.any(k))
+          store_some<sizeof(T)>(reinterpret_cast<char*>(dst), w, at.count[k], at.first[k] < 0);
+      }
+    }
+  }
+};
+
+// ---- sums over the L neighbouring lanes of a row, or over all threads of a CTA
+template <int L>
+struct LaneSum {
+  __device__ __forceinline__ float operator()(float a) const {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    return a;
+  }
+  __device__ __forceinline__ float2 operator()(float2 a) const { return make_float2((*this)(a.x), (*this)(a.y)); }
+};
+template <int WARPS>
+struct CtaSum {
+  static constexpr int FLOATS = 4 * WARPS;
+  // Two of WARPS for single sums, in turn, and one for pairs: a thread writes to one of them again only behind another
+  // barrier, which all pass when they have read it (pairs are never summed twice without single sums between).
+  float* buffer;
+  int at = 0;
+  // (zeros for the warps that the CTA has not)
+  __device__ __forceinline__ explicit CtaSum(float* b) : buffer(b) {
+    for (int k = threadIdx.x; k < FLOATS; k += blockDim.x) b[k] = 0.f;
+    __syncthreads();
+  }
+  __device__ __forceinline__ float2 operator()(float2 a) {
+    a = LaneSum<32>()(a);
+    float2* const b = reinterpret_cast<float2*>(buffer + 2 * WARPS);
+    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = a;
+    __syncthreads();
+    const float4 t = total(reinterpret_cast<const float*>(b), 2 * WARPS);
+    return make_float2(t.x + t.z, t.y + t.w);
+  }
+  __device__ __forceinline__ float operator()(float a) {
+    a = LaneSum<32>()(a);
+    float* const b = buffer + at;
+    at ^= WARPS;
+    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = a;
+    __syncthreads();
+    const float4 t = total(b, WARPS);
+    return (t.x + t.y) + (t.z + t.w);
+  }
+  static __device__ __forceinline__ float4 total(const float* b, int floats) {
+    float4 t = *reinterpret_cast<const float4*>(b);
+#pragma unroll
+    for (int k = 4; k < floats; k += 4) {
+      const float4 u = *reinterpret_cast<const float4*>(b + k);
+      t.x += u.x, t.y += u.y, t.z += u.z, t.w += u.w;
+    }
+    return t;
+  }
+};
+
+// A row's values become xhat; rstd is returned.  lead: one of the row's values.  Sums are taken of x - lead: a row of
+// equal values comes out as zeros, an offset common to the row costs no accuracy, and lead is never further from the
+// mean than sqrt(C) standard deviations.
+template <typename T, Layout LAYOUT, typename Sum>
+__device__ __forceinline__ float normalise(const Lane<T, LAYOUT>& at, float2* v, float lead, const LayerNorm& p, Sum& sum) {
+  constexpr int H = LN_VALUES / 2;
+#pragma unroll
+  for (int i = 0; i < H; ++i) v[i] = LAYOUT == FULL ? add2(v[i], both(-lead)) : fma2(both(-lead), at.on[i], v[i]);
+  const float2 a = add2(add2(v[0], v[1]), add2(v[2], v[3]));
+  const float mean = sum(a.x + a.y) * p.inv_C;
+#pragma unroll
+  for (int i = 0; i < H; ++i) v[i] = LAYOUT == FULL ? add2(v[i], both(-mean)) : fma2(both(-mean), at.on[i], v[i]);
+  const float2 q = add2(fma2(v[0], v[0], mul2(v[1], v[1])), fma2(v[2], v[2], mul2(v[3], v[3])));
+  const float rstd = rsqrtf(fmaf(sum(q.x + q.y), p.inv_C, p.eps));
+#pragma unroll
+  for (int i = 0; i < H; ++i) v[i] = mul2(v[i], both(rstd));
+  return rstd;
+}
+
+__device__ __forceinline__ float reciprocal(float a) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+  return r;
+}
+
+// s = 1 / (1 + exp(-z)).  Both functions are the hardware's (exp2 within 2 units in the last place of an argument that
+// rounds by |z| units, which count where exp(-z) outweighs the 1; the reciprocal within 1), and two values share a
+// reciprocal of their product: 12 of them instead of 16 for a lane's 8 values, whose pipe bounds 16-bit rows.  Values
+// whose product could overflow, or that are not numbers, are taken one by one.
+__device__ __forceinline__ void sigmoid(const float2* z, float2* s) {
+  constexpr int H = LN_VALUES / 2;
+  float2 a[H];
+#pragma unroll
+  for (int i = 0; i < H; ++i) {
+    const float2 e = mul2(z[i], both(-1.44269504f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a[i].x) : "f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a[i].y) : "f"(e.y));
+    a[i] = add2(a[i], both(1.f));
+  }
+  const float2 t = add2(add2(a[0], a[1]), add2(a[2], a[3]));
+  if (t.x + t.y <= 0x1p62f) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) s[i] = mul2(both(reciprocal(a[i].x * a[i].y)), make_float2(a[i].y, a[i].x));
+  } else {
+#pragma unroll
+    for (int i = 0; i < H; ++i) s[i] = make_float2(reciprocal(a[i].x), reciprocal(a[i].y));
+  }
+}
+
+// lanes of a row: 8 channels each (`head`: and the values before its start); a power of two up to a warp, then whole
+// warps
+inline int row_lanes(int C, int head) {
+  const int need = (C + head + LN_VALUES - 1) / LN_VALUES;
+  if (need > 32) return (need + 31) / 32 * 32;
+  int l = 4;
+  while (l < need) l *= 2;
+  return l;
+}
+
+// f(std::integral_constant<int, lanes>) for rows of up to 32 lanes
+template <typename F>
+int with_lanes(int lanes, F&& f) {
+  switch (lanes) {
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 8: return f(std::integral_constant<int, 8>{});
+    case 16: return f(std::integral_constant<int, 16>{});
+    default: return f(std::integral_constant<int, 32>{});
+  }
+}
+
+struct RowPlan {
+  Layout layout;
+  int lanes;
+};
+struct Operand {
+  const void* at;  // null: none
+  int64_t stride;
+};
+
+template <typename T>
+RowPlan row_plan(int64_t n, int C, std::initializer_list<Operand> operands) {
+  constexpr int V = 16 / sizeof(T);
+  bool alike = true, start = true, apart = true;
+  const Operand& x = *operands.begin();
+  for (const Operand& o : operands) {
+    if (!o.at) continue;
+    alike = alike && ((reinterpret_cast<uintptr_t>(o.at) - reinterpret_cast<uintptr_t>(x.at)) & 15) == 0 &&
+            (o.stride - x.stride) % V == 0;
+    start = start && (reinterpret_cast<uintptr_t>(o.at) & 15) == 0 && o.stride % V == 0;
+    apart = apart && (o.stride > 0 || n <= 1);
+  }
+  const int lanes = row_lanes(C, start ? 0 : V - 1);
+  if (start && lanes * LN_VALUES == C) return {FULL, lanes};
+  // (rows that repeat: a neighbour's values need not lie inside the tensor)
+  if (!alike || !apart || C <= V || lanes > 1024) return {APART, row_lanes(C, 0)};
+  return {PIECES, lanes};
+}
+
+// values between the 16-byte address before row r and the row
+template <typename T>
+__device__ __forceinline__ int row_head(const void* x, int64_t stride, int64_t r) {
+  return (int)((reinterpret_cast<uintptr_t>(static_cast<const T*>(x) + r * stride) & 15) / sizeof(T));
+}
+
+inline uint32_t inner_rows(int64_t n) { return n > 2 * LN_TURN ? (uint32_t)(n - 2 * LN_TURN) : 0; }
+
+inline bool bad_rows(int32_t dtype, int32_t param_dtype, int64_t n, int32_t C, float eps, int32_t activation) {
+  return (dtype != MACE_F32 && dtype != MACE_BF16) || (param_dtype != MACE_F32 && param_dtype != MACE_BF16) || n < 0 ||
+         n > INT32_MAX || C < 1 || C > MACE_LAYER_NORM_MAX_CHANNELS || !(eps >= 0.f) || !std::isfinite(eps) ||
+         (activation != MACE_ACT_NONE && activation != MACE_ACT_SILU);
+}
+
+// f(layout) with the layout as std::integral_constant
+template <typename F>
+int with_layout(Layout layout, F&& f) {
+  switch (layout) {
+    case FULL: return f(std::integral_constant<Layout, FULL>{});
+    case PIECES: return f(std::integral_constant<Layout, PIECES>{});
+    default: return f(std::integral_constant<Layout, APART>{});
+  }
+}
+
+}  // namespace mace

@@ -1,0 +1,275 @@
+// Gradients of the layer norm (layer_norm.cu) at its rows and parameters.
+//
+//   dz = dy or dy s (1 + z (1 - s)), s = 1 / (1 + exp(-z)); dw = sum over rows dz xhat, db = sum dz
+//   g = w dz, dx = rstd (g - mean(g) - xhat mean(g xhat))
+//
+// One pass: x and dy stay in registers until dx is stored, and mean and rstd are made once more from the x that has to
+// be read anyway, so the forward keeps nothing for it.  A CTA adds the parameters' gradients over its share of the rows
+// in registers and leaves one row of sums; a second launch adds those.
+#include "layer_norm.cuh"
+
+namespace mace {
+
+namespace {
+
+// xhat and dy of a row to dx (in g); the sums of dw and db move on
+template <bool SILU, typename Sum>
+__device__ __forceinline__ void row_grad(const float2* xhat, float2* g, const float2* w, const float2* b, float rstd,
+                                         float inv_C, float2* dw, float2* db, Sum& sum) {
+  constexpr int H = LN_VALUES / 2;
+  if (SILU) {
+    float2 z[H], s[H];
+#pragma unroll
+    for (int i = 0; i < H; ++i) z[i] = fma2(xhat[i], w[i], b[i]);
+    sigmoid(z, s);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const float2 rest = fma2(s[i], both(-1.f), both(1.f));
+      g[i] = mul2(g[i], mul2(s[i], fma2(z[i], rest, both(1.f))));
+    }
+  }
+  float2 c1 = both(0.f), c2 = both(0.f);
+#pragma unroll
+  for (int i = 0; i < H; ++i) {
+    dw[i] = fma2(g[i], xhat[i], dw[i]);
+    db[i] = add2(db[i], g[i]);
+    g[i] = mul2(g[i], w[i]);
+    c1 = add2(c1, g[i]);
+    c2 = fma2(g[i], xhat[i], c2);
+  }
+  const float2 c = sum(make_float2(c1.x + c1.y, c2.x + c2.y));
+  const float2 m1 = both(-c.x * inv_C), m2 = both(-c.y * inv_C);
+#pragma unroll
+  for (int i = 0; i < H; ++i) g[i] = mul2(both(rstd), fma2(xhat[i], m2, add2(g[i], m1)));
+}
+
+// Rows of up to 32 lanes: a CTA takes a share of neighbouring rows.  The next row of each lane group is in flight.
+template <typename T, Layout LAYOUT, int L, bool SILU>
+__global__ void __launch_bounds__(LN_THREADS, 2) k_layer_norm_grad(LayerNorm p) {
+  constexpr int GROUPS = LN_THREADS / L, WIDTH = L * LN_VALUES, H = LN_VALUES / 2;
+  __shared__ float sums[GROUPS][2][WIDTH];
+  const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L, group = threadIdx.x / L;
+  pdl_wait();
+  const int64_t begin = blockIdx.x * p.share;
+  const uint32_t end = (uint32_t)min(p.n, begin + p.share);
+  uint32_t r = (uint32_t)begin + group;
+  const T* x = static_cast<const T*>(p.x) + r * p.xs;
+  const T* dy = static_cast<const T*>(p.dy) + r * p.ds;
+  T* dx = static_cast<T*>(p.y) + r * p.ys;
+  const Lane<T, LAYOUT> at(lane, L, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
+  float2 w[H], b[H], dw[H], db[H];
+  at.param(p.w, p.param_f32, 1.f, p.C, w);
+  at.param(p.b, p.param_f32, 0.f, p.C, b);
+#pragma unroll
+  for (int i = 0; i < H; ++i) dw[i] = db[i] = both(0.f);
+  Part<T, LAYOUT> nx, nd;
+  nx.zero();
+  nd.zero();
+  if (r < end) {
+    nx.load(at, x, r - LN_TURN < p.inner);
+    nd.load(at, dy, r - LN_TURN < p.inner);
+  }
+  LaneSum<L> sum;
+  for (; r - sub < end; r += GROUPS) {
+    float2 v[H], g[H];
+    nx.values(at, v);
+    nd.values(at, g);
+    // (PIECES: the second piece is the row's whatever the first one holds)
+    const float lead = __shfl_sync(0xffffffffu, v[0].x, LAYOUT == PIECES ? 1 : 0, L);
+    x += GROUPS * p.xs;
+    dy += GROUPS * p.ds;
+    if (r + GROUPS < end) {
+      nx.load(at, x, r + GROUPS - LN_TURN < p.inner);
+      nd.load(at, dy, r + GROUPS - LN_TURN < p.inner);
+    }
+    const float rstd = normalise(at, v, lead, p, sum);
+    if (r >= end)  // no row
+#pragma unroll
+      for (int i = 0; i < H; ++i) v[i] = g[i] = both(0.f);
+    row_grad<SILU>(v, g, w, b, rstd, p.inv_C, dw, db, sum);
+    if (p.y && r < end) Part<T, LAYOUT>::store(at, dx, g);
+    dx += GROUPS * p.ys;
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int j = 0; j < LN_VALUES; ++j)
+    if (at.in(j, p.C)) {
+      sums[group][0][at.at(j)] = j & 1 ? dw[j / 2].y : dw[j / 2].x;
+      sums[group][1][at.at(j)] = j & 1 ? db[j / 2].y : db[j / 2].x;
+    }
+  __syncthreads();
+  float* const out = p.part + blockIdx.x * (int64_t)p.pitch;
+  for (int k = threadIdx.x; k < 2 * p.C; k += LN_THREADS) {
+    const int which = k >= p.C, c = k - which * p.C;
+    float t = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < GROUPS; ++i) t += sums[i][which][c];
+    out[k] = t;
+  }
+}
+
+// wider rows: a CTA takes every LN_TURN-th row of LN_TURN shares, one at a time
+template <typename T, Layout LAYOUT, bool SILU, int MOST>
+__global__ void __launch_bounds__(MOST) k_layer_norm_grad_wide(LayerNorm p) {
+  constexpr int H = LN_VALUES / 2;
+  __shared__ __align__(16) float sums[CtaSum<MOST / 32>::FLOATS];
+  pdl_wait();
+  const int64_t begin = (blockIdx.x / LN_TURN) * LN_TURN * p.share;
+  const uint32_t end = (uint32_t)min(p.n, begin + LN_TURN * p.share);
+  uint32_t r = (uint32_t)begin + blockIdx.x % LN_TURN;
+  const T* x = static_cast<const T*>(p.x) + r * p.xs;
+  const T* dy = static_cast<const T*>(p.dy) + r * p.ds;
+  T* dx = static_cast<T*>(p.y) + r * p.ys;
+  const Lane<T, LAYOUT> at(threadIdx.x, blockDim.x, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
+  float2 w[H], b[H], dw[H], db[H];
+  at.param(p.w, p.param_f32, 1.f, p.C, w);
+  at.param(p.b, p.param_f32, 0.f, p.C, b);
+#pragma unroll
+  for (int i = 0; i < H; ++i) dw[i] = db[i] = both(0.f);
+  Part<T, LAYOUT> nx, nd;
+  nx.zero();
+  nd.zero();
+  nx.load(at, x, r - LN_TURN < p.inner);
+  nd.load(at, dy, r - LN_TURN < p.inner);
+  float ahead = to_f32(load_in(x));
+  CtaSum<MOST / 32> sum(sums);
+  for (; r < end; r += LN_TURN) {
+    float2 v[H], g[H];
+    const float lead = ahead;
+    nx.values(at, v);
+    nd.values(at, g);
+    x += LN_TURN * p.xs;
+    dy += LN_TURN * p.ds;
+    if (r + LN_TURN < end) {
+      nx.load(at, x, r < p.inner);
+      nd.load(at, dy, r < p.inner);
+      ahead = to_f32(load_in(x));
+    }
+    const float rstd = normalise(at, v, lead, p, sum);
+    row_grad<SILU>(v, g, w, b, rstd, p.inv_C, dw, db, sum);
+    if (p.y) Part<T, LAYOUT>::store(at, dx, g);
+    dx += LN_TURN * p.ys;
+  }
+  if (!p.part) return;
+  float* const out = p.part + blockIdx.x * (int64_t)p.pitch;
+#pragma unroll
+  for (int j = 0; j < LN_VALUES; ++j)
+    if (at.in(j, p.C)) {
+      out[at.at(j)] = j & 1 ? dw[j / 2].y : dw[j / 2].x;
+      out[p.C + at.at(j)] = j & 1 ? db[j / 2].y : db[j / 2].x;
+    }
+}
+
+// dw and db from the shares' sums: a CTA adds 32 columns, 4 a lane, a lane group every 128th share
+__global__ void __launch_bounds__(1024) k_layer_norm_join(LayerNorm p) {
+  __shared__ float4 sums[128][8];
+  const int quad = threadIdx.x & 7, slot = threadIdx.x >> 3;
+  const int c0 = blockIdx.x * 32 + quad * 4;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  pdl_wait();
+  if (c0 < p.pitch) {
+#pragma unroll 8
+    for (int64_t s = slot; s < p.shares; s += 128) {
+      const float4 v = *reinterpret_cast<const float4*>(p.part + s * p.pitch + c0);
+      a.x += v.x;
+      a.y += v.y;
+      a.z += v.z;
+      a.w += v.w;
+    }
+  }
+  sums[slot][quad] = a;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float t = 0.f;
+#pragma unroll 16
+  for (int k = 0; k < 128; ++k) t += reinterpret_cast<const float*>(sums[k])[threadIdx.x];
+  if (c >= 2 * p.C) return;
+  void* const out = c < p.C ? p.dw : p.db;
+  const int at = c < p.C ? c : c - p.C;
+  if (!out) return;
+  if (p.param_f32)
+    static_cast<float*>(out)[at] = t;
+  else
+    static_cast<bf16*>(out)[at] = from_f32<bf16>(t);
+}
+
+// Rows of a CTA: enough CTAs to fill the GPU, and at most 256 rows for a lane, so that a sum's error stays that of a
+// few hundred terms.  From n and C alone.
+int64_t grad_share(int64_t n, int C) {
+  const int lanes = row_lanes(C, 0);
+  const int64_t rows = lanes > 32 ? 1 : LN_THREADS / lanes;  // at once
+  const int64_t ctas = lanes > 32 ? LN_SMS * std::max(1, 1024 / lanes) : LN_SMS * 4;
+  int64_t share = std::max((n + ctas - 1) / ctas, rows);
+  share = std::min(share, rows * 256);
+  return (share + rows - 1) / rows * rows;
+}
+int64_t grad_shares(int64_t n, int64_t share, bool wide) {
+  if (!wide) return (n + share - 1) / share;
+  const int64_t full = n / (LN_TURN * share);
+  return full * LN_TURN + std::min<int64_t>(n - full * LN_TURN * share, LN_TURN);
+}
+int grad_pitch(int C) { return (2 * C + 3) & ~3; }
+
+template <typename T, Layout LAYOUT, bool SILU>
+int backward(const LayerNorm& p, int lanes, cudaStream_t s) {
+  const dim3 grid((unsigned)p.shares);
+  if (lanes > 32)
+    return launch("layer_norm_grad", lanes <= 256 ? k_layer_norm_grad_wide<T, LAYOUT, SILU, 256> : k_layer_norm_grad_wide<T, LAYOUT, SILU, 1024>,
+                  grid, lanes, 0, s, p);
+  return with_lanes(lanes, [&](auto l) {
+    return launch("layer_norm_grad", k_layer_norm_grad<T, LAYOUT, decltype(l)::value, SILU>, grid, LN_THREADS, 0, s, p);
+  });
+}
+
+}  // namespace
+
+}  // namespace mace
+
+using namespace mace;
+
+extern "C" int mace_layer_norm_grad_workspace(int64_t n, int32_t C, int64_t* bytes) {
+  if (n < 0 || n > INT32_MAX || C < 1 || C > MACE_LAYER_NORM_MAX_CHANNELS || !bytes)
+    return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad_workspace: bad arguments");
+  const int64_t share = grad_share(n, C);
+  *bytes = std::max(grad_shares(n, share, false), grad_shares(n, share, true)) * grad_pitch(C) * 4;
+  return MACE_OK;
+}
+
+extern "C" int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t xs, const void* dy, int64_t ds,
+                                    int32_t param_dtype, const void* weight, const void* bias, int64_t n, int32_t C,
+                                    float eps, int32_t activation, void* dx, int64_t dxs, void* dweight, void* dbias,
+                                    void* ws, int64_t ws_bytes, void* stream) {
+  if (bad_rows(dtype, param_dtype, n, C, eps, activation) || xs < 0 || ds < 0 || (n > 0 && (!x || !dy)) ||
+      (dx && n > 1 && dxs < C))
+    return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad: bad arguments");
+  if (unaligned(value_size(dtype), x, dy, dx) || unaligned(value_size(param_dtype), weight, bias, dweight, dbias))
+    return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad: an address is not a multiple of its values' size");
+  const bool params = dweight || dbias;
+  int64_t need = 0;
+  mace_layer_norm_grad_workspace(n, C, &need);
+  if (params && need > 0 && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15) != 0))
+    return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad: workspace too small or not 16-byte aligned");
+  LayerNorm p{};
+  p.x = x, p.xs = n > 1 ? xs : 0, p.dy = dy, p.ds = n > 1 ? ds : 0, p.w = weight, p.b = bias;
+  p.param_f32 = param_dtype == MACE_F32, p.n = n, p.C = C, p.eps = eps, p.inv_C = 1.f / C, p.inner = inner_rows(n), p.y = dx, p.ys = n > 1 ? dxs : 0;
+  p.share = grad_share(n, C), p.part = params ? static_cast<float*>(ws) : nullptr;
+  p.pitch = grad_pitch(C), p.dw = dweight, p.db = dbias;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (n > 0 && (params || dx)) {
+    auto go = [&](auto t) {
+      using T = decltype(t);
+      const RowPlan plan = row_plan<T>(n, C, {{x, p.xs}, {dy, p.ds}, {dx, p.ys}});
+      p.shares = grad_shares(n, p.share, plan.lanes > 32);
+      return with_layout(plan.layout, [&](auto layout) {
+        constexpr Layout LAYOUT = decltype(layout)::value;
+        return activation == MACE_ACT_SILU ? backward<T, LAYOUT, true>(p, plan.lanes, s)
+                                           : backward<T, LAYOUT, false>(p, plan.lanes, s);
+      });
+    };
+    const int rc = dtype == MACE_F32 ? go(float{}) : go(bf16{});
+    if (rc) return rc;
+  }
+  if (!params) return MACE_OK;
+  return launch("layer_norm_join", k_layer_norm_join, dim3((unsigned)((p.pitch + 31) / 32)), 1024, 0, s, p);
+}

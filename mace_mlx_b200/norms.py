@@ -32,7 +32,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import native as nv
-from .species import _cuda, _dtype, _launch, _on, _workspace
+from .species import _DTYPES, _cuda, _dtype, _launch, _on, _workspace
 
 MAX_CHANNELS = nv.LAYER_NORM_MAX_CHANNELS
 _ACTIVATIONS = {None: nv.ACT_NONE, "silu": nv.ACT_SILU}
@@ -68,15 +68,20 @@ def _params(weight, bias, dev: int, c: int, dtype: torch.dtype) -> tuple[int, in
         if t is None:
             continue
         _on(name, t, dev)
-        if t.dim() != 1 or t.shape[0] != c or not t.is_contiguous():
+        if t.numel() != c or t.dim() != 1 or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous ({c},) tensor, got {tuple(t.shape)} with strides {t.stride()}")
-        if t.dtype != dtype and t.dtype != torch.float32:
-            raise ValueError(f"{name} is {t.dtype}, expected {dtype} or float32")
-        if kind is not None and t.dtype != kind:
+        if kind is None:
+            kind = t.dtype
+            if kind is not dtype and kind is not torch.float32:
+                raise ValueError(f"{name} is {kind}, expected {dtype} or float32")
+        elif t.dtype is not kind:
             raise ValueError(f"weight is {kind}, bias {t.dtype}: they must be of one type")
-        kind = t.dtype
-    return (_dtype("weight", dtype if kind is None else kind), None if weight is None else weight.data_ptr(),
+    return (_DTYPES[dtype if kind is None else kind], None if weight is None else weight.data_ptr(),
             None if bias is None else bias.data_ptr())
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _activation(activation: str | None) -> int:
@@ -99,7 +104,7 @@ def _layer_norm(x, weight, bias, eps, activation, out):
     pcode, w, b = _params(weight, bias, dev, c, x.dtype)
     act = _activation(activation)
     if out is None:
-        y = x.new_empty(x.shape)
+        y = _like(x)
         ys = c
     else:
         y = out
@@ -126,9 +131,9 @@ def _layer_norm_grad(x, grad, weight, bias, eps, activation, want_x, want_w, wan
     _, _, gs = _rows("grad", grad)
     pcode, w, b = _params(weight, bias, dev, c, x.dtype)
     act = _activation(activation)
-    dx = x.new_empty(x.shape) if want_x else None
-    dw = torch.empty_like(weight) if want_w else None
-    db = torch.empty_like(bias) if want_b else None
+    dx = _like(x) if want_x else None
+    dw = _like(weight) if want_w else None
+    db = _like(bias) if want_b else None
     ws, ptr, nbytes = None, None, 0
     if want_w or want_b:
         ws, ptr, nbytes = _workspace("mace_layer_norm_grad_workspace", dev, x, n, c)
@@ -206,25 +211,32 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int) -> tuple[array, array, array]:
-    """Pointers, sizes and type codes of dense tensors on device ``dev``."""
-    tangents = forward_ad._current_level >= 0
-    for i, t in enumerate(tensors):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name}[{i}] must be a torch.Tensor, got {type(t).__name__}")
-        if not t.is_cuda or t.get_device() != dev or tangents:
+# what the lists ask of every tensor, read without a Python frame each: a step's call is bound by it
+_device, _pointer, _numel, _contiguous = (getattr(torch.Tensor, f) for f in
+                                          ("get_device", "data_ptr", "numel", "is_contiguous"))
+
+
+def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int) -> tuple[array, array, array, bool]:
+    """Pointers, sizes and type codes of dense tensors on device ``dev``, and whether all are contiguous."""
+    contiguous = False
+    if not all(isinstance(t, torch.Tensor) for t in tensors) or forward_ad._current_level >= 0:
+        for i, t in enumerate(tensors):
             _on(f"{name}[{i}]", t, dev)
-        if not _dense(t):
-            raise ValueError(f"{name}[{i}] has gaps or repeated values (strides {t.stride()}); use .contiguous()"
-                             if t.layout is torch.strided else f"{name}[{i}] is not strided, got {t.layout}")
+    if tensors and set(map(_device, tensors)) != {dev}:
+        for i, t in enumerate(tensors):
+            _on(f"{name}[{i}]", t, dev)
+    if all(t.layout is torch.strided for t in tensors):
+        contiguous = all(map(_contiguous, tensors))
+    if not contiguous:
+        for i, t in enumerate(tensors):
+            if not _dense(t):
+                raise ValueError(f"{name}[{i}] has gaps or repeated values (strides {t.stride()}); use .contiguous()"
+                                 if t.layout is torch.strided else f"{name}[{i}] is not strided, got {t.layout}")
     try:
-        codes = array("i", [_CODES[t.dtype] for t in tensors])
+        codes = array("i", [_DTYPES[t.dtype] for t in tensors])
     except KeyError as e:
         raise ValueError(f"{name} must be float32 or bfloat16, got {e.args[0]}") from None
-    return array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]), codes
-
-
-_CODES = {torch.float32: nv.DTYPE_F32, torch.bfloat16: nv.DTYPE_BF16}
+    return array("Q", map(_pointer, tensors)), array("q", map(_numel, tensors)), codes, contiguous
 
 
 def _grads(grads: Iterable[torch.Tensor | None]) -> list[torch.Tensor]:
@@ -233,12 +245,11 @@ def _grads(grads: Iterable[torch.Tensor | None]) -> list[torch.Tensor]:
     return [g for g in grads if g is not None]
 
 
-def _grad_call(grads, dev, more):
-    ptrs, sizes, codes = _flat("grads", grads, dev)
-    norm = torch.empty((), dtype=torch.float32, device=torch.device("cuda", dev))
+def _norm_of(grads: list[torch.Tensor], dev: int, flat, fn, *more) -> torch.Tensor:
+    ptrs, sizes, codes, _ = flat
+    norm = grads[0].new_empty((), dtype=torch.float32) if grads else torch.empty((), device=torch.device("cuda", dev))
     ws, wptr, nbytes = _workspace("mace_grad_norm_workspace", dev, norm, len(grads))
-    fn, extra = more
-    _launch(dev, fn, len(grads), ptrs.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], *extra,
+    _launch(dev, fn, len(grads), ptrs.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], *more,
             norm.data_ptr(), wptr, nbytes)
     return norm
 
@@ -252,7 +263,7 @@ def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
     """
     grads = _grads(grads)
     dev = _cuda("grads[0]", grads[0]) if grads else torch.cuda.current_device()
-    return _grad_call(grads, dev, (nv.load_library().mace_grad_norm, ()))
+    return _norm_of(grads, dev, _flat("grads", grads, dev), nv.load_library().mace_grad_norm)
 
 
 def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
@@ -260,8 +271,8 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
     """Scales the gradients by ``min(1, max_norm / (norm + 1e-6))``, in place, and returns their ``grad_norm``.
 
     Gradients below the bound are left untouched, and nothing waits for the
-    norm on the host.  With ``out`` (a tensor for every gradient, of its shape
-    and order of dimensions, float32 or bfloat16) the results go there and the
+    norm on the host.  With ``out`` (a tensor for every gradient, with as many
+    values in the same order in memory, float32 or bfloat16) the results go there and the
     gradients stay, unless ``out`` holds the gradient itself.  No tensor that
     is written may overlap another one of the call, so none may be listed twice.
 
@@ -273,21 +284,22 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
     max_norm = float(max_norm)
     if not 0.0 <= max_norm < math.inf:
         raise ValueError(f"max_norm must be finite and not negative, got {max_norm}")
-    every = list(grads) if not isinstance(grads, torch.Tensor) else grads
+    every = grads if isinstance(grads, torch.Tensor) else list(grads)
     grads = _grads(every)
-    into = grads
+    dev = _cuda("grads[0]", grads[0]) if grads else torch.cuda.current_device()
+    flat = _flat("grads", grads, dev)
+    into, ptrs, codes = grads, flat[0], flat[2]
     if out is not None:
         if len(out) != len(every):
             raise ValueError(f"out has {len(out)} tensors, grads {len(every)}")
         into = [o for o, g in zip(out, every) if g is not None]
-    dev = _cuda("grads[0]", grads[0]) if grads else torch.cuda.current_device()
-    ptrs, _, codes = _flat("out" if out is not None else "grads", into, dev)
-    if out is not None:
-        for i, (g, o) in enumerate(zip(grads, into)):
-            if o.shape != g.shape or o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
-                raise ValueError(f"out[{i}] must be {tuple(g.shape)} with strides {g.stride()}, got {tuple(o.shape)} with "
-                                 f"strides {o.stride()}")
-    norm = _grad_call(grads, dev, (nv.load_library().mace_grad_clip,
-                                   (ptrs.buffer_info()[0], codes.buffer_info()[0], max_norm)))
+        ptrs, sizes, codes, contiguous = _flat("out", into, dev)
+        if sizes != flat[1] or not (contiguous and flat[3]):
+            for i, (g, o) in enumerate(zip(grads, into)):
+                if o.numel() != g.numel() or o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
+                    raise ValueError(f"out[{i}] must be {tuple(g.shape)} with strides {g.stride()}, got {tuple(o.shape)} "
+                                     f"with strides {o.stride()}")
+    norm = _norm_of(grads, dev, flat, nv.load_library().mace_grad_clip, ptrs.buffer_info()[0], codes.buffer_info()[0],
+                    max_norm)
     torch.autograd.graph.increment_version(into)
     return norm

@@ -186,7 +186,8 @@ def test_rows_in_a_wider_table(nm, dtype, c, pitch, at):
         into = table[:, at + c:at + 2 * c]
         before = table.clone()
         nm.layer_norm(table[:, at:at + c], w, b, activation="silu", out=into)
-        assert torch.equal(into, out)
+        # (the order of a row's sums follows its address modulo 16: within the bound, not equal bits)
+        assert_close(into, *Rows64(x, w, b, 1e-5, True).forward(), "slot")
         before[:, at + c:at + 2 * c] = into
         assert torch.equal(table, before)
     assert torch.equal(grads[:, at:at + c], dy)

@@ -123,7 +123,7 @@ def test_kernels_read_their_inputs_by_plain_loads():
     """As the species operators' kernels: one may start while the kernel before it still writes its inputs."""
     from pathlib import Path
 
-    for name in ("layer_norm.cu", "grad_norm.cu"):
+    for name in ("layer_norm.cu", "layer_norm_grad.cu", "layer_norm.cuh", "grad_norm.cu"):
         text = (Path(mace_mlx_b200.__file__).parent / "csrc" / name).read_text()
         for form in ("__ldg(", "global.nc", "__restrict__"):
             assert form not in text, (name, form)
