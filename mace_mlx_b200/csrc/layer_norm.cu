@@ -14,28 +14,37 @@ namespace mace {
 
 namespace {
 
-template <bool SILU>
-__device__ __forceinline__ void affine(float2* v, const float2* w, const float2* b) {
+template <bool SILU, int N, bool SHARED>
+__device__ __forceinline__ void affine(float2* v, const Params<N, SHARED>& params) {
 #pragma unroll
-  for (int i = 0; i < LN_VALUES / 2; ++i) v[i] = fma2(v[i], w[i], b[i]);
-  if (SILU) {
-    float2 s[LN_VALUES / 2];
-    sigmoid(v, s);
+  for (int c = 0; c < N / 8; ++c) {
+    float2 w[4], b[4], *const u = v + 4 * c;
+    params.weight(c, w);
+    params.bias(c, b);
 #pragma unroll
-    for (int i = 0; i < LN_VALUES / 2; ++i) v[i] = mul2(v[i], s[i]);
+    for (int i = 0; i < 4; ++i) u[i] = fma2(u[i], w[i], b[i]);
+    if (SILU) {
+      sigmoid(u, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = mul2(u[i], w[i]);
+    }
   }
 }
 
-// CTAs on an SM.  16-byte pieces of fp32 rows fill the memory's queues from three (2M rows of 64 with SiLU 162 us, 174
-// with four, 199 with five), 16-bit rows hide their arithmetic behind five (1M rows of 128 91 us, 99 with four).
+// CTAs on an SM, and where the lanes keep their parameters.  32 bytes of a row in flight for each lane of three CTAs
+// fill the memory's queues (2M fp32 rows of 64 with SiLU 162 us, 173 with four CTAs, 187 with two); rows that start
+// anywhere have less in a lane and take four in fp32 (500 003 rows of 96 69 us, 77 with three).  16 values of a lane
+// leave no registers for their parameters (2M bf16 rows of 64 with SiLU 89 us, 110 with parameters in registers).
 template <typename T, Layout LAYOUT>
-constexpr int LN_PER_SM = LAYOUT == FULL && sizeof(T) == 2 ? 5 : 3;
+constexpr int LN_PER_SM = sizeof(T) == 4 && LAYOUT == PIECES ? 4 : 3;
+template <Layout LAYOUT, int N>
+constexpr bool LN_SHARED = N == 16 || LAYOUT == PIECES;
 
-// Rows of up to 32 lanes.  The next row of each lane group is in flight (a second and third one in flight cost more
-// registers than they hide latency: 16-bit rows 117 us instead of 100).
-template <typename T, Layout LAYOUT, int L, bool SILU>
+// Rows of up to 32 lanes.  The next row of each lane group is in flight.
+template <typename T, Layout LAYOUT, int N, int L, bool SILU>
 __global__ void __launch_bounds__(LN_THREADS, LN_PER_SM<T, LAYOUT>) k_layer_norm(LayerNorm p) {
-  constexpr int H = LN_VALUES / 2;
+  constexpr bool SHARED = LN_SHARED<LAYOUT, N>;
+  __shared__ float4 own[SHARED ? Params<N, SHARED>::BYTES / 16 * LN_THREADS : 1];
   const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L;
   pdl_wait();
   const uint32_t n = (uint32_t)p.n, step = gridDim.x * (LN_THREADS / L);
@@ -43,75 +52,72 @@ __global__ void __launch_bounds__(LN_THREADS, LN_PER_SM<T, LAYOUT>) k_layer_norm
   const T* x = static_cast<const T*>(p.x) + r * p.xs;
   T* y = static_cast<T*>(p.y) + r * p.ys;
   const int64_t x_step = step * p.xs, y_step = step * p.ys;
-  const Lane<T, LAYOUT> at(lane, L, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
-  float2 w[H], b[H];
-  at.param(p.w, p.param_f32, 1.f, p.C, w);
-  at.param(p.b, p.param_f32, 0.f, p.C, b);
-  Part<T, LAYOUT> next;
+  const Lane<T, LAYOUT, N> at(lane, L, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
+  const Params<N, SHARED> params(at, p, own, threadIdx.x, LN_THREADS);
+  Part<T, LAYOUT, N> next;
   next.zero();
   if (r < n) next.load(at, x, r - LN_TURN < p.inner);
   LaneSum<L> sum;
   for (; r - sub < n; r += step) {
-    float2 v[H];
-    next.values(at, v);
-    // (PIECES: the second piece is the row's whatever the first one holds)
-    const float lead = __shfl_sync(0xffffffffu, v[0].x, LAYOUT == PIECES ? 1 : 0, L);
+    float2 v[N / 2];
+    const float lead = next.template lead<L>();
+    next.values(at, lead, v);
     x += x_step;
     if (r + step < n) next.load(at, x, r + step - LN_TURN < p.inner);
     normalise(at, v, lead, p, sum);
-    affine<SILU>(v, w, b);
-    if (r < n) Part<T, LAYOUT>::store(at, y, v);
+    affine<SILU>(v, params);
+    if (r < n) Part<T, LAYOUT, N>::store(at, y, v);
     y += y_step;
   }
 }
 
 // wider rows: a CTA each
-template <typename T, Layout LAYOUT, bool SILU, int MOST>
+template <typename T, Layout LAYOUT, int N, bool SILU, int MOST>
 __global__ void __launch_bounds__(MOST) k_layer_norm_wide(LayerNorm p) {
-  constexpr int H = LN_VALUES / 2;
   __shared__ __align__(16) float sums[CtaSum<MOST / 32>::FLOATS];
   pdl_wait();
   const uint32_t n = (uint32_t)p.n, step = gridDim.x;
   uint32_t r = blockIdx.x;  // (the grid is a multiple of LN_TURN, or each CTA has one row)
   const T* x = static_cast<const T*>(p.x) + r * p.xs;
   T* y = static_cast<T*>(p.y) + r * p.ys;
-  const Lane<T, LAYOUT> at(threadIdx.x, blockDim.x, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
-  float2 w[H], b[H];
-  at.param(p.w, p.param_f32, 1.f, p.C, w);
-  at.param(p.b, p.param_f32, 0.f, p.C, b);
-  Part<T, LAYOUT> next;
+  const Lane<T, LAYOUT, N> at(threadIdx.x, blockDim.x, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
+  const Params<N, false> params(at, p, nullptr, threadIdx.x, blockDim.x);
+  Part<T, LAYOUT, N> next;
   next.zero();
   next.load(at, x, r - LN_TURN < p.inner);
   float ahead = to_f32(load_in(x));
   CtaSum<MOST / 32> sum(sums);
   for (; r < n; r += step) {
-    float2 v[H];
+    float2 v[N / 2];
     const float lead = ahead;
-    next.values(at, v);
+    next.values(at, lead, v);
     x += step * p.xs;
     if (r + step < n) {
       next.load(at, x, r + step - LN_TURN < p.inner);
       ahead = to_f32(load_in(x));
     }
     normalise(at, v, lead, p, sum);
-    affine<SILU>(v, w, b);
-    Part<T, LAYOUT>::store(at, y, v);
+    affine<SILU>(v, params);
+    Part<T, LAYOUT, N>::store(at, y, v);
     y += step * p.ys;
   }
 }
 
-template <typename T, Layout LAYOUT, bool SILU>
+template <typename T, Layout LAYOUT, int N, bool SILU>
 int forward(const LayerNorm& p, int lanes, cudaStream_t s) {
-  if (lanes > 32) {
-    const int64_t grid = std::min<int64_t>(p.n, LN_SMS * std::max(1, 2048 / lanes) / LN_TURN * LN_TURN);
-    return launch("layer_norm", lanes <= 256 ? k_layer_norm_wide<T, LAYOUT, SILU, 256> : k_layer_norm_wide<T, LAYOUT, SILU, 1024>,
-                  dim3((unsigned)grid), lanes, 0, s, p);
+  if constexpr (may_be_wide(LAYOUT, N)) {
+    if (lanes > 32) {
+      constexpr int MOST = MACE_LAYER_NORM_MAX_CHANNELS / N;  // lanes
+      const int64_t grid = std::min<int64_t>(p.n, LN_SMS * std::max(1, 1024 / lanes) / LN_TURN * LN_TURN);
+      auto go = [&](auto kernel) { return launch("layer_norm", kernel, dim3((unsigned)grid), lanes, 0, s, p); };
+      return lanes <= 256 ? go(k_layer_norm_wide<T, LAYOUT, N, SILU, 256>) : go(k_layer_norm_wide<T, LAYOUT, N, SILU, MOST>);
+    }
   }
-  return with_lanes(lanes, [&](auto l) {
+  return with_lanes<(N > narrow_values<T, false>(LAYOUT))>(lanes, [&](auto l) {
     constexpr int L = decltype(l)::value;
     const int64_t per = LN_THREADS / L;
     const int64_t grid = std::min<int64_t>((p.n + per - 1) / per, LN_SMS * LN_PER_SM<T, LAYOUT>);
-    return launch("layer_norm", k_layer_norm<T, LAYOUT, L, SILU>, dim3((unsigned)grid), LN_THREADS, 0, s, p);
+    return launch("layer_norm", k_layer_norm<T, LAYOUT, N, L, SILU>, dim3((unsigned)grid), LN_THREADS, 0, s, p);
   });
 }
 
@@ -135,10 +141,12 @@ extern "C" int mace_layer_norm(int32_t dtype, const void* x, int64_t xs, int32_t
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto t) {
     using T = decltype(t);
-    const RowPlan plan = row_plan<T>(n, C, {{x, p.xs}, {y, p.ys}});
-    return with_layout(plan.layout, [&](auto layout) {
+    const RowPlan plan = row_plan<T, false>(n, C, {{x, p.xs}, {y, p.ys}});
+    return with_plan<T, false>(plan, [&](auto layout, auto values) {
       constexpr Layout LAYOUT = decltype(layout)::value;
-      return activation == MACE_ACT_SILU ? forward<T, LAYOUT, true>(p, plan.lanes, s) : forward<T, LAYOUT, false>(p, plan.lanes, s);
+      constexpr int N = decltype(values)::value;
+      return activation == MACE_ACT_SILU ? forward<T, LAYOUT, N, true>(p, plan.lanes, s)
+                                         : forward<T, LAYOUT, N, false>(p, plan.lanes, s);
     });
   };
   return dtype == MACE_F32 ? go(float{}) : go(bf16{});

@@ -12,7 +12,6 @@
 namespace mace {
 
 constexpr int LN_THREADS = 256;  // of a CTA whose rows have up to 32 lanes
-constexpr int LN_VALUES = 8;     // of a lane
 constexpr int LN_SMS = 148;
 constexpr int LN_TURN = 8;       // rows that many apart begin at the same address modulo 16
 
@@ -38,7 +37,7 @@ struct LayerNorm {
   void* db;
 };
 
-// How a row's channels reach its lanes, 8 each:
+// How a row's channels reach its lanes, N each:
 //   FULL    16-byte pieces, every row starts with one, and the lanes take exactly C channels
 //   PIECES  16-byte pieces at 16-byte addresses, wherever the row starts: its first and last piece may hold values of
 //           its neighbours, which are masked.  A row's start modulo 16 repeats every LN_TURN rows, so lanes that step
@@ -75,33 +74,32 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 __device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 // A lane's channels: value j is channel at(j), and in the row where 0 <= at(j) < C.
-template <typename T, Layout LAYOUT>
+template <typename T, Layout LAYOUT, int N>
 struct Lane {
-  static constexpr int V = LAYOUT == APART ? 1 : 16 / sizeof(T), K = LN_VALUES / V;
-  // values of a lane that are none of the row's come as zeros (PIECES: cut off the words as they lie in memory), and
-  // what is subtracted from the row's values is multiplied by `on` (1 or 0) for them
-  static constexpr int WORDS = LAYOUT == PIECES ? LN_VALUES * sizeof(T) / 4 : 1;
-  int first[K];             // channel of a piece's first value
-  int count[K];             // channels of the row in a piece
+  static constexpr int V = LAYOUT == APART ? 1 : 16 / sizeof(T), K = N / V;
+  // the bits of a lane's values that are the row's, in words as they lie in memory (APART: of 32 bits each)
+  static constexpr int WORDS = LAYOUT == FULL ? 1 : (LAYOUT == PIECES ? N * sizeof(T) / 4 : N);
+  int first[K];  // channel of a piece's first value
+  int count[K];  // channels of the row in a piece
   uint32_t keep[WORDS];
-  float2 on[LAYOUT == FULL ? 1 : LN_VALUES / 2];
+  float off;     // values of the lane that are not the row's
+  bool some;     // or all are
   // head: values between a 16-byte address and the row's start
   __device__ __forceinline__ Lane(int lane, int lanes, int C, int head) {
+    int all = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       first[k] = (k * lanes + lane) * V - head;
       count[k] = LAYOUT == FULL ? V : max(0, min(first[k] + V, C) - max(first[k], 0));
+      all += count[k];
     }
+    off = (float)(N - all);
+    some = all > 0;
     if constexpr (LAYOUT != FULL) {
 #pragma unroll
-      for (int i = 0; i < LN_VALUES / 2; ++i)
-        on[i] = make_float2(in(2 * i, C) ? 1.f : 0.f, in(2 * i + 1, C) ? 1.f : 0.f);
-    }
-    if constexpr (LAYOUT == PIECES) {
-#pragma unroll
       for (int i = 0; i < WORDS; ++i)
-        keep[i] = sizeof(T) == 4 ? (in(i, C) ? 0xffffffffu : 0u)
-                                 : (in(2 * i, C) ? 0xffffu : 0u) | (in(2 * i + 1, C) ? 0xffff0000u : 0u);
+        keep[i] = LAYOUT == APART || sizeof(T) == 4 ? (in(i, C) ? 0xffffffffu : 0u)
+                                                    : (in(2 * i, C) ? 0xffffu : 0u) | (in(2 * i + 1, C) ? 0xffff0000u : 0u);
     }
   }
   __device__ __forceinline__ int at(int j) const { return first[j / V] + j % V; }
@@ -110,16 +108,16 @@ struct Lane {
   __device__ __forceinline__ bool any(int k) const { return LAYOUT == FULL || count[k] > 0; }
 
   __device__ __forceinline__ void param(const void* p, int f32, float missing, int C, float2* v) const {
-    float t[LN_VALUES];
+    float t[N];
 #pragma unroll
-    for (int j = 0; j < LN_VALUES; ++j) {
+    for (int j = 0; j < N; ++j) {
       t[j] = 0.f;
       if (in(j, C))
         t[j] = !p ? missing
                   : (f32 ? load_in(static_cast<const float*>(p) + at(j)) : to_f32(load_in(static_cast<const bf16*>(p) + at(j))));
     }
 #pragma unroll
-    for (int i = 0; i < LN_VALUES / 2; ++i) v[i] = make_float2(t[2 * i], t[2 * i + 1]);
+    for (int i = 0; i < N / 2; ++i) v[i] = make_float2(t[2 * i], t[2 * i + 1]);
   }
 };
 
@@ -144,9 +142,9 @@ __device__ __forceinline__ void store_some(char* dst, const uint32_t* w, int m, 
 }
 
 // A lane's part of a row as it lies in memory.
-template <typename T, Layout LAYOUT>
+template <typename T, Layout LAYOUT, int N>
 struct Part {
-  using At = Lane<T, LAYOUT>;
+  using At = Lane<T, LAYOUT, N>;
   static constexpr int V = At::V, K = At::K;
   Raw<T, V> raw[K];
   __device__ __forceinline__ void zero() {
@@ -156,41 +154,53 @@ struct Part {
   // (what is not of the row stays as it was, or is a neighbour's); inner: no first or last row, whose pieces could
   // reach out of the tensor
   __device__ __forceinline__ void load(const At& at, const T* row, bool inner) {
+    if (LAYOUT != PIECES || inner) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const T* const src = row + at.first[k];
-      if constexpr (LAYOUT == PIECES) {
-        if (at.any(k)) {
-          if (inner || at.whole(k)) {
-            raw[k].load(src);
-          } else {
-            T t[V];
-            const int from = at.first[k] < 0 ? V - at.count[k] : 0;
+      for (int k = 0; k < K; ++k)
+        if (at.any(k)) raw[k].load(row + at.first[k]);
+    } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) t[i] = i >= from && i < from + at.count[k] ? load_in(src + i) : from_f32<T>(0.f);
-            raw[k].piece = *reinterpret_cast<const uint4*>(t);
-          }
-        }
-      } else {
-        if (at.any(k)) raw[k].load(src);
+      for (int k = 0; k < K; ++k) {
+        const T* const src = row + at.first[k];
+        T t[V];
+        const int from = at.first[k] < 0 ? V - at.count[k] : 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = i >= from && i < from + at.count[k] ? load_in(src + i) : from_f32<T>(0.f);
+        if constexpr (LAYOUT == PIECES) raw[k].piece = *reinterpret_cast<const uint4*>(t);
       }
     }
   }
-  __device__ __forceinline__ void values(const At& at, float2* v) const {
-    float t[LN_VALUES];
+  // the lane's values, and `fill` for those that are not the row's
+  __device__ __forceinline__ void values(const At& at, float fill, float2* v) const {
+    float t[N];
+    uint32_t f = __float_as_uint(fill);
+    if (LAYOUT == PIECES && sizeof(T) == 2) f = __byte_perm(f, f, 0x3232);  // (a value of the row, or 0: exact in 16 bits)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       Raw<T, V> r = raw[k];
       if constexpr (LAYOUT == PIECES) {
-        r.piece.x &= at.keep[4 * k];
-        r.piece.y &= at.keep[4 * k + 1];
-        r.piece.z &= at.keep[4 * k + 2];
-        r.piece.w &= at.keep[4 * k + 3];
+        uint32_t w[4] = {r.piece.x, r.piece.y, r.piece.z, r.piece.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (w[i] & at.keep[4 * k + i]) | (f & ~at.keep[4 * k + i]);
+        r.piece = make_uint4(w[0], w[1], w[2], w[3]);
       }
       r.values(t + k * V);
+      if constexpr (LAYOUT == APART)
+        t[k] = __uint_as_float((__float_as_uint(t[k]) & at.keep[k]) | (f & ~at.keep[k]));
     }
 #pragma unroll
-    for (int i = 0; i < LN_VALUES / 2; ++i) v[i] = make_float2(t[2 * i], t[2 * i + 1]);
+    for (int i = 0; i < N / 2; ++i) v[i] = make_float2(t[2 * i], t[2 * i + 1]);
+  }
+  // A value of the row from its L lanes (PIECES: the second piece is the row's whatever the first one holds).
+  template <int L>
+  __device__ __forceinline__ float lead() const {
+    uint32_t w;
+    if constexpr (LAYOUT == APART)
+      w = __float_as_uint(to_f32(raw[0].one[0]));
+    else
+      w = raw[0].piece.x;
+    w = __shfl_sync(0xffffffffu, w, LAYOUT == PIECES ? 1 : 0, L);
+    return __uint_as_float(LAYOUT != APART && sizeof(T) == 2 ? w << 16 : w);
   }
   static __device__ __forceinline__ void store(const At& at, T* row, const float2* v) {
 #pragma unroll
@@ -206,14 +216,14 @@ struct Part {
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h = __float22bfloat162_rn(v[i]);
+            const __nv_bfloat162 h = __float22bfloat162_rn(v[4 * k + i]);
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
           }
         }
         if (at.whole(k))
           *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         else if (at.any(k))
-          store_some<sizeof(T)>(reinterpret_cast<char*>(dst), w, at.count[k], at.first[k] < 0);
+          store_some<sizeof(T)>(reinterpret_cast<char*>(dst), w, at.count[k], k == 0 && at.first[k] < 0);
       }
     }
   }
@@ -232,6 +242,7 @@ struct LaneSum {
 template <int WARPS>
 struct CtaSum {
   static constexpr int FLOATS = 4 * WARPS;
+  static_assert(WARPS % 4 == 0, "each of the buffers starts at 16 bytes");
   // Two of WARPS for single sums, in turn, and one for pairs: a thread writes to one of them again only behind another
   // barrier, which all pass when they have read it (pairs are never summed twice without single sums between).
   float* buffer;
@@ -269,20 +280,39 @@ struct CtaSum {
   }
 };
 
-// A row's values become xhat; rstd is returned.  lead: one of the row's values.  Sums are taken of x - lead: a row of
-// equal values comes out as zeros, an offset common to the row costs no accuracy, and lead is never further from the
-// mean than sqrt(C) standard deviations.
-template <typename T, Layout LAYOUT, typename Sum>
-__device__ __forceinline__ float normalise(const Lane<T, LAYOUT>& at, float2* v, float lead, const LayerNorm& p, Sum& sum) {
-  constexpr int H = LN_VALUES / 2;
+template <int H>
+__device__ __forceinline__ float2 tree(float2* v) {  // (v is used up)
 #pragma unroll
-  for (int i = 0; i < H; ++i) v[i] = LAYOUT == FULL ? add2(v[i], both(-lead)) : fma2(both(-lead), at.on[i], v[i]);
-  const float2 a = add2(add2(v[0], v[1]), add2(v[2], v[3]));
-  const float mean = sum(a.x + a.y) * p.inv_C;
+  for (int o = H / 2; o > 0; o >>= 1)
 #pragma unroll
-  for (int i = 0; i < H; ++i) v[i] = LAYOUT == FULL ? add2(v[i], both(-mean)) : fma2(both(-mean), at.on[i], v[i]);
-  const float2 q = add2(fma2(v[0], v[0], mul2(v[1], v[1])), fma2(v[2], v[2], mul2(v[3], v[3])));
-  const float rstd = rsqrtf(fmaf(sum(q.x + q.y), p.inv_C, p.eps));
+    for (int i = 0; i < o; ++i) v[i] = add2(v[i], v[i + o]);
+  return v[0];
+}
+// A row's values become xhat; rstd is returned.  lead: one of the row's values, which those that are not the row's hold
+// too.  Sums are taken of x - lead: a row of equal values comes out as zeros, an offset common to the row costs no
+// accuracy, and lead is never further from the mean than sqrt(C) standard deviations.  The values that are not the
+// row's are then -mean, whose squares are taken off their lane's sum (its error, `off` units in the last place of
+// mean^2, is below that of the row's own sum, which holds mean^2 once: lead is one of its values).
+template <typename T, Layout LAYOUT, int N, typename Sum>
+__device__ __forceinline__ float normalise(const Lane<T, LAYOUT, N>& at, float2* v, float lead, const LayerNorm& p, Sum& sum) {
+  constexpr int H = N / 2;
+  float2 a[H];
+#pragma unroll
+  for (int i = 0; i < H; ++i) a[i] = v[i] = add2(v[i], both(-lead));
+  const float2 s = tree<H>(a);
+  const float mean = sum(s.x + s.y) * p.inv_C;
+#pragma unroll
+  for (int i = 0; i < H; ++i) v[i] = add2(v[i], both(-mean));
+  float2 q0 = mul2(v[0], v[0]), q1 = mul2(v[1], v[1]);
+#pragma unroll
+  for (int i = 2; i < H; i += 2) {
+    q0 = fma2(v[i], v[i], q0);
+    q1 = fma2(v[i + 1], v[i + 1], q1);
+  }
+  const float2 qq = add2(q0, q1);
+  float q = qq.x + qq.y;
+  if (LAYOUT != FULL) q = at.some ? fmaf(-at.off * mean, mean, q) : 0.f;
+  const float rstd = rsqrtf(fmaf(sum(q), p.inv_C, p.eps));
 #pragma unroll
   for (int i = 0; i < H; ++i) v[i] = mul2(v[i], both(rstd));
   return rstd;
@@ -296,59 +326,157 @@ __device__ __forceinline__ float reciprocal(float a) {
 
 // s = 1 / (1 + exp(-z)).  Both functions are the hardware's (exp2 within 2 units in the last place of an argument that
 // rounds by |z| units, which count where exp(-z) outweighs the 1; the reciprocal within 1), and two values share a
-// reciprocal of their product: 12 of them instead of 16 for a lane's 8 values, whose pipe bounds 16-bit rows.  Values
+// reciprocal of their product: 12 of them instead of 16 for 8 values, whose pipe bounds 16-bit rows.  Values
 // whose product could overflow, or that are not numbers, are taken one by one.
-__device__ __forceinline__ void sigmoid(const float2* z, float2* s) {
-  constexpr int H = LN_VALUES / 2;
-  float2 a[H];
+__device__ __forceinline__ void sigmoid(const float2* z, float2* s) {  // of 8 values
+  float2 a[4];
 #pragma unroll
-  for (int i = 0; i < H; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const float2 e = mul2(z[i], both(-1.44269504f));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a[i].x) : "f"(e.x));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a[i].y) : "f"(e.y));
     a[i] = add2(a[i], both(1.f));
   }
-  const float2 t = add2(add2(a[0], a[1]), add2(a[2], a[3]));
-  if (t.x + t.y <= 0x1p62f) {
+  const float2 top = add2(add2(a[0], a[1]), add2(a[2], a[3]));
+  if (top.x + top.y <= 0x1p62f) {
 #pragma unroll
-    for (int i = 0; i < H; ++i) s[i] = mul2(both(reciprocal(a[i].x * a[i].y)), make_float2(a[i].y, a[i].x));
+    for (int i = 0; i < 4; ++i) s[i] = mul2(both(reciprocal(a[i].x * a[i].y)), make_float2(a[i].y, a[i].x));
   } else {
 #pragma unroll
-    for (int i = 0; i < H; ++i) s[i] = make_float2(reciprocal(a[i].x), reciprocal(a[i].y));
+    for (int i = 0; i < 4; ++i) s[i] = make_float2(reciprocal(a[i].x), reciprocal(a[i].y));
   }
 }
 
-// lanes of a row: 8 channels each (`head`: and the values before its start); a power of two up to a warp, then whole
+// lanes of a row: N channels each (`head`: and the values before its start); a power of two up to a warp, then whole
 // warps
-inline int row_lanes(int C, int head) {
-  const int need = (C + head + LN_VALUES - 1) / LN_VALUES;
+inline int row_lanes(int N, int C, int head) {
+  const int need = (C + head + N - 1) / N;
   if (need > 32) return (need + 31) / 32 * 32;
-  int l = 4;
+  int l = 2;
   while (l < need) l *= 2;
   return l;
 }
 
-// f(std::integral_constant<int, lanes>) for rows of up to 32 lanes
-template <typename F>
-int with_lanes(int lanes, F&& f) {
-  switch (lanes) {
-    case 4: return f(std::integral_constant<int, 4>{});
-    case 8: return f(std::integral_constant<int, 8>{});
-    case 16: return f(std::integral_constant<int, 16>{});
-    default: return f(std::integral_constant<int, 32>{});
-  }
+// (volatile: not kept in registers over a loop)
+__device__ __forceinline__ float4 load_shared(const float4* a) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"((uint32_t)__cvta_generic_to_shared(a))
+               : "memory");
+  return v;
 }
+
+// A lane's weights and biases: in registers, or in shared memory of its own (16 bytes of every lane side by side).
+template <int N, bool SHARED>
+struct Params {
+  float2 w_[SHARED ? 1 : N / 2], b_[SHARED ? 1 : N / 2];
+  float4* at_;
+  int lanes_;
+  static constexpr int BYTES = 2 * N * 4;  // of a lane
+  template <typename At>
+  __device__ __forceinline__ Params(const At& at, const LayerNorm& p, void* shared, int lane, int lanes)
+      : at_(static_cast<float4*>(shared) + lane), lanes_(lanes) {
+    if constexpr (SHARED) {
+      float2 t[N / 2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        at.param(h ? p.b : p.w, p.param_f32, h ? 0.f : 1.f, p.C, t);
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i)
+          at_[(h * (N / 4) + i) * lanes] = make_float4(t[2 * i].x, t[2 * i].y, t[2 * i + 1].x, t[2 * i + 1].y);
+      }
+    } else {
+      at.param(p.w, p.param_f32, 1.f, p.C, w_);
+      at.param(p.b, p.param_f32, 0.f, p.C, b_);
+    }
+  }
+  // of values 8 c .. 8 c + 7
+  __device__ __forceinline__ void get(int h, int c, float2* v) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (SHARED) {
+        const float4 t = load_shared(at_ + (h * (N / 4) + 2 * c + i) * lanes_);
+        v[2 * i] = make_float2(t.x, t.y), v[2 * i + 1] = make_float2(t.z, t.w);
+      } else {
+        v[2 * i] = (h ? b_ : w_)[4 * c + 2 * i], v[2 * i + 1] = (h ? b_ : w_)[4 * c + 2 * i + 1];
+      }
+    }
+  }
+  __device__ __forceinline__ void weight(int c, float2* v) const { get(0, c, v); }
+  __device__ __forceinline__ void bias(int c, float2* v) const { get(1, c, v); }
+};
+
+// A lane's sums of the parameters' gradients, kept the same way.
+template <int N, bool SHARED>
+struct Sums {
+  float2 v_[2][SHARED ? 1 : N / 2];
+  float4* at_;
+  int lanes_;
+  static constexpr int BYTES = 2 * N * 4;  // of a lane
+  __device__ __forceinline__ Sums(void* shared, int lane, int lanes) : at_(static_cast<float4*>(shared) + lane), lanes_(lanes) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (SHARED)
+        at_[i * lanes] = make_float4(0.f, 0.f, 0.f, 0.f);
+      else
+        v_[0][i] = v_[1][i] = both(0.f);
+    }
+  }
+  // values 8 c .. 8 c + 7 of g xhat and of g
+  __device__ __forceinline__ void add(int c, const float2* g, const float2* xhat) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      if constexpr (SHARED) {
+        float4 *const w = at_ + (2 * c + i / 2) * lanes_, *const b = w + (N / 4) * lanes_;
+        float4 t = *w, u = *b;
+        const float2 t0 = fma2(g[i], xhat[i], make_float2(t.x, t.y)), t1 = fma2(g[i + 1], xhat[i + 1], make_float2(t.z, t.w));
+        const float2 u0 = add2(g[i], make_float2(u.x, u.y)), u1 = add2(g[i + 1], make_float2(u.z, u.w));
+        *w = make_float4(t0.x, t0.y, t1.x, t1.y);
+        *b = make_float4(u0.x, u0.y, u1.x, u1.y);
+      } else {
+#pragma unroll
+        for (int k = i; k < i + 2; ++k) {
+          v_[0][4 * c + k] = fma2(g[k], xhat[k], v_[0][4 * c + k]);
+          v_[1][4 * c + k] = add2(g[k], v_[1][4 * c + k]);
+        }
+      }
+    }
+  }
+  // the sums of g xhat (which: 0) and g (1), value j
+  __device__ __forceinline__ float get(int which, int j) const {
+    if constexpr (SHARED) {
+      const float4 t = at_[(which * (N / 4) + j / 4) * lanes_];
+      return j % 4 == 0 ? t.x : (j % 4 == 1 ? t.y : (j % 4 == 2 ? t.z : t.w));
+    } else {
+      return j & 1 ? v_[which][j / 2].y : v_[which][j / 2].x;
+    }
+  }
+};
 
 struct RowPlan {
   Layout layout;
-  int lanes;
+  int values, lanes;  // of a lane, of a row
 };
 struct Operand {
   const void* at;  // null: none
   int64_t stride;
 };
 
-template <typename T>
+// Values of a lane.  Rows of up to 32 lanes: two pieces, so that 32 bytes of each row are in flight for a lane and the
+// row's sums take few steps; but one piece of 16 bits in the backward where a row starts anywhere (300 007 rows of 97
+// 80 us; with two, whose masks leave too few registers, 102), and 8 single values.  Four pieces of fp32 where a row then
+// still fits a warp, and where it takes a CTA (gradients of 20 011 rows of 2048 87 us, 99 with two).
+constexpr int LN_WIDE = 16, LN_APART = 8;
+template <typename T, bool GRAD>
+constexpr int narrow_values(Layout layout) {
+  return sizeof(T) == 4 || layout == APART || (GRAD && layout == PIECES) ? 8 : 16;
+}
+
+// lanes of more than a warp
+constexpr bool may_be_wide(Layout layout, int values) { return layout == APART || values == LN_WIDE; }
+
+template <typename T, bool GRAD>
 RowPlan row_plan(int64_t n, int C, std::initializer_list<Operand> operands) {
   constexpr int V = 16 / sizeof(T);
   bool alike = true, start = true, apart = true;
@@ -360,11 +488,17 @@ RowPlan row_plan(int64_t n, int C, std::initializer_list<Operand> operands) {
     start = start && (reinterpret_cast<uintptr_t>(o.at) & 15) == 0 && o.stride % V == 0;
     apart = apart && (o.stride > 0 || n <= 1);
   }
-  const int lanes = row_lanes(C, start ? 0 : V - 1);
-  if (start && lanes * LN_VALUES == C) return {FULL, lanes};
+  const int head = start ? 0 : V - 1;
+  auto plan = [&](Layout layout) {
+    int values = narrow_values<T, GRAD>(layout);
+    if (row_lanes(values, C, head) > 32) values = LN_WIDE;
+    return RowPlan{layout, values, row_lanes(values, C, head)};
+  };
+  const RowPlan full = plan(FULL), pieces = plan(PIECES);
+  if (start && full.lanes * full.values == C) return full;
   // (rows that repeat: a neighbour's values need not lie inside the tensor)
-  if (!alike || !apart || C <= V || lanes > 1024) return {APART, row_lanes(C, 0)};
-  return {PIECES, lanes};
+  const bool any = alike && apart && C > V && pieces.lanes * pieces.values <= MACE_LAYER_NORM_MAX_CHANNELS;
+  return any ? pieces : RowPlan{APART, LN_APART, row_lanes(LN_APART, C, 0)};
 }
 
 // values between the 16-byte address before row r and the row
@@ -381,14 +515,35 @@ inline bool bad_rows(int32_t dtype, int32_t param_dtype, int64_t n, int32_t C, f
          (activation != MACE_ACT_NONE && activation != MACE_ACT_SILU);
 }
 
-// f(layout) with the layout as std::integral_constant
-template <typename F>
-int with_layout(Layout layout, F&& f) {
-  switch (layout) {
-    case FULL: return f(std::integral_constant<Layout, FULL>{});
-    case PIECES: return f(std::integral_constant<Layout, PIECES>{});
-    default: return f(std::integral_constant<Layout, APART>{});
+// f(layout, values) of a plan as constants
+template <typename T, bool GRAD, typename F>
+int with_plan(const RowPlan& plan, F&& f) {
+  auto go = [&](auto layout) {
+    constexpr int narrow = narrow_values<T, GRAD>(decltype(layout)::value);
+    if constexpr (decltype(layout)::value != APART && narrow != LN_WIDE)
+      if (plan.values == LN_WIDE) return f(layout, std::integral_constant<int, LN_WIDE>{});
+    return f(layout, std::integral_constant<int, narrow>{});
+  };
+  switch (plan.layout) {
+    case FULL: return go(std::integral_constant<Layout, FULL>{});
+    case PIECES: return go(std::integral_constant<Layout, PIECES>{});
+    default: return go(std::integral_constant<Layout, APART>{});
   }
+}
+
+// f(lanes) of a row of up to 32 lanes; one whose lanes have more values than narrow ones has a whole warp
+template <bool WARP, typename F>
+int with_lanes(int lanes, F&& f) {
+  if constexpr (!WARP) {
+    switch (lanes) {
+      case 2: return f(std::integral_constant<int, 2>{});
+      case 4: return f(std::integral_constant<int, 4>{});
+      case 8: return f(std::integral_constant<int, 8>{});
+      case 16: return f(std::integral_constant<int, 16>{});
+      default: break;
+    }
+  }
+  return f(std::integral_constant<int, 32>{});
 }
 
 }  // namespace mace

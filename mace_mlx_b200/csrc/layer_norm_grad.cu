@@ -13,41 +13,53 @@ namespace mace {
 namespace {
 
 // xhat and dy of a row to dx (in g); the sums of dw and db move on
-template <bool SILU, typename Sum>
-__device__ __forceinline__ void row_grad(const float2* xhat, float2* g, const float2* w, const float2* b, float rstd,
-                                         float inv_C, float2* dw, float2* db, Sum& sum) {
-  constexpr int H = LN_VALUES / 2;
-  if (SILU) {
-    float2 z[H], s[H];
-#pragma unroll
-    for (int i = 0; i < H; ++i) z[i] = fma2(xhat[i], w[i], b[i]);
-    sigmoid(z, s);
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-      const float2 rest = fma2(s[i], both(-1.f), both(1.f));
-      g[i] = mul2(g[i], mul2(s[i], fma2(z[i], rest, both(1.f))));
-    }
-  }
+template <bool SILU, int N, bool SP, bool SA, typename Sum>
+__device__ __forceinline__ void row_grad(const float2* xhat, float2* grad, const Params<N, SP>& params, float rstd,
+                                         float inv_C, Sums<N, SA>& acc, Sum& sum) {
   float2 c1 = both(0.f), c2 = both(0.f);
 #pragma unroll
-  for (int i = 0; i < H; ++i) {
-    dw[i] = fma2(g[i], xhat[i], dw[i]);
-    db[i] = add2(db[i], g[i]);
-    g[i] = mul2(g[i], w[i]);
-    c1 = add2(c1, g[i]);
-    c2 = fma2(g[i], xhat[i], c2);
+  for (int c = 0; c < N / 8; ++c) {
+    const float2* const xh = xhat + 4 * c;
+    float2 w[4], *const g = grad + 4 * c;
+    params.weight(c, w);
+    if (SILU) {
+      float2 z[4], s[4];
+      params.bias(c, z);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = fma2(xh[i], w[i], z[i]);
+      sigmoid(z, s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 rest = fma2(s[i], both(-1.f), both(1.f));
+        g[i] = mul2(g[i], mul2(s[i], fma2(z[i], rest, both(1.f))));
+      }
+    }
+    acc.add(c, g, xh);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      g[i] = mul2(g[i], w[i]);
+      c1 = add2(c1, g[i]);
+      c2 = fma2(g[i], xh[i], c2);
+    }
   }
   const float2 c = sum(make_float2(c1.x + c1.y, c2.x + c2.y));
   const float2 m1 = both(-c.x * inv_C), m2 = both(-c.y * inv_C);
 #pragma unroll
-  for (int i = 0; i < H; ++i) g[i] = mul2(both(rstd), fma2(xhat[i], m2, add2(g[i], m1)));
+  for (int i = 0; i < N / 2; ++i) grad[i] = mul2(both(rstd), fma2(xhat[i], m2, add2(grad[i], m1)));
 }
 
+// Where a lane keeps its parameters and the sums of their gradients.  Rows of up to 32 lanes: the parameters in shared
+// memory, the sums in registers.  Wider ones, whose CTAs the barriers of their sums keep waiting: both in registers
+// where rows are whole pieces; else, with the masks, in shared memory, so that four CTAs' threads fit an SM (50 007 rows
+// of 1000 105 us, 133 in registers).  (CTAs of more than 256 threads have an SM to themselves.)
+template <Layout LAYOUT, int MOST>
+constexpr bool LN_WIDE_SHARED = LAYOUT != FULL && MOST == 256;
+
 // Rows of up to 32 lanes: a CTA takes a share of neighbouring rows.  The next row of each lane group is in flight.
-template <typename T, Layout LAYOUT, int L, bool SILU>
+template <typename T, Layout LAYOUT, int N, int L, bool SILU>
 __global__ void __launch_bounds__(LN_THREADS, 2) k_layer_norm_grad(LayerNorm p) {
-  constexpr int GROUPS = LN_THREADS / L, WIDTH = L * LN_VALUES, H = LN_VALUES / 2;
-  __shared__ float sums[GROUPS][2][WIDTH];
+  constexpr int GROUPS = LN_THREADS / L, WIDTH = L * N, H = N / 2;
+  __shared__ float4 own[2 * N * LN_THREADS / 4];  // the lanes' parameters, in the end the sums
   const int lane = threadIdx.x % L, sub = (threadIdx.x & 31) / L, group = threadIdx.x / L;
   pdl_wait();
   const int64_t begin = blockIdx.x * p.share;
@@ -56,13 +68,10 @@ __global__ void __launch_bounds__(LN_THREADS, 2) k_layer_norm_grad(LayerNorm p) 
   const T* x = static_cast<const T*>(p.x) + r * p.xs;
   const T* dy = static_cast<const T*>(p.dy) + r * p.ds;
   T* dx = static_cast<T*>(p.y) + r * p.ys;
-  const Lane<T, LAYOUT> at(lane, L, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
-  float2 w[H], b[H], dw[H], db[H];
-  at.param(p.w, p.param_f32, 1.f, p.C, w);
-  at.param(p.b, p.param_f32, 0.f, p.C, b);
-#pragma unroll
-  for (int i = 0; i < H; ++i) dw[i] = db[i] = both(0.f);
-  Part<T, LAYOUT> nx, nd;
+  const Lane<T, LAYOUT, N> at(lane, L, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
+  const Params<N, true> params(at, p, own, threadIdx.x, LN_THREADS);
+  Sums<N, false> acc(nullptr, threadIdx.x, LN_THREADS);
+  Part<T, LAYOUT, N> nx, nd;
   nx.zero();
   nd.zero();
   if (r < end) {
@@ -72,10 +81,9 @@ __global__ void __launch_bounds__(LN_THREADS, 2) k_layer_norm_grad(LayerNorm p) 
   LaneSum<L> sum;
   for (; r - sub < end; r += GROUPS) {
     float2 v[H], g[H];
-    nx.values(at, v);
-    nd.values(at, g);
-    // (PIECES: the second piece is the row's whatever the first one holds)
-    const float lead = __shfl_sync(0xffffffffu, v[0].x, LAYOUT == PIECES ? 1 : 0, L);
+    const float lead = nx.template lead<L>();
+    nx.values(at, lead, v);
+    nd.values(at, 0.f, g);
     x += GROUPS * p.xs;
     dy += GROUPS * p.ds;
     if (r + GROUPS < end) {
@@ -86,16 +94,18 @@ __global__ void __launch_bounds__(LN_THREADS, 2) k_layer_norm_grad(LayerNorm p) 
     if (r >= end)  // no row
 #pragma unroll
       for (int i = 0; i < H; ++i) v[i] = g[i] = both(0.f);
-    row_grad<SILU>(v, g, w, b, rstd, p.inv_C, dw, db, sum);
-    if (p.y && r < end) Part<T, LAYOUT>::store(at, dx, g);
+    row_grad<SILU>(v, g, params, rstd, p.inv_C, acc, sum);
+    if (p.y && r < end) Part<T, LAYOUT, N>::store(at, dx, g);
     dx += GROUPS * p.ys;
   }
   if (!p.part) return;
+  float* const sums = reinterpret_cast<float*>(own);  // (GROUPS, 2, WIDTH)
+  __syncthreads();
 #pragma unroll
-  for (int j = 0; j < LN_VALUES; ++j)
+  for (int j = 0; j < N; ++j)
     if (at.in(j, p.C)) {
-      sums[group][0][at.at(j)] = j & 1 ? dw[j / 2].y : dw[j / 2].x;
-      sums[group][1][at.at(j)] = j & 1 ? db[j / 2].y : db[j / 2].x;
+      sums[group * 2 * WIDTH + at.at(j)] = acc.get(0, j);
+      sums[(group * 2 + 1) * WIDTH + at.at(j)] = acc.get(1, j);
     }
   __syncthreads();
   float* const out = p.part + blockIdx.x * (int64_t)p.pitch;
@@ -103,16 +113,18 @@ __global__ void __launch_bounds__(LN_THREADS, 2) k_layer_norm_grad(LayerNorm p) 
     const int which = k >= p.C, c = k - which * p.C;
     float t = 0.f;
 #pragma unroll 8
-    for (int i = 0; i < GROUPS; ++i) t += sums[i][which][c];
+    for (int i = 0; i < GROUPS; ++i) t += sums[(i * 2 + which) * WIDTH + c];
     out[k] = t;
   }
 }
 
 // wider rows: a CTA takes every LN_TURN-th row of LN_TURN shares, one at a time
-template <typename T, Layout LAYOUT, bool SILU, int MOST>
-__global__ void __launch_bounds__(MOST) k_layer_norm_grad_wide(LayerNorm p) {
-  constexpr int H = LN_VALUES / 2;
+template <typename T, Layout LAYOUT, int N, bool SILU, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) k_layer_norm_grad_wide(LayerNorm p) {
+  constexpr int H = N / 2;
+  constexpr bool SHARED = LN_WIDE_SHARED<LAYOUT, MOST>;
   __shared__ __align__(16) float sums[CtaSum<MOST / 32>::FLOATS];
+  extern __shared__ float4 own[];
   pdl_wait();
   const int64_t begin = (blockIdx.x / LN_TURN) * LN_TURN * p.share;
   const uint32_t end = (uint32_t)min(p.n, begin + LN_TURN * p.share);
@@ -120,13 +132,10 @@ __global__ void __launch_bounds__(MOST) k_layer_norm_grad_wide(LayerNorm p) {
   const T* x = static_cast<const T*>(p.x) + r * p.xs;
   const T* dy = static_cast<const T*>(p.dy) + r * p.ds;
   T* dx = static_cast<T*>(p.y) + r * p.ys;
-  const Lane<T, LAYOUT> at(threadIdx.x, blockDim.x, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
-  float2 w[H], b[H], dw[H], db[H];
-  at.param(p.w, p.param_f32, 1.f, p.C, w);
-  at.param(p.b, p.param_f32, 0.f, p.C, b);
-#pragma unroll
-  for (int i = 0; i < H; ++i) dw[i] = db[i] = both(0.f);
-  Part<T, LAYOUT> nx, nd;
+  const Lane<T, LAYOUT, N> at(threadIdx.x, blockDim.x, p.C, LAYOUT == PIECES ? row_head<T>(p.x, p.xs, r) : 0);
+  const Params<N, SHARED> params(at, p, own, threadIdx.x, blockDim.x);
+  Sums<N, SHARED> acc(own + blockDim.x * 2 * N / 4, threadIdx.x, blockDim.x);
+  Part<T, LAYOUT, N> nx, nd;
   nx.zero();
   nd.zero();
   nx.load(at, x, r - LN_TURN < p.inner);
@@ -136,8 +145,8 @@ __global__ void __launch_bounds__(MOST) k_layer_norm_grad_wide(LayerNorm p) {
   for (; r < end; r += LN_TURN) {
     float2 v[H], g[H];
     const float lead = ahead;
-    nx.values(at, v);
-    nd.values(at, g);
+    nx.values(at, lead, v);
+    nd.values(at, 0.f, g);
     x += LN_TURN * p.xs;
     dy += LN_TURN * p.ds;
     if (r + LN_TURN < end) {
@@ -146,17 +155,17 @@ __global__ void __launch_bounds__(MOST) k_layer_norm_grad_wide(LayerNorm p) {
       ahead = to_f32(load_in(x));
     }
     const float rstd = normalise(at, v, lead, p, sum);
-    row_grad<SILU>(v, g, w, b, rstd, p.inv_C, dw, db, sum);
-    if (p.y) Part<T, LAYOUT>::store(at, dx, g);
+    row_grad<SILU>(v, g, params, rstd, p.inv_C, acc, sum);
+    if (p.y) Part<T, LAYOUT, N>::store(at, dx, g);
     dx += LN_TURN * p.ys;
   }
   if (!p.part) return;
   float* const out = p.part + blockIdx.x * (int64_t)p.pitch;
 #pragma unroll
-  for (int j = 0; j < LN_VALUES; ++j)
+  for (int j = 0; j < N; ++j)
     if (at.in(j, p.C)) {
-      out[at.at(j)] = j & 1 ? dw[j / 2].y : dw[j / 2].x;
-      out[p.C + at.at(j)] = j & 1 ? db[j / 2].y : db[j / 2].x;
+      out[at.at(j)] = acc.get(0, j);
+      out[p.C + at.at(j)] = acc.get(1, j);
     }
 }
 
@@ -195,30 +204,46 @@ __global__ void __launch_bounds__(1024) k_layer_norm_join(LayerNorm p) {
 }
 
 // Rows of a CTA: enough CTAs to fill the GPU, and at most 256 rows for a lane, so that a sum's error stays that of a
-// few hundred terms.  From n and C alone.
-int64_t grad_share(int64_t n, int C) {
-  const int lanes = row_lanes(C, 0);
-  const int64_t rows = lanes > 32 ? 1 : LN_THREADS / lanes;  // at once
-  const int64_t ctas = lanes > 32 ? LN_SMS * std::max(1, 1024 / lanes) : LN_SMS * 4;
-  int64_t share = std::max((n + ctas - 1) / ctas, rows);
-  share = std::min(share, rows * 256);
-  return (share + rows - 1) / rows * rows;
+// few hundred terms.  From n, C and whether a row has more than 32 lanes (which its alignment decides too).
+int64_t grad_share(int64_t n, int C, bool wide) {
+  if (wide) {
+    const int64_t ctas = LN_SMS * std::max(1, 512 / row_lanes(LN_WIDE, C, 0));
+    return std::min<int64_t>(std::max<int64_t>((n + ctas - 1) / ctas, 1), 256);
+  }
+  const int64_t rows = LN_THREADS / std::min(row_lanes(8, C, 0), 32), ctas = LN_SMS * 4;  // rows at once
+  const int64_t share = std::min(std::max((n + ctas - 1) / ctas, rows), rows * 256);
+  return (share + LN_TURN - 1) / LN_TURN * LN_TURN;
 }
-int64_t grad_shares(int64_t n, int64_t share, bool wide) {
+int64_t grad_shares(int64_t n, int C, bool wide) {
+  const int64_t share = grad_share(n, C, wide);
   if (!wide) return (n + share - 1) / share;
   const int64_t full = n / (LN_TURN * share);
   return full * LN_TURN + std::min<int64_t>(n - full * LN_TURN * share, LN_TURN);
 }
 int grad_pitch(int C) { return (2 * C + 3) & ~3; }
 
-template <typename T, Layout LAYOUT, bool SILU>
+template <typename T, Layout LAYOUT, int N, bool SILU>
 int backward(const LayerNorm& p, int lanes, cudaStream_t s) {
   const dim3 grid((unsigned)p.shares);
-  if (lanes > 32)
-    return launch("layer_norm_grad", lanes <= 256 ? k_layer_norm_grad_wide<T, LAYOUT, SILU, 256> : k_layer_norm_grad_wide<T, LAYOUT, SILU, 1024>,
-                  grid, lanes, 0, s, p);
-  return with_lanes(lanes, [&](auto l) {
-    return launch("layer_norm_grad", k_layer_norm_grad<T, LAYOUT, decltype(l)::value, SILU>, grid, LN_THREADS, 0, s, p);
+  if constexpr (may_be_wide(LAYOUT, N)) {
+    if (lanes > 256)
+      return launch("layer_norm_grad", k_layer_norm_grad_wide<T, LAYOUT, N, SILU, MACE_LAYER_NORM_MAX_CHANNELS / N>, grid, lanes,
+                    0, s, p);
+    if (lanes > 32) {
+      const auto kernel = k_layer_norm_grad_wide<T, LAYOUT, N, SILU, 256>;
+      constexpr int OF_LANE = LN_WIDE_SHARED<LAYOUT, 256> ? Params<N, true>::BYTES + Sums<N, true>::BYTES : 0;
+      static bool attr_set[64] = {};  // per device: the attribute call is slow on the host
+      int dev = 0;
+      MACE_CUDA_TRY(cudaGetDevice(&dev));
+      if (OF_LANE * 256 > 49152 && (dev >= 64 || !attr_set[dev])) {
+        MACE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, OF_LANE * 256));
+        if (dev < 64) attr_set[dev] = true;
+      }
+      return launch("layer_norm_grad", kernel, grid, lanes, lanes * OF_LANE, s, p);
+    }
+  }
+  return with_lanes<(N > narrow_values<T, true>(LAYOUT))>(lanes, [&](auto l) {
+    return launch("layer_norm_grad", k_layer_norm_grad<T, LAYOUT, N, decltype(l)::value, SILU>, grid, LN_THREADS, 0, s, p);
   });
 }
 
@@ -231,8 +256,11 @@ using namespace mace;
 extern "C" int mace_layer_norm_grad_workspace(int64_t n, int32_t C, int64_t* bytes) {
   if (n < 0 || n > INT32_MAX || C < 1 || C > MACE_LAYER_NORM_MAX_CHANNELS || !bytes)
     return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad_workspace: bad arguments");
-  const int64_t share = grad_share(n, C);
-  *bytes = std::max(grad_shares(n, share, false), grad_shares(n, share, true)) * grad_pitch(C) * 4;
+  // (rows of these widths take a warp or a CTA, by their alignment)
+  int64_t shares = 0;
+  if (C <= 32 * LN_WIDE) shares = grad_shares(n, C, false);
+  if (C > 32 * LN_APART) shares = std::max(shares, grad_shares(n, C, true));
+  *bytes = shares * grad_pitch(C) * 4;
   return MACE_OK;
 }
 
@@ -253,18 +281,19 @@ extern "C" int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t xs, co
   LayerNorm p{};
   p.x = x, p.xs = n > 1 ? xs : 0, p.dy = dy, p.ds = n > 1 ? ds : 0, p.w = weight, p.b = bias;
   p.param_f32 = param_dtype == MACE_F32, p.n = n, p.C = C, p.eps = eps, p.inv_C = 1.f / C, p.inner = inner_rows(n), p.y = dx, p.ys = n > 1 ? dxs : 0;
-  p.share = grad_share(n, C), p.part = params ? static_cast<float*>(ws) : nullptr;
+  p.part = params ? static_cast<float*>(ws) : nullptr;
   p.pitch = grad_pitch(C), p.dw = dweight, p.db = dbias;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (n > 0 && (params || dx)) {
     auto go = [&](auto t) {
       using T = decltype(t);
-      const RowPlan plan = row_plan<T>(n, C, {{x, p.xs}, {dy, p.ds}, {dx, p.ys}});
-      p.shares = grad_shares(n, p.share, plan.lanes > 32);
-      return with_layout(plan.layout, [&](auto layout) {
+      const RowPlan plan = row_plan<T, true>(n, C, {{x, p.xs}, {dy, p.ds}, {dx, p.ys}});
+      p.share = grad_share(n, C, plan.lanes > 32), p.shares = grad_shares(n, C, plan.lanes > 32);
+      return with_plan<T, true>(plan, [&](auto layout, auto values) {
         constexpr Layout LAYOUT = decltype(layout)::value;
-        return activation == MACE_ACT_SILU ? backward<T, LAYOUT, true>(p, plan.lanes, s)
-                                           : backward<T, LAYOUT, false>(p, plan.lanes, s);
+        constexpr int N = decltype(values)::value;
+        return activation == MACE_ACT_SILU ? backward<T, LAYOUT, N, true>(p, plan.lanes, s)
+                                           : backward<T, LAYOUT, N, false>(p, plan.lanes, s);
       });
     };
     const int rc = dtype == MACE_F32 ? go(float{}) : go(bf16{});
