@@ -30,6 +30,7 @@ constexpr uint8_t IN_BF16 = 1, OUT_BF16 = 2, OUT_PIECES = 4;  // OUT_PIECES: a p
 template <int CAP>
 struct GradList {
   int count;
+  int elsewhere;  // some results go to other tensors
   uint32_t first[CAP + 1];  // first tile of a tensor
   int64_t size[CAP];
   const void* in[CAP];
@@ -51,17 +52,33 @@ __device__ __forceinline__ int tensor_of(const GradList<CAP>& list, uint32_t til
   return lo;
 }
 
-// this thread's pieces of a tile of tensor t: f(u, first element, whole piece)
+// A tile of a tensor: its first piece's first value (which may lie before the tensor), and whether all of its pieces lie
+// inside.
+struct Tile {
+  int64_t e;
+  bool whole;
+};
+template <typename T>
+__device__ __forceinline__ Tile tile_of(const void* in, int64_t size, uint32_t nth) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t e = (int64_t)nth * (GN_TILE * V) - (int64_t)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+  return {e, e >= 0 && e + GN_TILE * V <= size};
+}
+
+// One of this thread's pieces: its values inside the tensor are [max(e, 0), min(e + V, size)).
 template <typename T>
 struct Piece {
   static constexpr int V = 16 / sizeof(T);
   uint4 raw;
-  int64_t e;  // first element, which may lie before the tensor; its elements inside are [max(e, 0), min(e + V, size))
-  __device__ __forceinline__ bool whole(int64_t size) const { return e >= 0 && e + V <= size; }
-  __device__ __forceinline__ void load(const T* in, int64_t size, int64_t piece) {
-    e = piece * V - (int64_t)((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+  __device__ __forceinline__ void load(const T* in, const Tile& tile, int64_t size, int u) {
+    const int at = (u * GN_THREADS + (int)threadIdx.x) * V;
+    if (tile.whole) {
+      raw = load_in(reinterpret_cast<const uint4*>(in + tile.e + at));
+      return;
+    }
+    const int64_t e = tile.e + at;
     raw = make_uint4(0, 0, 0, 0);
-    if (whole(size)) {
+    if (e >= 0 && e + V <= size) {
       raw = load_in(reinterpret_cast<const uint4*>(in + e));
     } else {
       T t[V];
@@ -94,17 +111,35 @@ __device__ __forceinline__ double cta_sum(double a, double* buffer) {
   return t;
 }
 
-template <typename T>
-__device__ __forceinline__ void add_squares(const void* in, int64_t size, int64_t piece0, double* acc) {
+// 16-bit values without the conversion's pipe (16 lanes a cycle of an SM, 30 us of the 22 that 71M values' bytes take):
+// their bits, moved to where fp64 has them, are the value times 2^(127 - 1023) for zeros and subnormals too.  Infinities
+// and NaN come out as values from 2^128 on.
+constexpr double GN_BIAS = 0x1p896;
+constexpr double GN_SUSPECT = 0x1p255;  // a sum that may hold one
+
+template <typename T, bool EXACT>
+__device__ __forceinline__ void add_squares(const void* in, int64_t size, uint32_t nth, double* acc) {
+  const Tile tile = tile_of<T>(in, size, nth);
   Piece<T> p[GN_UNROLL];
 #pragma unroll
-  for (int u = 0; u < GN_UNROLL; ++u) p[u].load(static_cast<const T*>(in), size, piece0 + u * GN_THREADS);
+  for (int u = 0; u < GN_UNROLL; ++u) p[u].load(static_cast<const T*>(in), tile, size, u);
 #pragma unroll
   for (int u = 0; u < GN_UNROLL; ++u) {
-    float v[Piece<T>::V];
-    p[u].values(v);
+    if constexpr (sizeof(T) == 2 && !EXACT) {
+      const uint32_t w[4] = {p[u].raw.x, p[u].raw.y, p[u].raw.z, p[u].raw.w};
 #pragma unroll
-    for (int k = 0; k < Piece<T>::V; ++k) acc[k & 3] = fma((double)v[k], (double)v[k], acc[k & 3]);
+      for (int k = 0; k < 4; ++k) {
+        const double lo = __hiloint2double((int)(w[k] << 13 & 0x0fffe000u), 0) * GN_BIAS;
+        const double hi = __hiloint2double((int)(w[k] >> 3 & 0x0fffe000u), 0) * GN_BIAS;
+        acc[2 * (k & 1)] = fma(lo, lo, acc[2 * (k & 1)]);
+        acc[2 * (k & 1) + 1] = fma(hi, hi, acc[2 * (k & 1) + 1]);
+      }
+    } else {
+      float v[Piece<T>::V];
+      p[u].values(v);
+#pragma unroll
+      for (int k = 0; k < Piece<T>::V; ++k) acc[k & 3] = fma((double)v[k], (double)v[k], acc[k & 3]);
+    }
   }
 }
 
@@ -116,22 +151,27 @@ __device__ __forceinline__ Run run_of(uint32_t tiles) {
   return {(uint32_t)((uint64_t)tiles * blockIdx.x / gridDim.x), (uint32_t)((uint64_t)tiles * (blockIdx.x + 1) / gridDim.x)};
 }
 
-template <int CAP>
-__global__ void __launch_bounds__(GN_THREADS, GN_PER_SM) k_grad_squares(const __grid_constant__ GradList<CAP> list, double* part) {
-  __shared__ double sums[GN_THREADS / 32];
-  pdl_wait();
-  const Run run = run_of(list.first[list.count]);
+template <bool EXACT, int CAP>
+__device__ __forceinline__ double sum_of_run(const GradList<CAP>& list, const Run& run, double* buffer) {
   double acc[4] = {0., 0., 0., 0.};
   int t = tensor_of(list, run.lo);
   for (uint32_t tile = run.lo; tile < run.hi; ++tile) {
     while (tile >= list.first[t + 1]) ++t;
-    const int64_t piece0 = (int64_t)(tile - list.first[t]) * GN_TILE + threadIdx.x;
     if (list.type[t] & IN_BF16)
-      add_squares<bf16>(list.in[t], list.size[t], piece0, acc);
+      add_squares<bf16, EXACT>(list.in[t], list.size[t], tile - list.first[t], acc);
     else
-      add_squares<float>(list.in[t], list.size[t], piece0, acc);
+      add_squares<float, EXACT>(list.in[t], list.size[t], tile - list.first[t], acc);
   }
-  const double total = cta_sum((acc[0] + acc[1]) + (acc[2] + acc[3]), sums);
+  return cta_sum((acc[0] + acc[1]) + (acc[2] + acc[3]), buffer);
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(GN_THREADS, GN_PER_SM) k_grad_squares(const __grid_constant__ GradList<CAP> list, double* part) {
+  __shared__ double sums[2][GN_THREADS / 32];
+  pdl_wait();
+  const Run run = run_of(list.first[list.count]);
+  double total = sum_of_run<false>(list, run, sums[0]);
+  if (!(total < GN_SUSPECT)) total = sum_of_run<true>(list, run, sums[1]);
   if (threadIdx.x == 0) part[blockIdx.x] = total;
 }
 
@@ -150,31 +190,45 @@ __global__ void __launch_bounds__(GN_THREADS) k_grad_norm(const double* part, in
   if (threadIdx.x == 0) *norm = (float)total;
 }
 
+// eight values of fp32: a whole sector where they are aligned to it
+__device__ __forceinline__ void store8(float* dst, const float* v) {
+  if ((reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                 "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+  } else {
+    store4(dst, v);
+    store4(dst + 4, v + 4);
+  }
+}
+
 template <typename TI, typename TO>
-__device__ __forceinline__ void clip_tile(const void* in, void* out, int64_t size, int64_t piece0, bool pieces,
-                                          float scale) {
+__device__ __forceinline__ void clip_tile(const void* in, void* out, int64_t size, uint32_t nth, bool pieces, float scale) {
   constexpr int V = Piece<TI>::V;
+  const Tile tile = tile_of<TI>(in, size, nth);
   Piece<TI> p[GN_UNROLL];
 #pragma unroll
-  for (int u = 0; u < GN_UNROLL; ++u) p[u].load(static_cast<const TI*>(in), size, piece0 + u * GN_THREADS);
+  for (int u = 0; u < GN_UNROLL; ++u) p[u].load(static_cast<const TI*>(in), tile, size, u);
 #pragma unroll
   for (int u = 0; u < GN_UNROLL; ++u) {
     float v[V];
     p[u].values(v);
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] *= scale;
-    TO* const dst = static_cast<TO*>(out) + p[u].e;
-    if (pieces && p[u].whole(size)) {
+    const int64_t e = tile.e + (u * GN_THREADS + (int)threadIdx.x) * V;
+    TO* const dst = static_cast<TO*>(out) + e;
+    if (pieces && (tile.whole || (e >= 0 && e + V <= size))) {
       if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2) {
         store_channels<TO, 8>(dst, v);
+      } else if constexpr (V == 8) {
+        store8(dst, v);
       } else {
         store4(dst, v);
-        if constexpr (V == 8) store4(dst + 4, v + 4);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < V; ++k)
-        if (p[u].e + k >= 0 && p[u].e + k < size) dst[k] = from_f32<TO>(v[k]);
+        if (e + k >= 0 && e + k < size) dst[k] = from_f32<TO>(v[k]);
     }
   }
 }
@@ -189,20 +243,21 @@ __global__ void __launch_bounds__(GN_THREADS, GN_PER_SM) k_grad_clip(const __gri
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
   const double factor = max_norm / (total + 1e-6);
   const float scale = factor >= 1. ? 1.f : (float)factor;  // (a factor that is NaN stays so)
+  if (scale == 1.f && !list.elsewhere) return;
   const Run run = run_of(list.first[list.count]);
   if (run.lo >= run.hi) return;
   int t = tensor_of(list, run.hi - 1);
   for (uint32_t tile = run.hi; tile-- > run.lo;) {
     while (tile < list.first[t]) --t;
     if (scale == 1.f && list.out[t] == list.in[t]) continue;
-    const int64_t piece0 = (int64_t)(tile - list.first[t]) * GN_TILE + threadIdx.x;
+    const uint32_t nth = tile - list.first[t];
     const uint8_t type = list.type[t];
     const bool pieces = type & OUT_PIECES;
     switch (type & (IN_BF16 | OUT_BF16)) {
-      case 0: clip_tile<float, float>(list.in[t], list.out[t], list.size[t], piece0, pieces, scale); break;
-      case IN_BF16: clip_tile<bf16, float>(list.in[t], list.out[t], list.size[t], piece0, pieces, scale); break;
-      case OUT_BF16: clip_tile<float, bf16>(list.in[t], list.out[t], list.size[t], piece0, pieces, scale); break;
-      default: clip_tile<bf16, bf16>(list.in[t], list.out[t], list.size[t], piece0, pieces, scale);
+      case 0: clip_tile<float, float>(list.in[t], list.out[t], list.size[t], nth, pieces, scale); break;
+      case IN_BF16: clip_tile<bf16, float>(list.in[t], list.out[t], list.size[t], nth, pieces, scale); break;
+      case OUT_BF16: clip_tile<float, bf16>(list.in[t], list.out[t], list.size[t], nth, pieces, scale); break;
+      default: clip_tile<bf16, bf16>(list.in[t], list.out[t], list.size[t], nth, pieces, scale);
     }
   }
 }
@@ -267,6 +322,7 @@ bool overlap(const Tensors& a) {
 template <int CAP>
 int fill(const Tensors& a, int32_t at, GradList<CAP>* list) {
   int c = 0;
+  list->elsewhere = 0;
   uint32_t tiles = 0;
   for (; at < a.count && c < CAP; ++at) {
     if (a.size[at] == 0) continue;
@@ -276,6 +332,7 @@ int fill(const Tensors& a, int32_t at, GradList<CAP>* list) {
     void* out = nullptr;
     if (a.out) {
       out = a.out[at];
+      list->elsewhere |= out != a.in[at];
       const int os = value_size(a.out_type[at]), is = value_size(a.type[at]);
       if (a.out_type[at] == MACE_BF16) type |= OUT_BF16;
       // results of the piece that holds the first value begin this many values before it
@@ -311,10 +368,10 @@ int run(const Tensors& a, double max_norm, float* norm, void* ws, cudaStream_t s
     parts += (int)grid;
   }
   if (!a.out || parts == 0) return launch("grad_norm", k_grad_norm, 1, GN_THREADS, 0, s, part, parts, norm);
-  for (int32_t at = 0; at < a.count;) {
-    const bool begin = at == 0;
-    if (!begin || a.count > CAP) at = fill(a, at, &list);
-    else at = a.count;  // (still filled)
+  const bool once = a.count <= CAP;  // (then the list still holds them)
+  bool begin = true;
+  for (int32_t at = 0; at < a.count; begin = false) {
+    at = once ? a.count : fill(a, at, &list);
     if (list.count == 0) break;
     const int rc = launch("grad_clip", k_grad_clip<CAP>, ctas(list.first[list.count]), GN_THREADS, 0, s, list, part, parts,
                           max_norm, begin ? norm : nullptr);

@@ -211,31 +211,32 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-# what the lists ask of every tensor, read without a Python frame each: a step's call is bound by it
+# What the lists ask of every tensor, read without a Python frame each: a step's call is bound by it.
 _device, _pointer, _numel, _contiguous = (getattr(torch.Tensor, f) for f in
                                           ("get_device", "data_ptr", "numel", "is_contiguous"))
 
 
 def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int) -> tuple[array, array, array, bool]:
     """Pointers, sizes and type codes of dense tensors on device ``dev``, and whether all are contiguous."""
-    contiguous = False
-    if not all(isinstance(t, torch.Tensor) for t in tensors) or forward_ad._current_level >= 0:
+    try:
+        elsewhere = set(map(_device, tensors)) - {dev}
+    except TypeError:  # (no tensor)
+        elsewhere = True
+    if elsewhere or forward_ad._current_level >= 0:
         for i, t in enumerate(tensors):
             _on(f"{name}[{i}]", t, dev)
-    if tensors and set(map(_device, tensors)) != {dev}:
-        for i, t in enumerate(tensors):
-            _on(f"{name}[{i}]", t, dev)
-    if all(t.layout is torch.strided for t in tensors):
+    try:
         contiguous = all(map(_contiguous, tensors))
+    except RuntimeError:  # (not strided)
+        contiguous = False
     if not contiguous:
         for i, t in enumerate(tensors):
             if not _dense(t):
                 raise ValueError(f"{name}[{i}] has gaps or repeated values (strides {t.stride()}); use .contiguous()"
                                  if t.layout is torch.strided else f"{name}[{i}] is not strided, got {t.layout}")
-    try:
-        codes = array("i", [_DTYPES[t.dtype] for t in tensors])
-    except KeyError as e:
-        raise ValueError(f"{name} must be float32 or bfloat16, got {e.args[0]}") from None
+    dtypes = [t.dtype for t in tensors]
+    kinds = {dtype: _dtype(name, dtype) for dtype in set(dtypes)}
+    codes = array("i", kinds.values()) * len(dtypes) if len(kinds) == 1 else array("i", map(kinds.get, dtypes))
     return array("Q", map(_pointer, tensors)), array("q", map(_numel, tensors)), codes, contiguous
 
 
@@ -284,7 +285,7 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
     max_norm = float(max_norm)
     if not 0.0 <= max_norm < math.inf:
         raise ValueError(f"max_norm must be finite and not negative, got {max_norm}")
-    every = grads if isinstance(grads, torch.Tensor) else list(grads)
+    every = grads if out is None or isinstance(grads, torch.Tensor) else list(grads)
     grads = _grads(every)
     dev = _cuda("grads[0]", grads[0]) if grads else torch.cuda.current_device()
     flat = _flat("grads", grads, dev)
