@@ -18,16 +18,17 @@ template <bool SILU, int N, bool SHARED>
 __device__ __forceinline__ void affine(float2* v, const Params<N, SHARED>& params) {
 #pragma unroll
   for (int c = 0; c < N / 8; ++c) {
-    float2 w[4], b[4], *const u = v + 4 * c;
+    float2 w[4], b[4];
     params.weight(c, w);
     params.bias(c, b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = fma2(u[i], w[i], b[i]);
-    if (SILU) {
-      sigmoid(u, w);
+    for (int i = 0; i < 4; ++i) v[4 * c + i] = fma2(v[4 * c + i], w[i], b[i]);
+  }
+  if (SILU) {
+    float2 s[N / 2];
+    sigmoid<N / 2>(v, s);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = mul2(u[i], w[i]);
-    }
+    for (int i = 0; i < N / 2; ++i) v[i] = mul2(v[i], s[i]);
   }
 }
 
@@ -58,6 +59,8 @@ __global__ void __launch_bounds__(LN_THREADS, LN_PER_SM<T, LAYOUT>) k_layer_norm
   next.zero();
   if (r < n) next.load(at, x, r - LN_TURN < p.inner);
   LaneSum<L> sum;
+  __shared__ uint4 edge_slots[LAYOUT == PIECES ? 2 * LN_THREADS / L : 1];
+  Edges<T, LAYOUT, N, L> edges(at, p, edge_slots, r, y);
   for (; r - sub < n; r += step) {
     float2 v[N / 2];
     const float lead = next.template lead<L>();
@@ -66,7 +69,12 @@ __global__ void __launch_bounds__(LN_THREADS, LN_PER_SM<T, LAYOUT>) k_layer_norm
     if (r + step < n) next.load(at, x, r + step - LN_TURN < p.inner);
     normalise(at, v, lead, p, sum);
     affine<SILU>(v, params);
-    if (r < n) Part<T, LAYOUT, N>::store(at, y, v);
+    if constexpr (LAYOUT == PIECES) {
+      edges.store(at, y, v, r < n, n);
+      edges.step(step, y_step);
+    } else if (r < n) {
+      Part<T, LAYOUT, N>::store(at, y, v);
+    }
     y += y_step;
   }
 }

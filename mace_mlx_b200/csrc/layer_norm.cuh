@@ -124,7 +124,8 @@ struct Lane {
 // the first (from: LAST) or last `m` values of a 16-byte piece at dst, 0 < m < 16 / size: a store for each power of two
 // in m, each aligned to its size
 template <int SIZE>
-__device__ __forceinline__ void store_some(char* dst, const uint32_t* w, int m, bool last) {
+__device__ __forceinline__ void store_some(char* dst, uint4 piece, int m, bool last) {
+  const uint32_t w[4] = {piece.x, piece.y, piece.z, piece.w};
   const int bytes = m * SIZE;
   char* at = last ? dst + 16 - bytes : dst;
   // from the piece's end inwards, or from its start
@@ -202,6 +203,21 @@ struct Part {
     w = __shfl_sync(0xffffffffu, w, LAYOUT == PIECES ? 1 : 0, L);
     return __uint_as_float(LAYOUT != APART && sizeof(T) == 2 ? w << 16 : w);
   }
+  // piece k as it goes to memory
+  static __device__ __forceinline__ uint4 words(const float2* v, int k) {
+    if constexpr (sizeof(T) == 4) {
+      return make_uint4(__float_as_uint(v[2 * k].x), __float_as_uint(v[2 * k].y), __float_as_uint(v[2 * k + 1].x),
+                        __float_as_uint(v[2 * k + 1].y));
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __float22bfloat162_rn(v[4 * k + i]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
   static __device__ __forceinline__ void store(const At& at, T* row, const float2* v) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -209,22 +225,94 @@ struct Part {
       if constexpr (LAYOUT == APART) {
         if (at.any(k)) *dst = from_f32<T>(k & 1 ? v[k / 2].y : v[k / 2].x);
       } else {
-        uint32_t w[4];
-        if constexpr (sizeof(T) == 4) {
-          w[0] = __float_as_uint(v[2 * k].x), w[1] = __float_as_uint(v[2 * k].y);
-          w[2] = __float_as_uint(v[2 * k + 1].x), w[3] = __float_as_uint(v[2 * k + 1].y);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h = __float22bfloat162_rn(v[4 * k + i]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-        }
+        const uint4 w = words(v, k);
         if (at.whole(k))
-          *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(dst) = w;
         else if (at.any(k))
           store_some<sizeof(T)>(reinterpret_cast<char*>(dst), w, at.count[k], k == 0 && at.first[k] < 0);
       }
+    }
+  }
+};
+
+// values between the 16-byte address before row r and the row
+template <typename T>
+__device__ __forceinline__ int row_head(const void* x, int64_t stride, int64_t r) {
+  return (int)((reinterpret_cast<uintptr_t>(static_cast<const T*>(x) + r * stride) & 15) / sizeof(T));
+}
+
+// Stores of rows of L lanes that start anywhere.  A row's first and last piece, where it is not the row's alone, goes
+// through shared memory (two slots for each of the warp's rows), from where every lane takes single words whose place
+// in the rows does not change from step to step: 14 instructions where stores of what each lane has of a piece, in all
+// the sizes it can have, take a hundred.
+template <typename T, Layout LAYOUT, int N, int L>
+struct Edges {  // (of the other layouts: none)
+  template <typename... A>
+  __device__ __forceinline__ explicit Edges(const A&...) {}
+};
+template <typename T, int N, int L>
+struct Edges<T, PIECES, N, L> {
+  using At = Lane<T, PIECES, N>;
+  static constexpr int V = At::V, K = At::K, ROWS = 32 / L, SLOTS = 2 * ROWS, PER = (4 * SLOTS + 31) / 32;
+  static constexpr int OF_WORD = 4 / sizeof(T);
+  uint4* slots;      // of the warp
+  bool start, end[K];  // whether this lane's first piece starts the row in part, a piece ends it in part
+  int slot;          // of the row's start; its end's is the next
+  T* to[PER];
+  uint32_t row[PER];  // of a word, among the warp's next rows
+  uint32_t on;        // bits: the values of the words that are stored
+  // r: this lane's row
+  __device__ __forceinline__ Edges(const At& at, const LayerNorm& p, uint4* shared, uint32_t r, T* y) {
+    const int lane = threadIdx.x & 31, sub = lane / L;
+    slots = shared + (threadIdx.x >> 5) * SLOTS;
+    slot = 2 * sub;
+    start = at.first[0] < 0 && lane % L == 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) end[k] = !at.whole(k) && at.any(k) && !(k == 0 && start);
+    on = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int word = lane + 32 * i, s = word / 4;
+      const uint32_t first = r - sub, which = s / 2;
+      row[i] = first + which;
+      const int head = row_head<T>(p.x, p.xs, row[i]), last = (p.C + head - 1) / V;  // (its last piece)
+      const int c = (s & 1 ? last * V : 0) - head + word % 4 * OF_WORD;
+      to[i] = y + ((int64_t)row[i] - r) * p.ys + c;
+#pragma unroll
+      for (int e = 0; e < OF_WORD; ++e) {
+        const bool part = s & 1 ? (p.C + head) % V != 0 && c + e < p.C : head > 0 && c + e >= 0;
+        if (s < SLOTS && part) on |= 1u << (i * OF_WORD + e);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(const At& at, T* y, const float2* v, bool in, uint32_t n) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const uint4 w = Part<T, PIECES, N>::words(v, k);
+      if (in && at.whole(k)) *reinterpret_cast<uint4*>(y + at.first[k]) = w;
+      if (k == 0 && start) slots[slot] = w;
+      if (end[k]) slots[slot + 1] = w;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(slots)[(threadIdx.x & 31) + 32 * i < 4 * SLOTS ? (threadIdx.x & 31) + 32 * i : 0];
+      if (row[i] < n) {
+        if constexpr (sizeof(T) == 4) {
+          if (on >> i & 1) *reinterpret_cast<uint32_t*>(to[i]) = w;
+        } else {
+          if (on >> (2 * i) & 1) *reinterpret_cast<uint16_t*>(to[i]) = (uint16_t)w;
+          if (on >> (2 * i + 1) & 1) *reinterpret_cast<uint16_t*>(to[i] + 1) = (uint16_t)(w >> 16);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void step(uint32_t rows, int64_t values) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      row[i] += rows;
+      to[i] += values;
     }
   }
 };
@@ -328,22 +416,23 @@ __device__ __forceinline__ float reciprocal(float a) {
 // rounds by |z| units, which count where exp(-z) outweighs the 1; the reciprocal within 1), and two values share a
 // reciprocal of their product: 12 of them instead of 16 for 8 values, whose pipe bounds 16-bit rows.  Values
 // whose product could overflow, or that are not numbers, are taken one by one.
-__device__ __forceinline__ void sigmoid(const float2* z, float2* s) {  // of 8 values
-  float2 a[4];
+template <int H>
+__device__ __forceinline__ void sigmoid(const float2* z, float2* s) {  // of 2 H values
+  float2 a[H], t[H];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < H; ++i) {
     const float2 e = mul2(z[i], both(-1.44269504f));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a[i].x) : "f"(e.x));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a[i].y) : "f"(e.y));
-    a[i] = add2(a[i], both(1.f));
+    t[i] = a[i] = add2(a[i], both(1.f));
   }
-  const float2 top = add2(add2(a[0], a[1]), add2(a[2], a[3]));
+  const float2 top = tree<H>(t);
   if (top.x + top.y <= 0x1p62f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = mul2(both(reciprocal(a[i].x * a[i].y)), make_float2(a[i].y, a[i].x));
+    for (int i = 0; i < H; ++i) s[i] = mul2(both(reciprocal(a[i].x * a[i].y)), make_float2(a[i].y, a[i].x));
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = make_float2(reciprocal(a[i].x), reciprocal(a[i].y));
+    for (int i = 0; i < H; ++i) s[i] = make_float2(reciprocal(a[i].x), reciprocal(a[i].y));
   }
 }
 
@@ -499,12 +588,6 @@ RowPlan row_plan(int64_t n, int C, std::initializer_list<Operand> operands) {
   // (rows that repeat: a neighbour's values need not lie inside the tensor)
   const bool any = alike && apart && C > V && pieces.lanes * pieces.values <= MACE_LAYER_NORM_MAX_CHANNELS;
   return any ? pieces : RowPlan{APART, LN_APART, row_lanes(LN_APART, C, 0)};
-}
-
-// values between the 16-byte address before row r and the row
-template <typename T>
-__device__ __forceinline__ int row_head(const void* x, int64_t stride, int64_t r) {
-  return (int)((reinterpret_cast<uintptr_t>(static_cast<const T*>(x) + r * stride) & 15) / sizeof(T));
 }
 
 inline uint32_t inner_rows(int64_t n) { return n > 2 * LN_TURN ? (uint32_t)(n - 2 * LN_TURN) : 0; }

@@ -27,7 +27,7 @@ __device__ __forceinline__ void row_grad(const float2* xhat, float2* grad, const
       params.bias(c, z);
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] = fma2(xh[i], w[i], z[i]);
-      sigmoid(z, s);
+      sigmoid<4>(z, s);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 rest = fma2(s[i], both(-1.f), both(1.f));
@@ -79,6 +79,8 @@ __global__ void __launch_bounds__(LN_THREADS, 2) k_layer_norm_grad(LayerNorm p) 
     nd.load(at, dy, r - LN_TURN < p.inner);
   }
   LaneSum<L> sum;
+  __shared__ uint4 edge_slots[LAYOUT == PIECES ? 2 * LN_THREADS / L : 1];
+  Edges<T, LAYOUT, N, L> edges(at, p, edge_slots, r, dx);
   for (; r - sub < end; r += GROUPS) {
     float2 v[H], g[H];
     const float lead = nx.template lead<L>();
@@ -95,7 +97,14 @@ __global__ void __launch_bounds__(LN_THREADS, 2) k_layer_norm_grad(LayerNorm p) 
 #pragma unroll
       for (int i = 0; i < H; ++i) v[i] = g[i] = both(0.f);
     row_grad<SILU>(v, g, params, rstd, p.inv_C, acc, sum);
-    if (p.y && r < end) Part<T, LAYOUT, N>::store(at, dx, g);
+    if constexpr (LAYOUT == PIECES) {
+      if (p.y) {
+        edges.store(at, dx, g, r < end, end);
+        edges.step(GROUPS, GROUPS * p.ys);
+      }
+    } else if (p.y && r < end) {
+      Part<T, LAYOUT, N>::store(at, dx, g);
+    }
     dx += GROUPS * p.ys;
   }
   if (!p.part) return;
