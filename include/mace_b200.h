@@ -550,7 +550,7 @@ int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t x_stride, const v
  * are summed in fp64, in an order that depends on the sizes, types and
  * addresses modulo 16 alone.
  */
-int mace_grad_norm_workspace(int32_t count, int64_t* bytes);
+int mace_grad_norm_workspace(int32_t count, int64_t values, int64_t* bytes); /* values: the sum of sizes */
 int mace_grad_norm(int32_t count, const void* const* grads, const int64_t* sizes, const int32_t* dtypes, float* norm,
                    void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -29,9 +29,10 @@ struct LayerNorm {
   uint32_t inner;  // rows [LN_TURN, LN_TURN + inner) have LN_TURN neighbours on either side
   void* y;  // forward: the result; backward: dx, or null
   int64_t ys;
-  // backward: rows of a CTA, and its sums: (shares, pitch) with dw in columns [0, C), db behind them; null: not wanted
+  // backward: rows of a CTA, and its sums: (shares, pitch) with dw in columns [0, C), db behind them
   int64_t share, shares;
-  float* part;
+  bool params;  // dw or db is wanted
+  float* part;  // null: the CTAs are one cluster, which adds them itself
   int pitch;
   void* dw;
   void* db;

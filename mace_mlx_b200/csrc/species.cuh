@@ -23,21 +23,67 @@ template <typename... P>
 bool unaligned(int size, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) % size != 0) || ...); }
 inline int value_size(int32_t dtype) { return dtype == MACE_F32 ? 4 : 2; }
 
+// a grid of clusters of `cluster` CTAs
 template <typename... P, typename... A>
-int launch(const char* name, void (*kernel)(P...), dim3 grid, unsigned threads, unsigned smem, cudaStream_t s, A... args) {
+int launch_clusters(const char* name, void (*kernel)(P...), dim3 grid, unsigned cluster, unsigned threads, unsigned smem,
+                    cudaStream_t s, A... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
   if (e != cudaSuccess) return fail(MACE_ERR_CUDA, std::string("launch ") + name + ": " + cudaGetErrorString(e));
   return MACE_OK;
+}
+template <typename... P, typename... A>
+int launch(const char* name, void (*kernel)(P...), dim3 grid, unsigned threads, unsigned smem, cudaStream_t s, A... args) {
+  return launch_clusters(name, kernel, grid, 1, threads, smem, s, args...);
+}
+
+// a grid of one cluster, of at least n of at most 16 CTAs: a power of two (more than 8 are this GPU's, not every one's)
+constexpr unsigned MOST_OF_CLUSTER = 16;
+template <typename... P, typename... A>
+int launch_cluster(const char* name, void (*kernel)(P...), unsigned n, unsigned threads, cudaStream_t s, bool* allowed, A... args) {
+  int dev = 0;
+  MACE_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !allowed[dev]) {  // (of this kernel, per device: the attribute call is slow on the host)
+    MACE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (dev < 64) allowed[dev] = true;
+  }
+  unsigned c = 1;
+  while (c < n && c < MOST_OF_CLUSTER) c *= 2;
+  return launch_clusters(name, kernel, c, c, threads, 0, s, args...);
+}
+
+// all threads of a cluster's CTAs, with what they wrote to shared memory
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the shared variable at the same place in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t of_cta(const void* shared, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(shared)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float load_of_cta(const float* shared, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(of_cta(shared, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ double load_of_cta(const double* shared, uint32_t rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(of_cta(shared, rank)) : "memory");
+  return v;
 }
 
 __device__ __forceinline__ float to_f32(float x) { return x; }

@@ -213,7 +213,7 @@ def load_library(path: str | Path | None = None) -> C.CDLL:
         "mace_layer_norm_grad_workspace": ([i64, i32, C.POINTER(i64)], C.c_int),
         "mace_layer_norm_grad": ([i32, vp, i64, vp, i64, i32, vp, vp, i64, i32, f32, i32, vp, i64, vp, vp, vp, i64, vp],
                                  C.c_int),
-        "mace_grad_norm_workspace": ([i32, C.POINTER(i64)], C.c_int),
+        "mace_grad_norm_workspace": ([i32, i64, C.POINTER(i64)], C.c_int),
         "mace_grad_norm": ([i32, vp, vp, vp, vp, vp, i64, vp], C.c_int),
         "mace_grad_clip": ([i32, vp, vp, vp, vp, vp, C.c_double, vp, vp, i64, vp], C.c_int),
     }

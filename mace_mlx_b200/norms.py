@@ -97,8 +97,7 @@ def _eps(eps: float) -> float:
     return eps
 
 
-def _layer_norm(x, weight, bias, eps, activation, out):
-    dev = _cuda("x", x)
+def _layer_norm(x, dev, weight, bias, eps, activation, out):
     code = _dtype("x", x.dtype)
     n, c, xs = _rows("x", x)
     pcode, w, b = _params(weight, bias, dev, c, x.dtype)
@@ -156,16 +155,23 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     Statistics and products are fp32, rounded once to x's type.  Deviations
     from the mean are squared in fp32: rows whose values pass 1e18 lose them.
     """
-    grads = [t for t in (x, weight, bias) if isinstance(t, torch.Tensor) and t.requires_grad]
-    if grads and torch.is_grad_enabled():
+    dev = _cuda("x", x)
+    if torch.is_grad_enabled() and (x.requires_grad or _requires_grad("weight", weight) or _requires_grad("bias", bias)):
         if out is not None:
             raise ValueError("out= cannot take part in autograd")
-        _cuda("x", x)
         for name, t in (("weight", weight), ("bias", bias)):
             if t is not None:
                 _cuda(name, t)
         return _LayerNormFn.apply(x, weight, bias, eps, activation)
-    return _layer_norm(x, weight, bias, eps, activation, out)
+    return _layer_norm(x, dev, weight, bias, eps, activation, out)
+
+
+def _requires_grad(name: str, t: torch.Tensor | None) -> bool:
+    if t is None:
+        return False
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    return t.requires_grad
 
 
 def layer_norm_grad(x: torch.Tensor, grad: torch.Tensor, weight: torch.Tensor | None = None,
@@ -185,7 +191,7 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, activation):
         ctx.save_for_backward(x, weight, bias)
         ctx.more = eps, activation
-        return _layer_norm(x, weight, bias, eps, activation, None)
+        return _layer_norm(x, x.get_device(), weight, bias, eps, activation, None)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -249,7 +255,7 @@ def _grads(grads: Iterable[torch.Tensor | None]) -> list[torch.Tensor]:
 def _norm_of(grads: list[torch.Tensor], dev: int, flat, fn, *more) -> torch.Tensor:
     ptrs, sizes, codes, _ = flat
     norm = grads[0].new_empty((), dtype=torch.float32) if grads else torch.empty((), device=torch.device("cuda", dev))
-    ws, wptr, nbytes = _workspace("mace_grad_norm_workspace", dev, norm, len(grads))
+    ws, wptr, nbytes = _workspace("mace_grad_norm_workspace", dev, norm, len(grads), sum(sizes))
     _launch(dev, fn, len(grads), ptrs.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], *more,
             norm.data_ptr(), wptr, nbytes)
     return norm

@@ -67,7 +67,8 @@ def test_c_entries_check_their_arguments():
     assert lib.mace_layer_norm(0, None, 8, 0, None, None, 0, 8, 1e-5, 0, None, 8, None) == nv.MACE_OK  # no rows
 
     need = C.c_int64(-1)
-    assert lib.mace_layer_norm_grad_workspace(1000, 128, C.byref(need)) == nv.MACE_OK and need.value > 0
+    assert lib.mace_layer_norm_grad_workspace(100_000, 128, C.byref(need)) == nv.MACE_OK and need.value > 0
+    assert lib.mace_layer_norm_grad_workspace(1000, 128, C.byref(need)) == nv.MACE_OK and need.value == 0  # one cluster
     for args in ((-1, 8), (2**31, 8), (1, 0), (1, nv.LAYER_NORM_MAX_CHANNELS + 1)):
         assert lib.mace_layer_norm_grad_workspace(*args, C.byref(need)) == nv.MACE_ERR_BAD_ARG
     assert lib.mace_layer_norm_grad_workspace(1, 8, None) == nv.MACE_ERR_BAD_ARG
@@ -75,16 +76,20 @@ def test_c_entries_check_their_arguments():
     refused(lib.mace_layer_norm_grad, grad, [(0, 7), (1, None), (2, -1), (3, None), (4, -1), (5, 7), (8, -1), (9, 0),
                                              (10, -1.0), (11, 5), (13, 7)])
     refused(lib.mace_layer_norm_grad, grad, [(k, odd) for k in (1, 3, 6, 7, 12, 14, 15)], "values' size")
-    refused(lib.mace_layer_norm_grad, grad, [(16, None), (16, C.c_void_p(40)), (17, 3)], "workspace")
+    many = (*grad[:8], 100_000, *grad[9:])
+    refused(lib.mace_layer_norm_grad, many, [(16, None), (16, C.c_void_p(40)), (17, 3)], "workspace")
 
 
 def test_c_entries_check_lists_of_tensors():
     lib = nv.load_library()
     need = C.c_int64(-1)
-    assert lib.mace_grad_norm_workspace(0, C.byref(need)) == nv.MACE_OK and need.value == 0
-    assert lib.mace_grad_norm_workspace(5000, C.byref(need)) == nv.MACE_OK and need.value > 0
-    assert lib.mace_grad_norm_workspace(-1, C.byref(need)) == nv.MACE_ERR_BAD_ARG
-    assert lib.mace_grad_norm_workspace(1, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_grad_norm_workspace(0, 0, C.byref(need)) == nv.MACE_OK and need.value == 0
+    assert lib.mace_grad_norm_workspace(8, 1000, C.byref(need)) == nv.MACE_OK and need.value == 0  # one cluster
+    assert lib.mace_grad_norm_workspace(8, 10**7, C.byref(need)) == nv.MACE_OK and need.value > 0
+    assert lib.mace_grad_norm_workspace(5000, 5000, C.byref(need)) == nv.MACE_OK and need.value > 0
+    for args in ((-1, 0), (0, -1)):
+        assert lib.mace_grad_norm_workspace(*args, C.byref(need)) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_grad_norm_workspace(1, 1, None) == nv.MACE_ERR_BAD_ARG
     one = C.c_void_p(4096)
 
     def call(ptrs, sizes, types, out=None, out_types=None, max_norm=1.0, norm=one, ws=one, nbytes=1 << 20):
@@ -99,8 +104,8 @@ def test_c_entries_check_lists_of_tensors():
 
     bad = [
         call([64], [-1], [0]), call([64], [8], [2]), call([None], [8], [0]), call([66], [8], [0]), call([65], [8], [1]),
-        call([64], [8], [0], norm=None), call([64], [8], [0], ws=None), call([64], [8], [0], nbytes=8),
-        call([64], [8], [0], ws=C.c_void_p(4)), call([64], [2**41], [0]),
+        call([64], [8], [0], norm=None), call([64], [10**7], [0], ws=None), call([64], [10**7], [0], nbytes=8),
+        call([64], [10**7], [0], ws=C.c_void_p(4)), call([64], [2**41], [0]),
         call([64], [8], [0], out=[64], max_norm=-1.0), call([64], [8], [0], out=[64], max_norm=float("inf")),
         call([64], [8], [0], out=[64], max_norm=float("nan")), call([64], [8], [0], out=[None]),
         call([64], [8], [0], out=[64], out_types=[1]), call([64], [8], [0], out=[63], out_types=[1]),
