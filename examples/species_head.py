@@ -1,6 +1,6 @@
 """Train a species-dependent energy head on the node features of a frozen MACE model.
 
-    PYTHONPATH=. python examples/species_head.py [--structures 32] [--steps 200]
+    PYTHONPATH=. python examples/species_head.py [--structures 32] [--steps 200] [--max-norm 10]
 
 The model's own step (``MACEModel.evaluate``) gives the features h (N, d, C) of
 its first layer: a scalar and a vector per channel.  The head is the pair of
@@ -22,6 +22,7 @@ import argparse
 import numpy as np
 import torch
 
+from mace_mlx_b200 import norms
 from mace_mlx_b200 import species as sp
 from mace_mlx_b200.model import MACEModel
 from mace_mlx_b200.spec import ModelSpec
@@ -63,8 +64,10 @@ class SpeciesHead(torch.nn.Module):
         return torch.zeros(n_graphs, device=h.device).index_add(0, graph, atom) / graph.bincount(minlength=n_graphs)
 
 
-def train(n_structures: int = 32, steps: int = 200, width: int = 64, seed: int = 0, lr: float = 2e-2) -> list[float]:
-    """Fits the head; the loss (mean squared error of the energies per atom) at every step."""
+def train(n_structures: int = 32, steps: int = 200, width: int = 64, seed: int = 0, lr: float = 2e-2,
+          max_norm: float | None = None) -> list[float]:
+    """Fits the head, its gradients clipped to ``max_norm`` where one is given; the loss (mean squared error of the
+    energies per atom) at every step."""
     h, species, graph = frozen_features(n_structures, seed)
     groups = sp.group_species(species, 4)
     generator = torch.Generator(h.device).manual_seed(seed)
@@ -78,6 +81,8 @@ def train(n_structures: int = 32, steps: int = 200, width: int = 64, seed: int =
         optimiser.zero_grad(set_to_none=True)
         loss = (head(h, species, groups, graph, n_structures) - energy).square().mean()
         loss.backward()
+        if max_norm is not None:
+            norms.clip_grads([p.grad for p in head.parameters()], max_norm)
         optimiser.step()
         losses.append(loss.detach())
     return torch.stack(losses).tolist()
@@ -87,8 +92,9 @@ def main():
     parser = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     parser.add_argument("--structures", type=int, default=32)
     parser.add_argument("--steps", type=int, default=200)
+    parser.add_argument("--max-norm", type=float, default=None, help="bound of the gradients' norm (none)")
     args = parser.parse_args()
-    losses = train(args.structures, args.steps)
+    losses = train(args.structures, args.steps, max_norm=args.max_norm)
     for step in range(0, len(losses), max(1, len(losses) // 10)):
         print(f"step {step:4d}  loss {losses[step]:.4e}")
     print(f"step {len(losses) - 1:4d}  loss {losses[-1]:.4e}")

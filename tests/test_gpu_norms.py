@@ -786,3 +786,49 @@ def test_tangents_are_refused(nm, requires_grad):
                 pytest.fail(f"call {i} was accepted")
         nm.layer_norm(plain["x"], plain["w"])  # without a tangent: as ever
         nm.grad_norm([plain["w"]])
+
+
+# ------------------------------------------------------------------- together
+def example(name):
+    import importlib.util
+    import pathlib
+
+    path = pathlib.Path(__file__).resolve().parents[1] / "examples" / f"{name}.py"
+    spec = importlib.util.spec_from_file_location(name, path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_radial_mlp_has_the_plain_gradients(nm):
+    ex = example("radial_mlp")
+    x = ex.edge_features(6, seed=1)
+    mlp = ex.RadialMLP([8, 64, 64, 97], gen(110))
+    out = mlp(x)
+    v = randn(*out.shape, seed=111)
+    (out * v).sum().backward()
+    p = {k: q.detach().double().requires_grad_() for k, q in mlp.named_parameters()}
+    h = x.double()
+    for i in range(3):
+        h = h @ p[f"weights.{i}"].T + p[f"biases.{i}"]
+        if i < 2:
+            z = Rows64(h, p[f"gains.{i}"], p[f"shifts.{i}"], 1e-5, True).z
+            h = z * torch.sigmoid(z)
+    (h * v.double()).sum().backward()
+    # fp32 sums of a few thousand terms each way: 2^-16 of the largest value covers their roundings and torch's
+    assert (out.double() - h).abs().max() <= 2.0**-16 * h.abs().max()
+    grads = []
+    for name, q in mlp.named_parameters():
+        assert (q.grad.double() - p[name].grad).abs().max() <= 2.0**-16 * p[name].grad.abs().max(), name
+        grads.append(q.grad)
+    before = [g.clone() for g in grads]
+    want = clipped64(before, 0.1 * float(norm64(before)))
+    assert_norm(nm.clip_grads([q.grad for q in mlp.parameters()], 0.1 * float(norm64(before))), before)
+    assert_clipped(grads, want)
+
+
+def test_examples_run_with_clipping(nm):
+    losses, sizes = example("radial_mlp").train(n_structures=4, steps=5, max_norm=1e-3)
+    assert len(losses) == len(sizes) == 5 and all(s > 0 for s in sizes)
+    losses = example("species_head").train(n_structures=4, steps=5, max_norm=1e-3)
+    assert len(losses) == 5 and all(x == x for x in losses)
