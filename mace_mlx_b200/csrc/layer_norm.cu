@@ -79,9 +79,15 @@ __global__ void __launch_bounds__(LN_THREADS, LN_PER_SM<T, LAYOUT>) k_layer_norm
   }
 }
 
-// wider rows: a CTA each
+// Wider rows: a CTA each, as many as fit an SM at once.  16-bit rows, with half the bytes for the same barriers, want
+// more of them (40 003 rows of 2048 63 us, 71 with 512 threads on an SM), fp32 rows the registers (40 003 rows of 1000
+// with SiLU 58 us, 75 with 768).
+template <typename T>
+constexpr int wide_threads(int most) {  // on an SM, by CTAs of at most 256 or more threads
+  return sizeof(T) == 2 ? (most <= 256 ? 768 : 1024) : (most <= 256 ? 512 : most);
+}
 template <typename T, Layout LAYOUT, int N, bool SILU, int MOST>
-__global__ void __launch_bounds__(MOST) k_layer_norm_wide(LayerNorm p) {
+__global__ void __launch_bounds__(MOST, wide_threads<T>(MOST) / MOST) k_layer_norm_wide(LayerNorm p) {
   __shared__ __align__(16) float sums[CtaSum<MOST / 32>::FLOATS];
   pdl_wait();
   const uint32_t n = (uint32_t)p.n, step = gridDim.x;
@@ -116,7 +122,8 @@ int forward(const LayerNorm& p, int lanes, cudaStream_t s) {
   if constexpr (may_be_wide(LAYOUT, N)) {
     if (lanes > 32) {
       constexpr int MOST = MACE_LAYER_NORM_MAX_CHANNELS / N;  // lanes
-      const int64_t grid = std::min<int64_t>(p.n, LN_SMS * std::max(1, 1024 / lanes) / LN_TURN * LN_TURN);
+      const int threads = wide_threads<T>(lanes <= 256 ? 256 : MOST);
+      const int64_t grid = std::min<int64_t>(p.n, LN_SMS * std::max(1, threads / lanes) / LN_TURN * LN_TURN);
       auto go = [&](auto kernel) { return launch("layer_norm", kernel, dim3((unsigned)grid), lanes, 0, s, p); };
       return lanes <= 256 ? go(k_layer_norm_wide<T, LAYOUT, N, SILU, 256>) : go(k_layer_norm_wide<T, LAYOUT, N, SILU, MOST>);
     }
