@@ -534,8 +534,9 @@ int mace_layer_norm(int32_t dtype, const void* x, int64_t x_stride, int32_t para
 /*
  * Gradients of mace_layer_norm for the output gradient dy: dx (n rows of C),
  * dweight and dbias (C values of param_dtype); any may be NULL (not wanted).
- * The workspace serves dweight and dbias.  The order of their sums depends on
- * n and C alone.
+ * The workspace (16-byte aligned) serves dweight and dbias; few rows need none.
+ * dx must not overlap x or dy.  The order of all sums depends on the sizes and
+ * types and on the addresses modulo 16 alone.
  */
 int mace_layer_norm_grad_workspace(int64_t n, int32_t C, int64_t* bytes);
 int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride,
@@ -548,7 +549,8 @@ int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t x_stride, const v
  * Tensor t is sizes[t] values of dtypes[t] at grads[t] (host arrays, read
  * before the call returns, so a captured call keeps their contents).  Squares
  * are summed in fp64, in an order that depends on the sizes, types and
- * addresses modulo 16 alone.
+ * addresses modulo 16 alone.  The workspace (8-byte aligned) may be NULL where
+ * its size is 0: few tensors of few values.
  */
 int mace_grad_norm_workspace(int32_t count, int64_t values, int64_t* bytes); /* values: the sum of sizes */
 int mace_grad_norm(int32_t count, const void* const* grads, const int64_t* sizes, const int32_t* dtypes, float* norm,

@@ -1,4 +1,5 @@
-// Device helpers shared by the species operators (species.cu, species_linear.cu).
+// Device helpers shared by the species operators (species.cu, species_linear.cu) and the normalisation operators
+// (layer_norm.cu, layer_norm_grad.cu, grad_norm.cu).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -15,7 +15,8 @@ them again from x.
 Every call runs hand-written kernels of ``libmace_b200`` on the current stream
 of the tensors' device, allocates only its results and workspace through
 torch, and neither synchronises nor reads device values, so it can be captured
-into a CUDA graph.  Tensors last used on another stream need the caller's
+into a CUDA graph (a backward, as torch has it, while no eager graph of the
+same leaves lives).  Tensors last used on another stream need the caller's
 ``wait_stream``/``record_stream``, as for torch's own operators.
 
 Reference: Linear -> LayerNorm -> SiLU stacks ``mace_mlx/radial.py:344-357``;
@@ -180,8 +181,8 @@ def layer_norm_grad(x: torch.Tensor, grad: torch.Tensor, weight: torch.Tensor | 
     """Gradients of ``layer_norm`` at x, weight and bias for the output gradient ``grad``.
 
     Those of weight and bias have their type (None without them); their sums
-    over the rows are fp32, in an order that depends on the sizes alone, so
-    equal calls give equal bits.
+    over the rows are fp32, in an order that depends on the sizes, the types and
+    the addresses modulo 16 alone, so equal calls give equal bits.
     """
     return _layer_norm_grad(x, grad, weight, bias, eps, activation, True, weight is not None, bias is not None)
 
