@@ -193,6 +193,32 @@ def test_rows_in_a_wider_table(nm, dtype, c, pitch, at):
     assert torch.equal(grads[:, at:at + c], dy)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [3, 9, 17, 33, 65, 96, 97, 250, 257, 500, 511, 1001, 8189])
+def test_rows_among_neighbours_that_are_not_numbers(nm, dtype, c):
+    """Rows at every address modulo 16, one behind the other or with gaps: what lies around them does not enter, and
+    nothing but the rows is written."""
+    for n, gap, at in ((1, 0, 1), (2, 0, 0), (9, 0, 3), (21, 0, 5), (21, 1, 0), (17, 5, 7), (40, 8, 2)):
+        if c > 1000:
+            n = min(n, 9)
+        size = at + n * (c + gap) + 16
+
+        def rows(values, fill):
+            t = torch.full((size,), fill, dtype=dtype, device="cuda")
+            v = t.as_strided((n, c), (c + gap, 1), at)
+            v.copy_(values)
+            return t, v
+
+        x, dy, w, b = inputs(n, c, dtype, F32, seed=c + n)
+        x, dy = rows(x, float("nan"))[1], rows(dy, float("nan"))[1]
+        check_rows(nm, x, dy, w, b, silu=True, norm=False)
+        table, out = rows(torch.zeros(n, c), 7.0)
+        nm.layer_norm(x, w, b, activation="silu", out=out)
+        assert_close(out, *Rows64(x, w, b, 1e-5, True).forward(), "out", norm=False)
+        out.fill_(7.0)
+        assert (table == 7.0).all()
+
+
 def test_repeated_rows_and_other_shapes(nm):
     c = 64
     x, dy, w, b = inputs(1, c, F32, F32, seed=6)
@@ -440,10 +466,27 @@ def test_gradient_norm_of_extreme_values(nm):
     big = torch.full((4,), 3e38, device="cuda")  # the norm itself lies past fp32
     assert float(nm.grad_norm([big])) == float("inf")
     for value in (float("inf"), -float("inf"), float("nan")):
-        grads = [randn(100, seed=32), randn(5000, seed=33)]
-        grads[1][4321] = value
-        got = float(nm.grad_norm(grads))
-        assert got != got if value != value else got == float("inf")
+        for dtype in DTYPES:
+            for more in (0, 1_000_000):
+                grads = [randn(100, seed=32, dtype=dtype), randn(5000 + more, seed=33, dtype=dtype)]
+                grads[1][4321] = value
+                got = float(nm.grad_norm(grads))
+                assert got != got if value != value else got == float("inf")
+
+
+@pytest.mark.parametrize("size", [777, 2_000_000])
+def test_gradient_norm_of_16_bit_values_at_the_ends_of_their_range(nm, size):
+    zeros = torch.zeros(size, dtype=BF16, device="cuda")
+    assert float(nm.grad_norm([zeros, -zeros])) == 0.0
+    for value in (2.0**-133, 2.0**-126, 1.5 * 2.0**-127, 2.0**-60, 1.0, 2.0**127, float(torch.finfo(BF16).max)):
+        for where in (slice(0, 1), slice(5, 9), slice(size - 1, size)):  # subnormals, the least normal, the largest
+            g = zeros.clone()
+            g[where] = value
+            got, want = float(nm.grad_norm([g])), abs(value) * (where.stop - where.start) ** 0.5
+            assert got == float(torch.tensor(want, dtype=torch.float64).float()), (value, where)  # (2^128 rounds to inf)
+    both = zeros.clone()
+    both[3], both[4] = 2.0**-133, 3 * 2.0**-132
+    assert_norm(nm.grad_norm([both]), [both])
 
 
 def test_gradient_norm_in_any_order_of_dimensions(nm):
@@ -569,22 +612,31 @@ def test_clipping_counts_as_a_change(nm):
 def everything(nm, x, dy, w, b, grads, out):
     y = nm.layer_norm(x, w, b, activation="silu")
     more = nm.layer_norm_grad(x, dy, w, b, activation="silu")
-    wide = nm.layer_norm_grad(x.view(-1, x.numel() // 4), dy.view(-1, x.numel() // 4))[0]
+    wide = nm.layer_norm_grad(x.view(-1, 1536), dy.view(-1, 1536), activation="silu")[0]
     return [y, *more, wide, nm.grad_norm([*grads, more[1]]), nm.clip_grads([*grads, more[2]], 2.0, out=out), *out]
 
 
-def step_inputs(seed):
-    x, dy, w, b = inputs(64, 96, F32, F32, seed=seed)
-    grads = [randn(5000, seed=seed + 7), randn(33, 3, seed=seed + 8, dtype=BF16)]
+# one cluster each, or several launches with workspaces
+SIZES = {"small": (64, 5000), "large": (9008, 2_000_000)}
+
+
+def step_inputs(seed, size):
+    n, values = SIZES[size]
+    x, dy, w, b = inputs(n, 96, F32, F32, seed=seed)
+    grads = [randn(values, seed=seed + 7), randn(33, 3, seed=seed + 8, dtype=BF16)]
     return x, dy, w, b, grads
 
 
-def outputs():
-    return [torch.empty(5000, device="cuda"), torch.empty(33, 3, device="cuda"), torch.empty(96, device="cuda")]
+def step_outputs(size):
+    return [torch.empty(SIZES[size][1], device="cuda"), torch.empty(33, 3, device="cuda"), torch.empty(96, device="cuda")]
 
 
-def test_other_streams_and_cuda_graphs(nm):
-    x, dy, w, b, grads = step_inputs(50)
+@pytest.mark.parametrize("size", list(SIZES))
+def test_other_streams_and_cuda_graphs(nm, size):
+    def outputs():
+        return step_outputs(size)
+
+    x, dy, w, b, grads = step_inputs(50, size)
     want = [t.clone() for t in everything(nm, x, dy, w, b, grads, outputs())]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -651,10 +703,14 @@ def test_training_step_in_a_graph(nm):
     assert all(torch.equal(a, d) for a, d in zip(got, want))
 
 
-def test_calls_from_two_host_threads(nm):
+@pytest.mark.parametrize("size", list(SIZES))
+def test_calls_from_two_host_threads(nm, size):
     import threading
 
-    data = {seed: step_inputs(seed) for seed in (70, 80)}
+    def outputs():
+        return step_outputs(size)
+
+    data = {seed: step_inputs(seed, size) for seed in (70, 80)}
     want = {seed: [t.clone() for t in everything(nm, *d, outputs())] for seed, d in data.items()}
     torch.cuda.synchronize()
     got, errors = {}, []
