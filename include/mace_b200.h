@@ -552,6 +552,7 @@ int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t x_stride, const v
  * addresses modulo 16 alone.  The workspace (8-byte aligned) may be NULL where
  * its size is 0: few tensors of few values.
  */
+#define MACE_GRAD_FEW_TENSORS 64 /* more need a workspace whatever their values */
 int mace_grad_norm_workspace(int32_t count, int64_t values, int64_t* bytes); /* values: the sum of sizes */
 int mace_grad_norm(int32_t count, const void* const* grads, const int64_t* sizes, const int32_t* dtypes, float* norm,
                    void* workspace, int64_t workspace_bytes, void* stream);

@@ -34,7 +34,7 @@ __device__ __forceinline__ void affine(float2* v, const Params<N, SHARED>& param
 
 // CTAs on an SM, and where the lanes keep their parameters.  32 bytes of a row in flight for each lane of three CTAs
 // fill the memory's queues (2M fp32 rows of 64 with SiLU 162 us, 173 with four CTAs, 187 with two); rows that start
-// anywhere have less in a lane and take four in fp32 (500 003 rows of 96 69 us, 77 with three).  16 values of a lane
+// anywhere have less in a lane and take four in fp32 (500 003 rows of 96 71 us, 77 with three).  16 values of a lane
 // leave no registers for their parameters (2M bf16 rows of 64 with SiLU 89 us, 110 with parameters in registers).
 template <typename T, Layout LAYOUT>
 constexpr int LN_PER_SM = sizeof(T) == 4 && LAYOUT == PIECES ? 4 : 3;

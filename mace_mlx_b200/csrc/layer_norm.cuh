@@ -1,5 +1,5 @@
 // Rows of the layer norm in registers (layer_norm.cu, layer_norm_grad.cu): how a row is spread over its lanes, and the
-// arithmetic on a lane's 8 values, two at a time (the packed fp32 instructions of sm_100).
+// arithmetic on a lane's values, two at a time (the packed fp32 instructions of sm_100).
 #pragma once
 
 #include <algorithm>
@@ -122,8 +122,8 @@ struct Lane {
   }
 };
 
-// the first (from: LAST) or last `m` values of a 16-byte piece at dst, 0 < m < 16 / size: a store for each power of two
-// in m, each aligned to its size
+// the first m, or with `last` the last m, values of a 16-byte piece at dst, 0 < m < 16 / SIZE: a store for each power of
+// two in m, each aligned to its size
 template <int SIZE>
 __device__ __forceinline__ void store_some(char* dst, uint4 piece, int m, bool last) {
   const uint32_t w[4] = {piece.x, piece.y, piece.z, piece.w};
@@ -555,7 +555,7 @@ struct Operand {
 
 // Values of a lane.  Rows of up to 32 lanes: two pieces, so that 32 bytes of each row are in flight for a lane and the
 // row's sums take few steps; but one piece of 16 bits in the backward where a row starts anywhere (300 007 rows of 97
-// 80 us; with two, whose masks leave too few registers, 102), and 8 single values.  Four pieces of fp32 where a row then
+// 75 us; with two, whose masks leave too few registers, 87), and 8 single values.  Four pieces of fp32 where a row then
 // still fits a warp, and where it takes a CTA (gradients of 20 011 rows of 2048 87 us, 99 with two).
 constexpr int LN_WIDE = 16, LN_APART = 8;
 template <typename T, bool GRAD>

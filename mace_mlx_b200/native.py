@@ -154,6 +154,7 @@ CHECKPOINT_BLOCK = 128
 ACT_NONE = 0
 ACT_SILU = 1
 LAYER_NORM_MAX_CHANNELS = 8192
+GRAD_FEW_TENSORS = 64
 
 _lib = None
 

@@ -241,9 +241,8 @@ def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int) -> tuple[array, 
             if not _dense(t):
                 raise ValueError(f"{name}[{i}] has gaps or repeated values (strides {t.stride()}); use .contiguous()"
                                  if t.layout is torch.strided else f"{name}[{i}] is not strided, got {t.layout}")
-    dtypes = [t.dtype for t in tensors]
-    kinds = {dtype: _dtype(name, dtype) for dtype in set(dtypes)}
-    codes = array("i", kinds.values()) * len(dtypes) if len(kinds) == 1 else array("i", map(kinds.get, dtypes))
+    kinds = {dtype: _dtype(name, dtype) for dtype in {t.dtype for t in tensors}}
+    codes = array("i", kinds.values()) * len(tensors) if len(kinds) == 1 else array("i", [kinds[t.dtype] for t in tensors])
     return array("Q", map(_pointer, tensors)), array("q", map(_numel, tensors)), codes, contiguous
 
 
@@ -256,7 +255,9 @@ def _grads(grads: Iterable[torch.Tensor | None]) -> list[torch.Tensor]:
 def _norm_of(grads: list[torch.Tensor], dev: int, flat, fn, *more) -> torch.Tensor:
     ptrs, sizes, codes, _ = flat
     norm = grads[0].new_empty((), dtype=torch.float32) if grads else torch.empty((), device=torch.device("cuda", dev))
-    ws, wptr, nbytes = _workspace("mace_grad_norm_workspace", dev, norm, len(grads), sum(sizes))
+    # (the number of values tells few tensors from small ones)
+    values = sum(sizes) if len(grads) <= nv.GRAD_FEW_TENSORS else 0
+    ws, wptr, nbytes = _workspace("mace_grad_norm_workspace", dev, norm, len(grads), values)
     _launch(dev, fn, len(grads), ptrs.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], *more,
             norm.data_ptr(), wptr, nbytes)
     return norm
@@ -300,9 +301,9 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
     if out is not None:
         if len(out) != len(every):
             raise ValueError(f"out has {len(out)} tensors, grads {len(every)}")
-        into = [o for o, g in zip(out, every) if g is not None]
+        into = list(out) if len(grads) == len(every) else [o for o, g in zip(out, every) if g is not None]
         ptrs, sizes, codes, contiguous = _flat("out", into, dev)
-        if sizes != flat[1] or not (contiguous and flat[3]):
+        if sizes.tobytes() != flat[1].tobytes() or not (contiguous and flat[3]):
             for i, (g, o) in enumerate(zip(grads, into)):
                 if o.numel() != g.numel() or o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
                     raise ValueError(f"out[{i}] must be {tuple(g.shape)} with strides {g.stride()}, got {tuple(o.shape)} "
