@@ -569,6 +569,18 @@ int mace_grad_clip(int32_t count, const void* const* grads, const int64_t* sizes
                    void* const* out, const int32_t* out_dtypes, double max_norm, float* norm, void* workspace,
                    int64_t workspace_bytes, void* stream);
 
+/*
+ * For bindings that hold tensors as Python objects: address, number of values
+ * and type of each of `count` of them, as the entries above take them, read
+ * through the DLPack C exchange API of the objects' type
+ * (dltensor_from_py_object_no_sync, a function of (PyObject*, DLTensor*)).  The
+ * caller holds the interpreter's lock.  MACE_OK if all are contiguous fp32 or
+ * bf16 tensors on CUDA device `device`; else nothing about the arrays holds, and
+ * an exception that the function set is left set.
+ */
+int mace_tensor_list(int (*read)(void* object, void* tensor), int32_t count, void* const* objects, int32_t device,
+                     void** data, int64_t* sizes, int32_t* dtypes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -136,7 +136,7 @@ EXPORTED = (
     "mace_species_linear_wgrad_workspace", "mace_species_linear_wgrad", "mace_rows_checkpoint", "mace_rows_restore",
     "mace_species_error_flag",
     "mace_layer_norm", "mace_layer_norm_grad_workspace", "mace_layer_norm_grad", "mace_grad_norm_workspace",
-    "mace_grad_norm", "mace_grad_clip",
+    "mace_grad_norm", "mace_grad_clip", "mace_tensor_list",
 )
 NOALLOC_MAX_ATOMS = 131072
 NOALLOC_MAX_GRAPH_ATOMS = 16384
@@ -217,6 +217,7 @@ def load_library(path: str | Path | None = None) -> C.CDLL:
         "mace_grad_norm_workspace": ([i32, i64, C.POINTER(i64)], C.c_int),
         "mace_grad_norm": ([i32, vp, vp, vp, vp, vp, i64, vp], C.c_int),
         "mace_grad_clip": ([i32, vp, vp, vp, vp, vp, C.c_double, vp, vp, i64, vp], C.c_int),
+        "mace_tensor_list": ([vp, i32, vp, i32, vp, vp, vp], C.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -225,6 +226,29 @@ def load_library(path: str | Path | None = None) -> C.CDLL:
     if path is None:
         _lib = lib
     return lib
+
+
+def load_tensor_list():
+    """``mace_tensor_list`` called with the interpreter's lock held, as it reads Python objects."""
+    load_library()
+    fn = C.PyDLL(str(LIB_PATH)).mace_tensor_list
+    fn.argtypes = [C.c_void_p, i32, C.c_void_p, i32, C.c_void_p, C.c_void_p, C.c_void_p]
+    fn.restype = C.c_int
+    return fn
+
+
+def dlpack_reader(kind) -> int | None:
+    """Address of dltensor_from_py_object_no_sync in the DLPack C exchange API of a tensor type, if it has one."""
+    capsule = getattr(kind, "__dlpack_c_exchange_api__", None)
+    if capsule is None:
+        return None
+    get = C.pythonapi.PyCapsule_GetPointer
+    get.restype, get.argtypes = C.c_void_p, [C.py_object, C.c_char_p]
+    api = get(capsule, b"dlpack_exchange_api")
+    # (version, the API before it, then: allocator, two conversions of managed tensors, this function, the stream)
+    if C.c_uint32.from_address(api).value != 1:
+        return None
+    return C.c_void_p.from_address(api + 16 + 3 * C.sizeof(C.c_void_p)).value
 
 
 def last_error(lib=None) -> str:

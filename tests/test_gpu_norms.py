@@ -495,6 +495,33 @@ def test_gradient_norm_in_any_order_of_dimensions(nm):
         assert_norm(nm.grad_norm([t]), [t])
 
 
+@pytest.mark.parametrize("reader", ["dlpack", "attributes"])
+def test_lists_are_read_the_same_both_ways(nm, reader, monkeypatch):
+    base = randn(40, 50, seed=36)
+    tensors = [base, base[3:7], base[5], base.T, base[:, :1].contiguous(), base[:1, :1], base[2, 3], base[:0], base.view(-1)[7:],
+               base.bfloat16(), torch.nn.Parameter(base.clone()), base.view(40, 1, 50), base.view(-1)[1:1]]
+    if reader == "attributes":
+        monkeypatch.setattr(nm, "_reader", None)
+    ptrs, sizes, codes, contiguous = nm._flat("grads", tensors, 0)
+    assert not contiguous and list(sizes) == [t.numel() for t in tensors]
+    assert all(p == t.data_ptr() for p, t in zip(ptrs, tensors) if t.numel())
+    assert list(codes) == [int(t.dtype == BF16) for t in tensors]
+    tensors = [t for t in tensors if t.is_contiguous()]
+    ptrs, sizes, codes, contiguous = nm._flat("grads", tensors, 0)
+    assert contiguous and list(sizes) == [t.numel() for t in tensors]
+    assert all(p == t.data_ptr() for p, t in zip(ptrs, tensors) if t.numel())
+    assert_norm(nm.grad_norm(tensors), [t.detach() for t in tensors])
+    out = [torch.empty_like(t, requires_grad=False) for t in tensors]
+    want = clipped64([t.detach() for t in tensors], 3.0)
+    nm.clip_grads(tensors, 3.0, out=out)
+    assert_clipped(out, want)
+    for bad in (base.half(), base.double(), base.cpu(), base[:, ::2], base.to_sparse(), base[:1].expand(3, 50)):
+        with pytest.raises(ValueError):
+            nm.grad_norm([base, bad])
+    with pytest.raises(TypeError):
+        nm.grad_norm([base, 1.0])
+
+
 def test_gradient_norm_past_32_bits(nm):
     g = torch.empty(2**31 + 12345, dtype=BF16, device="cuda").normal_(generator=gen(35))
     want = sum(float(part.double().square().sum()) for part in g.split(2**28)) ** 0.5

@@ -141,3 +141,26 @@ def test_workspace_follows_the_shares_of_the_rows():
         assert lib.mace_layer_norm_grad_workspace(n, c, C.byref(need)) == nv.MACE_OK
         pitch = (2 * c + 3) // 4 * 16
         assert need.value % pitch == 0 and need.value // pitch <= min(n, n // 256 + 148 * 32)
+
+
+def test_lists_of_objects_are_read_through_dlpack():
+    """On tensors of the host: refused for their device, as are other objects (their reader's exception is raised)."""
+    from array import array
+
+    reader = nv.dlpack_reader(torch.Tensor)
+    if reader is None:
+        pytest.skip("this torch has no DLPack C exchange API")
+    read = nv.load_tensor_list()
+
+    def call(objects, device=0, reader=reader):
+        n = len(objects)
+        ids, out = array("Q", map(id, objects)), [array("Q", bytes(8 * n)), array("q", bytes(8 * n)), array("i", bytes(4 * n))]
+        return read(reader, n, ids.buffer_info()[0], device, *(a.buffer_info()[0] for a in out))
+
+    assert call([]) == nv.MACE_OK
+    assert call([torch.zeros(3)]) == nv.MACE_ERR_BAD_ARG
+    assert call([torch.zeros(3)], reader=None) == nv.MACE_ERR_BAD_ARG
+    for other in (1.0, None, "x"):
+        with pytest.raises(Exception):  # noqa: B017 (whatever the reader sets)
+            call([other])
+    assert nv.dlpack_reader(int) is None
