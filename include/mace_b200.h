@@ -581,6 +581,25 @@ int mace_grad_clip(int32_t count, const void* const* grads, const int64_t* sizes
 int mace_tensor_list(int (*read)(void* object, void* tensor), int32_t count, void* const* objects, int32_t device,
                      void** data, int64_t* sizes, int32_t* dtypes);
 
+/* The operands of a layer norm, read the same way: rows x (of any number of
+ * leading dimensions that lie one row stride apart), and where the object is not
+ * NULL the output gradient dy, weight and bias.  MACE_OK if they are operands
+ * that mace_layer_norm and mace_layer_norm_grad take, all on one CUDA device. */
+typedef struct {
+  int32_t dtype, param_dtype;
+  int32_t C, device;
+  int64_t n, x_stride, dy_stride;
+  const void *x, *dy, *weight, *bias;
+} mace_norm_rows;
+int mace_norm_rows_read(int (*read)(void* object, void* tensor), void* x, void* dy, void* weight, void* bias,
+                        mace_norm_rows* rows);
+
+/* mace_layer_norm and mace_layer_norm_grad on operands in a struct; the results
+ * at y and dx are contiguous. */
+int mace_norm_rows_forward(const mace_norm_rows* rows, float eps, int32_t activation, void* y, void* stream);
+int mace_norm_rows_backward(const mace_norm_rows* rows, float eps, int32_t activation, void* dx, void* dweight,
+                            void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

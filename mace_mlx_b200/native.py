@@ -118,6 +118,11 @@ class Outputs(C.Structure):
                 ("virial", C.c_void_p)]
 
 
+class NormRows(C.Structure):
+    _fields_ = [("dtype", i32), ("param_dtype", i32), ("C", i32), ("device", i32), ("n", i64), ("x_stride", i64),
+                ("dy_stride", i64), ("x", C.c_void_p), ("dy", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p)]
+
+
 class NativeError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"libmace_b200 error {code}: {msg}")
@@ -136,7 +141,8 @@ EXPORTED = (
     "mace_species_linear_wgrad_workspace", "mace_species_linear_wgrad", "mace_rows_checkpoint", "mace_rows_restore",
     "mace_species_error_flag",
     "mace_layer_norm", "mace_layer_norm_grad_workspace", "mace_layer_norm_grad", "mace_grad_norm_workspace",
-    "mace_grad_norm", "mace_grad_clip", "mace_tensor_list",
+    "mace_grad_norm", "mace_grad_clip", "mace_tensor_list", "mace_norm_rows_read", "mace_norm_rows_forward",
+    "mace_norm_rows_backward",
 )
 NOALLOC_MAX_ATOMS = 131072
 NOALLOC_MAX_GRAPH_ATOMS = 16384
@@ -218,6 +224,9 @@ def load_library(path: str | Path | None = None) -> C.CDLL:
         "mace_grad_norm": ([i32, vp, vp, vp, vp, vp, i64, vp], C.c_int),
         "mace_grad_clip": ([i32, vp, vp, vp, vp, vp, C.c_double, vp, vp, i64, vp], C.c_int),
         "mace_tensor_list": ([vp, i32, vp, i32, vp, vp, vp], C.c_int),
+        "mace_norm_rows_read": ([vp, vp, vp, vp, vp, vp], C.c_int),
+        "mace_norm_rows_forward": ([vp, f32, i32, vp, vp], C.c_int),
+        "mace_norm_rows_backward": ([vp, f32, i32, vp, vp, vp, vp, i64, vp], C.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -228,12 +237,11 @@ def load_library(path: str | Path | None = None) -> C.CDLL:
     return lib
 
 
-def load_tensor_list():
-    """``mace_tensor_list`` called with the interpreter's lock held, as it reads Python objects."""
-    load_library()
-    fn = C.PyDLL(str(LIB_PATH)).mace_tensor_list
-    fn.argtypes = [C.c_void_p, i32, C.c_void_p, i32, C.c_void_p, C.c_void_p, C.c_void_p]
-    fn.restype = C.c_int
+def load_reading(name: str):
+    """An entry that reads Python objects, called with the interpreter's lock held."""
+    typed = getattr(load_library(), name)
+    fn = getattr(C.PyDLL(str(LIB_PATH)), name)
+    fn.argtypes, fn.restype = typed.argtypes, typed.restype
     return fn
 
 

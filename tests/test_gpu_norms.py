@@ -495,6 +495,28 @@ def test_gradient_norm_in_any_order_of_dimensions(nm):
         assert_norm(nm.grad_norm([t]), [t])
 
 
+def test_operands_are_read_the_same_both_ways(nm, monkeypatch):
+    base, w = randn(24, 4, 96, seed=37), 1 + 0.1 * randn(96, seed=38)
+    b = randn(96, seed=39)
+    cases = [(t, w, b) for t in (base, base[:, 1], base[..., :96], base[0, 0], base[:1], base[::3, 2], base[:0], base[3:, :1],
+                                 base[:, :, None], base[2:3, 1:2], base[0, :1].expand(7, 96), base.view(6, 4, 4, 96)[:, :, 1])]
+    cases += [(base[..., 5:9], w[5:9], None), (base[..., :1], None, b[:1]), (base.bfloat16(), w, b), (base[:, 0, 7:8], w[:1], b[:1]),
+              (base.bfloat16()[:, 0], w.bfloat16(), b.bfloat16()), (torch.nn.Parameter(base[0].clone()), None, None)]
+    readers = [nm._reader, None]
+    assert nm._read_rows(base, base, w, b) is not None or readers[0] is None
+    for x, weight, bias in cases:
+        got = []
+        for reader in readers:
+            monkeypatch.setattr(nm, "_reader", reader)
+            assert reader is None or nm._read_rows(x, x, weight, bias) is not None
+            with torch.no_grad():
+                y = nm.layer_norm(x, weight, bias, activation="silu")
+                got.append([y, *nm.layer_norm_grad(x, x, weight, bias, activation="silu")])
+        assert got[0][0].shape == x.shape and got[0][0].is_contiguous()
+        for p, q in zip(*got):
+            assert (p is None and q is None) or (torch.equal(p, q) and p.dtype == q.dtype and p.stride() == q.stride())
+
+
 @pytest.mark.parametrize("reader", ["dlpack", "attributes"])
 def test_lists_are_read_the_same_both_ways(nm, reader, monkeypatch):
     base = randn(40, 50, seed=36)
@@ -800,7 +822,10 @@ def test_equal_calls_give_equal_bits(nm, dtype, n, c):
 
 
 # ------------------------------------------------------------------ refusals
-def test_refusals(nm):
+@pytest.mark.parametrize("reader", ["dlpack", "attributes"])
+def test_refusals(nm, reader, monkeypatch):
+    if reader == "attributes":
+        monkeypatch.setattr(nm, "_reader", None)
     x, w, b = torch.zeros(8, 16, device="cuda"), torch.ones(16, device="cuda"), torch.zeros(16, device="cuda")
     leaf = torch.zeros(8, 16, device="cuda", requires_grad=True)
     g, h = torch.zeros(40, device="cuda"), torch.zeros(40, device="cuda")

@@ -150,7 +150,7 @@ def test_lists_of_objects_are_read_through_dlpack():
     reader = nv.dlpack_reader(torch.Tensor)
     if reader is None:
         pytest.skip("this torch has no DLPack C exchange API")
-    read = nv.load_tensor_list()
+    read = nv.load_reading("mace_tensor_list")
 
     def call(objects, device=0, reader=reader):
         n = len(objects)
