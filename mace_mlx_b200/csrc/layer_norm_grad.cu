@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(1024) k_layer_norm_join(LayerNorm p) {
 
 // Few rows of up to 32 lanes go to one cluster of up to 16 CTAs, whose sums need no second launch and no workspace: up
 // to four steps of a CTA, where both take 5 us on the device (1000 rows of 128; 6.7 and 4.6 at twice as many steps), but
-// a call 15 us instead of 20 on the host.
+// a call 11.5 us instead of 15.4 on the host.
 constexpr int LN_FEW = 4, LN_CLUSTER = MOST_OF_CLUSTER;
 
 int64_t rows_at_once(int C) { return LN_THREADS / std::min(row_lanes(8, C, 0), 32); }

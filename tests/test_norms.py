@@ -2,6 +2,9 @@
 the C ABI (host-side argument checks only, no launch)."""
 
 import ctypes as C
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -126,8 +129,6 @@ def test_c_entries_check_lists_of_tensors():
 
 def test_kernels_read_their_inputs_by_plain_loads():
     """As the species operators' kernels: one may start while the kernel before it still writes its inputs."""
-    from pathlib import Path
-
     for name in ("layer_norm.cu", "layer_norm_grad.cu", "layer_norm.cuh", "grad_norm.cu"):
         text = (Path(mace_mlx_b200.__file__).parent / "csrc" / name).read_text()
         for form in ("__ldg(", "global.nc", "__restrict__"):
@@ -164,3 +165,28 @@ def test_lists_of_objects_are_read_through_dlpack():
         with pytest.raises(Exception):  # noqa: B017 (whatever the reader sets)
             call([other])
     assert nv.dlpack_reader(int) is None
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
+def test_struct_of_operands_matches_the_header(tmp_path):
+    fields = [name for name, _ in nv.NormRows._fields_]
+    prints = "".join(f'printf("%zu ", offsetof(mace_norm_rows, {f}));' for f in fields)
+    include = Path(mace_mlx_b200.__file__).resolve().parents[1] / "include"
+    (tmp_path / "l.c").write_text("#include <stdio.h>\n#include <stddef.h>\n#include \"mace_b200.h\"\n"
+                                  f'int main(void){{{prints}printf("%zu", sizeof(mace_norm_rows)); return 0;}}')
+    subprocess.run(["gcc", f"-I{include}", str(tmp_path / "l.c"), "-o", str(tmp_path / "l")], check=True)
+    got = subprocess.run([str(tmp_path / "l")], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(v) for v in got] == [*(getattr(nv.NormRows, f).offset for f in fields), C.sizeof(nv.NormRows)]
+
+
+def test_struct_entries_check_their_arguments():
+    lib = nv.load_library()
+    rows = nv.NormRows(dtype=0, param_dtype=0, C=8, device=0, n=4, x_stride=8, dy_stride=8, x=32, dy=32)
+    assert lib.mace_norm_rows_forward(None, 1e-5, 0, 32, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_norm_rows_backward(None, 1e-5, 0, 32, None, None, None, 0, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_norm_rows_forward(C.byref(rows), -1.0, 0, 32, None) == nv.MACE_ERR_BAD_ARG
+    assert lib.mace_norm_rows_backward(C.byref(rows), 1e-5, 7, 32, None, None, None, 0, None) == nv.MACE_ERR_BAD_ARG
+    if nv.dlpack_reader(torch.Tensor) is not None:
+        read, x = nv.load_reading("mace_norm_rows_read"), torch.zeros(4, 8)
+        for reader, obj in ((nv.dlpack_reader(torch.Tensor), x), (None, x)):  # (of the host; no reader)
+            assert read(reader, id(obj), None, None, None, C.byref(rows)) == nv.MACE_ERR_BAD_ARG
