@@ -584,7 +584,8 @@ int mace_tensor_list(int (*read)(void* object, void* tensor), int32_t count, voi
 /* The operands of a layer norm, read the same way: rows x (of any number of
  * leading dimensions that lie one row stride apart), and where the object is not
  * NULL the output gradient dy, weight and bias.  MACE_OK if they are operands
- * that mace_layer_norm and mace_layer_norm_grad take, all on one CUDA device. */
+ * that mace_layer_norm and mace_layer_norm_grad take, all on one CUDA device and
+ * with memory of their own. */
 typedef struct {
   int32_t dtype, param_dtype;
   int32_t C, device;

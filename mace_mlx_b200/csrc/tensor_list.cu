@@ -86,6 +86,7 @@ extern "C" int mace_norm_rows_read(int (*read)(void*, void*), void* x, void* dy,
   r.C = (int32_t)C;
   r.device = t.device_id;
   r.x = data_of(t);
+  if (!r.x && r.n > 0) return MACE_ERR_BAD_ARG;
   if (dy) {
     DlTensor g;
     int32_t dtype;
@@ -96,6 +97,7 @@ extern "C" int mace_norm_rows_read(int (*read)(void*, void*), void* x, void* dy,
     for (int32_t d = 0; d < t.ndim; ++d)
       if (g.shape[d] != t.shape[d]) return MACE_ERR_BAD_ARG;
     r.dy = data_of(g);
+    if (!r.dy && r.n > 0) return MACE_ERR_BAD_ARG;
   }
   r.param_dtype = r.dtype;
   void* const params[2] = {weight, bias};
@@ -107,7 +109,9 @@ extern "C" int mace_norm_rows_read(int (*read)(void*, void*), void* x, void* dy,
         q.ndim != 1 || q.shape[0] != C || (q.strides && q.strides[0] != 1 && C != 1) || (k == 1 && weight && dtype != r.param_dtype))
       return MACE_ERR_BAD_ARG;
     r.param_dtype = dtype;
-    (k == 0 ? r.weight : r.bias) = data_of(q);
+    void* const at = data_of(q);
+    if (!at) return MACE_ERR_BAD_ARG;  // (a tensor without memory: null would stand for no parameter)
+    (k == 0 ? r.weight : r.bias) = at;
   }
   *rows = r;
   return MACE_OK;

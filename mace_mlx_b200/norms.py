@@ -85,6 +85,8 @@ def _params(weight, bias, dev: int, c: int, dtype: torch.dtype) -> tuple[int, in
                 raise ValueError(f"{name} is {kind}, expected {dtype} or float32")
         elif t.dtype is not kind:
             raise ValueError(f"weight is {kind}, bias {t.dtype}: they must be of one type")
+        if not t.data_ptr():  # (null stands for no parameter in the C entries)
+            raise ValueError(f"{name} has no memory of its own (a wrapper of other tensors?)")
     return (_DTYPES[dtype if kind is None else kind], None if weight is None else weight.data_ptr(),
             None if bias is None else bias.data_ptr())
 

@@ -940,3 +940,27 @@ def test_examples_run_with_clipping(nm):
     assert len(losses) == len(sizes) == 5 and all(s > 0 for s in sizes)
     losses = example("species_head").train(n_structures=4, steps=5, max_norm=1e-3)
     assert len(losses) == 5 and all(x == x for x in losses)
+
+
+# --------------------------------------------- tensors that only look like some
+class Elsewhere(torch.Tensor):
+    """A tensor without memory of its own, as the wrappers of distributed tensors are."""
+
+    @staticmethod
+    def __new__(cls, *shape):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=F32, device=torch.device("cuda", 0))
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(func)
+
+
+@pytest.mark.parametrize("reader", ["dlpack", "attributes"])
+def test_tensors_without_memory_are_refused(nm, reader, monkeypatch):
+    if reader == "attributes":
+        monkeypatch.setattr(nm, "_reader", None)
+    x, w = randn(8, 16, seed=120), Elsewhere(16)
+    for call in (lambda: nm.layer_norm(x, w), lambda: nm.layer_norm(x, None, w), lambda: nm.layer_norm(x, w, out=x.clone()),
+                 lambda: nm.layer_norm_grad(x, x, w), lambda: nm.layer_norm_grad(x, x, x[0], w)):
+        with pytest.raises(ValueError, match="no memory"):
+            call()

@@ -190,3 +190,53 @@ def test_struct_entries_check_their_arguments():
         read, x = nv.load_reading("mace_norm_rows_read"), torch.zeros(4, 8)
         for reader, obj in ((nv.dlpack_reader(torch.Tensor), x), (None, x)):  # (of the host; no reader)
             assert read(reader, id(obj), None, None, None, C.byref(rows)) == nv.MACE_ERR_BAD_ARG
+
+
+class Elsewhere(torch.Tensor):
+    """A tensor without memory of its own, as the wrappers of distributed tensors are."""
+
+    @staticmethod
+    def __new__(cls, *shape, dtype=torch.float32):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype, device=torch.device("cuda", 0))
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(func)
+
+
+def test_parameters_without_memory_are_refused():
+    """A null address stands for no weight in the C entries: that of a parameter must not get there."""
+    for pair in ((Elsewhere(8), None), (None, Elsewhere(8)), (Elsewhere(8, dtype=torch.bfloat16),) * 2):
+        with pytest.raises(ValueError, match="no memory"):
+            norms._params(*pair, 0, 8, torch.bfloat16)
+
+
+def test_the_reader_of_operands_refuses_null_addresses():
+    class Tensor(C.Structure):
+        _fields_ = [("data", C.c_void_p), ("device_type", C.c_int32), ("device_id", C.c_int32), ("ndim", C.c_int32),
+                    ("code", C.c_uint8), ("bits", C.c_uint8), ("lanes", C.c_uint16), ("shape", C.POINTER(C.c_int64)),
+                    ("strides", C.POINTER(C.c_int64)), ("byte_offset", C.c_uint64)]
+
+    shapes = {1: (4, 8), 2: (4, 8), 3: (8,), 4: (8,), 5: (0, 8)}
+    memory = {k: ((C.c_int64 * len(s))(*s), s) for k, s in shapes.items()}
+    null = set()
+
+    @C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_void_p)
+    def read(key, tensor):  # fp32 tensors on CUDA device 0, at addresses that nothing reads
+        shape, sizes = memory[key]
+        t = Tensor.from_address(tensor)
+        t.data, t.device_type, t.device_id, t.ndim = None if key in null else 4096 * key, 2, 0, len(sizes)
+        t.code, t.bits, t.lanes, t.shape, t.strides, t.byte_offset = 2, 32, 1, shape, None, 0
+        return 0
+
+    entry = nv.load_reading("mace_norm_rows_read")
+    fn, rows = C.cast(read, C.c_void_p), nv.NormRows()
+    assert entry(fn, 1, 2, 3, 4, C.byref(rows)) == nv.MACE_OK
+    assert (rows.x, rows.dy, rows.weight, rows.bias) == (4096, 8192, 12288, 16384)
+    for key in (1, 2, 3, 4):
+        null.clear()
+        null.add(key)
+        assert entry(fn, 1, 2, 3, 4, C.byref(rows)) == nv.MACE_ERR_BAD_ARG, key
+    null.clear()
+    null.add(5)
+    assert entry(fn, 5, 5, 3, 4, C.byref(rows)) == nv.MACE_OK  # (no rows have no memory)
