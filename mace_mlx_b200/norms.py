@@ -306,7 +306,8 @@ def _grads(grads: Iterable[torch.Tensor | None]) -> list[torch.Tensor]:
 
 def _norm_of(grads: list[torch.Tensor], dev: int, flat, fn, *more) -> torch.Tensor:
     ptrs, sizes, codes, _ = flat
-    norm = grads[0].new_empty((), dtype=torch.float32) if grads else torch.empty((), device=torch.device("cuda", dev))
+    norm = (grads[0].new_empty((), dtype=torch.float32) if grads
+            else torch.empty((), dtype=torch.float32, device=torch.device("cuda", dev)))
     # (the number of values tells few tensors from small ones)
     values = sum(sizes) if len(grads) <= nv.GRAD_FEW_TENSORS else 0
     ws, wptr, nbytes = _workspace("mace_grad_norm_workspace", dev, norm, len(grads), values)

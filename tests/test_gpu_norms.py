@@ -964,3 +964,14 @@ def test_tensors_without_memory_are_refused(nm, reader, monkeypatch):
                  lambda: nm.layer_norm_grad(x, x, w), lambda: nm.layer_norm_grad(x, x, x[0], w)):
         with pytest.raises(ValueError, match="no memory"):
             call()
+
+
+@pytest.mark.parametrize("default", [torch.float64, BF16])
+def test_the_norm_of_nothing_under_other_default_types(nm, default):
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(default)
+        got = [nm.grad_norm([]), nm.grad_norm([None]), nm.clip_grads([], 1.0), nm.clip_grads([None], 1.0, out=[None])]
+    finally:
+        torch.set_default_dtype(before)
+    assert all(t.dtype == F32 and float(t) == 0.0 for t in got)

@@ -240,3 +240,21 @@ def test_the_reader_of_operands_refuses_null_addresses():
     null.clear()
     null.add(5)
     assert entry(fn, 5, 5, 3, 4, C.byref(rows)) == nv.MACE_OK  # (no rows have no memory)
+
+
+@pytest.mark.parametrize("default", [torch.float32, torch.float64, torch.bfloat16])
+def test_the_norm_of_nothing_is_fp32(default, monkeypatch):
+    """Four bytes are written whatever the program's default type is."""
+    empty, launched = torch.empty, []
+    monkeypatch.setattr(torch, "empty", lambda *a, device=None, **k: empty(*a, **k))  # (here on the host)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(norms, "_workspace", lambda *a: (None, None, 0))
+    monkeypatch.setattr(norms, "_launch", lambda *a: launched.append(a))
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(default)
+        for norm in (norms.grad_norm([]), norms.grad_norm([None]), norms.clip_grads([], 1.0), norms.clip_grads([None], 1.0)):
+            assert norm.dtype == torch.float32
+    finally:
+        torch.set_default_dtype(before)
+    assert len(launched) == 4
