@@ -524,8 +524,11 @@ int mace_species_error_flag(int32_t* flag);
 /*
  * y[i] = f(weight * (x[i] - mean) / sqrt(var + eps) + bias) for n rows of C
  * channels (strides in elements; x rows may overlap or repeat, y rows must not,
- * and y must not overlap x), f the identity or SiLU.  weight and bias hold
- * param_dtype; NULL stands for ones and zeros.
+ * and y must not overlap x, weight or bias: refused), f the identity or SiLU.
+ * Rows of one table beside each other do not overlap; rows of unlike strides
+ * that lie between each other count as overlapping where the strides' common
+ * divisor does not keep them apart.  weight and bias hold param_dtype; NULL
+ * stands for ones and zeros.
  */
 int mace_layer_norm(int32_t dtype, const void* x, int64_t x_stride, int32_t param_dtype, const void* weight,
                     const void* bias, int64_t n, int32_t C, float eps, int32_t activation, void* y, int64_t y_stride,
@@ -535,8 +538,8 @@ int mace_layer_norm(int32_t dtype, const void* x, int64_t x_stride, int32_t para
  * Gradients of mace_layer_norm for the output gradient dy: dx (n rows of C),
  * dweight and dbias (C values of param_dtype); any may be NULL (not wanted).
  * The workspace (16-byte aligned) serves dweight and dbias; few rows need none.
- * dx must not overlap x or dy.  The order of all sums depends on the sizes and
- * types and on the addresses modulo 16 alone.
+ * dx must not overlap x, dy, weight or bias (refused as above).  The order of
+ * all sums depends on the sizes and types and on the addresses modulo 16 alone.
  */
 int mace_layer_norm_grad_workspace(int64_t n, int32_t C, int64_t* bytes);
 int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride,

@@ -149,6 +149,12 @@ extern "C" int mace_layer_norm(int32_t dtype, const void* x, int64_t xs, int32_t
     return fail(MACE_ERR_BAD_ARG, "mace_layer_norm: bad arguments");
   if (unaligned(value_size(dtype), x, y) || unaligned(value_size(param_dtype), weight, bias))
     return fail(MACE_ERR_BAD_ARG, "mace_layer_norm: an address is not a multiple of its values' size");
+  const Span out{y, ys, value_size(dtype), false};
+  for (const void* param : {weight, bias})
+    if (rows_meet(out, {param, 0, value_size(param_dtype), true}, n, C))
+      return fail(MACE_ERR_BAD_ARG, "mace_layer_norm: the result overlaps a parameter");
+  if (rows_meet(out, {x, xs, value_size(dtype), false}, n, C))
+    return fail(MACE_ERR_BAD_ARG, "mace_layer_norm: the result overlaps x");
   if (n == 0) return MACE_OK;
   LayerNorm p{};
   p.x = x, p.xs = n > 1 ? xs : 0, p.w = weight, p.b = bias, p.param_f32 = param_dtype == MACE_F32, p.n = n, p.C = C;

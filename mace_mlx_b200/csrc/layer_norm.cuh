@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <numeric>
 
 #include "common.cuh"
 #include "species.cuh"
@@ -597,6 +598,27 @@ inline bool bad_rows(int32_t dtype, int32_t param_dtype, int64_t n, int32_t C, f
   return (dtype != MACE_F32 && dtype != MACE_BF16) || (param_dtype != MACE_F32 && param_dtype != MACE_BF16) || n < 0 ||
          n > INT32_MAX || C < 1 || C > MACE_LAYER_NORM_MAX_CHANNELS || !(eps >= 0.f) || !std::isfinite(eps) ||
          (activation != MACE_ACT_NONE && activation != MACE_ACT_SILU);
+}
+
+// Whether n rows of C values that are written meet what is read: n rows as well, or `one` of C values.  Rows of two
+// strides lie apart where no multiple of the strides' common divisor brings one to the other: exact for equal strides
+// (slots of one table) and for one row; interleaved rows of unlike strides count as meeting unless that shows them apart.
+struct Span {
+  const void* at;  // null: none
+  int64_t stride;  // in values
+  int size;        // of a value
+  bool one;
+};
+inline bool rows_meet(const Span& out, const Span& in, int64_t n, int C) {
+  if (!out.at || !in.at || n < 1) return false;
+  const int64_t row_out = (int64_t)C * out.size, row_in = (int64_t)C * in.size;
+  const int64_t step_out = n > 1 ? out.stride * out.size : 0, step_in = n > 1 && !in.one ? in.stride * in.size : 0;
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out.at), i = reinterpret_cast<uintptr_t>(in.at);
+  if (o + (n - 1) * step_out + row_out <= i || i + (n - 1) * step_in + row_in <= o) return false;
+  const int64_t period = std::gcd(step_out, step_in);
+  if (period == 0) return true;
+  const int64_t d = (int64_t)(i - o) % period, behind = d < 0 ? d + period : d;  // of a row that is read behind one that is written
+  return behind < row_out || period - behind < row_in;
 }
 
 // f(layout, values) of a plan as constants

@@ -312,6 +312,12 @@ extern "C" int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t xs, co
   mace_layer_norm_grad_workspace(n, C, &need);
   if (params && need > 0 && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15) != 0))
     return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad: workspace too small or not 16-byte aligned");
+  const Span out{dx, dxs, value_size(dtype), false};
+  for (const void* param : {weight, bias})
+    if (rows_meet(out, {param, 0, value_size(param_dtype), true}, n, C))
+      return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad: dx overlaps a parameter");
+  if (rows_meet(out, {x, xs, value_size(dtype), false}, n, C) || rows_meet(out, {dy, ds, value_size(dtype), false}, n, C))
+    return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad: dx overlaps x or dy");
   const bool cluster = params && n > 0 && few_rows(n, C);
   LayerNorm p{};
   p.x = x, p.xs = n > 1 ? xs : 0, p.dy = dy, p.ds = n > 1 ? ds : 0, p.w = weight, p.b = bias;

@@ -194,7 +194,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     ``activation`` is None (f the identity) or ``"silu"``.  x is float32 or
     bfloat16, (..., C) with contiguous channels and rows at one stride, so a
     slot of a node-feature table is passed in place; so may ``out``, which must
-    not overlap x.  weight and bias (C,), either or both, are of x's type or
+    not overlap x, weight or bias.  weight and bias (C,), either or both, are of x's type or
     float32; without them they are ones and zeros.
 
     Statistics and products are fp32, rounded once to x's type.  Deviations

@@ -975,3 +975,30 @@ def test_the_norm_of_nothing_under_other_default_types(nm, default):
     finally:
         torch.set_default_dtype(before)
     assert all(t.dtype == F32 and float(t) == 0.0 for t in got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [16, 33])
+def test_results_beside_operands(nm, dtype, c):
+    """Slots of one table, rows with a row between them and rows behind the last are taken; what overlaps is refused."""
+    from mace_mlx_b200.native import NativeError
+
+    n = 12
+    table, w, b = randn(n, 3 * c, seed=121, dtype=dtype), 1 + 0.1 * randn(c, seed=122), randn(c, seed=123)
+    flat = table.view(-1)
+    rows = table.view(3 * n, c)
+    for x, out in ((table[:, :c], table[:, c:2 * c]), (table[:, :c], table[:, 2 * c:]), (table[:, 2 * c:], table[:, c:2 * c]),
+                   (rows[::6], rows[1::3][:6]), (rows[::6], rows[3::6]), (rows[:6], rows[6:12]), (rows[6:12], rows[:6]),
+                   (rows[5], rows[6]), (rows[:1].expand(6, c), rows[1:7])):
+        ref = Rows64(x.reshape(-1, c).clone(), w, b, 1e-5, False).forward()
+        assert_close(nm.layer_norm(x, w, b, out=out).reshape(-1, c), *ref)
+    for x, out in ((rows, rows), (rows[:6], rows[5:11]), (table[:, :c], table[:, 1:c + 1]), (table[:, 1:c + 1], table[:, :c]),
+                   (table[:, :c], table[:, c - 1:2 * c - 1]),
+                   (rows[:1].expand(6, c), rows[:6]), (rows[5], rows[5]), (flat[:6 * c].view(6, c), flat[3:6 * c + 3].view(6, c))):
+        before = table.clone()
+        with pytest.raises(NativeError, match="overlaps x"):
+            nm.layer_norm(x, w, b, out=out)
+        assert torch.equal(before, table)
+    with pytest.raises(NativeError, match="overlaps a parameter"):
+        nm.layer_norm(table[:, :c], table[1, c:2 * c], out=table[:, c:2 * c])
+    nm.layer_norm(table[:, :c], table[1, 2 * c:], out=table[:, c:2 * c])

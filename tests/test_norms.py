@@ -258,3 +258,30 @@ def test_the_norm_of_nothing_is_fp32(default, monkeypatch):
     finally:
         torch.set_default_dtype(before)
     assert len(launched) == 4
+
+
+def test_results_over_operands_are_refused():
+    """Rows that lie between each other without meeting are told from rows that meet (the calls that are taken, as slots
+    of one table, run on the GPU)."""
+    lib = nv.load_library()
+
+    def forward(x, xs, y, ys, n=5, c=8, w=None, b=None, dtype=0, param=0):
+        rc = lib.mace_layer_norm(dtype, x, xs, param, w, b, n, c, 1e-5, 0, y, ys, None)
+        return rc == nv.MACE_ERR_BAD_ARG and "overlaps" in nv.last_error(lib)
+
+    def backward(x, xs, dy, ds, dx, dxs, n=5, c=8, w=None, b=None):
+        rc = lib.mace_layer_norm_grad(0, x, xs, dy, ds, 0, w, b, n, c, 1e-5, 0, dx, dxs, None, None, None, 0, None)
+        return rc == nv.MACE_ERR_BAD_ARG and "overlaps" in nv.last_error(lib)
+
+    at = 1 << 20
+    size = 4 * 8  # of a row
+    assert forward(at, 8, at, 8) and forward(at, 8, at + 4, 8) and forward(at + 4, 8, at, 8)
+    assert forward(at, 8, at + 5 * size - 4, 8) and forward(at, 20, at + 28, 20) and forward(at, 20, at + 4 * 80 + 28, 20)
+    assert forward(at + 3 * size, 0, at, 8) and forward(at, 8, at, 20) and forward(at, 8, at + 8, 20, n=1)
+    assert forward(at, 12, at + 32, 8) and forward(at, 16, at + 32, 24)  # unlike strides: x meets the second row of y
+    assert forward(at, 16, at + 16 * 6 - 2, 16, dtype=1) and forward(at, 16, at + 16, 16, c=9, dtype=1)
+    assert forward(at, 8, at + (1 << 16), 8, w=at + (1 << 16) + 4 * size + 4) and forward(at, 8, at + 4096, 20, b=at + 4096 + 76)
+    assert forward(at, 8, at + 4096, 8, w=at + 4096 - 4, dtype=1, param=0)
+    other = at + (1 << 16)
+    assert backward(at, 8, other, 8, at, 8) and backward(at, 8, other, 8, other + 16, 8) and backward(at, 0, other, 0, other - 64, 8)
+    assert backward(at, 8, at, 8, other, 8, w=other) and backward(at, 8, at, 8, other, 8, b=other + 4 * size + 28)
