@@ -28,6 +28,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import operator
 from array import array
 from collections.abc import Iterable, Sequence
 
@@ -91,6 +92,13 @@ def _params(weight, bias, dev: int, c: int, dtype: torch.dtype) -> tuple[int, in
             None if bias is None else bias.data_ptr())
 
 
+def _written(name: str, t: torch.Tensor) -> None:
+    """Refuses to write, unseen by autograd, to a tensor that it follows."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and what is written to it here has none: pass a tensor that needs "
+                         "none (a parameter's .grad, a detached one), or call under torch.no_grad()")
+
+
 def _like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
@@ -139,6 +147,7 @@ def _layer_norm(x, dev, weight, bias, eps, activation, out):
     else:
         y = out
         _on("out", y, dev)
+        _written("out", y)
         if y.dtype != x.dtype or y.shape != x.shape:
             raise ValueError(f"out must be {x.dtype} {tuple(x.shape)}, got {y.dtype} {tuple(y.shape)}")
         _, _, ys = _rows("out", y)
@@ -304,6 +313,9 @@ def _grads(grads: Iterable[torch.Tensor | None]) -> list[torch.Tensor]:
     return [g for g in grads if g is not None]
 
 
+_requires = operator.attrgetter("requires_grad")
+
+
 def _norm_of(grads: list[torch.Tensor], dev: int, flat, fn, *more) -> torch.Tensor:
     ptrs, sizes, codes, _ = flat
     norm = (grads[0].new_empty((), dtype=torch.float32) if grads
@@ -336,7 +348,9 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
     norm on the host.  With ``out`` (a tensor for every gradient, with as many
     values in the same order in memory, float32 or bfloat16) the results go there and the
     gradients stay, unless ``out`` holds the gradient itself.  No tensor that
-    is written may overlap another one of the call, so none may be listed twice.
+    is written may overlap another one of the call, so none may be listed twice,
+    and under grad mode none may require a gradient: pass the parameters'
+    gradients, not the parameters.
 
     A norm that is NaN makes every gradient NaN; an infinite one makes the
     finite values zero and the others NaN: test the norm where that can occur.
@@ -361,6 +375,9 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
                 if o.numel() != g.numel() or o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
                     raise ValueError(f"out[{i}] must be {tuple(g.shape)} with strides {g.stride()}, got {tuple(o.shape)} "
                                      f"with strides {o.stride()}")
+    if torch.is_grad_enabled() and any(map(_requires, into)):
+        for i, t in enumerate(into):
+            _written(f"{'grads' if out is None else 'out'}[{i}]", t)
     norm = _norm_of(grads, dev, flat, nv.load_library().mace_grad_clip, ptrs.buffer_info()[0], codes.buffer_info()[0],
                     max_norm)
     torch.autograd.graph.increment_version(into)

@@ -1002,3 +1002,28 @@ def test_results_beside_operands(nm, dtype, c):
     with pytest.raises(NativeError, match="overlaps a parameter"):
         nm.layer_norm(table[:, :c], table[1, c:2 * c], out=table[:, c:2 * c])
     nm.layer_norm(table[:, :c], table[1, 2 * c:], out=table[:, c:2 * c])
+
+
+# ------------------------------------------- tensors that autograd follows
+def test_writes_unseen_by_autograd_are_refused(nm):
+    """Parameters in place of their gradients, results into parameters: refused under grad mode, as torch does."""
+    leaf = torch.nn.Parameter(randn(40, seed=124))
+    carried = leaf * 2.0  # (has a graph)
+    g, h = randn(40, seed=125), torch.zeros(40, device="cuda")
+    x, into = randn(8, 16, seed=126), torch.zeros(8, 16, device="cuda", requires_grad=True)
+    before, kept = leaf.detach().clone(), g.clone()
+    for call in (lambda: nm.clip_grads([leaf], 0.1), lambda: nm.clip_grads([g, leaf], 0.1), lambda: nm.clip_grads([carried], 0.1),
+                 lambda: nm.clip_grads([None, g], 0.1, out=[None, leaf]), lambda: nm.clip_grads(iter([leaf]), 1e9),
+                 lambda: nm.layer_norm(x, out=into)):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+    assert torch.equal(leaf, before) and torch.equal(g, kept) and not into.any()
+    with torch.no_grad():
+        nm.clip_grads([leaf], 0.1)
+        nm.layer_norm(x, out=into)
+    assert_clipped([leaf.detach()], clipped64([before], 0.1))
+    assert torch.equal(into, nm.layer_norm(x))
+    nm.clip_grads([g], 0.1, out=[h])
+    now = leaf.detach().clone()
+    nm.clip_grads([leaf.detach()], 0.01)
+    assert_clipped([leaf.detach()], clipped64([now], 0.01))
