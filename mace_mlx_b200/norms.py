@@ -233,7 +233,8 @@ def layer_norm_grad(x: torch.Tensor, grad: torch.Tensor, weight: torch.Tensor | 
                     ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
     """Gradients of ``layer_norm`` at x, weight and bias for the output gradient ``grad``.
 
-    Those of weight and bias have their type (None without them); their sums
+    They have no graph, whatever the arguments require.  Those of weight and
+    bias have their type (None without them); their sums
     over the rows are fp32, in an order that depends on the sizes, the types and
     the addresses modulo 16 alone, so equal calls give equal bits.
     """
@@ -316,6 +317,15 @@ def _grads(grads: Iterable[torch.Tensor | None]) -> list[torch.Tensor]:
 _requires = operator.attrgetter("requires_grad")
 
 
+def _without_graph(grads: list[torch.Tensor]) -> None:
+    """Refuses, under grad mode, gradients that have a graph themselves: what is made of them here would have none."""
+    if torch.is_grad_enabled() and any(map(_requires, grads)):
+        for i, g in enumerate(grads):
+            if not g.is_leaf:
+                raise ValueError(f"grads[{i}] has a graph (create_graph=True?), which would end here without a word: detach it "
+                                 "or call under torch.no_grad(); a norm to differentiate is torch.linalg.vector_norm's")
+
+
 def _norm_of(grads: list[torch.Tensor], dev: int, flat, fn, *more) -> torch.Tensor:
     ptrs, sizes, codes, _ = flat
     norm = (grads[0].new_empty((), dtype=torch.float32) if grads
@@ -333,11 +343,15 @@ def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
 
     The gradients are float32 or bfloat16 (mixed as they come), on one device,
     without gaps in their memory; entries that are None (parameters without a
-    gradient) are passed over.  Squares are summed in fp64.
+    gradient) are passed over.  Squares are summed in fp64.  The norm has no
+    graph: leaves are taken by their values, and gradients with a graph of their
+    own (``create_graph=True``) are refused under grad mode.
     """
     grads = _grads(grads)
     dev = _cuda("grads[0]", grads[0]) if grads else torch.cuda.current_device()
-    return _norm_of(grads, dev, _flat("grads", grads, dev), nv.load_library().mace_grad_norm)
+    flat = _flat("grads", grads, dev)
+    _without_graph(grads)
+    return _norm_of(grads, dev, flat, nv.load_library().mace_grad_norm)
 
 
 def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
@@ -366,6 +380,7 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
     flat = _flat("grads", grads, dev)
     into, ptrs, codes = grads, flat[0], flat[2]
     if out is not None:
+        _without_graph(grads)
         if len(out) != len(every):
             raise ValueError(f"out has {len(out)} tensors, grads {len(every)}")
         into = list(out) if len(grads) == len(every) else [o for o, g in zip(out, every) if g is not None]

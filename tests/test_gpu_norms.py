@@ -1027,3 +1027,22 @@ def test_writes_unseen_by_autograd_are_refused(nm):
     now = leaf.detach().clone()
     nm.clip_grads([leaf.detach()], 0.01)
     assert_clipped([leaf.detach()], clipped64([now], 0.01))
+
+
+def test_gradients_with_a_graph_are_refused(nm):
+    """A gradient penalty on grad_norm would train nothing."""
+    w = randn(30, seed=127).requires_grad_()
+    (g,) = torch.autograd.grad((w**3).sum(), w, create_graph=True)
+    h = torch.zeros(30, device="cuda")
+    for call in (lambda: nm.grad_norm([g]), lambda: nm.grad_norm([h, g]), lambda: nm.clip_grads([h, g], 1.0, out=[h.clone(), h.clone()])):
+        with pytest.raises(ValueError, match="graph"):
+            call()
+    want = [g.detach()]
+    assert_norm(nm.grad_norm([g.detach()]), want)
+    with torch.no_grad():
+        assert_norm(nm.grad_norm([g]), want)
+        assert_norm(nm.clip_grads([g], 1.0, out=[h]), want)
+    assert_clipped([h], clipped64(want, 1.0))
+    norm = nm.grad_norm([w])  # of a leaf: by its values
+    assert_norm(norm, [w.detach()])
+    assert not norm.requires_grad
