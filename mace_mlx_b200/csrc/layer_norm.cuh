@@ -84,18 +84,24 @@ struct Lane {
   int first[K];  // channel of a piece's first value
   int count[K];  // channels of the row in a piece
   uint32_t keep[WORDS];
-  float off;     // values of the lane that are not the row's
+  static constexpr bool BY_PIECE = LAYOUT == PIECES && sizeof(T) == 4;
+  float has[BY_PIECE ? K : 1];  // 1 for a piece that has a value of the row, 0 for others
+  float off;     // values of the lane that are not the row's (BY_PIECE: in pieces that have one)
   bool some;     // or all are
   // head: values between a 16-byte address and the row's start
   __device__ __forceinline__ Lane(int lane, int lanes, int C, int head) {
-    int all = 0;
+    int all = 0, others = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       first[k] = (k * lanes + lane) * V - head;
       count[k] = LAYOUT == FULL ? V : max(0, min(first[k] + V, C) - max(first[k], 0));
       all += count[k];
+      if constexpr (BY_PIECE) {
+        has[k] = any(k) ? 1.f : 0.f;
+        if (any(k)) others += V - count[k];
+      }
     }
-    off = (float)(N - all);
+    off = (float)(BY_PIECE ? others : N - all);
     some = all > 0;
     if constexpr (LAYOUT != FULL) {
 #pragma unroll
@@ -108,6 +114,13 @@ struct Lane {
   __device__ __forceinline__ bool in(int j, int C) const { return LAYOUT == FULL || (at(j) >= 0 && at(j) < C); }
   __device__ __forceinline__ bool whole(int k) const { return LAYOUT == FULL || count[k] == V; }
   __device__ __forceinline__ bool any(int k) const { return LAYOUT == FULL || count[k] > 0; }
+
+  // zeros for the values that are not the row's
+  __device__ __forceinline__ void clear(float2* v) const {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      v[i] = make_float2(__uint_as_float(__float_as_uint(v[i].x) & keep[2 * i]), __uint_as_float(__float_as_uint(v[i].y) & keep[2 * i + 1]));
+  }
 
   __device__ __forceinline__ void param(const void* p, int f32, float missing, int C, float2* v) const {
     float t[N];
@@ -380,11 +393,15 @@ __device__ __forceinline__ float2 tree(float2* v) {  // (v is used up)
 }
 // A row's values become xhat; rstd is returned.  lead: one of the row's values, which those that are not the row's hold
 // too.  Sums are taken of x - lead: a row of equal values comes out as zeros, an offset common to the row costs no
-// accuracy, and lead is never further from the mean than sqrt(C) standard deviations.  The values that are not the
-// row's are then -mean, whose squares are taken off their lane's sum (its error, `off` units in the last place of
-// mean^2, is below that of the row's own sum, which holds mean^2 once: lead is one of its values).
+// accuracy, and lead is never further from the mean than sqrt(C) standard deviations: a row whose first value is alone in
+// size loses that many units in the last place, others a few.
+//   The values that are not the row's are then -mean.  fp32 rows leave out the squares of pieces that have none of the
+// row's values; of the pieces at a row's ends, and in 16 bits of all, they are taken off their lane's sum, with an error of
+// a unit in the last place of mean^2 for each.  (The row's own sum holds mean^2 once, for lead: all that are off in a lane of
+// a one-hot row of 4097 would make rstd wrong by 6e-5, below 16 bits' 2^-9.)
 template <typename T, Layout LAYOUT, int N, typename Sum>
 __device__ __forceinline__ float normalise(const Lane<T, LAYOUT, N>& at, float2* v, float lead, const LayerNorm& p, Sum& sum) {
+  using At = Lane<T, LAYOUT, N>;
   constexpr int H = N / 2;
   float2 a[H];
 #pragma unroll
@@ -393,15 +410,31 @@ __device__ __forceinline__ float normalise(const Lane<T, LAYOUT, N>& at, float2*
   const float mean = sum(s.x + s.y) * p.inv_C;
 #pragma unroll
   for (int i = 0; i < H; ++i) v[i] = add2(v[i], both(-mean));
-  float2 q0 = mul2(v[0], v[0]), q1 = mul2(v[1], v[1]);
+  float q = 0.f;
+  if constexpr (At::BY_PIECE) {
+    constexpr int P = At::V / 2;
 #pragma unroll
-  for (int i = 2; i < H; i += 2) {
-    q0 = fma2(v[i], v[i], q0);
-    q1 = fma2(v[i + 1], v[i + 1], q1);
+    for (int k = 0; k < At::K; ++k) {
+      float2 qk = mul2(v[k * P], v[k * P]);
+#pragma unroll
+      for (int i = 1; i < P; ++i) qk = fma2(v[k * P + i], v[k * P + i], qk);
+      q = fmaf(qk.x + qk.y, at.has[k], q);
+    }
+  } else {
+    if constexpr (LAYOUT == APART && sizeof(T) == 4) at.clear(v);
+    float2 q0 = mul2(v[0], v[0]), q1 = mul2(v[1], v[1]);
+#pragma unroll
+    for (int i = 2; i < H; i += 2) {
+      q0 = fma2(v[i], v[i], q0);
+      q1 = fma2(v[i + 1], v[i + 1], q1);
+    }
+    const float2 qq = add2(q0, q1);
+    q = qq.x + qq.y;
   }
-  const float2 qq = add2(q0, q1);
-  float q = qq.x + qq.y;
-  if (LAYOUT != FULL) q = at.some ? fmaf(-at.off * mean, mean, q) : 0.f;
+  if (At::BY_PIECE)
+    q = fmaf(-at.off * mean, mean, q);
+  else if (LAYOUT == PIECES || (LAYOUT == APART && sizeof(T) == 2))
+    q = at.some ? fmaf(-at.off * mean, mean, q) : 0.f;
   const float rstd = rsqrtf(fmaf(sum(q), p.inv_C, p.eps));
 #pragma unroll
   for (int i = 0; i < H; ++i) v[i] = mul2(v[i], both(rstd));
