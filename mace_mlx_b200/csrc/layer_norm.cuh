@@ -435,7 +435,9 @@ __device__ __forceinline__ float normalise(const Lane<T, LAYOUT, N>& at, float2*
     q = fmaf(-at.off * mean, mean, q);
   else if (LAYOUT == PIECES || (LAYOUT == APART && sizeof(T) == 2))
     q = at.some ? fmaf(-at.off * mean, mean, q) : 0.f;
-  const float rstd = rsqrtf(fmaf(sum(q), p.inv_C, p.eps));
+  // (a lane's share of the variance: values of up to 1e18, whose 2e18 of deviation 16 values of a lane square to less than
+  // 2^128, in rows of any width)
+  const float rstd = rsqrtf(sum(q * p.inv_C) + p.eps);
 #pragma unroll
   for (int i = 0; i < H; ++i) v[i] = mul2(v[i], both(rstd));
   return rstd;

@@ -207,7 +207,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     float32; without them they are ones and zeros.
 
     Statistics and products are fp32, rounded once to x's type.  Deviations
-    from the mean are squared in fp32: rows whose values pass 1e18 lose them.
+    from the mean are squared in fp32: rows whose values pass 1e18 lose them,
+    and with ``eps`` 0 rows whose deviations all stay below 1e-18.
     """
     dev = _cuda("x", x)
     if torch.is_grad_enabled() and (x.requires_grad or _requires_grad("weight", weight) or _requires_grad("bias", bias)):

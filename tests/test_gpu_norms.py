@@ -1071,3 +1071,16 @@ def test_one_hot_rows(nm, c):
         grads = nm.layer_norm_grad(x, dy, w, b, activation=act)
         for name, value, (want, bound) in zip(("dx", "dw", "db"), grads, ref.backward(dy)):
             assert_close(value, want, bound, name, norm=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [16, 97, 340, 513, 2048, 8191, 8192])
+def test_values_up_to_1e18_in_rows_of_any_width(nm, dtype, c):
+    x, dy, w, b = inputs(11, c, F32, F32, seed=141)
+    x = (x / x.abs().max() * 0.99e18).to(dtype)
+    x[3] = torch.where(torch.arange(c, device="cuda") % 2 == 0, 0.99e18, -0.99e18).to(dtype)  # as far apart as they go
+    for eps in (0.0, 1e-5):
+        check_rows(nm, x, dy.to(dtype), w, b, eps=eps, norm=False)
+        check_rows(nm, x, (dy * 1e18).to(dtype), w, b, eps=eps, silu=True, norm=False)
+    small = (x.double() * 1e-36).to(dtype)  # (deviations of 1e-18)
+    check_rows(nm, small, (dy * 1e-18).to(dtype), w, b, eps=0.0, norm=False)
