@@ -14,7 +14,7 @@ namespace mace {
 
 namespace {
 
-template <bool SILU, int N, bool SHARED>
+template <typename T, bool SILU, int N, bool SHARED>
 __device__ __forceinline__ void affine(float2* v, const Params<N, SHARED>& params) {
 #pragma unroll
   for (int c = 0; c < N / 8; ++c) {
@@ -26,7 +26,7 @@ __device__ __forceinline__ void affine(float2* v, const Params<N, SHARED>& param
   }
   if (SILU) {
     float2 s[N / 2];
-    sigmoid<N / 2>(v, s);
+    sigmoid<T, N / 2>(v, s);
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) v[i] = mul2(v[i], s[i]);
   }
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(LN_THREADS, LN_PER_SM<T, LAYOUT>) k_layer_norm
     x += x_step;
     if (r + step < n) next.load(at, x, r + step - LN_TURN < p.inner);
     normalise(at, v, lead, p, sum);
-    affine<SILU>(v, params);
+    affine<T, SILU>(v, params);
     if constexpr (LAYOUT == PIECES) {
       edges.store(at, y, v, r < n, n);
       edges.step(step, y_step);
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(MOST, wide_threads<T>(MOST) / MOST) k_layer_no
       ahead = to_f32(load_in(x));
     }
     normalise(at, v, lead, p, sum);
-    affine<SILU>(v, params);
+    affine<T, SILU>(v, params);
     Part<T, LAYOUT, N>::store(at, y, v);
     y += step * p.ys;
   }

@@ -24,7 +24,7 @@ __device__ __forceinline__ void store_param(const LayerNorm& p, int c, float t) 
 }
 
 // xhat and dy of a row to dx (in g); the sums of dw and db move on
-template <bool SILU, int N, bool SP, bool SA, typename Sum>
+template <typename T, bool SILU, int N, bool SP, bool SA, typename Sum>
 __device__ __forceinline__ void row_grad(const float2* xhat, float2* grad, const Params<N, SP>& params, float rstd,
                                          float inv_C, Sums<N, SA>& acc, Sum& sum) {
   float2 c1 = both(0.f), c2 = both(0.f);
@@ -38,7 +38,7 @@ __device__ __forceinline__ void row_grad(const float2* xhat, float2* grad, const
       params.bias(c, z);
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] = fma2(xh[i], w[i], z[i]);
-      sigmoid<4>(z, s);
+      sigmoid<T, 4>(z, s);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 rest = fma2(s[i], both(-1.f), both(1.f));
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(LN_THREADS, 2) k_layer_norm_grad(LayerNorm p) 
     if (r >= end)  // no row
 #pragma unroll
       for (int i = 0; i < H; ++i) v[i] = g[i] = both(0.f);
-    row_grad<SILU>(v, g, params, rstd, p.inv_C, acc, sum);
+    row_grad<T, SILU>(v, g, params, rstd, p.inv_C, acc, sum);
     if constexpr (LAYOUT == PIECES) {
       if (p.y) {
         edges.store(at, dx, g, r < end, end);
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) k_layer_norm_grad_w
       ahead = to_f32(load_in(x));
     }
     const float rstd = normalise(at, v, lead, p, sum);
-    row_grad<SILU>(v, g, params, rstd, p.inv_C, acc, sum);
+    row_grad<T, SILU>(v, g, params, rstd, p.inv_C, acc, sum);
     if (p.y) Part<T, LAYOUT, N>::store(at, dx, g);
     dx += LN_TURN * p.ys;
   }

@@ -1084,3 +1084,26 @@ def test_values_up_to_1e18_in_rows_of_any_width(nm, dtype, c):
         check_rows(nm, x, (dy * 1e18).to(dtype), w, b, eps=eps, silu=True, norm=False)
     small = (x.double() * 1e-36).to(dtype)  # (deviations of 1e-18)
     check_rows(nm, small, (dy * 1e-18).to(dtype), w, b, eps=0.0, norm=False)
+
+
+@pytest.mark.parametrize("n,c", [(1, 64), (50, 64), (33, 97), (7, 2048)])
+def test_silu_where_its_result_nears_the_least_normal_number(nm, n, c):
+    """z from -92 to -80: exp(-z) passes fp32's range from -88.7 on, z exp(z) stays a normal number to -91.9.  A relative error:
+    that of the bounds above, of z with a slope of z exp(z) below 1.02 of the value for a unit of z, and half a unit of the
+    subnormal numbers in the sigmoid."""
+    x, dy, w, _ = inputs(n, c, F32, F32, seed=142)
+    w = 0.01 * w
+    b = torch.linspace(-91.8, -80.0, c, device="cuda")
+    ref = Rows64(x, w, b, 1e-5, True)
+    y = nm.layer_norm(x, w, b, activation="silu")
+    want = ref.z * ref.sig
+    rel = 1.02 * ref.E_z + (12 + 2.4 * ref.z.abs()) * U
+    assert not ((y.double() - want).abs() > want.abs() * rel + (ref.z.abs() + 1) * 2.0**-149).any()
+    assert (want.abs() > 2.0**-126).sum() > 0.9 * want.numel()
+    dy = dy.abs() + 0.5
+    slope = ref.sig * (1 + ref.z * (1 - ref.sig))
+    db = nm.layer_norm_grad(x, dy, w, b, activation="silu")[2].double()
+    want = (dy.double() * slope).sum(0)
+    bound = (dy.double() * slope.abs() * (1.02 * ref.E_z + (16 + 10 * ref.z.abs()) * U)).sum(0)
+    bound = bound + (dy.double() * (ref.z.abs() + 2) * 2.0**-149).sum(0) + (n + 16) * U * (dy.double() * slope.abs()).sum(0)
+    assert not ((db - want).abs() > bound).any()
