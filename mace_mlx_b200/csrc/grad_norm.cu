@@ -202,8 +202,21 @@ __device__ __forceinline__ void store8(float* dst, const float* v) {
   }
 }
 
+// The factor as one of fp32, or as two whose product it is where it lies below fp32's normal numbers: 2^-126, which only
+// moves the exponent of values from 1 on, and the rest.  (Below 2^-252, where the rest is subnormal too, no result reaches
+// 2^-123; smaller values come out within two units of 2^-149.)
+struct Scale {
+  float a, b;
+  __device__ __forceinline__ explicit Scale(double factor) {
+    const bool two = factor < 0x1p-126;  // (a factor that is NaN stays so)
+    a = factor >= 1. ? 1.f : (two ? 0x1p-126f : (float)factor);
+    b = two ? (float)(factor * 0x1p126) : 1.f;
+  }
+  __device__ __forceinline__ bool none() const { return a == 1.f; }
+};
+
 template <typename TI, typename TO>
-__device__ __forceinline__ void clip_tile(const void* in, void* out, int64_t size, uint32_t nth, bool pieces, float scale) {
+__device__ __forceinline__ void clip_tile(const void* in, void* out, int64_t size, uint32_t nth, bool pieces, const Scale& scale) {
   constexpr int V = Piece<TI>::V;
   const Tile tile = tile_of<TI>(in, size, nth);
   Piece<TI> p[GN_UNROLL];
@@ -214,7 +227,7 @@ __device__ __forceinline__ void clip_tile(const void* in, void* out, int64_t siz
     float v[V];
     p[u].values(v);
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] *= scale;
+    for (int k = 0; k < V; ++k) v[k] = v[k] * scale.a * scale.b;
     const int64_t e = tile.e + (u * GN_THREADS + (int)threadIdx.x) * V;
     TO* const dst = static_cast<TO*>(out) + e;
     if (pieces && (tile.whole || (e >= 0 && e + V <= size))) {
@@ -233,19 +246,16 @@ __device__ __forceinline__ void clip_tile(const void* in, void* out, int64_t siz
   }
 }
 
-__device__ __forceinline__ float scale_of(double max_norm, double norm) {
-  const double factor = max_norm / (norm + 1e-6);
-  return factor >= 1. ? 1.f : (float)factor;  // (a factor that is NaN stays so)
-}
+__device__ __forceinline__ Scale scale_of(double max_norm, double norm) { return Scale(max_norm / (norm + 1e-6)); }
 
 // A CTA goes through its run from the end: what the sums read last is still in L2.
 template <int CAP>
-__device__ __forceinline__ void clip_run(const GradList<CAP>& list, const Run& run, float scale) {
-  if (run.lo >= run.hi || (scale == 1.f && !list.elsewhere)) return;
+__device__ __forceinline__ void clip_run(const GradList<CAP>& list, const Run& run, const Scale& scale) {
+  if (run.lo >= run.hi || (scale.none() && !list.elsewhere)) return;
   int t = tensor_of(list, run.hi - 1);
   for (uint32_t tile = run.hi; tile-- > run.lo;) {
     while (tile < list.first[t]) --t;
-    if (scale == 1.f && list.out[t] == list.in[t]) continue;
+    if (scale.none() && list.out[t] == list.in[t]) continue;
     const uint32_t nth = tile - list.first[t];
     const uint8_t type = list.type[t];
     const bool pieces = type & OUT_PIECES;

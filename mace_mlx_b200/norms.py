@@ -367,8 +367,10 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
     and under grad mode none may require a gradient: pass the parameters'
     gradients, not the parameters.
 
-    A norm that is NaN makes every gradient NaN; an infinite one makes the
-    finite values zero and the others NaN: test the norm where that can occur.
+    A norm that is NaN makes every gradient NaN, and infinities among the
+    gradients make the finite values zero and themselves NaN: test the norm where
+    that can occur.  One of finite gradients that passes fp32's range is returned
+    as infinity, and the gradients are scaled by it all the same, in fp64.
     """
     if isinstance(max_norm, torch.Tensor):
         raise TypeError("max_norm must be a number: a tensor's value would be waited for")

@@ -1107,3 +1107,26 @@ def test_silu_where_its_result_nears_the_least_normal_number(nm, n, c):
     bound = (dy.double() * slope.abs() * (1.02 * ref.E_z + (16 + 10 * ref.z.abs()) * U)).sum(0)
     bound = bound + (dy.double() * (ref.z.abs() + 2) * 2.0**-149).sum(0) + (n + 16) * U * (dy.double() * slope.abs()).sum(0)
     assert not ((db - want).abs() > bound).any()
+
+
+@pytest.mark.parametrize("size", [4, 3000, 2_000_003])
+@pytest.mark.parametrize("ins,outs", [(F32, F32), (BF16, F32), (F32, BF16), (BF16, BF16)])
+def test_clipping_of_norms_past_fp32(nm, size, ins, outs):
+    """Factors below fp32's normal numbers, down to 1e-62: the product rounds twice (the factor's rest, the product), and below
+    2^-123 by two units of 2^-149."""
+    grads = [(randn(size, seed=143).clamp(-3, 3) * 1e38).to(ins), torch.full((4,), 3e38, device="cuda").to(ins), randn(50, seed=144, dtype=ins)]
+    grads[0][0] = -3e38
+    for max_norm in (1e20, 1.0, 1e-3, 1e-7, 1e-20):
+        out = [torch.empty_like(g, dtype=outs) for g in grads]
+        norm = nm.clip_grads(grads, max_norm, out=out)
+        assert float(norm) == float(norm64(grads).float())
+        for got, want in zip(out, clipped64(grads, max_norm)):
+            bound = 2.01 * U * want.abs() + 2.0**-148 + (2.0**-8 * want.abs() + 2.0**-133 if outs == BF16 else 0.0)
+            assert not ((got.double() - want).abs() > bound).any()
+        assert (out[0] != 0).any()
+    if ins == outs:
+        want = clipped64(grads, 1e-7)
+        nm.clip_grads(grads, 1e-7)
+        for got, expected in zip(grads, want):
+            bound = 2.01 * U * expected.abs() + 2.0**-148 + (2.0**-8 * expected.abs() + 2.0**-133 if outs == BF16 else 0.0)
+            assert not ((got.double() - expected).abs() > bound).any()
