@@ -81,7 +81,7 @@ struct Piece {
     if (e >= 0 && e + V <= size) {
       raw = load_in(reinterpret_cast<const uint4*>(in + e));
     } else {
-      T t[V];
+      alignas(16) T t[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) t[k] = e + k >= 0 && e + k < size ? load_in(in + e + k) : from_f32<T>(0.f);
       raw = *reinterpret_cast<const uint4*>(t);

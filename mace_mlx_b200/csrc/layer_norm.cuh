@@ -178,7 +178,7 @@ struct Part {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const T* const src = row + at.first[k];
-        T t[V];
+        alignas(16) T t[V];
         const int from = at.first[k] < 0 ? V - at.count[k] : 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) t[i] = i >= from && i < from + at.count[k] ? load_in(src + i) : from_f32<T>(0.f);

@@ -162,7 +162,7 @@ __device__ __forceinline__ void store4(float* dst, const float* v) {
   *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
 }
 __device__ __forceinline__ void store4(bf16* dst, const float* v) {
-  bf16 t[4];
+  alignas(8) bf16 t[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) t[k] = from_f32<bf16>(v[k]);
   *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t);

@@ -285,3 +285,19 @@ def test_results_over_operands_are_refused():
     other = at + (1 << 16)
     assert backward(at, 8, other, 8, at, 8) and backward(at, 8, other, 8, other + 16, 8) and backward(at, 0, other, 0, other - 64, 8)
     assert backward(at, 8, at, 8, other, 8, w=other) and backward(at, 8, at, 8, other, 8, b=other + 4 * size + 28)
+
+
+def test_arrays_read_as_vectors_are_aligned():
+    """A local array whose values go out as one word of 8 or 16 bytes is declared with that alignment: in memory, where a
+    compiler may place it, the word would else be misaligned."""
+    import re
+
+    csrc, found = Path(mace_mlx_b200.__file__).parent / "csrc", 0
+    for name in ("layer_norm.cu", "layer_norm_grad.cu", "layer_norm.cuh", "grad_norm.cu", "species.cuh"):
+        text = (csrc / name).read_text()
+        for use in re.finditer(r"reinterpret_cast<const (?:uint|float)([24])\*>\((\w+)\)", text):
+            declared = list(re.finditer(rf"^\s*(alignas\((\d+)\) )?(?:T|bf16|float) {use[2]}\[\w+\];", text[:use.start()], re.M))
+            if declared and text.count("\n", declared[-1].start(), use.start()) < 12:
+                found += 1
+                assert declared[-1][1] and int(declared[-1][2]) == 4 * int(use[1]), (name, use[0])
+    assert found >= 3
