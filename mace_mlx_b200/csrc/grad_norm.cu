@@ -430,7 +430,7 @@ bool few_tiles(int64_t count, int64_t values) {
 int run_few(const Tensors& a, double max_norm, float* norm, cudaStream_t s) {
   GradList<64> list;
   fill(a, 0, &list);
-  static bool allowed[64] = {};
+  static DeviceFlags allowed;
   return launch_cluster("grad_few", k_grad_few, list.first[list.count], GN_THREADS, s, allowed, list, a.out ? max_norm : -1., norm);
 }
 

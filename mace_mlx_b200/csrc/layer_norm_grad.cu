@@ -263,12 +263,12 @@ int backward(const LayerNorm& p, int lanes, cudaStream_t s) {
     if (lanes > 32) {
       const auto kernel = k_layer_norm_grad_wide<T, LAYOUT, N, SILU, 256>;
       constexpr int OF_LANE = LN_WIDE_SHARED<LAYOUT, 256> ? Params<N, true>::BYTES + Sums<N, true>::BYTES : 0;
-      static bool attr_set[64] = {};  // per device: the attribute call is slow on the host
+      static DeviceFlags attr_set;  // per device: the attribute call is slow on the host
       int dev = 0;
       MACE_CUDA_TRY(cudaGetDevice(&dev));
-      if (OF_LANE * 256 > 49152 && (dev >= 64 || !attr_set[dev])) {
+      if (OF_LANE * 256 > 49152 && !attr_set.get(dev)) {
         MACE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, OF_LANE * 256));
-        if (dev < 64) attr_set[dev] = true;
+        attr_set.set(dev);
       }
       return launch("layer_norm_grad", kernel, grid, lanes, lanes * OF_LANE, s, p);
     }
@@ -276,7 +276,7 @@ int backward(const LayerNorm& p, int lanes, cudaStream_t s) {
   return with_lanes<(N > narrow_values<T, true>(LAYOUT))>(lanes, [&](auto l) {
     const auto kernel = k_layer_norm_grad<T, LAYOUT, N, decltype(l)::value, SILU>;
     if (!p.params || p.part) return launch("layer_norm_grad", kernel, grid, LN_THREADS, 0, s, p);
-    static bool allowed[64] = {};
+    static DeviceFlags allowed;
     return launch_cluster("layer_norm_grad", kernel, grid.x, LN_THREADS, s, allowed, p);
   });
 }

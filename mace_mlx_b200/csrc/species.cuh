@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace mace {
@@ -23,6 +25,15 @@ __device__ __forceinline__ void pdl_wait() {
 template <typename... P>
 bool unaligned(int size, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) % size != 0) || ...); }
 inline int value_size(int32_t dtype) { return dtype == MACE_F32 ? 4 : 2; }
+
+// What has been done once on a device (kernels' attributes); calls may come from several host threads.
+struct DeviceFlags {
+  std::atomic<bool> done[64] = {};
+  bool get(int dev) const { return dev < 64 && done[dev].load(std::memory_order_acquire); }
+  void set(int dev) {
+    if (dev < 64) done[dev].store(true, std::memory_order_release);
+  }
+};
 
 // a grid of clusters of `cluster` CTAs
 template <typename... P, typename... A>
@@ -53,12 +64,13 @@ int launch(const char* name, void (*kernel)(P...), dim3 grid, unsigned threads, 
 // a grid of one cluster, of at least n of at most 16 CTAs: a power of two (more than 8 are this GPU's, not every one's)
 constexpr unsigned MOST_OF_CLUSTER = 16;
 template <typename... P, typename... A>
-int launch_cluster(const char* name, void (*kernel)(P...), unsigned n, unsigned threads, cudaStream_t s, bool* allowed, A... args) {
+int launch_cluster(const char* name, void (*kernel)(P...), unsigned n, unsigned threads, cudaStream_t s, DeviceFlags& allowed,
+                   A... args) {
   int dev = 0;
   MACE_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev >= 64 || !allowed[dev]) {  // (of this kernel, per device: the attribute call is slow on the host)
+  if (!allowed.get(dev)) {  // (of this kernel, per device: the attribute call is slow on the host)
     MACE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    if (dev < 64) allowed[dev] = true;
+    allowed.set(dev);
   }
   unsigned c = 1;
   while (c < n && c < MOST_OF_CLUSTER) c *= 2;

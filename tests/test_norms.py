@@ -301,3 +301,13 @@ def test_arrays_read_as_vectors_are_aligned():
                 found += 1
                 assert declared[-1][1] and int(declared[-1][2]) == 4 * int(use[1]), (name, use[0])
     assert found >= 3
+
+
+def test_what_host_threads_share_is_atomic():
+    """Statics of the C entries, which two host threads may call at once, are atomic (or constant)."""
+    import re
+
+    for name in ("layer_norm.cu", "layer_norm_grad.cu", "layer_norm.cuh", "grad_norm.cu", "tensor_list.cu"):
+        text = (Path(mace_mlx_b200.__file__).parent / "csrc" / name).read_text()
+        kinds = set(re.findall(r"^ +static (?!constexpr|__device__|const |inline)([\w:]+)[^;()]*[;=]", text, re.M))
+        assert kinds <= {"DeviceFlags"}, (name, kinds)
