@@ -226,28 +226,31 @@ __global__ void __launch_bounds__(1024) k_layer_norm_join(LayerNorm p) {
 }
 
 // Few rows of up to 32 lanes go to one cluster of up to 16 CTAs, whose sums need no second launch and no workspace: up
-// to four steps of a CTA, where both take 5 us on the device (1000 rows of 128; 6.7 and 4.6 at twice as many steps), but
-// a call 11.5 us instead of 15.4 on the host.
+// to four steps of a CTA (eight where the rows' starts double their lanes), where both take 5 us on the device (1000 rows of
+// 128; 6.7 and 4.6 at twice as many steps), but a call 11.5 us instead of 15.4 on the host.
 constexpr int LN_FEW = 4, LN_CLUSTER = MOST_OF_CLUSTER;
 
-int64_t rows_at_once(int C) { return LN_THREADS / std::min(row_lanes(8, C, 0), 32); }
-bool few_rows(int64_t n, int C) { return C <= 32 * 8 && n <= LN_CLUSTER * LN_FEW * rows_at_once(C); }
+// lanes of a row that does not take a CTA: by 8 values without what lies before its start, and the most that any type and
+// start give it
+int least_lanes(int C) { return std::min(row_lanes(8, C, 0), 32); }
+int most_lanes(int C) { return std::min(row_lanes(8, C, 16 / 2 - 1), 32); }
+bool few_rows(int64_t n, int C) { return C <= 32 * 8 && n <= LN_CLUSTER * LN_FEW * (LN_THREADS / least_lanes(C)); }
 
-// Rows of a CTA: enough CTAs to fill the GPU, and at most 256 rows for a lane, so that a sum's error stays that of a
-// few hundred terms.  From n, C, whether a row has more than 32 lanes (which its alignment decides too) and whether
-// there is one cluster.
-int64_t grad_share(int64_t n, int C, bool wide, bool cluster) {
-  if (wide) {
+// Rows of a CTA: enough CTAs to fill the GPU, or as many times as many that no lane has more than 256 rows, so that a
+// sum's error stays that of a few hundred terms.  From n, C, the lanes of a row (which its alignment decides too) and whether there is one cluster.
+int64_t grad_share(int64_t n, int C, int lanes, bool cluster) {
+  if (lanes > 32) {
     const int64_t ctas = LN_SMS * std::max(1, 512 / row_lanes(LN_WIDE, C, 0));
     return std::min<int64_t>(std::max<int64_t>((n + ctas - 1) / ctas, 1), 256);
   }
-  const int64_t rows = rows_at_once(C), ctas = cluster ? LN_CLUSTER : LN_SMS * 4;
-  const int64_t share = std::min(std::max((n + ctas - 1) / ctas, rows), rows * 256);
+  const int64_t rows = LN_THREADS / std::max(lanes, least_lanes(C)), ctas = cluster ? LN_CLUSTER : LN_SMS * 4;
+  const int64_t times = std::max<int64_t>((n + ctas * rows * 256 - 1) / (ctas * rows * 256), 1);
+  const int64_t share = std::max((n + ctas * times - 1) / (ctas * times), rows);
   return (share + LN_TURN - 1) / LN_TURN * LN_TURN;
 }
-int64_t grad_shares(int64_t n, int C, bool wide, bool cluster) {
-  const int64_t share = grad_share(n, C, wide, cluster);
-  if (!wide) return (n + share - 1) / share;
+int64_t grad_shares(int64_t n, int C, int lanes, bool cluster) {
+  const int64_t share = grad_share(n, C, lanes, cluster);
+  if (lanes <= 32) return (n + share - 1) / share;
   const int64_t full = n / (LN_TURN * share);
   return full * LN_TURN + std::min<int64_t>(n - full * LN_TURN * share, LN_TURN);
 }
@@ -292,8 +295,8 @@ extern "C" int mace_layer_norm_grad_workspace(int64_t n, int32_t C, int64_t* byt
     return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad_workspace: bad arguments");
   // (rows of these widths take a warp or a CTA, by their alignment)
   int64_t shares = 0;
-  if (C <= 32 * LN_WIDE && !few_rows(n, C)) shares = grad_shares(n, C, false, false);
-  if (C > 32 * LN_APART) shares = std::max(shares, grad_shares(n, C, true, false));
+  if (C <= 32 * LN_WIDE && !few_rows(n, C)) shares = grad_shares(n, C, most_lanes(C), false);
+  if (C > 32 * LN_APART) shares = std::max(shares, grad_shares(n, C, 64, false));
   *bytes = shares * grad_pitch(C) * 4;
   return MACE_OK;
 }
@@ -329,8 +332,7 @@ extern "C" int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t xs, co
     auto go = [&](auto t) {
       using T = decltype(t);
       const RowPlan plan = row_plan<T, true>(n, C, {{x, p.xs}, {dy, p.ds}, {dx, p.ys}});
-      const bool wide = plan.lanes > 32;
-      p.share = grad_share(n, C, wide, cluster), p.shares = grad_shares(n, C, wide, cluster);
+      p.share = grad_share(n, C, plan.lanes, cluster), p.shares = grad_shares(n, C, plan.lanes, cluster);
       return with_plan<T, true>(plan, [&](auto layout, auto values) {
         constexpr Layout LAYOUT = decltype(layout)::value;
         constexpr int N = decltype(values)::value;

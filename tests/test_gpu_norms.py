@@ -1130,3 +1130,11 @@ def test_clipping_of_norms_past_fp32(nm, size, ins, outs):
         for got, expected in zip(grads, want):
             bound = 2.01 * U * expected.abs() + 2.0**-148 + (2.0**-8 * expected.abs() + 2.0**-133 if outs == BF16 else 0.0)
             assert not ((got.double() - expected).abs() > bound).any()
+
+
+@pytest.mark.parametrize("dtype,n,c", [(F32, 3_000_001, 63), (BF16, 1_500_003, 127), (F32, 1_300_001, 126)])
+def test_sums_of_one_sign_over_many_rows_that_start_anywhere(nm, dtype, n, c):
+    """Widths whose rows take twice the lanes where they start anywhere: still at most 256 rows a lane."""
+    x, _, w, b = inputs(n, c, dtype, F32, seed=145)
+    dy = (randn(n, c, seed=146).abs_() + 0.5).to(dtype)
+    check_rows(nm, x, dy, w, b)

@@ -311,3 +311,14 @@ def test_what_host_threads_share_is_atomic():
         text = (Path(mace_mlx_b200.__file__).parent / "csrc" / name).read_text()
         kinds = set(re.findall(r"^ +static (?!constexpr|__device__|const |inline)([\w:]+)[^;()]*[;=]", text, re.M))
         assert kinds <= {"DeviceFlags"}, (name, kinds)
+
+
+def test_a_lane_adds_256_rows_at_most_wherever_rows_start():
+    """Rows that start anywhere can take twice the lanes of aligned ones (fp32 of 62 to 64 channels 16, bf16 of 122 to 128
+    32), and a CTA then half the rows at once: the workspace holds the sums of as many more CTAs."""
+    lib, need = nv.load_library(), C.c_int64()
+    for c, lanes in ((16, 4), (62, 16), (64, 16), (122, 32), (128, 32), (256, 32), (300, 32)):
+        for n in (5_000_000, 50_000_000):
+            assert lib.mace_layer_norm_grad_workspace(n, c, C.byref(need)) == nv.MACE_OK
+            shares = need.value // ((2 * c + 3) // 4 * 16)
+            assert shares * 256 * (256 // lanes) >= n, (c, n)
