@@ -430,8 +430,12 @@ bool few_tiles(int64_t count, int64_t values) {
 int run_few(const Tensors& a, double max_norm, float* norm, cudaStream_t s) {
   GradList<64> list;
   fill(a, 0, &list);
-  static DeviceFlags allowed;
-  return launch_cluster("grad_few", k_grad_few, list.first[list.count], GN_THREADS, s, allowed, list, a.out ? max_norm : -1., norm);
+  static ClusterSizes known;
+  unsigned most = 0;
+  const int rc = most_of_cluster(k_grad_few, GN_THREADS, known, &most);
+  if (rc) return rc;
+  const unsigned c = cluster_of(list.first[list.count], most);
+  return launch_clusters("grad_few", k_grad_few, c, c, GN_THREADS, 0, s, list, a.out ? max_norm : -1., norm);
 }
 
 // parameters of 2, 8 or 30 KB

@@ -237,18 +237,19 @@ int most_lanes(int C) { return std::min(row_lanes(8, C, 16 / 2 - 1), 32); }
 bool few_rows(int64_t n, int C) { return C <= 32 * 8 && n <= LN_CLUSTER * LN_FEW * (LN_THREADS / least_lanes(C)); }
 
 // Rows of a CTA: enough CTAs to fill the GPU, or as many times as many that no lane has more than 256 rows, so that a
-// sum's error stays that of a few hundred terms.  From n, C, the lanes of a row (which its alignment decides too) and whether there is one cluster.
-int64_t grad_share(int64_t n, int C, int lanes, bool cluster) {
+// sum's error stays that of a few hundred terms.  From n, C, the lanes of a row (which its alignment decides too) and
+// the CTAs of one cluster, 0 where there is none.
+int64_t grad_share(int64_t n, int C, int lanes, unsigned cluster) {
   if (lanes > 32) {
     const int64_t ctas = LN_SMS * std::max(1, 512 / row_lanes(LN_WIDE, C, 0));
     return std::min<int64_t>(std::max<int64_t>((n + ctas - 1) / ctas, 1), 256);
   }
-  const int64_t rows = LN_THREADS / std::max(lanes, least_lanes(C)), ctas = cluster ? LN_CLUSTER : LN_SMS * 4;
+  const int64_t rows = LN_THREADS / std::max(lanes, least_lanes(C)), ctas = cluster ? cluster : LN_SMS * 4;
   const int64_t times = std::max<int64_t>((n + ctas * rows * 256 - 1) / (ctas * rows * 256), 1);
   const int64_t share = std::max((n + ctas * times - 1) / (ctas * times), rows);
   return (share + LN_TURN - 1) / LN_TURN * LN_TURN;
 }
-int64_t grad_shares(int64_t n, int C, int lanes, bool cluster) {
+int64_t grad_shares(int64_t n, int C, int lanes, unsigned cluster) {
   const int64_t share = grad_share(n, C, lanes, cluster);
   if (lanes <= 32) return (n + share - 1) / share;
   const int64_t full = n / (LN_TURN * share);
@@ -279,8 +280,14 @@ int backward(const LayerNorm& p, int lanes, cudaStream_t s) {
   return with_lanes<(N > narrow_values<T, true>(LAYOUT))>(lanes, [&](auto l) {
     const auto kernel = k_layer_norm_grad<T, LAYOUT, N, decltype(l)::value, SILU>;
     if (!p.params || p.part) return launch("layer_norm_grad", kernel, grid, LN_THREADS, 0, s, p);
-    static DeviceFlags allowed;
-    return launch_cluster("layer_norm_grad", kernel, grid.x, LN_THREADS, s, allowed, p);
+    static ClusterSizes known;
+    unsigned most = 0;
+    const int rc = most_of_cluster(kernel, LN_THREADS, known, &most);
+    if (rc) return rc;
+    LayerNorm q = p;  // (fewer CTAs take larger shares)
+    q.share = grad_share(p.n, p.C, lanes, most), q.shares = grad_shares(p.n, p.C, lanes, most);
+    const unsigned c = cluster_of((unsigned)q.shares, most);
+    return launch_clusters("layer_norm_grad", kernel, c, c, LN_THREADS, 0, s, q);
   });
 }
 
@@ -295,8 +302,8 @@ extern "C" int mace_layer_norm_grad_workspace(int64_t n, int32_t C, int64_t* byt
     return fail(MACE_ERR_BAD_ARG, "mace_layer_norm_grad_workspace: bad arguments");
   // (rows of these widths take a warp or a CTA, by their alignment)
   int64_t shares = 0;
-  if (C <= 32 * LN_WIDE && !few_rows(n, C)) shares = grad_shares(n, C, most_lanes(C), false);
-  if (C > 32 * LN_APART) shares = std::max(shares, grad_shares(n, C, 64, false));
+  if (C <= 32 * LN_WIDE && !few_rows(n, C)) shares = grad_shares(n, C, most_lanes(C), 0);
+  if (C > 32 * LN_APART) shares = std::max(shares, grad_shares(n, C, 64, 0));
   *bytes = shares * grad_pitch(C) * 4;
   return MACE_OK;
 }
@@ -332,7 +339,7 @@ extern "C" int mace_layer_norm_grad(int32_t dtype, const void* x, int64_t xs, co
     auto go = [&](auto t) {
       using T = decltype(t);
       const RowPlan plan = row_plan<T, true>(n, C, {{x, p.xs}, {dy, p.ds}, {dx, p.ys}});
-      p.share = grad_share(n, C, plan.lanes, cluster), p.shares = grad_shares(n, C, plan.lanes, cluster);
+      p.share = grad_share(n, C, plan.lanes, 0), p.shares = grad_shares(n, C, plan.lanes, 0);  // (a cluster: its own)
       return with_plan<T, true>(plan, [&](auto layout, auto values) {
         constexpr Layout LAYOUT = decltype(layout)::value;
         constexpr int N = decltype(values)::value;

@@ -61,20 +61,39 @@ int launch(const char* name, void (*kernel)(P...), dim3 grid, unsigned threads, 
   return launch_clusters(name, kernel, grid, 1, threads, smem, s, args...);
 }
 
-// a grid of one cluster, of at least n of at most 16 CTAs: a power of two (more than 8 are this GPU's, not every one's)
+// A grid of one cluster: a power of two of at most 16 CTAs.  More than 8 are this GPU's, not every one's, and a process that
+// holds a part of its SMs may have no room for them.
 constexpr unsigned MOST_OF_CLUSTER = 16;
-template <typename... P, typename... A>
-int launch_cluster(const char* name, void (*kernel)(P...), unsigned n, unsigned threads, cudaStream_t s, DeviceFlags& allowed,
-                   A... args) {
+struct ClusterSizes {  // of a kernel, per device (asked once: the calls are slow on the host)
+  std::atomic<unsigned> most[64] = {};
+};
+// the most CTAs of a cluster of this kernel that the current device can hold at once
+template <typename... P>
+int most_of_cluster(void (*kernel)(P...), unsigned threads, ClusterSizes& known, unsigned* most) {
   int dev = 0;
   MACE_CUDA_TRY(cudaGetDevice(&dev));
-  if (!allowed.get(dev)) {  // (of this kernel, per device: the attribute call is slow on the host)
-    MACE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    allowed.set(dev);
+  *most = dev < 64 ? known.most[dev].load(std::memory_order_acquire) : 0;
+  if (*most) return MACE_OK;
+  MACE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  for (*most = MOST_OF_CLUSTER; *most > 1; *most /= 2) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = *most, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(*most), cfg.blockDim = dim3(threads), cfg.attrs = &attr, cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess)
+      cudaGetLastError();  // (a size that it cannot have)
+    else if (clusters > 0)
+      break;
   }
+  if (dev < 64) known.most[dev].store(*most, std::memory_order_release);
+  return MACE_OK;
+}
+inline unsigned cluster_of(unsigned n, unsigned most) {
   unsigned c = 1;
-  while (c < n && c < MOST_OF_CLUSTER) c *= 2;
-  return launch_clusters(name, kernel, c, c, threads, 0, s, args...);
+  while (c < n && c < most) c *= 2;
+  return c;
 }
 
 // all threads of a cluster's CTAs, with what they wrote to shared memory
