@@ -350,7 +350,8 @@ bool overlap(const Tensors& a) {
     spans.push_back({out, out + a.size[t] * value_size(a.out_type[t]), true});
     if (in != out) spans.push_back({in, in + a.size[t] * value_size(a.type[t]), false});
   }
-  std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.lo < y.lo; });
+  const auto before = [](const Span& x, const Span& y) { return x.lo < y.lo; };
+  if (!std::is_sorted(spans.begin(), spans.end(), before)) std::sort(spans.begin(), spans.end(), before);
   uintptr_t out_end = 0, any_end = 0;
   for (const Span& s : spans) {
     if (s.lo < (s.out ? any_end : out_end)) return true;

@@ -29,6 +29,7 @@ import ctypes as C
 import functools
 import math
 import operator
+import struct
 from array import array
 from collections.abc import Iterable, Sequence
 
@@ -273,20 +274,39 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-# (153 tensors: 18 us through DLPack, 44 by these, which take no Python frame each)
+# (153 tensors: 16 us through DLPack, 44 by these, which take no Python frame each)
+_requires = operator.attrgetter("requires_grad")
 _device, _pointer, _numel, _contiguous = (getattr(torch.Tensor, f) for f in
                                           ("get_device", "data_ptr", "numel", "is_contiguous"))
-def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int) -> tuple[array, array, array, bool]:
-    """Pointers, sizes and type codes of dense tensors on device ``dev``, and whether all are contiguous."""
+
+
+def _objects(tensors: Sequence) -> bytes:
+    return struct.pack(f"{len(tensors)}P", *map(id, tensors))
+
+
+_NONE = _objects([None])
+
+
+def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int, objects: bytes | None = None, refuse=None
+          ) -> tuple[array, array, array, bool]:
+    """Pointers, sizes and type codes of dense tensors on device ``dev``, and whether all are contiguous.
+
+    ``objects`` are their addresses, where the caller has them; ``refuse`` looks at the tensors where, under grad mode,
+    one requires a gradient.
+    """
     if _reader is not None and forward_ad._current_level < 0:
         n = len(tensors)
-        objects, ptrs, sizes, codes = array("Q", map(id, tensors)), array("Q", bytes(8 * n)), array("q", bytes(8 * n)), array("i", bytes(4 * n))
+        if objects is None:
+            objects = _objects(tensors)
+        ptrs, sizes, codes = array("Q", bytes(8 * n)), array("q", bytes(8 * n)), array("i", bytes(4 * n))
         try:
-            rc = _reading("mace_tensor_list")(_reader, n, objects.buffer_info()[0], dev, ptrs.buffer_info()[0], sizes.buffer_info()[0],
-                                codes.buffer_info()[0])
+            rc = _reading("mace_tensor_list")(_reader, n, objects, dev, ptrs.buffer_info()[0], sizes.buffer_info()[0],
+                                              codes.buffer_info()[0])
         except Exception:  # noqa: BLE001 (of a type, or a layout, that DLPack has not: told below)
             rc = nv.MACE_ERR_BAD_ARG
         if rc == nv.MACE_OK:
+            if refuse is not None and torch.is_grad_enabled() and any(map(_requires, tensors)):
+                refuse(name, tensors)
             return ptrs, sizes, codes, True
     try:
         elsewhere = set(map(_device, tensors)) - {dev}
@@ -304,27 +324,36 @@ def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int) -> tuple[array, 
             if not _dense(t):
                 raise ValueError(f"{name}[{i}] has gaps or repeated values (strides {t.stride()}); use .contiguous()"
                                  if t.layout is torch.strided else f"{name}[{i}] is not strided, got {t.layout}")
+    if refuse is not None and torch.is_grad_enabled() and any(map(_requires, tensors)):
+        refuse(name, tensors)
     kinds = {dtype: _dtype(name, dtype) for dtype in {t.dtype for t in tensors}}
     codes = array("i", kinds.values()) * len(tensors) if len(kinds) == 1 else array("i", [kinds[t.dtype] for t in tensors])
     return array("Q", map(_pointer, tensors)), array("q", map(_numel, tensors)), codes, contiguous
 
 
-def _grads(grads: Iterable[torch.Tensor | None]) -> list[torch.Tensor]:
+def _grads(grads: Iterable[torch.Tensor | None]) -> tuple[list[torch.Tensor], bytes]:
+    """The gradients without the entries that are None, and the objects' addresses."""
     if isinstance(grads, torch.Tensor):
         raise TypeError("grads must be a sequence of tensors, got one tensor")
-    return [g for g in grads if g is not None]
+    grads = list(grads)
+    objects = _objects(grads)
+    if _NONE in objects:  # (or bytes of two addresses that look like it: a tenth of the time of comparing each entry)
+        grads = [g for g in grads if g is not None]
+        objects = _objects(grads)
+    return grads, objects
 
 
-_requires = operator.attrgetter("requires_grad")
+def _written_to(name: str, tensors: Sequence[torch.Tensor]) -> None:
+    for i, t in enumerate(tensors):
+        _written(f"{name}[{i}]", t)
 
 
-def _without_graph(grads: list[torch.Tensor]) -> None:
-    """Refuses, under grad mode, gradients that have a graph themselves: what is made of them here would have none."""
-    if torch.is_grad_enabled() and any(map(_requires, grads)):
-        for i, g in enumerate(grads):
-            if not g.is_leaf:
-                raise ValueError(f"grads[{i}] has a graph (create_graph=True?), which would end here without a word: detach it "
-                                 "or call under torch.no_grad(); a norm to differentiate is torch.linalg.vector_norm's")
+def _without_graph(name: str, grads: Sequence[torch.Tensor]) -> None:
+    """Refuses gradients that have a graph themselves: what is made of them here would have none."""
+    for i, g in enumerate(grads):
+        if not g.is_leaf:
+            raise ValueError(f"{name}[{i}] has a graph (create_graph=True?), which would end here without a word: detach it "
+                             "or call under torch.no_grad(); a norm to differentiate is torch.linalg.vector_norm's")
 
 
 def _norm_of(grads: list[torch.Tensor], dev: int, flat, fn, *more) -> torch.Tensor:
@@ -348,10 +377,9 @@ def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
     graph: leaves are taken by their values, and gradients with a graph of their
     own (``create_graph=True``) are refused under grad mode.
     """
-    grads = _grads(grads)
+    grads, objects = _grads(grads)
     dev = _cuda("grads[0]", grads[0]) if grads else torch.cuda.current_device()
-    flat = _flat("grads", grads, dev)
-    _without_graph(grads)
+    flat = _flat("grads", grads, dev, objects, _without_graph)
     return _norm_of(grads, dev, flat, nv.load_library().mace_grad_norm)
 
 
@@ -361,8 +389,8 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
 
     Gradients below the bound are left untouched, and nothing waits for the
     norm on the host.  With ``out`` (a tensor for every gradient, with as many
-    values in the same order in memory, float32 or bfloat16) the results go there and the
-    gradients stay, unless ``out`` holds the gradient itself.  No tensor that
+    values in the same order in memory, float32 or bfloat16) the results go there,
+    without a graph, and the gradients stay, unless ``out`` holds the gradient itself.  No tensor that
     is written may overlap another one of the call, so none may be listed twice,
     and under grad mode none may require a gradient: pass the parameters'
     gradients, not the parameters.
@@ -378,24 +406,20 @@ def clip_grads(grads: Iterable[torch.Tensor | None], max_norm: float, *,
     if not 0.0 <= max_norm < math.inf:
         raise ValueError(f"max_norm must be finite and not negative, got {max_norm}")
     every = grads if out is None or isinstance(grads, torch.Tensor) else list(grads)
-    grads = _grads(every)
+    grads, objects = _grads(every)
     dev = _cuda("grads[0]", grads[0]) if grads else torch.cuda.current_device()
-    flat = _flat("grads", grads, dev)
+    flat = _flat("grads", grads, dev, objects, _written_to if out is None else None)
     into, ptrs, codes = grads, flat[0], flat[2]
     if out is not None:
-        _without_graph(grads)
         if len(out) != len(every):
             raise ValueError(f"out has {len(out)} tensors, grads {len(every)}")
         into = list(out) if len(grads) == len(every) else [o for o, g in zip(out, every) if g is not None]
-        ptrs, sizes, codes, contiguous = _flat("out", into, dev)
+        ptrs, sizes, codes, contiguous = _flat("out", into, dev, None, _written_to)
         if sizes.tobytes() != flat[1].tobytes() or not (contiguous and flat[3]):
             for i, (g, o) in enumerate(zip(grads, into)):
                 if o.numel() != g.numel() or o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
                     raise ValueError(f"out[{i}] must be {tuple(g.shape)} with strides {g.stride()}, got {tuple(o.shape)} "
                                      f"with strides {o.stride()}")
-    if torch.is_grad_enabled() and any(map(_requires, into)):
-        for i, t in enumerate(into):
-            _written(f"{'grads' if out is None else 'out'}[{i}]", t)
     norm = _norm_of(grads, dev, flat, nv.load_library().mace_grad_clip, ptrs.buffer_info()[0], codes.buffer_info()[0],
                     max_norm)
     torch.autograd.graph.increment_version(into)
