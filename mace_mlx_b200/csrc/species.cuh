@@ -38,7 +38,7 @@ struct DeviceFlags {
 // a grid of clusters of `cluster` CTAs
 template <typename... P, typename... A>
 int launch_clusters(const char* name, void (*kernel)(P...), dim3 grid, unsigned cluster, unsigned threads, unsigned smem,
-                    cudaStream_t s, A... args) {
+                    cudaStream_t s, const A&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -52,12 +52,12 @@ int launch_clusters(const char* name, void (*kernel)(P...), dim3 grid, unsigned 
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<const P&>(args)...);
   if (e != cudaSuccess) return fail(MACE_ERR_CUDA, std::string("launch ") + name + ": " + cudaGetErrorString(e));
   return MACE_OK;
 }
 template <typename... P, typename... A>
-int launch(const char* name, void (*kernel)(P...), dim3 grid, unsigned threads, unsigned smem, cudaStream_t s, A... args) {
+int launch(const char* name, void (*kernel)(P...), dim3 grid, unsigned threads, unsigned smem, cudaStream_t s, const A&... args) {
   return launch_clusters(name, kernel, grid, 1, threads, smem, s, args...);
 }
 

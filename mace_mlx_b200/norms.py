@@ -285,6 +285,7 @@ def _objects(tensors: Sequence) -> bytes:
 
 
 _NONE = _objects([None])
+_ZERO_POINTERS, _ZERO_SIZES, _ZERO_CODES = array("Q", [0]), array("q", [0]), array("i", [0])
 
 
 def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int, objects: bytes | None = None, refuse=None
@@ -298,7 +299,7 @@ def _flat(name: str, tensors: Sequence[torch.Tensor], dev: int, objects: bytes |
         n = len(tensors)
         if objects is None:
             objects = _objects(tensors)
-        ptrs, sizes, codes = array("Q", bytes(8 * n)), array("q", bytes(8 * n)), array("i", bytes(4 * n))
+        ptrs, sizes, codes = _ZERO_POINTERS * n, _ZERO_SIZES * n, _ZERO_CODES * n
         try:
             rc = _reading("mace_tensor_list")(_reader, n, objects, dev, ptrs.buffer_info()[0], sizes.buffer_info()[0],
                                               codes.buffer_info()[0])
