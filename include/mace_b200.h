@@ -585,6 +585,11 @@ int mace_grad_clip(int32_t count, const void* const* grads, const int64_t* sizes
 int mace_tensor_list(int (*read)(void* object, void* tensor), int32_t count, void* const* objects, int32_t device,
                      void** data, int64_t* sizes, int32_t* dtypes);
 
+/* For the same bindings: the first `count` objects of a Python list, as the entry
+ * above takes them, through PyList_GetItem.  1 if the object `none` is among
+ * them, else 0; -1 if the list is shorter, with an exception set. */
+int mace_list_items(void* (*get)(void* list, intptr_t at), void* list, int32_t count, void* none, void** objects);
+
 /* The operands of a layer norm, read the same way: rows x (of any number of
  * leading dimensions that lie one row stride apart), and where the object is not
  * NULL the output gradient dy, weight and bias.  MACE_OK if they are operands

@@ -76,6 +76,16 @@ extern "C" int mace_tensor_list(int (*read)(void*, void*), int32_t count, void* 
   return MACE_OK;
 }
 
+extern "C" int mace_list_items(void* (*get)(void*, intptr_t), void* list, int32_t count, void* none, void** objects) {
+  int found = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    objects[i] = get(list, i);
+    if (!objects[i]) return -1;
+    if (objects[i] == none) found = 1;
+  }
+  return found;
+}
+
 extern "C" int mace_norm_rows_read(int (*read)(void*, void*), void* x, void* dy, void* weight, void* bias,
                                    mace_norm_rows* rows) {
   if (!read || !x || !rows) return fail(MACE_ERR_BAD_ARG, "mace_norm_rows_read: bad arguments");

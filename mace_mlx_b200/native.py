@@ -141,7 +141,7 @@ EXPORTED = (
     "mace_species_linear_wgrad_workspace", "mace_species_linear_wgrad", "mace_rows_checkpoint", "mace_rows_restore",
     "mace_species_error_flag",
     "mace_layer_norm", "mace_layer_norm_grad_workspace", "mace_layer_norm_grad", "mace_grad_norm_workspace",
-    "mace_grad_norm", "mace_grad_clip", "mace_tensor_list", "mace_norm_rows_read", "mace_norm_rows_forward",
+    "mace_grad_norm", "mace_grad_clip", "mace_tensor_list", "mace_list_items", "mace_norm_rows_read", "mace_norm_rows_forward",
     "mace_norm_rows_backward",
 )
 NOALLOC_MAX_ATOMS = 131072
@@ -224,6 +224,7 @@ def load_library(path: str | Path | None = None) -> C.CDLL:
         "mace_grad_norm": ([i32, vp, vp, vp, vp, vp, i64, vp], C.c_int),
         "mace_grad_clip": ([i32, vp, vp, vp, vp, vp, C.c_double, vp, vp, i64, vp], C.c_int),
         "mace_tensor_list": ([vp, i32, vp, i32, vp, vp, vp], C.c_int),
+        "mace_list_items": ([vp, vp, i32, vp, vp], C.c_int),
         "mace_norm_rows_read": ([vp, vp, vp, vp, vp, vp], C.c_int),
         "mace_norm_rows_forward": ([vp, f32, i32, vp, vp], C.c_int),
         "mace_norm_rows_backward": ([vp, f32, i32, vp, vp, vp, vp, i64, vp], C.c_int),
@@ -243,6 +244,11 @@ def load_reading(name: str):
     fn = getattr(C.PyDLL(str(LIB_PATH)), name)
     fn.argtypes, fn.restype = typed.argtypes, typed.restype
     return fn
+
+
+def list_reader() -> int:
+    """Address of PyList_GetItem, by which an entry reads a Python list."""
+    return C.cast(C.pythonapi.PyList_GetItem, C.c_void_p).value
 
 
 def dlpack_reader(kind) -> int | None:

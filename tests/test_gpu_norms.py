@@ -1034,8 +1034,8 @@ def test_gradients_with_a_graph_are_refused(nm):
     w = randn(30, seed=127).requires_grad_()
     (g,) = torch.autograd.grad((w**3).sum(), w, create_graph=True)
     h = torch.zeros(30, device="cuda")
-    for call in (lambda: nm.grad_norm([g]), lambda: nm.grad_norm([h, g]), lambda: nm.clip_grads([h, g], 1.0)):
-        with pytest.raises(ValueError, match="graph|requires a gradient"):
+    for call in (lambda: nm.grad_norm([g]), lambda: nm.grad_norm([h, g]), lambda: nm.clip_grads([h, g], 1.0, out=[h.clone(), h.clone()])):
+        with pytest.raises(ValueError, match="graph"):
             call()
     want = [g.detach()]
     assert_norm(nm.grad_norm([g.detach()]), want)

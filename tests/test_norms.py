@@ -322,3 +322,13 @@ def test_a_lane_adds_256_rows_at_most_wherever_rows_start():
             assert lib.mace_layer_norm_grad_workspace(n, c, C.byref(need)) == nv.MACE_OK
             shares = need.value // ((2 * c + 3) // 4 * 16)
             assert shares * 256 * (256 // lanes) >= n, (c, n)
+
+
+def test_lists_are_read_as_they_stand():
+    one, two = torch.zeros(1), torch.zeros(2)
+    for items, gaps in (([], False), ([one], False), ([one, two, one], False), ([None], True), ([one, None, two], True), ([one] * 300, False)):
+        objects, none = norms._objects(items)
+        assert list(objects) == [id(item) for item in items] and none == gaps
+    read, room, short = nv.load_reading("mace_list_items"), (C.c_void_p * 3)(), [one]
+    with pytest.raises(IndexError):
+        read(nv.list_reader(), id(short), 3, id(None), room)
