@@ -1051,19 +1051,22 @@ def test_gradients_with_a_graph_are_refused(nm):
 # ------------------------------------------------ rows with one value far off
 @pytest.mark.parametrize("c", [33, 61, 64, 97, 250, 257, 300, 513, 1001, 2049, 4097, 8191, 8192])
 def test_one_hot_rows(nm, c):
-    """A row whose first value is alone in size, the others alike: x - x[0] and its sums are exact, the mean rounds twice
-    in units of R = max |x - x[0]|, a deviation once more: D = 3 u R.  The squares round by 26 u of their sum, those that
+    """One of a row's first values (all are subtracted from that, or from the one in its place) is alone in size, the
+    others alike: differences and their sums are exact, the mean rounds twice in units of R, the value that is alone, a
+    deviation once more: D = 3 u R.  The squares round by 26 u of their sum, those that
     are taken off again, of at most three places at each end of a row, by 8 u each, the deviations by 2 u, rstd's own
     steps by 4 u: 42 u of rstd with the half that the root leaves."""
     n = 40
     x, dy, w, b = torch.zeros(n, c, device="cuda"), randn(n, c, seed=130), 1 + 0.3 * randn(c, seed=131), 0.3 * randn(c, seed=132)
-    x[:, 0] = 1.0 + torch.arange(n, device="cuda") / 64
+    rows = torch.arange(n, device="cuda")
+    size = 1.0 + rows[:, None].double() / 64
+    x[rows, rows % 8] = size[:, 0].float()
     table = torch.empty(n, 2 * c + 1, device="cuda")
     for silu in (False, True):
         act = "silu" if silu else None
         ref = Rows64(x, w, b, 1e-5, silu)
-        ref.D = 42 * U + 3 * U * x[:, :1].double() * ref.rstd
-        ref.E = 3 * U * x[:, :1].double() * ref.rstd + 42 * U * ref.xhat.abs()
+        ref.D = 42 * U + 3 * U * size * ref.rstd
+        ref.E = 3 * U * size * ref.rstd + 42 * U * ref.xhat.abs()
         ref.E_z = ref.w.abs() * ref.E + U * ref.z.abs()
         assert_close(nm.layer_norm(x, w, b, activation=act), *ref.forward(), "y", norm=c < 1000)
         nm.layer_norm(x, w, b, activation=act, out=table[:, c:2 * c])  # (rows that start differently in x and out)
