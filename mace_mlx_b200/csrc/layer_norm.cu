@@ -7,7 +7,7 @@
 //   mean = sum x / C, var = sum (x - mean)^2 / C, xhat = (x - mean) rstd, rstd = 1 / sqrt(var + eps)
 //   z = w xhat + b, y = z or z / (1 + exp(-z))
 //
-// One pass: a row stays in registers, 8 values a lane, between its load and its store.
+// One pass: a row stays in registers, 8 or 16 values a lane, between its load and its store.
 #include "layer_norm.cuh"
 
 namespace mace {

@@ -393,8 +393,8 @@ __device__ __forceinline__ float2 tree(float2* v) {  // (v is used up)
 }
 // A row's values become xhat; rstd is returned.  lead: one of the row's values, which those that are not the row's hold
 // too.  Sums are taken of x - lead: a row of equal values comes out as zeros, an offset common to the row costs no
-// accuracy, and lead is never further from the mean than sqrt(C) standard deviations: a row whose first value is alone in
-// size loses that many units in the last place, others a few.
+// accuracy, and lead is never further from the mean than sqrt(C) standard deviations: a row in which it is alone in size
+// loses that many units in the last place, others a few.
 //   The values that are not the row's are then -mean.  fp32 rows leave out the squares of pieces that have none of the
 // row's values; of the pieces at a row's ends, and in 16 bits of all, they are taken off their lane's sum, with an error of
 // a unit in the last place of mean^2 for each.  (The row's own sum holds mean^2 once, for lead: all that are off in a lane of
