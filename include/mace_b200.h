@@ -567,7 +567,8 @@ int mace_grad_norm(int32_t count, const void* const* grads, const int64_t* sizes
  * Apart from that no output may overlap another tensor of the call (checked).
  * A norm that is NaN makes every value NaN, infinities among the values make the
  * finite ones zero.  The factor follows the norm in fp64: where only the fp32
- * norm is infinite, finite values are scaled by the finite one.  The workspace is that of mace_grad_norm.
+ * norm is infinite, finite values are scaled by the finite one.  The workspace is
+ * that of mace_grad_norm.
  */
 int mace_grad_clip(int32_t count, const void* const* grads, const int64_t* sizes, const int32_t* dtypes,
                    void* const* out, const int32_t* out_dtypes, double max_norm, float* norm, void* workspace,

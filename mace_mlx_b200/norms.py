@@ -44,7 +44,7 @@ _ACTIVATIONS = {None: nv.ACT_NONE, "silu": nv.ACT_SILU}
 __all__ = ["layer_norm", "layer_norm_grad", "grad_norm", "clip_grads"]
 
 # Small calls are bound by the host.  The library reads the tensor objects itself through DLPack's C interface (a forward
-# of 1000 rows 7.6 us a call, 9.3 attribute by attribute, its gradients 11.4 and 14.6); what that interface has not, and
+# of 1000 rows 7.5 us a call, 9.3 attribute by attribute, its gradients 11.4 and 14.3); what that interface has not, and
 # what is to be refused, is looked at here.
 _reader = nv.dlpack_reader(torch.Tensor)
 _reading = functools.cache(nv.load_reading)
@@ -130,69 +130,54 @@ def _read_rows(x, grad, weight, bias) -> nv.NormRows | None:
     return rows if rc == nv.MACE_OK else None
 
 
-def _layer_norm(x, dev, weight, bias, eps, activation, out):
-    rows = _read_rows(x, None, weight, bias) if out is None else None
+def _operands(x, grad, weight, bias) -> nv.NormRows:
+    rows = _read_rows(x, grad, weight, bias)
     if rows is not None:
-        act = _activation(activation)
-        y = _like(x)
-        _launch(dev, nv.load_library().mace_norm_rows_forward, C.byref(rows), _eps(eps), act, y.data_ptr())
-        return y
-    code = _dtype("x", x.dtype)
-    n, c, xs = _rows("x", x)
-    pcode, w, b = _params(weight, bias, dev, c, x.dtype)
+        return rows
+    dev = _cuda("x", x)
+    rows = nv.NormRows(dtype=_dtype("x", x.dtype), device=dev, x=x.data_ptr())
+    rows.n, rows.C, rows.x_stride = _rows("x", x)
+    if grad is not None:
+        _on("grad", grad, dev)
+        if grad.dtype != x.dtype or grad.shape != x.shape:
+            raise ValueError(f"grad must be {x.dtype} {tuple(x.shape)}, got {grad.dtype} {tuple(grad.shape)}")
+        _, _, rows.dy_stride = _rows("grad", grad)
+        rows.dy = grad.data_ptr()
+    rows.param_dtype, rows.weight, rows.bias = _params(weight, bias, dev, rows.C, x.dtype)
+    return rows
+
+
+def _layer_norm(x, weight, bias, eps, activation, out):
+    rows = _operands(x, None, weight, bias)
     act = _activation(activation)
     if out is None:
         y = _like(x)
-        ys = c
-    else:
-        y = out
-        _on("out", y, dev)
-        _written("out", y)
-        if y.dtype != x.dtype or y.shape != x.shape:
-            raise ValueError(f"out must be {x.dtype} {tuple(x.shape)}, got {y.dtype} {tuple(y.shape)}")
-        _, _, ys = _rows("out", y)
-        if n > 1 and ys < c:
-            raise ValueError(f"out rows overlap (strides {y.stride()})")
-    _launch(dev, nv.load_library().mace_layer_norm, code, x.data_ptr(), xs, pcode, w, b, n, c, _eps(eps), act,
-            y.data_ptr(), ys)
-    if out is not None:
-        torch.autograd.graph.increment_version(out)
-    return y
+        _launch(rows.device, nv.load_library().mace_norm_rows_forward, C.byref(rows), _eps(eps), act, y.data_ptr())
+        return y
+    _on("out", out, rows.device)
+    _written("out", out)
+    if out.dtype != x.dtype or out.shape != x.shape:
+        raise ValueError(f"out must be {x.dtype} {tuple(x.shape)}, got {out.dtype} {tuple(out.shape)}")
+    n, c, stride = _rows("out", out)
+    if n > 1 and stride < c:
+        raise ValueError(f"out rows overlap (strides {out.stride()})")
+    _launch(rows.device, nv.load_library().mace_layer_norm, rows.dtype, rows.x, rows.x_stride, rows.param_dtype, rows.weight,
+            rows.bias, n, c, _eps(eps), act, out.data_ptr(), stride)
+    torch.autograd.graph.increment_version(out)
+    return out
 
 
 def _layer_norm_grad(x, grad, weight, bias, eps, activation, want_x, want_w, want_b):
-    rows = _read_rows(x, grad, weight, bias)
-    if rows is not None:
-        act = _activation(activation)
-        dev, n, c = rows.device, rows.n, rows.C
-        dx = _like(x) if want_x else None
-        dw = _like(weight) if want_w else None
-        db = _like(bias) if want_b else None
-        ws, ptr, nbytes = None, None, 0
-        if want_w or want_b:
-            ws, ptr, nbytes = _workspace("mace_layer_norm_grad_workspace", dev, x, n, c)
-        _launch(dev, nv.load_library().mace_norm_rows_backward, C.byref(rows), _eps(eps), act,
-                dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None, db.data_ptr() if want_b else None, ptr,
-                nbytes)
-        return dx, dw, db
-    dev = _cuda("x", x)
-    code = _dtype("x", x.dtype)
-    n, c, xs = _rows("x", x)
-    _on("grad", grad, dev)
-    if grad.dtype != x.dtype or grad.shape != x.shape:
-        raise ValueError(f"grad must be {x.dtype} {tuple(x.shape)}, got {grad.dtype} {tuple(grad.shape)}")
-    _, _, gs = _rows("grad", grad)
-    pcode, w, b = _params(weight, bias, dev, c, x.dtype)
+    rows = _operands(x, grad, weight, bias)
     act = _activation(activation)
     dx = _like(x) if want_x else None
     dw = _like(weight) if want_w else None
     db = _like(bias) if want_b else None
     ws, ptr, nbytes = None, None, 0
     if want_w or want_b:
-        ws, ptr, nbytes = _workspace("mace_layer_norm_grad_workspace", dev, x, n, c)
-    _launch(dev, nv.load_library().mace_layer_norm_grad, code, x.data_ptr(), xs, grad.data_ptr(), gs, pcode, w, b, n, c,
-            _eps(eps), act, dx.data_ptr() if want_x else None, c, dw.data_ptr() if want_w else None,
-            db.data_ptr() if want_b else None, ptr, nbytes)
+        ws, ptr, nbytes = _workspace("mace_layer_norm_grad_workspace", rows.device, x, rows.n, rows.C)
+    _launch(rows.device, nv.load_library().mace_norm_rows_backward, C.byref(rows), _eps(eps), act,
+            dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None, db.data_ptr() if want_b else None, ptr, nbytes)
     return dx, dw, db
 
 
@@ -203,8 +188,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     ``activation`` is None (f the identity) or ``"silu"``.  x is float32 or
     bfloat16, (..., C) with contiguous channels and rows at one stride, so a
     slot of a node-feature table is passed in place; so may ``out``, which must
-    not overlap x, weight or bias.  weight and bias (C,), either or both, are of x's type or
-    float32; without them they are ones and zeros.
+    not overlap x, weight or bias.  weight and bias (C,), either or both, are of
+    x's type or float32; without them they are ones and zeros.
 
     Statistics and products are fp32, rounded once to x's type.  Sums are taken
     of x minus one of the row's first values: an offset common to a row costs no
@@ -214,7 +199,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     SiLU's exponential and reciprocal are approximate: its sigmoid is off by about
     2 + 1.2 |z| units of fp32's last place.
     """
-    dev = _cuda("x", x)
+    _cuda("x", x)
     if torch.is_grad_enabled() and (x.requires_grad or _requires_grad("weight", weight) or _requires_grad("bias", bias)):
         if out is not None:
             raise ValueError("out= cannot take part in autograd")
@@ -222,7 +207,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
             if t is not None:
                 _cuda(name, t)
         return _LayerNormFn.apply(x, weight, bias, eps, activation)
-    return _layer_norm(x, dev, weight, bias, eps, activation, out)
+    return _layer_norm(x, weight, bias, eps, activation, out)
 
 
 def _requires_grad(name: str, t: torch.Tensor | None) -> bool:
@@ -238,10 +223,10 @@ def layer_norm_grad(x: torch.Tensor, grad: torch.Tensor, weight: torch.Tensor | 
                     ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
     """Gradients of ``layer_norm`` at x, weight and bias for the output gradient ``grad``.
 
-    They have no graph, whatever the arguments require.  Those of weight and
-    bias have their type (None without them); their sums
-    over the rows are fp32, in an order that depends on the sizes, the types and
-    the addresses modulo 16 alone, so equal calls give equal bits.
+    They have no graph, whatever the arguments require.  Those of weight and bias
+    have their type (None without them); their sums over the rows are fp32, in an
+    order that depends on the sizes, the types and the addresses modulo 16 alone,
+    so equal calls give equal bits.
     """
     return _layer_norm_grad(x, grad, weight, bias, eps, activation, True, weight is not None, bias is not None)
 
@@ -251,7 +236,7 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, activation):
         ctx.save_for_backward(x, weight, bias)
         ctx.more = eps, activation
-        return _layer_norm(x, x.get_device(), weight, bias, eps, activation, None)
+        return _layer_norm(x, weight, bias, eps, activation, None)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
